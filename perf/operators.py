@@ -31,38 +31,38 @@ def listed():
     return [
         # a decoding step's router: eight tokens, where the launches count
         {"name": "route_8_f32", "kind": "route", "tokens": 8, "experts": 64, "k": 6, "dtype": "f32", "renormalize": True,
-         "masked": False, "grad": False},
+         "masked": False, "grad": False, "bound": True},
         # a training batch's router of odd length, forward and backward, with forbidden experts and padding tokens
         {"name": "route_32k_bf16_grad", "kind": "route", "tokens": 32771, "experts": 256, "k": 8, "dtype": "bf16",
-         "renormalize": False, "masked": True, "grad": True},
+         "renormalize": False, "masked": True, "grad": True, "bound": False},
         # one token's choices: eight matrices of 64 are read, a row each
         {"name": "grouped_1token_bf16", "kind": "grouped", "tokens": 1, "k": 8, "experts": 64, "n": 2048, "kdim": 4096,
-         "dtype": "bf16", "skew": 0.0},
+         "dtype": "bf16", "skew": 0.0, "bound": True},
         # a batch of decoding requests: a few rows on every expert
         {"name": "grouped_decode_f16", "kind": "grouped", "tokens": 48, "k": 6, "experts": 64, "n": 1408, "kdim": 2048,
-         "dtype": "f16", "skew": 0.3},
+         "dtype": "f16", "skew": 0.3, "bound": True},
         # odd sizes, most rows on few experts, some experts without rows
         {"name": "grouped_ragged_f16", "kind": "grouped", "tokens": 5003, "k": 1, "experts": 40, "n": 1000, "kdim": 1416,
-         "dtype": "f16", "skew": 2.0},
+         "dtype": "f16", "skew": 2.0, "bound": False},
         # a prompt or a training batch through the layer's first matrix
         {"name": "grouped_prompt_bf16", "kind": "grouped", "tokens": 8192, "k": 4, "experts": 32, "n": 4096, "kdim": 2048,
-         "dtype": "bf16", "skew": 0.3},
+         "dtype": "bf16", "skew": 0.3, "bound": False},
         # gradients of a small layer, weights' gradients kept in 32 bits
         {"name": "grouped_grad_4k_f32dw", "kind": "grouped_grad", "tokens": 2051, "k": 2, "experts": 16, "n": 1024, "kdim": 2048,
-         "dtype": "bf16", "dw_dtype": "f32", "skew": 1.0},
+         "dtype": "bf16", "dw_dtype": "f32", "skew": 1.0, "bound": False},
         # gradients of a large one, in the weights' own type
         {"name": "grouped_grad_32k_bf16", "kind": "grouped_grad", "tokens": 8192, "k": 4, "experts": 32, "n": 4096, "kdim": 2048,
-         "dtype": "bf16", "dw_dtype": "bf16", "skew": 0.3},
+         "dtype": "bf16", "dw_dtype": "bf16", "skew": 0.3, "bound": False},
         # a decoding step's last operator
-        {"name": "combine_16_bf16", "kind": "combine", "tokens": 16, "k": 8, "width": 2048, "dtype": "bf16", "grad": False},
+        {"name": "combine_16_bf16", "kind": "combine", "tokens": 16, "k": 8, "width": 2048, "dtype": "bf16", "grad": False, "bound": True},
         # its gradient in a training batch
-        {"name": "combine_16k_bf16_grad", "kind": "combine", "tokens": 16384, "k": 4, "width": 4096, "dtype": "bf16", "grad": True},
+        {"name": "combine_16k_bf16_grad", "kind": "combine", "tokens": 16384, "k": 4, "width": 4096, "dtype": "bf16", "grad": True, "bound": False},
         # a small model's gradients: many short tensors of odd lengths
         {"name": "clip_261_small_f32", "kind": "clip", "tensors": 261, "elements": 2_600_003, "dtype": "f32", "out_dtype": "f32",
-         "max_norm": 1.0},
+         "max_norm": 1.0, "bound": True},
         # a large model's gradients in 16 bits, clipped into the optimizer's 32-bit buffers
         {"name": "clip_96_large_bf16", "kind": "clip", "tensors": 96, "elements": 400_000_001, "dtype": "bf16", "out_dtype": "f32",
-         "max_norm": 1.0},
+         "max_norm": 1.0, "bound": True},
     ]
 
 
@@ -78,7 +78,7 @@ def _feature_size(rng, lo, hi):
 
 def draw(rng):
     kind = rng.choice(["route", "grouped", "grouped", "grouped_grad", "combine", "clip"])
-    case = {"kind": kind}
+    case = {"kind": kind, "bound": rng.random() < 0.5}
     if kind == "route":
         experts = rng.choice([8, 16, 40, 60, 64, 128, 160, 256, 384])
         case.update(tokens=_log_size(rng, 1, 32771), experts=experts, k=rng.randint(1, 8), dtype=rng.choice(["f32", "bf16", "f16"]),
@@ -201,38 +201,52 @@ def prepare(case, seed):
         # the optimizer's flat buffer, a piece for each tensor
         state["flat"] = torch.zeros(total, dtype=DTYPES[case["out_dtype"]], device="cuda")
         state["outs"] = [state["flat"][a:a + s] for a, s in zip(starts, sizes)]
+    if own:
+        state["pass"] = _own_pass(state)
     return state
 
 
 # ---- one pass ----------------------------------------------------------------------------------------------------
 
 def run(state):
-    return (_run_own if own else _run_plain)(state)
+    return state["pass"]() if own else _run_plain(state)
 
 
-def _run_own(state):
+def _own_pass(state):
+    """The framework's calls of one pass.  ``bound``: a serving or training loop over fixed buffers, which binds its arguments once and
+    launches every step; otherwise the plain calls, which check their arguments and allocate their outputs."""
     from flexspmv_b200 import experts
     case = state["case"]
     kind = case["kind"]
+
+    def call(op, *args, **kwargs):
+        return experts.bind(op, *args, **kwargs).launch if case["bound"] else lambda: op(*args, **kwargs)
+
     if kind == "route":
-        plan = experts.route(state["logits"], case["k"], renormalize=case["renormalize"])
-        out = {"weights": plan.weights, "experts": plan.experts, "offsets": plan.offsets, "rows": plan.rows, "slots": plan.slots}
-        if case["grad"]:
-            out["dlogits"] = experts.route_backward(state["dweights"], state["logits"], plan)
-        return out
+        forward = call(experts.route, state["logits"], case["k"], renormalize=case["renormalize"])
+
+        def route():
+            plan = forward()
+            out = {"weights": plan.weights, "experts": plan.experts, "offsets": plan.offsets, "rows": plan.rows, "slots": plan.slots}
+            if case["grad"]:
+                out["dlogits"] = experts.route_backward(state["dweights"], state["logits"], plan)
+            return out
+        return route
     if kind == "grouped":
-        return {"y": experts.grouped_matmul(state["x"], state["weight"], state["offsets"], rows=state["rows"])}
+        y = call(experts.grouped_matmul, state["x"], state["weight"], state["offsets"], rows=state["rows"])
+        return lambda: {"y": y()}
     if kind == "grouped_grad":
-        return {"dx": experts.grouped_matmul_dx(state["dy"], state["weight"], state["offsets"]),
-                "dw": experts.grouped_matmul_dw(state["dy"], state["x"], state["offsets"], rows=state["rows"],
-                                                dtype=DTYPES[case["dw_dtype"]])}
+        dx = call(experts.grouped_matmul_dx, state["dy"], state["weight"], state["offsets"])
+        dw = call(experts.grouped_matmul_dw, state["dy"], state["x"], state["offsets"], rows=state["rows"], dtype=DTYPES[case["dw_dtype"]])
+        return lambda: {"dx": dx(), "dw": dw()}
+    if kind == "combine" and case["grad"]:
+        backward = call(experts.combine_backward, state["dout"], state["z"], state["slots"], state["weights"], state["offsets"])
+        return lambda: dict(zip(("dz", "dweights"), backward()))
     if kind == "combine":
-        if case["grad"]:
-            dz, dweights = experts.combine_backward(state["dout"], state["z"], state["slots"], state["weights"], state["offsets"])
-            return {"dz": dz, "dweights": dweights}
-        return {"out": experts.combine(state["z"], state["slots"], state["weights"])}
-    norm = experts.clip_grad_norm(state["grads"], case["max_norm"], out=state["outs"])
-    return {"norm": norm, "flat": state["flat"]}
+        out = call(experts.combine, state["z"], state["slots"], state["weights"])
+        return lambda: {"out": out()}
+    clip = call(experts.clip_grad_norm, state["grads"], case["max_norm"], out=state["outs"])
+    return lambda: {"norm": clip(), "flat": state["flat"]}
 
 
 def _run_plain(state):
