@@ -1,0 +1,55 @@
+// Value types of the expert operators: 16- and 32-bit floats, W of them in one access.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "../../include/flexspmv.h"
+
+namespace flex {
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <class T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// W values: 16 bytes where they are that many, else a value on its own.
+template <class T, int W>
+struct Pack {
+  union { uint4 raw[(sizeof(T) * W + 15) / 16]; T v[W]; };
+  __device__ __forceinline__ Pack() {}
+  static constexpr bool kWide = sizeof(T) * W % 16 == 0;
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kWide) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) * W / 16; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) v[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kWide) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) * W / 16; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) p[i] = v[i];
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = from_float<T>(0.f);
+  }
+  __device__ __forceinline__ float get(int i) const { return to_float(v[i]); }
+  __device__ __forceinline__ void set(int i, float x) { v[i] = from_float<T>(x); }
+};
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool known_type(int t) { return t == FLEXSPMV_TYPE_F32 || t == FLEXSPMV_TYPE_BF16 || t == FLEXSPMV_TYPE_F16; }
+inline int type_bytes(int t) { return t == FLEXSPMV_TYPE_F32 ? 4 : 2; }
+
+}  // namespace flex

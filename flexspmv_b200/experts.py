@@ -1,0 +1,415 @@
+"""Operators of a routed expert layer: ``y[t] = sum_j w[t, j] * W[e[t, j]] x[t]``.
+
+It is this library's gather -> per-edge map -> segmented reduce with (token, choice) pairs as the edges, the expert that a router chose
+as an edge's type, and that expert's matrix as the map.  (The reference has no operator of the kind: its maps work on records of a few
+values, data_struct_shared.cuh:80-659.)
+
+    plan = route(logits, k)                                     # weights, experts, and the plan: offsets, rows, slots
+    h = grouped_matmul(x, w1, plan.offsets, rows=plan.rows)     # h[i] = w1[e] x[rows[i]], places in expert order
+    z = grouped_matmul(act(h), w2, plan.offsets)
+    y = combine(z, plan.slots, plan.weights)                    # y[t] = sum_j weights[t, j] z[slots[t, j]]
+
+with the gradients ``route_backward``, ``grouped_matmul_dx``, ``grouped_matmul_dw`` and ``combine_backward``, and ``grad_norm`` and
+``clip_grad_norm`` over the many tensors that such a layer's training has.  ``expert_layer.RoutedExperts`` runs them together.
+
+The operators take CUDA tensors, enqueue on torch's current stream of the tensors' device and never synchronise; the plan stays on the
+device.  Arguments that do not fit raise ``FlexSpmvError``; there is no CPU path.  ``bind(op, *args)`` checks and allocates once and returns
+an object whose ``launch()`` is one foreign call on the same tensors, as ``GraphExtension.prepare`` does for graphs: for loops over fixed
+buffers and for capture in a CUDA graph.  Index arrays that do not fit their arrays (offsets that descend, rows out of range) are
+noticed on the device, where nothing is read or written out of range: the next call of a grouped product on the device, or ``check()``, raises.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Dict, NamedTuple, Optional, Sequence
+
+import torch
+
+from .binding import FlexSpmvError, _current_device, _pointers, _raw_stream, check as _check_status, load_library
+
+MAX_EXPERTS, MAX_CHOICES = 1024, 32          # FLEXSPMV_MAX_EXPERTS, FLEXSPMV_MAX_CHOICES
+_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_HALF = (torch.bfloat16, torch.float16)
+_RENORMALIZE = 1
+_FORWARD, _DX, _DW = 0, 1, 2
+
+
+class Desc(ctypes.Structure):
+    """flexspmv_expert_desc (include/flexspmv.h)."""
+    _fields_ = [("tokens", ctypes.c_int64), ("slots", ctypes.c_int64)] + \
+               [(n, ctypes.c_int32) for n in ("experts", "choices", "n", "k", "type", "out_type", "flags", "reserved")] + \
+               [("in_stride", ctypes.c_int64), ("in2_stride", ctypes.c_int64)]
+
+
+class Plan(NamedTuple):
+    """What ``route`` returns.  A *place* is a pair's position in the order by expert, then token."""
+    weights: torch.Tensor        # (tokens, k) float32, largest first; 0 where there is no expert
+    experts: torch.Tensor        # (tokens, k) int32, -1: none
+    offsets: torch.Tensor        # (experts + 1) int32: places offsets[e] .. offsets[e + 1] are expert e's
+    rows: torch.Tensor           # (tokens * k) int32: the token of a place, -1 from offsets[-1] on
+    slots: torch.Tensor          # (tokens, k) int32: a pair's place, -1: none
+    renormalize: bool
+
+
+class BoundCall:
+    """One operator bound to its tensors: ``launch()`` enqueues it on the current stream of their device and returns the outputs, the
+    same tensors every time.  Launches of one object must be ordered with one another: they share outputs and workspace."""
+    __slots__ = ("_fn", "_args", "_device", "_keep", "_flag", "outputs")
+
+    def __init__(self, fn, args, device, keep, outputs, flag=None):
+        self._fn, self._args, self._device, self._keep, self.outputs, self._flag = fn, args, device, keep, outputs, flag
+
+    def launch(self):
+        if self._flag is not None and self._flag[0]:
+            _raise_flag(self._device)
+        if _current_device() != self._device:
+            with torch.cuda.device(self._device):
+                st = self._fn(*self._args, _raw_stream(self._device))
+        else:
+            st = self._fn(*self._args, _raw_stream(self._device))
+        if st != 0:
+            _check_status(load_library(), st, "launch")
+        return self.outputs
+
+    __call__ = launch
+
+
+_P, _I, _N = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
+_WITH_WORKSPACE = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P, _N, _P)
+_GROUPED = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P, _N, _P, _P)
+_PLAIN = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P)
+_CLIP = ctypes.CFUNCTYPE(_I, ctypes.c_int32, _P, _P, _P, _P, _P, ctypes.c_float, _P, _P, _N, _P)
+_functions: Dict[str, object] = {}
+
+
+def _function(name: str, proto):
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = proto((f"flexspmv_{name}", load_library()))
+    return f
+
+
+class _Flag:
+    __slots__ = ("tensor", "view")
+
+    def __init__(self):
+        self.tensor = torch.zeros(1, dtype=torch.int32).pin_memory()
+        self.view = self.tensor.numpy()
+
+
+_flags: Dict[int, _Flag] = {}
+
+
+def _flag(device: int) -> _Flag:
+    """The page-locked int in which the kernels of a device leave an error."""
+    if device not in _flags:
+        _flags[device] = _Flag()
+    return _flags[device]
+
+
+def _raise_flag(device: int):
+    st = int(_flag(device).view[0])
+    _flag(device).view[0] = 0
+    text = "offsets or rows that do not fit their arrays" if st == -5 else load_library().flexspmv_error_string(st).decode()
+    raise FlexSpmvError(f"an earlier grouped product on cuda:{device} failed: {text} (status {st}); its outputs are undefined", st)
+
+
+def check(device=None) -> None:
+    """Waits for the device and raises where a grouped product on it has found an error."""
+    index = torch.device(device).index if device is not None else None
+    index = _current_device() if index is None else index
+    torch.cuda.synchronize(index)
+    if index in _flags and _flags[index].view[0]:
+        _raise_flag(index)
+
+
+def _need(ok: bool, what: str):
+    if not ok:
+        raise FlexSpmvError(what)
+
+
+def _tensor(t, name: str, dtypes, dim: int, device=None) -> int:
+    """Checks a tensor argument; returns its device's index."""
+    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
+    if t.dtype not in dtypes or t.dim() != dim:
+        raise FlexSpmvError(f"{name} must have {dim} dimension(s) and one of the types {', '.join(str(d) for d in dtypes)}, "
+                            f"not {tuple(t.shape)} {t.dtype}")
+    if device is not None and t.device.index != device:
+        raise FlexSpmvError(f"{name} is on cuda:{t.device.index}, not cuda:{device}")
+    return t.device.index
+
+
+def _rows_of(t: torch.Tensor, name: str, aligned: bool = True) -> int:
+    """Row stride of a matrix whose rows are contiguous."""
+    n, stride = t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    _need((n <= 1 or t.stride(1) == 1) and stride >= n, f"{name}: rows must be contiguous and must not overlap")
+    if aligned:
+        _need(n % 8 == 0 and stride % 8 == 0 and t.data_ptr() % 16 == 0,
+              f"{name}: rows must be multiples of 8 values, apart by multiples of 8, the first on 16 bytes")
+    return stride
+
+
+def _whole(t: torch.Tensor, name: str):
+    _need(t.is_contiguous(), f"{name} must be contiguous")
+
+
+def _out(out, shape, dtype, device, name="out"):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _tensor(out, name, (dtype,), len(shape), device.index)
+    _need(tuple(out.shape) == tuple(shape), f"{name} must have the shape {tuple(shape)}, not {tuple(out.shape)}")
+    _whole(out, name)
+    return out
+
+
+# ---- the operators -----------------------------------------------------------------------------------------------
+
+_BINDERS = {}
+
+
+def _operator(binder):
+    """The public function of a binder: the call bound and launched once."""
+    def op(*args, **kwargs):
+        return binder(*args, **kwargs).launch()
+    op.__name__, op.__doc__, op.__wrapped__ = binder.__name__, binder.__doc__, binder
+    op.__qualname__ = binder.__name__
+    op.__module__ = __name__
+    _BINDERS[op] = binder
+    return op
+
+
+def bind(op, *args, **kwargs) -> BoundCall:
+    """Checks the arguments of an operator of this module and allocates its outputs and workspace once; the ``BoundCall``'s ``launch()``
+    runs it on them as often as wanted."""
+    _need(op in _BINDERS, "bind takes an operator of this module")
+    return _BINDERS[op](*args, **kwargs)
+
+
+@_operator
+def route(logits: torch.Tensor, k: int, renormalize: bool = False) -> Plan:
+    """Softmax over each row of ``logits`` (tokens, experts; float32, bfloat16 or float16), its k largest values and the plan.
+
+    Equal logits: the lowest expert first.  A logit of -infinity forbids an expert; a row with fewer than k others has experts of -1 and
+    weights of 0 for the rest, a row without any takes no place.  ``renormalize`` divides a row's weights by their sum."""
+    dev = _tensor(logits, "logits", tuple(_TYPE), 2)
+    tokens, experts = logits.shape
+    _need(1 <= k <= experts, f"k must be 1 to the number of experts, not {k}")
+    _need(experts <= MAX_EXPERTS and k <= MAX_CHOICES, f"at most {MAX_EXPERTS} experts and {MAX_CHOICES} choices")
+    stride = _rows_of(logits, "logits", aligned=False)
+    d = Desc(tokens=tokens, slots=tokens * k, experts=experts, choices=k, type=_TYPE[logits.dtype], flags=_RENORMALIZE if renormalize else 0,
+             in_stride=stride)
+    lib = load_library()
+    need = ctypes.c_size_t()
+    _check_status(lib, lib.flexspmv_expert_route_bytes(ctypes.byref(d), ctypes.byref(need)), "route")
+    # one allocation: the plan's arrays behind one another, then the workspace
+    pairs = tokens * k
+    buf = torch.empty(4 * pairs + experts + 1 + need.value // 4, dtype=torch.int32, device=logits.device)
+    weights = buf[:pairs].view(torch.float32).view(tokens, k)
+    ids, slots = buf[pairs:2 * pairs].view(tokens, k), buf[2 * pairs:3 * pairs].view(tokens, k)
+    rows, offsets = buf[3 * pairs:4 * pairs], buf[4 * pairs:4 * pairs + experts + 1]
+    plan = Plan(weights, ids, offsets, rows, slots, bool(renormalize))
+    base = buf.data_ptr()
+    outs = (ctypes.c_void_p * 5)(base, base + 4 * pairs, base + 16 * pairs, base + 12 * pairs, base + 8 * pairs)
+    ins = (ctypes.c_void_p * 1)(logits.data_ptr())
+    return BoundCall(_function("expert_route", _WITH_WORKSPACE),
+                     (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), base + 16 * pairs + 4 * (experts + 1), need.value), dev,
+                     (d, ins, outs, logits, buf), plan)
+
+
+@_operator
+def route_backward(dweights: torch.Tensor, logits: torch.Tensor, plan: Plan, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of ``route``'s weights with respect to ``logits``, of their type; the choice itself has none."""
+    dev = _tensor(logits, "logits", tuple(_TYPE), 2)
+    tokens, experts = logits.shape
+    stride = _rows_of(logits, "logits", aligned=False)
+    _tensor(dweights, "dweights", (torch.float32,), 2, dev)
+    for name, t, dt in (("weights", plan.weights, torch.float32), ("experts", plan.experts, torch.int32)):
+        _tensor(t, f"plan.{name}", (dt,), 2, dev)
+        _whole(t, f"plan.{name}")
+    k = plan.weights.shape[1]
+    _need(plan.weights.shape[0] == tokens and plan.experts.shape == plan.weights.shape and dweights.shape == plan.weights.shape,
+          "dweights and the plan must be of the logits' rows")
+    _whole(dweights, "dweights")
+    out = _out(out, (tokens, experts), logits.dtype, logits.device)
+    d = Desc(tokens=tokens, slots=tokens * k, experts=experts, choices=k, type=_TYPE[logits.dtype], flags=_RENORMALIZE if plan.renormalize else 0,
+             in_stride=stride)
+    ins, outs = _pointers((dweights, logits, plan.weights, plan.experts)), _pointers((out,))
+    return BoundCall(_function("expert_route_backward", _PLAIN), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs)), dev,
+                     (d, ins, outs, dweights, logits, plan, out), out)
+
+
+def _grouped(which: int, name: str, d: Desc, ins, out, offsets, dev: int) -> BoundCall:
+    lib = load_library()
+    need = ctypes.c_size_t()
+    _check_status(lib, lib.flexspmv_grouped_matmul_bytes(ctypes.byref(d), which, ctypes.byref(need)), name)
+    ws = torch.empty(need.value, dtype=torch.uint8, device=out.device) if need.value else None
+    flag = _flag(dev)
+    pin, pout = (ctypes.c_void_p * len(ins))(*[t.data_ptr() if t is not None else 0 for t in ins]), _pointers((out,))
+    return BoundCall(_function(name, _GROUPED), (ctypes.addressof(d), ctypes.addressof(pin), ctypes.addressof(pout),
+                                                 ws.data_ptr() if ws is not None else 0, need.value, flag.tensor.data_ptr()), dev,
+                     (d, pin, pout, ins, out, ws, flag), out, flag.view)
+
+
+def _plan_arrays(offsets, rows, experts: int, dev: int):
+    _tensor(offsets, "offsets", (torch.int32,), 1, dev)
+    _need(offsets.numel() == experts + 1, f"offsets must have {experts + 1} entries, not {offsets.numel()}")
+    _whole(offsets, "offsets")
+    if rows is not None:
+        _tensor(rows, "rows", (torch.int32,), 1, dev)
+        _whole(rows, "rows")
+
+
+def _weights_of(weight, dtype, dev: int):
+    _tensor(weight, "weight", (dtype,), 3, dev)
+    _whole(weight, "weight")
+    e, n, k = weight.shape
+    _need(1 <= e <= MAX_EXPERTS, f"1 to {MAX_EXPERTS} experts, not {e}")
+    _need(n >= 8 and k >= 8 and n % 8 == 0 and k % 8 == 0 and weight.data_ptr() % 16 == 0,
+          f"weight: both sides of a matrix must be multiples of 8 and the first value on 16 bytes, not {n} x {k}")
+    return e, n, k
+
+
+@_operator
+def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, rows: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``y[i] = weight[e] @ x[rows[i]]`` for the places ``offsets[e] <= i < offsets[e + 1]`` (``rows`` None: ``x[i]``).
+
+    ``x`` (tokens, k) and ``weight`` (experts, n, k) of one 16-bit type; n and k multiples of 8; x's rows may be apart.  ``y`` is (places, n), the
+    places being ``rows.numel()`` or x's rows; sums are in 32 bits, rounded once.  Rows of no expert are zeros."""
+    dev = _tensor(x, "x", _HALF, 2)
+    e, n, k = _weights_of(weight, x.dtype, dev)
+    _need(x.shape[1] == k, f"x's rows must have {k} values, not {x.shape[1]}")
+    _plan_arrays(offsets, rows, e, dev)
+    slots = rows.numel() if rows is not None else x.shape[0]
+    _need(slots == 0 or x.shape[0] > 0, "x has no rows to take")
+    out = _out(out, (slots, n), x.dtype, x.device)
+    d = Desc(tokens=x.shape[0], slots=slots, experts=e, n=n, k=k, type=_TYPE[x.dtype], out_type=_TYPE[x.dtype], in_stride=_rows_of(x, "x"))
+    return _grouped(_FORWARD, "grouped_matmul", d, (x, weight, offsets, rows), out, offsets, dev)
+
+
+@_operator
+def grouped_matmul_dx(dy: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dx[i] = weight[e].T @ dy[i]``: the gradient of ``grouped_matmul`` with respect to the rows it took, one for each place (``combine(dx,
+    slots)`` adds a token's).  ``dy`` (places, n), its rows may be apart."""
+    dev = _tensor(dy, "dy", _HALF, 2)
+    e, n, k = _weights_of(weight, dy.dtype, dev)
+    _need(dy.shape[1] == n, f"dy's rows must have {n} values, not {dy.shape[1]}")
+    _plan_arrays(offsets, None, e, dev)
+    slots = dy.shape[0]
+    out = _out(out, (slots, k), dy.dtype, dy.device)
+    d = Desc(tokens=slots, slots=slots, experts=e, n=n, k=k, type=_TYPE[dy.dtype], out_type=_TYPE[dy.dtype], in_stride=_rows_of(dy, "dy"))
+    return _grouped(_DX, "grouped_matmul_dx", d, (dy, weight, offsets), out, offsets, dev)
+
+
+@_operator
+def grouped_matmul_dw(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, rows: Optional[torch.Tensor] = None,
+                      dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dw[e] = sum over e's places i of outer(dy[i], x[rows[i]])``: (experts, n, k) of ``dtype`` (the inputs', or float32); experts without
+    places have zeros."""
+    dev = _tensor(dy, "dy", _HALF, 2)
+    _tensor(x, "x", (dy.dtype,), 2, dev)
+    _need(isinstance(offsets, torch.Tensor) and offsets.dim() == 1 and offsets.numel() >= 2, "offsets must have an entry for each expert and one more")
+    e = offsets.numel() - 1
+    _need(e <= MAX_EXPERTS, f"at most {MAX_EXPERTS} experts")
+    _plan_arrays(offsets, rows, e, dev)
+    slots, n, k = dy.shape[0], dy.shape[1], x.shape[1]
+    _need(n >= 8 and k >= 8, "dy and x must have rows of at least 8 values")
+    _need((rows.numel() if rows is not None else x.shape[0]) == slots, "dy must have a row for each place")
+    _need(slots == 0 or x.shape[0] > 0, "x has no rows to take")
+    dtype = dtype or (out.dtype if out is not None else dy.dtype)
+    _need(dtype in (torch.float32, dy.dtype), f"dw is {dy.dtype} or torch.float32, not {dtype}")
+    out = _out(out, (e, n, k), dtype, dy.device)
+    d = Desc(tokens=x.shape[0], slots=slots, experts=e, n=n, k=k, type=_TYPE[dy.dtype], out_type=_TYPE[dtype], in_stride=_rows_of(dy, "dy"),
+             in2_stride=_rows_of(x, "x"))
+    return _grouped(_DW, "grouped_matmul_dw", d, (dy, x, offsets, rows), out, offsets, dev)
+
+
+def _combine_arrays(slots, weights, dev: int):
+    _tensor(slots, "slots", (torch.int32,), 2, dev)
+    _whole(slots, "slots")
+    _need(1 <= slots.shape[1] <= MAX_CHOICES, f"1 to {MAX_CHOICES} choices, not {slots.shape[1]}")
+    if weights is not None:
+        _tensor(weights, "weights", (torch.float32,), 2, dev)
+        _whole(weights, "weights")
+        _need(weights.shape == slots.shape, "weights must have the shape of slots")
+
+
+@_operator
+def combine(z: torch.Tensor, slots: torch.Tensor, weights: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``out[t] = sum_j weights[t, j] * z[slots[t, j]]`` (no weights: ones), sums in 32 bits in the order of j, rounded once; slots of -1 add nothing."""
+    dev = _tensor(z, "z", _HALF, 2)
+    _combine_arrays(slots, weights, dev)
+    _need(z.shape[1] >= 1, "z must have columns")
+    out = _out(out, (slots.shape[0], z.shape[1]), z.dtype, z.device)
+    d = Desc(tokens=slots.shape[0], slots=z.shape[0], choices=slots.shape[1], n=z.shape[1], type=_TYPE[z.dtype],
+             in_stride=_rows_of(z, "z", aligned=False))
+    ins = (ctypes.c_void_p * 3)(z.data_ptr(), slots.data_ptr(), weights.data_ptr() if weights is not None else 0)
+    outs = _pointers((out,))
+    return BoundCall(_function("expert_combine", _PLAIN), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs)), dev,
+                     (d, ins, outs, z, slots, weights, out), out)
+
+
+@_operator
+def combine_backward(dout: torch.Tensor, z: torch.Tensor, slots: torch.Tensor, weights: Optional[torch.Tensor], offsets: torch.Tensor):
+    """Gradients of ``combine``: ``dz`` (z's shape; rows from ``offsets[-1]`` on are zeros) and ``dweights`` (float32).  ``slots`` names each of
+    the other rows once, as ``route``'s does."""
+    dev = _tensor(z, "z", _HALF, 2)
+    _tensor(dout, "dout", (z.dtype,), 2, dev)
+    _combine_arrays(slots, weights, dev)
+    _tensor(offsets, "offsets", (torch.int32,), 1, dev)
+    _whole(offsets, "offsets")
+    _need(offsets.numel() >= 2, "offsets must have an entry for each expert and one more")
+    _need(z.shape[1] >= 1 and tuple(dout.shape) == (slots.shape[0], z.shape[1]), "dout must have combine's result's shape")
+    dz, dweights = torch.empty(z.shape, dtype=z.dtype, device=z.device), torch.empty(slots.shape, dtype=torch.float32, device=z.device)
+    d = Desc(tokens=slots.shape[0], slots=z.shape[0], experts=offsets.numel() - 1, choices=slots.shape[1], n=z.shape[1], type=_TYPE[z.dtype],
+             in_stride=_rows_of(dout, "dout", aligned=False), in2_stride=_rows_of(z, "z", aligned=False))
+    ins = (ctypes.c_void_p * 5)(dout.data_ptr(), z.data_ptr(), slots.data_ptr(), weights.data_ptr() if weights is not None else 0, offsets.data_ptr())
+    outs = _pointers((dz, dweights))
+    return BoundCall(_function("expert_combine_backward", _PLAIN), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs)), dev,
+                     (d, ins, outs, dout, z, slots, weights, offsets, dz, dweights), (dz, dweights))
+
+
+def _clip(tensors: Sequence[torch.Tensor], max_norm: float, outs) -> BoundCall:
+    tensors = list(tensors)
+    _need(len(tensors) > 0, "there must be a tensor")
+    dev = None
+    for i, t in enumerate(tensors):
+        _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _TYPE, f"tensor {i} must be a CUDA tensor of float32, bfloat16 or float16")
+        dev = t.device.index if dev is None else dev
+        _need(t.device.index == dev, f"tensor {i} is on cuda:{t.device.index}, not cuda:{dev}")
+        _whole(t, f"tensor {i}")
+    n = len(tensors)
+    lengths = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
+    types = (ctypes.c_int32 * n)(*[_TYPE[t.dtype] for t in tensors])
+    pin, pout, out_types = _pointers(tensors), None, None
+    if outs is not None:
+        outs = list(outs)
+        _need(len(outs) == n, f"out must have {n} tensors, not {len(outs)}")
+        for i, (o, t) in enumerate(zip(outs, tensors)):
+            _need(isinstance(o, torch.Tensor) and o.is_cuda and o.dtype in _TYPE and o.device.index == dev and o.shape == t.shape,
+                  f"out {i} must be of its tensor's shape and device, float32, bfloat16 or float16")
+            _whole(o, f"out {i}")
+        pout, out_types = _pointers(outs), (ctypes.c_int32 * n)(*[_TYPE[o.dtype] for o in outs])
+    lib = load_library()
+    need = ctypes.c_size_t()
+    _check_status(lib, lib.flexspmv_clip_gradients_bytes(n, ctypes.byref(need)), "clip_gradients")
+    ws = torch.empty(need.value // 8, dtype=torch.float64, device=tensors[0].device)
+    norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
+    args = (n, ctypes.addressof(pin), ctypes.addressof(types), ctypes.addressof(lengths), ctypes.addressof(pout) if pout is not None else None,
+            ctypes.addressof(out_types) if out_types is not None else None, float(max_norm), norm.data_ptr(), ws.data_ptr(), need.value)
+    return BoundCall(_function("clip_gradients", _CLIP), args, dev, (pin, pout, types, out_types, lengths, ws, tensors, outs), norm)
+
+
+@_operator
+def grad_norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
+    """``sqrt(sum of all squares)`` over contiguous tensors of any of the three types: one float32 on the device, the same bits every time."""
+    return _clip(tensors, 0.0, None)
+
+
+@_operator
+def clip_grad_norm(tensors: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
+    """Scales the tensors by ``min(1, max_norm / (norm + 1e-6))``, in place or into ``out`` (tensors of the same shapes, of any of the three
+    types), and returns the norm before it."""
+    tensors = list(tensors)
+    _need(max_norm >= 0, f"max_norm must not be negative or NaN: {max_norm}")
+    return _clip(tensors, max_norm, tensors if out is None else out)

@@ -446,6 +446,85 @@ int flexspmv_spmv_f64_launch_static(const flexspmv_desc *desc, const void *const
                                     void *const *outputs, void *stream);
 int flexspmv_spmv_f64_static_device_status(int32_t *d_status_out, void *stream);
 
+/*
+ * Routed expert layers (no reference counterpart): y[t] = sum_j w[t, j] * W[e[t, j]] x[t], where a router chooses each token's
+ * experts e and weights w.  It is the gather -> per-edge map -> segmented reduce of this library with the (token, choice) pairs as
+ * edges and a dense matrix, chosen by the edge's type, as the map.  flexspmv_b200/experts.py is the torch side.
+ *
+ * All matrices are row-major with contiguous rows of 16-bit values (FLEXSPMV_TYPE_BF16 or _F16); sums, softmax statistics and weights are
+ * 32-bit floats; index arrays are int32.  `slots` in the descriptor is the number of (token, choice) pairs; pairs that have no expert
+ * (all of the row's other logits are -infinity) take no place, so offsets[experts] may be less.
+ */
+enum { FLEXSPMV_TYPE_F32 = 0, FLEXSPMV_TYPE_BF16 = 1, FLEXSPMV_TYPE_F16 = 2 };
+enum { FLEXSPMV_EXPERT_RENORMALIZE = 1 };       /* flags: the chosen weights are divided by their sum */
+#define FLEXSPMV_MAX_EXPERTS 1024
+#define FLEXSPMV_MAX_CHOICES 32
+
+typedef struct flexspmv_expert_desc {
+  int64_t tokens;      /* rows of the logits, of x before the gather, of the combined result         */
+  int64_t slots;       /* rows of y, dy and z: places in expert order                                 */
+  int32_t experts;
+  int32_t choices;     /* experts that a token takes                                                  */
+  int32_t n, k;        /* an expert's matrix: n rows of k values; combine: n is the rows' width        */
+  int32_t type;        /* FLEXSPMV_TYPE_* of the inputs                                               */
+  int32_t out_type;    /* grouped_matmul_dw: of dw (the inputs' or FLEXSPMV_TYPE_F32)                 */
+  int32_t flags;
+  int32_t reserved;    /* 0 */
+  int64_t in_stride;   /* values between the rows of the first streamed input                        */
+  int64_t in2_stride;  /* and of the second                                                           */
+} flexspmv_expert_desc;
+
+/*
+ * Router.  in: logits (tokens x experts, any type).  out: weights (tokens x choices, f32), experts (the same, -1: none), offsets
+ * (experts + 1), rows (slots: the token of a place, -1 beyond the last offset), slots (tokens x choices: a pair's place, -1: none).
+ * The `choices` largest softmax values of a row, largest first, equal ones lowest expert first; logits of -infinity and NaN are never chosen
+ * (a NaN makes the row's weights NaN unless they are renormalized).  Places are in order of expert, then token.
+ * Workspace: flexspmv_expert_route_bytes.  Backward: in: dweights, logits, weights, experts; out: dlogits (tokens x experts, of the logits' type).
+ */
+int flexspmv_expert_route_bytes(const flexspmv_expert_desc *desc, size_t *bytes);
+int flexspmv_expert_route(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *d_workspace,
+                          size_t workspace_bytes, void *stream);
+int flexspmv_expert_route_backward(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *stream);
+
+/*
+ * Matrix products grouped by expert, ragged groups.  offsets (experts + 1) say which places are an expert's.
+ *   grouped_matmul     in: x, weight (experts x n x k), offsets, rows (slots entries, or null: place i is x's row i); out: y (slots x n)
+ *                      y[i] = weight[e] x[rows[i]]
+ *   grouped_matmul_dx  in: dy, weight, offsets; out: dx (slots x k);   dx[i] = weight[e]^T dy[i]
+ *   grouped_matmul_dw  in: dy, x, offsets, rows (or null); out: dw (experts x n x k);   dw[e] = sum_i dy[i] x[rows[i]]^T
+ * n, k and the strides are multiples of 8, the arrays 16-byte aligned (FLEXSPMV_ERR_ALIGN).  Rows of y and dx in no expert's places, and
+ * matrices of experts without places, are zeros.  d_status (int32 in device or page-locked memory, may be null): the kernels store
+ * FLEXSPMV_ERR_BAD_CSR there where offsets descend or leave [0, slots], or an entry of rows leaves [0, tokens) -- it counts as a row of
+ * zeros or any other row; nothing is read or written out of range -- and FLEXSPMV_ERR_TIMEOUT where a bounded wait ran out.
+ */
+enum { FLEXSPMV_GROUPED_FORWARD = 0, FLEXSPMV_GROUPED_DX = 1, FLEXSPMV_GROUPED_DW = 2 };
+int flexspmv_grouped_matmul_bytes(const flexspmv_expert_desc *desc, int32_t which, size_t *bytes);
+int flexspmv_grouped_matmul(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *d_workspace,
+                            size_t workspace_bytes, int32_t *d_status, void *stream);
+int flexspmv_grouped_matmul_dx(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *d_workspace,
+                               size_t workspace_bytes, int32_t *d_status, void *stream);
+int flexspmv_grouped_matmul_dw(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *d_workspace,
+                               size_t workspace_bytes, int32_t *d_status, void *stream);
+
+/*
+ * The end of the layer.  combine: in: z (slots x n), slots, weights (or null: ones); out: tokens x n;  out[t] = sum_j w[t, j] z[slots[t, j]].
+ * combine_backward: in: dout (tokens x n), z, slots, weights (or null), offsets; out: dz (slots x n), dweights (tokens x choices).
+ * Entries of slots outside [0, slots) add nothing and have a gradient of zero; others name a row once.  dz's rows from offsets[experts]
+ * on are zeros.  Any n; rows of 16-byte multiples that start on 16 bytes are faster.
+ */
+int flexspmv_expert_combine(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *stream);
+int flexspmv_expert_combine_backward(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *stream);
+
+/*
+ * The norm over many tensors, norm = sqrt(sum of all squares), and, where outs is not null, outs[i] = grads[i] * min(1, max_norm /
+ * (norm + 1e-6)).  grads, types, lengths, outs and out_types are HOST arrays of count entries, read before the call returns; the tensors
+ * are contiguous device memory.  outs[i] may be grads[i] of the same type, and is left alone then where the norm is within max_norm.
+ * d_norm: one float.  A norm that is not finite scales as the formula says (infinity: 0 and NaN; NaN: NaN).
+ */
+int flexspmv_clip_gradients_bytes(int32_t count, size_t *bytes);
+int flexspmv_clip_gradients(int32_t count, const void *const *grads, const int32_t *types, const int64_t *lengths, void *const *outs,
+                            const int32_t *out_types, float max_norm, float *d_norm, void *d_workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
