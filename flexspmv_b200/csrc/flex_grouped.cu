@@ -2,8 +2,11 @@
 //   forward  y[i] = W[e] x[rows[i]]        dx  dx[i] = W[e]^T dy[i]        dw  dW[e] = sum_i dy[i] x[rows[i]]^T
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "flex_common.cuh"
 #include "flex_expert_types.cuh"
+#include "flex_umma.cuh"
 
 namespace flex {
 
@@ -37,73 +40,369 @@ __device__ __forceinline__ long long row_of(const GroupedArgs& a, int place) {
   return r;
 }
 
-// 64 x 64 outputs by 256 threads, 16 of the inner length at a time through shared memory.
-template <class T, class TO, int MODE>
-__global__ void __launch_bounds__(256) grouped_simple_kernel(GroupedArgs a) {
-  __shared__ float sa[16][65], sb[16][65];
-  const int e = blockIdx.z, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  int from, to;
-  group_of(a, e, from, to);
-  const T *pa = static_cast<const T*>(a.a), *pb = static_cast<const T*>(a.b);
-  const int cols = MODE == FLEXSPMV_GROUPED_FORWARD ? a.n : a.k;
-  const int inner = MODE == FLEXSPMV_GROUPED_FORWARD ? a.k : MODE == FLEXSPMV_GROUPED_DX ? a.n : to - from;
-  const int m_end = MODE == FLEXSPMV_GROUPED_DW ? a.n : to - from;
-  const int c0 = blockIdx.x * 64;
-  for (int m0 = blockIdx.y * 64; m0 < m_end; m0 += gridDim.y * 64) {
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < inner; k0 += 16) {
-      for (int i = tid; i < 1024; i += 256) {
-        const int kk = i & 15, r = i >> 4, k = k0 + kk;
-        float va = 0.f, vb = 0.f;
-        if (k < inner) {
-          if (m0 + r < m_end) {
-            if (MODE == FLEXSPMV_GROUPED_FORWARD) va = to_float(pa[row_of(a, from + m0 + r) * a.a_stride + k]);
-            else if (MODE == FLEXSPMV_GROUPED_DX) va = to_float(pa[(long long)(from + m0 + r) * a.a_stride + k]);
-            else va = to_float(pa[(long long)(from + k) * a.a_stride + m0 + r]);
+// One CTA an SM walks over tiles of 128 rows by NT columns of the accumulator; the accumulator's rows are a matrix side, so that
+//   forward, dx   128 values of y (dx) by up to NT places: the weights are the first operand, and a group's last tile is as narrow as its
+//                 rows need (a multiple of 16), down to one place
+//   dw            128 of n by 256 of k, summed over the expert's places
+// Warps 0-3 store finished accumulators, warp 4 issues the tile copies, warp 5 the matrix instructions; two accumulators in tensor memory,
+// so that one is stored while the next is computed.  The sum goes 64 values (128 bytes of a row) a stage.
+constexpr int kGroupedThreads = 192;
+constexpr int kTileBytesA = 128 * 128;
+constexpr uint64_t kWaitLimitNs = 1000000000ull;
+
+template <int MODE, int NT>
+struct GroupedCfg {
+  static constexpr int kBytesB = NT * 128;
+  static constexpr int kStageBytes = kTileBytesA + kBytesB;
+  static constexpr int kStages = NT > 64 ? 4 : 9;
+  static constexpr int kTmemCols = 2 * NT < 32 ? 32 : 2 * NT;
+  static constexpr int kStoreBytes = MODE == FLEXSPMV_GROUPED_DW ? 4 * 4096 : 4 * 2048;
+};
+
+struct GroupedTable {            // of an expert: its first place, its places, its first tile; and of one past the last: the number of tiles
+  int from, count, first;
+};
+
+struct GroupedBars {
+  uint64_t full[9], empty[9], acc_full[2], acc_empty[2];
+  uint32_t tmem;
+  int abort;
+};
+
+struct GroupedTile {
+  int e, m0, n0, from, count, cols;     // dw: m0 of n, n0 of k; else m0 of the features, places from .. from + count; cols: the accumulator's
+};
+
+// How many places a tile of a group of `count` takes: the group in equal parts, in 16s.
+template <int NT>
+__device__ __forceinline__ int tile_places(int count) {
+  const int tiles = (count + NT - 1) / NT;
+  return ((count + tiles - 1) / tiles + 15) & ~15;
+}
+
+template <int MODE, int NT>
+__device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const GroupedTable* table, int t) {
+  GroupedTile r;
+  const int m = MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n;
+  const int m_tiles = (m + 127) / 128;
+  if (MODE == FLEXSPMV_GROUPED_DW) {
+    const int n_tiles = (a.k + NT - 1) / NT, each = m_tiles * n_tiles;
+    r.e = t / each;
+    const int i = t - r.e * each;
+    r.m0 = i / n_tiles * 128;
+    r.n0 = i % n_tiles * NT;
+    r.from = table[r.e].from;
+    r.count = table[r.e].count;
+    const int left = a.k - r.n0;
+    r.cols = left < NT ? (left + 15) & ~15 : NT;
+    return r;
+  }
+  int lo = 0, hi = a.experts;             // the last expert whose first tile is at or before t
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (table[mid].first <= t) lo = mid;
+    else hi = mid;
+  }
+  r.e = lo;
+  const int i = t - table[lo].first, size = tile_places<NT>(table[lo].count), part = i / m_tiles * size;
+  r.m0 = i % m_tiles * 128;
+  r.n0 = 0;
+  r.from = table[lo].from + part;
+  r.count = table[lo].count - part < size ? table[lo].count - part : size;
+  r.cols = (r.count + 15) & ~15;
+  return r;
+}
+
+template <class T, class TO, int MODE, int NT>
+__global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                                     GroupedArgs a) {
+  using Cfg = GroupedCfg<MODE, NT>;
+  extern __shared__ __align__(1024) unsigned char grouped_sm[];
+  unsigned char* const base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(grouped_sm) + 1023) & ~(uintptr_t)1023);
+  unsigned char* const store = base + Cfg::kStages * Cfg::kStageBytes;
+  GroupedBars& bars = *reinterpret_cast<GroupedBars*>(store + Cfg::kStoreBytes);
+  GroupedTable* const table = reinterpret_cast<GroupedTable*>(&bars + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr bool kA_mn = MODE != FLEXSPMV_GROUPED_FORWARD, kB_mn = MODE == FLEXSPMV_GROUPED_DW;
+
+  if (tid == 0) {
+    for (int i = 0; i < Cfg::kStages; ++i) { mbar_init(&bars.full[i], 1); mbar_init(&bars.empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&bars.acc_full[i], 1); mbar_init(&bars.acc_empty[i], 4); }
+    bars.abort = 0;
+    mbar_fence_init();
+    tma_prefetch_map(&map_a);
+    tma_prefetch_map(&map_b);
+  }
+  if (warp == 5) tmem_alloc<Cfg::kTmemCols>(&bars.tmem);
+  pdl_wait();
+  for (int e = tid; e < a.experts; e += kGroupedThreads) {
+    int from, to;
+    group_of(a, e, from, to);
+    table[e].from = from;
+    table[e].count = to - from;
+  }
+  __syncthreads();
+  const int m_tiles = ((MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n) + 127) / 128;
+  if (warp == 0) {                         // exclusive sums of the experts' tiles
+    int done = 0;
+    for (int e0 = 0; e0 <= a.experts; e0 += 32) {
+      const int e = e0 + lane;
+      const int n = e < a.experts ? (table[e].count + NT - 1) / NT * m_tiles : 0;
+      int s = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += up;
+      }
+      if (e <= a.experts) table[e].first = done + s - n;
+      done += __shfl_sync(0xffffffffu, s, 31);
+    }
+  }
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = bars.tmem;
+  const int tiles = MODE == FLEXSPMV_GROUPED_DW ? a.experts * m_tiles * ((a.k + NT - 1) / NT) : table[a.experts].first;
+  volatile int* const abort = &bars.abort;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (*abort) return false;
+    if (mbar_wait_bounded(bar, parity, kWaitLimitNs)) return true;
+    *abort = 1;
+    raise(a.status, FLEXSPMV_ERR_TIMEOUT);
+    return false;
+  };
+  auto steps_of = [&](const GroupedTile& t) {
+    return ((MODE == FLEXSPMV_GROUPED_FORWARD ? a.k : MODE == FLEXSPMV_GROUPED_DX ? a.n : t.count) + 63) / 64;
+  };
+
+  if (warp == 4) {
+    int stage = 0;
+    uint32_t phase = 0;
+    int issued = 0;
+    for (int i = blockIdx.x; i < tiles && !*abort; i += gridDim.x) {
+      const GroupedTile t = tile_at<MODE, NT>(a, table, i);
+      const int steps = steps_of(t);
+      // the rows of x that this lane copies, four at a time
+      int row[2][4];
+      if (MODE == FLEXSPMV_GROUPED_FORWARD && a.rows) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int p = (lane + 32 * u) * 4 + j;
+            row[u][j] = (int)row_of(a, t.from + (p < t.count ? p : t.count - 1));
           }
-          if (c0 + r < cols) {
-            if (MODE == FLEXSPMV_GROUPED_FORWARD) vb = to_float(pb[((long long)e * a.n + c0 + r) * a.k + k]);
-            else if (MODE == FLEXSPMV_GROUPED_DX) vb = to_float(pb[((long long)e * a.n + k) * a.k + c0 + r]);
-            else vb = to_float(pb[row_of(a, from + k) * a.b_stride + c0 + r]);
+      }
+      for (int s = 0; s < steps; ++s) {
+        if (!wait(&bars.empty[stage], phase ^ 1)) break;
+        unsigned char* const sa = base + stage * Cfg::kStageBytes;
+        unsigned char* const sb = sa + kTileBytesA;
+        const uint32_t bar = smem_u32(&bars.full[stage]);
+        if (MODE == FLEXSPMV_GROUPED_DW) {
+          const int groups = (t.cols + 63) / 64, place = t.from + s * 64;
+          if (lane == 0) {
+            mbar_expect_tx(&bars.full[stage], kTileBytesA + groups * 8192);
+            tma_2d(sa, &map_a, t.m0, place, bar);
+            tma_2d(sa + 8192, &map_a, t.m0 + 64, place, bar);
+          }
+          __syncwarp();
+          if (a.rows) {
+            const int p = s * 64 + (lane & 15) * 4, last = t.count - 1;
+            int r[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = (int)row_of(a, t.from + (p + j < last ? p + j : last));
+            for (int g = lane >> 4; g < groups; g += 2)
+              tma_gather4(sb + g * 8192 + (lane & 15) * 512, &map_b, t.n0 + g * 64, r[0], r[1], r[2], r[3], bar);
+          } else if (lane < groups) {
+            tma_2d(sb + lane * 8192, &map_b, t.n0 + lane * 64, place, bar);
+          }
+        } else {
+          const int pieces = a.rows ? t.cols / 4 : (t.cols + 31) / 32;
+          if (lane == 0) {
+            mbar_expect_tx(&bars.full[stage], kTileBytesA + pieces * (a.rows ? 512 : 4096));
+            if (MODE == FLEXSPMV_GROUPED_FORWARD) {
+              tma_3d(sa, &map_a, s * 64, t.m0, t.e, bar);
+            } else {
+              tma_3d(sa, &map_a, t.m0, s * 64, t.e, bar);
+              tma_3d(sa + 8192, &map_a, t.m0 + 64, s * 64, t.e, bar);
+            }
+          }
+          __syncwarp();
+          if (MODE == FLEXSPMV_GROUPED_FORWARD && a.rows) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int g = lane + 32 * u;
+              if (g < pieces) tma_gather4(sb + g * 512, &map_b, s * 64, row[u][0], row[u][1], row[u][2], row[u][3], bar);
+            }
+          } else if (lane < pieces) {
+            tma_2d(sb + lane * 4096, &map_b, s * 64, t.from + lane * 32, bar);
           }
         }
-        sa[kk][r] = va;
-        sb[kk][r] = vb;
+        ++issued;
+        if (++stage == Cfg::kStages) { stage = 0; phase ^= 1; }
       }
-      __syncthreads();
-#pragma unroll
-      for (int kk = 0; kk < 16; ++kk)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[kk][ty + 16 * i], sb[kk][tx + 16 * j], acc[i][j]);
-      __syncthreads();
     }
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j) {
-        const int m = m0 + ty + 16 * i, c = c0 + tx + 16 * j;
-        if (m >= m_end || c >= cols) continue;
-        const long long at = MODE == FLEXSPMV_GROUPED_DW ? ((long long)e * a.n + m) * a.k + c : (long long)(from + m) * cols + c;
-        static_cast<TO*>(a.out)[at] = from_float<TO>(acc[i][j]);
+    if (*abort) {                          // copies in flight land before the CTA leaves
+      for (int i = 0; i < Cfg::kStages && i < issued; ++i) {
+        if (stage == 0) { stage = Cfg::kStages; phase ^= 1; }
+        --stage;
+        mbar_wait_bounded(&bars.full[stage], phase, kWaitLimitNs);
       }
-  }
-  // rows in no expert's places
-  if (MODE != FLEXSPMV_GROUPED_DW && (e == 0 || e == a.experts - 1)) {
-    const long long lo = e == 0 ? 0 : to, hi = e == 0 ? from : a.slots;
-    for (int part = 0; part < (a.experts == 1 ? 2 : 1); ++part) {
-      const long long l = part ? to : lo, h = part ? a.slots : hi;
-      for (long long m = l + blockIdx.y; m < h; m += gridDim.y)
-        for (int c = c0 + tid; c < cols && c < c0 + 64; c += 256) static_cast<TO*>(a.out)[m * cols + c] = from_float<TO>(0.f);
+    }
+  } else if (warp == 5) {
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    const bool bf16 = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value;
+    for (int i = blockIdx.x; i < tiles && !*abort; i += gridDim.x) {
+      const GroupedTile t = tile_at<MODE, NT>(a, table, i);
+      const int steps = steps_of(t);
+      if (MODE == FLEXSPMV_GROUPED_DW && steps == 0) continue;
+      if (!wait(&bars.acc_empty[acc], acc_phase ^ 1)) break;
+      tmem_fence_after();
+      const uint32_t d = tmem + acc * NT, instr = umma_instr(bf16, kA_mn, kB_mn, 128, t.cols);
+      for (int s = 0; s < steps; ++s) {
+        if (!wait(&bars.full[stage], phase)) break;
+        tmem_fence_after();
+        const uint32_t sa = smem_u32(base + stage * Cfg::kStageBytes), sb = sa + kTileBytesA;
+        int inner = 4;                     // matrix instructions of this step, 16 of the sum each
+        if (MODE == FLEXSPMV_GROUPED_DW && t.count - s * 64 < 64) {
+          // the group ends in this step: what follows it in the copied rows must not count, whatever it holds
+          const int valid = t.count - s * 64, groups = 2 + (t.cols + 63) / 64;
+          inner = (valid + 15) / 16;
+          const int clear = (inner * 16 - valid) * 8;
+          for (int x = lane; x < groups * clear; x += 32) {
+            const int g = x / clear, c = x - g * clear;
+            *reinterpret_cast<uint4*>(base + stage * Cfg::kStageBytes + g * 8192 + valid * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (elect_one()) {
+          for (int x = 0; x < inner; ++x) {
+            const uint64_t da = kA_mn ? umma_desc(sa + x * 2048, 8192, 1024) : umma_desc(sa + x * 32, 16, 1024);
+            const uint64_t db = kB_mn ? umma_desc(sb + x * 2048, 8192, 1024) : umma_desc(sb + x * 32, 16, 1024);
+            umma(d, da, db, instr, (s | x) != 0);
+          }
+          umma_commit(&bars.empty[stage]);
+          if (s + 1 == steps) umma_commit(&bars.acc_full[acc]);
+        }
+        __syncwarp();
+        if (++stage == Cfg::kStages) { stage = 0; phase ^= 1; }
+      }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+  } else {
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    TO* const out = static_cast<TO*>(a.out);
+    unsigned char* const mine = store + warp * (Cfg::kStoreBytes / 4);
+    for (int i = blockIdx.x; i < tiles && !*abort; i += gridDim.x) {
+      const GroupedTile t = tile_at<MODE, NT>(a, table, i);
+      const int m = t.m0 + warp * 32;      // this warp's first row of the accumulator
+      if (MODE == FLEXSPMV_GROUPED_DW && t.count == 0) {
+        constexpr int kW = 16 / (int)sizeof(TO);
+        const int pieces = t.cols / kW;
+        for (int x = lane; x < 32 * pieces; x += 32) {
+          const int r = m + x / pieces, c = t.n0 + x % pieces * kW;
+          if (r < a.n && c < a.k) *reinterpret_cast<uint4*>(out + ((size_t)t.e * a.n + r) * a.k + c) = make_uint4(0, 0, 0, 0);
+        }
+        continue;
+      }
+      if (!wait(&bars.acc_full[acc], acc_phase)) break;
+      tmem_fence_after();
+      const uint32_t d = tmem + acc * NT + ((uint32_t)(warp * 32) << 16);
+      for (int c0 = 0; c0 < t.cols; c0 += 32) {
+        uint32_t v[32];
+        tmem_load32(d + c0, v);
+        if (c0 + 32 >= t.cols) {           // the accumulator is free once the last of it is in registers
+          tmem_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.acc_empty[acc]);
+        }
+        if (MODE == FLEXSPMV_GROUPED_DW) {
+          // lane l holds 32 columns of row m + l: through shared memory, so that a row's pieces leave together
+          constexpr int kP = 32 * (int)sizeof(TO) / 16, kW = 16 / (int)sizeof(TO);          // 16-byte pieces of a row
+#pragma unroll
+          for (int p = 0; p < kP; ++p) {
+            Pack<TO, kW> q;
+#pragma unroll
+            for (int x = 0; x < kW; ++x) q.set(x, __uint_as_float(v[p * kW + x]));
+            reinterpret_cast<uint4*>(mine)[lane * kP + (p ^ (kP == 8 ? lane & 7 : (lane >> 1) & 3))] = q.raw[0];
+          }
+          __syncwarp();
+#pragma unroll
+          for (int x = 0; x < kP; ++x) {
+            const int at = x * 32 + lane, r = at / kP, p = at % kP;
+            const uint4 q = reinterpret_cast<const uint4*>(mine)[r * kP + (p ^ (kP == 8 ? r & 7 : (r >> 1) & 3))];
+            const int c = t.n0 + c0 + p * kW;
+            if (m + r < a.n && c < a.k) *reinterpret_cast<uint4*>(out + ((size_t)t.e * a.n + m + r) * a.k + c) = q;
+          }
+          __syncwarp();
+        } else {
+          // lane l holds 32 places of feature m + l: turned in shared memory into rows of 32 features a place
+#pragma unroll
+          for (int x = 0; x < 32; ++x) reinterpret_cast<TO*>(mine)[x * 32 + lane] = from_float<TO>(__uint_as_float(v[x]));
+          __syncwarp();
+          const int width = MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int p = x * 8 + (lane >> 2), c = m + (lane & 3) * 8;
+            if (c0 + p < t.count && c < width)
+              *reinterpret_cast<uint4*>(out + (size_t)(t.from + c0 + p) * width + c) = reinterpret_cast<const uint4*>(mine)[p * 4 + (lane & 3)];
+          }
+          __syncwarp();
+        }
+      }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+    if (MODE != FLEXSPMV_GROUPED_DW) {     // places of no expert: before the first group and after the last
+      const int width = (MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n) / 8;
+      const long long head = table[0].from, tail = table[a.experts - 1].from + table[a.experts - 1].count, none = head + a.slots - tail;
+      for (long long x = blockIdx.x; x < none; x += gridDim.x) {
+        uint4* const row = reinterpret_cast<uint4*>(out + (size_t)(x < head ? x : tail + x - head) * width * 8);
+        for (int c = tid; c < width; c += 128) row[c] = make_uint4(0, 0, 0, 0);
+      }
     }
   }
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  if (warp == 5) tmem_free<Cfg::kTmemCols>(tmem);
+}
+
+template <class T, class TO, int MODE, int NT>
+static int grouped_launch_as(const GroupedArgs& a, cudaStream_t st) {
+  using Cfg = GroupedCfg<MODE, NT>;
+  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  CUtensorMap ma, mb;
+  if (MODE == FLEXSPMV_GROUPED_DW) {
+    const uint64_t da[2] = {(uint64_t)a.n, (uint64_t)(a.slots ? a.slots : 1)}, sa[1] = {(uint64_t)a.a_stride};
+    const uint64_t db[2] = {(uint64_t)a.k, (uint64_t)(a.tokens ? a.tokens : 1)}, sb[1] = {(uint64_t)a.b_stride};
+    const uint32_t box[2] = {64, 64}, one[2] = {64, 1};
+    if (int e = make_map(&ma, a.slots ? a.a : a.out, bf16, 2, da, sa, box)) return e;
+    if (int e = make_map(&mb, a.slots ? a.b : a.out, bf16, 2, db, sb, a.rows ? one : box)) return e;
+  } else {
+    const uint64_t dw[3] = {(uint64_t)a.k, (uint64_t)a.n, (uint64_t)a.experts}, sw[2] = {(uint64_t)a.k, (uint64_t)a.k * a.n};
+    const uint32_t wide[3] = {64, 128, 1}, high[3] = {64, 64, 1};
+    if (int e = make_map(&ma, a.b, bf16, 3, dw, sw, MODE == FLEXSPMV_GROUPED_FORWARD ? wide : high)) return e;
+    const uint64_t dx[2] = {(uint64_t)(MODE == FLEXSPMV_GROUPED_FORWARD ? a.k : a.n), (uint64_t)a.tokens}, sx[1] = {(uint64_t)a.a_stride};
+    const uint32_t box[2] = {64, 32}, one[2] = {64, 1};
+    if (int e = make_map(&mb, a.a, bf16, 2, dx, sx, a.rows ? one : box)) return e;
+  }
+  const int smem = 1024 + Cfg::kStages * Cfg::kStageBytes + Cfg::kStoreBytes + (int)sizeof(GroupedBars) + (a.experts + 1) * (int)sizeof(GroupedTable);
+  auto kernel = grouped_kernel<T, TO, MODE, NT>;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return (int)e;
+  return launch_pdl(kernel, device_sm_count(), kGroupedThreads, smem, st, ma, mb, a);
 }
 
 template <class T, class TO, int MODE>
 static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
-  const int cols = MODE == FLEXSPMV_GROUPED_FORWARD ? a.n : a.k;
-  const int m = MODE == FLEXSPMV_GROUPED_DW ? (a.n + 63) / 64 : 16;
-  grouped_simple_kernel<T, TO, MODE><<<dim3((cols + 63) / 64, m, a.experts), 256, 0, st>>>(a);
-  return (int)cudaGetLastError();
+  if constexpr (MODE == FLEXSPMV_GROUPED_DW) {
+    return grouped_launch_as<T, TO, MODE, 256>(a, st);
+  } else {
+    if (a.slots <= 16ll * a.experts) return grouped_launch_as<T, TO, MODE, 32>(a, st);
+    return grouped_launch_as<T, TO, MODE, 256>(a, st);
+  }
 }
 
 static int check_grouped(const flexspmv_expert_desc* d, int which) {
@@ -112,6 +411,10 @@ static int check_grouped(const flexspmv_expert_desc* d, int which) {
   if (which == FLEXSPMV_GROUPED_DW && d->out_type != FLEXSPMV_TYPE_F32 && d->out_type != d->type) return FLEXSPMV_ERR_BAD_ARG;
   if (d->in_stride < (which == FLEXSPMV_GROUPED_FORWARD ? d->k : d->n) || (which == FLEXSPMV_GROUPED_DW && d->in2_stride < d->k)) return FLEXSPMV_ERR_BAD_ARG;
   if (d->experts > FLEXSPMV_MAX_EXPERTS || d->slots > 0x7fffffffLL || d->tokens > 0x7fffffffLL) return FLEXSPMV_ERR_TOO_LARGE;
+  // tiles and places are counted in 32 bits
+  const long long sides = (long long)((d->n + 127) / 128) * ((d->k + 127) / 128);
+  if (d->slots > 0x7fff0000LL || sides > 0x7fffffffLL / d->experts || (d->slots / 32 + d->experts) > 0x7fffffffLL / ((d->n > d->k ? d->n : d->k) / 128 + 1))
+    return FLEXSPMV_ERR_TOO_LARGE;
   if (d->n % 8 || d->k % 8 || d->in_stride % 8 || (which == FLEXSPMV_GROUPED_DW && d->in2_stride % 8)) return FLEXSPMV_ERR_ALIGN;
   return 0;
 }
