@@ -14,9 +14,9 @@ int device_sm_count();
 
 struct GroupedArgs {
   const void *a, *b;             // forward: x, weight; dx: dy, weight; dw: dy, x
-  const int *offsets, *rows;
+  const int* offsets;
   void* out;
-  long long tokens, slots, a_stride, b_stride;
+  long long slots, a_stride, b_stride;
   int experts, n, k;
   int* status;
 };
@@ -33,28 +33,40 @@ __device__ __forceinline__ void group_of(const GroupedArgs& a, int e, int& from,
   if (f != from || t != to) raise(a.status, FLEXSPMV_ERR_BAD_CSR);
 }
 
-__device__ __forceinline__ long long row_of(const GroupedArgs& a, int place) {
-  if (!a.rows) return place;
-  const int r = a.rows[place];
-  if (r < 0 || r >= a.tokens) { raise(a.status, FLEXSPMV_ERR_BAD_CSR); return 0; }
-  return r;
+// The rows of x in the places' order: a copy in the workspace, so that the products' tiles are tiles of a matrix.  (Tile copies that gather four
+// rows each took 72 cycles an instruction here: 2.2 ms for 32 768 rows of 2048 against 4096 columns, 0.51 ms from contiguous rows.)
+__global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict__ x, const int* __restrict__ rows, const int* __restrict__ offsets, uint4* __restrict__ out,
+                                                        long long tokens, long long slots, long long stride, int experts, int pieces, int* status) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const long long from = offsets[0] < 0 ? 0 : offsets[0], to = offsets[experts] < slots ? offsets[experts] : slots;
+  const long long work = (to - from) * pieces;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < work; i += (long long)gridDim.x * 256) {
+    const long long p = from + i / pieces;
+    const int c = (int)(i % pieces), r = rows[p];
+    const bool in = r >= 0 && r < tokens;
+    if (!in) raise(status, FLEXSPMV_ERR_BAD_CSR);
+    out[p * pieces + c] = in ? x[r * stride + c] : make_uint4(0, 0, 0, 0);
+  }
 }
 
 // One CTA an SM walks over tiles of 128 rows by NT columns of the accumulator; the accumulator's rows are a matrix side, so that
 //   forward, dx   128 values of y (dx) by up to NT places: the weights are the first operand, and a group's last tile is as narrow as its
 //                 rows need (a multiple of 16), down to one place
 //   dw            128 of n by 256 of k, summed over the expert's places
+// PAIR = 2: two CTAs on two neighbouring SMs take a tile of 256 rows, 128 each; each copies half of the columns' operand for both, which
+// halves what those columns cost the L2 (from 48 KB to 32 KB an SM for 64 of the sum).
 // Warps 0-3 store finished accumulators, warp 4 issues the tile copies, warp 5 the matrix instructions; two accumulators in tensor memory,
 // so that one is stored while the next is computed.  The sum goes 64 values (128 bytes of a row) a stage.
 constexpr int kGroupedThreads = 192;
 constexpr int kTileBytesA = 128 * 128;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 
-template <int MODE, int NT>
+template <int MODE, int NT, int PAIR>
 struct GroupedCfg {
-  static constexpr int kBytesB = NT * 128;
+  static constexpr int kBytesB = NT / PAIR * 128;
   static constexpr int kStageBytes = kTileBytesA + kBytesB;
-  static constexpr int kStages = NT > 64 ? 4 : 9;
+  static constexpr int kStages = 196608 / kStageBytes;
   static constexpr int kTmemCols = 2 * NT < 32 ? 32 : 2 * NT;
   static constexpr int kStoreBytes = MODE == FLEXSPMV_GROUPED_DW ? 4 * 4096 : 4 * 2048;
 };
@@ -73,28 +85,30 @@ struct GroupedTile {
   int e, m0, n0, from, count, cols;     // dw: m0 of n, n0 of k; else m0 of the features, places from .. from + count; cols: the accumulator's
 };
 
-// How many places a tile of a group of `count` takes: the group in equal parts, in 16s.
-template <int NT>
+// How many places a tile of a group of `count` takes: the group in equal parts, in 16s (a pair: in 32s).
+template <int NT, int PAIR>
 __device__ __forceinline__ int tile_places(int count) {
+  constexpr int kStep = 16 * PAIR;
   const int tiles = (count + NT - 1) / NT;
-  return ((count + tiles - 1) / tiles + 15) & ~15;
+  return ((count + tiles - 1) / tiles + kStep - 1) & ~(kStep - 1);
 }
 
-template <int MODE, int NT>
+template <int MODE, int NT, int PAIR>
 __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const GroupedTable* table, int t) {
   GroupedTile r;
   const int m = MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n;
-  const int m_tiles = (m + 127) / 128;
+  const int m_tiles = (m + 128 * PAIR - 1) / (128 * PAIR);
+  constexpr int kStep = 16 * PAIR;
   if (MODE == FLEXSPMV_GROUPED_DW) {
     const int n_tiles = (a.k + NT - 1) / NT, each = m_tiles * n_tiles;
     r.e = t / each;
     const int i = t - r.e * each;
-    r.m0 = i / n_tiles * 128;
+    r.m0 = i / n_tiles * 128 * PAIR;
     r.n0 = i % n_tiles * NT;
     r.from = table[r.e].from;
     r.count = table[r.e].count;
     const int left = a.k - r.n0;
-    r.cols = left < NT ? (left + 15) & ~15 : NT;
+    r.cols = left < NT ? (left + kStep - 1) & ~(kStep - 1) : NT;
     return r;
   }
   int lo = 0, hi = a.experts;             // the last expert whose first tile is at or before t
@@ -104,36 +118,38 @@ __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const Group
     else hi = mid;
   }
   r.e = lo;
-  const int i = t - table[lo].first, size = tile_places<NT>(table[lo].count), part = i / m_tiles * size;
-  r.m0 = i % m_tiles * 128;
+  const int i = t - table[lo].first, size = tile_places<NT, PAIR>(table[lo].count), part = i / m_tiles * size;
+  r.m0 = i % m_tiles * 128 * PAIR;
   r.n0 = 0;
   r.from = table[lo].from + part;
   r.count = table[lo].count - part < size ? table[lo].count - part : size;
-  r.cols = (r.count + 15) & ~15;
+  r.cols = (r.count + kStep - 1) & ~(kStep - 1);
   return r;
 }
 
-template <class T, class TO, int MODE, int NT>
+template <class T, class TO, int MODE, int NT, int PAIR>
 __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                                     const __grid_constant__ CUtensorMap row_a, const __grid_constant__ CUtensorMap row_b,
                                                                      GroupedArgs a) {
-  using Cfg = GroupedCfg<MODE, NT>;
+  using Cfg = GroupedCfg<MODE, NT, PAIR>;
   extern __shared__ __align__(1024) unsigned char grouped_sm[];
   unsigned char* const base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(grouped_sm) + 1023) & ~(uintptr_t)1023);
   unsigned char* const store = base + Cfg::kStages * Cfg::kStageBytes;
   GroupedBars& bars = *reinterpret_cast<GroupedBars*>(store + Cfg::kStoreBytes);
   GroupedTable* const table = reinterpret_cast<GroupedTable*>(&bars + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = PAIR == 2 ? (int)cluster_rank() : 0;
   constexpr bool kA_mn = MODE != FLEXSPMV_GROUPED_FORWARD, kB_mn = MODE == FLEXSPMV_GROUPED_DW;
 
   if (tid == 0) {
     for (int i = 0; i < Cfg::kStages; ++i) { mbar_init(&bars.full[i], 1); mbar_init(&bars.empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&bars.acc_full[i], 1); mbar_init(&bars.acc_empty[i], 4); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&bars.acc_full[i], 1); mbar_init(&bars.acc_empty[i], 4 * PAIR); }
     bars.abort = 0;
     mbar_fence_init();
     tma_prefetch_map(&map_a);
     tma_prefetch_map(&map_b);
   }
-  if (warp == 5) tmem_alloc<Cfg::kTmemCols>(&bars.tmem);
+  if (warp == 5) tmem_alloc<PAIR, Cfg::kTmemCols>(&bars.tmem);
   pdl_wait();
   for (int e = tid; e < a.experts; e += kGroupedThreads) {
     int from, to;
@@ -142,7 +158,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
     table[e].count = to - from;
   }
   __syncthreads();
-  const int m_tiles = ((MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n) + 127) / 128;
+  const int m_tiles = ((MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n) + 128 * PAIR - 1) / (128 * PAIR);
   if (warp == 0) {                         // exclusive sums of the experts' tiles
     int done = 0;
     for (int e0 = 0; e0 <= a.experts; e0 += 32) {
@@ -160,11 +176,14 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
   }
   tmem_fence_before();
   __syncthreads();
+  if (PAIR == 2) cluster_sync();           // the other CTA's barriers are set up
   tmem_fence_after();
   const uint32_t tmem = bars.tmem;
   const int tiles = MODE == FLEXSPMV_GROUPED_DW ? a.experts * m_tiles * ((a.k + NT - 1) / NT) : table[a.experts].first;
+  const int first = blockIdx.x / PAIR, stride = gridDim.x / PAIR;
   volatile int* const abort = &bars.abort;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
     if (*abort) return false;
     if (mbar_wait_bounded(bar, parity, kWaitLimitNs)) return true;
     *abort = 1;
@@ -176,129 +195,98 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
   };
 
   if (warp == 4) {
-    int stage = 0;
+    int stage = 0, issued = 0;
     uint32_t phase = 0;
-    int issued = 0;
-    for (int i = blockIdx.x; i < tiles && !*abort; i += gridDim.x) {
-      const GroupedTile t = tile_at<MODE, NT>(a, table, i);
-      const int steps = steps_of(t);
-      // the rows of x that this lane copies, four at a time
-      int row[2][4];
-      if (MODE == FLEXSPMV_GROUPED_FORWARD && a.rows) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int p = (lane + 32 * u) * 4 + j;
-            row[u][j] = (int)row_of(a, t.from + (p < t.count ? p : t.count - 1));
-          }
-      }
-      for (int s = 0; s < steps; ++s) {
-        if (!wait(&bars.empty[stage], phase ^ 1)) break;
-        unsigned char* const sa = base + stage * Cfg::kStageBytes;
-        unsigned char* const sb = sa + kTileBytesA;
-        const uint32_t bar = smem_u32(&bars.full[stage]);
-        if (MODE == FLEXSPMV_GROUPED_DW) {
-          const int groups = (t.cols + 63) / 64, place = t.from + s * 64;
-          if (lane == 0) {
-            mbar_expect_tx(&bars.full[stage], kTileBytesA + groups * 8192);
-            tma_2d(sa, &map_a, t.m0, place, bar);
-            tma_2d(sa + 8192, &map_a, t.m0 + 64, place, bar);
-          }
-          __syncwarp();
-          if (a.rows) {
-            const int p = s * 64 + (lane & 15) * 4, last = t.count - 1;
-            int r[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) r[j] = (int)row_of(a, t.from + (p + j < last ? p + j : last));
-            for (int g = lane >> 4; g < groups; g += 2)
-              tma_gather4(sb + g * 8192 + (lane & 15) * 512, &map_b, t.n0 + g * 64, r[0], r[1], r[2], r[3], bar);
-          } else if (lane < groups) {
-            tma_2d(sb + lane * 8192, &map_b, t.n0 + lane * 64, place, bar);
-          }
-        } else {
-          const int pieces = a.rows ? t.cols / 4 : (t.cols + 31) / 32;
-          if (lane == 0) {
-            mbar_expect_tx(&bars.full[stage], kTileBytesA + pieces * (a.rows ? 512 : 4096));
+    if (elect_one()) {
+      for (int i = first; i < tiles && !*abort; i += stride) {
+        const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
+        const int steps = steps_of(t), half = t.cols / PAIR;
+        const int pieces = MODE == FLEXSPMV_GROUPED_DW ? (half + 63) / 64 : (half + 31) / 32;
+        const int bytes = PAIR * (kTileBytesA + pieces * 4096);
+        const int m0 = t.m0 + rank * 128;
+        for (int s = 0; s < steps; ++s) {
+          if (!wait(&bars.empty[stage], phase ^ 1)) break;
+          unsigned char* const sa = base + stage * Cfg::kStageBytes;
+          unsigned char* const sb = sa + kTileBytesA;
+          // dw: the group's rows in this step, and how many rows are copied for them
+          const int valid = t.count - s * 64 < 64 ? t.count - s * 64 : 64;
+          const int rows = MODE == FLEXSPMV_GROUPED_DW && t.from + s * 64 + valid < 64 ? (valid + 15) & ~15 : 64;
+          if (rank == 0) mbar_expect_tx(&bars.full[stage], MODE == FLEXSPMV_GROUPED_DW ? PAIR * (2 + pieces) * rows * 128 : bytes);
+          const uint32_t bar = PAIR == 2 ? cluster_smem(&bars.full[stage], 0) : smem_u32(&bars.full[stage]);
+          if (MODE == FLEXSPMV_GROUPED_DW) {
+            // A step's last rows may be the next group's.  The maps count rows by two dimensions of one stride, y + z, and y ends at 64: with the
+            // step's last valid row at y = 63, what follows it is out of range and zero.
+            const int place = t.from + s * 64, z = place + valid - 64, n0 = t.n0 + rank * half;
+            if (z >= 0) {
+              tma_3d<PAIR>(sa, &map_a, m0, 64 - valid, z, bar);
+              tma_3d<PAIR>(sa + 8192, &map_a, m0 + 64, 64 - valid, z, bar);
+              for (int g = 0; g < pieces; ++g) tma_3d<PAIR>(sb + g * 8192, &map_b, n0 + g * 64, 64 - valid, z, bar);
+            } else {                       // a group that ends in the first 64 rows: row by row, rows out of range for the rest
+              for (int r = 0; r < rows; ++r) {
+                const int y = r < valid ? place + r : (int)a.slots;
+                tma_2d<PAIR>(sa + r * 128, &row_a, m0, y, bar);
+                tma_2d<PAIR>(sa + 8192 + r * 128, &row_a, m0 + 64, y, bar);
+                for (int g = 0; g < pieces; ++g) tma_2d<PAIR>(sb + g * 8192 + r * 128, &row_b, n0 + g * 64, y, bar);
+              }
+            }
+          } else {
             if (MODE == FLEXSPMV_GROUPED_FORWARD) {
-              tma_3d(sa, &map_a, s * 64, t.m0, t.e, bar);
+              tma_3d<PAIR>(sa, &map_a, s * 64, m0, t.e, bar);
             } else {
-              tma_3d(sa, &map_a, t.m0, s * 64, t.e, bar);
-              tma_3d(sa + 8192, &map_a, t.m0 + 64, s * 64, t.e, bar);
+              tma_3d<PAIR>(sa, &map_a, m0, s * 64, t.e, bar);
+              tma_3d<PAIR>(sa + 8192, &map_a, m0 + 64, s * 64, t.e, bar);
             }
+            for (int g = 0; g < pieces; ++g) tma_2d<PAIR>(sb + g * 4096, &map_b, s * 64, t.from + rank * half + g * 32, bar);
           }
-          __syncwarp();
-          if (MODE == FLEXSPMV_GROUPED_FORWARD && a.rows) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int g = lane + 32 * u;
-              if (g < pieces) tma_gather4(sb + g * 512, &map_b, s * 64, row[u][0], row[u][1], row[u][2], row[u][3], bar);
-            }
-          } else if (lane < pieces) {
-            tma_2d(sb + lane * 4096, &map_b, s * 64, t.from + lane * 32, bar);
-          }
+          ++issued;
+          if (++stage == Cfg::kStages) { stage = 0; phase ^= 1; }
         }
-        ++issued;
-        if (++stage == Cfg::kStages) { stage = 0; phase ^= 1; }
+      }
+      if (*abort && rank == 0) {           // copies in flight land before the CTA leaves
+        for (int i = 0; i < Cfg::kStages && i < issued; ++i) {
+          if (stage == 0) { stage = Cfg::kStages; phase ^= 1; }
+          --stage;
+          mbar_wait_bounded(&bars.full[stage], phase, kWaitLimitNs);
+        }
       }
     }
-    if (*abort) {                          // copies in flight land before the CTA leaves
-      for (int i = 0; i < Cfg::kStages && i < issued; ++i) {
-        if (stage == 0) { stage = Cfg::kStages; phase ^= 1; }
-        --stage;
-        mbar_wait_bounded(&bars.full[stage], phase, kWaitLimitNs);
-      }
-    }
+    __syncwarp();
   } else if (warp == 5) {
-    int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
-    const bool bf16 = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value;
-    for (int i = blockIdx.x; i < tiles && !*abort; i += gridDim.x) {
-      const GroupedTile t = tile_at<MODE, NT>(a, table, i);
-      const int steps = steps_of(t);
-      if (MODE == FLEXSPMV_GROUPED_DW && steps == 0) continue;
-      if (!wait(&bars.acc_empty[acc], acc_phase ^ 1)) break;
-      tmem_fence_after();
-      const uint32_t d = tmem + acc * NT, instr = umma_instr(bf16, kA_mn, kB_mn, 128, t.cols);
-      for (int s = 0; s < steps; ++s) {
-        if (!wait(&bars.full[stage], phase)) break;
+    if (rank == 0 && elect_one()) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      for (int i = first; i < tiles && !*abort; i += stride) {
+        const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
+        const int steps = steps_of(t);
+        if (MODE == FLEXSPMV_GROUPED_DW && steps == 0) continue;
+        if (!wait(&bars.acc_empty[acc], acc_phase ^ 1)) break;
         tmem_fence_after();
-        const uint32_t sa = smem_u32(base + stage * Cfg::kStageBytes), sb = sa + kTileBytesA;
-        int inner = 4;                     // matrix instructions of this step, 16 of the sum each
-        if (MODE == FLEXSPMV_GROUPED_DW && t.count - s * 64 < 64) {
-          // the group ends in this step: what follows it in the copied rows must not count, whatever it holds
-          const int valid = t.count - s * 64, groups = 2 + (t.cols + 63) / 64;
-          inner = (valid + 15) / 16;
-          const int clear = (inner * 16 - valid) * 8;
-          for (int x = lane; x < groups * clear; x += 32) {
-            const int g = x / clear, c = x - g * clear;
-            *reinterpret_cast<uint4*>(base + stage * Cfg::kStageBytes + g * 8192 + valid * 128 + c * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
+        const uint32_t d = tmem + acc * NT, instr = umma_instr(std::is_same<T, __nv_bfloat16>::value, kA_mn, kB_mn, 128 * PAIR, t.cols);
+        for (int s = 0; s < steps; ++s) {
+          if (!wait(&bars.full[stage], phase)) break;
+          tmem_fence_after();
+          const uint32_t sa = smem_u32(base + stage * Cfg::kStageBytes), sb = sa + kTileBytesA;
+          const uint64_t da = kA_mn ? umma_desc(sa, 8192, 1024) : umma_desc(sa, 16, 1024);
+          const uint64_t db = kB_mn ? umma_desc(sb, 8192, 1024) : umma_desc(sb, 16, 1024);
+          const int inner = MODE == FLEXSPMV_GROUPED_DW && t.count - s * 64 < 64 ? (t.count - s * 64 + 15) / 16 : 4;
+          for (int x = 0; x < inner; ++x)  // the descriptors' addresses are in 16 bytes
+            umma<PAIR>(d, da + x * (kA_mn ? 128 : 2), db + x * (kB_mn ? 128 : 2), instr, (s | x) != 0);
+          umma_commit<PAIR>(&bars.empty[stage]);
+          if (s + 1 == steps) umma_commit<PAIR>(&bars.acc_full[acc]);
+          if (++stage == Cfg::kStages) { stage = 0; phase ^= 1; }
         }
-        if (elect_one()) {
-          for (int x = 0; x < inner; ++x) {
-            const uint64_t da = kA_mn ? umma_desc(sa + x * 2048, 8192, 1024) : umma_desc(sa + x * 32, 16, 1024);
-            const uint64_t db = kB_mn ? umma_desc(sb + x * 2048, 8192, 1024) : umma_desc(sb + x * 32, 16, 1024);
-            umma(d, da, db, instr, (s | x) != 0);
-          }
-          umma_commit(&bars.empty[stage]);
-          if (s + 1 == steps) umma_commit(&bars.acc_full[acc]);
-        }
-        __syncwarp();
-        if (++stage == Cfg::kStages) { stage = 0; phase ^= 1; }
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
-      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
+    __syncwarp();
   } else {
     int acc = 0;
     uint32_t acc_phase = 0;
     TO* const out = static_cast<TO*>(a.out);
     unsigned char* const mine = store + warp * (Cfg::kStoreBytes / 4);
-    for (int i = blockIdx.x; i < tiles && !*abort; i += gridDim.x) {
-      const GroupedTile t = tile_at<MODE, NT>(a, table, i);
-      const int m = t.m0 + warp * 32;      // this warp's first row of the accumulator
+    for (int i = first; i < tiles && !*abort; i += stride) {
+      const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
+      const int m = t.m0 + rank * 128 + warp * 32;      // this warp's first row of the accumulator
       if (MODE == FLEXSPMV_GROUPED_DW && t.count == 0) {
         constexpr int kW = 16 / (int)sizeof(TO);
         const int pieces = t.cols / kW;
@@ -317,7 +305,10 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
         if (c0 + 32 >= t.cols) {           // the accumulator is free once the last of it is in registers
           tmem_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.acc_empty[acc]);
+          if (lane == 0) {
+            if (PAIR == 2) mbar_arrive_cluster(cluster_smem(&bars.acc_empty[acc], 0));
+            else mbar_arrive(&bars.acc_empty[acc]);
+          }
         }
         if (MODE == FLEXSPMV_GROUPED_DW) {
           // lane l holds 32 columns of row m + l: through shared memory, so that a row's pieces leave together
@@ -366,43 +357,76 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
   }
   tmem_fence_before();
   __syncthreads();
+  if (PAIR == 2) cluster_sync();           // neither CTA leaves while the other's instructions may reach its memory
   tmem_fence_after();
-  if (warp == 5) tmem_free<Cfg::kTmemCols>(tmem);
+  if (warp == 5) tmem_free<PAIR, Cfg::kTmemCols>(tmem);
 }
 
-template <class T, class TO, int MODE, int NT>
+template <class T, class TO, int MODE, int NT, int PAIR>
 static int grouped_launch_as(const GroupedArgs& a, cudaStream_t st) {
-  using Cfg = GroupedCfg<MODE, NT>;
+  using Cfg = GroupedCfg<MODE, NT, PAIR>;
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-  CUtensorMap ma, mb;
+  CUtensorMap ma, mb, row_a, row_b;
   if (MODE == FLEXSPMV_GROUPED_DW) {
-    const uint64_t da[2] = {(uint64_t)a.n, (uint64_t)(a.slots ? a.slots : 1)}, sa[1] = {(uint64_t)a.a_stride};
-    const uint64_t db[2] = {(uint64_t)a.k, (uint64_t)(a.tokens ? a.tokens : 1)}, sb[1] = {(uint64_t)a.b_stride};
-    const uint32_t box[2] = {64, 64}, one[2] = {64, 1};
-    if (int e = make_map(&ma, a.slots ? a.a : a.out, bf16, 2, da, sa, box)) return e;
-    if (int e = make_map(&mb, a.slots ? a.b : a.out, bf16, 2, db, sb, a.rows ? one : box)) return e;
+    const uint64_t rows = a.slots ? a.slots : 1;
+    const uint64_t da[3] = {(uint64_t)a.n, 64, rows}, sa[2] = {(uint64_t)a.a_stride, (uint64_t)a.a_stride};
+    const uint64_t db[3] = {(uint64_t)a.k, 64, rows}, sb[2] = {(uint64_t)a.b_stride, (uint64_t)a.b_stride};
+    const uint64_t ra[2] = {(uint64_t)a.n, rows}, rb[2] = {(uint64_t)a.k, rows};
+    const uint32_t box[3] = {64, 64, 1}, one[2] = {64, 1};
+    const void *pa = a.slots ? a.a : a.out, *pb = a.slots ? a.b : a.out;          // without rows nothing is copied
+    if (int e = make_map(&ma, pa, bf16, 3, da, sa, box)) return e;
+    if (int e = make_map(&mb, pb, bf16, 3, db, sb, box)) return e;
+    if (int e = make_map(&row_a, pa, bf16, 2, ra, sa, one)) return e;
+    if (int e = make_map(&row_b, pb, bf16, 2, rb, sb, one)) return e;
   } else {
     const uint64_t dw[3] = {(uint64_t)a.k, (uint64_t)a.n, (uint64_t)a.experts}, sw[2] = {(uint64_t)a.k, (uint64_t)a.k * a.n};
     const uint32_t wide[3] = {64, 128, 1}, high[3] = {64, 64, 1};
     if (int e = make_map(&ma, a.b, bf16, 3, dw, sw, MODE == FLEXSPMV_GROUPED_FORWARD ? wide : high)) return e;
-    const uint64_t dx[2] = {(uint64_t)(MODE == FLEXSPMV_GROUPED_FORWARD ? a.k : a.n), (uint64_t)a.tokens}, sx[1] = {(uint64_t)a.a_stride};
-    const uint32_t box[2] = {64, 32}, one[2] = {64, 1};
-    if (int e = make_map(&mb, a.a, bf16, 2, dx, sx, a.rows ? one : box)) return e;
+    const uint64_t dx[2] = {(uint64_t)(MODE == FLEXSPMV_GROUPED_FORWARD ? a.k : a.n), (uint64_t)a.slots}, sx[1] = {(uint64_t)a.a_stride};
+    const uint32_t box[2] = {64, 32};
+    if (int e = make_map(&mb, a.a, bf16, 2, dx, sx, box)) return e;
+    row_a = ma;
+    row_b = mb;
   }
   const int smem = 1024 + Cfg::kStages * Cfg::kStageBytes + Cfg::kStoreBytes + (int)sizeof(GroupedBars) + (a.experts + 1) * (int)sizeof(GroupedTable);
-  auto kernel = grouped_kernel<T, TO, MODE, NT>;
+  auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR>;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return (int)e;
-  return launch_pdl(kernel, device_sm_count(), kGroupedThreads, smem, st, ma, mb, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(device_sm_count() / PAIR * PAIR)); cfg.blockDim = dim3(kGroupedThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = PAIR; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, kernel, ma, mb, row_a, row_b, a);
 }
 
 template <class T, class TO, int MODE>
 static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
   if constexpr (MODE == FLEXSPMV_GROUPED_DW) {
-    return grouped_launch_as<T, TO, MODE, 256>(a, st);
+    return grouped_launch_as<T, TO, MODE, 256, 2>(a, st);
   } else {
-    if (a.slots <= 16ll * a.experts) return grouped_launch_as<T, TO, MODE, 32>(a, st);
-    return grouped_launch_as<T, TO, MODE, 256>(a, st);
+    if (a.slots <= 16ll * a.experts) return grouped_launch_as<T, TO, MODE, 32, 1>(a, st);
+    return grouped_launch_as<T, TO, MODE, 256, 2>(a, st);
   }
+}
+
+// Where there is a list of rows, x's rows in its order in the workspace; `x` and `stride` become the copy's.
+static int take_rows(const flexspmv_expert_desc& d, const void*& x, int64_t& stride, const void* rows, const void* offsets, void* ws, size_t ws_bytes, int* status,
+                     cudaStream_t st) {
+  if (!rows || d.slots == 0) return 0;
+  if (!ws || ws_bytes < (size_t)d.slots * d.k * 2) return FLEXSPMV_ERR_WORKSPACE;
+  if (!aligned16(ws)) return FLEXSPMV_ERR_ALIGN;
+  const int pieces = d.k / 8;
+  const long long ctas = ((long long)d.slots * pieces + 1023) / 1024, most = device_sm_count() * 8ll;
+  if (int e = launch_pdl(take_rows_kernel, (unsigned)(ctas < most ? ctas : most), 256, 0, st, static_cast<const uint4*>(x), static_cast<const int*>(rows),
+                         static_cast<const int*>(offsets), static_cast<uint4*>(ws), (long long)d.tokens, (long long)d.slots, (long long)stride / 8, d.experts,
+                         pieces, status))
+    return e;
+  x = ws;
+  stride = d.k;
+  return 0;
 }
 
 static int check_grouped(const flexspmv_expert_desc* d, int which) {
@@ -426,7 +450,7 @@ extern "C" {
 int flexspmv_grouped_matmul_bytes(const flexspmv_expert_desc* d, int32_t which, size_t* bytes) {
   if (!bytes || which < FLEXSPMV_GROUPED_FORWARD || which > FLEXSPMV_GROUPED_DW) return FLEXSPMV_ERR_BAD_ARG;
   if (int e = flex::check_grouped(d, which)) return e;
-  *bytes = 0;
+  *bytes = which == FLEXSPMV_GROUPED_DX ? 0 : (size_t)d->slots * d->k * 2;         // a copy of x's rows; not needed without a list of rows
   return 0;
 }
 
@@ -437,9 +461,11 @@ int flexspmv_grouped_matmul(const flexspmv_expert_desc* d, const void* const* in
   if (d->slots == 0) return 0;
   if (!in[0] || !in[1] || !in[2] || !out[0] || d->tokens < (in[3] ? 1 : d->slots)) return FLEXSPMV_ERR_BAD_ARG;
   if (!flex::aligned16(in[0]) || !flex::aligned16(in[1]) || !flex::aligned16(out[0])) return FLEXSPMV_ERR_ALIGN;
-  flex::GroupedArgs a = {in[0], in[1], static_cast<const int*>(in[2]), static_cast<const int*>(in[3]), out[0], d->tokens, d->slots, d->in_stride, 0,
-                         d->experts, d->n, d->k, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const void* x = in[0];
+  int64_t stride = d->in_stride;
+  if (int e = flex::take_rows(*d, x, stride, in[3], in[2], ws, ws_bytes, status, st)) return e;
+  flex::GroupedArgs a = {x, in[1], static_cast<const int*>(in[2]), out[0], d->slots, stride, 0, d->experts, d->n, d->k, status};
   if (d->type == FLEXSPMV_TYPE_BF16) return flex::grouped_launch<__nv_bfloat16, __nv_bfloat16, FLEXSPMV_GROUPED_FORWARD>(a, st);
   return flex::grouped_launch<__half, __half, FLEXSPMV_GROUPED_FORWARD>(a, st);
 }
@@ -451,7 +477,7 @@ int flexspmv_grouped_matmul_dx(const flexspmv_expert_desc* d, const void* const*
   if (d->slots == 0) return 0;
   if (!in[0] || !in[1] || !in[2] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
   if (!flex::aligned16(in[0]) || !flex::aligned16(in[1]) || !flex::aligned16(out[0])) return FLEXSPMV_ERR_ALIGN;
-  flex::GroupedArgs a = {in[0], in[1], static_cast<const int*>(in[2]), nullptr, out[0], d->slots, d->slots, d->in_stride, 0, d->experts, d->n, d->k, status};
+  flex::GroupedArgs a = {in[0], in[1], static_cast<const int*>(in[2]), out[0], d->slots, d->in_stride, 0, d->experts, d->n, d->k, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (d->type == FLEXSPMV_TYPE_BF16) return flex::grouped_launch<__nv_bfloat16, __nv_bfloat16, FLEXSPMV_GROUPED_DX>(a, st);
   return flex::grouped_launch<__half, __half, FLEXSPMV_GROUPED_DX>(a, st);
@@ -463,9 +489,11 @@ int flexspmv_grouped_matmul_dw(const flexspmv_expert_desc* d, const void* const*
   if (!in || !out || !in[2] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
   if (d->slots && (!in[0] || !in[1] || d->tokens < (in[3] ? 1 : d->slots))) return FLEXSPMV_ERR_BAD_ARG;
   if (!flex::aligned16(in[0]) || !flex::aligned16(in[1]) || !flex::aligned16(out[0])) return FLEXSPMV_ERR_ALIGN;
-  flex::GroupedArgs a = {in[0], in[1], static_cast<const int*>(in[2]), static_cast<const int*>(in[3]), out[0], d->tokens, d->slots, d->in_stride,
-                         d->in2_stride, d->experts, d->n, d->k, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const void* x = in[1];
+  int64_t stride = d->in2_stride;
+  if (int e = flex::take_rows(*d, x, stride, in[3], in[2], ws, ws_bytes, status, st)) return e;
+  flex::GroupedArgs a = {in[0], x, static_cast<const int*>(in[2]), out[0], d->slots, d->in_stride, stride, d->experts, d->n, d->k, status};
   const bool wide = d->out_type == FLEXSPMV_TYPE_F32;
   if (d->type == FLEXSPMV_TYPE_BF16)
     return wide ? flex::grouped_launch<__nv_bfloat16, float, FLEXSPMV_GROUPED_DW>(a, st)

@@ -242,6 +242,7 @@ def _grouped(which: int, name: str, d: Desc, ins, out, offsets, dev: int) -> Bou
     lib = load_library()
     need = ctypes.c_size_t()
     _check_status(lib, lib.flexspmv_grouped_matmul_bytes(ctypes.byref(d), which, ctypes.byref(need)), name)
+    need = need if which != _DX and ins[3] is not None else ctypes.c_size_t()          # a copy of x's rows
     ws = torch.empty(need.value, dtype=torch.uint8, device=out.device) if need.value else None
     flag = _flag(dev)
     pin, pout = (ctypes.c_void_p * len(ins))(*[t.data_ptr() if t is not None else 0 for t in ins]), _pointers((out,))
