@@ -16,16 +16,18 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// W values: 16 bytes where they are that many, else a value on its own.
+// W values: in pieces of 16 bytes or one of 8, where they are that many, else a value on its own.
 template <class T, int W>
 struct Pack {
-  union { uint4 raw[(sizeof(T) * W + 15) / 16]; T v[W]; };
+  union { uint4 raw[(sizeof(T) * W + 15) / 16]; uint2 half; T v[W]; };
   __device__ __forceinline__ Pack() {}
-  static constexpr bool kWide = sizeof(T) * W % 16 == 0;
+  static constexpr bool kWide = sizeof(T) * W % 16 == 0, kHalf = sizeof(T) * W == 8;
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (kWide) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T) * W / 16; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else if constexpr (kHalf) {
+      half = *reinterpret_cast<const uint2*>(p);
     } else {
 #pragma unroll
       for (int i = 0; i < W; ++i) v[i] = p[i];
@@ -35,6 +37,8 @@ struct Pack {
     if constexpr (kWide) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T) * W / 16; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
+    } else if constexpr (kHalf) {
+      *reinterpret_cast<uint2*>(p) = half;
     } else {
 #pragma unroll
       for (int i = 0; i < W; ++i) p[i] = v[i];

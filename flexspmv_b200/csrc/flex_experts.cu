@@ -16,48 +16,106 @@ int device_sm_count();
 
 // ---- router --------------------------------------------------------------------------------------------------------
 
-// A float as an unsigned number of the same order; NaN and -infinity are 0, which is never chosen.
-__device__ __forceinline__ unsigned choice_key(float v) {
-  const unsigned u = __float_as_uint(v + 0.f);         // -0 and 0 are equal
-  const unsigned key = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return (v != v || v == -INFINITY) ? 0u : key;
+// What a choice goes by: a number that is larger for a larger logit and, among equal ones, for a lower expert.  0: NaN and -infinity, never
+// chosen.  A 16-bit logit and the expert fit 32 bits, so that one instruction finds the largest of a warp; a 32-bit one takes 64.
+template <class T>
+struct Choice {
+  using Key = uint32_t;
+  static __device__ __forceinline__ Key make(float v, int e) {
+    const uint32_t u = bits(v + 0.f);                         // -0 and 0 are equal
+    const uint32_t order = (u & 0x8000u) ? ~u & 0xffffu : u | 0x8000u;
+    return (v != v || v == -INFINITY) ? 0u : order << 16 | (0xffffu - (uint32_t)e);
+  }
+  static __device__ __forceinline__ uint32_t bits(float v) {
+    if constexpr (std::is_same<T, __half>::value) return __half_as_ushort(__float2half_rn(v));
+    else return __float_as_uint(v) >> 16;
+  }
+  static __device__ __forceinline__ int expert(Key k) { return (int)(0xffffu - (k & 0xffffu)); }
+  static __device__ __forceinline__ float logit(Key k) {
+    const uint32_t order = k >> 16, u = (order & 0x8000u) ? order & 0x7fffu : ~order & 0xffffu;
+    if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)u));
+    else return __uint_as_float(u << 16);
+  }
+  static __device__ __forceinline__ Key warp_max(Key k) { return __reduce_max_sync(0xffffffffu, k); }
+};
+template <>
+struct Choice<float> {
+  using Key = unsigned long long;
+  static __device__ __forceinline__ Key make(float v, int e) {
+    const uint32_t u = __float_as_uint(v + 0.f), order = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+    return (v != v || v == -INFINITY) ? 0ull : (Key)order << 32 | (0xffffu - (uint32_t)e);
+  }
+  static __device__ __forceinline__ int expert(Key k) { return (int)(0xffffu - (uint32_t)k); }
+  static __device__ __forceinline__ float logit(Key k) {
+    const uint32_t order = (uint32_t)(k >> 32);
+    return __uint_as_float((order & 0x80000000u) ? order & 0x7fffffffu : ~order);
+  }
+  static __device__ __forceinline__ Key warp_max(Key k) {
+    const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
+    return (Key)high << 32 | __reduce_max_sync(0xffffffffu, high == (uint32_t)(k >> 32) ? (uint32_t)k : 0u);
+  }
+};
+
+// Largest first, by odd-even merging (Batcher): V log^2 V exchanges whose places are known when it is compiled.
+template <class K, int V>
+__device__ __forceinline__ void sort_down(K (&k)[V]) {
+#pragma unroll
+  for (int p = 1; p < V; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j + q < V; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < V && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const K x = k[i + j], y = k[i + j + q];
+            k[i + j] = x > y ? x : y;
+            k[i + j + q] = x > y ? y : x;
+          }
 }
 
-// One token by one warp; lane l holds the experts l, l + 32, ...: V of them.  The k largest by k rounds of a maximum over the warp (equal
-// logits: the lowest expert, as the plain form's stable sort has it), each after the chosen one's key has been taken out.
-// Lane j ends with choice j.  The softmax is over the true logits, largest subtracted, sums in 32 bits.
-template <class T, int V>
-__device__ __forceinline__ void choose_token(const T* row, int experts, int k, bool renormalize, int lane, int& my_id, float& my_weight) {
-  float v[V];
-  unsigned key[V];
-  unsigned best = 0;
-  int best_at = 0;
+// A row's part of lane l: V experts, W neighbouring ones at a time.
+template <class T, int V, int W>
+struct LanePart {
+  Pack<T, W> piece[V / W];
+  __device__ __forceinline__ void load(const T* row, int experts, int lane) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int e = i * 32 + lane;
-    v[i] = e < experts ? to_float(row[e]) : -INFINITY;
-    key[i] = choice_key(v[i]);
-    if (key[i] > best) { best = key[i]; best_at = i; }
-  }
-  my_id = -1;
-  float my_logit = -INFINITY, top = -INFINITY;
-  for (int j = 0; j < k; ++j) {
-    const unsigned most = __reduce_max_sync(0xffffffffu, best);
-    if (most == 0) break;
-    const int at = __reduce_min_sync(0xffffffffu, best == most ? best_at * 32 + lane : 0x7fffffff);
-    const float logit = __uint_as_float((most & 0x80000000u) ? (most & 0x7fffffffu) : ~most);
-    if (j == 0) top = logit;
-    if (lane == j) { my_id = at; my_logit = logit; }
-    if ((at & 31) == lane) {
-      best = 0;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (i == (at >> 5)) key[i] = 0;
-        if (key[i] > best) { best = key[i]; best_at = i; }
-      }
+    for (int i = 0; i < V / W; ++i) {
+      const int e = (i * 32 + lane) * W;
+      if (e < experts) piece[i].load(row + e);
     }
   }
-  const float mine = my_id >= 0 ? expf(my_logit - top) : 0.f;
+};
+
+// One token by one warp.  Each lane's experts are sorted once; then k rounds of a maximum over the lanes' first ones, the winner's lane
+// moving up its next (equal logits: the lowest expert, as the plain form's stable sort has it).  Lane j ends with choice j.  The softmax is
+// over the true logits, largest subtracted, sums in 32 bits.
+template <class T, int V, int W>
+__device__ __forceinline__ void choose_token(const LanePart<T, V, W>& part, int experts, int k, bool renormalize, int lane, int& my_id, float& my_weight) {
+  using C = Choice<T>;
+  float v[V];
+  typename C::Key key[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = (i / W * 32 + lane) * W;
+    v[i] = e < experts ? part.piece[i / W].get(i % W) : -INFINITY;
+    key[i] = C::make(v[i], e + i % W);
+  }
+  sort_down(key);
+  typename C::Key mine_key = 0, top_key = 0;
+  for (int j = 0; j < k; ++j) {
+    const typename C::Key most = C::warp_max(key[0]);
+    if (most == 0) break;
+    if (j == 0) top_key = most;
+    if (lane == j) mine_key = most;
+    const bool won = key[0] == most;
+#pragma unroll
+    for (int i = 0; i + 1 < V; ++i) key[i] = won ? key[i + 1] : key[i];
+    key[V - 1] = won ? 0 : key[V - 1];
+  }
+  my_id = mine_key ? C::expert(mine_key) : -1;
+  const float top = top_key ? C::logit(top_key) : 0.f;
+  const float mine = mine_key ? expf(C::logit(mine_key) - top) : 0.f;
   float sum = 0.f;
   if (renormalize) {
     sum = mine;
@@ -67,10 +125,8 @@ __device__ __forceinline__ void choose_token(const T* row, int experts, int k, b
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  my_weight = my_id >= 0 ? mine / sum : 0.f;
+  my_weight = mine_key ? mine / sum : 0.f;
 }
-
-constexpr int kRouteThreads = 256, kRouteWarps = kRouteThreads / 32;
 
 struct RouteArgs {
   const void* logits;
@@ -82,75 +138,66 @@ struct RouteArgs {
   unsigned* counts;                // [CTAs][experts]
 };
 
-// Choices of this CTA's tokens; `hist` (shared, zeroed, experts entries) gets their number for each expert.
-template <class T, int V>
-__device__ __forceinline__ void choose_chunk(const RouteArgs& a, unsigned* hist) {
+// Choices of this CTA's tokens, a run of them for each warp.  `seen` (shared, [warps][experts]) counts each warp's pairs of an expert, in
+// their order and without atomics: a token's experts are different ones.  In the end slots[pair] is the pair's number among the CTA's pairs of its
+// expert, and total[e] (shared) how many there are.
+template <class T, int V, int W, int THREADS>
+__device__ __forceinline__ void choose_chunk(const RouteArgs& a, unsigned* seen, unsigned* total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long from = a.chunk * blockIdx.x, to = from + a.chunk < a.tokens ? from + a.chunk : a.tokens;
-  for (long long t = from + warp; t < to; t += kRouteWarps) {
+  for (int i = threadIdx.x; i < a.experts * (THREADS / 32); i += THREADS) seen[i] = 0;
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+  const long long first = a.chunk * blockIdx.x, last = first + a.chunk < a.tokens ? first + a.chunk : a.tokens;
+  const long long each = (a.chunk + THREADS / 32 - 1) / (THREADS / 32);
+  const long long from = first + warp * each, to = from + each < last ? from + each : last;
+  const T* const logits = static_cast<const T*>(a.logits);
+  unsigned* const mine = seen + warp * a.experts;
+  LanePart<T, V, W> next;
+  if (from < to) next.load(logits + from * a.stride, a.experts, lane);
+  for (long long t = from; t < to; ++t) {
+    const LanePart<T, V, W> part = next;
+    if (t + 1 < to) next.load(logits + (t + 1) * a.stride, a.experts, lane);
     int id;
     float weight;
-    choose_token<T, V>(static_cast<const T*>(a.logits) + t * a.stride, a.experts, a.k, a.renormalize != 0, lane, id, weight);
+    choose_token<T, V, W>(part, a.experts, a.k, a.renormalize != 0, lane, id, weight);
     if (lane < a.k) {
       a.weights[t * a.k + lane] = weight;
       a.ids[t * a.k + lane] = id;
-      if (id >= 0) atomicAdd(&hist[id], 1u);
+      int number = -1;
+      if (id >= 0) number = (int)mine[id]++;
+      a.slots[t * a.k + lane] = number;
     }
-  }
-}
-
-// Places this CTA's pairs: `start` (shared, [warps][experts]) holds for each warp and expert the place of the warp's first pair of it.  A warp
-// takes 32 pairs at a time in their order, so that the order by expert is stable and no atomic decides it.
-__device__ __forceinline__ void warp_pairs(const RouteArgs& a, long long& from, long long& to) {
-  const long long first = a.chunk * blockIdx.x, last = first + a.chunk < a.tokens ? first + a.chunk : a.tokens;
-  const long long pairs = last > first ? (last - first) * a.k : 0;
-  const long long each = (pairs + kRouteWarps * 32 - 1) / (kRouteWarps * 32) * 32;
-  from = first * a.k + min(each * (threadIdx.x >> 5), pairs);
-  to = first * a.k + min(each * (threadIdx.x >> 5) + each, pairs);
-}
-
-__device__ __forceinline__ void place_chunk(const RouteArgs& a, unsigned* start) {
-  const int lane = threadIdx.x & 31;
-  unsigned* mine = start + (threadIdx.x >> 5) * a.experts;
-  long long from, to;
-  warp_pairs(a, from, to);
-  for (long long p = from; p < to; p += 32) {
-    const long long pair = p + lane;
-    const int id = pair < to ? a.ids[pair] : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, id);
-    unsigned place = 0;
-    if (id >= 0) place = mine[id] + __popc(same & ((1u << lane) - 1u));
     __syncwarp();
-    if (id >= 0 && (same >> lane) == 1u) mine[id] = place + 1u;          // the last of its kind
-    __syncwarp();
-    if (pair < to) {
-      a.slots[pair] = id >= 0 ? (int)place : -1;
-      if (id >= 0) a.rows[place] = (int)(pair / a.k);
-    }
   }
-}
-
-// In: `total` and `before` (shared, experts entries): an expert's pairs altogether, and those of the CTAs before this one.  Out: `start` as
-// place_chunk wants it.  Needs the CTA's ids visible to it.
-__device__ __forceinline__ unsigned plan_chunk(const RouteArgs& a, unsigned* total, const unsigned* before, unsigned* start) {
-  __shared__ unsigned warp_sum[kRouteWarps + 1];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  for (int i = tid; i < a.experts * kRouteWarps; i += kRouteThreads) start[i] = 0;
   __syncthreads();
-  {
-    long long from, to;
-    warp_pairs(a, from, to);
-    unsigned* mine = start + warp * a.experts;
-    for (long long p = from + lane; p < to; p += 32) {
-      const int id = a.ids[p];
-      if (id >= 0) atomicAdd(&mine[id], 1u);
+  for (int e = threadIdx.x; e < a.experts; e += THREADS) {
+    unsigned sum = 0;
+#pragma unroll 8
+    for (int w = 0; w < THREADS / 32; ++w) {
+      const unsigned n = seen[w * a.experts + e];
+      seen[w * a.experts + e] = sum;
+      sum += n;
     }
+    total[e] = sum;
   }
-  // exclusive sums of the totals, kRouteThreads at a time
+  __syncthreads();
+  for (long long p = from * a.k + lane; p < to * a.k; p += 32) {
+    const int id = a.ids[p];
+    if (id >= 0) a.slots[p] += (int)mine[id];
+  }
+}
+
+// total[e] becomes the sum of those before it; returns the sum of all.  With `offsets`, they are also written there.
+template <int THREADS>
+__device__ __forceinline__ unsigned sums_before(unsigned* total, int experts, int* offsets) {
+  constexpr int kWarps = THREADS / 32;
+  __shared__ unsigned warp_sum[32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   unsigned done = 0;
-  for (int base = 0; base < a.experts; base += kRouteThreads) {
+  for (int base = 0; base < experts; base += THREADS) {
     const int e = base + tid;
-    const unsigned n = e < a.experts ? total[e] : 0u;
+    const unsigned n = e < experts ? total[e] : 0u;
     unsigned s = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -160,89 +207,98 @@ __device__ __forceinline__ unsigned plan_chunk(const RouteArgs& a, unsigned* tot
     __syncthreads();
     if (lane == 31) warp_sum[warp] = s;
     __syncthreads();
-    unsigned all = 0, prior = 0;
-#pragma unroll
-    for (int w = 0; w < kRouteWarps; ++w) {
-      if (w < warp) prior += warp_sum[w];
-      all += warp_sum[w];
-    }
-    if (e < a.experts) {
-      const unsigned off = done + prior + s - n;
-      if (blockIdx.x == 0) a.offsets[e] = (int)off;
-      unsigned at = off + before[e];
-      for (int w = 0; w < kRouteWarps; ++w) {
-        const unsigned c = start[w * a.experts + e];
-        start[w * a.experts + e] = at;
-        at += c;
-      }
+    const unsigned mine = lane < kWarps ? warp_sum[lane] : 0u;
+    const unsigned prior = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0u), all = __reduce_add_sync(0xffffffffu, mine);
+    if (e < experts) {
+      total[e] = done + prior + s - n;
+      if (offsets) offsets[e] = (int)(done + prior + s - n);
     }
     done += all;
   }
-  if (blockIdx.x == 0 && tid == 0) a.offsets[a.experts] = (int)done;
+  if (offsets && tid == 0) offsets[experts] = (int)done;
   __syncthreads();
   return done;
 }
 
 // Small batches: everything in one CTA and one launch.
-template <class T, int V>
-__global__ void __launch_bounds__(kRouteThreads) route_small_kernel(RouteArgs a) {
+template <class T, int V, int W, int THREADS>
+__global__ void __launch_bounds__(THREADS) route_small_kernel(RouteArgs a) {
   extern __shared__ unsigned route_sm[];
-  unsigned *total = route_sm, *before = total + a.experts, *start = before + a.experts;
-  for (int i = threadIdx.x; i < a.experts; i += kRouteThreads) total[i] = before[i] = 0;
-  __syncthreads();
-  pdl_wait();
-  choose_chunk<T, V>(a, total);
-  __syncthreads();
-  const unsigned used = plan_chunk(a, total, before, start);
-  place_chunk(a, start);
-  for (long long i = used + threadIdx.x; i < a.tokens * a.k; i += kRouteThreads) a.rows[i] = -1;
+  unsigned* const total = route_sm;
+  choose_chunk<T, V, W, THREADS>(a, total + a.experts, total);
+  const unsigned used = sums_before<THREADS>(total, a.experts, a.offsets);
+  const int pairs = (int)a.tokens * a.k;
+  for (int p = threadIdx.x; p < pairs; p += THREADS) {
+    const int id = a.ids[p];
+    if (id >= 0) {
+      const int place = a.slots[p] + (int)total[id];
+      a.slots[p] = place;
+      a.rows[place] = p / a.k;
+    }
+    if (p >= (int)used) a.rows[p] = -1;
+  }
 }
 
-template <class T, int V>
-__global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(RouteArgs a) {
+template <class T, int V, int W, int THREADS>
+__global__ void __launch_bounds__(THREADS) route_choose_kernel(RouteArgs a) {
   extern __shared__ unsigned route_sm[];
-  for (int i = threadIdx.x; i < a.experts; i += kRouteThreads) route_sm[i] = 0;
-  __syncthreads();
-  pdl_wait();
-  pdl_launch_dependents();
-  choose_chunk<T, V>(a, route_sm);
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.experts; i += kRouteThreads) a.counts[(size_t)blockIdx.x * a.experts + i] = route_sm[i];
+  unsigned* const total = route_sm;
+  choose_chunk<T, V, W, THREADS>(a, total + a.experts, total);
+  for (int i = threadIdx.x; i < a.experts; i += THREADS) a.counts[(size_t)blockIdx.x * a.experts + i] = total[i];
 }
 
 // Every CTA adds up the counts of all CTAs by itself (they lie in L2): a launch fewer than a scan between the two would take.
-__global__ void __launch_bounds__(kRouteThreads) route_place_kernel(RouteArgs a) {
+constexpr int kPlaceThreads = 512;
+__global__ void __launch_bounds__(kPlaceThreads) route_place_kernel(RouteArgs a) {
   extern __shared__ unsigned route_sm[];
-  unsigned *total = route_sm, *before = total + a.experts, *start = before + a.experts;
+  unsigned *total = route_sm, *before = total + a.experts;
+  for (int i = threadIdx.x; i < a.experts; i += kPlaceThreads) total[i] = before[i] = 0;
+  __syncthreads();
   pdl_wait();
-  for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) {
+  // as many threads on an expert as there are; each adds every parts-th CTA's count
+  const int parts = kPlaceThreads / a.experts > 0 ? kPlaceThreads / a.experts : 1;
+  for (int i = threadIdx.x; i < a.experts * parts; i += kPlaceThreads) {
+    const int e = i % a.experts, part = i / a.experts;
     unsigned all = 0, prior = 0;
-#pragma unroll 8
-    for (unsigned b = 0; b < gridDim.x; ++b) {
+#pragma unroll 16
+    for (unsigned b = part; b < gridDim.x; b += parts) {
       const unsigned n = a.counts[(size_t)b * a.experts + e];
       all += n;
       prior += b < blockIdx.x ? n : 0u;
     }
-    total[e] = all;
-    before[e] = prior;
+    if (parts == 1) {
+      total[e] = all;
+      before[e] = prior;
+    } else {
+      atomicAdd(&total[e], all);
+      atomicAdd(&before[e], prior);
+    }
   }
   __syncthreads();
-  const unsigned used = plan_chunk(a, total, before, start);
-  place_chunk(a, start);
-  for (long long i = used + (long long)blockIdx.x * kRouteThreads + threadIdx.x; i < a.tokens * a.k; i += (long long)gridDim.x * kRouteThreads)
-    a.rows[i] = -1;
+  const unsigned used = sums_before<kPlaceThreads>(total, a.experts, blockIdx.x == 0 ? a.offsets : nullptr);
+  for (int e = threadIdx.x; e < a.experts; e += kPlaceThreads) before[e] += total[e];
+  __syncthreads();
+  const long long from = a.chunk * blockIdx.x * a.k, end = from + a.chunk * a.k, pairs = a.tokens * a.k, to = end < pairs ? end : pairs;
+#pragma unroll 4
+  for (long long p = from + threadIdx.x; p < to; p += kPlaceThreads) {
+    const int id = a.ids[p];
+    if (id >= 0) {
+      const int place = a.slots[p] + (int)before[id];
+      a.slots[p] = place;
+      a.rows[place] = (int)((unsigned)p / (unsigned)a.k);
+    }
+    if (p >= (long long)used) a.rows[p] = -1;
+  }
 }
 
 // Gradient of the chosen weights with respect to the logits.  p_i = w_0 exp(l_i - l_{e_0}): the largest weight and its logit stand for the
-// softmax's maximum and sum, so that one pass over the row is enough.  A warp takes a token.
-template <class T>
+// softmax's maximum and sum, so that one pass over the row is enough.  A warp takes a token: first the row as if nothing were chosen,
+// -p_i sum_j g_j w_j (renormalized: zeros), then the chosen ones' w_j (g_j - sum g w) over it.
+template <class T, int W>
 __global__ void __launch_bounds__(256) route_backward_kernel(const float* __restrict__ dweights, const T* __restrict__ logits, const float* __restrict__ weights,
                                                              const int* __restrict__ ids, T* __restrict__ dlogits, long long tokens, long long stride,
                                                              int experts, int k, int renormalize) {
-  extern __shared__ float route_grad_sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* grad = route_grad_sm + warp * experts;
-  for (int e = lane; e < experts; e += 32) grad[e] = 0.f;
   pdl_wait();
   for (long long t = (long long)blockIdx.x * 8 + warp; t < tokens; t += (long long)gridDim.x * 8) {
     const int id = lane < k ? ids[t * k + lane] : -1;
@@ -252,22 +308,24 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const float* __rest
     for (int o = 16; o; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
     const int top_id = __shfl_sync(0xffffffffu, id, 0);
     const float top_w = __shfl_sync(0xffffffffu, w, 0);
-    __syncwarp();
-    if (id >= 0) grad[id] = renormalize ? w * (g - mean) : g;
-    __syncwarp();
     T* out = dlogits + t * experts;
     if (renormalize || top_id < 0) {
-      for (int e = lane; e < experts; e += 32) out[e] = from_float<T>(grad[e]);
+      Pack<T, W> none;
+      none.zero();
+      for (int e = lane * W; e < experts; e += 32 * W) none.store(out + e);
     } else {
       const T* row = logits + t * stride;
-      const float top = to_float(row[top_id]);
-      for (int e = lane; e < experts; e += 32) {
-        const float v = to_float(row[e]);
-        out[e] = from_float<T>(v == -INFINITY ? 0.f : top_w * expf(v - top) * (grad[e] - mean));
+      const float top = to_float(row[top_id]), scale = -top_w * mean;
+      for (int e = lane * W; e < experts; e += 32 * W) {
+        Pack<T, W> v, r;
+        v.load(row + e);
+#pragma unroll
+        for (int x = 0; x < W; ++x) r.set(x, v.get(x) == -INFINITY ? 0.f : scale * expf(v.get(x) - top));
+        r.store(out + e);
       }
     }
     __syncwarp();
-    if (id >= 0) grad[id] = 0.f;
+    if (id >= 0) out[id] = from_float<T>(w * (g - mean));
   }
 }
 
@@ -380,28 +438,38 @@ static int route_ctas(long long tokens) {
 }
 constexpr long long kRouteSmall = 64;      // tokens up to which one CTA does it all
 
-template <class T, int V>
+// THREADS: as many as leave `seen` (a word for each warp and expert) within 48 KB of shared memory.
+template <class T, int V, int W, int THREADS>
 static int route_launch(const RouteArgs& args, cudaStream_t st) {
   RouteArgs a = args;
-  const size_t lists = (size_t)a.experts * 4 * (2 + kRouteWarps);
+  const auto smem = [&](int threads) { return (size_t)a.experts * 4 * (1 + threads / 32); };
   if (a.tokens <= kRouteSmall) {
     a.chunk = a.tokens;
-    return launch_pdl(route_small_kernel<T, V>, 1, kRouteThreads, lists, st, a);
+    if (a.tokens <= 8) return launch_pdl(route_small_kernel<T, V, W, 256>, 1, 256, smem(256), st, a);
+    return launch_pdl(route_small_kernel<T, V, W, THREADS>, 1, THREADS, smem(THREADS), st, a);
   }
   const int ctas = route_ctas(a.tokens);
   a.chunk = (a.tokens + ctas - 1) / ctas;
-  if (int e = launch_pdl(route_choose_kernel<T, V>, ctas, kRouteThreads, (size_t)a.experts * 4, st, a)) return e;
-  return launch_pdl(route_place_kernel, ctas, kRouteThreads, lists, st, a);
+  if (int e = launch_pdl(route_choose_kernel<T, V, W, THREADS>, ctas, THREADS, smem(THREADS), st, a)) return e;
+  return launch_pdl(route_place_kernel, ctas, kPlaceThreads, (size_t)a.experts * 8, st, a);
+}
+
+template <class T, int V, int THREADS>
+static int route_width(const RouteArgs& a, cudaStream_t st) {
+  constexpr int kFull = 16 / (int)sizeof(T), W = V < kFull ? 1 : kFull;
+  // 16-byte loads where every row allows them
+  const bool wide = a.experts % W == 0 && a.stride % W == 0 && aligned16(a.logits);
+  return wide ? route_launch<T, V, W, THREADS>(a, st) : route_launch<T, V, 1, THREADS>(a, st);
 }
 
 template <class T>
 static int route_typed(const RouteArgs& a, cudaStream_t st) {
-  if (a.experts <= 32) return route_launch<T, 1>(a, st);
-  if (a.experts <= 64) return route_launch<T, 2>(a, st);
-  if (a.experts <= 128) return route_launch<T, 4>(a, st);
-  if (a.experts <= 256) return route_launch<T, 8>(a, st);
-  if (a.experts <= 512) return route_launch<T, 16>(a, st);
-  return route_launch<T, 32>(a, st);
+  if (a.experts <= 32) return route_width<T, 1, 1024>(a, st);
+  if (a.experts <= 64) return route_width<T, 2, 1024>(a, st);
+  if (a.experts <= 128) return route_width<T, 4, 1024>(a, st);
+  if (a.experts <= 256) return route_width<T, 8, 1024>(a, st);
+  if (a.experts <= 512) return route_width<T, 16, 512>(a, st);
+  return route_width<T, 32, 256>(a, st);
 }
 
 static int grid_of(long long ctas, int most) { return (int)(ctas < 1 ? 1 : ctas > most ? most : ctas); }
@@ -465,10 +533,11 @@ int flexspmv_expert_route_backward(const flexspmv_expert_desc* d, const void* co
   if (!in[0] || !in[1] || !in[2] || !in[3] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int grid = flex::grid_of((d->tokens + 7) / 8, flex::device_sm_count() * 8);
-  const size_t smem = (size_t)8 * d->experts * 4;
   auto go = [&](auto zero) {
     using T = decltype(zero);
-    return flex::launch_pdl(flex::route_backward_kernel<T>, grid, 256, smem, st, static_cast<const float*>(in[0]), static_cast<const T*>(in[1]),
+    constexpr int W = 16 / (int)sizeof(T);
+    const bool wide = d->experts % W == 0 && d->in_stride % W == 0 && flex::aligned16(in[1]) && flex::aligned16(out[0]);
+    return flex::launch_pdl(wide ? flex::route_backward_kernel<T, W> : flex::route_backward_kernel<T, 1>, grid, 256, 0, st, static_cast<const float*>(in[0]), static_cast<const T*>(in[1]),
                             static_cast<const float*>(in[2]), static_cast<const int*>(in[3]), static_cast<T*>(out[0]), (long long)d->tokens,
                             (long long)d->in_stride, d->experts, d->choices, d->flags & FLEXSPMV_EXPERT_RENORMALIZE);
   };

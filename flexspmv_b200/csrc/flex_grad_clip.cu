@@ -2,9 +2,9 @@
 //
 //   norm = sqrt(sum of all squares);  out = grad * min(1, max_norm / (norm + 1e-6))
 //
-// Two launches for up to kMost tensors, which travel in the kernels' parameters: no table is copied to the device.  Bound by memory:
-// the gradients are read twice (the scale needs the whole sum) and the result written once.  The tensors are cut into pieces that go round the
-// CTAs in order; the second launch takes them in the opposite order, so that what the first read last is still in L2.
+// A plan cuts the tensors into pieces and writes a record of each into the workspace, once for tensors that stay where they are.  The pieces
+// go round the CTAs in order; the second of the two launches takes them in the opposite order, so that what the first read last is still in
+// L2.  Bound by memory: the gradients are read twice (the scale needs the whole sum) and the result written once.
 // A thread adds the squares of a piece in 32 bits and the pieces in 64, the CTAs' sums are added in one fixed order: no atomics, the same
 // bits every time.
 #include <cuda_runtime.h>
@@ -16,27 +16,41 @@ namespace flex {
 
 int device_sm_count();
 
-constexpr int kClipThreads = 256, kClipCtasPerSm = 4;
+constexpr int kClipThreads = 256, kClipCtasPerSm = 6;
 constexpr float kClipEps = 1e-6f;
-constexpr int kMost = 1000;                 // 28 KB of parameters; a launch may have 32 764 bytes
 
-struct ClipTensor {
+struct ClipPiece {
   const void* in;
   void* out;
-  long long length;
+  int length, types;             // types: the input's in bits 0-1, the output's in bits 2-3
 };
-template <int N>
-struct ClipArgs {
-  ClipTensor tensor[N];
-  int first[N + 1];              // first piece of each tensor: pieces of tensor i are first[i] .. first[i + 1]
-  unsigned char types[N];        // in: bits 0-1, out: bits 2-3
-  int count, piece;              // tensors, elements of a piece
-  double* partial;               // a sum for each CTA of every first launch
-  int partial_at, partials;      // this launch's place among them, and how many there are
-  float max_norm;
-  float* norm;
-  int write;
+
+// The tensors of one planning launch travel in its parameters.
+constexpr int kPlanTensors = 128;
+struct ClipTensors {
+  const void* in[kPlanTensors];
+  void* out[kPlanTensors];
+  long long length[kPlanTensors];
+  long long first[kPlanTensors];         // number of the tensor's first piece
+  unsigned char types[kPlanTensors];
+  ClipPiece* piece;
+  int size;                      // elements of a piece
 };
+__global__ void __launch_bounds__(256) clip_plan_kernel(const __grid_constant__ ClipTensors t) {
+  const int i = blockIdx.x;
+  const long long length = t.length[i], pieces = (length + t.size - 1) / t.size;
+  const int types = t.types[i], in_bytes = (types & 3) == FLEXSPMV_TYPE_F32 ? 4 : 2, out_bytes = types >> 2 == FLEXSPMV_TYPE_F32 ? 4 : 2;
+  pdl_wait();
+  for (long long p = threadIdx.x; p < pieces; p += 256) {
+    const long long at = p * t.size, left = length - at;
+    ClipPiece r;
+    r.in = static_cast<const char*>(t.in[i]) + at * in_bytes;
+    r.out = t.out[i] ? static_cast<char*>(t.out[i]) + at * out_bytes : nullptr;
+    r.length = (int)(left < t.size ? left : t.size);
+    r.types = types;
+    t.piece[t.first[i] + p] = r;
+  }
+}
 
 template <class T, int W>
 __device__ __forceinline__ float square_sum(const T* p, int n) {
@@ -68,8 +82,8 @@ __device__ __forceinline__ float square_sum(const T* p, int n) {
 }
 
 template <class T>
-__device__ __forceinline__ float square_sum_of(const void* in, long long at, int n) {
-  const T* p = static_cast<const T*>(in) + at;
+__device__ __forceinline__ float square_sum_of(const void* in, int n) {
+  const T* p = static_cast<const T*>(in);
   // a tensor that does not start on 16 bytes is read a value at a time
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 ? square_sum<T, 16 / (int)sizeof(T)>(p, n) : square_sum<T, 1>(p, n);
 }
@@ -87,41 +101,42 @@ __device__ __forceinline__ double block_sum(double v) {
   return s;
 }
 
-template <int N>
-__global__ void __launch_bounds__(kClipThreads, kClipCtasPerSm) clip_norm_kernel(const __grid_constant__ ClipArgs<N> a) {
+__global__ void __launch_bounds__(kClipThreads, kClipCtasPerSm) clip_norm_kernel(const ClipPiece* __restrict__ piece, int pieces, double* __restrict__ partial) {
   pdl_wait();
   pdl_launch_dependents();
   double sum = 0;
-  int t = 0;
-  for (int c = blockIdx.x; c < a.first[a.count]; c += gridDim.x) {
-    while (a.first[t + 1] <= c) ++t;
-    const long long at = (long long)(c - a.first[t]) * a.piece, left = a.tensor[t].length - at;
-    const int n = (int)(left < a.piece ? left : a.piece);
-    const int type = a.types[t] & 3;
+  ClipPiece next;
+  if ((int)blockIdx.x < pieces) next = piece[blockIdx.x];
+  for (int c = blockIdx.x; c < pieces; c += gridDim.x) {
+    const ClipPiece p = next;
+    if (c + (int)gridDim.x < pieces) next = piece[c + gridDim.x];
+    const int type = p.types & 3;
     float s;
-    if (type == FLEXSPMV_TYPE_F32) s = square_sum_of<float>(a.tensor[t].in, at, n);
-    else if (type == FLEXSPMV_TYPE_BF16) s = square_sum_of<__nv_bfloat16>(a.tensor[t].in, at, n);
-    else s = square_sum_of<__half>(a.tensor[t].in, at, n);
+    if (type == FLEXSPMV_TYPE_F32) s = square_sum_of<float>(p.in, p.length);
+    else if (type == FLEXSPMV_TYPE_BF16) s = square_sum_of<__nv_bfloat16>(p.in, p.length);
+    else s = square_sum_of<__half>(p.in, p.length);
     sum += (double)s;
   }
   sum = block_sum(sum);
-  if (threadIdx.x == 0) a.partial[a.partial_at + blockIdx.x] = sum;
+  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-// kW values at a time (the number that fills 16 bytes of the narrower side).
+// kW values at a time: 16 bytes of the wider side, so that a warp's stores are whole lines (8 values of bfloat16 into 32 bits as two stores of 16
+// bytes each, 32 bytes apart, took 580 us for 400 M values).
 template <class TI, class TO>
 __device__ __forceinline__ void scale_piece(const TI* in, TO* out, int n, float scale) {
-  constexpr int kW = 16 / (int)(sizeof(TI) < sizeof(TO) ? sizeof(TI) : sizeof(TO));
+  constexpr int kW = 16 / (int)(sizeof(TI) < sizeof(TO) ? sizeof(TO) : sizeof(TI));
   int done = 0;
   if (((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0) {
     const int full = n / kW;
     int i = threadIdx.x;
-    for (; i + 3 * kClipThreads < full; i += 4 * kClipThreads) {
-      Pack<TI, kW> v[4];
+    constexpr int kU = 8;
+    for (; i + (kU - 1) * kClipThreads < full; i += kU * kClipThreads) {
+      Pack<TI, kW> v[kU];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u].load(in + (size_t)(i + u * kClipThreads) * kW);
+      for (int u = 0; u < kU; ++u) v[u].load(in + (size_t)(i + u * kClipThreads) * kW);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kU; ++u) {
         Pack<TO, kW> r;
 #pragma unroll
         for (int x = 0; x < kW; ++x) r.set(x, v[u].get(x) * scale);
@@ -142,77 +157,58 @@ __device__ __forceinline__ void scale_piece(const TI* in, TO* out, int n, float 
 }
 
 template <class TI>
-__device__ __forceinline__ void scale_piece_to(const TI* in, void* out, int type, long long at, int n, float scale) {
-  if (type == FLEXSPMV_TYPE_F32) scale_piece(in, static_cast<float*>(out) + at, n, scale);
-  else if (type == FLEXSPMV_TYPE_BF16) scale_piece(in, static_cast<__nv_bfloat16*>(out) + at, n, scale);
-  else scale_piece(in, static_cast<__half*>(out) + at, n, scale);
+__device__ __forceinline__ void scale_piece_to(const void* in, void* out, int type, int n, float scale) {
+  const TI* from = static_cast<const TI*>(in);
+  if (type == FLEXSPMV_TYPE_F32) scale_piece(from, static_cast<float*>(out), n, scale);
+  else if (type == FLEXSPMV_TYPE_BF16) scale_piece(from, static_cast<__nv_bfloat16*>(out), n, scale);
+  else scale_piece(from, static_cast<__half*>(out), n, scale);
 }
 
-template <int N>
-__global__ void __launch_bounds__(kClipThreads, kClipCtasPerSm) clip_scale_kernel(const __grid_constant__ ClipArgs<N> a) {
+__global__ void __launch_bounds__(kClipThreads, kClipCtasPerSm) clip_scale_kernel(const ClipPiece* __restrict__ piece, int pieces, const double* __restrict__ partial,
+                                                                                  int partials, float max_norm, float* __restrict__ norm_out, int write) {
   pdl_wait();
   pdl_launch_dependents();
+  const int first = pieces - 1 - (int)blockIdx.x;
+  ClipPiece next;
+  if (first >= 0) next = piece[first];
   double sum = 0;
-  for (int i = threadIdx.x; i < a.partials; i += kClipThreads) sum += a.partial[i];
+  for (int i = threadIdx.x; i < partials; i += kClipThreads) sum += partial[i];
   const float norm = (float)sqrt(block_sum(sum));
-  if (a.partial_at == 0 && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
-  if (!a.write) return;
-  const float ratio = a.max_norm / (norm + kClipEps);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+  if (!write) return;
+  const float ratio = max_norm / (norm + kClipEps);
   const float scale = ratio > 1.f ? 1.f : ratio;           // a NaN stays one
-  int t = a.count - 1;
-  const int all = a.first[a.count];
-  for (int c = all - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
-    while (a.first[t] > c) --t;
-    const int type = a.types[t] & 3, out_type = a.types[t] >> 2;
-    if (scale == 1.f && a.tensor[t].in == a.tensor[t].out && type == out_type) continue;       // nothing to change
-    const long long at = (long long)(c - a.first[t]) * a.piece, left = a.tensor[t].length - at;
-    const int n = (int)(left < a.piece ? left : a.piece);
-    if (type == FLEXSPMV_TYPE_F32) scale_piece_to(static_cast<const float*>(a.tensor[t].in) + at, a.tensor[t].out, out_type, at, n, scale);
-    else if (type == FLEXSPMV_TYPE_BF16) scale_piece_to(static_cast<const __nv_bfloat16*>(a.tensor[t].in) + at, a.tensor[t].out, out_type, at, n, scale);
-    else scale_piece_to(static_cast<const __half*>(a.tensor[t].in) + at, a.tensor[t].out, out_type, at, n, scale);
+  for (int c = first; c >= 0; c -= gridDim.x) {
+    const ClipPiece p = next;
+    if (c >= (int)gridDim.x) next = piece[c - gridDim.x];
+    const int type = p.types & 3, out_type = p.types >> 2;
+    if (scale == 1.f && p.in == p.out && type == out_type) continue;       // nothing to change
+    if (type == FLEXSPMV_TYPE_F32) scale_piece_to<float>(p.in, p.out, out_type, p.length, scale);
+    else if (type == FLEXSPMV_TYPE_BF16) scale_piece_to<__nv_bfloat16>(p.in, p.out, out_type, p.length, scale);
+    else scale_piece_to<__half>(p.in, p.out, out_type, p.length, scale);
   }
 }
 
 static int clip_ctas() { return device_sm_count() * kClipCtasPerSm; }
 
-template <int N>
-static int clip_launches(int count, const void* const* grads, void* const* outs, const int64_t* lengths, const int32_t* types, const int32_t* out_types,
-                         long long total, float max_norm, float* norm, double* partial, cudaStream_t st) {
-  static_assert(sizeof(ClipArgs<N>) <= 32764, "kernel parameters");
-  // pieces of 4096 elements, larger where every CTA would have many
-  const int ctas = clip_ctas();
-  long long piece = (total / ((long long)ctas * 8) + 4095) / 4096 * 4096;
-  piece = piece < 4096 ? 4096 : piece > 65536 ? 65536 : piece;
-  const int parts = (count + N - 1) / N > 0 ? (count + N - 1) / N : 1;
-  for (int pass = 0; pass < 2; ++pass) {
-    // the second launches run from the last part to the first, as each runs from its last piece to its first
-    for (int i = 0; i < parts; ++i) {
-      const int part = pass ? parts - 1 - i : i, from = part * N, n = count - from < N ? count - from : N;
-      ClipArgs<N> a;
-      long long pieces = 0;
-      for (int j = 0; j < n; ++j) {
-        a.tensor[j] = {grads[from + j], outs ? outs[from + j] : nullptr, lengths[from + j]};
-        a.types[j] = (unsigned char)(types[from + j] | ((outs ? out_types[from + j] : 0) << 2));
-        a.first[j] = (int)pieces;
-        pieces += (lengths[from + j] + piece - 1) / piece;
-        if (pieces > 0x3fffffffLL) return FLEXSPMV_ERR_TOO_LARGE;
-      }
-      a.first[n] = (int)pieces;
-      a.count = n;
-      a.piece = (int)piece;
-      a.partial = partial;
-      a.partial_at = part * ctas;
-      a.partials = parts * ctas;
-      a.max_norm = max_norm;
-      a.norm = norm;
-      a.write = outs != nullptr;
-      if (pass == 0) {
-        if (int e = launch_pdl(clip_norm_kernel<N>, ctas, kClipThreads, 0, st, a)) return e;
-      } else if (a.write || part == 0) {
-        if (int e = launch_pdl(clip_scale_kernel<N>, a.write ? ctas : 1, kClipThreads, 0, st, a)) return e;
-      }
-    }
+// Pieces of 4096 elements, larger ones where every CTA would have many.
+struct ClipSizes {
+  long long size, pieces;
+  size_t piece_at, bytes;              // the workspace: a sum for each CTA, then the pieces
+};
+static int clip_sizes(int count, const int64_t* lengths, ClipSizes& z) {
+  long long total = 0;
+  for (int i = 0; i < count; ++i) {
+    if (lengths[i] < 0) return FLEXSPMV_ERR_BAD_ARG;
+    total += lengths[i];
   }
+  z.size = (total / ((long long)clip_ctas() * 8) + 4095) / 4096 * 4096;
+  z.size = z.size < 4096 ? 4096 : z.size > 65536 ? 65536 : z.size;
+  z.pieces = 0;
+  for (int i = 0; i < count; ++i) z.pieces += (lengths[i] + z.size - 1) / z.size;
+  if (z.pieces > 0x3fffffffLL) return FLEXSPMV_ERR_TOO_LARGE;
+  z.piece_at = (size_t)clip_ctas() * sizeof(double);
+  z.bytes = z.piece_at + (size_t)z.pieces * sizeof(ClipPiece);
   return 0;
 }
 
@@ -220,34 +216,59 @@ static int clip_launches(int count, const void* const* grads, void* const* outs,
 
 extern "C" {
 
-int flexspmv_clip_gradients_bytes(int32_t count, size_t* bytes) {
-  if (!bytes || count < 0) return FLEXSPMV_ERR_BAD_ARG;
-  *bytes = (size_t)((count + flex::kMost - 1) / flex::kMost + 1) * flex::clip_ctas() * sizeof(double);
+int flexspmv_clip_gradients_bytes(int32_t count, const int64_t* lengths, size_t* bytes, int32_t* pieces) {
+  if (!bytes || !pieces || count < 0 || (count && !lengths)) return FLEXSPMV_ERR_BAD_ARG;
+  flex::ClipSizes z;
+  if (int e = flex::clip_sizes(count, lengths, z)) return e;
+  *bytes = z.bytes;
+  *pieces = (int32_t)z.pieces;
   return 0;
 }
 
-int flexspmv_clip_gradients(int32_t count, const void* const* grads, const int32_t* types, const int64_t* lengths, void* const* outs,
-                            const int32_t* out_types, float max_norm, float* norm, void* ws, size_t ws_bytes, void* stream) {
-  if (count < 0 || !norm || (count && (!grads || !types || !lengths)) || (outs && !out_types)) return FLEXSPMV_ERR_BAD_ARG;
-  long long total = 0;
+int flexspmv_clip_gradients_plan(int32_t count, const void* const* grads, const int32_t* types, const int64_t* lengths, void* const* outs,
+                                 const int32_t* out_types, void* ws, size_t ws_bytes, void* stream) {
+  if (count < 0 || (count && (!grads || !types || !lengths)) || (outs && !out_types)) return FLEXSPMV_ERR_BAD_ARG;
+  flex::ClipSizes z;
+  if (int e = flex::clip_sizes(count, lengths, z)) return e;
   for (int i = 0; i < count; ++i) {
-    if (lengths[i] < 0 || (lengths[i] && (!grads[i] || (outs && !outs[i]))) || !flex::known_type(types[i]) || (outs && !flex::known_type(out_types[i])))
+    if ((lengths[i] && (!grads[i] || (outs && !outs[i]))) || !flex::known_type(types[i]) || (outs && !flex::known_type(out_types[i])))
       return FLEXSPMV_ERR_BAD_ARG;
     const uintptr_t off = (reinterpret_cast<uintptr_t>(grads[i]) & (uintptr_t)(flex::type_bytes(types[i]) - 1)) |
                           (outs ? reinterpret_cast<uintptr_t>(outs[i]) & (uintptr_t)(flex::type_bytes(out_types[i]) - 1) : 0);
     if (off) return FLEXSPMV_ERR_ALIGN;
     if (outs && lengths[i] && outs[i] == grads[i] && out_types[i] != types[i]) return FLEXSPMV_ERR_BAD_ARG;      // in place: one type
-    total += lengths[i];
   }
-  size_t need = 0;
-  flexspmv_clip_gradients_bytes(count, &need);
-  if (!ws || ws_bytes < need) return FLEXSPMV_ERR_WORKSPACE;
-  if (reinterpret_cast<uintptr_t>(ws) & 7u) return FLEXSPMV_ERR_ALIGN;
+  if (!ws || ws_bytes < z.bytes) return FLEXSPMV_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(ws) & 15u) return FLEXSPMV_ERR_ALIGN;
+  flex::ClipTensors t;
+  t.piece = reinterpret_cast<flex::ClipPiece*>(static_cast<char*>(ws) + z.piece_at);
+  t.size = (int)z.size;
+  long long first = 0;
+  for (int from = 0; from < count; from += flex::kPlanTensors) {
+    const int n = count - from < flex::kPlanTensors ? count - from : flex::kPlanTensors;
+    for (int i = 0; i < n; ++i) {
+      t.in[i] = grads[from + i];
+      t.out[i] = outs ? outs[from + i] : nullptr;
+      t.length[i] = lengths[from + i];
+      t.first[i] = first;
+      t.types[i] = (unsigned char)(types[from + i] | ((outs ? out_types[from + i] : types[from + i]) << 2));
+      first += (lengths[from + i] + z.size - 1) / z.size;
+    }
+    if (int e = flex::launch_pdl(flex::clip_plan_kernel, n, 256, 0, static_cast<cudaStream_t>(stream), t)) return e;
+  }
+  return 0;
+}
+
+int flexspmv_clip_gradients(int32_t pieces, int32_t write, float max_norm, float* norm, void* ws, size_t ws_bytes, void* stream) {
+  const int most = flex::clip_ctas();
+  if (pieces < 0 || !norm) return FLEXSPMV_ERR_BAD_ARG;
+  if (!ws || ws_bytes < (size_t)most * sizeof(double) + (size_t)pieces * sizeof(flex::ClipPiece)) return FLEXSPMV_ERR_WORKSPACE;
+  double* const partial = static_cast<double*>(ws);
+  const flex::ClipPiece* const piece = reinterpret_cast<const flex::ClipPiece*>(static_cast<char*>(ws) + (size_t)most * sizeof(double));
+  const int ctas = pieces < 1 ? 1 : pieces < most ? pieces : most;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // a launch copies its parameters, so lists that fit 100 entries take the smaller ones
-  if (count <= 100) return flex::clip_launches<100>(count, grads, outs, lengths, types, out_types, total, max_norm, norm, static_cast<double*>(ws), st);
-  if (count <= 300) return flex::clip_launches<300>(count, grads, outs, lengths, types, out_types, total, max_norm, norm, static_cast<double*>(ws), st);
-  return flex::clip_launches<flex::kMost>(count, grads, outs, lengths, types, out_types, total, max_norm, norm, static_cast<double*>(ws), st);
+  if (int e = flex::launch_pdl(flex::clip_norm_kernel, ctas, flex::kClipThreads, 0, st, piece, pieces, partial)) return e;
+  return flex::launch_pdl(flex::clip_scale_kernel, write ? ctas : 1, flex::kClipThreads, 0, st, piece, pieces, static_cast<const double*>(partial), ctas, max_norm, norm, write);
 }
 
 }  // extern "C"

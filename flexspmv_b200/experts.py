@@ -78,7 +78,8 @@ _P, _I, _N = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
 _WITH_WORKSPACE = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P, _N, _P)
 _GROUPED = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P, _N, _P, _P)
 _PLAIN = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P)
-_CLIP = ctypes.CFUNCTYPE(_I, ctypes.c_int32, _P, _P, _P, _P, _P, ctypes.c_float, _P, _P, _N, _P)
+_CLIP = ctypes.CFUNCTYPE(_I, ctypes.c_int32, ctypes.c_int32, ctypes.c_float, _P, _P, _N, _P)
+_CLIP_PLAN = ctypes.CFUNCTYPE(_I, ctypes.c_int32, _P, _P, _P, _P, _P, _P, _N, _P)
 _functions: Dict[str, object] = {}
 
 
@@ -392,13 +393,18 @@ def _clip(tensors: Sequence[torch.Tensor], max_norm: float, outs) -> BoundCall:
             _whole(o, f"out {i}")
         pout, out_types = _pointers(outs), (ctypes.c_int32 * n)(*[_TYPE[o.dtype] for o in outs])
     lib = load_library()
-    need = ctypes.c_size_t()
-    _check_status(lib, lib.flexspmv_clip_gradients_bytes(n, ctypes.byref(need)), "clip_gradients")
+    need, pieces = ctypes.c_size_t(), ctypes.c_int32()
+    _check_status(lib, lib.flexspmv_clip_gradients_bytes(n, lengths, ctypes.byref(need), ctypes.byref(pieces)), "clip_gradients")
     ws = torch.empty(need.value // 8, dtype=torch.float64, device=tensors[0].device)
     norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
-    args = (n, ctypes.addressof(pin), ctypes.addressof(types), ctypes.addressof(lengths), ctypes.addressof(pout) if pout is not None else None,
-            ctypes.addressof(out_types) if out_types is not None else None, float(max_norm), norm.data_ptr(), ws.data_ptr(), need.value)
-    return BoundCall(_function("clip_gradients", _CLIP), args, dev, (pin, pout, types, out_types, lengths, ws, tensors, outs), norm)
+    with torch.cuda.device(dev):
+        st = _function("clip_gradients_plan", _CLIP_PLAN)(n, ctypes.addressof(pin), ctypes.addressof(types), ctypes.addressof(lengths),
+                                                          ctypes.addressof(pout) if pout is not None else None,
+                                                          ctypes.addressof(out_types) if out_types is not None else None, ws.data_ptr(), need.value,
+                                                          _raw_stream(dev))
+    _check_status(lib, st, "clip_gradients_plan")
+    args = (pieces.value, outs is not None, float(max_norm), norm.data_ptr(), ws.data_ptr(), need.value)
+    return BoundCall(_function("clip_gradients", _CLIP), args, dev, (ws, tensors, outs), norm)
 
 
 @_operator

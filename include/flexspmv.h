@@ -516,14 +516,18 @@ int flexspmv_expert_combine(const flexspmv_expert_desc *desc, const void *const 
 int flexspmv_expert_combine_backward(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *stream);
 
 /*
- * The norm over many tensors, norm = sqrt(sum of all squares), and, where outs is not null, outs[i] = grads[i] * min(1, max_norm /
- * (norm + 1e-6)).  grads, types, lengths, outs and out_types are HOST arrays of count entries, read before the call returns; the tensors
- * are contiguous device memory.  outs[i] may be grads[i] of the same type, and is left alone then where the norm is within max_norm.
- * d_norm: one float.  A norm that is not finite scales as the formula says (infinity: 0 and NaN; NaN: NaN).
+ * The norm over many tensors, norm = sqrt(sum of all squares), and their scaling, out[i] = grad[i] * min(1, max_norm / (norm + 1e-6)).
+ *   _bytes  the workspace, and the number of pieces that the tensors are cut into
+ *   _plan   writes the pieces into the workspace, once for tensors that stay where they are.  grads, types, lengths, outs and out_types are
+ *           HOST arrays of count entries, read before the call returns; the tensors are contiguous device memory of any of the three types.
+ *           outs null: for the norm alone; outs[i] may be grads[i] of the same type, and is left alone then where the norm is within max_norm
+ *   flexspmv_clip_gradients  on a planned workspace: *d_norm, and with write != 0 (the plan has outs) the scaled tensors
+ * A norm that is not finite scales as the formula says (infinity: 0 and NaN; NaN: NaN).
  */
-int flexspmv_clip_gradients_bytes(int32_t count, size_t *bytes);
-int flexspmv_clip_gradients(int32_t count, const void *const *grads, const int32_t *types, const int64_t *lengths, void *const *outs,
-                            const int32_t *out_types, float max_norm, float *d_norm, void *d_workspace, size_t workspace_bytes, void *stream);
+int flexspmv_clip_gradients_bytes(int32_t count, const int64_t *lengths, size_t *bytes, int32_t *pieces);
+int flexspmv_clip_gradients_plan(int32_t count, const void *const *grads, const int32_t *types, const int64_t *lengths, void *const *outs,
+                                 const int32_t *out_types, void *d_workspace, size_t workspace_bytes, void *stream);
+int flexspmv_clip_gradients(int32_t pieces, int32_t write, float max_norm, float *d_norm, void *d_workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
