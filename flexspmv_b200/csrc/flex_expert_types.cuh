@@ -4,6 +4,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/flexspmv.h"
 
 namespace flex {
@@ -48,9 +50,26 @@ struct Pack {
 #pragma unroll
     for (int i = 0; i < W; ++i) v[i] = from_float<T>(0.f);
   }
+  // 16-bit values as they are: two of them, or the only one.
+  __device__ __forceinline__ uint32_t word(int i) const { return i % 4 == 0 ? raw[i / 4].x : i % 4 == 1 ? raw[i / 4].y : i % 4 == 2 ? raw[i / 4].z : raw[i / 4].w; }
+  __device__ __forceinline__ uint32_t bits() const { return *reinterpret_cast<const unsigned short*>(&v[0]); }
   __device__ __forceinline__ float get(int i) const { return to_float(v[i]); }
   __device__ __forceinline__ void set(int i, float x) { v[i] = from_float<T>(x); }
 };
+
+// Lets a kernel have this much dynamic shared memory; the runtime is asked once for a kernel, a device and a size above 48 KB.
+template <auto KERNEL>
+int allow_smem(int bytes) {
+  static std::atomic<int> allowed[64];
+  int device = 0;
+  if (bytes <= 48 * 1024) return 0;
+  if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return (int)e;
+  const bool known = device >= 0 && device < 64;
+  if (known && allowed[device].load(std::memory_order_relaxed) >= bytes) return 0;
+  if (cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); e != cudaSuccess) return (int)e;
+  if (known) allowed[device].store(bytes, std::memory_order_relaxed);
+  return 0;
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool known_type(int t) { return t == FLEXSPMV_TYPE_F32 || t == FLEXSPMV_TYPE_BF16 || t == FLEXSPMV_TYPE_F16; }

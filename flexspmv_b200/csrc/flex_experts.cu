@@ -16,39 +16,54 @@ int device_sm_count();
 
 // ---- router --------------------------------------------------------------------------------------------------------
 
-// What a choice goes by: a number that is larger for a larger logit and, among equal ones, for a lower expert.  0: NaN and -infinity, never
-// chosen.  A 16-bit logit and the expert fit 32 bits, so that one instruction finds the largest of a warp; a 32-bit one takes 64.
+// 2^x by the special-function unit (relative error 2^-22, results below 2^-126 are 0).
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+// e^(v - top).  The difference first: top log2 e as one rounded number would put an error of 2^-24 |top| into the power.
+__device__ __forceinline__ float exp_below(float v, float top) { return exp2_fast((v - top) * kLog2e); }
+
+// What a choice goes by: a number that is larger for a larger logit and, among equal ones, for a lower expert.  The order of a sign and
+// magnitude number x is 0x8000... +- its magnitude (so that -0 and 0 are equal); NaN is 0.  kNone: the key of -infinity and below, never chosen.
+// A 16-bit logit and the expert fit 32 bits, so that one instruction finds the largest of a warp; a 32-bit one takes 64.
 template <class T>
 struct Choice {
   using Key = uint32_t;
-  static __device__ __forceinline__ Key make(float v, int e) {
-    const uint32_t u = bits(v + 0.f);                         // -0 and 0 are equal
-    const uint32_t order = (u & 0x8000u) ? ~u & 0xffffu : u | 0x8000u;
-    return (v != v || v == -INFINITY) ? 0u : order << 16 | (0xffffu - (uint32_t)e);
-  }
-  static __device__ __forceinline__ uint32_t bits(float v) {
-    if constexpr (std::is_same<T, __half>::value) return __half_as_ushort(__float2half_rn(v));
-    else return __float_as_uint(v) >> 16;
-  }
+  static constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  static constexpr Key kNone = (0x8000u - kInf) << 16 | 0xffffu;
   static __device__ __forceinline__ int expert(Key k) { return (int)(0xffffu - (k & 0xffffu)); }
   static __device__ __forceinline__ float logit(Key k) {
-    const uint32_t order = k >> 16, u = (order & 0x8000u) ? order & 0x7fffu : ~order & 0xffffu;
+    const uint32_t order = k >> 16, u = order & 0x8000u ? order & 0x7fffu : 0x10000u - order;      // 0x8000 | (0x8000 - order)
     if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)u));
     else return __uint_as_float(u << 16);
   }
   static __device__ __forceinline__ Key warp_max(Key k) { return __reduce_max_sync(0xffffffffu, k); }
+  // The orders of two logits in one word.  Sign bits spread over their halves by a byte permutation (0xbb99).
+  static __device__ __forceinline__ uint32_t spread(uint32_t two) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(r) : "r"(two));
+    return r;
+  }
+  static __device__ __forceinline__ uint32_t orders(uint32_t two) {
+    const uint32_t negative = spread(two), nan = spread((two & 0x7fff7fffu) + (0x7fffu - kInf) * 0x00010001u);
+    return ((two ^ ((negative & 0x7fff7fffu) ^ 0x80008000u)) + (negative & 0x00010001u)) & ~nan;
+  }
 };
 template <>
 struct Choice<float> {
   using Key = unsigned long long;
+  static constexpr Key kNone = (Key)0x00800000u << 32 | 0xffffu;
   static __device__ __forceinline__ Key make(float v, int e) {
-    const uint32_t u = __float_as_uint(v + 0.f), order = (u & 0x80000000u) ? ~u : u | 0x80000000u;
-    return (v != v || v == -INFINITY) ? 0ull : (Key)order << 32 | (0xffffu - (uint32_t)e);
+    const uint32_t u = __float_as_uint(v), order = u & 0x80000000u ? 0u - u : u | 0x80000000u;       // 0x80000000 - magnitude
+    return v != v ? 0ull : (Key)order << 32 | (0xffffu - (uint32_t)e);
   }
   static __device__ __forceinline__ int expert(Key k) { return (int)(0xffffu - (uint32_t)k); }
   static __device__ __forceinline__ float logit(Key k) {
     const uint32_t order = (uint32_t)(k >> 32);
-    return __uint_as_float((order & 0x80000000u) ? order & 0x7fffffffu : ~order);
+    return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : 0u - order);
   }
   static __device__ __forceinline__ Key warp_max(Key k) {
     const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
@@ -56,7 +71,7 @@ struct Choice<float> {
   }
 };
 
-// Largest first, by odd-even merging (Batcher): V log^2 V exchanges whose places are known when it is compiled.
+// Largest first, by odd-even merging (Batcher): exchanges whose places are known when it is compiled.
 template <class K, int V>
 __device__ __forceinline__ void sort_down(K (&k)[V]) {
 #pragma unroll
@@ -74,10 +89,14 @@ __device__ __forceinline__ void sort_down(K (&k)[V]) {
           }
 }
 
-// A row's part of lane l: V experts, W neighbouring ones at a time.
+// A row's part of lane l: V experts, W neighbouring ones at a time.  What lies beyond the experts is -infinity.
 template <class T, int V, int W>
 struct LanePart {
   Pack<T, W> piece[V / W];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < V; ++i) piece[i / W].set(i % W, -INFINITY);
+  }
   __device__ __forceinline__ void load(const T* row, int experts, int lane) {
 #pragma unroll
     for (int i = 0; i < V / W; ++i) {
@@ -87,45 +106,58 @@ struct LanePart {
   }
 };
 
-// One token by one warp.  Each lane's experts are sorted once; then k rounds of a maximum over the lanes' first ones, the winner's lane
-// moving up its next (equal logits: the lowest expert, as the plain form's stable sort has it).  Lane j ends with choice j.  The softmax is
-// over the true logits, largest subtracted, sums in 32 bits.
+// One token by one warp.  Each lane sorts its experts once and leaves them in shared memory (`list`, V + 1 keys a lane); then k rounds of a
+// maximum over the lanes' first ones, the winner's lane taking up its next (equal logits: the lowest expert, as the plain form's stable
+// sort has it).  Lane j ends with choice j.  The softmax is over the true logits, largest subtracted, sums in 32 bits.
+// Bound by instructions: 660 a token of 256 experts where every round moved the sorted keys up in registers and every logit was made a key
+// and a power on its own.
 template <class T, int V, int W>
-__device__ __forceinline__ void choose_token(const LanePart<T, V, W>& part, int experts, int k, bool renormalize, int lane, int& my_id, float& my_weight) {
+__device__ __forceinline__ void choose_token(const LanePart<T, V, W>& part, int k, bool renormalize, int lane, typename Choice<T>::Key* list, int& my_id,
+                                             float& my_weight) {
   using C = Choice<T>;
-  float v[V];
-  typename C::Key key[V];
+  using Key = typename C::Key;
+  Key key[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int e = (i / W * 32 + lane) * W;
-    v[i] = e < experts ? part.piece[i / W].get(i % W) : -INFINITY;
-    key[i] = C::make(v[i], e + i % W);
+    const uint32_t e = (uint32_t)((i / W * 32 + lane) * W + i % W);
+    if constexpr (std::is_same<T, float>::value) {
+      key[i] = C::make(part.piece[i / W].get(i % W), (int)e);
+    } else if constexpr (W > 1) {
+      if (i % 2 == 0) {
+        const uint32_t order = C::orders(part.piece[i / W].word(i % W / 2));
+        key[i] = order << 16 | (0xffffu - e);
+        key[i + 1] = (order & 0xffff0000u) | (0xfffeu - e);
+      }
+    } else {
+      key[i] = C::orders(part.piece[i].bits()) << 16 | (0xffffu - e);
+    }
   }
   sort_down(key);
-  typename C::Key mine_key = 0, top_key = 0;
-  for (int j = 0; j < k; ++j) {
-    const typename C::Key most = C::warp_max(key[0]);
-    if (most == 0) break;
-    if (j == 0) top_key = most;
-    if (lane == j) mine_key = most;
-    const bool won = key[0] == most;
 #pragma unroll
-    for (int i = 0; i + 1 < V; ++i) key[i] = won ? key[i + 1] : key[i];
-    key[V - 1] = won ? 0 : key[V - 1];
+  for (int i = 1; i < V; ++i) list[i] = key[i];
+  Key first = key[0], mine_key = 0;
+  const Key* next = list + 1;
+#pragma unroll 4
+  for (int j = 0; j < k; ++j) {
+    const Key most = C::warp_max(first);
+    if (lane == j) mine_key = most;
+    if (first == most) first = *next++;          // 32 V keys are no fewer than the experts, so that k rounds never run out of them
   }
+  if (mine_key <= C::kNone) mine_key = 0;
+  const Key top_key = __shfl_sync(0xffffffffu, mine_key, 0);
   my_id = mine_key ? C::expert(mine_key) : -1;
   const float top = top_key ? C::logit(top_key) : 0.f;
-  const float mine = mine_key ? expf(C::logit(mine_key) - top) : 0.f;
+  const float mine = mine_key ? exp_below(C::logit(mine_key), top) : 0.f;
   float sum = 0.f;
   if (renormalize) {
     sum = mine;
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum += (v[i] == -INFINITY) ? 0.f : expf(v[i] - top);
+    for (int i = 0; i < V; ++i) sum += exp_below(part.piece[i / W].get(i % W), top);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  my_weight = mine_key ? mine / sum : 0.f;
+  my_weight = mine_key ? __fdividef(mine, sum) : 0.f;
 }
 
 struct RouteArgs {
@@ -143,7 +175,11 @@ struct RouteArgs {
 // expert, and total[e] (shared) how many there are.
 template <class T, int V, int W, int THREADS>
 __device__ __forceinline__ void choose_chunk(const RouteArgs& a, unsigned* seen, unsigned* total) {
+  using Key = typename Choice<T>::Key;
+  Key* const lists = reinterpret_cast<Key*>(seen + (a.experts * (THREADS / 32) + 1) / 2 * 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Key* const list = lists + threadIdx.x * (V + 1);
+  list[V] = 0;
   for (int i = threadIdx.x; i < a.experts * (THREADS / 32); i += THREADS) seen[i] = 0;
   __syncthreads();
   pdl_wait();
@@ -154,13 +190,14 @@ __device__ __forceinline__ void choose_chunk(const RouteArgs& a, unsigned* seen,
   const T* const logits = static_cast<const T*>(a.logits);
   unsigned* const mine = seen + warp * a.experts;
   LanePart<T, V, W> next;
+  next.clear();
   if (from < to) next.load(logits + from * a.stride, a.experts, lane);
   for (long long t = from; t < to; ++t) {
     const LanePart<T, V, W> part = next;
     if (t + 1 < to) next.load(logits + (t + 1) * a.stride, a.experts, lane);
     int id;
     float weight;
-    choose_token<T, V, W>(part, a.experts, a.k, a.renormalize != 0, lane, id, weight);
+    choose_token<T, V, W>(part, a.k, a.renormalize != 0, lane, list, id, weight);
     if (lane < a.k) {
       a.weights[t * a.k + lane] = weight;
       a.ids[t * a.k + lane] = id;
@@ -223,9 +260,9 @@ __device__ __forceinline__ unsigned sums_before(unsigned* total, int experts, in
 // Small batches: everything in one CTA and one launch.
 template <class T, int V, int W, int THREADS>
 __global__ void __launch_bounds__(THREADS) route_small_kernel(RouteArgs a) {
-  extern __shared__ unsigned route_sm[];
+  extern __shared__ __align__(16) unsigned route_sm[];
   unsigned* const total = route_sm;
-  choose_chunk<T, V, W, THREADS>(a, total + a.experts, total);
+  choose_chunk<T, V, W, THREADS>(a, total + (a.experts + 1) / 2 * 2, total);
   const unsigned used = sums_before<THREADS>(total, a.experts, a.offsets);
   const int pairs = (int)a.tokens * a.k;
   for (int p = threadIdx.x; p < pairs; p += THREADS) {
@@ -241,14 +278,14 @@ __global__ void __launch_bounds__(THREADS) route_small_kernel(RouteArgs a) {
 
 template <class T, int V, int W, int THREADS>
 __global__ void __launch_bounds__(THREADS) route_choose_kernel(RouteArgs a) {
-  extern __shared__ unsigned route_sm[];
+  extern __shared__ __align__(16) unsigned route_sm[];
   unsigned* const total = route_sm;
-  choose_chunk<T, V, W, THREADS>(a, total + a.experts, total);
+  choose_chunk<T, V, W, THREADS>(a, total + (a.experts + 1) / 2 * 2, total);
   for (int i = threadIdx.x; i < a.experts; i += THREADS) a.counts[(size_t)blockIdx.x * a.experts + i] = total[i];
 }
 
 // Every CTA adds up the counts of all CTAs by itself (they lie in L2): a launch fewer than a scan between the two would take.
-constexpr int kPlaceThreads = 512;
+constexpr int kPlaceThreads = 1024;
 __global__ void __launch_bounds__(kPlaceThreads) route_place_kernel(RouteArgs a) {
   extern __shared__ unsigned route_sm[];
   unsigned *total = route_sm, *before = total + a.experts;
@@ -303,6 +340,9 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const float* __rest
   for (long long t = (long long)blockIdx.x * 8 + warp; t < tokens; t += (long long)gridDim.x * 8) {
     const int id = lane < k ? ids[t * k + lane] : -1;
     const float w = id >= 0 ? weights[t * k + lane] : 0.f, g = id >= 0 ? dweights[t * k + lane] : 0.f;
+    const T* row = logits + t * stride;
+    Pack<T, W> v;
+    if (!renormalize && lane * W < experts) v.load(row + lane * W);          // under way while the sum is made
     float mean = w * g;
 #pragma unroll
     for (int o = 16; o; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
@@ -314,13 +354,12 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const float* __rest
       none.zero();
       for (int e = lane * W; e < experts; e += 32 * W) none.store(out + e);
     } else {
-      const T* row = logits + t * stride;
       const float top = to_float(row[top_id]), scale = -top_w * mean;
       for (int e = lane * W; e < experts; e += 32 * W) {
-        Pack<T, W> v, r;
-        v.load(row + e);
+        if (e >= 32 * W) v.load(row + e);
+        Pack<T, W> r;
 #pragma unroll
-        for (int x = 0; x < W; ++x) r.set(x, v.get(x) == -INFINITY ? 0.f : scale * expf(v.get(x) - top));
+        for (int x = 0; x < W; ++x) r.set(x, scale * exp_below(v.get(x), top));
         r.store(out + e);
       }
     }
@@ -438,19 +477,25 @@ static int route_ctas(long long tokens) {
 }
 constexpr long long kRouteSmall = 64;      // tokens up to which one CTA does it all
 
-// THREADS: as many as leave `seen` (a word for each warp and expert) within 48 KB of shared memory.
+// THREADS: as many as leave `seen` (a word for each warp and expert) within 64 KB of shared memory, beside them 17 KB to 72 KB for the lists.
+template <class T, int V, int W, int THREADS, bool SMALL>
+static int route_kernel(const RouteArgs& a, int ctas, cudaStream_t st) {
+  constexpr auto kernel = SMALL ? route_small_kernel<T, V, W, THREADS> : route_choose_kernel<T, V, W, THREADS>;
+  const int smem = ((a.experts + 1) / 2 * 2 + (a.experts * (THREADS / 32) + 1) / 2 * 2) * 4 + THREADS * (V + 1) * (int)sizeof(typename Choice<T>::Key);
+  if (int e = allow_smem<kernel>(smem)) return e;
+  return launch_pdl(kernel, ctas, THREADS, smem, st, a);
+}
+
 template <class T, int V, int W, int THREADS>
 static int route_launch(const RouteArgs& args, cudaStream_t st) {
   RouteArgs a = args;
-  const auto smem = [&](int threads) { return (size_t)a.experts * 4 * (1 + threads / 32); };
   if (a.tokens <= kRouteSmall) {
     a.chunk = a.tokens;
-    if (a.tokens <= 8) return launch_pdl(route_small_kernel<T, V, W, 256>, 1, 256, smem(256), st, a);
-    return launch_pdl(route_small_kernel<T, V, W, THREADS>, 1, THREADS, smem(THREADS), st, a);
+    return a.tokens <= 8 ? route_kernel<T, V, W, 256, true>(a, 1, st) : route_kernel<T, V, W, THREADS, true>(a, 1, st);
   }
   const int ctas = route_ctas(a.tokens);
   a.chunk = (a.tokens + ctas - 1) / ctas;
-  if (int e = launch_pdl(route_choose_kernel<T, V, W, THREADS>, ctas, THREADS, smem(THREADS), st, a)) return e;
+  if (int e = route_kernel<T, V, W, THREADS, false>(a, ctas, st)) return e;
   return launch_pdl(route_place_kernel, ctas, kPlaceThreads, (size_t)a.experts * 8, st, a);
 }
 

@@ -389,8 +389,8 @@ static int grouped_launch_as(const GroupedArgs& a, cudaStream_t st) {
     row_b = mb;
   }
   const int smem = 1024 + Cfg::kStages * Cfg::kStageBytes + Cfg::kStoreBytes + (int)sizeof(GroupedBars) + (a.experts + 1) * (int)sizeof(GroupedTable);
-  auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR>;
-  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return (int)e;
+  constexpr auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR>;
+  if (int e = allow_smem<kernel>(smem)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(device_sm_count() / PAIR * PAIR)); cfg.blockDim = dim3(kGroupedThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
   cudaLaunchAttribute attr[2];
