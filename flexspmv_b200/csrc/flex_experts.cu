@@ -167,7 +167,7 @@ struct RouteArgs {
   long long chunk;                 // tokens of a CTA
   float* weights;
   int *ids, *offsets, *rows, *slots;
-  unsigned* counts;                // [CTAs][experts]
+  unsigned* counts;                // [CTAs][experts, a multiple of four]
 };
 
 // Choices of this CTA's tokens, a run of them for each warp.  `seen` (shared, [warps][experts]) counts each warp's pairs of an expert, in
@@ -281,7 +281,8 @@ __global__ void __launch_bounds__(THREADS) route_choose_kernel(RouteArgs a) {
   extern __shared__ __align__(16) unsigned route_sm[];
   unsigned* const total = route_sm;
   choose_chunk<T, V, W, THREADS>(a, total + (a.experts + 1) / 2 * 2, total);
-  for (int i = threadIdx.x; i < a.experts; i += THREADS) a.counts[(size_t)blockIdx.x * a.experts + i] = total[i];
+  const int wide = (a.experts + 3) / 4 * 4;              // the place kernel reads four at a time
+  for (int i = threadIdx.x; i < wide; i += THREADS) a.counts[(size_t)blockIdx.x * wide + i] = i < a.experts ? total[i] : 0u;
 }
 
 // Every CTA adds up the counts of all CTAs by itself (they lie in L2): a launch fewer than a scan between the two would take.
@@ -292,40 +293,54 @@ __global__ void __launch_bounds__(kPlaceThreads) route_place_kernel(RouteArgs a)
   for (int i = threadIdx.x; i < a.experts; i += kPlaceThreads) total[i] = before[i] = 0;
   __syncthreads();
   pdl_wait();
-  // as many threads on an expert as there are; each adds every parts-th CTA's count
-  const int parts = kPlaceThreads / a.experts > 0 ? kPlaceThreads / a.experts : 1;
-  for (int i = threadIdx.x; i < a.experts * parts; i += kPlaceThreads) {
-    const int e = i % a.experts, part = i / a.experts;
-    unsigned all = 0, prior = 0;
-#pragma unroll 16
+  const long long from = a.chunk * blockIdx.x * a.k, end = from + a.chunk * a.k, pairs = a.tokens * a.k, to = end < pairs ? end : pairs;
+  int id[2], number[2];                    // this thread's first pairs, under way while the counts are added up
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const long long p = from + threadIdx.x + u * kPlaceThreads;
+    id[u] = p < to ? a.ids[p] : -1;
+    number[u] = p < to ? a.slots[p] : -1;
+  }
+  // as many threads on four experts as there are; each adds every parts-th CTA's counts
+  const int fours = (a.experts + 3) / 4, parts = kPlaceThreads / fours;
+  for (int i = threadIdx.x; i < fours * parts; i += kPlaceThreads) {
+    const int e = i % fours * 4, part = i / fours;
+    unsigned all[4] = {}, prior[4] = {};
+#pragma unroll 8
     for (unsigned b = part; b < gridDim.x; b += parts) {
-      const unsigned n = a.counts[(size_t)b * a.experts + e];
-      all += n;
-      prior += b < blockIdx.x ? n : 0u;
+      const uint4 n = *reinterpret_cast<const uint4*>(a.counts + (size_t)b * fours * 4 + e);
+      const unsigned c[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        all[x] += c[x];
+        prior[x] += b < blockIdx.x ? c[x] : 0u;
+      }
     }
-    if (parts == 1) {
-      total[e] = all;
-      before[e] = prior;
-    } else {
-      atomicAdd(&total[e], all);
-      atomicAdd(&before[e], prior);
-    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (e + x < a.experts) {
+        atomicAdd(&total[e + x], all[x]);
+        if (prior[x]) atomicAdd(&before[e + x], prior[x]);
+      }
   }
   __syncthreads();
   const unsigned used = sums_before<kPlaceThreads>(total, a.experts, blockIdx.x == 0 ? a.offsets : nullptr);
   for (int e = threadIdx.x; e < a.experts; e += kPlaceThreads) before[e] += total[e];
   __syncthreads();
-  const long long from = a.chunk * blockIdx.x * a.k, end = from + a.chunk * a.k, pairs = a.tokens * a.k, to = end < pairs ? end : pairs;
-#pragma unroll 4
-  for (long long p = from + threadIdx.x; p < to; p += kPlaceThreads) {
-    const int id = a.ids[p];
-    if (id >= 0) {
-      const int place = a.slots[p] + (int)before[id];
+  const auto put = [&](long long p, int i, int n) {
+    if (i >= 0) {
+      const int place = n + (int)before[i];
       a.slots[p] = place;
       a.rows[place] = (int)((unsigned)p / (unsigned)a.k);
     }
     if (p >= (long long)used) a.rows[p] = -1;
+  };
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const long long p = from + threadIdx.x + u * kPlaceThreads;
+    if (p < to) put(p, id[u], number[u]);
   }
+  for (long long p = from + threadIdx.x + 2 * kPlaceThreads; p < to; p += kPlaceThreads) put(p, a.ids[p], a.slots[p]);
 }
 
 // Gradient of the chosen weights with respect to the logits.  p_i = w_0 exp(l_i - l_{e_0}): the largest weight and its logit stand for the
@@ -542,7 +557,7 @@ extern "C" {
 int flexspmv_expert_route_bytes(const flexspmv_expert_desc* d, size_t* bytes) {
   if (!d || !bytes || d->tokens < 0 || d->experts < 1) return FLEXSPMV_ERR_BAD_ARG;
   if (d->experts > FLEXSPMV_MAX_EXPERTS) return FLEXSPMV_ERR_TOO_LARGE;
-  *bytes = (size_t)flex::route_ctas(d->tokens) * d->experts * 4;
+  *bytes = (size_t)flex::route_ctas(d->tokens) * ((d->experts + 3) / 4 * 16);
   return 0;
 }
 
@@ -560,6 +575,7 @@ int flexspmv_expert_route(const flexspmv_expert_desc* d, const void* const* in, 
   size_t need = 0;
   flexspmv_expert_route_bytes(d, &need);
   if (!ws || ws_bytes < need) return FLEXSPMV_ERR_WORKSPACE;
+  if (!flex::aligned16(ws)) return FLEXSPMV_ERR_ALIGN;
   flex::RouteArgs a = {in[0], d->tokens, d->in_stride, d->experts, d->choices, d->flags & FLEXSPMV_EXPERT_RENORMALIZE, 0,
                        static_cast<float*>(out[0]), static_cast<int*>(out[1]), static_cast<int*>(out[2]), static_cast<int*>(out[3]),
                        static_cast<int*>(out[4]), static_cast<unsigned*>(ws)};

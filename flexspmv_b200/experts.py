@@ -202,18 +202,19 @@ def route(logits: torch.Tensor, k: int, renormalize: bool = False) -> Plan:
     lib = load_library()
     need = ctypes.c_size_t()
     _check_status(lib, lib.flexspmv_expert_route_bytes(ctypes.byref(d), ctypes.byref(need)), "route")
-    # one allocation: the plan's arrays behind one another, then the workspace
+    # one allocation: the plan's arrays and the workspace behind one another, each on 16 bytes
     pairs = tokens * k
-    buf = torch.empty(4 * pairs + experts + 1 + need.value // 4, dtype=torch.int32, device=logits.device)
+    step, ends = -(-pairs // 4) * 4, -(-(experts + 1) // 4) * 4
+    buf = torch.empty(4 * step + ends + need.value // 4, dtype=torch.int32, device=logits.device)
     weights = buf[:pairs].view(torch.float32).view(tokens, k)
-    ids, slots = buf[pairs:2 * pairs].view(tokens, k), buf[2 * pairs:3 * pairs].view(tokens, k)
-    rows, offsets = buf[3 * pairs:4 * pairs], buf[4 * pairs:4 * pairs + experts + 1]
+    ids, slots = buf[step:step + pairs].view(tokens, k), buf[2 * step:2 * step + pairs].view(tokens, k)
+    rows, offsets = buf[3 * step:3 * step + pairs], buf[4 * step:4 * step + experts + 1]
     plan = Plan(weights, ids, offsets, rows, slots, bool(renormalize))
     base = buf.data_ptr()
-    outs = (ctypes.c_void_p * 5)(base, base + 4 * pairs, base + 16 * pairs, base + 12 * pairs, base + 8 * pairs)
+    outs = (ctypes.c_void_p * 5)(base, base + 4 * step, base + 16 * step, base + 12 * step, base + 8 * step)
     ins = (ctypes.c_void_p * 1)(logits.data_ptr())
     return BoundCall(_function("expert_route", _WITH_WORKSPACE),
-                     (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), base + 16 * pairs + 4 * (experts + 1), need.value), dev,
+                     (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), base + 16 * step + 4 * ends, need.value), dev,
                      (d, ins, outs, logits, buf), plan)
 
 
