@@ -19,6 +19,7 @@ struct GroupedArgs {
   long long slots, a_stride, b_stride;
   int experts, n, k;
   int* status;
+  int behind_copy;               // launched behind take_rows_kernel, of which nothing but x's copy is waited for
 };
 
 __device__ __forceinline__ void raise(int* status, int code) {
@@ -56,9 +57,9 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict_
 //   dw            128 of n by 256 of k, summed over the expert's places
 // PAIR = 2: two CTAs on two neighbouring SMs take a tile of 256 rows, 128 each; each copies half of the columns' operand for both, which
 // halves what those columns cost the L2 (from 48 KB to 32 KB an SM for 64 of the sum).
-// Warps 0-3 store finished accumulators, warp 4 issues the tile copies, warp 5 the matrix instructions; two accumulators in tensor memory,
+// Warps 0-7 store finished accumulators, warp 8 issues the tile copies, warp 9 the matrix instructions; two accumulators in tensor memory,
 // so that one is stored while the next is computed.  The sum goes 64 values (128 bytes of a row) a stage.
-constexpr int kGroupedThreads = 192;
+constexpr int kStoreWarps = 8, kCopyWarp = kStoreWarps, kMathWarp = kStoreWarps + 1, kGroupedThreads = (kStoreWarps + 2) * 32;
 constexpr int kTileBytesA = 128 * 128;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 
@@ -68,7 +69,7 @@ struct GroupedCfg {
   static constexpr int kStageBytes = kTileBytesA + kBytesB;
   static constexpr int kStages = 196608 / kStageBytes;
   static constexpr int kTmemCols = 2 * NT < 32 ? 32 : 2 * NT;
-  static constexpr int kStoreBytes = MODE == FLEXSPMV_GROUPED_DW ? 4 * 4096 : 4 * 2048;
+  static constexpr int kStoreBytes = kStoreWarps * 2048;
 };
 
 struct GroupedTable {            // of an expert: its first place, its places, its first tile; and of one past the last: the number of tiles
@@ -143,14 +144,14 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
 
   if (tid == 0) {
     for (int i = 0; i < Cfg::kStages; ++i) { mbar_init(&bars.full[i], 1); mbar_init(&bars.empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&bars.acc_full[i], 1); mbar_init(&bars.acc_empty[i], 4 * PAIR); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&bars.acc_full[i], 1); mbar_init(&bars.acc_empty[i], kStoreWarps * PAIR); }
     bars.abort = 0;
     mbar_fence_init();
     tma_prefetch_map(&map_a);
     tma_prefetch_map(&map_b);
   }
-  if (warp == 5) tmem_alloc<PAIR, Cfg::kTmemCols>(&bars.tmem);
-  pdl_wait();
+  if (warp == kMathWarp) tmem_alloc<PAIR, Cfg::kTmemCols>(&bars.tmem);
+  if (!a.behind_copy) pdl_wait();
   for (int e = tid; e < a.experts; e += kGroupedThreads) {
     int from, to;
     group_of(a, e, from, to);
@@ -194,29 +195,44 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
     return ((MODE == FLEXSPMV_GROUPED_FORWARD ? a.k : MODE == FLEXSPMV_GROUPED_DX ? a.n : t.count) + 63) / 64;
   };
 
-  if (warp == 4) {
+  if (warp == kCopyWarp) {
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     if (elect_one()) {
+      int ahead = 0;                       // steps whose weights are on their way before x's copy is there
       for (int i = first; i < tiles && !*abort; i += stride) {
         const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
         const int steps = steps_of(t), half = t.cols / PAIR;
         const int pieces = MODE == FLEXSPMV_GROUPED_DW ? (half + 63) / 64 : (half + 31) / 32;
         const int bytes = PAIR * (kTileBytesA + pieces * 4096);
         const int m0 = t.m0 + rank * 128;
+        auto copy_weights = [&](int s, int to) {
+          unsigned char* const sa = base + to * Cfg::kStageBytes;
+          const uint32_t bar = PAIR == 2 ? cluster_smem(&bars.full[to], 0) : smem_u32(&bars.full[to]);
+          if (rank == 0) mbar_expect_tx(&bars.full[to], bytes);
+          if (MODE == FLEXSPMV_GROUPED_FORWARD) {
+            tma_3d<PAIR>(sa, &map_a, s * 64, m0, t.e, bar);
+          } else {
+            tma_3d<PAIR>(sa, &map_a, m0, s * 64, t.e, bar);
+            tma_3d<PAIR>(sa + 8192, &map_a, m0 + 64, s * 64, t.e, bar);
+          }
+        };
+        if (a.behind_copy && i == first) {
+          if (MODE != FLEXSPMV_GROUPED_DW)
+            for (; ahead < Cfg::kStages && ahead < steps; ++ahead) copy_weights(ahead, ahead);
+          pdl_wait();
+        }
         for (int s = 0; s < steps; ++s) {
           if (!wait(&bars.empty[stage], phase ^ 1)) break;
           unsigned char* const sa = base + stage * Cfg::kStageBytes;
           unsigned char* const sb = sa + kTileBytesA;
-          // dw: the group's rows in this step, and how many rows are copied for them
-          const int valid = t.count - s * 64 < 64 ? t.count - s * 64 : 64;
-          const int rows = MODE == FLEXSPMV_GROUPED_DW && t.from + s * 64 + valid < 64 ? (valid + 15) & ~15 : 64;
-          if (rank == 0) mbar_expect_tx(&bars.full[stage], MODE == FLEXSPMV_GROUPED_DW ? PAIR * (2 + pieces) * rows * 128 : bytes);
           const uint32_t bar = PAIR == 2 ? cluster_smem(&bars.full[stage], 0) : smem_u32(&bars.full[stage]);
           if (MODE == FLEXSPMV_GROUPED_DW) {
             // A step's last rows may be the next group's.  The maps count rows by two dimensions of one stride, y + z, and y ends at 64: with the
             // step's last valid row at y = 63, what follows it is out of range and zero.
-            const int place = t.from + s * 64, z = place + valid - 64, n0 = t.n0 + rank * half;
+            const int valid = t.count - s * 64 < 64 ? t.count - s * 64 : 64, place = t.from + s * 64, z = place + valid - 64;
+            const int rows = z >= 0 ? 64 : (valid + 15) & ~15, n0 = t.n0 + rank * half;          // rows: how many are copied
+            if (rank == 0) mbar_expect_tx(&bars.full[stage], PAIR * (2 + pieces) * rows * 128);
             if (z >= 0) {
               tma_3d<PAIR>(sa, &map_a, m0, 64 - valid, z, bar);
               tma_3d<PAIR>(sa + 8192, &map_a, m0 + 64, 64 - valid, z, bar);
@@ -230,12 +246,8 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
               }
             }
           } else {
-            if (MODE == FLEXSPMV_GROUPED_FORWARD) {
-              tma_3d<PAIR>(sa, &map_a, s * 64, m0, t.e, bar);
-            } else {
-              tma_3d<PAIR>(sa, &map_a, m0, s * 64, t.e, bar);
-              tma_3d<PAIR>(sa + 8192, &map_a, m0 + 64, s * 64, t.e, bar);
-            }
+            if (ahead > 0) --ahead;
+            else copy_weights(s, stage);
             for (int g = 0; g < pieces; ++g) tma_2d<PAIR>(sb + g * 4096, &map_b, s * 64, t.from + rank * half + g * 32, bar);
           }
           ++issued;
@@ -251,7 +263,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
       }
     }
     __syncwarp();
-  } else if (warp == 5) {
+  } else if (warp == kMathWarp) {
     if (rank == 0 && elect_one()) {
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
@@ -283,14 +295,15 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
     int acc = 0;
     uint32_t acc_phase = 0;
     TO* const out = static_cast<TO*>(a.out);
-    unsigned char* const mine = store + warp * (Cfg::kStoreBytes / 4);
+    unsigned char* const mine = store + warp * 2048;
+    const int quarter = warp & 3, part = warp >> 2;     // of the accumulator's rows, of its columns
     for (int i = first; i < tiles && !*abort; i += stride) {
       const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
-      const int m = t.m0 + rank * 128 + warp * 32;      // this warp's first row of the accumulator
+      const int m = t.m0 + rank * 128 + quarter * 32;   // this warp's first row of the accumulator
       if (MODE == FLEXSPMV_GROUPED_DW && t.count == 0) {
         constexpr int kW = 16 / (int)sizeof(TO);
         const int pieces = t.cols / kW;
-        for (int x = lane; x < 32 * pieces; x += 32) {
+        for (int x = part * 32 + lane; x < 32 * pieces; x += 64) {
           const int r = m + x / pieces, c = t.n0 + x % pieces * kW;
           if (r < a.n && c < a.k) *reinterpret_cast<uint4*>(out + ((size_t)t.e * a.n + r) * a.k + c) = make_uint4(0, 0, 0, 0);
         }
@@ -298,37 +311,41 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
       }
       if (!wait(&bars.acc_full[acc], acc_phase)) break;
       tmem_fence_after();
-      const uint32_t d = tmem + acc * NT + ((uint32_t)(warp * 32) << 16);
-      for (int c0 = 0; c0 < t.cols; c0 += 32) {
+      const uint32_t d = tmem + acc * NT + ((uint32_t)(quarter * 32) << 16);
+      for (int c0 = part * 32;; c0 += 64) {
         uint32_t v[32];
-        tmem_load32(d + c0, v);
-        if (c0 + 32 >= t.cols) {           // the accumulator is free once the last of it is in registers
+        const bool there = c0 < t.cols, last = c0 + 64 >= t.cols;
+        if (there) tmem_load32(d + c0, v);
+        if (last) {                        // the accumulator is free once this warp's last of it is in registers
           tmem_fence_before();
           __syncwarp();
           if (lane == 0) {
-            if (PAIR == 2) mbar_arrive_cluster(cluster_smem(&bars.acc_empty[acc], 0));
+            if (PAIR == 2) mbar_arrive_cluster_relaxed(cluster_smem(&bars.acc_empty[acc], 0));
             else mbar_arrive(&bars.acc_empty[acc]);
           }
         }
+        if (!there) break;
         if (MODE == FLEXSPMV_GROUPED_DW) {
-          // lane l holds 32 columns of row m + l: through shared memory, so that a row's pieces leave together
-          constexpr int kP = 32 * (int)sizeof(TO) / 16, kW = 16 / (int)sizeof(TO);          // 16-byte pieces of a row
+          // lane l holds 32 columns of row m + l: through shared memory, 64 bytes of a row at a time, so that a row's pieces leave together
+          constexpr int kW = 16 / (int)sizeof(TO), kCols = 4 * kW;          // values of a 16-byte piece, of four
 #pragma unroll
-          for (int p = 0; p < kP; ++p) {
-            Pack<TO, kW> q;
+          for (int h = 0; h < 32; h += kCols) {
 #pragma unroll
-            for (int x = 0; x < kW; ++x) q.set(x, __uint_as_float(v[p * kW + x]));
-            reinterpret_cast<uint4*>(mine)[lane * kP + (p ^ (kP == 8 ? lane & 7 : (lane >> 1) & 3))] = q.raw[0];
+            for (int p = 0; p < 4; ++p) {
+              Pack<TO, kW> q;
+#pragma unroll
+              for (int x = 0; x < kW; ++x) q.set(x, __uint_as_float(v[h + p * kW + x]));
+              reinterpret_cast<uint4*>(mine)[lane * 4 + (p ^ ((lane >> 1) & 3))] = q.raw[0];
+            }
+            __syncwarp();
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int r = x * 8 + (lane >> 2), p = lane & 3, c = t.n0 + c0 + h + p * kW;
+              const uint4 q = reinterpret_cast<const uint4*>(mine)[r * 4 + (p ^ ((r >> 1) & 3))];
+              if (m + r < a.n && c < a.k) *reinterpret_cast<uint4*>(out + ((size_t)t.e * a.n + m + r) * a.k + c) = q;
+            }
+            __syncwarp();
           }
-          __syncwarp();
-#pragma unroll
-          for (int x = 0; x < kP; ++x) {
-            const int at = x * 32 + lane, r = at / kP, p = at % kP;
-            const uint4 q = reinterpret_cast<const uint4*>(mine)[r * kP + (p ^ (kP == 8 ? r & 7 : (r >> 1) & 3))];
-            const int c = t.n0 + c0 + p * kW;
-            if (m + r < a.n && c < a.k) *reinterpret_cast<uint4*>(out + ((size_t)t.e * a.n + m + r) * a.k + c) = q;
-          }
-          __syncwarp();
         } else {
           // lane l holds 32 places of feature m + l: turned in shared memory into rows of 32 features a place
 #pragma unroll
@@ -343,6 +360,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
           }
           __syncwarp();
         }
+        if (last) break;
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
@@ -351,15 +369,16 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
       const long long head = table[0].from, tail = table[a.experts - 1].from + table[a.experts - 1].count, none = head + a.slots - tail;
       for (long long x = blockIdx.x; x < none; x += gridDim.x) {
         uint4* const row = reinterpret_cast<uint4*>(out + (size_t)(x < head ? x : tail + x - head) * width * 8);
-        for (int c = tid; c < width; c += 128) row[c] = make_uint4(0, 0, 0, 0);
+        for (int c = tid; c < width; c += kStoreWarps * 32) row[c] = make_uint4(0, 0, 0, 0);
       }
     }
   }
+  if (a.behind_copy) pdl_wait();           // the launch is not over before the copy is, tiles or none
   tmem_fence_before();
   __syncthreads();
   if (PAIR == 2) cluster_sync();           // neither CTA leaves while the other's instructions may reach its memory
   tmem_fence_after();
-  if (warp == 5) tmem_free<PAIR, Cfg::kTmemCols>(tmem);
+  if (warp == kMathWarp) tmem_free<PAIR, Cfg::kTmemCols>(tmem);
 }
 
 template <class T, class TO, int MODE, int NT, int PAIR>
@@ -413,7 +432,7 @@ static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
 }
 
 // Where there is a list of rows, x's rows in its order in the workspace; `x` and `stride` become the copy's.
-static int take_rows(const flexspmv_expert_desc& d, const void*& x, int64_t& stride, const void* rows, const void* offsets, void* ws, size_t ws_bytes, int* status,
+static int take_rows(const flexspmv_expert_desc& d, const void*& x, int64_t& stride, int& behind_copy, const void* rows, const void* offsets, void* ws, size_t ws_bytes, int* status,
                      cudaStream_t st) {
   if (!rows || d.slots == 0) return 0;
   if (!ws || ws_bytes < (size_t)d.slots * d.k * 2) return FLEXSPMV_ERR_WORKSPACE;
@@ -426,6 +445,7 @@ static int take_rows(const flexspmv_expert_desc& d, const void*& x, int64_t& str
     return e;
   x = ws;
   stride = d.k;
+  behind_copy = pdl_enabled();
   return 0;
 }
 
@@ -435,10 +455,9 @@ static int check_grouped(const flexspmv_expert_desc* d, int which) {
   if (which == FLEXSPMV_GROUPED_DW && d->out_type != FLEXSPMV_TYPE_F32 && d->out_type != d->type) return FLEXSPMV_ERR_BAD_ARG;
   if (d->in_stride < (which == FLEXSPMV_GROUPED_FORWARD ? d->k : d->n) || (which == FLEXSPMV_GROUPED_DW && d->in2_stride < d->k)) return FLEXSPMV_ERR_BAD_ARG;
   if (d->experts > FLEXSPMV_MAX_EXPERTS || d->slots > 0x7fffffffLL || d->tokens > 0x7fffffffLL) return FLEXSPMV_ERR_TOO_LARGE;
-  // tiles and places are counted in 32 bits
-  const long long sides = (long long)((d->n + 127) / 128) * ((d->k + 127) / 128);
-  if (d->slots > 0x7fff0000LL || sides > 0x7fffffffLL / d->experts || (d->slots / 32 + d->experts) > 0x7fffffffLL / ((d->n > d->k ? d->n : d->k) / 128 + 1))
-    return FLEXSPMV_ERR_TOO_LARGE;
+  // places and tiles are counted in 32 bits
+  const double sides = (d->n / 128 + 1.0) * (d->k / 128 + 1.0);
+  if (d->slots > 0x7fff0000LL || sides * (d->slots / 32 + 2.0 * d->experts) > 2e9) return FLEXSPMV_ERR_TOO_LARGE;
   if (d->n % 8 || d->k % 8 || d->in_stride % 8 || (which == FLEXSPMV_GROUPED_DW && d->in2_stride % 8)) return FLEXSPMV_ERR_ALIGN;
   return 0;
 }
@@ -464,8 +483,9 @@ int flexspmv_grouped_matmul(const flexspmv_expert_desc* d, const void* const* in
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const void* x = in[0];
   int64_t stride = d->in_stride;
-  if (int e = flex::take_rows(*d, x, stride, in[3], in[2], ws, ws_bytes, status, st)) return e;
-  flex::GroupedArgs a = {x, in[1], static_cast<const int*>(in[2]), out[0], d->slots, stride, 0, d->experts, d->n, d->k, status};
+  int behind_copy = 0;
+  if (int e = flex::take_rows(*d, x, stride, behind_copy, in[3], in[2], ws, ws_bytes, status, st)) return e;
+  flex::GroupedArgs a = {x, in[1], static_cast<const int*>(in[2]), out[0], d->slots, stride, 0, d->experts, d->n, d->k, status, behind_copy};
   if (d->type == FLEXSPMV_TYPE_BF16) return flex::grouped_launch<__nv_bfloat16, __nv_bfloat16, FLEXSPMV_GROUPED_FORWARD>(a, st);
   return flex::grouped_launch<__half, __half, FLEXSPMV_GROUPED_FORWARD>(a, st);
 }
@@ -477,7 +497,7 @@ int flexspmv_grouped_matmul_dx(const flexspmv_expert_desc* d, const void* const*
   if (d->slots == 0) return 0;
   if (!in[0] || !in[1] || !in[2] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
   if (!flex::aligned16(in[0]) || !flex::aligned16(in[1]) || !flex::aligned16(out[0])) return FLEXSPMV_ERR_ALIGN;
-  flex::GroupedArgs a = {in[0], in[1], static_cast<const int*>(in[2]), out[0], d->slots, d->in_stride, 0, d->experts, d->n, d->k, status};
+  flex::GroupedArgs a = {in[0], in[1], static_cast<const int*>(in[2]), out[0], d->slots, d->in_stride, 0, d->experts, d->n, d->k, status, 0};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (d->type == FLEXSPMV_TYPE_BF16) return flex::grouped_launch<__nv_bfloat16, __nv_bfloat16, FLEXSPMV_GROUPED_DX>(a, st);
   return flex::grouped_launch<__half, __half, FLEXSPMV_GROUPED_DX>(a, st);
@@ -492,8 +512,9 @@ int flexspmv_grouped_matmul_dw(const flexspmv_expert_desc* d, const void* const*
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const void* x = in[1];
   int64_t stride = d->in2_stride;
-  if (int e = flex::take_rows(*d, x, stride, in[3], in[2], ws, ws_bytes, status, st)) return e;
-  flex::GroupedArgs a = {in[0], x, static_cast<const int*>(in[2]), out[0], d->slots, d->in_stride, stride, d->experts, d->n, d->k, status};
+  int behind_copy = 0;
+  if (int e = flex::take_rows(*d, x, stride, behind_copy, in[3], in[2], ws, ws_bytes, status, st)) return e;
+  flex::GroupedArgs a = {in[0], x, static_cast<const int*>(in[2]), out[0], d->slots, d->in_stride, stride, d->experts, d->n, d->k, status, behind_copy};
   const bool wide = d->out_type == FLEXSPMV_TYPE_F32;
   if (d->type == FLEXSPMV_TYPE_BF16)
     return wide ? flex::grouped_launch<__nv_bfloat16, float, FLEXSPMV_GROUPED_DW>(a, st)

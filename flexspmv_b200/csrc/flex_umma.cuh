@@ -25,8 +25,10 @@ __device__ __forceinline__ uint32_t cluster_smem(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// Without ordering of this thread's memory accesses: a release at the cluster's scope waits for all of a warp's stores to global memory (it took
+// half of the time of a launch that stores much).  For a barrier that frees tensor memory whose loads are complete.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // ---- tile copies -----------------------------------------------------------------------------------------------

@@ -164,6 +164,7 @@ def test_route_backward_against_differences():
 GROUPS = [
     ([1], 8, 8), ([3], 128, 64), ([0, 0, 5, 0], 136, 72), ([1, 0, 127, 128, 129, 0, 300, 17, 256, 257], 264, 200),
     ([2, 1, 1, 3, 0, 1, 1, 1], 512, 1024), ([40, 700, 3], 1000, 416), ([16] * 33, 128, 136), ([1100], 256, 64), ([64, 31, 33, 32, 15, 16, 17, 8], 384, 2048),
+    ([5] * 60, 2048, 128), ([300, 20, 0, 500] * 10, 1024, 192),          # many tiles for every CTA, narrow and wide
 ]
 
 
