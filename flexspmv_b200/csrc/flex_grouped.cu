@@ -2,6 +2,7 @@
 //   forward  y[i] = W[e] x[rows[i]]        dx  dx[i] = W[e]^T dy[i]        dw  dW[e] = sum_i dy[i] x[rows[i]]^T
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "flex_common.cuh"
@@ -57,6 +58,8 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict_
 //   dw            128 of n by 256 of k, summed over the expert's places
 // PAIR = 2: two CTAs on two neighbouring SMs take a tile of 256 rows, 128 each; each copies half of the columns' operand for both, which
 // halves what those columns cost the L2 (from 48 KB to 32 KB an SM for 64 of the sum).
+// SPLIT: few tiles.  A cluster of up to eight CTAs takes one tile, each its share of the sum; the parts meet in shared memory, where every CTA
+// adds up some of the columns in the CTAs' order.  No workspace, no atomics.
 // Warps 0-7 store finished accumulators, warp 8 issues the tile copies, warp 9 the matrix instructions; two accumulators in tensor memory,
 // so that one is stored while the next is computed.  The sum goes 64 values (128 bytes of a row) a stage.
 constexpr int kStoreWarps = 8, kCopyWarp = kStoreWarps, kMathWarp = kStoreWarps + 1, kGroupedThreads = (kStoreWarps + 2) * 32;
@@ -128,7 +131,7 @@ __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const Group
   return r;
 }
 
-template <class T, class TO, int MODE, int NT, int PAIR>
+template <class T, class TO, int MODE, int NT, int PAIR, bool SPLIT>
 __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                      const __grid_constant__ CUtensorMap row_a, const __grid_constant__ CUtensorMap row_b,
                                                                      GroupedArgs a) {
@@ -140,6 +143,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
   GroupedTable* const table = reinterpret_cast<GroupedTable*>(&bars + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = PAIR == 2 ? (int)cluster_rank() : 0;
+  const int split = SPLIT ? (int)cluster_size() : 1, share = SPLIT ? (int)cluster_rank() : 0;
   constexpr bool kA_mn = MODE != FLEXSPMV_GROUPED_FORWARD, kB_mn = MODE == FLEXSPMV_GROUPED_DW;
 
   if (tid == 0) {
@@ -181,7 +185,8 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
   tmem_fence_after();
   const uint32_t tmem = bars.tmem;
   const int tiles = MODE == FLEXSPMV_GROUPED_DW ? a.experts * m_tiles * ((a.k + NT - 1) / NT) : table[a.experts].first;
-  const int first = blockIdx.x / PAIR, stride = gridDim.x / PAIR;
+  const int first = blockIdx.x / (PAIR * split);
+  const int stride = SPLIT ? 1 << 30 : gridDim.x / PAIR;      // SPLIT: one tile
   volatile int* const abort = &bars.abort;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -194,6 +199,9 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
   auto steps_of = [&](const GroupedTile& t) {
     return ((MODE == FLEXSPMV_GROUPED_FORWARD ? a.k : MODE == FLEXSPMV_GROUPED_DX ? a.n : t.count) + 63) / 64;
   };
+  // this CTA's steps of a tile
+  auto step_from = [&](int steps) { return SPLIT ? steps * share / split : 0; };
+  auto step_to = [&](int steps) { return SPLIT ? steps * (share + 1) / split : steps; };
 
   if (warp == kCopyWarp) {
     int stage = 0, issued = 0;
@@ -202,7 +210,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
       int ahead = 0;                       // steps whose weights are on their way before x's copy is there
       for (int i = first; i < tiles && !*abort; i += stride) {
         const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
-        const int steps = steps_of(t), half = t.cols / PAIR;
+        const int steps = steps_of(t), from = step_from(steps), to = step_to(steps), half = t.cols / PAIR;
         const int pieces = MODE == FLEXSPMV_GROUPED_DW ? (half + 63) / 64 : (half + 31) / 32;
         const int bytes = PAIR * (kTileBytesA + pieces * 4096);
         const int m0 = t.m0 + rank * 128;
@@ -219,10 +227,10 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
         };
         if (a.behind_copy && i == first) {
           if (MODE != FLEXSPMV_GROUPED_DW)
-            for (; ahead < Cfg::kStages && ahead < steps; ++ahead) copy_weights(ahead, ahead);
+            for (; ahead < Cfg::kStages && from + ahead < to; ++ahead) copy_weights(from + ahead, ahead);
           pdl_wait();
         }
-        for (int s = 0; s < steps; ++s) {
+        for (int s = from; s < to; ++s) {
           if (!wait(&bars.empty[stage], phase ^ 1)) break;
           unsigned char* const sa = base + stage * Cfg::kStageBytes;
           unsigned char* const sb = sa + kTileBytesA;
@@ -269,12 +277,12 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
       uint32_t phase = 0, acc_phase = 0;
       for (int i = first; i < tiles && !*abort; i += stride) {
         const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
-        const int steps = steps_of(t);
-        if (MODE == FLEXSPMV_GROUPED_DW && steps == 0) continue;
+        const int steps = steps_of(t), from = step_from(steps), to = step_to(steps);
+        if (from == to) continue;
         if (!wait(&bars.acc_empty[acc], acc_phase ^ 1)) break;
         tmem_fence_after();
         const uint32_t d = tmem + acc * NT, instr = umma_instr(std::is_same<T, __nv_bfloat16>::value, kA_mn, kB_mn, 128 * PAIR, t.cols);
-        for (int s = 0; s < steps; ++s) {
+        for (int s = from; s < to; ++s) {
           if (!wait(&bars.full[stage], phase)) break;
           tmem_fence_after();
           const uint32_t sa = smem_u32(base + stage * Cfg::kStageBytes), sb = sa + kTileBytesA;
@@ -282,9 +290,9 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
           const uint64_t db = kB_mn ? umma_desc(sb, 8192, 1024) : umma_desc(sb, 16, 1024);
           const int inner = MODE == FLEXSPMV_GROUPED_DW && t.count - s * 64 < 64 ? (t.count - s * 64 + 15) / 16 : 4;
           for (int x = 0; x < inner; ++x)  // the descriptors' addresses are in 16 bytes
-            umma<PAIR>(d, da + x * (kA_mn ? 128 : 2), db + x * (kB_mn ? 128 : 2), instr, (s | x) != 0);
+            umma<PAIR>(d, da + x * (kA_mn ? 128 : 2), db + x * (kB_mn ? 128 : 2), instr, s > from || x > 0);
           umma_commit<PAIR>(&bars.empty[stage]);
-          if (s + 1 == steps) umma_commit<PAIR>(&bars.acc_full[acc]);
+          if (s + 1 == to) umma_commit<PAIR>(&bars.acc_full[acc]);
           if (++stage == Cfg::kStages) { stage = 0; phase ^= 1; }
         }
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
@@ -300,6 +308,21 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
     for (int i = first; i < tiles && !*abort; i += stride) {
       const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
       const int m = t.m0 + rank * 128 + quarter * 32;   // this warp's first row of the accumulator
+      if (SPLIT) {
+        // this CTA's part of the sum, 128 rows a column, over the stages: all that was copied there has been used
+        float* const sums = reinterpret_cast<float*>(base);
+        const int steps = steps_of(t);
+        const bool any = step_from(steps) < step_to(steps);
+        if (any && !wait(&bars.acc_full[0], 0)) break;
+        tmem_fence_after();
+        for (int c0 = part * 32; c0 < t.cols; c0 += 64) {
+          uint32_t v[32];
+          if (any) tmem_load32(tmem + ((uint32_t)(quarter * 32) << 16) + c0, v);
+#pragma unroll
+          for (int x = 0; x < 32; ++x) sums[(c0 + x) * 128 + quarter * 32 + lane] = any ? __uint_as_float(v[x]) : 0.f;
+        }
+        break;
+      }
       if (MODE == FLEXSPMV_GROUPED_DW && t.count == 0) {
         constexpr int kW = 16 / (int)sizeof(TO);
         const int pieces = t.cols / kW;
@@ -373,17 +396,86 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
       }
     }
   }
+  if (SPLIT) {
+    // every CTA stores some of the tile's columns, eight neighbouring rows (dw: columns) at a time
+    cluster_sync();
+    if (first < tiles && !*abort) {
+      const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, first);
+      const int eights = (t.cols + 7) / 8, c_from = eights * share / split * 8, c_to = eights * (share + 1) / split * 8;
+      const uint32_t sums = smem_u32(base);
+      TO* const out = static_cast<TO*>(a.out);
+      constexpr bool kDw = MODE == FLEXSPMV_GROUPED_DW;
+      const int items = (c_to - c_from) * 16;            // of eight values
+      for (int i = tid; i < items; i += kGroupedThreads) {
+        // forward, dx: 16 items a column; dw: 128 items for eight columns
+        const int c = kDw ? c_from + i / 128 * 8 : c_from + i / 16, r = kDw ? i % 128 : i % 16 * 8;
+        float sum[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) sum[x] = 0.f;
+        for (int p = 0; p < split; ++p) {
+          const uint32_t from = cluster_address(sums, p) + (uint32_t)(c * 128 + r) * 4;
+          float v[8];
+          if (kDw) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = cluster_load(from + x * 512);
+          } else {
+            cluster_load4(from, v);
+            cluster_load4(from + 16, v + 4);
+          }
+#pragma unroll
+          for (int x = 0; x < 8; ++x) sum[x] += v[x];
+        }
+        Pack<TO, 8> q;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) q.set(x, sum[x]);
+        if (kDw) {
+          if (t.m0 + r < a.n && t.n0 + c < a.k) q.store(out + ((size_t)t.e * a.n + t.m0 + r) * a.k + t.n0 + c);
+        } else {
+          const int width = MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n;
+          if (c < t.count && t.m0 + r < width) q.store(out + (size_t)(t.from + c) * width + t.m0 + r);
+        }
+      }
+    }
+  }
   if (a.behind_copy) pdl_wait();           // the launch is not over before the copy is, tiles or none
   tmem_fence_before();
   __syncthreads();
-  if (PAIR == 2) cluster_sync();           // neither CTA leaves while the other's instructions may reach its memory
+  if (PAIR == 2 || SPLIT) cluster_sync();  // no CTA leaves while another one's instructions may reach its memory
   tmem_fence_after();
   if (warp == kMathWarp) tmem_free<PAIR, Cfg::kTmemCols>(tmem);
 }
 
-template <class T, class TO, int MODE, int NT, int PAIR>
-static int grouped_launch_as(const GroupedArgs& a, cudaStream_t st) {
+// How many clusters of `ctas` of this kernel a device holds at once; what the runtime says is kept for a kernel, a device and a size.
+template <auto KERNEL>
+static int clusters_at_once(int ctas, int smem) {
+  static std::atomic<int> known[64][4];
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 0;
+  std::atomic<int>& slot = known[device][ctas >= 8 ? 3 : ctas >= 4 ? 2 : ctas >= 2 ? 1 : 0];
+  int n = slot.load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas); cfg.blockDim = dim3(kGroupedThreads); cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ctas; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess || n < 0) { cudaGetLastError(); n = 0; }
+    slot.store(n + 1, std::memory_order_relaxed);
+    return n;
+  }
+  return n - 1;
+}
+
+template <int MODE, int NT, int PAIR>
+static int grouped_smem(int experts) {
   using Cfg = GroupedCfg<MODE, NT, PAIR>;
+  return 1024 + Cfg::kStages * Cfg::kStageBytes + Cfg::kStoreBytes + (int)sizeof(GroupedBars) + (experts + 1) * (int)sizeof(GroupedTable);
+}
+
+// `split`: CTAs that share a tile, `grid` of them altogether; 1: whole tiles.
+template <class T, class TO, int MODE, int NT, int PAIR, bool SPLIT>
+static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStream_t st) {
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   CUtensorMap ma, mb, row_a, row_b;
   if (MODE == FLEXSPMV_GROUPED_DW) {
@@ -407,27 +499,48 @@ static int grouped_launch_as(const GroupedArgs& a, cudaStream_t st) {
     row_a = ma;
     row_b = mb;
   }
-  const int smem = 1024 + Cfg::kStages * Cfg::kStageBytes + Cfg::kStoreBytes + (int)sizeof(GroupedBars) + (a.experts + 1) * (int)sizeof(GroupedTable);
-  constexpr auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR>;
+  const int smem = grouped_smem<MODE, NT, PAIR>(a.experts);
+  constexpr auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR, SPLIT>;
   if (int e = allow_smem<kernel>(smem)) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(device_sm_count() / PAIR * PAIR)); cfg.blockDim = dim3(kGroupedThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(kGroupedThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = PAIR; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[0].val.clusterDim.x = PAIR * split; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr; cfg.numAttrs = pdl_enabled() ? 2 : 1;
   return (int)cudaLaunchKernelEx(&cfg, kernel, ma, mb, row_a, row_b, a);
 }
 
+template <class T, class TO, int MODE, int NT, int PAIR>
+static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
+  const int sms = device_sm_count();
+  // tiles of 128 rows, no more than these whatever the groups are
+  const long long m_tiles = ((MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n) + 127) / 128;
+  const long long most = m_tiles * (MODE == FLEXSPMV_GROUPED_DW ? (long long)a.experts * ((a.k + NT - 1) / NT)
+                                                                : (a.slots < a.experts ? a.slots : a.experts) + a.slots / NT);
+  const long long steps = (MODE == FLEXSPMV_GROUPED_FORWARD ? a.k : MODE == FLEXSPMV_GROUPED_DX ? a.n : a.slots / a.experts) / 64;
+  // What dividing saves is most of a tile's steps, 0.3 us each (a narrow tile's 0.13); what it costs is the parts' meeting, about 5 us (1.5).
+  // us, whole / divided: 8 rows, one expert of 2048 x 4096 17.4 / 9.4; dw of 8192 rows, 1024 x 1024 43.8 / 22; but 4096 rows, two experts of
+  // 512 x 512 (8 steps) 9.8 / 12.6.
+  constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, true>;
+  const int smem = grouped_smem<MODE, NT, 1>(a.experts);
+  for (int split = 8; split > 1; split /= 2) {
+    if (most * split > sms || steps - steps / split < (NT > 64 ? 20 : 12)) continue;
+    if (int e = allow_smem<divided>(smem)) return e;
+    if (most <= clusters_at_once<divided>(split, smem)) return grouped_launch_as<T, TO, MODE, NT, 1, true>(a, (int)most * split, split, st);
+  }
+  return grouped_launch_as<T, TO, MODE, NT, PAIR, false>(a, sms / PAIR * PAIR, 1, st);
+}
+
 template <class T, class TO, int MODE>
 static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
   if constexpr (MODE == FLEXSPMV_GROUPED_DW) {
-    return grouped_launch_as<T, TO, MODE, 256, 2>(a, st);
+    return grouped_tiles<T, TO, MODE, 256, 2>(a, st);
   } else {
-    if (a.slots <= 16ll * a.experts) return grouped_launch_as<T, TO, MODE, 32, 1>(a, st);
-    return grouped_launch_as<T, TO, MODE, 256, 2>(a, st);
+    if (a.slots <= 16ll * a.experts) return grouped_tiles<T, TO, MODE, 32, 1>(a, st);
+    return grouped_tiles<T, TO, MODE, 256, 2>(a, st);
   }
 }
 

@@ -16,14 +16,28 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The address, for the whole cluster, of CTA `rank`'s copy of a shared variable.
-__device__ __forceinline__ uint32_t cluster_smem(const void* p, uint32_t rank) {
+__device__ __forceinline__ uint32_t cluster_address(uint32_t own, uint32_t rank) {
   uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(own), "r"(rank));
   return r;
+}
+__device__ __forceinline__ uint32_t cluster_smem(const void* p, uint32_t rank) { return cluster_address(smem_u32(p), rank); }
+__device__ __forceinline__ float cluster_load(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_load4(uint32_t addr, float* v) {
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr) : "memory");
 }
 // Without ordering of this thread's memory accesses: a release at the cluster's scope waits for all of a warp's stores to global memory (it took
 // half of the time of a launch that stores much).  For a barrier that frees tensor memory whose loads are complete.

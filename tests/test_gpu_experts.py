@@ -165,6 +165,7 @@ GROUPS = [
     ([1], 8, 8), ([3], 128, 64), ([0, 0, 5, 0], 136, 72), ([1, 0, 127, 128, 129, 0, 300, 17, 256, 257], 264, 200),
     ([2, 1, 1, 3, 0, 1, 1, 1], 512, 1024), ([40, 700, 3], 1000, 416), ([16] * 33, 128, 136), ([1100], 256, 64), ([64, 31, 33, 32, 15, 16, 17, 8], 384, 2048),
     ([5] * 60, 2048, 128), ([300, 20, 0, 500] * 10, 1024, 192),          # many tiles for every CTA, narrow and wide
+    ([3, 0, 9], 264, 4096), ([150, 90], 200, 2048), ([2000], 128, 264),          # few tiles and long sums
 ]
 
 
@@ -334,10 +335,10 @@ def test_grouped_empty():
 
 
 def test_grouped_wrong_plans_are_noticed_on_the_device():
-    counts, n, k = [4, 60, 9], 128, 64
+    counts, n, k = [4, 60, 9], 128, 1024
     x, w, offsets, rows, of, take = grouped_case(counts, n, k, torch.bfloat16, True)
     dy = normal(4, (of.numel(), n), torch.bfloat16)
-    for wrong in ([0, 5, 3, 73], [0, 4, 64, 74], [-1, 4, 64, 73], [0, 2 ** 30, 64, 73]):
+    for wrong in ([0, 5, 3, 73], [0, 4, 64, 74], [-1, 4, 64, 73], [0, 2 ** 30, 64, 73], [0, 73, 0, 73]):
         for call in (lambda o: experts.grouped_matmul(x, w, o, rows=rows), lambda o: experts.grouped_matmul_dx(dy, w, o),
                      lambda o: experts.grouped_matmul_dw(dy, x, o, rows=rows)):
             call(torch.tensor(wrong, dtype=torch.int32, device="cuda"))
