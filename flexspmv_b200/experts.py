@@ -68,7 +68,7 @@ class BoundCall:
         else:
             st = self._fn(*self._args, _raw_stream(self._device))
         if st != 0:
-            _check_status(load_library(), st, "launch")
+            _check(st, "launch")
         return self.outputs
 
     __call__ = launch
@@ -80,6 +80,9 @@ _GROUPED = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P, _N, _P, _P)
 _PLAIN = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P)
 _CLIP = ctypes.CFUNCTYPE(_I, ctypes.c_int32, ctypes.c_int32, ctypes.c_float, _P, _P, _N, _P)
 _CLIP_PLAN = ctypes.CFUNCTYPE(_I, ctypes.c_int32, _P, _P, _P, _P, _P, _P, _N, _P)
+_BYTES = ctypes.CFUNCTYPE(_I, _P, _P)
+_GROUPED_BYTES = ctypes.CFUNCTYPE(_I, _P, ctypes.c_int32, _P)
+_FIVE = _P * 5
 _functions: Dict[str, object] = {}
 
 
@@ -88,6 +91,11 @@ def _function(name: str, proto):
     if f is None:
         f = _functions[name] = proto((f"flexspmv_{name}", load_library()))
     return f
+
+
+def _check(status: int, what: str):
+    if status != 0:
+        _check_status(load_library(), status, what)
 
 
 class _Flag:
@@ -131,34 +139,38 @@ def _need(ok: bool, what: str):
 
 def _tensor(t, name: str, dtypes, dim: int, device=None) -> int:
     """Checks a tensor argument; returns its device's index."""
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise FlexSpmvError(f"{name} must be a CUDA tensor")
     if t.dtype not in dtypes or t.dim() != dim:
         raise FlexSpmvError(f"{name} must have {dim} dimension(s) and one of the types {', '.join(str(d) for d in dtypes)}, "
                             f"not {tuple(t.shape)} {t.dtype}")
-    if device is not None and t.device.index != device:
+    if device is not None and t.get_device() != device:
         raise FlexSpmvError(f"{name} is on cuda:{t.device.index}, not cuda:{device}")
-    return t.device.index
+    return t.get_device()
 
 
 def _rows_of(t: torch.Tensor, name: str, aligned: bool = True) -> int:
     """Row stride of a matrix whose rows are contiguous."""
     n, stride = t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    _need((n <= 1 or t.stride(1) == 1) and stride >= n, f"{name}: rows must be contiguous and must not overlap")
+    if not ((n <= 1 or t.stride(1) == 1) and stride >= n):
+        raise FlexSpmvError(f"{name}: rows must be contiguous and must not overlap")
     if aligned:
-        _need(n % 8 == 0 and stride % 8 == 0 and t.data_ptr() % 16 == 0,
-              f"{name}: rows must be multiples of 8 values, apart by multiples of 8, the first on 16 bytes")
+        if not (n % 8 == 0 and stride % 8 == 0 and t.data_ptr() % 16 == 0):
+            raise FlexSpmvError(f"{name}: rows must be multiples of 8 values, apart by multiples of 8, the first on 16 bytes")
     return stride
 
 
 def _whole(t: torch.Tensor, name: str):
-    _need(t.is_contiguous(), f"{name} must be contiguous")
+    if not t.is_contiguous():
+        raise FlexSpmvError(f"{name} must be contiguous")
 
 
 def _out(out, shape, dtype, device, name="out"):
     if out is None:
         return torch.empty(shape, dtype=dtype, device=device)
     _tensor(out, name, (dtype,), len(shape), device.index)
-    _need(tuple(out.shape) == tuple(shape), f"{name} must have the shape {tuple(shape)}, not {tuple(out.shape)}")
+    if not (tuple(out.shape) == tuple(shape)):
+        raise FlexSpmvError(f"{name} must have the shape {tuple(shape)}, not {tuple(out.shape)}")
     _whole(out, name)
     return out
 
@@ -194,27 +206,26 @@ def route(logits: torch.Tensor, k: int, renormalize: bool = False) -> Plan:
     weights of 0 for the rest, a row without any takes no place.  ``renormalize`` divides a row's weights by their sum."""
     dev = _tensor(logits, "logits", tuple(_TYPE), 2)
     tokens, experts = logits.shape
-    _need(1 <= k <= experts, f"k must be 1 to the number of experts, not {k}")
-    _need(experts <= MAX_EXPERTS and k <= MAX_CHOICES, f"at most {MAX_EXPERTS} experts and {MAX_CHOICES} choices")
+    if not (1 <= k <= experts):
+        raise FlexSpmvError(f"k must be 1 to the number of experts, not {k}")
+    if not (experts <= MAX_EXPERTS and k <= MAX_CHOICES):
+        raise FlexSpmvError(f"at most {MAX_EXPERTS} experts and {MAX_CHOICES} choices")
     stride = _rows_of(logits, "logits", aligned=False)
-    d = Desc(tokens=tokens, slots=tokens * k, experts=experts, choices=k, type=_TYPE[logits.dtype], flags=_RENORMALIZE if renormalize else 0,
-             in_stride=stride)
-    lib = load_library()
+    d = Desc(tokens, tokens * k, experts, k, 0, 0, _TYPE[logits.dtype], 0, _RENORMALIZE if renormalize else 0, 0, stride)
     need = ctypes.c_size_t()
-    _check_status(lib, lib.flexspmv_expert_route_bytes(ctypes.byref(d), ctypes.byref(need)), "route")
-    # one allocation: the plan's arrays and the workspace behind one another, each on 16 bytes
+    _check(_function("expert_route_bytes", _BYTES)(ctypes.addressof(d), ctypes.addressof(need)), "route")
+    # one allocation: the plan's arrays behind one another, then the workspace, on 16 bytes
     pairs = tokens * k
-    step, ends = -(-pairs // 4) * 4, -(-(experts + 1) // 4) * 4
-    buf = torch.empty(4 * step + ends + need.value // 4, dtype=torch.int32, device=logits.device)
-    weights = buf[:pairs].view(torch.float32).view(tokens, k)
-    ids, slots = buf[step:step + pairs].view(tokens, k), buf[2 * step:2 * step + pairs].view(tokens, k)
-    rows, offsets = buf[3 * step:3 * step + pairs], buf[4 * step:4 * step + experts + 1]
-    plan = Plan(weights, ids, offsets, rows, slots, bool(renormalize))
+    used = 4 * pairs + experts + 1
+    at = -(-used // 4) * 4
+    buf = torch.empty(at + need.value // 4, dtype=torch.int32, device=logits.device)
+    weights, ids, slots, rows, offsets, _ = buf.split_with_sizes((pairs, pairs, pairs, pairs, experts + 1, at + need.value // 4 - used))
+    plan = Plan(weights.view(torch.float32).view(tokens, k), ids.view(tokens, k), offsets, rows, slots.view(tokens, k), bool(renormalize))
     base = buf.data_ptr()
-    outs = (ctypes.c_void_p * 5)(base, base + 4 * step, base + 16 * step, base + 12 * step, base + 8 * step)
+    outs = _FIVE(base, base + 4 * pairs, base + 16 * pairs, base + 12 * pairs, base + 8 * pairs)
     ins = (ctypes.c_void_p * 1)(logits.data_ptr())
     return BoundCall(_function("expert_route", _WITH_WORKSPACE),
-                     (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), base + 16 * step + 4 * ends, need.value), dev,
+                     (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), base + 4 * at, need.value), dev,
                      (d, ins, outs, logits, buf), plan)
 
 
@@ -233,17 +244,15 @@ def route_backward(dweights: torch.Tensor, logits: torch.Tensor, plan: Plan, out
           "dweights and the plan must be of the logits' rows")
     _whole(dweights, "dweights")
     out = _out(out, (tokens, experts), logits.dtype, logits.device)
-    d = Desc(tokens=tokens, slots=tokens * k, experts=experts, choices=k, type=_TYPE[logits.dtype], flags=_RENORMALIZE if plan.renormalize else 0,
-             in_stride=stride)
+    d = Desc(tokens, tokens * k, experts, k, 0, 0, _TYPE[logits.dtype], 0, _RENORMALIZE if plan.renormalize else 0, 0, stride)
     ins, outs = _pointers((dweights, logits, plan.weights, plan.experts)), _pointers((out,))
     return BoundCall(_function("expert_route_backward", _PLAIN), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs)), dev,
                      (d, ins, outs, dweights, logits, plan, out), out)
 
 
 def _grouped(which: int, name: str, d: Desc, ins, out, offsets, dev: int) -> BoundCall:
-    lib = load_library()
     need = ctypes.c_size_t()
-    _check_status(lib, lib.flexspmv_grouped_matmul_bytes(ctypes.byref(d), which, ctypes.byref(need)), name)
+    _check(_function("grouped_matmul_bytes", _GROUPED_BYTES)(ctypes.addressof(d), which, ctypes.addressof(need)), name)
     need = need if which != _DX and ins[3] is not None else ctypes.c_size_t()          # a copy of x's rows
     ws = torch.empty(need.value, dtype=torch.uint8, device=out.device) if need.value else None
     flag = _flag(dev)
@@ -255,7 +264,8 @@ def _grouped(which: int, name: str, d: Desc, ins, out, offsets, dev: int) -> Bou
 
 def _plan_arrays(offsets, rows, experts: int, dev: int):
     _tensor(offsets, "offsets", (torch.int32,), 1, dev)
-    _need(offsets.numel() == experts + 1, f"offsets must have {experts + 1} entries, not {offsets.numel()}")
+    if not (offsets.numel() == experts + 1):
+        raise FlexSpmvError(f"offsets must have {experts + 1} entries, not {offsets.numel()}")
     _whole(offsets, "offsets")
     if rows is not None:
         _tensor(rows, "rows", (torch.int32,), 1, dev)
@@ -266,9 +276,10 @@ def _weights_of(weight, dtype, dev: int):
     _tensor(weight, "weight", (dtype,), 3, dev)
     _whole(weight, "weight")
     e, n, k = weight.shape
-    _need(1 <= e <= MAX_EXPERTS, f"1 to {MAX_EXPERTS} experts, not {e}")
-    _need(n >= 8 and k >= 8 and n % 8 == 0 and k % 8 == 0 and weight.data_ptr() % 16 == 0,
-          f"weight: both sides of a matrix must be multiples of 8 and the first value on 16 bytes, not {n} x {k}")
+    if not (1 <= e <= MAX_EXPERTS):
+        raise FlexSpmvError(f"1 to {MAX_EXPERTS} experts, not {e}")
+    if not (n >= 8 and k >= 8 and n % 8 == 0 and k % 8 == 0 and weight.data_ptr() % 16 == 0):
+        raise FlexSpmvError(f"weight: both sides of a matrix must be multiples of 8 and the first value on 16 bytes, not {n} x {k}")
     return e, n, k
 
 
@@ -281,12 +292,13 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     places being ``rows.numel()`` or x's rows; sums are in 32 bits, rounded once.  Rows of no expert are zeros."""
     dev = _tensor(x, "x", _HALF, 2)
     e, n, k = _weights_of(weight, x.dtype, dev)
-    _need(x.shape[1] == k, f"x's rows must have {k} values, not {x.shape[1]}")
+    if not (x.shape[1] == k):
+        raise FlexSpmvError(f"x's rows must have {k} values, not {x.shape[1]}")
     _plan_arrays(offsets, rows, e, dev)
     slots = rows.numel() if rows is not None else x.shape[0]
     _need(slots == 0 or x.shape[0] > 0, "x has no rows to take")
     out = _out(out, (slots, n), x.dtype, x.device)
-    d = Desc(tokens=x.shape[0], slots=slots, experts=e, n=n, k=k, type=_TYPE[x.dtype], out_type=_TYPE[x.dtype], in_stride=_rows_of(x, "x"))
+    d = Desc(x.shape[0], slots, e, 0, n, k, _TYPE[x.dtype], _TYPE[x.dtype], 0, 0, _rows_of(x, "x"))
     return _grouped(_FORWARD, "grouped_matmul", d, (x, weight, offsets, rows), out, offsets, dev)
 
 
@@ -296,11 +308,12 @@ def grouped_matmul_dx(dy: torch.Tensor, weight: torch.Tensor, offsets: torch.Ten
     slots)`` adds a token's).  ``dy`` (places, n), its rows may be apart."""
     dev = _tensor(dy, "dy", _HALF, 2)
     e, n, k = _weights_of(weight, dy.dtype, dev)
-    _need(dy.shape[1] == n, f"dy's rows must have {n} values, not {dy.shape[1]}")
+    if not (dy.shape[1] == n):
+        raise FlexSpmvError(f"dy's rows must have {n} values, not {dy.shape[1]}")
     _plan_arrays(offsets, None, e, dev)
     slots = dy.shape[0]
     out = _out(out, (slots, k), dy.dtype, dy.device)
-    d = Desc(tokens=slots, slots=slots, experts=e, n=n, k=k, type=_TYPE[dy.dtype], out_type=_TYPE[dy.dtype], in_stride=_rows_of(dy, "dy"))
+    d = Desc(slots, slots, e, 0, n, k, _TYPE[dy.dtype], _TYPE[dy.dtype], 0, 0, _rows_of(dy, "dy"))
     return _grouped(_DX, "grouped_matmul_dx", d, (dy, weight, offsets), out, offsets, dev)
 
 
@@ -313,24 +326,26 @@ def grouped_matmul_dw(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, 
     _tensor(x, "x", (dy.dtype,), 2, dev)
     _need(isinstance(offsets, torch.Tensor) and offsets.dim() == 1 and offsets.numel() >= 2, "offsets must have an entry for each expert and one more")
     e = offsets.numel() - 1
-    _need(e <= MAX_EXPERTS, f"at most {MAX_EXPERTS} experts")
+    if not (e <= MAX_EXPERTS):
+        raise FlexSpmvError(f"at most {MAX_EXPERTS} experts")
     _plan_arrays(offsets, rows, e, dev)
     slots, n, k = dy.shape[0], dy.shape[1], x.shape[1]
     _need(n >= 8 and k >= 8, "dy and x must have rows of at least 8 values")
     _need((rows.numel() if rows is not None else x.shape[0]) == slots, "dy must have a row for each place")
     _need(slots == 0 or x.shape[0] > 0, "x has no rows to take")
     dtype = dtype or (out.dtype if out is not None else dy.dtype)
-    _need(dtype in (torch.float32, dy.dtype), f"dw is {dy.dtype} or torch.float32, not {dtype}")
+    if not (dtype in (torch.float32, dy.dtype)):
+        raise FlexSpmvError(f"dw is {dy.dtype} or torch.float32, not {dtype}")
     out = _out(out, (e, n, k), dtype, dy.device)
-    d = Desc(tokens=x.shape[0], slots=slots, experts=e, n=n, k=k, type=_TYPE[dy.dtype], out_type=_TYPE[dtype], in_stride=_rows_of(dy, "dy"),
-             in2_stride=_rows_of(x, "x"))
+    d = Desc(x.shape[0], slots, e, 0, n, k, _TYPE[dy.dtype], _TYPE[dtype], 0, 0, _rows_of(dy, "dy"), _rows_of(x, "x"))
     return _grouped(_DW, "grouped_matmul_dw", d, (dy, x, offsets, rows), out, offsets, dev)
 
 
 def _combine_arrays(slots, weights, dev: int):
     _tensor(slots, "slots", (torch.int32,), 2, dev)
     _whole(slots, "slots")
-    _need(1 <= slots.shape[1] <= MAX_CHOICES, f"1 to {MAX_CHOICES} choices, not {slots.shape[1]}")
+    if not (1 <= slots.shape[1] <= MAX_CHOICES):
+        raise FlexSpmvError(f"1 to {MAX_CHOICES} choices, not {slots.shape[1]}")
     if weights is not None:
         _tensor(weights, "weights", (torch.float32,), 2, dev)
         _whole(weights, "weights")
@@ -344,8 +359,7 @@ def combine(z: torch.Tensor, slots: torch.Tensor, weights: Optional[torch.Tensor
     _combine_arrays(slots, weights, dev)
     _need(z.shape[1] >= 1, "z must have columns")
     out = _out(out, (slots.shape[0], z.shape[1]), z.dtype, z.device)
-    d = Desc(tokens=slots.shape[0], slots=z.shape[0], choices=slots.shape[1], n=z.shape[1], type=_TYPE[z.dtype],
-             in_stride=_rows_of(z, "z", aligned=False))
+    d = Desc(slots.shape[0], z.shape[0], 0, slots.shape[1], z.shape[1], 0, _TYPE[z.dtype], 0, 0, 0, _rows_of(z, "z", aligned=False))
     ins = (ctypes.c_void_p * 3)(z.data_ptr(), slots.data_ptr(), weights.data_ptr() if weights is not None else 0)
     outs = _pointers((out,))
     return BoundCall(_function("expert_combine", _PLAIN), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs)), dev,
@@ -364,8 +378,8 @@ def combine_backward(dout: torch.Tensor, z: torch.Tensor, slots: torch.Tensor, w
     _need(offsets.numel() >= 2, "offsets must have an entry for each expert and one more")
     _need(z.shape[1] >= 1 and tuple(dout.shape) == (slots.shape[0], z.shape[1]), "dout must have combine's result's shape")
     dz, dweights = torch.empty(z.shape, dtype=z.dtype, device=z.device), torch.empty(slots.shape, dtype=torch.float32, device=z.device)
-    d = Desc(tokens=slots.shape[0], slots=z.shape[0], experts=offsets.numel() - 1, choices=slots.shape[1], n=z.shape[1], type=_TYPE[z.dtype],
-             in_stride=_rows_of(dout, "dout", aligned=False), in2_stride=_rows_of(z, "z", aligned=False))
+    d = Desc(slots.shape[0], z.shape[0], offsets.numel() - 1, slots.shape[1], z.shape[1], 0, _TYPE[z.dtype], 0, 0, 0,
+             _rows_of(dout, "dout", aligned=False), _rows_of(z, "z", aligned=False))
     ins = (ctypes.c_void_p * 5)(dout.data_ptr(), z.data_ptr(), slots.data_ptr(), weights.data_ptr() if weights is not None else 0, offsets.data_ptr())
     outs = _pointers((dz, dweights))
     return BoundCall(_function("expert_combine_backward", _PLAIN), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs)), dev,
@@ -377,9 +391,11 @@ def _clip(tensors: Sequence[torch.Tensor], max_norm: float, outs) -> BoundCall:
     _need(len(tensors) > 0, "there must be a tensor")
     dev = None
     for i, t in enumerate(tensors):
-        _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _TYPE, f"tensor {i} must be a CUDA tensor of float32, bfloat16 or float16")
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _TYPE):
+            raise FlexSpmvError(f"tensor {i} must be a CUDA tensor of float32, bfloat16 or float16")
         dev = t.device.index if dev is None else dev
-        _need(t.device.index == dev, f"tensor {i} is on cuda:{t.device.index}, not cuda:{dev}")
+        if not (t.device.index == dev):
+            raise FlexSpmvError(f"tensor {i} is on cuda:{t.device.index}, not cuda:{dev}")
         _whole(t, f"tensor {i}")
     n = len(tensors)
     lengths = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
@@ -387,10 +403,11 @@ def _clip(tensors: Sequence[torch.Tensor], max_norm: float, outs) -> BoundCall:
     pin, pout, out_types = _pointers(tensors), None, None
     if outs is not None:
         outs = list(outs)
-        _need(len(outs) == n, f"out must have {n} tensors, not {len(outs)}")
+        if not (len(outs) == n):
+            raise FlexSpmvError(f"out must have {n} tensors, not {len(outs)}")
         for i, (o, t) in enumerate(zip(outs, tensors)):
-            _need(isinstance(o, torch.Tensor) and o.is_cuda and o.dtype in _TYPE and o.device.index == dev and o.shape == t.shape,
-                  f"out {i} must be of its tensor's shape and device, float32, bfloat16 or float16")
+            if not (isinstance(o, torch.Tensor) and o.is_cuda and o.dtype in _TYPE and o.device.index == dev and o.shape == t.shape):
+                raise FlexSpmvError(f"out {i} must be of its tensor's shape and device, float32, bfloat16 or float16")
             _whole(o, f"out {i}")
         pout, out_types = _pointers(outs), (ctypes.c_int32 * n)(*[_TYPE[o.dtype] for o in outs])
     lib = load_library()
@@ -419,5 +436,6 @@ def clip_grad_norm(tensors: Sequence[torch.Tensor], max_norm: float, out: Option
     """Scales the tensors by ``min(1, max_norm / (norm + 1e-6))``, in place or into ``out`` (tensors of the same shapes, of any of the three
     types), and returns the norm before it."""
     tensors = list(tensors)
-    _need(max_norm >= 0, f"max_norm must not be negative or NaN: {max_norm}")
+    if not (max_norm >= 0):
+        raise FlexSpmvError(f"max_norm must not be negative or NaN: {max_norm}")
     return _clip(tensors, max_norm, tensors if out is None else out)
