@@ -336,9 +336,17 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
       tmem_fence_after();
       const uint32_t d = tmem + acc * NT + ((uint32_t)(quarter * 32) << 16);
       for (int c0 = part * 32;; c0 += 64) {
-        uint32_t v[32];
+        uint32_t v[32], low[16], high[16];
         const bool there = c0 < t.cols, last = c0 + 64 >= t.cols;
-        if (there) tmem_load32(d + c0, v);
+        if (there) {
+          if (MODE == FLEXSPMV_GROUPED_DW) {
+            tmem_load32(d + c0, v);
+          } else {
+            tmem_load_blocks(d + c0, low);
+            tmem_load_blocks(d + (16u << 16) + c0, high);
+            tmem_wait_loads();
+          }
+        }
         if (last) {                        // the accumulator is free once this warp's last of it is in registers
           tmem_fence_before();
           __syncwarp();
@@ -370,16 +378,25 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
             __syncwarp();
           }
         } else {
-          // lane l holds 32 places of feature m + l: turned in shared memory into rows of 32 features a place
+          // blocks of 8 features by 8 places, turned on their way into rows of 32 features a place (16-byte pieces, exchanged so that neither
+          // way meets in a bank)
+          if constexpr (sizeof(TO) == 2) {
 #pragma unroll
-          for (int x = 0; x < 32; ++x) reinterpret_cast<TO*>(mine)[x * 32 + lane] = from_float<TO>(__uint_as_float(v[x]));
+            for (int b = 0; b < 4; ++b) {
+              const auto pair = [&](const uint32_t (&w)[16], int i) {
+                return two_of<TO>(__uint_as_float(w[b * 4 + i]), __uint_as_float(w[b * 4 + i + 1]));
+              };
+              const int p = b * 8 + (lane & 7);
+              store_blocks_turned(mine + p * 64 + (((lane >> 3) ^ (p >> 1)) & 3) * 16, pair(low, 0), pair(low, 2), pair(high, 0), pair(high, 2));
+            }
+          }
           __syncwarp();
           const int width = MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n;
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int p = x * 8 + (lane >> 2), c = m + (lane & 3) * 8;
             if (c0 + p < t.count && c < width)
-              *reinterpret_cast<uint4*>(out + (size_t)(t.from + c0 + p) * width + c) = reinterpret_cast<const uint4*>(mine)[p * 4 + (lane & 3)];
+              *reinterpret_cast<uint4*>(out + (size_t)(t.from + c0 + p) * width + c) = reinterpret_cast<const uint4*>(mine)[p * 4 + (((lane & 3) ^ (p >> 1)) & 3)];
           }
           __syncwarp();
         }

@@ -108,6 +108,22 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// 32 columns of 16 lanes from `addr` on: for each 8 columns, lane l gets of row l / 4 the columns 2 (l % 4) and the next one, then the same of
+// row l / 4 + 8.
+__device__ __forceinline__ void tmem_load_blocks(uint32_t addr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+        "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Four 8 x 8 blocks of 16-bit values, two of a row in each lane's register (rows l / 4, columns 2 (l % 4) and the next), stored turned:
+// lane 8 i + j has the address of column j of block i.
+__device__ __forceinline__ void store_blocks_turned(void* row, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(row)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 // ---- matrix instructions ---------------------------------------------------------------------------------------
 // Shared-memory descriptors of operands in rows of 128 bytes with the 128-byte swizzle that the tile copies write.
 //   along the sum (K-major): rows are the tile's rows, 64 values of the inner length each; groups of 8 rows are 1024 bytes apart.
