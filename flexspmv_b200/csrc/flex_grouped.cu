@@ -13,14 +13,15 @@ namespace flex {
 
 int device_sm_count();
 
+enum GroupedMode { kGroupedForward, kGroupedDx, kGroupedDw };
+
 struct GroupedArgs {
   const void *a, *b;             // forward: x, weight; dx: dy, weight; dw: dy, x
-  const int* offsets;
+  const int *offsets, *rows;     // rows: of x, in the places' order; null: place i is x's row i
   void* out;
-  long long slots, a_stride, b_stride;
+  long long tokens, slots, a_stride, b_stride;
   int experts, n, k;
   int* status;
-  int behind_copy;               // launched behind take_rows_kernel, of which nothing but x's copy is waited for
 };
 
 __device__ __forceinline__ void raise(int* status, int code) {
@@ -35,8 +36,7 @@ __device__ __forceinline__ void group_of(const GroupedArgs& a, int e, int& from,
   if (f != from || t != to) raise(a.status, FLEXSPMV_ERR_BAD_CSR);
 }
 
-// The rows of x in the places' order: a copy in the workspace, so that the products' tiles are tiles of a matrix.  (Tile copies that gather four
-// rows each took 72 cycles an instruction here: 2.2 ms for 32 768 rows of 2048 against 4096 columns, 0.51 ms from contiguous rows.)
+// dw with a list of rows: x's rows in the places' order, in the workspace.
 __global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict__ x, const int* __restrict__ rows, const int* __restrict__ offsets, uint4* __restrict__ out,
                                                         long long tokens, long long slots, long long stride, int experts, int pieces, int* status) {
   pdl_wait();
@@ -60,9 +60,15 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict_
 // halves what those columns cost the L2 (from 48 KB to 32 KB an SM for 64 of the sum).
 // SPLIT: few tiles.  A cluster of up to eight CTAs takes one tile, each its share of the sum; the parts meet in shared memory, where every CTA
 // adds up some of the columns in the CTAs' order.  No workspace, no atomics.
+// GATHER (forward): x's rows by a list.  Four more warps copy them, 16 bytes a thread, to where a tile copy would have put them; as fast as contiguous
+// rows up to some thousand rows, 7 % slower for 32 768 of 2048.  (Tile copies that gather four rows each took 72 cycles an instruction: 2.2 ms
+// there instead of 0.43.)  dw's rows are other ones in every step: gathered like this they take 0.57 ms of the 32 768; a copy of them in the
+// workspace and contiguous tile copies 0.44.
 // Warps 0-7 store finished accumulators, warp 8 issues the tile copies, warp 9 the matrix instructions; two accumulators in tensor memory,
 // so that one is stored while the next is computed.  The sum goes 64 values (128 bytes of a row) a stage.
 constexpr int kStoreWarps = 8, kCopyWarp = kStoreWarps, kMathWarp = kStoreWarps + 1, kGroupedThreads = (kStoreWarps + 2) * 32;
+constexpr int kGatherWarps = 4;
+constexpr int grouped_threads(bool gather) { return kGroupedThreads + (gather ? kGatherWarps * 32 : 0); }
 constexpr int kTileBytesA = 128 * 128;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 
@@ -80,7 +86,7 @@ struct GroupedTable {            // of an expert: its first place, its places, i
 };
 
 struct GroupedBars {
-  uint64_t full[9], empty[9], acc_full[2], acc_empty[2];
+  uint64_t full[9], empty[9], gathered[9], acc_full[2], acc_empty[2];
   uint32_t tmem;
   int abort;
 };
@@ -100,10 +106,10 @@ __device__ __forceinline__ int tile_places(int count) {
 template <int MODE, int NT, int PAIR>
 __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const GroupedTable* table, int t) {
   GroupedTile r;
-  const int m = MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n;
+  const int m = MODE == kGroupedDx ? a.k : a.n;
   const int m_tiles = (m + 128 * PAIR - 1) / (128 * PAIR);
   constexpr int kStep = 16 * PAIR;
-  if (MODE == FLEXSPMV_GROUPED_DW) {
+  if (MODE == kGroupedDw) {
     const int n_tiles = (a.k + NT - 1) / NT, each = m_tiles * n_tiles;
     r.e = t / each;
     const int i = t - r.e * each;
@@ -131,11 +137,12 @@ __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const Group
   return r;
 }
 
-template <class T, class TO, int MODE, int NT, int PAIR, bool SPLIT>
-__global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+template <class T, class TO, int MODE, int NT, int PAIR, bool SPLIT, bool GATHER>
+__global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                      const __grid_constant__ CUtensorMap row_a, const __grid_constant__ CUtensorMap row_b,
                                                                      GroupedArgs a) {
   using Cfg = GroupedCfg<MODE, NT, PAIR>;
+  constexpr int kThreads = grouped_threads(GATHER);
   extern __shared__ __align__(1024) unsigned char grouped_sm[];
   unsigned char* const base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(grouped_sm) + 1023) & ~(uintptr_t)1023);
   unsigned char* const store = base + Cfg::kStages * Cfg::kStageBytes;
@@ -144,10 +151,14 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = PAIR == 2 ? (int)cluster_rank() : 0;
   const int split = SPLIT ? (int)cluster_size() : 1, share = SPLIT ? (int)cluster_rank() : 0;
-  constexpr bool kA_mn = MODE != FLEXSPMV_GROUPED_FORWARD, kB_mn = MODE == FLEXSPMV_GROUPED_DW;
+  constexpr bool kA_mn = MODE != kGroupedForward, kB_mn = MODE == kGroupedDw;
 
   if (tid == 0) {
-    for (int i = 0; i < Cfg::kStages; ++i) { mbar_init(&bars.full[i], 1); mbar_init(&bars.empty[i], 1); }
+    for (int i = 0; i < Cfg::kStages; ++i) {
+      mbar_init(&bars.full[i], GATHER && PAIR == 2 ? 2 : 1);          // the copies, and the other CTA's gathered rows
+      mbar_init(&bars.empty[i], 1);
+      mbar_init(&bars.gathered[i], kGatherWarps * 32);
+    }
     for (int i = 0; i < 2; ++i) { mbar_init(&bars.acc_full[i], 1); mbar_init(&bars.acc_empty[i], kStoreWarps * PAIR); }
     bars.abort = 0;
     mbar_fence_init();
@@ -155,15 +166,15 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
     tma_prefetch_map(&map_b);
   }
   if (warp == kMathWarp) tmem_alloc<PAIR, Cfg::kTmemCols>(&bars.tmem);
-  if (!a.behind_copy) pdl_wait();
-  for (int e = tid; e < a.experts; e += kGroupedThreads) {
+  pdl_wait();
+  for (int e = tid; e < a.experts; e += kThreads) {
     int from, to;
     group_of(a, e, from, to);
     table[e].from = from;
     table[e].count = to - from;
   }
   __syncthreads();
-  const int m_tiles = ((MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n) + 128 * PAIR - 1) / (128 * PAIR);
+  const int m_tiles = ((MODE == kGroupedDx ? a.k : a.n) + 128 * PAIR - 1) / (128 * PAIR);
   if (warp == 0) {                         // exclusive sums of the experts' tiles
     int done = 0;
     for (int e0 = 0; e0 <= a.experts; e0 += 32) {
@@ -184,7 +195,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
   if (PAIR == 2) cluster_sync();           // the other CTA's barriers are set up
   tmem_fence_after();
   const uint32_t tmem = bars.tmem;
-  const int tiles = MODE == FLEXSPMV_GROUPED_DW ? a.experts * m_tiles * ((a.k + NT - 1) / NT) : table[a.experts].first;
+  const int tiles = MODE == kGroupedDw ? a.experts * m_tiles * ((a.k + NT - 1) / NT) : table[a.experts].first;
   const int first = blockIdx.x / (PAIR * split);
   const int stride = SPLIT ? 1 << 30 : gridDim.x / PAIR;      // SPLIT: one tile
   volatile int* const abort = &bars.abort;
@@ -196,8 +207,11 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
     raise(a.status, FLEXSPMV_ERR_TIMEOUT);
     return false;
   };
+  // for a whole warp: all of its lanes go on, or none
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+  auto stopped = [&] { return __any_sync(0xffffffffu, *abort) != 0; };
   auto steps_of = [&](const GroupedTile& t) {
-    return ((MODE == FLEXSPMV_GROUPED_FORWARD ? a.k : MODE == FLEXSPMV_GROUPED_DX ? a.n : t.count) + 63) / 64;
+    return ((MODE == kGroupedForward ? a.k : MODE == kGroupedDx ? a.n : t.count) + 63) / 64;
   };
   // this CTA's steps of a tile
   auto step_from = [&](int steps) { return SPLIT ? steps * share / split : 0; };
@@ -207,35 +221,17 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     if (elect_one()) {
-      int ahead = 0;                       // steps whose weights are on their way before x's copy is there
       for (int i = first; i < tiles && !*abort; i += stride) {
         const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
         const int steps = steps_of(t), from = step_from(steps), to = step_to(steps), half = t.cols / PAIR;
-        const int pieces = MODE == FLEXSPMV_GROUPED_DW ? (half + 63) / 64 : (half + 31) / 32;
-        const int bytes = PAIR * (kTileBytesA + pieces * 4096);
+        const int pieces = GATHER ? 0 : MODE == kGroupedDw ? (half + 63) / 64 : (half + 31) / 32;          // of the columns' operand
         const int m0 = t.m0 + rank * 128;
-        auto copy_weights = [&](int s, int to) {
-          unsigned char* const sa = base + to * Cfg::kStageBytes;
-          const uint32_t bar = PAIR == 2 ? cluster_smem(&bars.full[to], 0) : smem_u32(&bars.full[to]);
-          if (rank == 0) mbar_expect_tx(&bars.full[to], bytes);
-          if (MODE == FLEXSPMV_GROUPED_FORWARD) {
-            tma_3d<PAIR>(sa, &map_a, s * 64, m0, t.e, bar);
-          } else {
-            tma_3d<PAIR>(sa, &map_a, m0, s * 64, t.e, bar);
-            tma_3d<PAIR>(sa + 8192, &map_a, m0 + 64, s * 64, t.e, bar);
-          }
-        };
-        if (a.behind_copy && i == first) {
-          if (MODE != FLEXSPMV_GROUPED_DW)
-            for (; ahead < Cfg::kStages && from + ahead < to; ++ahead) copy_weights(from + ahead, ahead);
-          pdl_wait();
-        }
         for (int s = from; s < to; ++s) {
           if (!wait(&bars.empty[stage], phase ^ 1)) break;
           unsigned char* const sa = base + stage * Cfg::kStageBytes;
           unsigned char* const sb = sa + kTileBytesA;
           const uint32_t bar = PAIR == 2 ? cluster_smem(&bars.full[stage], 0) : smem_u32(&bars.full[stage]);
-          if (MODE == FLEXSPMV_GROUPED_DW) {
+          if (MODE == kGroupedDw) {
             // A step's last rows may be the next group's.  The maps count rows by two dimensions of one stride, y + z, and y ends at 64: with the
             // step's last valid row at y = 63, what follows it is out of range and zero.
             const int valid = t.count - s * 64 < 64 ? t.count - s * 64 : 64, place = t.from + s * 64, z = place + valid - 64;
@@ -254,8 +250,13 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
               }
             }
           } else {
-            if (ahead > 0) --ahead;
-            else copy_weights(s, stage);
+            if (rank == 0) mbar_expect_tx(&bars.full[stage], PAIR * (kTileBytesA + pieces * 4096));
+            if (MODE == kGroupedForward) {
+              tma_3d<PAIR>(sa, &map_a, s * 64, m0, t.e, bar);
+            } else {
+              tma_3d<PAIR>(sa, &map_a, m0, s * 64, t.e, bar);
+              tma_3d<PAIR>(sa + 8192, &map_a, m0 + 64, s * 64, t.e, bar);
+            }
             for (int g = 0; g < pieces; ++g) tma_2d<PAIR>(sb + g * 4096, &map_b, s * 64, t.from + rank * half + g * 32, bar);
           }
           ++issued;
@@ -284,11 +285,15 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
         const uint32_t d = tmem + acc * NT, instr = umma_instr(std::is_same<T, __nv_bfloat16>::value, kA_mn, kB_mn, 128 * PAIR, t.cols);
         for (int s = from; s < to; ++s) {
           if (!wait(&bars.full[stage], phase)) break;
+          if (GATHER) {
+            if (!wait(&bars.gathered[stage], phase)) break;
+            fence_proxy_async_smem();      // here, where nothing is under way, for the threads that copied
+          }
           tmem_fence_after();
           const uint32_t sa = smem_u32(base + stage * Cfg::kStageBytes), sb = sa + kTileBytesA;
           const uint64_t da = kA_mn ? umma_desc(sa, 8192, 1024) : umma_desc(sa, 16, 1024);
           const uint64_t db = kB_mn ? umma_desc(sb, 8192, 1024) : umma_desc(sb, 16, 1024);
-          const int inner = MODE == FLEXSPMV_GROUPED_DW && t.count - s * 64 < 64 ? (t.count - s * 64 + 15) / 16 : 4;
+          const int inner = MODE == kGroupedDw && t.count - s * 64 < 64 ? (t.count - s * 64 + 15) / 16 : 4;
           for (int x = 0; x < inner; ++x)  // the descriptors' addresses are in 16 bytes
             umma<PAIR>(d, da + x * (kA_mn ? 128 : 2), db + x * (kB_mn ? 128 : 2), instr, s > from || x > 0);
           umma_commit<PAIR>(&bars.empty[stage]);
@@ -298,14 +303,73 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
     }
+    if (GATHER && rank == 1 && elect_one()) {
+      // Tells the first CTA of rows that are gathered here.  Not the gathering warps themselves: a fence, and an arrival at the cluster's scope,
+      // wait for all that their thread has under way (1.0 to 1.8 us a step).
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int i = first; i < tiles && !*abort; i += stride) {
+        const int steps = steps_of(tile_at<MODE, NT, PAIR>(a, table, i));
+        for (int s = step_from(steps); s < step_to(steps); ++s) {
+          if (!wait(&bars.gathered[stage], phase)) break;
+          fence_proxy_async_smem();
+          mbar_arrive_cluster_shared(cluster_smem(&bars.full[stage], 0));
+          if (++stage == Cfg::kStages) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
     __syncwarp();
+  } else if (GATHER && warp > kMathWarp) {
+    // 8 pieces of 16 bytes a row, 16 rows a pass
+    constexpr int kPasses = NT / PAIR / 16;
+    const int l = tid - kGroupedThreads, piece = l & 7, row0 = l >> 3;
+    const char* const x = static_cast<const char*>(a.a);
+    const long long row_bytes = a.a_stride * 2;
+    const int x_rows = (int)a.tokens, x_columns = a.k;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int i = first; i < tiles && !stopped(); i += stride) {
+      const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
+      const int steps = steps_of(t), from = step_from(steps), to = step_to(steps), half = t.cols / PAIR;
+      int row[kPasses];                    // of x; -1: beyond the group, or not a row of x: zeros
+#pragma unroll
+      for (int j = 0; j < kPasses; ++j) {
+        const int r = row0 + j * 16, p = rank * half + r;
+        row[j] = r < half && p < t.count ? a.rows[t.from + p] : -1;
+      }
+#pragma unroll
+      for (int j = 0; j < kPasses; ++j) {
+        const int r = row0 + j * 16, p = rank * half + r;
+        if ((unsigned)row[j] >= (unsigned)x_rows) {
+          if (r < half && p < t.count) raise(a.status, FLEXSPMV_ERR_BAD_CSR);
+          row[j] = -1;
+        }
+      }
+      for (int s = from; s < to; ++s) {
+        if (!wait_warp(&bars.empty[stage], phase ^ 1)) break;
+        const uint32_t sb = smem_u32(base + stage * Cfg::kStageBytes + kTileBytesA);
+        const int c = s * 64 + piece * 8;
+        const bool inside = c < x_columns;
+        const char* const x_piece = x + c * 2;
+#pragma unroll
+        for (int j = 0; j < kPasses; ++j) {
+          const int r = row0 + j * 16;
+          if (r >= half) continue;
+          const bool copied = inside && row[j] >= 0;
+          copy16(sb + r * 128 + ((piece ^ (r & 7)) << 4), copied ? x_piece + row[j] * row_bytes : x, copied ? 16 : 0);
+        }
+        copy16_arrive(&bars.gathered[stage]);
+        if (++stage == Cfg::kStages) { stage = 0; phase ^= 1; }
+      }
+    }
+    copy16_wait_all();
   } else {
     int acc = 0;
     uint32_t acc_phase = 0;
     TO* const out = static_cast<TO*>(a.out);
     unsigned char* const mine = store + warp * 2048;
     const int quarter = warp & 3, part = warp >> 2;     // of the accumulator's rows, of its columns
-    for (int i = first; i < tiles && !*abort; i += stride) {
+    for (int i = first; i < tiles && !stopped(); i += stride) {
       const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
       const int m = t.m0 + rank * 128 + quarter * 32;   // this warp's first row of the accumulator
       if (SPLIT) {
@@ -313,7 +377,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
         float* const sums = reinterpret_cast<float*>(base);
         const int steps = steps_of(t);
         const bool any = step_from(steps) < step_to(steps);
-        if (any && !wait(&bars.acc_full[0], 0)) break;
+        if (any && !wait_warp(&bars.acc_full[0], 0)) break;
         tmem_fence_after();
         for (int c0 = part * 32; c0 < t.cols; c0 += 64) {
           uint32_t v[32];
@@ -323,7 +387,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
         }
         break;
       }
-      if (MODE == FLEXSPMV_GROUPED_DW && t.count == 0) {
+      if (MODE == kGroupedDw && t.count == 0) {
         constexpr int kW = 16 / (int)sizeof(TO);
         const int pieces = t.cols / kW;
         for (int x = part * 32 + lane; x < 32 * pieces; x += 64) {
@@ -332,14 +396,14 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
         }
         continue;
       }
-      if (!wait(&bars.acc_full[acc], acc_phase)) break;
+      if (!wait_warp(&bars.acc_full[acc], acc_phase)) break;
       tmem_fence_after();
       const uint32_t d = tmem + acc * NT + ((uint32_t)(quarter * 32) << 16);
       for (int c0 = part * 32;; c0 += 64) {
         uint32_t v[32], low[16], high[16];
         const bool there = c0 < t.cols, last = c0 + 64 >= t.cols;
         if (there) {
-          if (MODE == FLEXSPMV_GROUPED_DW) {
+          if (MODE == kGroupedDw) {
             tmem_load32(d + c0, v);
           } else {
             tmem_load_blocks(d + c0, low);
@@ -356,7 +420,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
           }
         }
         if (!there) break;
-        if (MODE == FLEXSPMV_GROUPED_DW) {
+        if (MODE == kGroupedDw) {
           // lane l holds 32 columns of row m + l: through shared memory, 64 bytes of a row at a time, so that a row's pieces leave together
           constexpr int kW = 16 / (int)sizeof(TO), kCols = 4 * kW;          // values of a 16-byte piece, of four
 #pragma unroll
@@ -391,7 +455,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
             }
           }
           __syncwarp();
-          const int width = MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n;
+          const int width = MODE == kGroupedDx ? a.k : a.n;
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int p = x * 8 + (lane >> 2), c = m + (lane & 3) * 8;
@@ -404,8 +468,8 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
-    if (MODE != FLEXSPMV_GROUPED_DW) {     // places of no expert: before the first group and after the last
-      const int width = (MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n) / 8;
+    if (MODE != kGroupedDw) {     // places of no expert: before the first group and after the last
+      const int width = (MODE == kGroupedDx ? a.k : a.n) / 8;
       const long long head = table[0].from, tail = table[a.experts - 1].from + table[a.experts - 1].count, none = head + a.slots - tail;
       for (long long x = blockIdx.x; x < none; x += gridDim.x) {
         uint4* const row = reinterpret_cast<uint4*>(out + (size_t)(x < head ? x : tail + x - head) * width * 8);
@@ -421,9 +485,9 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
       const int eights = (t.cols + 7) / 8, c_from = eights * share / split * 8, c_to = eights * (share + 1) / split * 8;
       const uint32_t sums = smem_u32(base);
       TO* const out = static_cast<TO*>(a.out);
-      constexpr bool kDw = MODE == FLEXSPMV_GROUPED_DW;
+      constexpr bool kDw = MODE == kGroupedDw;
       const int items = (c_to - c_from) * 16;            // of eight values
-      for (int i = tid; i < items; i += kGroupedThreads) {
+      for (int i = tid; i < items; i += kThreads) {
         // forward, dx: 16 items a column; dw: 128 items for eight columns
         const int c = kDw ? c_from + i / 128 * 8 : c_from + i / 16, r = kDw ? i % 128 : i % 16 * 8;
         float sum[8];
@@ -448,13 +512,12 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
         if (kDw) {
           if (t.m0 + r < a.n && t.n0 + c < a.k) q.store(out + ((size_t)t.e * a.n + t.m0 + r) * a.k + t.n0 + c);
         } else {
-          const int width = MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n;
+          const int width = MODE == kGroupedDx ? a.k : a.n;
           if (c < t.count && t.m0 + r < width) q.store(out + (size_t)(t.from + c) * width + t.m0 + r);
         }
       }
     }
   }
-  if (a.behind_copy) pdl_wait();           // the launch is not over before the copy is, tiles or none
   tmem_fence_before();
   __syncthreads();
   if (PAIR == 2 || SPLIT) cluster_sync();  // no CTA leaves while another one's instructions may reach its memory
@@ -463,7 +526,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_kernel(const __gri
 }
 
 // How many clusters of `ctas` of this kernel a device holds at once; what the runtime says is kept for a kernel, a device and a size.
-template <auto KERNEL>
+template <auto KERNEL, int THREADS>
 static int clusters_at_once(int ctas, int smem) {
   static std::atomic<int> known[64][4];
   int device = 0;
@@ -472,7 +535,7 @@ static int clusters_at_once(int ctas, int smem) {
   int n = slot.load(std::memory_order_relaxed);
   if (n == 0) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas); cfg.blockDim = dim3(kGroupedThreads); cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3((unsigned)ctas); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)ctas; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -491,11 +554,11 @@ static int grouped_smem(int experts) {
 }
 
 // `split`: CTAs that share a tile, `grid` of them altogether; 1: whole tiles.
-template <class T, class TO, int MODE, int NT, int PAIR, bool SPLIT>
+template <class T, class TO, int MODE, int NT, int PAIR, bool SPLIT, bool GATHER>
 static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStream_t st) {
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   CUtensorMap ma, mb, row_a, row_b;
-  if (MODE == FLEXSPMV_GROUPED_DW) {
+  if (MODE == kGroupedDw) {
     const uint64_t rows = a.slots ? a.slots : 1;
     const uint64_t da[3] = {(uint64_t)a.n, 64, rows}, sa[2] = {(uint64_t)a.a_stride, (uint64_t)a.a_stride};
     const uint64_t db[3] = {(uint64_t)a.k, 64, rows}, sb[2] = {(uint64_t)a.b_stride, (uint64_t)a.b_stride};
@@ -503,24 +566,26 @@ static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStre
     const uint32_t box[3] = {64, 64, 1}, one[2] = {64, 1};
     const void *pa = a.slots ? a.a : a.out, *pb = a.slots ? a.b : a.out;          // without rows nothing is copied
     if (int e = make_map(&ma, pa, bf16, 3, da, sa, box)) return e;
-    if (int e = make_map(&mb, pb, bf16, 3, db, sb, box)) return e;
     if (int e = make_map(&row_a, pa, bf16, 2, ra, sa, one)) return e;
+    if (int e = make_map(&mb, pb, bf16, 3, db, sb, box)) return e;
     if (int e = make_map(&row_b, pb, bf16, 2, rb, sb, one)) return e;
   } else {
     const uint64_t dw[3] = {(uint64_t)a.k, (uint64_t)a.n, (uint64_t)a.experts}, sw[2] = {(uint64_t)a.k, (uint64_t)a.k * a.n};
     const uint32_t wide[3] = {64, 128, 1}, high[3] = {64, 64, 1};
-    if (int e = make_map(&ma, a.b, bf16, 3, dw, sw, MODE == FLEXSPMV_GROUPED_FORWARD ? wide : high)) return e;
-    const uint64_t dx[2] = {(uint64_t)(MODE == FLEXSPMV_GROUPED_FORWARD ? a.k : a.n), (uint64_t)a.slots}, sx[1] = {(uint64_t)a.a_stride};
+    if (int e = make_map(&ma, a.b, bf16, 3, dw, sw, MODE == kGroupedForward ? wide : high)) return e;
+    const uint64_t dx[2] = {(uint64_t)(MODE == kGroupedForward ? a.k : a.n), (uint64_t)a.slots}, sx[1] = {(uint64_t)a.a_stride};
     const uint32_t box[2] = {64, 32};
-    if (int e = make_map(&mb, a.a, bf16, 2, dx, sx, box)) return e;
+    mb = ma;
+    if (!GATHER)
+      if (int e = make_map(&mb, a.a, bf16, 2, dx, sx, box)) return e;
     row_a = ma;
     row_b = mb;
   }
   const int smem = grouped_smem<MODE, NT, PAIR>(a.experts);
-  constexpr auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR, SPLIT>;
+  constexpr auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR, SPLIT, GATHER>;
   if (int e = allow_smem<kernel>(smem)) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(kGroupedThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3((unsigned)grouped_threads(GATHER)); cfg.dynamicSmemBytes = smem; cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = PAIR * split; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -530,126 +595,108 @@ static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStre
   return (int)cudaLaunchKernelEx(&cfg, kernel, ma, mb, row_a, row_b, a);
 }
 
-template <class T, class TO, int MODE, int NT, int PAIR>
+template <class T, class TO, int MODE, int NT, int PAIR, bool GATHER>
 static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
   const int sms = device_sm_count();
   // tiles of 128 rows, no more than these whatever the groups are
-  const long long m_tiles = ((MODE == FLEXSPMV_GROUPED_DX ? a.k : a.n) + 127) / 128;
-  const long long most = m_tiles * (MODE == FLEXSPMV_GROUPED_DW ? (long long)a.experts * ((a.k + NT - 1) / NT)
+  const long long m_tiles = ((MODE == kGroupedDx ? a.k : a.n) + 127) / 128;
+  const long long most = m_tiles * (MODE == kGroupedDw ? (long long)a.experts * ((a.k + NT - 1) / NT)
                                                                 : (a.slots < a.experts ? a.slots : a.experts) + a.slots / NT);
-  const long long steps = (MODE == FLEXSPMV_GROUPED_FORWARD ? a.k : MODE == FLEXSPMV_GROUPED_DX ? a.n : a.slots / a.experts) / 64;
+  const long long steps = (MODE == kGroupedForward ? a.k : MODE == kGroupedDx ? a.n : a.slots / a.experts) / 64;
   // What dividing saves is most of a tile's steps, 0.3 us each (a narrow tile's 0.13); what it costs is the parts' meeting, about 5 us (1.5).
   // us, whole / divided: 8 rows, one expert of 2048 x 4096 17.4 / 9.4; dw of 8192 rows, 1024 x 1024 43.8 / 22; but 4096 rows, two experts of
   // 512 x 512 (8 steps) 9.8 / 12.6.
-  constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, true>;
+  constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, true, GATHER>;
   const int smem = grouped_smem<MODE, NT, 1>(a.experts);
   for (int split = 8; split > 1; split /= 2) {
     if (most * split > sms || steps - steps / split < (NT > 64 ? 20 : 12)) continue;
     if (int e = allow_smem<divided>(smem)) return e;
-    if (most <= clusters_at_once<divided>(split, smem)) return grouped_launch_as<T, TO, MODE, NT, 1, true>(a, (int)most * split, split, st);
+    if (most <= clusters_at_once<divided, grouped_threads(GATHER)>(split, smem)) return grouped_launch_as<T, TO, MODE, NT, 1, true, GATHER>(a, (int)most * split, split, st);
   }
-  return grouped_launch_as<T, TO, MODE, NT, PAIR, false>(a, sms / PAIR * PAIR, 1, st);
+  return grouped_launch_as<T, TO, MODE, NT, PAIR, false, GATHER>(a, sms / PAIR * PAIR, 1, st);
 }
 
-template <class T, class TO, int MODE>
+template <class T, class TO, int MODE, bool GATHER>
 static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
-  if constexpr (MODE == FLEXSPMV_GROUPED_DW) {
-    return grouped_tiles<T, TO, MODE, 256, 2>(a, st);
+  if constexpr (MODE == kGroupedDw) {
+    return grouped_tiles<T, TO, MODE, 256, 2, GATHER>(a, st);
   } else {
-    if (a.slots <= 16ll * a.experts) return grouped_tiles<T, TO, MODE, 32, 1>(a, st);
-    return grouped_tiles<T, TO, MODE, 256, 2>(a, st);
+    // narrow tiles (32 places) for up to 16 places an expert on average: NARROW0
+    if (a.slots <= 16ll * a.experts) return grouped_tiles<T, TO, MODE, 32, 1, GATHER>(a, st);
+    return grouped_tiles<T, TO, MODE, 256, 2, GATHER>(a, st);
   }
-}
-
-// Where there is a list of rows, x's rows in its order in the workspace; `x` and `stride` become the copy's.
-static int take_rows(const flexspmv_expert_desc& d, const void*& x, int64_t& stride, int& behind_copy, const void* rows, const void* offsets, void* ws, size_t ws_bytes, int* status,
-                     cudaStream_t st) {
-  if (!rows || d.slots == 0) return 0;
-  if (!ws || ws_bytes < (size_t)d.slots * d.k * 2) return FLEXSPMV_ERR_WORKSPACE;
-  if (!aligned16(ws)) return FLEXSPMV_ERR_ALIGN;
-  const int pieces = d.k / 8;
-  const long long ctas = ((long long)d.slots * pieces + 1023) / 1024, most = device_sm_count() * 8ll;
-  if (int e = launch_pdl(take_rows_kernel, (unsigned)(ctas < most ? ctas : most), 256, 0, st, static_cast<const uint4*>(x), static_cast<const int*>(rows),
-                         static_cast<const int*>(offsets), static_cast<uint4*>(ws), (long long)d.tokens, (long long)d.slots, (long long)stride / 8, d.experts,
-                         pieces, status))
-    return e;
-  x = ws;
-  stride = d.k;
-  behind_copy = pdl_enabled();
-  return 0;
 }
 
 static int check_grouped(const flexspmv_expert_desc* d, int which) {
   if (!d || d->tokens < 0 || d->slots < 0 || d->experts < 1 || d->n < 1 || d->k < 1) return FLEXSPMV_ERR_BAD_ARG;
   if (d->type != FLEXSPMV_TYPE_BF16 && d->type != FLEXSPMV_TYPE_F16) return FLEXSPMV_ERR_BAD_ARG;
-  if (which == FLEXSPMV_GROUPED_DW && d->out_type != FLEXSPMV_TYPE_F32 && d->out_type != d->type) return FLEXSPMV_ERR_BAD_ARG;
-  if (d->in_stride < (which == FLEXSPMV_GROUPED_FORWARD ? d->k : d->n) || (which == FLEXSPMV_GROUPED_DW && d->in2_stride < d->k)) return FLEXSPMV_ERR_BAD_ARG;
+  if (which == kGroupedDw && d->out_type != FLEXSPMV_TYPE_F32 && d->out_type != d->type) return FLEXSPMV_ERR_BAD_ARG;
+  if (d->in_stride < (which == kGroupedForward ? d->k : d->n) || (which == kGroupedDw && d->in2_stride < d->k)) return FLEXSPMV_ERR_BAD_ARG;
   if (d->experts > FLEXSPMV_MAX_EXPERTS || d->slots > 0x7fffffffLL || d->tokens > 0x7fffffffLL) return FLEXSPMV_ERR_TOO_LARGE;
   // places and tiles are counted in 32 bits
   const double sides = (d->n / 128 + 1.0) * (d->k / 128 + 1.0);
   if (d->slots > 0x7fff0000LL || sides * (d->slots / 32 + 2.0 * d->experts) > 2e9) return FLEXSPMV_ERR_TOO_LARGE;
-  if (d->n % 8 || d->k % 8 || d->in_stride % 8 || (which == FLEXSPMV_GROUPED_DW && d->in2_stride % 8)) return FLEXSPMV_ERR_ALIGN;
+  if (d->n % 8 || d->k % 8 || d->in_stride % 8 || (which == kGroupedDw && d->in2_stride % 8)) return FLEXSPMV_ERR_ALIGN;
   return 0;
+}
+
+// in: forward x, weight, offsets, rows; dx dy, weight, offsets; dw dy, x, offsets, rows
+template <int MODE>
+static int grouped_call(const flexspmv_expert_desc* d, const void* const* in, void* const* out, void* ws, size_t ws_bytes, int32_t* status, void* stream) {
+  if (int e = check_grouped(d, MODE)) return e;
+  constexpr bool kDw = MODE == kGroupedDw, kDx = MODE == kGroupedDx;
+  if (!in || !out) return FLEXSPMV_ERR_BAD_ARG;
+  if (d->slots == 0 && !kDw) return 0;
+  const int* const rows = kDx ? nullptr : static_cast<const int*>(in[3]);
+  if (!in[2] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
+  if (d->slots && (!in[0] || !in[1] || (!kDx && d->tokens < (rows ? 1 : d->slots)))) return FLEXSPMV_ERR_BAD_ARG;
+  if (!aligned16(in[0]) || !aligned16(in[1]) || !aligned16(out[0])) return FLEXSPMV_ERR_ALIGN;
+  GroupedArgs a = {in[0], in[1], static_cast<const int*>(in[2]), rows, out[0], d->tokens, d->slots, d->in_stride, d->in2_stride, d->experts,
+                   d->n, d->k, status};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (kDw && rows && d->slots) {
+    if (!ws || ws_bytes < (size_t)d->slots * d->k * 2) return FLEXSPMV_ERR_WORKSPACE;
+    if (!aligned16(ws)) return FLEXSPMV_ERR_ALIGN;
+    const int pieces = d->k / 8;
+    const long long ctas = ((long long)d->slots * pieces + 1023) / 1024, most = device_sm_count() * 8ll;
+    if (int e = launch_pdl(take_rows_kernel, (unsigned)(ctas < most ? ctas : most), 256, 0, st, static_cast<const uint4*>(in[1]), rows, a.offsets,
+                           static_cast<uint4*>(ws), (long long)d->tokens, (long long)d->slots, (long long)d->in2_stride / 8, d->experts, pieces, status))
+      return e;
+    a.b = ws;
+    a.b_stride = d->k;
+  }
+  const auto go = [&](auto zero) {
+    using T = decltype(zero);
+    if constexpr (kDw) {
+      return d->out_type == FLEXSPMV_TYPE_F32 ? grouped_launch<T, float, MODE, false>(a, st) : grouped_launch<T, T, MODE, false>(a, st);
+    } else if constexpr (kDx) {
+      return grouped_launch<T, T, MODE, false>(a, st);
+    } else {
+      return rows ? grouped_launch<T, T, MODE, true>(a, st) : grouped_launch<T, T, MODE, false>(a, st);
+    }
+  };
+  return d->type == FLEXSPMV_TYPE_BF16 ? go(__nv_bfloat16()) : go(__half());
 }
 
 }  // namespace flex
 
 extern "C" {
 
-int flexspmv_grouped_matmul_bytes(const flexspmv_expert_desc* d, int32_t which, size_t* bytes) {
-  if (!bytes || which < FLEXSPMV_GROUPED_FORWARD || which > FLEXSPMV_GROUPED_DW) return FLEXSPMV_ERR_BAD_ARG;
-  if (int e = flex::check_grouped(d, which)) return e;
-  *bytes = which == FLEXSPMV_GROUPED_DX ? 0 : (size_t)d->slots * d->k * 2;         // a copy of x's rows; not needed without a list of rows
+int flexspmv_grouped_matmul(const flexspmv_expert_desc* d, const void* const* in, void* const* out, int32_t* status, void* stream) {
+  return flex::grouped_call<flex::kGroupedForward>(d, in, out, nullptr, 0, status, stream);
+}
+int flexspmv_grouped_matmul_dx(const flexspmv_expert_desc* d, const void* const* in, void* const* out, int32_t* status, void* stream) {
+  return flex::grouped_call<flex::kGroupedDx>(d, in, out, nullptr, 0, status, stream);
+}
+int flexspmv_grouped_matmul_dw_bytes(const flexspmv_expert_desc* d, size_t* bytes) {
+  if (!bytes) return FLEXSPMV_ERR_BAD_ARG;
+  if (int e = flex::check_grouped(d, flex::kGroupedDw)) return e;
+  *bytes = (size_t)d->slots * d->k * 2;
   return 0;
 }
-
-int flexspmv_grouped_matmul(const flexspmv_expert_desc* d, const void* const* in, void* const* out, void* ws, size_t ws_bytes, int32_t* status,
-                            void* stream) {
-  if (int e = flex::check_grouped(d, FLEXSPMV_GROUPED_FORWARD)) return e;
-  if (!in || !out) return FLEXSPMV_ERR_BAD_ARG;
-  if (d->slots == 0) return 0;
-  if (!in[0] || !in[1] || !in[2] || !out[0] || d->tokens < (in[3] ? 1 : d->slots)) return FLEXSPMV_ERR_BAD_ARG;
-  if (!flex::aligned16(in[0]) || !flex::aligned16(in[1]) || !flex::aligned16(out[0])) return FLEXSPMV_ERR_ALIGN;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const void* x = in[0];
-  int64_t stride = d->in_stride;
-  int behind_copy = 0;
-  if (int e = flex::take_rows(*d, x, stride, behind_copy, in[3], in[2], ws, ws_bytes, status, st)) return e;
-  flex::GroupedArgs a = {x, in[1], static_cast<const int*>(in[2]), out[0], d->slots, stride, 0, d->experts, d->n, d->k, status, behind_copy};
-  if (d->type == FLEXSPMV_TYPE_BF16) return flex::grouped_launch<__nv_bfloat16, __nv_bfloat16, FLEXSPMV_GROUPED_FORWARD>(a, st);
-  return flex::grouped_launch<__half, __half, FLEXSPMV_GROUPED_FORWARD>(a, st);
-}
-
-int flexspmv_grouped_matmul_dx(const flexspmv_expert_desc* d, const void* const* in, void* const* out, void* ws, size_t ws_bytes, int32_t* status,
-                               void* stream) {
-  if (int e = flex::check_grouped(d, FLEXSPMV_GROUPED_DX)) return e;
-  if (!in || !out) return FLEXSPMV_ERR_BAD_ARG;
-  if (d->slots == 0) return 0;
-  if (!in[0] || !in[1] || !in[2] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
-  if (!flex::aligned16(in[0]) || !flex::aligned16(in[1]) || !flex::aligned16(out[0])) return FLEXSPMV_ERR_ALIGN;
-  flex::GroupedArgs a = {in[0], in[1], static_cast<const int*>(in[2]), out[0], d->slots, d->in_stride, 0, d->experts, d->n, d->k, status, 0};
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (d->type == FLEXSPMV_TYPE_BF16) return flex::grouped_launch<__nv_bfloat16, __nv_bfloat16, FLEXSPMV_GROUPED_DX>(a, st);
-  return flex::grouped_launch<__half, __half, FLEXSPMV_GROUPED_DX>(a, st);
-}
-
 int flexspmv_grouped_matmul_dw(const flexspmv_expert_desc* d, const void* const* in, void* const* out, void* ws, size_t ws_bytes, int32_t* status,
                                void* stream) {
-  if (int e = flex::check_grouped(d, FLEXSPMV_GROUPED_DW)) return e;
-  if (!in || !out || !in[2] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
-  if (d->slots && (!in[0] || !in[1] || d->tokens < (in[3] ? 1 : d->slots))) return FLEXSPMV_ERR_BAD_ARG;
-  if (!flex::aligned16(in[0]) || !flex::aligned16(in[1]) || !flex::aligned16(out[0])) return FLEXSPMV_ERR_ALIGN;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const void* x = in[1];
-  int64_t stride = d->in2_stride;
-  int behind_copy = 0;
-  if (int e = flex::take_rows(*d, x, stride, behind_copy, in[3], in[2], ws, ws_bytes, status, st)) return e;
-  flex::GroupedArgs a = {in[0], x, static_cast<const int*>(in[2]), out[0], d->slots, d->in_stride, stride, d->experts, d->n, d->k, status, behind_copy};
-  const bool wide = d->out_type == FLEXSPMV_TYPE_F32;
-  if (d->type == FLEXSPMV_TYPE_BF16)
-    return wide ? flex::grouped_launch<__nv_bfloat16, float, FLEXSPMV_GROUPED_DW>(a, st)
-                : flex::grouped_launch<__nv_bfloat16, __nv_bfloat16, FLEXSPMV_GROUPED_DW>(a, st);
-  return wide ? flex::grouped_launch<__half, float, FLEXSPMV_GROUPED_DW>(a, st) : flex::grouped_launch<__half, __half, FLEXSPMV_GROUPED_DW>(a, st);
+  return flex::grouped_call<flex::kGroupedDw>(d, in, out, ws, ws_bytes, status, stream);
 }
 
 }  // extern "C"

@@ -39,11 +39,27 @@ __device__ __forceinline__ float cluster_load(uint32_t addr) {
 __device__ __forceinline__ void cluster_load4(uint32_t addr, float* v) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr) : "memory");
 }
+// Orders what this thread knows of its CTA's shared memory before the arrival, and nothing else (an arrival that releases at the cluster's scope
+// waits for all memory accesses).
+__device__ __forceinline__ void mbar_arrive_cluster_shared(uint32_t bar) {
+  asm volatile("fence.release.sync_restrict::shared::cta.cluster;\n\tmbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 // Without ordering of this thread's memory accesses: a release at the cluster's scope waits for all of a warp's stores to global memory (it took
 // half of the time of a launch that stores much).  For a barrier that frees tensor memory whose loads are complete.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+
+// ---- copies of 16 bytes -----------------------------------------------------------------------------------------
+// `bytes`: 16, or 0 for zeros (the source is not read then).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(bytes));
+}
+// The barrier (which counts threads) is arrived on when this thread's copies so far have landed; the thread does not wait.
+__device__ __forceinline__ void copy16_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void copy16_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // ---- tile copies -----------------------------------------------------------------------------------------------
 // `bar`: a cluster address; PAIR = 2: of either CTA of the pair.

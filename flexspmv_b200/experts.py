@@ -31,7 +31,6 @@ MAX_EXPERTS, MAX_CHOICES = 1024, 32          # FLEXSPMV_MAX_EXPERTS, FLEXSPMV_MA
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _HALF = (torch.bfloat16, torch.float16)
 _RENORMALIZE = 1
-_FORWARD, _DX, _DW = 0, 1, 2
 
 
 class Desc(ctypes.Structure):
@@ -76,12 +75,11 @@ class BoundCall:
 
 _P, _I, _N = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
 _WITH_WORKSPACE = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P, _N, _P)
-_GROUPED = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P, _N, _P, _P)
+_GROUPED, _GROUPED_DW = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P, _P), ctypes.CFUNCTYPE(_I, _P, _P, _P, _P, _N, _P, _P)
 _PLAIN = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P)
 _CLIP = ctypes.CFUNCTYPE(_I, ctypes.c_int32, ctypes.c_int32, ctypes.c_float, _P, _P, _N, _P)
 _CLIP_PLAN = ctypes.CFUNCTYPE(_I, ctypes.c_int32, _P, _P, _P, _P, _P, _P, _N, _P)
 _BYTES = ctypes.CFUNCTYPE(_I, _P, _P)
-_GROUPED_BYTES = ctypes.CFUNCTYPE(_I, _P, ctypes.c_int32, _P)
 _FIVE = _P * 5
 _functions: Dict[str, object] = {}
 
@@ -250,16 +248,14 @@ def route_backward(dweights: torch.Tensor, logits: torch.Tensor, plan: Plan, out
                      (d, ins, outs, dweights, logits, plan, out), out)
 
 
-def _grouped(which: int, name: str, d: Desc, ins, out, offsets, dev: int) -> BoundCall:
-    need = ctypes.c_size_t()
-    _check(_function("grouped_matmul_bytes", _GROUPED_BYTES)(ctypes.addressof(d), which, ctypes.addressof(need)), name)
-    need = need if which != _DX and ins[3] is not None else ctypes.c_size_t()          # a copy of x's rows
-    ws = torch.empty(need.value, dtype=torch.uint8, device=out.device) if need.value else None
+def _grouped(name: str, d: Desc, ins, out, dev: int, ws=None) -> BoundCall:
     flag = _flag(dev)
-    pin, pout = (ctypes.c_void_p * len(ins))(*[t.data_ptr() if t is not None else 0 for t in ins]), _pointers((out,))
-    return BoundCall(_function(name, _GROUPED), (ctypes.addressof(d), ctypes.addressof(pin), ctypes.addressof(pout),
-                                                 ws.data_ptr() if ws is not None else 0, need.value, flag.tensor.data_ptr()), dev,
-                     (d, pin, pout, ins, out, ws, flag), out, flag.view)
+    pin, pout = (_P * len(ins))(*[t.data_ptr() if t is not None else 0 for t in ins]), _pointers((out,))
+    args = (ctypes.addressof(d), ctypes.addressof(pin), ctypes.addressof(pout))
+    if ws is not None:
+        args += (ws.data_ptr(), ws.numel())
+    return BoundCall(_function(name, _GROUPED if ws is None else _GROUPED_DW), args + (flag.tensor.data_ptr(),), dev,
+                     (d, pin, pout, ins, out, flag, ws), out, flag.view)
 
 
 def _plan_arrays(offsets, rows, experts: int, dev: int):
@@ -299,7 +295,7 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     _need(slots == 0 or x.shape[0] > 0, "x has no rows to take")
     out = _out(out, (slots, n), x.dtype, x.device)
     d = Desc(x.shape[0], slots, e, 0, n, k, _TYPE[x.dtype], _TYPE[x.dtype], 0, 0, _rows_of(x, "x"))
-    return _grouped(_FORWARD, "grouped_matmul", d, (x, weight, offsets, rows), out, offsets, dev)
+    return _grouped("grouped_matmul", d, (x, weight, offsets, rows), out, dev)
 
 
 @_operator
@@ -314,7 +310,7 @@ def grouped_matmul_dx(dy: torch.Tensor, weight: torch.Tensor, offsets: torch.Ten
     slots = dy.shape[0]
     out = _out(out, (slots, k), dy.dtype, dy.device)
     d = Desc(slots, slots, e, 0, n, k, _TYPE[dy.dtype], _TYPE[dy.dtype], 0, 0, _rows_of(dy, "dy"))
-    return _grouped(_DX, "grouped_matmul_dx", d, (dy, weight, offsets), out, offsets, dev)
+    return _grouped("grouped_matmul_dx", d, (dy, weight, offsets), out, dev)
 
 
 @_operator
@@ -338,7 +334,8 @@ def grouped_matmul_dw(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, 
         raise FlexSpmvError(f"dw is {dy.dtype} or torch.float32, not {dtype}")
     out = _out(out, (e, n, k), dtype, dy.device)
     d = Desc(x.shape[0], slots, e, 0, n, k, _TYPE[dy.dtype], _TYPE[dtype], 0, 0, _rows_of(dy, "dy"), _rows_of(x, "x"))
-    return _grouped(_DW, "grouped_matmul_dw", d, (dy, x, offsets, rows), out, offsets, dev)
+    ws = torch.empty(2 * slots * k if rows is not None else 0, dtype=torch.uint8, device=dy.device)          # a copy of x's rows
+    return _grouped("grouped_matmul_dw", d, (dy, x, offsets, rows), out, dev, ws)
 
 
 def _combine_arrays(slots, weights, dev: int):

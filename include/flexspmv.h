@@ -495,14 +495,12 @@ int flexspmv_expert_route_backward(const flexspmv_expert_desc *desc, const void 
  * n, k and the strides are multiples of 8, the arrays 16-byte aligned (FLEXSPMV_ERR_ALIGN).  Rows of y and dx in no expert's places, and
  * matrices of experts without places, are zeros.  d_status (int32 in device or page-locked memory, may be null): the kernels store
  * FLEXSPMV_ERR_BAD_CSR there where offsets descend or leave [0, slots], or an entry of rows leaves [0, tokens) -- it counts as a row of
- * zeros or any other row; nothing is read or written out of range -- and FLEXSPMV_ERR_TIMEOUT where a bounded wait ran out.
+ * zeros; nothing is read or written out of range -- and FLEXSPMV_ERR_TIMEOUT where a bounded wait ran out.  dw with a list of rows needs a
+ * workspace for a copy of them (_dw_bytes, 16-byte aligned); otherwise it may be null.
  */
-enum { FLEXSPMV_GROUPED_FORWARD = 0, FLEXSPMV_GROUPED_DX = 1, FLEXSPMV_GROUPED_DW = 2 };
-int flexspmv_grouped_matmul_bytes(const flexspmv_expert_desc *desc, int32_t which, size_t *bytes);
-int flexspmv_grouped_matmul(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *d_workspace,
-                            size_t workspace_bytes, int32_t *d_status, void *stream);
-int flexspmv_grouped_matmul_dx(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *d_workspace,
-                               size_t workspace_bytes, int32_t *d_status, void *stream);
+int flexspmv_grouped_matmul(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, int32_t *d_status, void *stream);
+int flexspmv_grouped_matmul_dx(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, int32_t *d_status, void *stream);
+int flexspmv_grouped_matmul_dw_bytes(const flexspmv_expert_desc *desc, size_t *bytes);
 int flexspmv_grouped_matmul_dw(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *d_workspace,
                                size_t workspace_bytes, int32_t *d_status, void *stream);
 
