@@ -71,14 +71,17 @@ constexpr int kGatherWarps = 4;
 constexpr int grouped_threads(bool gather) { return kGroupedThreads + (gather ? kGatherWarps * 32 : 0); }
 constexpr int kTileBytesA = 128 * 128;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
+// The tensor cores cut a sum's low bits at every addition, 2^-24 of it and always towards zero: relative errors of 1e-6 after 1024 rows and 1e-5 after
+// 10 000, lost in a result of 16 bits but not in one of 32.  So that one is added up, correctly rounded, from parts of this many steps (512 rows).
+constexpr int kPartSteps = 8;
 
-template <int MODE, int NT, int PAIR>
+template <int MODE, int NT, int PAIR, int OUT_BYTES>
 struct GroupedCfg {
   static constexpr int kBytesB = NT / PAIR * 128;
   static constexpr int kStageBytes = kTileBytesA + kBytesB;
-  static constexpr int kStages = 196608 / kStageBytes;
+  static constexpr int kStages = (OUT_BYTES == 4 ? 180224 : 196608) / kStageBytes;
   static constexpr int kTmemCols = 2 * NT < 32 ? 32 : 2 * NT;
-  static constexpr int kStoreBytes = kStoreWarps * 2048;
+  static constexpr int kStoreBytes = kStoreWarps * 1024 * OUT_BYTES;        // 32 x 32 results a warp
 };
 
 struct GroupedTable {            // of an expert: its first place, its places, its first tile; and of one past the last: the number of tiles
@@ -140,8 +143,9 @@ __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const Group
 template <class T, class TO, int MODE, int NT, int PAIR, bool SPLIT, bool GATHER>
 __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                      const __grid_constant__ CUtensorMap row_a, const __grid_constant__ CUtensorMap row_b,
+                                                                     const __grid_constant__ CUtensorMap map_out,
                                                                      GroupedArgs a) {
-  using Cfg = GroupedCfg<MODE, NT, PAIR>;
+  using Cfg = GroupedCfg<MODE, NT, PAIR, (int)sizeof(TO)>;
   constexpr int kThreads = grouped_threads(GATHER);
   extern __shared__ __align__(1024) unsigned char grouped_sm[];
   unsigned char* const base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(grouped_sm) + 1023) & ~(uintptr_t)1023);
@@ -152,6 +156,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   const int rank = PAIR == 2 ? (int)cluster_rank() : 0;
   const int split = SPLIT ? (int)cluster_size() : 1, share = SPLIT ? (int)cluster_rank() : 0;
   constexpr bool kA_mn = MODE != kGroupedForward, kB_mn = MODE == kGroupedDw;
+  constexpr bool kInParts = sizeof(TO) == 4;
 
   if (tid == 0) {
     for (int i = 0; i < Cfg::kStages; ++i) {
@@ -164,6 +169,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
     mbar_fence_init();
     tma_prefetch_map(&map_a);
     tma_prefetch_map(&map_b);
+    if (MODE == kGroupedDw) tma_prefetch_map(&map_out);
   }
   if (warp == kMathWarp) tmem_alloc<PAIR, Cfg::kTmemCols>(&bars.tmem);
   pdl_wait();
@@ -280,10 +286,15 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
         const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
         const int steps = steps_of(t), from = step_from(steps), to = step_to(steps);
         if (from == to) continue;
-        if (!wait(&bars.acc_empty[acc], acc_phase ^ 1)) break;
-        tmem_fence_after();
-        const uint32_t d = tmem + acc * NT, instr = umma_instr(std::is_same<T, __nv_bfloat16>::value, kA_mn, kB_mn, 128 * PAIR, t.cols);
+        const uint32_t instr = umma_instr(std::is_same<T, __nv_bfloat16>::value, kA_mn, kB_mn, 128 * PAIR, t.cols);
         for (int s = from; s < to; ++s) {
+          const bool begins = s == from || (kInParts && (s - from) % kPartSteps == 0);
+          const bool ends = s + 1 == to || (kInParts && (s + 1 - from) % kPartSteps == 0);
+          if (begins) {
+            if (!wait(&bars.acc_empty[acc], acc_phase ^ 1)) break;
+            tmem_fence_after();
+          }
+          const uint32_t d = tmem + acc * NT;
           if (!wait(&bars.full[stage], phase)) break;
           if (GATHER) {
             if (!wait(&bars.gathered[stage], phase)) break;
@@ -295,12 +306,14 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           const uint64_t db = kB_mn ? umma_desc(sb, 8192, 1024) : umma_desc(sb, 16, 1024);
           const int inner = MODE == kGroupedDw && t.count - s * 64 < 64 ? (t.count - s * 64 + 15) / 16 : 4;
           for (int x = 0; x < inner; ++x)  // the descriptors' addresses are in 16 bytes
-            umma<PAIR>(d, da + x * (kA_mn ? 128 : 2), db + x * (kB_mn ? 128 : 2), instr, s > from || x > 0);
+            umma<PAIR>(d, da + x * (kA_mn ? 128 : 2), db + x * (kB_mn ? 128 : 2), instr, !begins || x > 0);
           umma_commit<PAIR>(&bars.empty[stage]);
-          if (s + 1 == to) umma_commit<PAIR>(&bars.acc_full[acc]);
+          if (ends) {
+            umma_commit<PAIR>(&bars.acc_full[acc]);
+            if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+          }
           if (++stage == Cfg::kStages) { stage = 0; phase ^= 1; }
         }
-        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
     }
     if (GATHER && rank == 1 && elect_one()) {
@@ -367,16 +380,59 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
     int acc = 0;
     uint32_t acc_phase = 0;
     TO* const out = static_cast<TO*>(a.out);
-    unsigned char* const mine = store + warp * 2048;
+    unsigned char* const mine = store + warp * (Cfg::kStoreBytes / kStoreWarps);
     const int quarter = warp & 3, part = warp >> 2;     // of the accumulator's rows, of its columns
     for (int i = first; i < tiles && !stopped(); i += stride) {
       const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
       const int m = t.m0 + rank * 128 + quarter * 32;   // this warp's first row of the accumulator
+      const int steps = steps_of(t), from = step_from(steps), to = step_to(steps);
+      const auto free_accumulator = [&] {  // once this warp's last of it is in registers
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR == 2) mbar_arrive_cluster_relaxed(cluster_smem(&bars.acc_empty[acc], 0));
+          else mbar_arrive(&bars.acc_empty[acc]);
+        }
+      };
+      // 32-bit results: this warp's four times 32 columns, added up from the parts
+      float sum[kInParts ? NT / 64 : 1][32];
+      if (kInParts) {
+#pragma unroll
+        for (int g = 0; g < NT / 64; ++g)
+#pragma unroll
+          for (int x = 0; x < 32; ++x) sum[kInParts ? g : 0][x] = 0.f;
+        bool there = true;
+        for (int s = from; s < to && there; s += kPartSteps) {
+          there = wait_warp(&bars.acc_full[acc], acc_phase);
+          if (!there) break;
+          tmem_fence_after();
+          const uint32_t d = tmem + acc * NT + ((uint32_t)(quarter * 32) << 16) + part * 32;
+#pragma unroll
+          for (int g = 0; g < NT / 64; ++g)
+            if (part * 32 + g * 64 < t.cols) {
+              uint32_t v[32];
+              tmem_load32(d + g * 64, v);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) sum[kInParts ? g : 0][x] += __uint_as_float(v[x]);
+            }
+          free_accumulator();
+          if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+        }
+        if (!there) break;
+      }
+      if (SPLIT && kInParts) {
+        float* const sums = reinterpret_cast<float*>(base);
+#pragma unroll
+        for (int g = 0; g < NT / 64; ++g)
+          if (part * 32 + g * 64 < t.cols)
+#pragma unroll
+            for (int x = 0; x < 32; ++x) sums[(part * 32 + g * 64 + x) * 128 + quarter * 32 + lane] = sum[kInParts ? g : 0][x];
+        break;
+      }
       if (SPLIT) {
         // this CTA's part of the sum, 128 rows a column, over the stages: all that was copied there has been used
         float* const sums = reinterpret_cast<float*>(base);
-        const int steps = steps_of(t);
-        const bool any = step_from(steps) < step_to(steps);
+        const bool any = from < to;
         if (any && !wait_warp(&bars.acc_full[0], 0)) break;
         tmem_fence_after();
         for (int c0 = part * 32; c0 < t.cols; c0 += 64) {
@@ -396,6 +452,28 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
         }
         continue;
       }
+      // dw: 32 columns from c0 on, of row m + lane, to shared memory and from there as a tile, which leaves out what the matrix does not have
+      const auto store_rows = [&](int c0, const auto& value) {
+        constexpr int kW = 16 / (int)sizeof(TO), kPieces = 32 / kW;         // values of a 16-byte piece, pieces of a row
+        if (lane == 0) tma_stores_read();
+        __syncwarp();
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+          Pack<TO, kW> q;
+#pragma unroll
+          for (int x = 0; x < kW; ++x) q.set(x, value(p * kW + x));
+          reinterpret_cast<uint4*>(mine)[lane * kPieces + (p ^ (kPieces == 8 ? lane & 7 : (lane >> 1) & 3))] = q.raw[0];          // the map's swizzle
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && m < a.n && t.n0 + c0 < a.k) tma_store_3d(&map_out, mine, t.n0 + c0, m, t.e);
+      };
+      if constexpr (kInParts) {
+#pragma unroll
+        for (int g = 0; g < NT / 64; ++g)
+          if (part * 32 + g * 64 < t.cols) store_rows(part * 32 + g * 64, [&](int x) { return sum[g][x]; });
+        continue;
+      }
       if (!wait_warp(&bars.acc_full[acc], acc_phase)) break;
       tmem_fence_after();
       const uint32_t d = tmem + acc * NT + ((uint32_t)(quarter * 32) << 16);
@@ -411,36 +489,10 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
             tmem_wait_loads();
           }
         }
-        if (last) {                        // the accumulator is free once this warp's last of it is in registers
-          tmem_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if (PAIR == 2) mbar_arrive_cluster_relaxed(cluster_smem(&bars.acc_empty[acc], 0));
-            else mbar_arrive(&bars.acc_empty[acc]);
-          }
-        }
+        if (last) free_accumulator();
         if (!there) break;
         if (MODE == kGroupedDw) {
-          // lane l holds 32 columns of row m + l: through shared memory, 64 bytes of a row at a time, so that a row's pieces leave together
-          constexpr int kW = 16 / (int)sizeof(TO), kCols = 4 * kW;          // values of a 16-byte piece, of four
-#pragma unroll
-          for (int h = 0; h < 32; h += kCols) {
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-              Pack<TO, kW> q;
-#pragma unroll
-              for (int x = 0; x < kW; ++x) q.set(x, __uint_as_float(v[h + p * kW + x]));
-              reinterpret_cast<uint4*>(mine)[lane * 4 + (p ^ ((lane >> 1) & 3))] = q.raw[0];
-            }
-            __syncwarp();
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int r = x * 8 + (lane >> 2), p = lane & 3, c = t.n0 + c0 + h + p * kW;
-              const uint4 q = reinterpret_cast<const uint4*>(mine)[r * 4 + (p ^ ((r >> 1) & 3))];
-              if (m + r < a.n && c < a.k) *reinterpret_cast<uint4*>(out + ((size_t)t.e * a.n + m + r) * a.k + c) = q;
-            }
-            __syncwarp();
-          }
+          store_rows(c0, [&](int x) { return __uint_as_float(v[x]); });
         } else {
           // blocks of 8 features by 8 places, turned on their way into rows of 32 features a place (16-byte pieces, exchanged so that neither
           // way meets in a bank)
@@ -468,6 +520,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
+    if (MODE == kGroupedDw && lane == 0) tma_stores_done();
     if (MODE != kGroupedDw) {     // places of no expert: before the first group and after the last
       const int width = (MODE == kGroupedDx ? a.k : a.n) / 8;
       const long long head = table[0].from, tail = table[a.experts - 1].from + table[a.experts - 1].count, none = head + a.slots - tail;
@@ -547,17 +600,17 @@ static int clusters_at_once(int ctas, int smem) {
   return n - 1;
 }
 
-template <int MODE, int NT, int PAIR>
+template <int MODE, int NT, int PAIR, int OUT_BYTES>
 static int grouped_smem(int experts) {
-  using Cfg = GroupedCfg<MODE, NT, PAIR>;
+  using Cfg = GroupedCfg<MODE, NT, PAIR, OUT_BYTES>;
   return 1024 + Cfg::kStages * Cfg::kStageBytes + Cfg::kStoreBytes + (int)sizeof(GroupedBars) + (experts + 1) * (int)sizeof(GroupedTable);
 }
 
 // `split`: CTAs that share a tile, `grid` of them altogether; 1: whole tiles.
 template <class T, class TO, int MODE, int NT, int PAIR, bool SPLIT, bool GATHER>
 static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStream_t st) {
-  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-  CUtensorMap ma, mb, row_a, row_b;
+  constexpr CUtensorMapDataType kIn = std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap ma, mb, row_a, row_b, out;
   if (MODE == kGroupedDw) {
     const uint64_t rows = a.slots ? a.slots : 1;
     const uint64_t da[3] = {(uint64_t)a.n, 64, rows}, sa[2] = {(uint64_t)a.a_stride, (uint64_t)a.a_stride};
@@ -565,23 +618,29 @@ static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStre
     const uint64_t ra[2] = {(uint64_t)a.n, rows}, rb[2] = {(uint64_t)a.k, rows};
     const uint32_t box[3] = {64, 64, 1}, one[2] = {64, 1};
     const void *pa = a.slots ? a.a : a.out, *pb = a.slots ? a.b : a.out;          // without rows nothing is copied
-    if (int e = make_map(&ma, pa, bf16, 3, da, sa, box)) return e;
-    if (int e = make_map(&row_a, pa, bf16, 2, ra, sa, one)) return e;
-    if (int e = make_map(&mb, pb, bf16, 3, db, sb, box)) return e;
-    if (int e = make_map(&row_b, pb, bf16, 2, rb, sb, one)) return e;
+    if (int e = make_map(&ma, pa, kIn, 3, da, sa, box)) return e;
+    if (int e = make_map(&row_a, pa, kIn, 2, ra, sa, one)) return e;
+    if (int e = make_map(&mb, pb, kIn, 3, db, sb, box)) return e;
+    if (int e = make_map(&row_b, pb, kIn, 2, rb, sb, one)) return e;
+    const uint64_t dims[3] = {(uint64_t)a.k, (uint64_t)a.n, (uint64_t)a.experts}, strides[2] = {(uint64_t)a.k, (uint64_t)a.k * a.n};
+    const uint32_t block[3] = {32, 32, 1};
+    constexpr bool kWide = sizeof(TO) == 4;
+    if (int e = make_map(&out, a.out, kWide ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : kIn, 3, dims, strides, block,
+                         kWide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
+      return e;
   } else {
     const uint64_t dw[3] = {(uint64_t)a.k, (uint64_t)a.n, (uint64_t)a.experts}, sw[2] = {(uint64_t)a.k, (uint64_t)a.k * a.n};
     const uint32_t wide[3] = {64, 128, 1}, high[3] = {64, 64, 1};
-    if (int e = make_map(&ma, a.b, bf16, 3, dw, sw, MODE == kGroupedForward ? wide : high)) return e;
+    if (int e = make_map(&ma, a.b, kIn, 3, dw, sw, MODE == kGroupedForward ? wide : high)) return e;
     const uint64_t dx[2] = {(uint64_t)(MODE == kGroupedForward ? a.k : a.n), (uint64_t)a.slots}, sx[1] = {(uint64_t)a.a_stride};
     const uint32_t box[2] = {64, 32};
     mb = ma;
     if (!GATHER)
-      if (int e = make_map(&mb, a.a, bf16, 2, dx, sx, box)) return e;
-    row_a = ma;
+      if (int e = make_map(&mb, a.a, kIn, 2, dx, sx, box)) return e;
+    row_a = out = ma;
     row_b = mb;
   }
-  const int smem = grouped_smem<MODE, NT, PAIR>(a.experts);
+  const int smem = grouped_smem<MODE, NT, PAIR, (int)sizeof(TO)>(a.experts);
   constexpr auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR, SPLIT, GATHER>;
   if (int e = allow_smem<kernel>(smem)) return e;
   cudaLaunchConfig_t cfg = {};
@@ -592,7 +651,7 @@ static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStre
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr; cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, kernel, ma, mb, row_a, row_b, a);
+  return (int)cudaLaunchKernelEx(&cfg, kernel, ma, mb, row_a, row_b, out, a);
 }
 
 template <class T, class TO, int MODE, int NT, int PAIR, bool GATHER>
@@ -607,7 +666,7 @@ static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
   // us, whole / divided: 8 rows, one expert of 2048 x 4096 17.4 / 9.4; dw of 8192 rows, 1024 x 1024 43.8 / 22; but 4096 rows, two experts of
   // 512 x 512 (8 steps) 9.8 / 12.6.
   constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, true, GATHER>;
-  const int smem = grouped_smem<MODE, NT, 1>(a.experts);
+  const int smem = grouped_smem<MODE, NT, 1, (int)sizeof(TO)>(a.experts);
   for (int split = 8; split > 1; split /= 2) {
     if (most * split > sms || steps - steps / split < (NT > 64 ? 20 : 12)) continue;
     if (int e = allow_smem<divided>(smem)) return e;

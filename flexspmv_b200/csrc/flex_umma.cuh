@@ -88,6 +88,15 @@ __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x,
                  "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
 }
+// From shared memory; what lies beyond the tensor is left out.  The source may be written again after tma_stores_read, and is needed till then.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x),
+               "r"(y), "r"(z), "r"(smem_u32(src))
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tma_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -187,7 +196,7 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // ---- host: tensor maps -----------------------------------------------------------------------------------------
-// 16-bit values in rows of 64 (128 bytes, swizzled); dims and box innermost first, strides in values of dims 1...
+// Rows of 128 bytes, swizzled, or of 64; dims and box innermost first, strides in values, of the second dimension on.
 using TensorMapEncode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                      const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 inline TensorMapEncode tensor_map_encode() {
@@ -200,16 +209,16 @@ inline TensorMapEncode tensor_map_encode() {
   }();
   return fn;
 }
-inline int make_map(CUtensorMap* map, const void* base, bool bf16, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+inline int make_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
+                    CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   const TensorMapEncode encode = tensor_map_encode();
   if (!encode) return (int)cudaErrorNotSupported;
   cuuint64_t d[3], s[2];
   cuuint32_t b[3], one[3] = {1, 1, 1};
   for (int i = 0; i < rank; ++i) { d[i] = dims[i]; b[i] = box[i]; }
-  for (int i = 0; i + 1 < rank; ++i) s[i] = strides[i] * 2;
-  const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, one,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  for (int i = 0; i + 1 < rank; ++i) s[i] = strides[i] * (type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2);
+  const CUresult r = encode(map, type, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : FLEXSPMV_ERR_BAD_ARG;
 }
 

@@ -232,6 +232,21 @@ def test_grouped_matmul_dw(counts, n, k, dtype, out_dtype, gather):
         close(dw[e], d.t() @ xe, d.abs().t() @ xe.abs(), max(1, counts[e]))
 
 
+@pytest.mark.parametrize("counts,n,k", [([9001, 513, 512, 40], 264, 328), ([30_000], 128, 256)])
+def test_grouped_matmul_dw_in_32_bits_over_many_rows(counts, n, k):
+    """Parts of 512 rows, each by 32 matrix instructions that cut at most two units of their partial sum, then as many correctly rounded
+    additions as there are parts: 64 * 2^-23 of the magnitude and 2^-24 for each part, whatever the number of rows."""
+    x, _, offsets, _, of, _ = grouped_case(counts, n, k, torch.bfloat16, False)
+    dy = normal(7, (of.numel(), n), torch.bfloat16)
+    dw = experts.grouped_matmul_dw(dy, x, offsets, dtype=torch.float32)
+    for e, c in enumerate(counts):
+        at = torch.nonzero(of == e).view(-1).cuda()
+        d, xe = dy[at].double(), x[at].double()
+        want = d.t() @ xe
+        close(dw[e], want, d.abs().t() @ xe.abs(), 64 + c / 1024)
+        assert float((dw[e].double() - want).norm() / want.norm()) < 1.5e-6
+
+
 @pytest.mark.parametrize("gather", [False, True])
 def test_grouped_rows_of_others_do_not_leak(gather):
     """NaN and infinity in the rows of some experts, and of none, stay there: groups end inside tiles."""
