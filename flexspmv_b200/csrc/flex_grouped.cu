@@ -680,8 +680,9 @@ static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
   if constexpr (MODE == kGroupedDw) {
     return grouped_tiles<T, TO, MODE, 256, 2, GATHER>(a, st);
   } else {
-    // narrow tiles (32 places) for up to 16 places an expert on average: NARROW0
-    if (a.slots <= 16ll * a.experts) return grouped_tiles<T, TO, MODE, 32, 1, GATHER>(a, st);
+    // Tiles of 64 places and single CTAs for up to 32 places an expert on average: more of the weights on their way at once.  us, 64 / 256 places:
+    // 16 an expert, 64 experts of 1408 x 2048 59.8 / 66.8; 32 experts of 2048 x 2048, 32 an expert 47.0 / 49.7, 48 51.0 / 50.5, 128 72.1 / 54.9.
+    if (a.slots <= 32ll * a.experts) return grouped_tiles<T, TO, MODE, 64, 1, GATHER>(a, st);
     return grouped_tiles<T, TO, MODE, 256, 2, GATHER>(a, st);
   }
 }
