@@ -21,6 +21,7 @@ noticed on the device, where nothing is read or written out of range: the next c
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Dict, NamedTuple, Optional, Sequence
 
 import torch
@@ -52,7 +53,8 @@ class Plan(NamedTuple):
 
 class BoundCall:
     """One operator bound to its tensors: ``launch()`` enqueues it on the current stream of their device and returns the outputs, the
-    same tensors every time.  Launches of one object must be ordered with one another: they share outputs and workspace."""
+    same tensors every time.  Launches of one object must be ordered with one another: they share outputs and workspace.  It holds its
+    tensors; like them it must outlive what it has enqueued on streams other than theirs."""
     __slots__ = ("_fn", "_args", "_device", "_keep", "_flag", "outputs")
 
     def __init__(self, fn, args, device, keep, outputs, flag=None):
@@ -73,11 +75,40 @@ class BoundCall:
     __call__ = launch
 
 
+class PlannedCall(BoundCall):
+    """A bound call whose workspace was planned on the stream that was current when it was bound; a first launch on another one waits for that."""
+    __slots__ = ("_planned", "_ordered")
+
+    def __init__(self, *args):
+        super().__init__(*args)
+        self._planned, self._ordered = None, None
+
+    def bound(self):
+        self._planned = torch.cuda.Event()
+        stream = torch.cuda.current_stream(self._device)
+        self._planned.record(stream)
+        self._ordered = {stream.cuda_stream}
+
+    def launch(self):
+        if self._ordered is not None:
+            stream = _raw_stream(self._device)
+            if stream not in self._ordered:
+                if torch.cuda.is_current_stream_capturing():
+                    raise FlexSpmvError("first launch of a bound call on a stream that is being captured: launch it once on that stream before the "
+                                        "capture begins")
+                torch.cuda.current_stream(self._device).wait_event(self._planned)
+                self._ordered.add(stream)
+        return super().launch()
+
+    __call__ = launch
+
+
 _P, _I, _N = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
 _WITH_WORKSPACE = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P, _N, _P)
 _GROUPED, _GROUPED_DW = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P, _P), ctypes.CFUNCTYPE(_I, _P, _P, _P, _P, _N, _P, _P)
 _PLAIN = ctypes.CFUNCTYPE(_I, _P, _P, _P, _P)
 _CLIP = ctypes.CFUNCTYPE(_I, ctypes.c_int32, ctypes.c_int32, ctypes.c_float, _P, _P, _N, _P)
+_CLIP_BYTES = ctypes.CFUNCTYPE(_I, ctypes.c_int32, _P, _P, _P)
 _CLIP_PLAN = ctypes.CFUNCTYPE(_I, ctypes.c_int32, _P, _P, _P, _P, _P, _P, _N, _P)
 _BYTES = ctypes.CFUNCTYPE(_I, _P, _P)
 _FIVE = _P * 5
@@ -193,7 +224,18 @@ def bind(op, *args, **kwargs) -> BoundCall:
     """Checks the arguments of an operator of this module and allocates its outputs and workspace once; the ``BoundCall``'s ``launch()``
     runs it on them as often as wanted."""
     _need(op in _BINDERS, "bind takes an operator of this module")
-    return _BINDERS[op](*args, **kwargs)
+    call = _BINDERS[op](*args, **kwargs)
+    if isinstance(call, PlannedCall):
+        call.bound()
+    return call
+
+
+@functools.lru_cache(maxsize=256)
+def _route_bytes(tokens: int, experts: int) -> int:
+    need = ctypes.c_size_t()
+    d = Desc(tokens, 0, experts)
+    _check(_function("expert_route_bytes", _BYTES)(ctypes.addressof(d), ctypes.addressof(need)), "route")
+    return need.value
 
 
 @_operator
@@ -210,20 +252,19 @@ def route(logits: torch.Tensor, k: int, renormalize: bool = False) -> Plan:
         raise FlexSpmvError(f"at most {MAX_EXPERTS} experts and {MAX_CHOICES} choices")
     stride = _rows_of(logits, "logits", aligned=False)
     d = Desc(tokens, tokens * k, experts, k, 0, 0, _TYPE[logits.dtype], 0, _RENORMALIZE if renormalize else 0, 0, stride)
-    need = ctypes.c_size_t()
-    _check(_function("expert_route_bytes", _BYTES)(ctypes.addressof(d), ctypes.addressof(need)), "route")
+    need = _route_bytes(tokens, experts)
     # one allocation: the plan's arrays behind one another, then the workspace, on 16 bytes
     pairs = tokens * k
     used = 4 * pairs + experts + 1
     at = -(-used // 4) * 4
-    buf = torch.empty(at + need.value // 4, dtype=torch.int32, device=logits.device)
-    weights, ids, slots, rows, offsets, _ = buf.split_with_sizes((pairs, pairs, pairs, pairs, experts + 1, at + need.value // 4 - used))
+    buf = torch.empty(at + need // 4, dtype=torch.int32, device=logits.device)
+    weights, ids, slots, rows, offsets, _ = buf.split_with_sizes((pairs, pairs, pairs, pairs, experts + 1, at + need // 4 - used))
     plan = Plan(weights.view(torch.float32).view(tokens, k), ids.view(tokens, k), offsets, rows, slots.view(tokens, k), bool(renormalize))
     base = buf.data_ptr()
     outs = _FIVE(base, base + 4 * pairs, base + 16 * pairs, base + 12 * pairs, base + 8 * pairs)
     ins = (ctypes.c_void_p * 1)(logits.data_ptr())
     return BoundCall(_function("expert_route", _WITH_WORKSPACE),
-                     (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), base + 4 * at, need.value), dev,
+                     (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), base + 4 * at, need), dev,
                      (d, ins, outs, logits, buf), plan)
 
 
@@ -388,38 +429,38 @@ def _clip(tensors: Sequence[torch.Tensor], max_norm: float, outs) -> BoundCall:
     _need(len(tensors) > 0, "there must be a tensor")
     dev = None
     for i, t in enumerate(tensors):
-        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _TYPE):
-            raise FlexSpmvError(f"tensor {i} must be a CUDA tensor of float32, bfloat16 or float16")
-        dev = t.device.index if dev is None else dev
-        if not (t.device.index == dev):
-            raise FlexSpmvError(f"tensor {i} is on cuda:{t.device.index}, not cuda:{dev}")
-        _whole(t, f"tensor {i}")
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _TYPE and t.is_contiguous()):
+            raise FlexSpmvError(f"tensor {i} must be a contiguous CUDA tensor of float32, bfloat16 or float16")
+        dev = t.get_device() if dev is None else dev
+        if t.get_device() != dev:
+            raise FlexSpmvError(f"tensor {i} is on cuda:{t.get_device()}, not cuda:{dev}")
     n = len(tensors)
     lengths = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
     types = (ctypes.c_int32 * n)(*[_TYPE[t.dtype] for t in tensors])
     pin, pout, out_types = _pointers(tensors), None, None
     if outs is not None:
         outs = list(outs)
-        if not (len(outs) == n):
+        if len(outs) != n:
             raise FlexSpmvError(f"out must have {n} tensors, not {len(outs)}")
         for i, (o, t) in enumerate(zip(outs, tensors)):
-            if not (isinstance(o, torch.Tensor) and o.is_cuda and o.dtype in _TYPE and o.device.index == dev and o.shape == t.shape):
-                raise FlexSpmvError(f"out {i} must be of its tensor's shape and device, float32, bfloat16 or float16")
-            _whole(o, f"out {i}")
+            if o is not t and not (isinstance(o, torch.Tensor) and o.is_cuda and o.dtype in _TYPE and o.get_device() == dev and o.shape == t.shape and
+                                   o.is_contiguous()):
+                raise FlexSpmvError(f"out {i} must be contiguous, of its tensor's shape and device, float32, bfloat16 or float16")
         pout, out_types = _pointers(outs), (ctypes.c_int32 * n)(*[_TYPE[o.dtype] for o in outs])
-    lib = load_library()
     need, pieces = ctypes.c_size_t(), ctypes.c_int32()
-    _check_status(lib, lib.flexspmv_clip_gradients_bytes(n, lengths, ctypes.byref(need), ctypes.byref(pieces)), "clip_gradients")
+    _check(_function("clip_gradients_bytes", _CLIP_BYTES)(n, ctypes.addressof(lengths), ctypes.addressof(need), ctypes.addressof(pieces)), "clip_gradients")
     ws = torch.empty(need.value // 8, dtype=torch.float64, device=tensors[0].device)
     norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
-    with torch.cuda.device(dev):
-        st = _function("clip_gradients_plan", _CLIP_PLAN)(n, ctypes.addressof(pin), ctypes.addressof(types), ctypes.addressof(lengths),
-                                                          ctypes.addressof(pout) if pout is not None else None,
-                                                          ctypes.addressof(out_types) if out_types is not None else None, ws.data_ptr(), need.value,
-                                                          _raw_stream(dev))
-    _check_status(lib, st, "clip_gradients_plan")
+    plan = (n, ctypes.addressof(pin), ctypes.addressof(types), ctypes.addressof(lengths), ctypes.addressof(pout) if pout is not None else None,
+            ctypes.addressof(out_types) if out_types is not None else None, ws.data_ptr(), need.value, _raw_stream(dev))
+    if _current_device() == dev:
+        st = _function("clip_gradients_plan", _CLIP_PLAN)(*plan)
+    else:
+        with torch.cuda.device(dev):
+            st = _function("clip_gradients_plan", _CLIP_PLAN)(*plan)
+    _check(st, "clip_gradients_plan")
     args = (pieces.value, outs is not None, float(max_norm), norm.data_ptr(), ws.data_ptr(), need.value)
-    return BoundCall(_function("clip_gradients", _CLIP), args, dev, (ws, tensors, outs), norm)
+    return PlannedCall(_function("clip_gradients", _CLIP), args, dev, (ws, tensors, outs), norm)
 
 
 @_operator

@@ -513,6 +513,27 @@ def test_bound_clip_follows_its_tensors():
         assert all(torch.allclose(o, t.float() * min(1.0, 1.0 / (exact + 1e-6)), rtol=1e-4) for o, t in zip(outs, ts))
 
 
+def test_bound_calls_on_another_stream():
+    """Bound on one stream and launched on another at once: the plan comes first."""
+    ts = tensors_of([300_000, 17], [torch.bfloat16])
+    exact = math.sqrt(sum(float((t.double() ** 2).sum()) for t in ts))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        torch.cuda._sleep(1_000_000)                            # the binding stream is busy before the plan
+        call = experts.bind(experts.grad_norm, ts)
+        with torch.cuda.stream(side):
+            norm = call.launch().clone()
+        side.synchronize()
+        assert abs(float(norm) - exact) <= 1e-4 * exact
+        torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    call = experts.bind(experts.grad_norm, ts)
+    with pytest.raises(FlexSpmvError, match="captured"):
+        with torch.cuda.graph(graph):
+            call.launch()
+
+
 # ---- refusals ----------------------------------------------------------------------------------------------------
 
 def test_refusals():
