@@ -534,6 +534,48 @@ def test_bound_calls_on_another_stream():
             call.launch()
 
 
+# ---- beyond 32 bits ----------------------------------------------------------------------------------------------
+
+def test_arrays_of_more_than_2_to_the_32_values():
+    """600 000 rows of 8192: the last group's rows lie beyond 2^32 values, in every operand that can be so long."""
+    counts, n, k = [1000, 598_800, 200], 8192, 64
+    slots = sum(counts)
+    x, w = normal(1, (slots, k), torch.bfloat16), normal(2, (3, n, k), torch.bfloat16, 0.125)
+    offsets = offsets_of(counts)
+    y = experts.grouped_matmul(x, w, offsets)
+    last = slice(slots - 200, slots)
+    xe, we = x[last].double(), w[2].double()
+    close(y[last], xe @ we.t(), xe.abs() @ we.abs().t(), k)
+    xm = x[550_000:550_100].double()
+    close(y[550_000:550_100], xm @ w[1].double().t(), xm.abs() @ w[1].double().abs().t(), k)
+    dx = experts.grouped_matmul_dx(y, w, offsets)
+    d = y[last].double()
+    close(dx[last], d @ we, d.abs() @ we.abs(), n)
+    dw = experts.grouped_matmul_dw(y, x, offsets, dtype=torch.float32)
+    close(dw[2], d.t() @ xe, d.abs().t() @ xe.abs(), 200)
+    rows = torch.arange(slots - 200, slots, device="cuda", dtype=torch.int32)          # taken from the far end of a long x
+    dw = experts.grouped_matmul_dw(xe.to(torch.bfloat16), y, offsets_of([200]), rows=rows, dtype=torch.float32)
+    close(dw[0], xe.t() @ d, xe.abs().t() @ d.abs(), 200)
+    w2 = normal(3, (1, 64, n), torch.bfloat16, n ** -0.5)
+    close(experts.grouped_matmul(y, w2, offsets_of([200]), rows=rows), d @ w2[0].double().t(), d.abs() @ w2[0].double().abs().t(), n)
+    slots2 = torch.arange(slots, device="cuda", dtype=torch.int32).view(-1, 2)
+    weights = torch.rand(slots2.shape, generator=gen(4), device="cuda")
+    out = experts.combine(y, slots2, weights)
+    picked = y[last].double().view(100, 2, n)
+    close(out[-100:], torch.einsum("tk,tkh->th", weights[-100:].double(), picked), torch.einsum("tk,tkh->th", weights[-100:].double(), picked.abs()), 3)
+    dz, dweights = experts.combine_backward(out, y, slots2, weights, offsets)
+    want = (weights[-100:].double()[..., None] * out[-100:].double()[:, None, :]).reshape(200, n)
+    close(dz[last], want, want.abs(), 1)
+    close(dweights[-100:], torch.einsum("th,tkh->tk", out[-100:].double(), picked), torch.einsum("th,tkh->tk", out[-100:].double().abs(), picked.abs()), n)
+    experts.check()
+    long = y.view(-1)[: (1 << 32) + 12_345]
+    long.fill_(0.5)
+    norm = experts.clip_grad_norm([long], 1.0)
+    assert abs(float(norm) - 0.5 * math.sqrt(long.numel())) <= 1e-5 * float(norm)
+    scaled = (torch.tensor(0.5) * (1.0 / (norm.cpu() + 1e-6))).to(torch.bfloat16)
+    assert float(long[-1]) == float(scaled) and float(long[0]) == float(scaled) and float(y.view(-1)[long.numel()]) != float(scaled)
+
+
 # ---- refusals ----------------------------------------------------------------------------------------------------
 
 def test_refusals():
