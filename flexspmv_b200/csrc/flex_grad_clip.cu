@@ -26,7 +26,7 @@ struct ClipPiece {
 };
 
 // The tensors of one planning launch travel in its parameters.
-constexpr int kPlanTensors = 128;
+constexpr int kPlanTensors = 256;
 struct ClipTensors {
   const void* in[kPlanTensors];
   void* out[kPlanTensors];

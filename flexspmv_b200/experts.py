@@ -20,8 +20,10 @@ noticed on the device, where nothing is read or written out of range: the next c
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
+import operator
 from typing import Dict, NamedTuple, Optional, Sequence
 
 import torch
@@ -424,35 +426,50 @@ def combine_backward(dout: torch.Tensor, z: torch.Tensor, slots: torch.Tensor, w
                      (d, ins, outs, dout, z, slots, weights, offsets, dz, dweights), (dz, dweights))
 
 
-def _clip(tensors: Sequence[torch.Tensor], max_norm: float, outs) -> BoundCall:
-    tensors = list(tensors)
+_get_device, _numel, _is_contiguous, _data_ptr = torch.Tensor.get_device, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+_dtype_of = operator.attrgetter("dtype")
+
+
+def _at(values: array.array) -> int:
+    return values.buffer_info()[0]
+
+
+def _list_of(tensors, name: str):
+    """Checks a list of tensors; returns their device, types, lengths and addresses.  Several hundred of them are usual, so each question is one
+    loop inside the interpreter."""
+    try:
+        devices, types = set(map(_get_device, tensors)), list(map(_TYPE.get, map(_dtype_of, tensors)))
+        good = len(devices) == 1 and None not in types and all(map(_is_contiguous, tensors))
+    except (TypeError, AttributeError):
+        good, devices = False, ()
+    dev = next(iter(devices), -1)
+    if not good or dev < 0:
+        raise FlexSpmvError(f"{name} must be contiguous CUDA tensors of float32, bfloat16 or float16 on one device")
+    return dev, types, list(map(_numel, tensors)), list(map(_data_ptr, tensors))
+
+
+def _clip(tensors: list, max_norm: float, outs) -> BoundCall:
     _need(len(tensors) > 0, "there must be a tensor")
-    dev = None
-    for i, t in enumerate(tensors):
-        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _TYPE and t.is_contiguous()):
-            raise FlexSpmvError(f"tensor {i} must be a contiguous CUDA tensor of float32, bfloat16 or float16")
-        dev = t.get_device() if dev is None else dev
-        if t.get_device() != dev:
-            raise FlexSpmvError(f"tensor {i} is on cuda:{t.get_device()}, not cuda:{dev}")
     n = len(tensors)
-    lengths = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
-    types = (ctypes.c_int32 * n)(*[_TYPE[t.dtype] for t in tensors])
-    pin, pout, out_types = _pointers(tensors), None, None
-    if outs is not None:
+    dev, type_list, length_list, addresses = _list_of(tensors, "the tensors")
+    lengths, types, pin = array.array("q", length_list), array.array("i", type_list), array.array("Q", addresses)
+    pout, out_types = None, None
+    if outs is tensors:
+        pout, out_types = pin, types
+    elif outs is not None:
         outs = list(outs)
         if len(outs) != n:
             raise FlexSpmvError(f"out must have {n} tensors, not {len(outs)}")
-        for i, (o, t) in enumerate(zip(outs, tensors)):
-            if o is not t and not (isinstance(o, torch.Tensor) and o.is_cuda and o.dtype in _TYPE and o.get_device() == dev and o.shape == t.shape and
-                                   o.is_contiguous()):
-                raise FlexSpmvError(f"out {i} must be contiguous, of its tensor's shape and device, float32, bfloat16 or float16")
-        pout, out_types = _pointers(outs), (ctypes.c_int32 * n)(*[_TYPE[o.dtype] for o in outs])
+        out_dev, out_type_list, out_lengths, out_addresses = _list_of(outs, "out")
+        if out_dev != dev or out_lengths != length_list:
+            raise FlexSpmvError("out must be on the tensors' device and have as many values, each as its tensor")
+        pout, out_types = array.array("Q", out_addresses), array.array("i", out_type_list)
     need, pieces = ctypes.c_size_t(), ctypes.c_int32()
-    _check(_function("clip_gradients_bytes", _CLIP_BYTES)(n, ctypes.addressof(lengths), ctypes.addressof(need), ctypes.addressof(pieces)), "clip_gradients")
+    _check(_function("clip_gradients_bytes", _CLIP_BYTES)(n, _at(lengths), ctypes.addressof(need), ctypes.addressof(pieces)), "clip_gradients")
     ws = torch.empty(need.value // 8, dtype=torch.float64, device=tensors[0].device)
     norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
-    plan = (n, ctypes.addressof(pin), ctypes.addressof(types), ctypes.addressof(lengths), ctypes.addressof(pout) if pout is not None else None,
-            ctypes.addressof(out_types) if out_types is not None else None, ws.data_ptr(), need.value, _raw_stream(dev))
+    plan = (n, _at(pin), _at(types), _at(lengths), _at(pout) if pout is not None else None, _at(out_types) if out_types is not None else None,
+            ws.data_ptr(), need.value, _raw_stream(dev))
     if _current_device() == dev:
         st = _function("clip_gradients_plan", _CLIP_PLAN)(*plan)
     else:
@@ -466,12 +483,12 @@ def _clip(tensors: Sequence[torch.Tensor], max_norm: float, outs) -> BoundCall:
 @_operator
 def grad_norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
     """``sqrt(sum of all squares)`` over contiguous tensors of any of the three types: one float32 on the device, the same bits every time."""
-    return _clip(tensors, 0.0, None)
+    return _clip(list(tensors), 0.0, None)
 
 
 @_operator
 def clip_grad_norm(tensors: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
-    """Scales the tensors by ``min(1, max_norm / (norm + 1e-6))``, in place or into ``out`` (tensors of the same shapes, of any of the three
+    """Scales the tensors by ``min(1, max_norm / (norm + 1e-6))``, in place or into ``out`` (tensors of the same lengths, of any of the three
     types), and returns the norm before it."""
     tensors = list(tensors)
     if not (max_norm >= 0):
