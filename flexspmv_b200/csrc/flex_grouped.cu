@@ -58,6 +58,7 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict_
 //   dw            128 of n by 256 of k, summed over the expert's places
 // PAIR = 2: two CTAs on two neighbouring SMs take a tile of 256 rows, 128 each; each copies half of the columns' operand for both, which
 // halves what those columns cost the L2 (from 48 KB to 32 KB an SM for 64 of the sum).
+// HALVES = 2: a tile has twice the rows, half of them in each accumulator; the columns' operand is copied once for both.
 // SPLIT: few tiles.  A cluster of up to eight CTAs takes one tile, each its share of the sum; the parts meet in shared memory, where every CTA
 // adds up some of the columns in the CTAs' order.  No workspace, no atomics.
 // GATHER (forward): x's rows by a list.  Four more warps copy them, 16 bytes a thread, to where a tile copy would have put them; as fast as contiguous
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict_
 // there instead of 0.43.)  dw's rows are other ones in every step: gathered like this they take 0.57 ms of the 32 768; a copy of them in the
 // workspace and contiguous tile copies 0.44.
 // Warps 0-7 store finished accumulators, warp 8 issues the tile copies, warp 9 the matrix instructions; two accumulators in tensor memory,
-// so that one is stored while the next is computed.  The sum goes 64 values (128 bytes of a row) a stage.
+// so that one is stored while the next is computed (HALVES = 2: while the other half of the next tile begins).  The sum goes 64 values (128 bytes of a row) a stage.
 constexpr int kStoreWarps = 8, kCopyWarp = kStoreWarps, kMathWarp = kStoreWarps + 1, kGroupedThreads = (kStoreWarps + 2) * 32;
 constexpr int kGatherWarps = 4;
 constexpr int grouped_threads(bool gather) { return kGroupedThreads + (gather ? kGatherWarps * 32 : 0); }
@@ -75,10 +76,10 @@ constexpr uint64_t kWaitLimitNs = 1000000000ull;
 // 10 000, lost in a result of 16 bits but not in one of 32.  So that one is added up, correctly rounded, from parts of this many steps (512 rows).
 constexpr int kPartSteps = 8;
 
-template <int MODE, int NT, int PAIR, int OUT_BYTES>
+template <int MODE, int NT, int PAIR, int HALVES, int OUT_BYTES>
 struct GroupedCfg {
-  static constexpr int kBytesB = NT / PAIR * 128;
-  static constexpr int kStageBytes = kTileBytesA + kBytesB;
+  static constexpr int kBytesA = HALVES * kTileBytesA, kBytesB = NT / PAIR * 128;
+  static constexpr int kStageBytes = kBytesA + kBytesB;
   static constexpr int kStages = (OUT_BYTES == 4 ? 180224 : 196608) / kStageBytes;
   static constexpr int kTmemCols = 2 * NT < 32 ? 32 : 2 * NT;
   static constexpr int kStoreBytes = kStoreWarps * 1024 * OUT_BYTES;        // 32 x 32 results a warp
@@ -96,6 +97,7 @@ struct GroupedBars {
 
 struct GroupedTile {
   int e, m0, n0, from, count, cols;     // dw: m0 of n, n0 of k; else m0 of the features, places from .. from + count; cols: the accumulator's
+  int half, halves_end;                 // the halves of its rows that are this cluster's: half .. halves_end - 1
 };
 
 // How many places a tile of a group of `count` takes: the group in equal parts, in 16s (a pair: in 32s).
@@ -106,17 +108,18 @@ __device__ __forceinline__ int tile_places(int count) {
   return ((count + tiles - 1) / tiles + kStep - 1) & ~(kStep - 1);
 }
 
-template <int MODE, int NT, int PAIR>
+template <int MODE, int NT, int PAIR, int HALVES>
 __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const GroupedTable* table, int t) {
   GroupedTile r;
   const int m = MODE == kGroupedDx ? a.k : a.n;
-  const int m_tiles = (m + 128 * PAIR - 1) / (128 * PAIR);
+  constexpr int kRows = 128 * PAIR * HALVES;
+  const int m_tiles = (m + kRows - 1) / kRows;
   constexpr int kStep = 16 * PAIR;
   if (MODE == kGroupedDw) {
     const int n_tiles = (a.k + NT - 1) / NT, each = m_tiles * n_tiles;
     r.e = t / each;
     const int i = t - r.e * each;
-    r.m0 = i / n_tiles * 128 * PAIR;
+    r.m0 = i / n_tiles * kRows;
     r.n0 = i % n_tiles * NT;
     r.from = table[r.e].from;
     r.count = table[r.e].count;
@@ -132,7 +135,7 @@ __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const Group
   }
   r.e = lo;
   const int i = t - table[lo].first, size = tile_places<NT, PAIR>(table[lo].count), part = i / m_tiles * size;
-  r.m0 = i % m_tiles * 128 * PAIR;
+  r.m0 = i % m_tiles * kRows;
   r.n0 = 0;
   r.from = table[lo].from + part;
   r.count = table[lo].count - part < size ? table[lo].count - part : size;
@@ -140,12 +143,12 @@ __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const Group
   return r;
 }
 
-template <class T, class TO, int MODE, int NT, int PAIR, bool SPLIT, bool GATHER>
+template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER>
 __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                      const __grid_constant__ CUtensorMap row_a, const __grid_constant__ CUtensorMap row_b,
                                                                      const __grid_constant__ CUtensorMap map_out,
                                                                      GroupedArgs a) {
-  using Cfg = GroupedCfg<MODE, NT, PAIR, (int)sizeof(TO)>;
+  using Cfg = GroupedCfg<MODE, NT, PAIR, HALVES, (int)sizeof(TO)>;
   constexpr int kThreads = grouped_threads(GATHER);
   extern __shared__ __align__(1024) unsigned char grouped_sm[];
   unsigned char* const base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(grouped_sm) + 1023) & ~(uintptr_t)1023);
@@ -180,7 +183,8 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
     table[e].count = to - from;
   }
   __syncthreads();
-  const int m_tiles = ((MODE == kGroupedDx ? a.k : a.n) + 128 * PAIR - 1) / (128 * PAIR);
+  const int m_rows = MODE == kGroupedDx ? a.k : a.n;
+  const int m_tiles = (m_rows + 128 * PAIR * HALVES - 1) / (128 * PAIR * HALVES);
   if (warp == 0) {                         // exclusive sums of the experts' tiles
     int done = 0;
     for (int e0 = 0; e0 <= a.experts; e0 += 32) {
@@ -203,7 +207,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   const uint32_t tmem = bars.tmem;
   const int tiles = MODE == kGroupedDw ? a.experts * m_tiles * ((a.k + NT - 1) / NT) : table[a.experts].first;
   const int first = blockIdx.x / (PAIR * split);
-  const int stride = SPLIT ? 1 << 30 : gridDim.x / PAIR;      // SPLIT: one tile
+  const int stride = gridDim.x / PAIR;
   volatile int* const abort = &bars.abort;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -219,6 +223,16 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   auto steps_of = [&](const GroupedTile& t) {
     return ((MODE == kGroupedForward ? a.k : MODE == kGroupedDx ? a.n : t.count) + 63) / 64;
   };
+  // This cluster's tile of round u.  HALVES = 2: where the last round has tiles for half of the clusters at most, a cluster takes half a tile.
+  const int rounds = SPLIT ? 0 : tiles / stride, rest = SPLIT ? tiles : tiles - rounds * stride;
+  auto tile_of = [&](int u, GroupedTile& t) {
+    const bool by_halves = HALVES == 2 && u == rounds && rest * 2 <= stride;
+    if (u > rounds || (u == rounds && first >= (by_halves ? rest * 2 : rest))) return false;
+    t = tile_at<MODE, NT, PAIR, HALVES>(a, table, u * stride + (by_halves ? first / 2 : first));
+    t.half = by_halves ? first % 2 : 0;
+    t.halves_end = HALVES == 2 && t.m0 + 128 * PAIR < m_rows ? (by_halves ? t.half + 1 : 2) : 1;
+    return true;
+  };
   // this CTA's steps of a tile
   auto step_from = [&](int steps) { return SPLIT ? steps * share / split : 0; };
   auto step_to = [&](int steps) { return SPLIT ? steps * (share + 1) / split : steps; };
@@ -227,41 +241,50 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     if (elect_one()) {
-      for (int i = first; i < tiles && !*abort; i += stride) {
-        const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
+      GroupedTile t;
+      for (int u = 0; !*abort && tile_of(u, t); ++u) {
         const int steps = steps_of(t), from = step_from(steps), to = step_to(steps), half = t.cols / PAIR;
+        if (t.half >= t.halves_end) continue;
         const int pieces = GATHER ? 0 : MODE == kGroupedDw ? (half + 63) / 64 : (half + 31) / 32;          // of the columns' operand
-        const int m0 = t.m0 + rank * 128;
+        const int m0 = t.m0 + rank * 128, halves = t.halves_end - t.half;
         for (int s = from; s < to; ++s) {
           if (!wait(&bars.empty[stage], phase ^ 1)) break;
           unsigned char* const sa = base + stage * Cfg::kStageBytes;
-          unsigned char* const sb = sa + kTileBytesA;
+          unsigned char* const sb = sa + Cfg::kBytesA;
           const uint32_t bar = PAIR == 2 ? cluster_smem(&bars.full[stage], 0) : smem_u32(&bars.full[stage]);
           if (MODE == kGroupedDw) {
             // A step's last rows may be the next group's.  The maps count rows by two dimensions of one stride, y + z, and y ends at 64: with the
             // step's last valid row at y = 63, what follows it is out of range and zero.
             const int valid = t.count - s * 64 < 64 ? t.count - s * 64 : 64, place = t.from + s * 64, z = place + valid - 64;
             const int rows = z >= 0 ? 64 : (valid + 15) & ~15, n0 = t.n0 + rank * half;          // rows: how many are copied
-            if (rank == 0) mbar_expect_tx(&bars.full[stage], PAIR * (2 + pieces) * rows * 128);
+            if (rank == 0) mbar_expect_tx(&bars.full[stage], PAIR * (2 * halves + pieces) * rows * 128);
             if (z >= 0) {
-              tma_3d<PAIR>(sa, &map_a, m0, 64 - valid, z, bar);
-              tma_3d<PAIR>(sa + 8192, &map_a, m0 + 64, 64 - valid, z, bar);
+              for (int h = t.half; h < t.halves_end; ++h) {
+                tma_3d<PAIR>(sa + h * kTileBytesA, &map_a, m0 + h * 128 * PAIR, 64 - valid, z, bar);
+                tma_3d<PAIR>(sa + h * kTileBytesA + 8192, &map_a, m0 + h * 128 * PAIR + 64, 64 - valid, z, bar);
+              }
               for (int g = 0; g < pieces; ++g) tma_3d<PAIR>(sb + g * 8192, &map_b, n0 + g * 64, 64 - valid, z, bar);
             } else {                       // a group that ends in the first 64 rows: row by row, rows out of range for the rest
               for (int r = 0; r < rows; ++r) {
                 const int y = r < valid ? place + r : (int)a.slots;
-                tma_2d<PAIR>(sa + r * 128, &row_a, m0, y, bar);
-                tma_2d<PAIR>(sa + 8192 + r * 128, &row_a, m0 + 64, y, bar);
+                for (int h = t.half; h < t.halves_end; ++h) {
+                  tma_2d<PAIR>(sa + h * kTileBytesA + r * 128, &row_a, m0 + h * 128 * PAIR, y, bar);
+                  tma_2d<PAIR>(sa + h * kTileBytesA + 8192 + r * 128, &row_a, m0 + h * 128 * PAIR + 64, y, bar);
+                }
                 for (int g = 0; g < pieces; ++g) tma_2d<PAIR>(sb + g * 8192 + r * 128, &row_b, n0 + g * 64, y, bar);
               }
             }
           } else {
-            if (rank == 0) mbar_expect_tx(&bars.full[stage], PAIR * (kTileBytesA + pieces * 4096));
-            if (MODE == kGroupedForward) {
-              tma_3d<PAIR>(sa, &map_a, s * 64, m0, t.e, bar);
-            } else {
-              tma_3d<PAIR>(sa, &map_a, m0, s * 64, t.e, bar);
-              tma_3d<PAIR>(sa + 8192, &map_a, m0 + 64, s * 64, t.e, bar);
+            if (rank == 0) mbar_expect_tx(&bars.full[stage], PAIR * (halves * kTileBytesA + pieces * 4096));
+            for (int h = t.half; h < t.halves_end; ++h) {
+              unsigned char* const half_a = sa + h * kTileBytesA;
+              const int row = m0 + h * 128 * PAIR;
+              if (MODE == kGroupedForward) {
+                tma_3d<PAIR>(half_a, &map_a, s * 64, row, t.e, bar);
+              } else {
+                tma_3d<PAIR>(half_a, &map_a, row, s * 64, t.e, bar);
+                tma_3d<PAIR>(half_a + 8192, &map_a, row + 64, s * 64, t.e, bar);
+              }
             }
             for (int g = 0; g < pieces; ++g) tma_2d<PAIR>(sb + g * 4096, &map_b, s * 64, t.from + rank * half + g * 32, bar);
           }
@@ -281,12 +304,64 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   } else if (warp == kMathWarp) {
     if (rank == 0 && elect_one()) {
       int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      for (int i = first; i < tiles && !*abort; i += stride) {
-        const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
+      uint32_t phase = 0, acc_phase = 0, phases = 0;         // phases: HALVES = 2, a bit for each accumulator
+      const auto copied = [&](int stage, uint32_t phase) {
+        if (!wait(&bars.full[stage], phase)) return false;
+        if (GATHER) {
+          if (!wait(&bars.gathered[stage], phase)) return false;
+          fence_proxy_async_smem();        // here, where nothing is under way, for the threads that copied
+        }
+        tmem_fence_after();
+        return true;
+      };
+      GroupedTile t;
+      for (int u = 0; !*abort && tile_of(u, t); ++u) {
         const int steps = steps_of(t), from = step_from(steps), to = step_to(steps);
-        if (from == to) continue;
+        if (from == to || t.half >= t.halves_end) continue;
         const uint32_t instr = umma_instr(std::is_same<T, __nv_bfloat16>::value, kA_mn, kB_mn, 128 * PAIR, t.cols);
+        // step s of the tile: half h of its rows, from a stage into accumulator `acc`
+        const auto multiply = [&](int s, int stage, int h, int acc, bool begins) {
+          const uint32_t sa = smem_u32(base + stage * Cfg::kStageBytes) + h * kTileBytesA, sb = smem_u32(base + stage * Cfg::kStageBytes) + Cfg::kBytesA;
+          const uint64_t da = kA_mn ? umma_desc(sa, 8192, 1024) : umma_desc(sa, 16, 1024);
+          const uint64_t db = kB_mn ? umma_desc(sb, 8192, 1024) : umma_desc(sb, 16, 1024);
+          const int inner = MODE == kGroupedDw && t.count - s * 64 < 64 ? (t.count - s * 64 + 15) / 16 : 4;
+          for (int x = 0; x < inner; ++x)  // the descriptors' addresses are in 16 bytes
+            umma<PAIR>(tmem + acc * NT, da + x * (kA_mn ? 128 : 2), db + x * (kB_mn ? 128 : 2), instr, !begins || x > 0);
+        };
+        if constexpr (HALVES == 2) {
+          // Both accumulators belong to the tile, one to each half.  The first half of its first steps goes ahead while the last tile's second half
+          // is still being stored; their stages are free once the second half has followed.
+          const int h = t.half, lead = to - from < Cfg::kStages ? to - from : Cfg::kStages;
+          const bool both = t.halves_end - h == 2;
+          if (!wait(&bars.acc_empty[h], (phases >> h & 1) ^ 1)) break;
+          tmem_fence_after();
+          int ahead = stage;
+          uint32_t ahead_phase = phase;
+          bool good = true;
+          for (int s = from; s < from + lead && good; ++s) {
+            good = copied(ahead, ahead_phase);
+            if (good) multiply(s, ahead, h, h, s == from);
+            if (++ahead == Cfg::kStages) { ahead = 0; ahead_phase ^= 1; }
+          }
+          if (!good) break;
+          if (both) {
+            if (!wait(&bars.acc_empty[1], (phases >> 1) ^ 1)) break;
+            tmem_fence_after();
+          }
+          for (int s = from; s < to; ++s) {
+            if (s >= from + lead) {
+              if (!copied(stage, phase)) break;
+              multiply(s, stage, h, h, false);
+            }
+            if (s + 1 == to) umma_commit<PAIR>(&bars.acc_full[h]);
+            if (both) multiply(s, stage, 1, 1, s == from);
+            umma_commit<PAIR>(&bars.empty[stage]);
+            if (++stage == Cfg::kStages) { stage = 0; phase ^= 1; }
+          }
+          if (both) umma_commit<PAIR>(&bars.acc_full[1]);
+          phases ^= both ? 3u : 1u << h;
+          continue;
+        }
         for (int s = from; s < to; ++s) {
           const bool begins = s == from || (kInParts && (s - from) % kPartSteps == 0);
           const bool ends = s + 1 == to || (kInParts && (s + 1 - from) % kPartSteps == 0);
@@ -294,19 +369,8 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
             if (!wait(&bars.acc_empty[acc], acc_phase ^ 1)) break;
             tmem_fence_after();
           }
-          const uint32_t d = tmem + acc * NT;
-          if (!wait(&bars.full[stage], phase)) break;
-          if (GATHER) {
-            if (!wait(&bars.gathered[stage], phase)) break;
-            fence_proxy_async_smem();      // here, where nothing is under way, for the threads that copied
-          }
-          tmem_fence_after();
-          const uint32_t sa = smem_u32(base + stage * Cfg::kStageBytes), sb = sa + kTileBytesA;
-          const uint64_t da = kA_mn ? umma_desc(sa, 8192, 1024) : umma_desc(sa, 16, 1024);
-          const uint64_t db = kB_mn ? umma_desc(sb, 8192, 1024) : umma_desc(sb, 16, 1024);
-          const int inner = MODE == kGroupedDw && t.count - s * 64 < 64 ? (t.count - s * 64 + 15) / 16 : 4;
-          for (int x = 0; x < inner; ++x)  // the descriptors' addresses are in 16 bytes
-            umma<PAIR>(d, da + x * (kA_mn ? 128 : 2), db + x * (kB_mn ? 128 : 2), instr, !begins || x > 0);
+          if (!copied(stage, phase)) break;
+          multiply(s, stage, 0, acc, begins);
           umma_commit<PAIR>(&bars.empty[stage]);
           if (ends) {
             umma_commit<PAIR>(&bars.acc_full[acc]);
@@ -321,8 +385,10 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
       // wait for all that their thread has under way (1.0 to 1.8 us a step).
       int stage = 0;
       uint32_t phase = 0;
-      for (int i = first; i < tiles && !*abort; i += stride) {
-        const int steps = steps_of(tile_at<MODE, NT, PAIR>(a, table, i));
+      GroupedTile t;
+      for (int u = 0; !*abort && tile_of(u, t); ++u) {
+        if (t.half >= t.halves_end) continue;
+        const int steps = steps_of(t);
         for (int s = step_from(steps); s < step_to(steps); ++s) {
           if (!wait(&bars.gathered[stage], phase)) break;
           fence_proxy_async_smem();
@@ -341,8 +407,9 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
     const int x_rows = (int)a.tokens, x_columns = a.k;
     int stage = 0;
     uint32_t phase = 0;
-    for (int i = first; i < tiles && !stopped(); i += stride) {
-      const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
+    GroupedTile t;
+    for (int u = 0; !stopped() && tile_of(u, t); ++u) {
+      if (t.half >= t.halves_end) continue;
       const int steps = steps_of(t), from = step_from(steps), to = step_to(steps), half = t.cols / PAIR;
       int row[kPasses];                    // of x; -1: beyond the group, or not a row of x: zeros
 #pragma unroll
@@ -360,7 +427,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
       }
       for (int s = from; s < to; ++s) {
         if (!wait_warp(&bars.empty[stage], phase ^ 1)) break;
-        const uint32_t sb = smem_u32(base + stage * Cfg::kStageBytes + kTileBytesA);
+        const uint32_t sb = smem_u32(base + stage * Cfg::kStageBytes + Cfg::kBytesA);
         const int c = s * 64 + piece * 8;
         const bool inside = c < x_columns;
         const char* const x_piece = x + c * 2;
@@ -378,13 +445,17 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
     copy16_wait_all();
   } else {
     int acc = 0;
-    uint32_t acc_phase = 0;
+    uint32_t acc_phase = 0, second_phase = 0;
     TO* const out = static_cast<TO*>(a.out);
     unsigned char* const mine = store + warp * (Cfg::kStoreBytes / kStoreWarps);
     const int quarter = warp & 3, part = warp >> 2;     // of the accumulator's rows, of its columns
-    for (int i = first; i < tiles && !stopped(); i += stride) {
-      const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, i);
-      const int m = t.m0 + rank * 128 + quarter * 32;   // this warp's first row of the accumulator
+    GroupedTile t;
+    for (int u = 0; !stopped() && tile_of(u / HALVES, t); ++u) {           // tiles, or their halves
+      const int half = u % HALVES;
+      if (half < t.half || half >= t.halves_end) continue;
+      if (HALVES == 2) acc = half;
+      const uint32_t full_phase = half ? second_phase : acc_phase;
+      const int m = t.m0 + half * 128 * PAIR + rank * 128 + quarter * 32;          // this warp's first row of the accumulator
       const int steps = steps_of(t), from = step_from(steps), to = step_to(steps);
       const auto free_accumulator = [&] {  // once this warp's last of it is in registers
         tmem_fence_before();
@@ -474,7 +545,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           if (part * 32 + g * 64 < t.cols) store_rows(part * 32 + g * 64, [&](int x) { return sum[g][x]; });
         continue;
       }
-      if (!wait_warp(&bars.acc_full[acc], acc_phase)) break;
+      if (!wait_warp(&bars.acc_full[acc], full_phase)) break;
       tmem_fence_after();
       const uint32_t d = tmem + acc * NT + ((uint32_t)(quarter * 32) << 16);
       for (int c0 = part * 32;; c0 += 64) {
@@ -518,7 +589,13 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
         }
         if (last) break;
       }
-      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      if (HALVES == 2) {
+        if (half) second_phase ^= 1;
+        else acc_phase ^= 1;
+      } else if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
     }
     if (MODE == kGroupedDw && lane == 0) tma_stores_done();
     if (MODE != kGroupedDw) {     // places of no expert: before the first group and after the last
@@ -534,7 +611,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
     // every CTA stores some of the tile's columns, eight neighbouring rows (dw: columns) at a time
     cluster_sync();
     if (first < tiles && !*abort) {
-      const GroupedTile t = tile_at<MODE, NT, PAIR>(a, table, first);
+      const GroupedTile t = tile_at<MODE, NT, PAIR, HALVES>(a, table, first);
       const int eights = (t.cols + 7) / 8, c_from = eights * share / split * 8, c_to = eights * (share + 1) / split * 8;
       const uint32_t sums = smem_u32(base);
       TO* const out = static_cast<TO*>(a.out);
@@ -600,14 +677,14 @@ static int clusters_at_once(int ctas, int smem) {
   return n - 1;
 }
 
-template <int MODE, int NT, int PAIR, int OUT_BYTES>
+template <int MODE, int NT, int PAIR, int HALVES, int OUT_BYTES>
 static int grouped_smem(int experts) {
-  using Cfg = GroupedCfg<MODE, NT, PAIR, OUT_BYTES>;
+  using Cfg = GroupedCfg<MODE, NT, PAIR, HALVES, OUT_BYTES>;
   return 1024 + Cfg::kStages * Cfg::kStageBytes + Cfg::kStoreBytes + (int)sizeof(GroupedBars) + (experts + 1) * (int)sizeof(GroupedTable);
 }
 
 // `split`: CTAs that share a tile, `grid` of them altogether; 1: whole tiles.
-template <class T, class TO, int MODE, int NT, int PAIR, bool SPLIT, bool GATHER>
+template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER>
 static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStream_t st) {
   constexpr CUtensorMapDataType kIn = std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap ma, mb, row_a, row_b, out;
@@ -640,8 +717,8 @@ static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStre
     row_a = out = ma;
     row_b = mb;
   }
-  const int smem = grouped_smem<MODE, NT, PAIR, (int)sizeof(TO)>(a.experts);
-  constexpr auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR, SPLIT, GATHER>;
+  const int smem = grouped_smem<MODE, NT, PAIR, HALVES, (int)sizeof(TO)>(a.experts);
+  constexpr auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR, HALVES, SPLIT, GATHER>;
   if (int e = allow_smem<kernel>(smem)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3((unsigned)grouped_threads(GATHER)); cfg.dynamicSmemBytes = smem; cfg.stream = st;
@@ -665,14 +742,24 @@ static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
   // What dividing saves is most of a tile's steps, 0.3 us each (a narrow tile's 0.13); what it costs is the parts' meeting, about 5 us (1.5).
   // us, whole / divided: 8 rows, one expert of 2048 x 4096 17.4 / 9.4; dw of 8192 rows, 1024 x 1024 43.8 / 22; but 4096 rows, two experts of
   // 512 x 512 (8 steps) 9.8 / 12.6.
-  constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, true, GATHER>;
-  const int smem = grouped_smem<MODE, NT, 1, (int)sizeof(TO)>(a.experts);
+  constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, 1, true, GATHER>;
+  const int smem = grouped_smem<MODE, NT, 1, 1, (int)sizeof(TO)>(a.experts);
   for (int split = 8; split > 1; split /= 2) {
     if (most * split > sms || steps - steps / split < (NT > 64 ? 20 : 12)) continue;
     if (int e = allow_smem<divided>(smem)) return e;
-    if (most <= clusters_at_once<divided, grouped_threads(GATHER)>(split, smem)) return grouped_launch_as<T, TO, MODE, NT, 1, true, GATHER>(a, (int)most * split, split, st);
+    if (most <= clusters_at_once<divided, grouped_threads(GATHER)>(split, smem)) return grouped_launch_as<T, TO, MODE, NT, 1, 1, true, GATHER>(a, (int)most * split, split, st);
   }
-  return grouped_launch_as<T, TO, MODE, NT, PAIR, false, GATHER>(a, sms / PAIR * PAIR, 1, st);
+  // Tiles of both accumulators (HALVES = 2): a quarter less between L2 and the SMs for a tile's step, a stage less under way, and the end of a tile's
+  // sum that only half of it is behind.  It pays where the sums are long and the tiles go round the pairs, most with gathered rows, which are gathered
+  // half as often.  us, one / both: 32 768 rows, 32 experts of 4096 x 2048, with a list 437 / 419, without 411 / 413, dw 418 / 410, dx 411 / 419;
+  // 10 599 rows, 8 experts of 1488 x 2792 87.6 / 75.7; 8192 x 8192 x 8192 737 / 688; but 8192 rows of 328 85 / 89, 4102 rows of 2048 28 / 30.
+  if constexpr (NT > 64 && sizeof(TO) == 2 && MODE != kGroupedDx) {
+    const long long columns = MODE == kGroupedDw ? (long long)a.experts * ((a.k + NT - 1) / NT) : a.slots / NT + a.experts / 2;          // of tiles, about
+    const int long_sum = MODE == kGroupedDw ? 16 : GATHER ? 32 : 40, half_rounds = MODE == kGroupedDw ? 20 : 3;
+    if (steps >= long_sum && columns * ((a.n + 511) / 512) * 2 >= half_rounds * (sms / 2))
+      return grouped_launch_as<T, TO, MODE, NT, 2, 2, false, GATHER>(a, sms / 2 * 2, 1, st);
+  }
+  return grouped_launch_as<T, TO, MODE, NT, PAIR, 1, false, GATHER>(a, sms / PAIR * PAIR, 1, st);
 }
 
 template <class T, class TO, int MODE, bool GATHER>

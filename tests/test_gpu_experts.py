@@ -232,6 +232,26 @@ def test_grouped_matmul_dw(counts, n, k, dtype, out_dtype, gather):
         close(dw[e], d.t() @ xe, d.abs().t() @ xe.abs(), max(1, counts[e]))
 
 
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("counts,n,k", [([3000, 0, 1, 4100, 257, 2000], 1560, 2624), ([1100] * 12, 2048, 4096), ([6000], 3400, 2560)])
+def test_grouped_large(counts, n, k, gather):
+    """Tiles of both accumulators, the last of them half a tile, a round by halves; sampled rows and matrices."""
+    x, w, offsets, rows, of, take = grouped_case(counts, n, k, torch.bfloat16, gather, extra=3, start=1)
+    dy = normal(7, (of.numel(), n), torch.bfloat16)
+    y = experts.grouped_matmul(x, w, offsets, rows=rows)
+    dw = experts.grouped_matmul_dw(dy, x, offsets, rows=rows)
+    experts.check()
+    assert not y[0].any() and not y[-3:].any()
+    for e in range(len(counts)):
+        at = torch.nonzero(of == e).view(-1).cuda()
+        if counts[e] == 0:
+            assert not dw[e].any()
+            continue
+        xe, we, d = x[take[at]].double(), w[e].double(), dy[at].double()
+        close(y[at], xe @ we.t(), xe.abs() @ we.abs().t(), k)
+        close(dw[e], d.t() @ xe, d.abs().t() @ xe.abs(), counts[e])
+
+
 @pytest.mark.parametrize("counts,n,k", [([9001, 513, 512, 40], 264, 328), ([30_000], 128, 256)])
 def test_grouped_matmul_dw_in_32_bits_over_many_rows(counts, n, k):
     """Parts of 512 rows, each by 32 matrix instructions that cut at most two units of their partial sum, then as many correctly rounded
