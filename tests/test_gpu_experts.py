@@ -86,6 +86,22 @@ def test_route(tokens, n, k, dtype):
         assert np.all(np.abs(plan.weights.double().cpu().numpy() - w) <= (n + 8) * 2.0 ** -23 * w + 1e-37)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [257, 300, 383, 384, 385, 500, 512, 516, 1000, 1023])
+def test_route_of_many_experts(n, dtype):
+    """Each number of keys a lane sorts, rows with and without wide loads; rising, falling and equal logits."""
+    logits = normal(n, (301, n), dtype)
+    logits[0] = torch.arange(n, device="cuda").to(dtype)
+    logits[1] = -torch.arange(n, device="cuda").to(dtype)
+    logits[2] = 1.0
+    for k in (1, 9, 32):
+        plan = experts.route(logits, k)
+        w, ids, offsets, rows, slots, _ = plain_route(logits, k, False)
+        assert np.array_equal(plan.experts.cpu().numpy(), ids) and np.array_equal(plan.slots.cpu().numpy(), slots)
+        assert np.array_equal(plan.offsets.cpu().numpy(), offsets) and np.array_equal(plan.rows.cpu().numpy(), rows)
+        assert np.all(np.abs(plan.weights.double().cpu().numpy() - w) <= (n + 8) * 2.0 ** -23 * w + 1e-37)
+
+
 def test_route_of_a_part_of_a_wider_matrix_and_bound():
     wide = normal(3, (300, 96), torch.float32)
     logits = wide[:, 16:56]
