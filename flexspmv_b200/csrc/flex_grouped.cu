@@ -787,7 +787,11 @@ static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
   } else {
     // Tiles of 64 places and single CTAs for up to 32 places an expert on average: more of the weights on their way at once.  us, 64 / 256 places:
     // 16 an expert, 64 experts of 1408 x 2048 59.8 / 66.8; 32 experts of 2048 x 2048, 32 an expert 47.0 / 49.7, 48 51.0 / 50.5, 128 72.1 / 54.9.
-    if (a.slots <= 32ll * a.experts) return grouped_tiles<T, TO, MODE, 64, 1, GATHER>(a, st);
+    // And where as narrow tiles all of them run at once: a part of the sum is a quarter as much to add up, a gathered step a quarter of the rows.
+    // us, narrow / wide: 753 rows, 4 experts of 104 x 1512 8.9 / 15.1; 256 rows of 2048 x 2048 10.5 / 14.3, of a list 11.0 / 16.0; 512 rows of 1024 x 1024
+    // 7.3 / 8.1; but 100 rows of 4096 x 4096 13.0 / 12.3.
+    const long long narrow = ((MODE == kGroupedDx ? a.k : a.n) + 127) / 128 * ((a.slots < a.experts ? a.slots : a.experts) + a.slots / 64);
+    if (a.slots <= 32ll * a.experts || narrow <= device_sm_count()) return grouped_tiles<T, TO, MODE, 64, 1, GATHER>(a, st);
     return grouped_tiles<T, TO, MODE, 256, 2, GATHER>(a, st);
   }
 }
