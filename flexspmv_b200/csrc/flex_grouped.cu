@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict_
 // SPLIT: few tiles.  A cluster of up to eight CTAs takes one tile, each its share of the sum; the parts meet in shared memory, where every CTA
 // adds up some of the columns in the CTAs' order.  No workspace, no atomics.
 // GATHER (forward): x's rows by a list.  Four more warps copy them, 16 bytes a thread, to where a tile copy would have put them; as fast as contiguous
-// rows up to some thousand rows, 7 % slower for 32 768 of 2048.  (Tile copies that gather four rows each took 72 cycles an instruction: 2.2 ms
+// rows up to some thousand rows, 2 - 4 % slower for 32 768 of 2048.  (Tile copies that gather four rows each took 72 cycles an instruction: 2.2 ms
 // there instead of 0.43.)  dw's rows are other ones in every step: gathered like this they take 0.57 ms of the 32 768; a copy of them in the
 // workspace and contiguous tile copies 0.44.
 // Warps 0-7 store finished accumulators, warp 8 issues the tile copies, warp 9 the matrix instructions; two accumulators in tensor memory,
