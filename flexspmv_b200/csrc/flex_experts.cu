@@ -27,7 +27,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float exp_below(float v, float top) { return exp2_fast((v - top) * kLog2e); }
 
 // What a choice goes by: a number that is larger for a larger logit and, among equal ones, for a lower expert.  The order of a sign and
-// magnitude number x is 0x8000... +- its magnitude (so that -0 and 0 are equal); NaN is 0.  kNone: the key of -infinity and below, never chosen.
+// magnitude number x is 0x8000... +- its magnitude (so that -0 and 0 are equal); NaN's is 0.  kNone: the key of -infinity and below, never chosen.
+// The expert makes all keys of a row different, NaN's too, and none of them 0.
 // A 16-bit logit and the expert fit 32 bits, so that one instruction finds the largest of a warp; a 32-bit one takes 64.
 template <class T>
 struct Choice {
@@ -58,7 +59,7 @@ struct Choice<float> {
   static constexpr Key kNone = (Key)0x00800000u << 32 | 0xffffu;
   static __device__ __forceinline__ Key make(float v, int e) {
     const uint32_t u = __float_as_uint(v), order = u & 0x80000000u ? 0u - u : u | 0x80000000u;       // 0x80000000 - magnitude
-    return v != v ? 0ull : (Key)order << 32 | (0xffffu - (uint32_t)e);
+    return (Key)(v != v ? 0u : order) << 32 | (0xffffu - (uint32_t)e);
   }
   static __device__ __forceinline__ int expert(Key k) { return (int)(0xffffu - (uint32_t)k); }
   static __device__ __forceinline__ float logit(Key k) {
@@ -146,7 +147,7 @@ __device__ __forceinline__ void choose_token(const LanePart<T, V, W>& part, int 
   for (int j = 0; j < k; ++j) {
     const Key most = C::warp_max(first);
     if (lane == j) mine_key = most;
-    if (first == most) first = *next++;          // 32 V keys are no fewer than the experts, so that k rounds never run out of them
+    if (first == most) first = *next++;          // one lane's: all 32 V keys differ, and as k <= experts <= 32 V a round always finds one before the zeros
   }
   if (mine_key <= C::kNone) mine_key = 0;
   const Key top_key = __shfl_sync(0xffffffffu, mine_key, 0);

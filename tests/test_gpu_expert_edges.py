@@ -1,0 +1,77 @@
+"""Where the expert operators' arguments leave the usual: rows of NaN, ids, ranges and sums at their ends.
+
+Bounds as in ``test_gpu_experts``: n additions in 32 bits err by at most n * 2^-23 of the sum of magnitudes, one rounding to 16 bits by half a
+unit (2^-8 of a bfloat16, 2^-11 of a float16); what is in whole numbers is equal."""
+import numpy as np
+import pytest
+import torch
+
+from flexspmv_b200 import experts
+
+from test_gpu_experts import normal
+
+pytestmark = pytest.mark.gpu
+
+NEGATIVE_NAN = {torch.float32: (torch.int32, -0x400000), torch.bfloat16: (torch.int16, -0x40), torch.float16: (torch.int16, -0x200)}
+
+
+# ---- router ------------------------------------------------------------------------------------------------------
+
+def plain_route(logits, k):
+    """The choice and the plan where NaN is never chosen: experts, offsets, rows, slots."""
+    l = logits.double().cpu().numpy()
+    l = np.where(np.isnan(l), -np.inf, l)
+    tokens, n = l.shape
+    ids = np.argsort(-l, axis=1, kind="stable")[:, :k]
+    ids = np.where(np.isneginf(np.take_along_axis(l, ids, axis=1)), -1, ids)
+    flat = ids.reshape(-1)
+    pair = np.flatnonzero(flat >= 0)
+    pair = pair[np.argsort(flat[pair], kind="stable")]
+    rows, slots = np.full(flat.size, -1), np.full(flat.size, -1)
+    rows[:pair.size] = pair // k
+    slots[pair] = np.arange(pair.size)
+    return ids, np.concatenate([[0], np.cumsum(np.bincount(flat[pair], minlength=n))]), rows, slots.reshape(tokens, k)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [8, 32, 60, 64, 128, 256, 384, 512, 1000, 1024])
+def test_route_of_rows_of_nan(n, dtype):
+    """Rows of NaN alone, of either sign, and rows with fewer than k other logits, among ordinary ones."""
+    for tokens in (7, 41, 300):
+        for k in (1, 8, min(n, 32)):
+            clean = normal(n + tokens, (tokens, n), dtype)
+            bad = torch.zeros((tokens, n), dtype=torch.bool, device="cuda")
+            others = torch.rand((tokens, n), generator=torch.Generator(device="cuda").manual_seed(k), device="cuda").argsort(dim=1)
+            for first, kept in ((1, 0), (2, 0), (3, k // 2), (4, k - 1), (5, k + 1)):          # of every six tokens the first is ordinary
+                bad[first::6] = others[first::6] >= kept
+            logits = clean.masked_fill(bad, float("nan"))
+            as_int, pattern = NEGATIVE_NAN[dtype]
+            logits[2::6] = torch.where(bad[2::6], torch.full_like(clean[2::6].view(as_int), pattern), clean[2::6].view(as_int)).view(dtype)
+            logits[4::12, 0] = float("-inf")
+            ids, offsets, rows, slots = plain_route(logits, k)
+            spoiled = torch.isnan(logits).any(1).cpu().numpy()
+            for renormalize in (False, True):
+                plan = experts.route(logits, k, renormalize=renormalize)
+                assert np.array_equal(plan.experts.cpu().numpy(), ids) and np.array_equal(plan.offsets.cpu().numpy(), offsets)
+                assert np.array_equal(plan.rows.cpu().numpy(), rows) and np.array_equal(plan.slots.cpu().numpy(), slots)
+                got = plan.weights.double().cpu().numpy()
+                l = np.where(np.isnan(x := logits.double().cpu().numpy()), -np.inf, x)
+                top = np.where(ids >= 0, np.take_along_axis(l, np.maximum(ids, 0), axis=1), -np.inf)
+                base = np.where(np.isneginf(top[:, :1]), 0.0, top[:, :1])
+                chosen, whole = np.exp(top - base), np.exp(l - base).sum(1, keepdims=True)
+                total = chosen.sum(1, keepdims=True) if renormalize else whole
+                want = chosen / np.where(total == 0, 1, total)
+                if not renormalize:
+                    want[spoiled] = np.where(ids[spoiled] >= 0, np.nan, 0.0)
+                assert np.array_equal(np.isnan(got), np.isnan(want))
+                assert np.all((np.abs(got - want) <= (n + 8) * 2.0 ** -23 * want + 1e-37) | np.isnan(want))
+                # the gradient: rows without a choice are zeros, the other rows with NaN are NaN unless renormalized, and no row reaches another
+                grad = experts.route_backward(torch.ones_like(plan.weights), logits, plan)
+                none = torch.from_numpy(ids[:, 0] < 0)
+                assert not grad[none.cuda()].any()
+                lost = torch.from_numpy(spoiled) & ~none if not renormalize else torch.zeros_like(none)
+                assert torch.equal(torch.isnan(grad).all(1).cpu(), lost) and torch.equal(torch.isnan(grad).any(1).cpu(), lost)
+                ordinary = torch.arange(0, tokens, 6, device="cuda")
+                alone = experts.route(clean[ordinary].contiguous(), k, renormalize=renormalize)
+                assert torch.equal(plan.weights[ordinary], alone.weights)
+                assert torch.equal(grad[ordinary], experts.route_backward(torch.ones_like(alone.weights), clean[ordinary].contiguous(), alone))
