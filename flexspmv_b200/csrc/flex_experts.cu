@@ -359,7 +359,8 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const float* __rest
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   for (long long t = (long long)blockIdx.x * 8 + warp; t < tokens; t += (long long)gridDim.x * 8) {
-    const int id = lane < k ? ids[t * k + lane] : -1;
+    int id = lane < k ? ids[t * k + lane] : -1;
+    if (id >= experts) id = -1;              // a plan of other logits: not an expert of these
     const float w = id >= 0 ? weights[t * k + lane] : 0.f, g = id >= 0 ? dweights[t * k + lane] : 0.f;
     const T* row = logits + t * stride;
     Pack<T, W> v;

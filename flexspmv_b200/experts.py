@@ -283,6 +283,7 @@ def route_backward(dweights: torch.Tensor, logits: torch.Tensor, plan: Plan, out
     k = plan.weights.shape[1]
     _need(plan.weights.shape[0] == tokens and plan.experts.shape == plan.weights.shape and dweights.shape == plan.weights.shape,
           "dweights and the plan must be of the logits' rows")
+    _need(plan.offsets.numel() == experts + 1, "the plan must be of the logits' experts")
     _whole(dweights, "dweights")
     out = _out(out, (tokens, experts), logits.dtype, logits.device)
     d = Desc(tokens, tokens * k, experts, k, 0, 0, _TYPE[logits.dtype], 0, _RENORMALIZE if plan.renormalize else 0, 0, stride)

@@ -479,7 +479,8 @@ typedef struct flexspmv_expert_desc {
  * (experts + 1), rows (slots: the token of a place, -1 beyond the last offset), slots (tokens x choices: a pair's place, -1: none).
  * The `choices` largest softmax values of a row, largest first, equal ones lowest expert first; logits of -infinity and NaN are never chosen
  * (a NaN makes the row's weights NaN unless they are renormalized).  Places are in order of expert, then token.
- * Workspace: flexspmv_expert_route_bytes.  Backward: in: dweights, logits, weights, experts; out: dlogits (tokens x experts, of the logits' type).
+ * Workspace: flexspmv_expert_route_bytes.  Backward: in: dweights, logits, weights, experts (entries outside [0, experts): no choice; others once in
+ * a row); out: dlogits (tokens x experts, of the logits' type).
  */
 int flexspmv_expert_route_bytes(const flexspmv_expert_desc *desc, size_t *bytes);
 int flexspmv_expert_route(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *d_workspace,

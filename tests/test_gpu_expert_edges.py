@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from flexspmv_b200 import experts
+from flexspmv_b200.binding import FlexSpmvError
 
 from test_gpu_experts import normal
 
@@ -75,3 +76,25 @@ def test_route_of_rows_of_nan(n, dtype):
                 alone = experts.route(clean[ordinary].contiguous(), k, renormalize=renormalize)
                 assert torch.equal(plan.weights[ordinary], alone.weights)
                 assert torch.equal(grad[ordinary], experts.route_backward(torch.ones_like(alone.weights), clean[ordinary].contiguous(), alone))
+
+
+def test_route_backward_of_a_plan_of_other_logits():
+    """Refused where the plan shows it; experts that the logits do not have are no choice, and nothing is written for them."""
+    logits = normal(1, (50, 64), torch.float32)
+    plan = experts.route(logits, 4)
+    g = normal(2, (50, 4), torch.float32)
+    with pytest.raises(FlexSpmvError, match="experts"):
+        experts.route_backward(g, logits[:, :16].contiguous(), plan)
+    for dtype, n in ((torch.float32, 64), (torch.bfloat16, 64), (torch.float16, 33)):
+        logits = normal(3, (50, n), dtype)
+        for renormalize in (False, True):
+            plan = experts.route(logits, 4, renormalize=renormalize)
+            want = experts.route_backward(torch.where(torch.arange(4, device="cuda") == 2, 0.0, g), logits,
+                                          plan._replace(weights=plan.weights.clone(), experts=torch.where(torch.arange(4, device="cuda") == 2, -1, plan.experts)))
+            for beyond in (n, n + 1, 2 ** 31 - 1, -2 ** 31):
+                ids = torch.where(torch.arange(4, device="cuda") == 2, torch.full_like(plan.experts, beyond), plan.experts)
+                around = torch.full((52, n), 7.0, dtype=dtype, device="cuda")
+                got = experts.route_backward(g, logits, plan._replace(experts=ids), out=around[1:51])
+                assert torch.equal(got, want) and bool((around[0] == 7.0).all()) and bool((around[51] == 7.0).all())
+            all_beyond = plan._replace(experts=plan.experts + n)
+            assert not experts.route_backward(g, logits, all_beyond).any()
