@@ -24,15 +24,17 @@ class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, renormalize):
         plan = experts.route(logits, k, renormalize=renormalize)
-        ctx.save_for_backward(logits)
-        ctx.plan = plan
+        # kept as autograd keeps outputs: on the context itself they, the node and the context would hold one another
+        ctx.save_for_backward(logits, plan.weights, plan.experts, plan.offsets)
+        ctx.renormalize = renormalize
         ctx.mark_non_differentiable(plan.experts, plan.offsets, plan.rows, plan.slots)
         return plan.weights, plan.experts, plan.offsets, plan.rows, plan.slots
 
     @staticmethod
     def backward(ctx, dweights, *_):
-        (logits,) = ctx.saved_tensors
-        return experts.route_backward(dweights.contiguous(), logits, ctx.plan), None, None
+        logits, weights, ids, offsets = ctx.saved_tensors
+        plan = experts.Plan(weights, ids, offsets, None, None, ctx.renormalize)
+        return experts.route_backward(dweights.contiguous(), logits, plan), None, None
 
 
 class _Grouped(torch.autograd.Function):

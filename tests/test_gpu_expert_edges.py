@@ -2,12 +2,15 @@
 
 Bounds as in ``test_gpu_experts``: n additions in 32 bits err by at most n * 2^-23 of the sum of magnitudes, one rounding to 16 bits by half a
 unit (2^-8 of a bfloat16, 2^-11 of a float16); what is in whole numbers is equal."""
+import gc
+
 import numpy as np
 import pytest
 import torch
 
 from flexspmv_b200 import experts
 from flexspmv_b200.binding import FlexSpmvError
+from flexspmv_b200.expert_layer import RoutedExperts
 
 from test_gpu_experts import normal
 
@@ -98,3 +101,22 @@ def test_route_backward_of_a_plan_of_other_logits():
                 assert torch.equal(got, want) and bool((around[0] == 7.0).all()) and bool((around[51] == 7.0).all())
             all_beyond = plan._replace(experts=plan.experts + n)
             assert not experts.route_backward(g, logits, all_beyond).any()
+
+
+# ---- the layer ---------------------------------------------------------------------------------------------------
+
+def test_layer_frees_its_plans():
+    """Steps of a training loop leave nothing behind, with Python's cyclic collector off."""
+    layer = RoutedExperts(64, 128, 8, 2, generator=torch.Generator(device="cuda").manual_seed(1))
+    x = normal(2, (3000, 64), torch.bfloat16)
+    gc.collect()
+    gc.disable()
+    try:
+        used = []
+        for _ in range(6):
+            layer(x).float().sum().backward()
+            torch.cuda.synchronize()
+            used.append(torch.cuda.memory_allocated())
+        assert used[-1] == used[1]
+    finally:
+        gc.enable()
