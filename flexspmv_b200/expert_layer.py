@@ -2,7 +2,7 @@
 
     y[t] = sum_j w[t, j] * W2[e] silu(W1[e] x[t]),   e = e[t, j] the j-th choice of a router,  w its renormalized softmax weights
 
-``RoutedExperts`` is the module (differentiable in x, the router's matrix, W1 and W2); ``train_step`` runs it forward and backward, clips all
+``RoutedExperts`` is the module (differentiable once in x, the router's matrix, W1 and W2); ``train_step`` runs it forward and backward, clips all
 gradients by their common norm and updates the weights; ``DecodingStep`` binds the layer to the buffers of a fixed number of tokens, whose
 ``launch()`` can be captured in a CUDA graph.  The reference has no counterpart: its models are stencils and finite volumes
 (shallow_water_equation/swe_main.py:13-146).
@@ -16,6 +16,7 @@ from typing import Iterable, Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import experts
 
@@ -31,6 +32,7 @@ class _Route(torch.autograd.Function):
         return plan.weights, plan.experts, plan.offsets, plan.rows, plan.slots
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dweights, *_):
         logits, weights, ids, offsets = ctx.saved_tensors
         plan = experts.Plan(weights, ids, offsets, None, None, ctx.renormalize)
@@ -46,6 +48,7 @@ class _Grouped(torch.autograd.Function):
         return experts.grouped_matmul(x, weight, offsets, rows=rows)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, weight, offsets, rows, slots = ctx.saved_tensors
         dy = dy.contiguous()
@@ -66,6 +69,7 @@ class _Combine(torch.autograd.Function):
         return experts.combine(z, slots, weights)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         z, slots, weights, offsets = ctx.saved_tensors
         dz, dweights = experts.combine_backward(dout.contiguous(), z, slots, weights, offsets)
