@@ -12,6 +12,9 @@ values, data_struct_shared.cuh:80-659.)
 with the gradients ``route_backward``, ``grouped_matmul_dx``, ``grouped_matmul_dw`` and ``combine_backward``, and ``grad_norm`` and
 ``clip_grad_norm`` over the many tensors that such a layer's training has.  ``expert_layer.RoutedExperts`` runs them together.
 
+Results carry no gradient: while gradients are recorded, tensors that require one are refused (``expert_layer`` has the functions that do carry
+them); only the norm of the last two, as usual, is a plain number.
+
 The operators take CUDA tensors, enqueue on torch's current stream of the tensors' device and never synchronise; the plan stays on the
 device.  Arguments that do not fit raise ``FlexSpmvError``; there is no CPU path.  ``bind(op, *args)`` checks and allocates once and returns
 an object whose ``launch()`` is one foreign call on the same tensors, as ``GraphExtension.prepare`` does for graphs: for loops over fixed
@@ -177,6 +180,9 @@ def _tensor(t, name: str, dtypes, dim: int, device=None) -> int:
                             f"not {tuple(t.shape)} {t.dtype}")
     if device is not None and t.get_device() != device:
         raise FlexSpmvError(f"{name} is on cuda:{t.device.index}, not cuda:{device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise FlexSpmvError(f"{name} requires a gradient, which the result would not carry: call expert_layer's functions, or this one under torch.no_grad() "
+                            "or on detached tensors")
     return t.get_device()
 
 

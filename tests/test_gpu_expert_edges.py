@@ -120,3 +120,30 @@ def test_layer_frees_its_plans():
         assert used[-1] == used[1]
     finally:
         gc.enable()
+
+
+def test_tensors_that_require_a_gradient_are_refused():
+    """Results of the operators carry none, so that one would be lost without a word; without recording they are taken."""
+    bf = torch.bfloat16
+    x, w, logits = normal(1, (10, 64), bf), normal(2, (3, 32, 64), bf), normal(3, (10, 3), torch.float32)
+    plan = experts.route(logits, 2)
+    y = experts.grouped_matmul(x, w, plan.offsets, rows=plan.rows)
+    dy, dout, g = normal(4, (20, 32), bf), normal(5, (10, 32), bf), normal(6, (10, 2), torch.float32)
+    r = lambda t: t.detach().requires_grad_()
+    calls = [
+        lambda f: experts.route(f(logits), 2), lambda f: experts.route_backward(f(g), logits, plan), lambda f: experts.route_backward(g, f(logits), plan),
+        lambda f: experts.grouped_matmul(f(x), w, plan.offsets, rows=plan.rows), lambda f: experts.grouped_matmul(x, f(w), plan.offsets, rows=plan.rows),
+        lambda f: experts.grouped_matmul_dx(f(dy), w, plan.offsets), lambda f: experts.grouped_matmul_dx(dy, f(w), plan.offsets),
+        lambda f: experts.grouped_matmul_dw(f(dy), x, plan.offsets, rows=plan.rows), lambda f: experts.grouped_matmul_dw(dy, f(x), plan.offsets, rows=plan.rows),
+        lambda f: experts.combine(f(y), plan.slots, plan.weights), lambda f: experts.combine(y, plan.slots, f(plan.weights)),
+        lambda f: experts.combine_backward(f(dout), y, plan.slots, plan.weights, plan.offsets),
+        lambda f: experts.combine_backward(dout, f(y), plan.slots, plan.weights, plan.offsets),
+        lambda f: experts.bind(experts.combine, f(y), plan.slots),
+    ]
+    for call in calls:
+        with pytest.raises(FlexSpmvError, match="gradient"):
+            call(r)
+        with torch.no_grad():
+            call(r)
+        call(lambda t: t)
+    experts.check()
