@@ -87,4 +87,31 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 inline bool known_type(int t) { return t == FLEXSPMV_TYPE_F32 || t == FLEXSPMV_TYPE_BF16 || t == FLEXSPMV_TYPE_F16; }
 inline int type_bytes(int t) { return t == FLEXSPMV_TYPE_F32 ? 4 : 2; }
 
+// Where an array lies: rows of `row` bytes, `stride` bytes apart (one row: contiguous).
+struct Region {
+  const void* at;
+  long long row, rows = 1, stride = 1;
+};
+inline Region rows_at(const void* at, long long rows, long long n, long long stride, int type) {
+  return {at, n * type_bytes(type), rows, stride * type_bytes(type)};
+}
+// Whether the first row of `out`, which is all of it, shares a byte with `in`; between the rows of `in` it may lie.
+inline bool meets(const Region& out, const Region& in) {
+  if (!out.at || !in.at || out.row <= 0 || in.row <= 0) return false;
+  const long long o = (long long)(reinterpret_cast<uintptr_t>(out.at) - reinterpret_cast<uintptr_t>(in.at));
+  const long long i = o < in.row ? 0 : (o - in.row) / in.stride + 1;          // the first row that ends after out begins
+  return i < in.rows && i * in.stride < o + out.row;
+}
+// What a launch writes lies apart from all that it reads, and from what else it writes.
+template <int OUTS, int INS>
+bool apart(const Region (&outs)[OUTS], const Region (&ins)[INS]) {
+  for (int o = 0; o < OUTS; ++o) {
+    for (const Region& in : ins)
+      if (meets(outs[o], in)) return false;
+    for (int p = 0; p < o; ++p)
+      if (meets(outs[o], outs[p])) return false;
+  }
+  return true;
+}
+
 }  // namespace flex

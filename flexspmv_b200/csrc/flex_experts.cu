@@ -615,6 +615,10 @@ int flexspmv_expert_route(const flexspmv_expert_desc* d, const void* const* in, 
   flexspmv_expert_route_bytes(d, &need);
   if (!ws || ws_bytes < need) return FLEXSPMV_ERR_WORKSPACE;
   if (!flex::aligned16(ws)) return FLEXSPMV_ERR_ALIGN;
+  const long long pairs = 4 * d->tokens * d->choices;
+  if (!flex::apart({{out[0], pairs}, {out[1], pairs}, {out[2], 4ll * d->experts + 4}, {out[3], pairs}, {out[4], pairs}, {ws, (long long)need}},
+                   {flex::rows_at(in[0], d->tokens, d->experts, d->in_stride, d->type)}))
+    return FLEXSPMV_ERR_BAD_ARG;
   flex::RouteArgs a = {in[0], d->tokens, d->in_stride, d->experts, d->choices, d->flags & FLEXSPMV_EXPERT_RENORMALIZE, 0,
                        static_cast<float*>(out[0]), static_cast<int*>(out[1]), static_cast<int*>(out[2]), static_cast<int*>(out[3]),
                        static_cast<int*>(out[4]), static_cast<unsigned*>(ws)};
@@ -631,6 +635,10 @@ int flexspmv_expert_route_backward(const flexspmv_expert_desc* d, const void* co
   if (!in || !out) return FLEXSPMV_ERR_BAD_ARG;
   if (d->tokens == 0) return 0;
   if (!in[0] || !in[1] || !in[2] || !in[3] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
+  const long long pairs = 4 * d->tokens * d->choices;
+  if (!flex::apart({{out[0], d->tokens * d->experts * flex::type_bytes(d->type)}},
+                   {{in[0], pairs}, flex::rows_at(in[1], d->tokens, d->experts, d->in_stride, d->type), {in[2], pairs}, {in[3], pairs}}))
+    return FLEXSPMV_ERR_BAD_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int grid = flex::grid_of((d->tokens + 7) / 8, flex::device_sm_count() * 8);
   auto go = [&](auto zero) {
@@ -661,6 +669,9 @@ int flexspmv_expert_combine(const flexspmv_expert_desc* d, const void* const* in
   if (!in || !out) return FLEXSPMV_ERR_BAD_ARG;
   if (d->tokens == 0) return 0;
   if ((d->slots && !in[0]) || !in[1] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
+  const long long pairs = 4 * d->tokens * d->choices;
+  if (!flex::apart({{out[0], 2 * d->tokens * d->n}}, {flex::rows_at(in[0], d->slots, d->n, d->in_stride, d->type), {in[1], pairs}, {in[2], pairs}}))
+    return FLEXSPMV_ERR_BAD_ARG;
   // 16-byte accesses where every row allows them
   const bool wide = d->n % 8 == 0 && d->in_stride % 8 == 0 && flex::aligned16(in[0]) && flex::aligned16(out[0]);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -673,6 +684,11 @@ int flexspmv_expert_combine_backward(const flexspmv_expert_desc* d, const void* 
   if (int e = check_combine(d)) return e;
   if (!in || !out || d->experts < 1 || d->in2_stride < d->n) return FLEXSPMV_ERR_BAD_ARG;
   if (!in[4] || (d->tokens && (!in[0] || !in[2] || !out[1])) || (d->slots && (!in[1] || !out[0]))) return FLEXSPMV_ERR_BAD_ARG;
+  const long long pairs = 4 * d->tokens * d->choices;
+  if (!flex::apart({{out[0], 2 * d->slots * d->n}, {out[1], pairs}},
+                   {flex::rows_at(in[0], d->tokens, d->n, d->in_stride, d->type), flex::rows_at(in[1], d->slots, d->n, d->in2_stride, d->type), {in[2], pairs},
+                    {in[3], pairs}, {in[4], 4ll * d->experts + 4}}))
+    return FLEXSPMV_ERR_BAD_ARG;
   const bool wide = d->n % 8 == 0 && d->in_stride % 8 == 0 && d->in2_stride % 8 == 0 && flex::aligned16(in[0]) && flex::aligned16(in[1]) &&
                     flex::aligned16(out[0]);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

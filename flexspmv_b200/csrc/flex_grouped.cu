@@ -809,6 +809,16 @@ static int check_grouped(const flexspmv_expert_desc* d, int which) {
   return 0;
 }
 
+static bool grouped_apart(const flexspmv_expert_desc* d, int mode, const void* const* in, const int* rows, void* out, void* ws) {
+  const bool dw = mode == kGroupedDw, forward = mode == kGroupedForward;
+  const long long matrices = (long long)d->experts * d->n * d->k, x_rows = rows ? d->tokens : d->slots;
+  const Region results[2] = {{out, dw ? matrices * type_bytes(d->out_type) : 2 * d->slots * (forward ? d->n : d->k)}, {ws, 2 * d->slots * d->k}};
+  Region inputs[4] = {rows_at(in[0], forward ? x_rows : d->slots, forward ? d->k : d->n, d->in_stride, d->type), {in[1], 2 * matrices},
+                      {in[2], 4ll * d->experts + 4}, {rows, 4 * d->slots}};
+  if (dw) inputs[1] = rows_at(in[1], x_rows, d->k, d->in2_stride, d->type);
+  return apart(results, inputs);
+}
+
 // in: forward x, weight, offsets, rows; dx dy, weight, offsets; dw dy, x, offsets, rows
 template <int MODE>
 static int grouped_call(const flexspmv_expert_desc* d, const void* const* in, void* const* out, void* ws, size_t ws_bytes, int32_t* status, void* stream) {
@@ -823,9 +833,13 @@ static int grouped_call(const flexspmv_expert_desc* d, const void* const* in, vo
   GroupedArgs a = {in[0], in[1], static_cast<const int*>(in[2]), rows, out[0], d->tokens, d->slots, d->in_stride, d->in2_stride, d->experts,
                    d->n, d->k, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (kDw && rows && d->slots) {
+  const bool copied = kDw && rows && d->slots;
+  if (copied) {
     if (!ws || ws_bytes < (size_t)d->slots * d->k * 2) return FLEXSPMV_ERR_WORKSPACE;
     if (!aligned16(ws)) return FLEXSPMV_ERR_ALIGN;
+  }
+  if (!grouped_apart(d, MODE, in, rows, out[0], copied ? ws : nullptr)) return FLEXSPMV_ERR_BAD_ARG;
+  if (copied) {
     const int pieces = d->k / 8;
     const long long ctas = ((long long)d->slots * pieces + 1023) / 1024, most = device_sm_count() * 8ll;
     if (int e = launch_pdl(take_rows_kernel, (unsigned)(ctas < most ? ctas : most), 256, 0, st, static_cast<const uint4*>(in[1]), rows, a.offsets,

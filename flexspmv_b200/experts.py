@@ -16,7 +16,7 @@ Results carry no gradient: while gradients are recorded, tensors that require on
 them); only the norm of the last two, as usual, is a plain number.
 
 The operators take CUDA tensors, enqueue on torch's current stream of the tensors' device and never synchronise; the plan stays on the
-device.  Arguments that do not fit raise ``FlexSpmvError``; there is no CPU path.  ``bind(op, *args)`` checks and allocates once and returns
+device.  Arguments that do not fit, an ``out`` that shares memory with an input among them, raise ``FlexSpmvError``; there is no CPU path.  ``bind(op, *args)`` checks and allocates once and returns
 an object whose ``launch()`` is one foreign call on the same tensors, as ``GraphExtension.prepare`` does for graphs: for loops over fixed
 buffers and for capture in a CUDA graph.  Index arrays that do not fit their arrays (offsets that descend, rows out of range) are
 noticed on the device, where nothing is read or written out of range: the next call of a grouped product on the device, or ``check()``, raises.
@@ -202,13 +202,26 @@ def _whole(t: torch.Tensor, name: str):
         raise FlexSpmvError(f"{name} must be contiguous")
 
 
-def _out(out, shape, dtype, device, name="out"):
+def _meets(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether the contiguous ``out`` shares memory with ``t``, whose rows are contiguous; between the rows it may lie."""
+    if out.numel() == 0 or t.numel() == 0:
+        return False
+    size, at = t.element_size(), out.data_ptr() - t.data_ptr()
+    rows, row, stride = (1, t.numel() * size, 1) if t.is_contiguous() else (t.shape[0], t.shape[1] * size, t.stride(0) * size)
+    first = 0 if at < row else (at - row) // stride + 1
+    return first < rows and first * stride < at + out.numel() * out.element_size()
+
+
+def _out(out, shape, dtype, device, **inputs):
     if out is None:
         return torch.empty(shape, dtype=dtype, device=device)
-    _tensor(out, name, (dtype,), len(shape), device.index)
+    _tensor(out, "out", (dtype,), len(shape), device.index)
     if not (tuple(out.shape) == tuple(shape)):
-        raise FlexSpmvError(f"{name} must have the shape {tuple(shape)}, not {tuple(out.shape)}")
-    _whole(out, name)
+        raise FlexSpmvError(f"out must have the shape {tuple(shape)}, not {tuple(out.shape)}")
+    _whole(out, "out")
+    for name, t in inputs.items():
+        if t is not None and _meets(out, t):
+            raise FlexSpmvError(f"out and {name} share memory")
     return out
 
 
@@ -291,7 +304,7 @@ def route_backward(dweights: torch.Tensor, logits: torch.Tensor, plan: Plan, out
           "dweights and the plan must be of the logits' rows")
     _need(plan.offsets.numel() == experts + 1, "the plan must be of the logits' experts")
     _whole(dweights, "dweights")
-    out = _out(out, (tokens, experts), logits.dtype, logits.device)
+    out = _out(out, (tokens, experts), logits.dtype, logits.device, dweights=dweights, logits=logits, weights=plan.weights, experts=plan.experts)
     d = Desc(tokens, tokens * k, experts, k, 0, 0, _TYPE[logits.dtype], 0, _RENORMALIZE if plan.renormalize else 0, 0, stride)
     ins, outs = _pointers((dweights, logits, plan.weights, plan.experts)), _pointers((out,))
     return BoundCall(_function("expert_route_backward", _PLAIN), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs)), dev,
@@ -343,8 +356,9 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     _plan_arrays(offsets, rows, e, dev)
     slots = rows.numel() if rows is not None else x.shape[0]
     _need(slots == 0 or x.shape[0] > 0, "x has no rows to take")
-    out = _out(out, (slots, n), x.dtype, x.device)
-    d = Desc(x.shape[0], slots, e, 0, n, k, _TYPE[x.dtype], _TYPE[x.dtype], 0, 0, _rows_of(x, "x"))
+    stride = _rows_of(x, "x")
+    out = _out(out, (slots, n), x.dtype, x.device, x=x, weight=weight, offsets=offsets, rows=rows)
+    d = Desc(x.shape[0], slots, e, 0, n, k, _TYPE[x.dtype], _TYPE[x.dtype], 0, 0, stride)
     return _grouped("grouped_matmul", d, (x, weight, offsets, rows), out, dev)
 
 
@@ -357,9 +371,9 @@ def grouped_matmul_dx(dy: torch.Tensor, weight: torch.Tensor, offsets: torch.Ten
     if not (dy.shape[1] == n):
         raise FlexSpmvError(f"dy's rows must have {n} values, not {dy.shape[1]}")
     _plan_arrays(offsets, None, e, dev)
-    slots = dy.shape[0]
-    out = _out(out, (slots, k), dy.dtype, dy.device)
-    d = Desc(slots, slots, e, 0, n, k, _TYPE[dy.dtype], _TYPE[dy.dtype], 0, 0, _rows_of(dy, "dy"))
+    slots, stride = dy.shape[0], _rows_of(dy, "dy")
+    out = _out(out, (slots, k), dy.dtype, dy.device, dy=dy, weight=weight, offsets=offsets)
+    d = Desc(slots, slots, e, 0, n, k, _TYPE[dy.dtype], _TYPE[dy.dtype], 0, 0, stride)
     return _grouped("grouped_matmul_dx", d, (dy, weight, offsets), out, dev)
 
 
@@ -382,8 +396,9 @@ def grouped_matmul_dw(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, 
     dtype = dtype or (out.dtype if out is not None else dy.dtype)
     if not (dtype in (torch.float32, dy.dtype)):
         raise FlexSpmvError(f"dw is {dy.dtype} or torch.float32, not {dtype}")
-    out = _out(out, (e, n, k), dtype, dy.device)
-    d = Desc(x.shape[0], slots, e, 0, n, k, _TYPE[dy.dtype], _TYPE[dtype], 0, 0, _rows_of(dy, "dy"), _rows_of(x, "x"))
+    dy_stride, x_stride = _rows_of(dy, "dy"), _rows_of(x, "x")
+    out = _out(out, (e, n, k), dtype, dy.device, dy=dy, x=x, offsets=offsets, rows=rows)
+    d = Desc(x.shape[0], slots, e, 0, n, k, _TYPE[dy.dtype], _TYPE[dtype], 0, 0, dy_stride, x_stride)
     ws = torch.empty(2 * slots * k if rows is not None else 0, dtype=torch.uint8, device=dy.device)          # a copy of x's rows
     return _grouped("grouped_matmul_dw", d, (dy, x, offsets, rows), out, dev, ws)
 
@@ -405,8 +420,9 @@ def combine(z: torch.Tensor, slots: torch.Tensor, weights: Optional[torch.Tensor
     dev = _tensor(z, "z", _HALF, 2)
     _combine_arrays(slots, weights, dev)
     _need(z.shape[1] >= 1, "z must have columns")
-    out = _out(out, (slots.shape[0], z.shape[1]), z.dtype, z.device)
-    d = Desc(slots.shape[0], z.shape[0], 0, slots.shape[1], z.shape[1], 0, _TYPE[z.dtype], 0, 0, 0, _rows_of(z, "z", aligned=False))
+    stride = _rows_of(z, "z", aligned=False)
+    out = _out(out, (slots.shape[0], z.shape[1]), z.dtype, z.device, z=z, slots=slots, weights=weights)
+    d = Desc(slots.shape[0], z.shape[0], 0, slots.shape[1], z.shape[1], 0, _TYPE[z.dtype], 0, 0, 0, stride)
     ins = (ctypes.c_void_p * 3)(z.data_ptr(), slots.data_ptr(), weights.data_ptr() if weights is not None else 0)
     outs = _pointers((out,))
     return BoundCall(_function("expert_combine", _PLAIN), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs)), dev,

@@ -1,0 +1,68 @@
+"""The expert operators' refusal of results that share memory with what a call reads: checked before anything is enqueued, so that
+addresses which nothing reads will do."""
+import ctypes
+import random
+
+import pytest
+import torch
+
+from flexspmv_b200.binding import load_library
+from flexspmv_b200.experts import Desc, _meets
+
+BAD_ARG, FAR = -1, 1 << 32
+SIZES = dict(tokens=16, slots=32, experts=4, choices=2, n=64, k=128, type=1, out_type=1, in_stride=128, in2_stride=136)
+PAIRS, OFFSETS, MATRICES = 16 * 2 * 4, 5 * 4, 4 * 64 * 128 * 2
+
+
+def rows(count, n, stride, size=2):
+    """Bytes from the first row's beginning to the last one's end."""
+    return ((count - 1) * stride + n) * size
+
+
+# of each call: the inputs' and results' lengths in bytes, the workspace last
+CALLS = {
+    "expert_route": ([rows(16, 4, 128)], [PAIRS, PAIRS, OFFSETS, PAIRS, PAIRS, 16]),
+    "expert_route_backward": ([PAIRS, rows(16, 4, 128), PAIRS, PAIRS], [16 * 4 * 2]),
+    "grouped_matmul": ([rows(16, 128, 128), MATRICES, OFFSETS, 32 * 4], [32 * 64 * 2]),
+    "grouped_matmul_dx": ([rows(32, 64, 128), MATRICES, OFFSETS], [32 * 128 * 2]),
+    "grouped_matmul_dw": ([rows(32, 64, 128), rows(16, 128, 136), OFFSETS, 32 * 4], [MATRICES, 32 * 128 * 2]),
+    "expert_combine": ([rows(32, 64, 128), PAIRS, PAIRS], [16 * 64 * 2]),
+    "expert_combine_backward": ([rows(16, 64, 128), rows(32, 64, 136), PAIRS, PAIRS, OFFSETS], [32 * 64 * 2, PAIRS]),
+}
+
+
+def status(name, ins, outs):
+    d = Desc(**SIZES)
+    pointers = lambda p: (ctypes.c_void_p * len(p))(*p)
+    args = [ctypes.byref(d), pointers(ins), pointers(outs)]
+    if name in ("expert_route", "grouped_matmul_dw"):
+        args += [ctypes.c_void_p(outs[-1]), ctypes.c_size_t(1 << 30)]
+    if name.startswith("grouped"):
+        args.append(None)
+    return getattr(load_library(), f"flexspmv_{name}")(*args, None)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_results_that_meet_what_is_read_or_written(name):
+    in_bytes, out_bytes = CALLS[name]
+    ins = [FAR * (1 + i) for i in range(len(in_bytes))]
+    outs = [FAR * (20 + i) for i in range(len(out_bytes))]
+    step = 16                                        # addresses stay on 16 bytes, so that no other check comes first
+    for o, length in enumerate(out_bytes):
+        others = list(zip(ins, in_bytes)) + [(a, n) for i, (a, n) in enumerate(zip(outs, out_bytes)) if i != o]
+        for at, n in others:
+            for place in {at, at + (n - 1) // step * step, at - (length - 1) // step * step}:
+                moved = outs[:o] + [place] + outs[o + 1:]
+                assert status(name, ins, moved) == BAD_ARG, (name, o, at, place)
+
+
+def test_rows_apart():
+    """Against the bytes themselves: what lies between the rows of a strided tensor, and beside it, is free."""
+    r, base = random.Random(0), torch.zeros(4096, dtype=torch.uint8)
+    for _ in range(5000):
+        count, n, start, at, length = r.randint(1, 6), r.randint(1, 9), r.randint(0, 40), r.randint(0, 110), r.randint(1, 30)
+        stride = n + r.randint(0, 5)
+        t, out = base[start:].as_strided((count, n), (stride, 1)), base[at:at + length]
+        held = {start + i * stride + j for i in range(count) for j in range(n)}
+        assert _meets(out, t) == (not held.isdisjoint(range(at, at + length)))
+    assert not _meets(base[:0], base) and not _meets(base, base[:0].view(0, 8))

@@ -12,7 +12,7 @@ from flexspmv_b200 import experts
 from flexspmv_b200.binding import FlexSpmvError
 from flexspmv_b200.expert_layer import RoutedExperts
 
-from test_gpu_experts import normal
+from test_gpu_experts import normal, offsets_of
 
 pytestmark = pytest.mark.gpu
 
@@ -146,4 +146,37 @@ def test_tensors_that_require_a_gradient_are_refused():
         with torch.no_grad():
             call(r)
         call(lambda t: t)
+    experts.check()
+
+
+# ---- results in given memory -------------------------------------------------------------------------------------
+
+def test_outputs_that_share_memory_with_inputs_are_refused():
+    bf = torch.bfloat16
+    x, w, logits = normal(1, (40, 64), bf), normal(2, (4, 64, 64), bf), normal(3, (40, 4), torch.float32)
+    plan = experts.route(logits, 2)
+    g = normal(4, (40, 2), torch.float32)
+    rows, off = plan.rows[:40], offsets_of([7, 0, 20, 13])
+    ones = torch.zeros((40, 1), dtype=torch.int32, device="cuda")
+    wide = normal(5, (41, 128), bf)
+    for bad in (
+        lambda: experts.route_backward(g, logits, plan, out=logits), lambda: experts.grouped_matmul(x, w, off, out=x),
+        lambda: experts.grouped_matmul(x[:39], w, off, out=x[1:]), lambda: experts.grouped_matmul(x, w, off, rows=rows, out=x),
+        lambda: experts.grouped_matmul(x, w, off, out=w.view(-1, 64)[216:]), lambda: experts.grouped_matmul_dx(x, w, off, out=x),
+        lambda: experts.grouped_matmul_dw(x, wide[:40, :64], off, out=wide.view(-1)[:4 * 64 * 64 // 4].view(1, 64, 64).expand(4, 64, 64)),
+        lambda: experts.combine(x, ones, out=x), lambda: experts.bind(experts.grouped_matmul, x, w, off, out=x),
+        lambda: experts.grouped_matmul(wide[:40, :64], w, off, out=wide.view(-1)[64:64 + 40 * 64].view(40, 64)),
+    ):
+        with pytest.raises(FlexSpmvError):
+            bad()
+    # beside the input, and between its rows, it may lie
+    both = torch.cat([x, x])
+    want = experts.grouped_matmul(x, w, off)
+    assert torch.equal(experts.grouped_matmul(both[:40], w, off, out=both[40:]), want)
+    assert torch.equal(experts.grouped_matmul(both[:40], w, off, out=both[40:]), want)
+    one = torch.tensor([0, 1, 1, 1, 1], dtype=torch.int32, device="cuda")
+    first = wide[:40, :64].clone()
+    rows = torch.tensor([3], dtype=torch.int32, device="cuda")
+    got = experts.grouped_matmul(wide[:40, :64], w, one, rows=rows, out=wide[7:8, 64:])
+    assert torch.equal(got, experts.grouped_matmul(first, w, one, rows=rows)) and torch.equal(wide[:40, :64], first)
     experts.check()
