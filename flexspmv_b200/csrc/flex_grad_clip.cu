@@ -8,6 +8,9 @@
 // A thread adds the squares of a piece in 32 bits and the pieces in 64, the CTAs' sums are added in one fixed order: no atomics, the same
 // bits every time.
 #include <cuda_runtime.h>
+#include <stdlib.h>
+
+#include <algorithm>
 
 #include "flex_common.cuh"
 #include "flex_expert_types.cuh"
@@ -189,6 +192,31 @@ __global__ void __launch_bounds__(kClipThreads, kClipCtasPerSm) clip_scale_kerne
   }
 }
 
+// Pieces are scaled in any order: what is written may meet nothing else, other tensors' results as little as other tensors.  Only a tensor and its
+// own result may be the same.
+static int clip_apart(int count, const void* const* grads, const int32_t* types, const int64_t* lengths, void* const* outs, const int32_t* out_types,
+                      const void* ws, size_t ws_bytes) {
+  struct Span { uintptr_t from, to; };
+  Span* const written = static_cast<Span*>(malloc(((size_t)(outs ? count : 0) + 1) * sizeof(Span)));
+  if (!written) return FLEXSPMV_ERR_WORKSPACE;
+  const auto span = [](const void* p, size_t bytes) { return Span{reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes}; };
+  int n = 0;
+  written[n++] = span(ws, ws_bytes);
+  for (int i = 0; outs && i < count; ++i)
+    if (lengths[i]) written[n++] = span(outs[i], (size_t)lengths[i] * type_bytes(out_types[i]));
+  std::sort(written, written + n, [](const Span& a, const Span& b) { return a.from < b.from; });
+  bool good = true;
+  for (int i = 1; i < n; ++i) good &= written[i - 1].to <= written[i].from;
+  for (int i = 0; good && i < count; ++i) {
+    if (!lengths[i] || (outs && outs[i] == grads[i])) continue;
+    const Span in = span(grads[i], (size_t)lengths[i] * type_bytes(types[i]));
+    const Span* const after = std::lower_bound(written, written + n, in.to, [](const Span& a, uintptr_t at) { return a.from < at; });
+    good = after == written || after[-1].to <= in.from;
+  }
+  free(written);
+  return good ? 0 : FLEXSPMV_ERR_BAD_ARG;
+}
+
 static int clip_ctas() { return device_sm_count() * kClipCtasPerSm; }
 
 // Pieces of 4096 elements, larger ones where every CTA would have many.
@@ -240,6 +268,7 @@ int flexspmv_clip_gradients_plan(int32_t count, const void* const* grads, const 
   }
   if (!ws || ws_bytes < z.bytes) return FLEXSPMV_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(ws) & 15u) return FLEXSPMV_ERR_ALIGN;
+  if (int e = flex::clip_apart(count, grads, types, lengths, outs, out_types, ws, z.bytes)) return e;
   flex::ClipTensors t;
   t.piece = reinterpret_cast<flex::ClipPiece*>(static_cast<char*>(ws) + z.piece_at);
   t.size = (int)z.size;

@@ -219,8 +219,9 @@ def _out(out, shape, dtype, device, **inputs):
     if not (tuple(out.shape) == tuple(shape)):
         raise FlexSpmvError(f"out must have the shape {tuple(shape)}, not {tuple(out.shape)}")
     _whole(out, "out")
+    end = out.data_ptr() + out.nbytes
     for name, t in inputs.items():
-        if t is not None and _meets(out, t):
+        if t is not None and t.data_ptr() < end and _meets(out, t):
             raise FlexSpmvError(f"out and {name} share memory")
     return out
 
@@ -498,6 +499,8 @@ def _clip(tensors: list, max_norm: float, outs) -> BoundCall:
     else:
         with torch.cuda.device(dev):
             st = _function("clip_gradients_plan", _CLIP_PLAN)(*plan)
+    if st == -1:
+        raise FlexSpmvError("tensors that are written must not share memory with others", st)
     _check(st, "clip_gradients_plan")
     args = (pieces.value, outs is not None, float(max_norm), norm.data_ptr(), ws.data_ptr(), need.value)
     return PlannedCall(_function("clip_gradients", _CLIP), args, dev, (ws, tensors, outs), norm)
@@ -512,7 +515,7 @@ def grad_norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
 @_operator
 def clip_grad_norm(tensors: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Scales the tensors by ``min(1, max_norm / (norm + 1e-6))``, in place or into ``out`` (tensors of the same lengths, of any of the three
-    types), and returns the norm before it."""
+    types), and returns the norm before it.  No two of them may share memory, but a tensor and its own result."""
     tensors = list(tensors)
     if not (max_norm >= 0):
         raise FlexSpmvError(f"max_norm must not be negative or NaN: {max_norm}")

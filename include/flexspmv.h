@@ -520,7 +520,8 @@ int flexspmv_expert_combine_backward(const flexspmv_expert_desc *desc, const voi
  *   _bytes  the workspace, and the number of pieces that the tensors are cut into
  *   _plan   writes the pieces into the workspace, once for tensors that stay where they are.  grads, types, lengths, outs and out_types are
  *           HOST arrays of count entries, read before the call returns; the tensors are contiguous device memory of any of the three types.
- *           outs null: for the norm alone; outs[i] may be grads[i] of the same type, and is left alone then where the norm is within max_norm
+ *           outs null: for the norm alone; outs[i] may be grads[i] of the same type, and is left alone then where the norm is within max_norm.
+ *           Else what is written, the workspace too, may share no byte with another tensor or result (FLEXSPMV_ERR_BAD_ARG)
  *   flexspmv_clip_gradients  on a planned workspace: *d_norm, and with write != 0 (the plan has outs) the scaled tensors
  * A norm that is not finite scales as the formula says (infinity: 0 and NaN; NaN: NaN).
  */

@@ -66,3 +66,25 @@ def test_rows_apart():
         held = {start + i * stride + j for i in range(count) for j in range(n)}
         assert _meets(out, t) == (not held.isdisjoint(range(at, at + length)))
     assert not _meets(base[:0], base) and not _meets(base, base[:0].view(0, 8))
+
+
+def test_clip_of_tensors_that_meet():
+    """The same tensor twice in place, results that meet one another, another tensor, a part of their own one, or the workspace."""
+    lib, n = load_library(), 3
+    lengths = (ctypes.c_int64 * n)(1000, 0, 500)
+    types, wide = (ctypes.c_int32 * n)(1, 1, 1), (ctypes.c_int32 * n)(0, 0, 0)
+    need, pieces = ctypes.c_size_t(), ctypes.c_int32()
+    assert lib.flexspmv_clip_gradients_bytes(n, lengths, ctypes.byref(need), ctypes.byref(pieces)) == 0
+    ws = FAR * 9
+
+    def plan(grads, outs=None, out_types=types):
+        return lib.flexspmv_clip_gradients_plan(n, (ctypes.c_void_p * n)(*grads), types, lengths, (ctypes.c_void_p * n)(*outs) if outs else None,
+                                                out_types if outs else None, ctypes.c_void_p(ws), need, None)
+    a, b, c = FAR, FAR * 2, FAR * 3
+    for grads, outs, out_types in (
+        ((a, 0, a), (a, 0, a), types), ((a, 0, a + 1998), (a, 0, a + 1998), types), ((a, 0, a - 998), (a, 0, a - 998), types),
+        ((a, 0, b), (c, 0, c), types), ((a, 0, b), (c, 0, c + 1998), types), ((a, 0, b), (c, 0, c + 3996), wide), ((a, 0, b), (b, 0, c), types),
+        ((a, 0, b), (c, 0, a), types), ((a, 0, b), (a + 2, 0, c), types), ((a, 0, b), (a - 2, 0, c), types),
+    ):
+        assert plan(grads, outs, out_types) == BAD_ARG, (grads, outs)
+    assert plan((ws + need.value - 16, 0, b)) == BAD_ARG and plan((a, 0, b), (ws - 1984, 0, c)) == BAD_ARG and plan((a, 0, ws)) == BAD_ARG

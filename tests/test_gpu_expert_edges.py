@@ -180,3 +180,22 @@ def test_outputs_that_share_memory_with_inputs_are_refused():
     got = experts.grouped_matmul(wide[:40, :64], w, one, rows=rows, out=wide[7:8, 64:])
     assert torch.equal(got, experts.grouped_matmul(first, w, one, rows=rows)) and torch.equal(wide[:40, :64], first)
     experts.check()
+
+
+def test_clip_of_tensors_that_share_memory():
+    """A tensor given twice would be scaled once or twice, as its pieces come: refused.  Neighbours in one buffer are scaled each once."""
+    flat = normal(1, (100_000,), torch.float32)
+    a, b = flat[:40_000], flat[40_000:]
+    for bad in (lambda: experts.clip_grad_norm([flat, flat], 1.0), lambda: experts.clip_grad_norm([flat, b], 1.0),
+                lambda: experts.clip_grad_norm([a, b], 1.0, out=[b[:40_000], flat[:60_000].clone()]),
+                lambda: experts.clip_grad_norm([flat[:50_000]], 1.0, out=[flat[4:50_004]]), lambda: experts.bind(experts.clip_grad_norm, [a, a], 1.0)):
+        before = flat.clone()
+        with pytest.raises(FlexSpmvError, match="share"):
+            bad()
+        assert torch.equal(flat, before)
+    twice = float(experts.grad_norm([flat, flat]))                       # nothing is written: both count
+    once = float(flat.double().norm())
+    assert abs(twice - 2 ** 0.5 * once) <= 1e-5 * once
+    before = flat.clone()
+    norm = experts.clip_grad_norm([b, a], 1.0)
+    assert abs(float(norm) - once) <= 1e-5 * once and torch.allclose(flat, before / (once + 1e-6), rtol=1e-5, atol=0)
