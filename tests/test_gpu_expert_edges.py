@@ -199,3 +199,28 @@ def test_clip_of_tensors_that_share_memory():
     before = flat.clone()
     norm = experts.clip_grad_norm([b, a], 1.0)
     assert abs(float(norm) - once) <= 1e-5 * once and torch.allclose(flat, before / (once + 1e-6), rtol=1e-5, atol=0)
+
+
+def test_clip_is_not_bound_inside_a_capture():
+    """Its plan would only be recorded.  The plain call in a capture is, plan and all, and follows the tensors."""
+    ts = [normal(1, (5000,), torch.bfloat16), normal(2, (77,), torch.float32)]
+    outs = [torch.zeros(t.shape, device="cuda") for t in ts]
+    experts.clip_grad_norm(ts, 1.0, out=outs)
+    torch.cuda.synchronize()
+    for bind in (lambda: experts.bind(experts.clip_grad_norm, ts, 1.0, out=outs), lambda: experts.bind(experts.grad_norm, ts)):
+        refused = []
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            try:
+                bind()
+            except FlexSpmvError as e:
+                refused.append(str(e))
+            norm = experts.clip_grad_norm(ts, 1.0, out=outs)
+        assert len(refused) == 1 and "captured" in refused[0]
+        for _ in range(2):
+            for t in ts:
+                t.mul_(2)
+            graph.replay()
+            exact = sum(float((t.double() ** 2).sum()) for t in ts) ** 0.5
+            assert abs(float(norm) - exact) <= 1e-5 * exact
+            assert all(torch.allclose(o, t.float() / (exact + 1e-6), rtol=1e-5) for o, t in zip(outs, ts))
