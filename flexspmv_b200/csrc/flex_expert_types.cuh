@@ -65,6 +65,22 @@ struct Pack {
   // 16-bit values as they are: two of them, or the only one.
   __device__ __forceinline__ uint32_t word(int i) const { return i % 4 == 0 ? raw[i / 4].x : i % 4 == 1 ? raw[i / 4].y : i % 4 == 2 ? raw[i / 4].z : raw[i / 4].w; }
   __device__ __forceinline__ uint32_t bits() const { return *reinterpret_cast<const unsigned short*>(&v[0]); }
+  // The bits of all values, those of 16 bits by two.
+  __device__ __forceinline__ uint32_t all_bits() const {
+    if constexpr (kWide) {
+      uint32_t r = 0;
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) * W / 16; ++i) r |= raw[i].x | raw[i].y | raw[i].z | raw[i].w;
+      return r;
+    } else {
+      uint32_t r = 0;
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if constexpr (sizeof(T) == 4) r |= *reinterpret_cast<const uint32_t*>(&v[i]);
+        else r |= *reinterpret_cast<const unsigned short*>(&v[i]);
+      return r;
+    }
+  }
   __device__ __forceinline__ float get(int i) const { return to_float(v[i]); }
   __device__ __forceinline__ void set(int i, float x) { v[i] = from_float<T>(x); }
 };

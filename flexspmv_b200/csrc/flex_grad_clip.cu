@@ -5,8 +5,8 @@
 // A plan cuts the tensors into pieces and writes a record of each into the workspace, once for tensors that stay where they are.  The pieces
 // go round the CTAs in order; the second of the two launches takes them in the opposite order, so that what the first read last is still in
 // L2.  Bound by memory: the gradients are read twice (the scale needs the whole sum) and the result written once.
-// A thread adds the squares of a piece in 32 bits and the pieces in 64, the CTAs' sums are added in one fixed order: no atomics, the same
-// bits every time.
+// A thread adds the squares of a piece in 32 bits (where those leave its range, once more in 64) and the pieces in 64, the CTAs' sums are
+// added in one fixed order: no atomics, the same bits every time.
 #include <cuda_runtime.h>
 #include <stdlib.h>
 
@@ -55,8 +55,9 @@ __global__ void __launch_bounds__(256) clip_plan_kernel(const __grid_constant__ 
   }
 }
 
+// `bits`: those of all values together, by which a sum of nothing but zeros is known.
 template <class T, int W>
-__device__ __forceinline__ float square_sum(const T* p, int n) {
+__device__ __forceinline__ float square_sum(const T* p, int n, uint32_t& bits) {
   float acc[W];
 #pragma unroll
   for (int i = 0; i < W; ++i) acc[i] = 0.f;
@@ -67,28 +68,62 @@ __device__ __forceinline__ float square_sum(const T* p, int n) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) v[u].load(p + (size_t)(i + u * kClipThreads) * W);
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < 4; ++u) {
+      bits |= v[u].all_bits();
 #pragma unroll
       for (int x = 0; x < W; ++x) acc[x] = fmaf(v[u].get(x), v[u].get(x), acc[x]);
+    }
   }
   for (; i < full; i += kClipThreads) {
     Pack<T, W> v;
     v.load(p + (size_t)i * W);
+    bits |= v.all_bits();
 #pragma unroll
     for (int x = 0; x < W; ++x) acc[x] = fmaf(v.get(x), v.get(x), acc[x]);
   }
-  for (int j = full * W + threadIdx.x; j < n; j += kClipThreads) acc[0] = fmaf(to_float(p[j]), to_float(p[j]), acc[0]);
+  for (int j = full * W + threadIdx.x; j < n; j += kClipThreads) {
+    Pack<T, 1> v;
+    v.load(p + j);
+    bits |= v.all_bits();
+    acc[0] = fmaf(v.get(0), v.get(0), acc[0]);
+  }
   float s = 0.f;
 #pragma unroll
   for (int x = 0; x < W; ++x) s += acc[x];
   return s;
 }
 
+// The same values' squares in 64 bits.
+template <class T, int W>
+__device__ __forceinline__ double square_sum_wide(const T* p, int n) {
+  double s = 0;
+  const int full = n / W * W;
+  for (int i = threadIdx.x * W; i < full; i += kClipThreads * W)
+#pragma unroll 1
+    for (int x = 0; x < W; ++x) {
+      const double d = (double)to_float(p[i + x]);
+      s = fma(d, d, s);
+    }
+  for (int j = full + threadIdx.x; j < n; j += kClipThreads) s = fma((double)to_float(p[j]), (double)to_float(p[j]), s);
+  return s;
+}
+
+template <class T, int W>
+__device__ __forceinline__ double square_sum_as(const T* p, int n) {
+  uint32_t bits = 0;
+  const float s = square_sum<T, W>(p, n, bits);
+  // Squares leave the 32 bits' range from 1.8e19 on (sums of them earlier) and below 1e-19; float16's do not.  A sum inside these bounds has lost
+  // nothing: at most 65536 / 256 squares below 2^-126, each by less than 2^-149.
+  if (std::is_same<T, __half>::value || (s >= 0x1p-100f && s <= 0x1.fffffep127f)) return (double)s;
+  if ((bits & (sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu)) == 0) return 0;
+  return square_sum_wide<T, W>(p, n);
+}
+
 template <class T>
-__device__ __forceinline__ float square_sum_of(const void* in, int n) {
+__device__ __forceinline__ double square_sum_of(const void* in, int n) {
   const T* p = static_cast<const T*>(in);
   // a tensor that does not start on 16 bytes is read a value at a time
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 ? square_sum<T, 16 / (int)sizeof(T)>(p, n) : square_sum<T, 1>(p, n);
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 ? square_sum_as<T, 16 / (int)sizeof(T)>(p, n) : square_sum_as<T, 1>(p, n);
 }
 
 __device__ __forceinline__ double block_sum(double v) {
@@ -114,11 +149,9 @@ __global__ void __launch_bounds__(kClipThreads, kClipCtasPerSm) clip_norm_kernel
     const ClipPiece p = next;
     if (c + (int)gridDim.x < pieces) next = piece[c + gridDim.x];
     const int type = p.types & 3;
-    float s;
-    if (type == FLEXSPMV_TYPE_F32) s = square_sum_of<float>(p.in, p.length);
-    else if (type == FLEXSPMV_TYPE_BF16) s = square_sum_of<__nv_bfloat16>(p.in, p.length);
-    else s = square_sum_of<__half>(p.in, p.length);
-    sum += (double)s;
+    if (type == FLEXSPMV_TYPE_F32) sum += square_sum_of<float>(p.in, p.length);
+    else if (type == FLEXSPMV_TYPE_BF16) sum += square_sum_of<__nv_bfloat16>(p.in, p.length);
+    else sum += square_sum_of<__half>(p.in, p.length);
   }
   sum = block_sum(sum);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;

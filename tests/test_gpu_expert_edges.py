@@ -224,3 +224,33 @@ def test_clip_is_not_bound_inside_a_capture():
             exact = sum(float((t.double() ** 2).sum()) for t in ts) ** 0.5
             assert abs(float(norm) - exact) <= 1e-5 * exact
             assert all(torch.allclose(o, t.float() / (exact + 1e-6), rtol=1e-5) for o, t in zip(outs, ts))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norm_of_values_whose_squares_leave_32_bits(dtype):
+    """Finite gradients have a finite norm as far as 32 bits hold it.  A thread adds at most 256 squares, in 32 bits or in 64, and the rest in 64:
+    256 * 2^-24 and a square root's rounding."""
+    tol = 300 * 2.0 ** -24
+    for scales in ([1e20], [1e-25], [3e37, 1.0], [1e-30, 1e-38], [2e18, 1e18], [1e-22, 0.0], [1e-19, 1e-19], [1e20, 1e-25, 1.0, 0.0], [0.0]):
+        for length in (1, 4099, 300_001):
+            ts = [normal(i, (length + i,), torch.float32).mul_(s * (0.1 if s > 1e30 else 1.0)).to(dtype)[i % 2:] for i, s in enumerate(scales)]
+            exact = sum(float((t.double() ** 2).sum()) for t in ts) ** 0.5
+            if exact > 3e38:
+                continue
+            norm = experts.grad_norm(ts)
+            assert abs(float(norm) - exact) <= tol * exact, (scales, length)
+            for max_norm in (1.0, exact / 3):
+                if max_norm == 0.0:
+                    continue
+                mine = [t.clone() for t in ts]
+                assert torch.equal(experts.clip_grad_norm(mine, max_norm), norm)
+                scale = min(1.0, max_norm / (exact + 1e-6))
+                half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+                # below the types' normal range a rounding is up to half of their smallest value, 2^-149 or 2^-133; the scale, too, is held in 32 bits
+                low = 2.0 ** -149 if dtype == torch.float32 else 2.0 ** -133
+                for t, m in zip(ts, mine):
+                    want = t.double() * scale
+                    bound = (1.01 * half + tol + 2.0 ** -22 + 2.0 ** -149 / scale) * want.abs() + low
+                    assert bool(((m.double() - want).abs() <= bound).all()), (scales, length, max_norm)
+    beyond = [torch.full((300_000,), 3e38, device="cuda").to(dtype)]
+    assert float(experts.grad_norm(beyond)) == float("inf")
