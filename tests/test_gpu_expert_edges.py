@@ -12,7 +12,7 @@ from flexspmv_b200 import experts
 from flexspmv_b200.binding import FlexSpmvError
 from flexspmv_b200.expert_layer import RoutedExperts
 
-from test_gpu_experts import normal, offsets_of
+from test_gpu_experts import HALF, normal, offsets_of
 
 pytestmark = pytest.mark.gpu
 
@@ -254,3 +254,38 @@ def test_norm_of_values_whose_squares_leave_32_bits(dtype):
                     assert bool(((m.double() - want).abs() <= bound).all()), (scales, length, max_norm)
     beyond = [torch.full((300_000,), 3e38, device="cuda").to(dtype)]
     assert float(experts.grad_norm(beyond)) == float("inf")
+
+
+# ---- logits far apart --------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,k", [(2, 2), (8, 8), (16, 4), (64, 32), (300, 32)])
+def test_route_of_logits_far_apart(n, k, dtype):
+    """Weights to the bound that near logits have, (n + 8) * 2^-23 of each, however small: a power of a difference as rounded would be off by as many
+    units as the difference has.  The sum's terms count by what they are, so that their powers' d * 2^-23 stays below one of its n units."""
+    for tokens in (5, 700):
+        logits = (torch.rand((tokens, n), generator=torch.Generator(device="cuda").manual_seed(n), device="cuda") * 80 - 40).to(dtype)
+        logits[0] = torch.linspace(-40.1, 39.7, n, device="cuda").to(dtype)
+        logits[1] = torch.linspace(0.3, -79.9, n, device="cuda").to(dtype)
+        l = logits.double().cpu().numpy()
+        ids = np.argsort(-l, axis=1, kind="stable")[:, :k]
+        for renormalize in (False, True):
+            plan = experts.route(logits, k, renormalize=renormalize)
+            assert np.array_equal(plan.experts.cpu().numpy(), ids)
+            e = np.exp(l - l.max(1, keepdims=True))
+            top = np.take_along_axis(e, ids, axis=1)
+            want = top / (top if renormalize else e).sum(1, keepdims=True)
+            assert np.all(np.abs(plan.weights.double().cpu().numpy() - want) <= (n + 8) * 2.0 ** -23 * want + 1e-37)
+            g = normal(7, (tokens, k), torch.float32)
+            got = experts.route_backward(g, logits, plan).double().cpu().numpy()
+            p, gd = e / e.sum(1, keepdims=True), np.zeros_like(l)
+            np.put_along_axis(gd, ids, g.double().cpu().numpy(), axis=1)
+            gw = np.take_along_axis(gd, ids, axis=1) * want
+            mean, size = gw.sum(1, keepdims=True), np.abs(gw).sum(1, keepdims=True)
+            if renormalize:
+                p = np.zeros_like(l)
+                np.put_along_axis(p, ids, want, axis=1)
+            bound = (n + k + 24) * 2.0 ** -23 * p * (np.abs(gd) + size) + 1e-37
+            if dtype != torch.float32:                 # one rounding, and float16's smallest values
+                bound += HALF[dtype] * 1.01 * np.abs(p * (gd - mean)) + (2.0 ** -25 if dtype == torch.float16 else 0)
+            assert np.all(np.abs(got - p * (gd - mean)) <= bound)
