@@ -72,9 +72,12 @@ constexpr int kGatherWarps = 4;
 constexpr int grouped_threads(bool gather) { return kGroupedThreads + (gather ? kGatherWarps * 32 : 0); }
 constexpr int kTileBytesA = 128 * 128;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
-// The tensor cores cut a sum's low bits at every addition, 2^-24 of it and always towards zero: relative errors of 1e-6 after 1024 rows and 1e-5 after
-// 10 000, lost in a result of 16 bits but not in one of 32.  So that one is added up, correctly rounded, from parts of this many steps (512 rows).
-constexpr int kPartSteps = 8;
+// The tensor cores cut a sum's low bits at every addition, always towards zero: a relative error of 4e-9 to 6e-9 a row where all products have one sign
+// (1e-9 of random ones).  PARTS (dw): sums are added up, correctly rounded, from parts of so many steps that the result does not show it.  Of 32 bits:
+// always, from 512 rows each.  Of 16, whose half unit is 2.4e-4 of a float16 and 2e-3 of a bfloat16 at the least: from 4096 (2e-5), where there are more rows
+// than keep a whole sum below 0.4 of that.  A kernel of its own, since the sums' registers cost all others 2 - 10 %.
+constexpr int kPartSteps32 = 8, kPartSteps16 = 64;
+template <class T> constexpr int kWholeRows = std::is_same<T, __half>::value ? 16384 : 131072;
 
 template <int MODE, int NT, int PAIR, int HALVES, int OUT_BYTES>
 struct GroupedCfg {
@@ -143,7 +146,7 @@ __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const Group
   return r;
 }
 
-template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER>
+template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER, bool PARTS>
 __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                      const __grid_constant__ CUtensorMap row_a, const __grid_constant__ CUtensorMap row_b,
                                                                      const __grid_constant__ CUtensorMap map_out,
@@ -159,7 +162,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   const int rank = PAIR == 2 ? (int)cluster_rank() : 0;
   const int split = SPLIT ? (int)cluster_size() : 1, share = SPLIT ? (int)cluster_rank() : 0;
   constexpr bool kA_mn = MODE != kGroupedForward, kB_mn = MODE == kGroupedDw;
-  constexpr bool kInParts = sizeof(TO) == 4;
+  constexpr int kPartSteps = sizeof(TO) == 4 ? kPartSteps32 : kPartSteps16;
 
   if (tid == 0) {
     for (int i = 0; i < Cfg::kStages; ++i) {
@@ -381,8 +384,8 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           continue;
         }
         for (int s = from; s < to; ++s) {
-          const bool begins = s == from || (kInParts && (s - from) % kPartSteps == 0);
-          const bool ends = s + 1 == to || (kInParts && (s + 1 - from) % kPartSteps == 0);
+          const bool begins = s == from || (PARTS && (s - from) % kPartSteps == 0);
+          const bool ends = s + 1 == to || (PARTS && (s + 1 - from) % kPartSteps == 0);
           if (begins) {
             if (!wait(&bars.acc_empty[acc], acc_phase ^ 1)) break;
             tmem_fence_after();
@@ -483,13 +486,13 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           else mbar_arrive(&bars.acc_empty[acc]);
         }
       };
-      // 32-bit results: this warp's four times 32 columns, added up from the parts
-      float sum[kInParts ? NT / 64 : 1][32];
-      if (kInParts) {
+      // this warp's four times 32 columns, added up from the parts
+      float sum[PARTS ? NT / 64 : 1][32];
+      if (PARTS) {
 #pragma unroll
         for (int g = 0; g < NT / 64; ++g)
 #pragma unroll
-          for (int x = 0; x < 32; ++x) sum[kInParts ? g : 0][x] = 0.f;
+          for (int x = 0; x < 32; ++x) sum[PARTS ? g : 0][x] = 0.f;
         bool there = true;
         for (int s = from; s < to && there; s += kPartSteps) {
           there = wait_warp(&bars.acc_full[acc], acc_phase);
@@ -502,20 +505,20 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
               uint32_t v[32];
               tmem_load32(d + g * 64, v);
 #pragma unroll
-              for (int x = 0; x < 32; ++x) sum[kInParts ? g : 0][x] += __uint_as_float(v[x]);
+              for (int x = 0; x < 32; ++x) sum[PARTS ? g : 0][x] += __uint_as_float(v[x]);
             }
           free_accumulator();
           if (++acc == 2) { acc = 0; acc_phase ^= 1; }
         }
         if (!there) break;
       }
-      if (SPLIT && kInParts) {
+      if (SPLIT && PARTS) {
         float* const sums = reinterpret_cast<float*>(base);
 #pragma unroll
         for (int g = 0; g < NT / 64; ++g)
           if (part * 32 + g * 64 < t.cols)
 #pragma unroll
-            for (int x = 0; x < 32; ++x) sums[(part * 32 + g * 64 + x) * 128 + quarter * 32 + lane] = sum[kInParts ? g : 0][x];
+            for (int x = 0; x < 32; ++x) sums[(part * 32 + g * 64 + x) * 128 + quarter * 32 + lane] = sum[PARTS ? g : 0][x];
         break;
       }
       if (SPLIT) {
@@ -557,7 +560,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
         __syncwarp();
         if (lane == 0 && m < a.n && t.n0 + c0 < a.k) tma_store_3d(&map_out, mine, t.n0 + c0, m, t.e);
       };
-      if constexpr (kInParts) {
+      if constexpr (PARTS) {
 #pragma unroll
         for (int g = 0; g < NT / 64; ++g)
           if (part * 32 + g * 64 < t.cols) store_rows(part * 32 + g * 64, [&](int x) { return sum[g][x]; });
@@ -702,7 +705,7 @@ static int grouped_smem(int experts) {
 }
 
 // `split`: CTAs that share a tile, `grid` of them altogether; 1: whole tiles.
-template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER>
+template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER, bool PARTS>
 static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStream_t st) {
   constexpr CUtensorMapDataType kIn = std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap ma, mb, row_a, row_b, out;
@@ -736,7 +739,7 @@ static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStre
     row_b = mb;
   }
   const int smem = grouped_smem<MODE, NT, PAIR, HALVES, (int)sizeof(TO)>(a.experts);
-  constexpr auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR, HALVES, SPLIT, GATHER>;
+  constexpr auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR, HALVES, SPLIT, GATHER, PARTS>;
   if (int e = allow_smem<kernel>(smem)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3((unsigned)grouped_threads(GATHER)); cfg.dynamicSmemBytes = smem; cfg.stream = st;
@@ -749,7 +752,7 @@ static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStre
   return (int)cudaLaunchKernelEx(&cfg, kernel, ma, mb, row_a, row_b, out, a);
 }
 
-template <class T, class TO, int MODE, int NT, int PAIR, bool GATHER>
+template <class T, class TO, int MODE, int NT, int PAIR, bool GATHER, bool PARTS = false>
 static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
   const int sms = device_sm_count();
   // tiles of 128 rows, no more than these whatever the groups are
@@ -760,30 +763,33 @@ static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
   // What dividing saves is most of a tile's steps, 0.3 us each (a narrow tile's 0.13); what it costs is the parts' meeting, about 5 us (1.5).
   // us, whole / divided: 8 rows, one expert of 2048 x 4096 17.4 / 9.4; dw of 8192 rows, 1024 x 1024 43.8 / 22; but 4096 rows, two experts of
   // 512 x 512 (8 steps) 9.8 / 12.6.
-  constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, 1, true, GATHER>;
+  constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, 1, true, GATHER, PARTS>;
   const int smem = grouped_smem<MODE, NT, 1, 1, (int)sizeof(TO)>(a.experts);
   for (int split = 8; split > 1; split /= 2) {
     if (most * split > sms || steps - steps / split < (NT > 64 ? 20 : 12)) continue;
     if (int e = allow_smem<divided>(smem)) return e;
-    if (most <= clusters_at_once<divided, grouped_threads(GATHER)>(split, smem)) return grouped_launch_as<T, TO, MODE, NT, 1, 1, true, GATHER>(a, (int)most * split, split, st);
+    if (most <= clusters_at_once<divided, grouped_threads(GATHER)>(split, smem)) return grouped_launch_as<T, TO, MODE, NT, 1, 1, true, GATHER, PARTS>(a, (int)most * split, split, st);
   }
   // Tiles of both accumulators (HALVES = 2): a quarter less between L2 and the SMs for a tile's step, a stage less under way, and the end of a tile's
   // sum that only half of it is behind.  It pays where the sums are long and the tiles go round the pairs, most with gathered rows, which are gathered
   // half as often.  us, one / both: 32 768 rows, 32 experts of 4096 x 2048, with a list 437 / 419, without 411 / 413, dw 418 / 410, dx 411 / 419;
   // 10 599 rows, 8 experts of 1488 x 2792 87.6 / 75.7; 8192 x 8192 x 8192 737 / 688; but 8192 rows of 328 85 / 89, 4102 rows of 2048 28 / 30.
-  if constexpr (NT > 64 && sizeof(TO) == 2 && MODE != kGroupedDx) {
+  if constexpr (NT > 64 && !PARTS && MODE != kGroupedDx) {
     const long long columns = MODE == kGroupedDw ? (long long)a.experts * ((a.k + NT - 1) / NT) : a.slots / NT + a.experts / 2;          // of tiles, about
     const int long_sum = MODE == kGroupedDw ? 16 : GATHER ? 32 : 40, half_rounds = MODE == kGroupedDw ? 20 : 3;
     if (steps >= long_sum && columns * ((a.n + 511) / 512) * 2 >= half_rounds * (sms / 2))
-      return grouped_launch_as<T, TO, MODE, NT, 2, 2, false, GATHER>(a, sms / 2 * 2, 1, st);
+      return grouped_launch_as<T, TO, MODE, NT, 2, 2, false, GATHER, false>(a, sms / 2 * 2, 1, st);
   }
-  return grouped_launch_as<T, TO, MODE, NT, PAIR, 1, false, GATHER>(a, sms / PAIR * PAIR, 1, st);
+  return grouped_launch_as<T, TO, MODE, NT, PAIR, 1, false, GATHER, PARTS>(a, sms / PAIR * PAIR, 1, st);
 }
 
 template <class T, class TO, int MODE, bool GATHER>
 static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
   if constexpr (MODE == kGroupedDw) {
-    return grouped_tiles<T, TO, MODE, 256, 2, GATHER>(a, st);
+    // us, whole / in parts: 200 000 rows of 2048 x 2048 in float16 1160 / 1195, 600 000 of 512 x 512 512 / 540, 102 400 in 32 such groups 591 / 597
+    if constexpr (sizeof(TO) == 2)
+      if (a.slots <= kWholeRows<T>) return grouped_tiles<T, TO, MODE, 256, 2, GATHER, false>(a, st);
+    return grouped_tiles<T, TO, MODE, 256, 2, GATHER, true>(a, st);
   } else {
     // Tiles of 64 places and single CTAs for up to 32 places an expert on average: more of the weights on their way at once.  us, 64 / 256 places:
     // 16 an expert, 64 experts of 1408 x 2048 59.8 / 66.8; 32 experts of 2048 x 2048, 32 an expert 47.0 / 49.7, 48 51.0 / 50.5, 128 72.1 / 54.9.

@@ -289,3 +289,38 @@ def test_route_of_logits_far_apart(n, k, dtype):
             if dtype != torch.float32:                 # one rounding, and float16's smallest values
                 bound += HALF[dtype] * 1.01 * np.abs(p * (gd - mean)) + (2.0 ** -25 if dtype == torch.float16 else 0)
             assert np.all(np.abs(got - p * (gd - mean)) <= bound)
+
+
+# ---- long sums ---------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,counts,n,k", [
+    (torch.float16, [600_000], 72, 64),                        # a cluster divides the sum
+    (torch.float16, [3, 70_000, 0, 600_000, 65_536, 65_600, 1], 136, 264),
+    (torch.float16, [200_000, 17], 2048, 1024),                # tiles that go round the pairs
+    (torch.bfloat16, [4_000_000], 72, 64),
+    (torch.bfloat16, [100, 3_000_000], 520, 8),
+    (torch.float16, [16_384, 16_448, 40, 8000], 264, 136),
+])
+def test_dw_in_16_bits_over_many_rows(dtype, counts, n, k):
+    """Rows of one sign, of which the matrix instructions' cut sums fall short the more the longer they are.  With more than 16 384 (131 072) rows all
+    sums are in parts of 4096: 256 instructions that cut two units at most, then the parts' correctly rounded additions."""
+    slots = sum(counts)
+    g = torch.Generator(device="cuda").manual_seed(slots)
+    x, dy = torch.empty((slots, k), dtype=dtype, device="cuda"), torch.empty((slots, n), dtype=dtype, device="cuda")
+    for at in range(0, slots, 100_000):
+        x[at:at + 100_000] = torch.rand(x[at:at + 100_000].shape, generator=g, device="cuda") + 0.5
+        dy[at:at + 100_000] = (torch.rand(dy[at:at + 100_000].shape, generator=g, device="cuda") + 0.5) * 2.0 ** -8
+    dw = experts.grouped_matmul_dw(dy, x, offsets_of(counts))
+    experts.check()
+    long = 16_384 if dtype == torch.float16 else 131_072
+    at, columns = 0, slice(0, 64)
+    for e, c in enumerate(counts):
+        want = torch.zeros((n, min(k, 64)), dtype=torch.float64, device="cuda")
+        for b in range(at, at + c, 100_000):
+            rows = slice(b, min(b + 100_000, at + c))
+            want += dy[rows].double().t() @ x[rows, columns].double()
+        at += c
+        got = dw[e, :, columns].double()
+        cut = (512 + c / 8192 if c > long else c) * 2.0 ** -23
+        low = 2.0 ** -25 if dtype == torch.float16 else 0.0
+        assert bool(((got - want).abs() <= (cut + 1.01 * HALF[dtype]) * want + low).all()), (e, c)
