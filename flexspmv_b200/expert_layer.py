@@ -108,7 +108,10 @@ class RoutedExperts(nn.Module):
 
     def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``x`` (tokens, width).  ``mask`` (tokens) bool: tokens that are there; the others take no expert and give zeros."""
-        logits = x.float() @ self.router.t()
+        rows = x.float()
+        if mask is not None:                     # whatever lies there: a row's gradient of zeros times a NaN would be one in the router's
+            rows = rows.masked_fill(~mask[:, None], 0.0)
+        logits = rows @ self.router.t()
         if mask is not None:
             logits = logits.masked_fill(~mask[:, None], float("-inf"))
         plan = route(logits, self.k, renormalize=True)

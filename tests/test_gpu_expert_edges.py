@@ -324,3 +324,24 @@ def test_dw_in_16_bits_over_many_rows(dtype, counts, n, k):
         cut = (512 + c / 8192 if c > long else c) * 2.0 ** -23
         low = 2.0 ** -25 if dtype == torch.float16 else 0.0
         assert bool(((got - want).abs() <= (cut + 1.01 * HALF[dtype]) * want + low).all()), (e, c)
+
+
+def test_layer_where_masked_tokens_hold_anything():
+    """NaN and infinity in tokens that the mask leaves out reach neither the result nor a gradient."""
+    layer = RoutedExperts(64, 128, 8, 2, generator=torch.Generator(device="cuda").manual_seed(1))
+    clean = normal(2, (300, 64), torch.bfloat16)
+    mask = torch.rand(300, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda") < 0.7
+    dirty = clean.clone()
+    dirty[~mask] = float("nan")
+    dirty[torch.nonzero(~mask)[0]] = float("inf")
+    dy = normal(4, (300, 64), torch.bfloat16)
+    results = []
+    for x in (clean, dirty):
+        x = x.clone().requires_grad_()
+        layer.zero_grad()
+        y = layer(x, mask)
+        y.backward(dy)
+        results.append([y.detach(), x.grad] + [p.grad.clone() for p in layer.parameters()])
+    experts.check()
+    assert not results[1][0][~mask].any() and not results[1][1][~mask].any()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
