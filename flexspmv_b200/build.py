@@ -27,6 +27,7 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-fmad=false",            # one IEEE operation per map operation, as the reference CPU code evaluates it
     "--expt-relaxed-constexpr", "-diag-suppress", "177", "-Xcompiler", "-fPIC", "-Xcompiler", "-O2",
+    "-Xcompiler", "-fno-gnu-unique",      # what a template keeps (shared memory asked for, CTAs that fit) is its library's own, not the process's
     "-I", CSRC, "-I", os.path.join(ROOT, "include"),
 ] + os.environ.get("FLEXSPMV_NVCC_EXTRA", "").split()
 

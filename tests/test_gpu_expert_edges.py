@@ -3,12 +3,13 @@
 Bounds as in ``test_gpu_experts``: n additions in 32 bits err by at most n * 2^-23 of the sum of magnitudes, one rounding to 16 bits by half a
 unit (2^-8 of a bfloat16, 2^-11 of a float16); what is in whole numbers is equal."""
 import gc
+import shutil
 
 import numpy as np
 import pytest
 import torch
 
-from flexspmv_b200 import experts
+from flexspmv_b200 import binding, experts
 from flexspmv_b200.binding import FlexSpmvError
 from flexspmv_b200.expert_layer import RoutedExperts
 
@@ -345,3 +346,16 @@ def test_layer_where_masked_tokens_hold_anything():
     experts.check()
     assert not results[1][0][~mask].any() and not results[1][1][~mask].any()
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_two_copies_of_the_library(tmp_path, monkeypatch):
+    """load_library takes a path: each copy in a process asks for its own kernels' shared memory."""
+    x, w, off = normal(1, (300, 256), torch.bfloat16), normal(2, (3, 128, 256), torch.bfloat16), offsets_of([100, 0, 200])
+    logits = normal(3, (5000, 256), torch.float32)
+    want = experts.grouped_matmul(x, w, off), experts.route(logits, 8).slots
+    path = str(shutil.copy(binding.DEFAULT_LIB, tmp_path / "copy.so"))
+    lib = binding.load_library(path)
+    monkeypatch.setattr(experts, "load_library", lambda: lib)
+    monkeypatch.setattr(experts, "_functions", {})
+    assert torch.equal(experts.grouped_matmul(x, w, off), want[0]) and torch.equal(experts.route(logits, 8).slots, want[1])
+    experts.check()
