@@ -100,6 +100,9 @@ int allow_smem(int bytes) {
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Whether every array begins on a value of so many bytes; null ones do.
+template <class... P>
+bool aligned_to(int bytes, P... p) { return (((reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) | ...) == 0); }
 inline bool known_type(int t) { return t == FLEXSPMV_TYPE_F32 || t == FLEXSPMV_TYPE_BF16 || t == FLEXSPMV_TYPE_F16; }
 inline int type_bytes(int t) { return t == FLEXSPMV_TYPE_F32 ? 4 : 2; }
 

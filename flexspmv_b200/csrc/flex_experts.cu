@@ -630,7 +630,8 @@ int flexspmv_expert_route(const flexspmv_expert_desc* d, const void* const* in, 
   size_t need = 0;
   flexspmv_expert_route_bytes(d, &need);
   if (!ws || ws_bytes < need) return FLEXSPMV_ERR_WORKSPACE;
-  if (!flex::aligned16(ws)) return FLEXSPMV_ERR_ALIGN;
+  if (!flex::aligned16(ws) || !flex::aligned_to(flex::type_bytes(d->type), in[0]) || !flex::aligned_to(4, out[0], out[1], out[2], out[3], out[4]))
+    return FLEXSPMV_ERR_ALIGN;
   const long long pairs = 4 * d->tokens * d->choices;
   if (!flex::apart({{out[0], pairs}, {out[1], pairs}, {out[2], 4ll * d->experts + 4}, {out[3], pairs}, {out[4], pairs}, {ws, (long long)need}},
                    {flex::rows_at(in[0], d->tokens, d->experts, d->in_stride, d->type)}))
@@ -651,6 +652,7 @@ int flexspmv_expert_route_backward(const flexspmv_expert_desc* d, const void* co
   if (!in || !out) return FLEXSPMV_ERR_BAD_ARG;
   if (d->tokens == 0) return 0;
   if (!in[0] || !in[1] || !in[2] || !in[3] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
+  if (!flex::aligned_to(flex::type_bytes(d->type), in[1], out[0]) || !flex::aligned_to(4, in[0], in[2], in[3])) return FLEXSPMV_ERR_ALIGN;
   const long long pairs = 4 * d->tokens * d->choices;
   if (!flex::apart({{out[0], d->tokens * d->experts * flex::type_bytes(d->type)}},
                    {{in[0], pairs}, flex::rows_at(in[1], d->tokens, d->experts, d->in_stride, d->type), {in[2], pairs}, {in[3], pairs}}))
@@ -685,6 +687,7 @@ int flexspmv_expert_combine(const flexspmv_expert_desc* d, const void* const* in
   if (!in || !out) return FLEXSPMV_ERR_BAD_ARG;
   if (d->tokens == 0) return 0;
   if ((d->slots && !in[0]) || !in[1] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
+  if (!flex::aligned_to(2, in[0], out[0]) || !flex::aligned_to(4, in[1], in[2])) return FLEXSPMV_ERR_ALIGN;
   const long long pairs = 4 * d->tokens * d->choices;
   if (!flex::apart({{out[0], 2 * d->tokens * d->n}}, {flex::rows_at(in[0], d->slots, d->n, d->in_stride, d->type), {in[1], pairs}, {in[2], pairs}}))
     return FLEXSPMV_ERR_BAD_ARG;
@@ -700,6 +703,7 @@ int flexspmv_expert_combine_backward(const flexspmv_expert_desc* d, const void* 
   if (int e = check_combine(d)) return e;
   if (!in || !out || d->experts < 1 || d->in2_stride < d->n) return FLEXSPMV_ERR_BAD_ARG;
   if (!in[4] || (d->tokens && (!in[0] || !in[2] || !out[1])) || (d->slots && (!in[1] || !out[0]))) return FLEXSPMV_ERR_BAD_ARG;
+  if (!flex::aligned_to(2, in[0], in[1], out[0]) || !flex::aligned_to(4, in[2], in[3], in[4], out[1])) return FLEXSPMV_ERR_ALIGN;
   const long long pairs = 4 * d->tokens * d->choices;
   if (!flex::apart({{out[0], 2 * d->slots * d->n}, {out[1], pairs}},
                    {flex::rows_at(in[0], d->tokens, d->n, d->in_stride, d->type), flex::rows_at(in[1], d->slots, d->n, d->in2_stride, d->type), {in[2], pairs},

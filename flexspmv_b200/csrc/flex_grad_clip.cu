@@ -325,6 +325,7 @@ int flexspmv_clip_gradients(int32_t pieces, int32_t write, float max_norm, float
   const int most = flex::clip_ctas();
   if (pieces < 0 || !norm) return FLEXSPMV_ERR_BAD_ARG;
   if (!ws || ws_bytes < (size_t)most * sizeof(double) + (size_t)pieces * sizeof(flex::ClipPiece)) return FLEXSPMV_ERR_WORKSPACE;
+  if (!flex::aligned16(ws) || !flex::aligned_to(4, norm)) return FLEXSPMV_ERR_ALIGN;
   double* const partial = static_cast<double*>(ws);
   const flex::ClipPiece* const piece = reinterpret_cast<const flex::ClipPiece*>(static_cast<char*>(ws) + (size_t)most * sizeof(double));
   const int ctas = pieces < 1 ? 1 : pieces < most ? pieces : most;

@@ -835,7 +835,7 @@ static int grouped_call(const flexspmv_expert_desc* d, const void* const* in, vo
   const int* const rows = kDx ? nullptr : static_cast<const int*>(in[3]);
   if (!in[2] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
   if (d->slots && (!in[0] || !in[1] || (!kDx && d->tokens < (rows ? 1 : d->slots)))) return FLEXSPMV_ERR_BAD_ARG;
-  if (!aligned16(in[0]) || !aligned16(in[1]) || !aligned16(out[0])) return FLEXSPMV_ERR_ALIGN;
+  if (!aligned16(in[0]) || !aligned16(in[1]) || !aligned16(out[0]) || !aligned_to(4, in[2], rows, status)) return FLEXSPMV_ERR_ALIGN;
   GroupedArgs a = {in[0], in[1], static_cast<const int*>(in[2]), rows, out[0], d->tokens, d->slots, d->in_stride, d->in2_stride, d->experts,
                    d->n, d->k, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -453,7 +453,7 @@ int flexspmv_spmv_f64_static_device_status(int32_t *d_status_out, void *stream);
  *
  * All matrices are row-major with contiguous rows of 16-bit values (FLEXSPMV_TYPE_BF16 or _F16); sums, softmax statistics and weights are
  * 32-bit floats; index arrays are int32.  What a call writes (its workspace too) may share no byte with what it reads or else writes
- * (FLEXSPMV_ERR_BAD_ARG); clipping has its own rule.  `slots` in the descriptor is the number of (token, choice) pairs; pairs that have no expert
+ * (FLEXSPMV_ERR_BAD_ARG); clipping has its own rule.  Every array begins on a value of its type, a workspace on 16 bytes (FLEXSPMV_ERR_ALIGN).  `slots` in the descriptor is the number of (token, choice) pairs; pairs that have no expert
  * (all of the row's other logits are -infinity) take no place, so offsets[experts] may be less.
  */
 enum { FLEXSPMV_TYPE_F32 = 0, FLEXSPMV_TYPE_BF16 = 1, FLEXSPMV_TYPE_F16 = 2 };

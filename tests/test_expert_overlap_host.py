@@ -88,3 +88,29 @@ def test_clip_of_tensors_that_meet():
     ):
         assert plan(grads, outs, out_types) == BAD_ARG, (grads, outs)
     assert plan((ws + need.value - 16, 0, b)) == BAD_ARG and plan((a, 0, b), (ws - 1984, 0, c)) == BAD_ARG and plan((a, 0, ws)) == BAD_ARG
+
+
+ALIGN = -2
+# bytes of a value, in the order of CALLS: bfloat16 in and out, 32-bit weights and indices; the products' matrices begin on 16 bytes
+VALUES = {
+    "expert_route": ([2], [4] * 5 + [16]), "expert_route_backward": ([4, 2, 4, 4], [2]), "grouped_matmul": ([16, 16, 4, 4], [16]),
+    "grouped_matmul_dx": ([16, 16, 4], [16]), "grouped_matmul_dw": ([16, 16, 4, 4], [16, 16]), "expert_combine": ([2, 4, 4], [2]),
+    "expert_combine_backward": ([2, 2, 4, 4, 4], [2, 4]),
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_arrays_that_begin_inside_a_value(name):
+    in_bytes, out_bytes = CALLS[name]
+    base = [FAR * (1 + i) for i in range(len(in_bytes) + len(out_bytes))]
+    for i, value in enumerate(VALUES[name][0] + VALUES[name][1]):
+        for off in {1, value // 2, value - 1}:
+            at = list(base)
+            at[i] += off
+            assert status(name, at[:len(in_bytes)], at[len(in_bytes):]) == ALIGN, (name, i, off)
+
+
+def test_clip_of_a_workspace_that_begins_inside_a_record():
+    run = load_library().flexspmv_clip_gradients
+    for norm, ws in ((FAR, FAR * 2 + 8), (FAR, FAR * 2 + 4), (FAR + 2, FAR * 2)):
+        assert run(1, 0, ctypes.c_float(1), ctypes.c_void_p(norm), ctypes.c_void_p(ws), ctypes.c_size_t(1 << 30), None) == ALIGN
