@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kClipThreads, kClipCtasPerSm) clip_scale_kerne
     const ClipPiece p = next;
     if (c >= (int)gridDim.x) next = piece[c - gridDim.x];
     const int type = p.types & 3, out_type = p.types >> 2;
-    if (scale == 1.f && p.in == p.out && type == out_type) continue;       // nothing to change
+    if (!p.out || (scale == 1.f && p.in == p.out && type == out_type)) continue;       // a plan for the norm alone; nothing to change
     if (type == FLEXSPMV_TYPE_F32) scale_piece_to<float>(p.in, p.out, out_type, p.length, scale);
     else if (type == FLEXSPMV_TYPE_BF16) scale_piece_to<__nv_bfloat16>(p.in, p.out, out_type, p.length, scale);
     else scale_piece_to<__half>(p.in, p.out, out_type, p.length, scale);

@@ -522,7 +522,7 @@ int flexspmv_expert_combine_backward(const flexspmv_expert_desc *desc, const voi
  *           HOST arrays of count entries, read before the call returns; the tensors are contiguous device memory of any of the three types.
  *           outs null: for the norm alone; outs[i] may be grads[i] of the same type, and is left alone then where the norm is within max_norm.
  *           Else what is written, the workspace too, may share no byte with another tensor or result (FLEXSPMV_ERR_BAD_ARG)
- *   flexspmv_clip_gradients  on a planned workspace: *d_norm, and with write != 0 (the plan has outs) the scaled tensors
+ *   flexspmv_clip_gradients  on a planned workspace: *d_norm, and with write != 0 the scaled tensors (none where the plan has no outs)
  * Any finite values are squared without loss of range; a norm beyond the largest 32-bit float is infinite.
  * A norm that is not finite scales as the formula says (infinity: 0 and NaN; NaN: NaN).
  */

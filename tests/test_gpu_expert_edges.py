@@ -359,3 +359,13 @@ def test_two_copies_of_the_library(tmp_path, monkeypatch):
     monkeypatch.setattr(experts, "_functions", {})
     assert torch.equal(experts.grouped_matmul(x, w, off), want[0]) and torch.equal(experts.route(logits, 8).slots, want[1])
     experts.check()
+
+
+def test_clip_asked_to_write_by_a_plan_for_the_norm_alone():
+    t = normal(1, (100_000,), torch.float32)
+    before = t.clone()
+    call = experts.bind(experts.grad_norm, [t])
+    want = float(call.launch())
+    pieces, _, _, *rest = call._args                      # C arguments: pieces, write, max_norm, norm, workspace, its bytes
+    call._args = (pieces, 1, 0.5, *rest)
+    assert float(call.launch()) == want and torch.equal(t, before)
