@@ -247,7 +247,7 @@ def bind(op, *args, **kwargs) -> BoundCall:
     runs it on them as often as wanted."""
     _need(op in _BINDERS, "bind takes an operator of this module")
     # the plan would run with the graph's replays only, and a launch before the first would take whatever the workspace holds for one
-    if op in (grad_norm, clip_grad_norm) and torch.cuda.is_current_stream_capturing():
+    if op in (grad_norm, clip_grad_norm) and torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
         raise FlexSpmvError(f"{op.__name__} is bound while a stream is captured: bind it before, or call it unbound")
     call = _BINDERS[op](*args, **kwargs)
     if isinstance(call, PlannedCall):

@@ -6,7 +6,8 @@ import random
 import pytest
 import torch
 
-from flexspmv_b200.binding import load_library
+from flexspmv_b200 import experts
+from flexspmv_b200.binding import FlexSpmvError, load_library
 from flexspmv_b200.experts import Desc, _meets
 
 BAD_ARG, FAR = -1, 1 << 32
@@ -114,3 +115,9 @@ def test_clip_of_a_workspace_that_begins_inside_a_record():
     run = load_library().flexspmv_clip_gradients
     for norm, ws in ((FAR, FAR * 2 + 8), (FAR, FAR * 2 + 4), (FAR + 2, FAR * 2)):
         assert run(1, 0, ctypes.c_float(1), ctypes.c_void_p(norm), ctypes.c_void_p(ws), ctypes.c_size_t(1 << 30), None) == ALIGN
+
+
+def test_host_tensors_of_a_bound_clip():
+    for call in (lambda: experts.bind(experts.grad_norm, [torch.zeros(3)]), lambda: experts.bind(experts.clip_grad_norm, [torch.zeros(3)], 1.0)):
+        with pytest.raises(FlexSpmvError, match="CUDA"):
+            call()
