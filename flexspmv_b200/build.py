@@ -78,7 +78,7 @@ def build(force: bool = False, jobs: int | None = None, verbose_ptxas: bool = Fa
     work = []   # (src, obj)
     core_src = os.path.join(CSRC, "flex_core.cu")
     work.append((core_src, os.path.join(BUILD, "flex_core.o")))
-    for unit in ("flex_sort", "flex_experts", "flex_grouped", "flex_grad_clip"):
+    for unit in ("flex_sort", "flex_experts", "flex_grouped", "flex_grad_clip", "flex_residual", "flex_adapters"):
         work.append((os.path.join(CSRC, f"{unit}.cu"), os.path.join(BUILD, f"{unit}.o")))
     for sym, text in generated_units():
         src = os.path.join(BUILD, f"graph_{sym}.cu")

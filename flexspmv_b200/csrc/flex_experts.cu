@@ -406,6 +406,234 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const float* __rest
   }
 }
 
+// ---- balance -------------------------------------------------------------------------------------------------------
+
+// The softmax of a row whose part is in this warp's lanes: powers in e, their base and the factor that makes probabilities of them.  A row of -infinity
+// alone has none: its powers are 0.
+template <class T, int V, int W>
+__device__ __forceinline__ bool softmax_of(const LanePart<T, V, W>& part, bool exact, float (&e)[V], float& base, float& factor) {
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) top = fmaxf(top, part.piece[i / W].get(i % W));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const bool there = top > -INFINITY;
+  base = there ? top : 0.f;
+  // results of 32 bits far below the largest: as in the router's gradient
+  bool far = false;
+  if constexpr (std::is_same<T, float>::value)
+    if (exact)
+#pragma unroll
+      for (int i = 0; i < V; ++i) far |= part.piece[i / W].get(i % W) < base - 8.f;
+  if (far) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = exp_below_exact(part.piece[i / W].get(i % W), base);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = exp_below(part.piece[i / W].get(i % W), base);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) sum += e[i];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  factor = there ? __frcp_rn(sum) : 1.f;
+  return there;
+}
+
+struct BalanceArgs {
+  const void* logits;
+  const int* offsets;
+  long long tokens, stride;
+  int experts;
+  float* parts;                    // [CTAs][experts]: sums of the probabilities of a CTA's tokens
+  int* part_tokens;                // [CTAs]: its rows that are not all -infinity
+  float *loss, *mean;
+  int *counts, *there;
+};
+
+// loss = experts / (pairs tokens) sum_e counts[e] total[e], counts from the plan's offsets; total in shared memory.
+template <int THREADS>
+__device__ __forceinline__ void balance_end(const BalanceArgs& a, const float* total, int tokens) {
+  __shared__ float warp_sum[THREADS / 32];
+  const float inverse = __frcp_rn((float)(tokens > 0 ? tokens : 1));
+  float sum = 0.f;
+  for (int e = threadIdx.x; e < a.experts; e += THREADS) {
+    const int count = a.offsets[e + 1] - a.offsets[e];
+    const float mean = total[e] * inverse;
+    a.counts[e] = count;
+    a.mean[e] = mean;
+    sum = fmaf((float)count, mean, sum);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (threadIdx.x % 32 == 0) warp_sum[threadIdx.x / 32] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float all = 0.f;
+    for (int w = 0; w < THREADS / 32; ++w) all += warp_sum[w];
+    const int pairs = a.offsets[a.experts] - a.offsets[0];
+    *a.loss = all * (float)a.experts / (float)(pairs > 0 ? pairs : 1);
+    *a.there = tokens;
+  }
+}
+
+// A warp takes every so-many-th token and keeps its lanes' experts' sums in registers; the warps' sums meet in shared memory, the CTAs' in a second
+// launch, each in a fixed order.  Bound by memory with many tokens (the logits are read once), by the launch with few (SMALL: one CTA does it all).
+template <class T, int V, int W, int THREADS, bool SMALL>
+__global__ void __launch_bounds__(THREADS) balance_kernel(BalanceArgs a) {
+  extern __shared__ __align__(16) float balance_sm[];          // [warps][experts]
+  __shared__ int seen[THREADS / 32];
+  constexpr int kWarps = THREADS / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long step = (long long)gridDim.x * kWarps;
+  const T* const logits = static_cast<const T*>(a.logits);
+  pdl_wait();
+  pdl_launch_dependents();
+  float acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+  int there = 0;
+  LanePart<T, V, W> next;
+  next.clear();
+  long long t = (long long)blockIdx.x * kWarps + warp;
+  if (t < a.tokens) next.load(logits + t * a.stride, a.experts, lane);
+  for (; t < a.tokens; t += step) {
+    const LanePart<T, V, W> part = next;
+    if (t + step < a.tokens) next.load(logits + (t + step) * a.stride, a.experts, lane);
+    float e[V], base, factor;
+    there += softmax_of<T, V, W>(part, false, e, base, factor);
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = fmaf(e[i], factor, acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = (i / W * 32 + lane) * W + i % W;
+    if (e < a.experts) balance_sm[warp * a.experts + e] = acc[i];
+  }
+  if (lane == 0) seen[warp] = there;
+  __syncthreads();
+  int tokens = 0;
+  for (int w = 0; w < kWarps; ++w) tokens += seen[w];
+  for (int e = threadIdx.x; e < a.experts; e += THREADS) {
+    float sum = 0.f;
+#pragma unroll 8
+    for (int w = 0; w < kWarps; ++w) sum += balance_sm[w * a.experts + e];
+    if (SMALL) balance_sm[e] = sum;          // column e is this thread's alone
+    else a.parts[(size_t)blockIdx.x * a.experts + e] = sum;
+  }
+  if (SMALL) {
+    __syncthreads();
+    balance_end<THREADS>(a, balance_sm, tokens);
+  } else if (threadIdx.x == 0) {
+    a.part_tokens[blockIdx.x] = tokens;
+  }
+}
+
+__global__ void __launch_bounds__(1024) balance_end_kernel(BalanceArgs a, int ctas) {
+  __shared__ float total[FLEXSPMV_MAX_EXPERTS], group_sum[1024];
+  __shared__ int tokens;
+  const int tid = threadIdx.x, wide = (a.experts + 31) / 32 * 32, groups = 1024 / wide, group = tid / wide, e = tid % wide;
+  pdl_wait();
+  if (tid < 32) {
+    int n = 0;
+    for (int p = tid; p < ctas; p += 32) n += a.part_tokens[p];
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (tid == 0) tokens = n;
+  }
+  float sum = 0.f;
+  if (e < a.experts && group < groups)
+#pragma unroll 8
+    for (int p = group; p < ctas; p += groups) sum += a.parts[(size_t)p * a.experts + e];
+  group_sum[tid] = sum;
+  __syncthreads();
+  if (tid < a.experts) {
+    for (int g = 1; g < groups; ++g) sum += group_sum[g * wide + tid];
+    total[tid] = sum;
+  }
+  __syncthreads();
+  balance_end<1024>(a, total, tokens);
+}
+
+struct BalanceGradArgs {
+  const float* dloss;
+  const void* logits;
+  const int *counts, *there;
+  const float *dweights, *weights;     // of the router, or null
+  const int* ids;
+  void* dlogits;
+  long long tokens, stride;
+  int experts, k, renormalize;
+};
+
+// dlogits = dloss experts / (pairs tokens) p (counts - sum p counts), and with dweights the router's gradient on top, in one pass over the logits: first
+// every value as if it were not chosen, then the chosen ones' over it.  A warp takes a token; the counts stay in its registers.
+template <class T, int V, int W>
+__global__ void __launch_bounds__(256) balance_backward_kernel(BalanceGradArgs a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  float count[V];
+  int pairs = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = (i / W * 32 + lane) * W + i % W, n = e < a.experts ? a.counts[e] : 0;
+    count[i] = (float)n;
+    pairs += n;
+  }
+  pairs = __reduce_add_sync(0xffffffffu, pairs);
+  const int there = *a.there;
+  const float scale = *a.dloss * (float)a.experts / ((float)(pairs > 0 ? pairs : 1) * (float)(there > 0 ? there : 1));
+  const T* const logits = static_cast<const T*>(a.logits);
+  const long long step = (long long)gridDim.x * 8;
+  LanePart<T, V, W> next;
+  next.clear();
+  long long t = (long long)blockIdx.x * 8 + warp;
+  if (t < a.tokens) next.load(logits + t * a.stride, a.experts, lane);
+  for (; t < a.tokens; t += step) {
+    const LanePart<T, V, W> part = next;
+    if (t + step < a.tokens) next.load(logits + (t + step) * a.stride, a.experts, lane);
+    int id = -1;
+    float w = 0.f, g = 0.f, chosen_logit = 0.f, chosen_count = 0.f;
+    if (a.dweights && lane < a.k) {
+      id = a.ids[t * a.k + lane];
+      if (id < 0 || id >= a.experts) id = -1;          // not an expert of these logits: no choice
+      else {
+        w = a.weights[t * a.k + lane];
+        g = a.dweights[t * a.k + lane];
+        chosen_logit = to_float(logits[t * a.stride + id]);
+        chosen_count = (float)a.counts[id];
+      }
+    }
+    float e[V], base, factor, mean = w * g, expected = 0.f;
+    softmax_of<T, V, W>(part, true, e, base, factor);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      e[i] *= factor;
+      expected = fmaf(e[i], count[i], expected);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      mean += __shfl_xor_sync(0xffffffffu, mean, o);
+      expected += __shfl_xor_sync(0xffffffffu, expected, o);
+    }
+    const float common = a.renormalize ? 0.f : mean;
+    T* const out = static_cast<T*>(a.dlogits) + t * a.experts;
+#pragma unroll
+    for (int i = 0; i < V / W; ++i) {
+      const int first = (i * 32 + lane) * W;
+      Pack<T, W> r;
+#pragma unroll
+      for (int x = 0; x < W; ++x) r.set(x, e[i * W + x] * (scale * (count[i * W + x] - expected) - common));
+      if (first < a.experts) r.store(out + first);
+    }
+    __syncwarp();
+    if (id >= 0) {
+      const float p = exp_below_exact(chosen_logit, base) * factor;
+      out[id] = from_float<T>(fmaf(p, scale * (chosen_count - expected) - common, a.renormalize ? w * (g - mean) : w * g));
+    }
+    __syncwarp();
+  }
+}
+
 // ---- combine -------------------------------------------------------------------------------------------------------
 
 // out[t] = sum_j w[t, j] z[slots[t, j]]: a thread takes W neighbouring columns at U places, 256 threads apart, and has the loads of K choices of
@@ -573,6 +801,55 @@ static int route_typed(const RouteArgs& a, cudaStream_t st) {
   return route_width<T, 32, 256>(a, st);
 }
 
+// CTAs of the balance loss: a token a warp up to one CTA an SM.
+constexpr long long kBalanceSmall = 64;      // tokens up to which one CTA does it all
+static int balance_ctas(long long tokens) {
+  const long long want = (tokens + 15) / 16;
+  const int sms = device_sm_count();
+  return (int)(want < 1 ? 1 : want > sms ? sms : want);
+}
+
+template <class T, int V, int W>
+static int balance_launch(const BalanceArgs& a, cudaStream_t st) {
+  constexpr int kThreads = V <= 12 ? 512 : 256;          // 32 KB for the warps' sums at the most
+  const size_t smem = (size_t)a.experts * (kThreads / 32) * 4;
+  if (a.tokens <= kBalanceSmall) return launch_pdl(balance_kernel<T, V, W, kThreads, true>, 1, kThreads, smem, st, a);
+  const int ctas = balance_ctas(a.tokens);
+  if (int e = launch_pdl(balance_kernel<T, V, W, kThreads, false>, ctas, kThreads, smem, st, a)) return e;
+  return launch_pdl(balance_end_kernel, 1, 1024, 0, st, a, ctas);
+}
+template <class T, int V, int W>
+static int balance_launch(const BalanceGradArgs& a, cudaStream_t st) {
+  const long long want = (a.tokens + 7) / 8;
+  return launch_pdl(balance_backward_kernel<T, V, W>, (unsigned)(want < device_sm_count() * 8ll ? want : device_sm_count() * 8ll), 256, 0, st, a);
+}
+
+template <class T, int V, class A>
+static int balance_width(const A& a, bool aligned, cudaStream_t st) {
+  constexpr int kFull = 16 / (int)sizeof(T), W = V < kFull ? 1 : V % kFull == 0 ? kFull : 4;
+  return aligned && a.experts % W == 0 && a.stride % W == 0 ? balance_launch<T, V, W>(a, st) : balance_launch<T, V, 1>(a, st);
+}
+
+// `aligned`: the logits and their gradient begin on 16 bytes.
+template <class A>
+static int balance_call(const A& a, int type, bool aligned, cudaStream_t st) {
+  const auto go = [&](auto zero) {
+    using T = decltype(zero);
+    if (a.experts <= 32) return balance_width<T, 1>(a, aligned, st);
+    if (a.experts <= 64) return balance_width<T, 2>(a, aligned, st);
+    if (a.experts <= 128) return balance_width<T, 4>(a, aligned, st);
+    if (a.experts <= 256) return balance_width<T, 8>(a, aligned, st);
+    if (a.experts <= 384) return balance_width<T, 12>(a, aligned, st);
+    if (a.experts <= 512) return balance_width<T, 16>(a, aligned, st);
+    return balance_width<T, 32>(a, aligned, st);
+  };
+  switch (type) {
+    case FLEXSPMV_TYPE_F32: return go(0.f);
+    case FLEXSPMV_TYPE_BF16: return go(__nv_bfloat16());
+    default: return go(__half());
+  }
+}
+
 static int grid_of(long long ctas, int most) { return (int)(ctas < 1 ? 1 : ctas > most ? most : ctas); }
 
 template <class T, int W, int K, int U>
@@ -672,6 +949,58 @@ int flexspmv_expert_route_backward(const flexspmv_expert_desc* d, const void* co
     case FLEXSPMV_TYPE_BF16: return go(__nv_bfloat16());
     default: return go(__half());
   }
+}
+
+// Checks that the balance loss and its gradient share.
+static int check_balance(const flexspmv_expert_desc* d) {
+  if (!d || d->tokens < 0 || d->experts < 1 || d->in_stride < d->experts || !flex::known_type(d->type)) return FLEXSPMV_ERR_BAD_ARG;
+  if (d->experts > FLEXSPMV_MAX_EXPERTS || d->tokens > 0x7fffffffLL) return FLEXSPMV_ERR_TOO_LARGE;
+  return 0;
+}
+
+int flexspmv_balance_loss_bytes(const flexspmv_expert_desc* d, size_t* bytes) {
+  if (!d || !bytes || d->tokens < 0 || d->experts < 1) return FLEXSPMV_ERR_BAD_ARG;
+  if (d->experts > FLEXSPMV_MAX_EXPERTS) return FLEXSPMV_ERR_TOO_LARGE;
+  *bytes = (size_t)flex::balance_ctas(d->tokens) * (d->experts + 1) * 4;
+  return 0;
+}
+
+int flexspmv_balance_loss(const flexspmv_expert_desc* d, const void* const* in, void* const* out, void* ws, size_t ws_bytes, void* stream) {
+  if (int e = check_balance(d)) return e;
+  if (!in || !out || (d->tokens && !in[0]) || !in[1] || !out[0] || !out[1] || !out[2] || !out[3]) return FLEXSPMV_ERR_BAD_ARG;
+  size_t need = 0;
+  flexspmv_balance_loss_bytes(d, &need);
+  if (!ws || ws_bytes < need) return FLEXSPMV_ERR_WORKSPACE;
+  if (!flex::aligned16(ws) || !flex::aligned_to(flex::type_bytes(d->type), in[0]) || !flex::aligned_to(4, in[1], out[0], out[1], out[2], out[3]))
+    return FLEXSPMV_ERR_ALIGN;
+  const long long each = 4ll * d->experts;
+  if (!flex::apart({{out[0], 4}, {out[1], each}, {out[2], each}, {out[3], 4}, {ws, (long long)need}},
+                   {flex::rows_at(in[0], d->tokens, d->experts, d->in_stride, d->type), {in[1], each + 4}}))
+    return FLEXSPMV_ERR_BAD_ARG;
+  float* const parts = static_cast<float*>(ws);
+  const flex::BalanceArgs a = {in[0], static_cast<const int*>(in[1]), d->tokens, d->in_stride, d->experts, parts,
+                               reinterpret_cast<int*>(parts + (size_t)flex::balance_ctas(d->tokens) * d->experts), static_cast<float*>(out[0]),
+                               static_cast<float*>(out[2]), static_cast<int*>(out[1]), static_cast<int*>(out[3])};
+  return flex::balance_call(a, d->type, flex::aligned16(in[0]), static_cast<cudaStream_t>(stream));
+}
+
+int flexspmv_balance_loss_backward(const flexspmv_expert_desc* d, const void* const* in, void* const* out, void* stream) {
+  if (int e = check_balance(d)) return e;
+  if (!in || !out) return FLEXSPMV_ERR_BAD_ARG;
+  if (d->tokens == 0) return 0;
+  if (!in[0] || !in[1] || !in[2] || !in[3] || !out[0] || (in[4] && (!in[5] || !in[6]))) return FLEXSPMV_ERR_BAD_ARG;
+  if (in[4] && (d->choices < 1 || d->choices > d->experts)) return FLEXSPMV_ERR_BAD_ARG;
+  if (in[4] && d->choices > FLEXSPMV_MAX_CHOICES) return FLEXSPMV_ERR_TOO_LARGE;
+  if (!flex::aligned_to(flex::type_bytes(d->type), in[1], out[0]) || !flex::aligned_to(4, in[0], in[2], in[3], in[4], in[5], in[6])) return FLEXSPMV_ERR_ALIGN;
+  const long long pairs = in[4] ? 4 * d->tokens * d->choices : 0;
+  if (!flex::apart({{out[0], d->tokens * d->experts * flex::type_bytes(d->type)}},
+                   {{in[0], 4}, flex::rows_at(in[1], d->tokens, d->experts, d->in_stride, d->type), {in[2], 4ll * d->experts}, {in[3], 4}, {in[4], pairs},
+                    {in[5], pairs}, {in[6], pairs}}))
+    return FLEXSPMV_ERR_BAD_ARG;
+  const flex::BalanceGradArgs a = {static_cast<const float*>(in[0]), in[1], static_cast<const int*>(in[2]), static_cast<const int*>(in[3]),
+                                   static_cast<const float*>(in[4]), static_cast<const float*>(in[5]), static_cast<const int*>(in[6]), out[0], d->tokens,
+                                   d->in_stride, d->experts, d->choices, d->flags & FLEXSPMV_EXPERT_RENORMALIZE};
+  return flex::balance_call(a, d->type, flex::aligned16(in[1]) && flex::aligned16(out[0]), static_cast<cudaStream_t>(stream));
 }
 
 // Checks that combine and its gradient share.

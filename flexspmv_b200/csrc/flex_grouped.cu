@@ -5,6 +5,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "flex_adapters.cuh"
 #include "flex_common.cuh"
 #include "flex_expert_types.cuh"
 #include "flex_umma.cuh"
@@ -22,6 +23,10 @@ struct GroupedArgs {
   long long tokens, slots, a_stride, b_stride;
   int experts, n, k;
   int* status;
+  // low-rank adapters (flex_adapters.cu): each place's adapter, all adapters' second matrices (adapters x n x rank), each place's scaled A x
+  const int* ids;
+  const void *up, *low;
+  int adapters, rank, low_width;
 };
 
 __device__ __forceinline__ void raise(int* status, int code) {
@@ -65,6 +70,7 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict_
 // rows up to some thousand rows, 2 - 4 % slower for 32 768 of 2048.  (Tile copies that gather four rows each took 72 cycles an instruction: 2.2 ms
 // there instead of 0.43.)  dw's rows are other ones in every step: gathered like this they take 0.57 ms of the 32 768; a copy of them in the
 // workspace and contiguous tile copies 0.44.
+// ADAPT (forward, one expert): on a place's way out its adapter's up matrix times its vector of `rank` values is added (add_low_rank), before the only rounding.
 // Warps 0-7 store finished accumulators, warp 8 issues the tile copies, warp 9 the matrix instructions; two accumulators in tensor memory,
 // so that one is stored while the next is computed (HALVES = 2: while the other half of the next tile begins).  The sum goes 64 values (128 bytes of a row) a stage.
 constexpr int kStoreWarps = 8, kCopyWarp = kStoreWarps, kMathWarp = kStoreWarps + 1, kGroupedThreads = (kStoreWarps + 2) * 32;
@@ -146,7 +152,87 @@ __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const Group
   return r;
 }
 
-template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER, bool PARTS>
+// Adds the low-rank parts of 32 features from m on by 32 places: the accumulator's registers (tmem_load_blocks) are laid out as those of the warp's own
+// matrix instruction, 16 features by 8 places, so that it can finish here what the tensor memory holds.  Each adapter among the places has a product of
+// its own and only its places take it up: what is not finite in one request's adapter stays out of the others.  The sum's index may be permuted as long as both
+// operands are alike, so a lane takes 8 neighbouring values of a row in one load, which are its share of two instructions.
+template <class T>
+__device__ __forceinline__ void add_low_rank(const GroupedArgs& a, int m, int place, int left, int lane, uint32_t (&low)[16], uint32_t (&high)[16]) {
+  const int q = lane & 3, g = lane >> 2;
+  const int id = lane < left ? a.ids[place + lane] : -1;
+  unsigned todo = __ballot_sync(0xffffffffu, (unsigned)id < (unsigned)a.adapters);
+  while (todo) {
+    const int adapter = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
+    const unsigned mine = __ballot_sync(0xffffffffu, id == adapter);
+    todo &= ~mine;
+    float d[2][4][4];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) d[i / 16][i / 4 % 4][i % 4] = 0.f;
+    const T* const up = static_cast<const T*>(a.up) + ((size_t)adapter * a.n + m + g) * a.rank;
+    for (int k = q * 8; k - q * 8 < a.rank; k += 32) {
+      const bool inside = k < a.rank;
+      uint4 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = inside && m + g + i * 8 < a.n ? *reinterpret_cast<const uint4*>(up + (size_t)i * 8 * a.rank + k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        if (!(mine >> (b * 8) & 0xffu)) continue;
+        uint4 h = make_uint4(0, 0, 0, 0), rest = h;
+        if (inside && (mine >> (b * 8 + g) & 1u)) {
+          const T* const row = static_cast<const T*>(a.low) + (size_t)(place + b * 8 + g) * a.low_width;
+          h = *reinterpret_cast<const uint4*>(row + low_high(k, a.rank));
+          rest = *reinterpret_cast<const uint4*>(row + low_rest(k, a.rank));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          warp_mma<T>(d[i][b], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h.x, h.y);
+          warp_mma<T>(d[i][b], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, h.z, h.w);
+          warp_mma<T>(d[i][b], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, rest.x, rest.y);
+          warp_mma<T>(d[i][b], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, rest.z, rest.w);
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (mine >> (b * 8 + q * 2 + (x & 1)) & 1u) {
+          low[b * 4 + x] = __float_as_uint(__uint_as_float(low[b * 4 + x]) + d[0][b][x]);
+          high[b * 4 + x] = __float_as_uint(__uint_as_float(high[b * 4 + x]) + d[1][b][x]);
+        }
+  }
+}
+
+// The same for eight neighbouring features of one place, by one thread.
+template <class T>
+__device__ __forceinline__ void add_low_rank(const GroupedArgs& a, int m, int place, float (&sum)[8]) {
+  const int id = a.ids[place];
+  if ((unsigned)id >= (unsigned)a.adapters) return;
+  const T* const up = static_cast<const T*>(a.up) + ((size_t)id * a.n + m) * a.rank;
+  const T* const row = static_cast<const T*>(a.low) + (size_t)place * a.low_width;
+  float part[8];
+#pragma unroll
+  for (int x = 0; x < 8; ++x) part[x] = 0.f;
+  for (int k = 0; k < a.rank; k += 8) {
+    Pack<T, 8> h, rest, w[8];
+    h.load(row + low_high(k, a.rank));
+    rest.load(row + low_rest(k, a.rank));
+#pragma unroll
+    for (int x = 0; x < 8; ++x) w[x].load(up + (size_t)x * a.rank + k);          // n is a multiple of 8: all eight are there
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = h.get(i) + rest.get(i);
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) part[x] = fmaf(w[x].get(i), v[i], part[x]);
+  }
+#pragma unroll
+  for (int x = 0; x < 8; ++x) sum[x] += part[x];
+}
+
+template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER, bool PARTS, bool ADAPT>
 __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                      const __grid_constant__ CUtensorMap row_a, const __grid_constant__ CUtensorMap row_b,
                                                                      const __grid_constant__ CUtensorMap map_out,
@@ -178,7 +264,9 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
     if (MODE == kGroupedDw) tma_prefetch_map(&map_out);
   }
   if (warp == kMathWarp) tmem_alloc<PAIR, Cfg::kTmemCols>(&bars.tmem);
-  pdl_wait();
+  // ADAPT: the launch before this one is the adapters' first product, which lets this one begin once all before it is done; only the stores need
+  // its result.
+  if (!ADAPT) pdl_wait();
   for (int e = tid; e < a.experts; e += kThreads) {
     int from, to;
     group_of(a, e, from, to);
@@ -465,6 +553,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
     }
     copy16_wait_all();
   } else {
+    if (ADAPT) pdl_wait();
     int acc = 0;
     uint32_t acc_phase = 0, second_phase = 0;
     TO* const out = static_cast<TO*>(a.out);
@@ -583,6 +672,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
         }
         if (last) free_accumulator();
         if (!there) break;
+        if constexpr (ADAPT) add_low_rank<T>(a, m, t.from + c0, t.count - c0, lane, low, high);
         if (MODE == kGroupedDw) {
           store_rows(c0, [&](int x) { return __uint_as_float(v[x]); });
         } else {
@@ -631,6 +721,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   if (SPLIT) {
     // every CTA stores some of the tile's columns, eight neighbouring rows (dw: columns) at a time
     cluster_sync();
+    if (ADAPT) pdl_wait();
     if (first < tiles && !*abort) {
       const GroupedTile t = tile_at<MODE, NT, PAIR, HALVES>(a, table, first);
       const int eights = (t.cols + 7) / 8, c_from = eights * share / split * 8, c_to = eights * (share + 1) / split * 8;
@@ -657,6 +748,8 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
 #pragma unroll
           for (int x = 0; x < 8; ++x) sum[x] += v[x];
         }
+        if constexpr (ADAPT)
+          if (c < t.count && t.m0 + r < a.n) add_low_rank<T>(a, t.m0 + r, t.from + c, sum);
         Pack<TO, 8> q;
 #pragma unroll
         for (int x = 0; x < 8; ++x) q.set(x, sum[x]);
@@ -705,7 +798,7 @@ static int grouped_smem(int experts) {
 }
 
 // `split`: CTAs that share a tile, `grid` of them altogether; 1: whole tiles.
-template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER, bool PARTS>
+template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER, bool PARTS, bool ADAPT>
 static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStream_t st) {
   constexpr CUtensorMapDataType kIn = std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap ma, mb, row_a, row_b, out;
@@ -739,7 +832,7 @@ static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStre
     row_b = mb;
   }
   const int smem = grouped_smem<MODE, NT, PAIR, HALVES, (int)sizeof(TO)>(a.experts);
-  constexpr auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR, HALVES, SPLIT, GATHER, PARTS>;
+  constexpr auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR, HALVES, SPLIT, GATHER, PARTS, ADAPT>;
   if (int e = allow_smem<kernel>(smem)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3((unsigned)grouped_threads(GATHER)); cfg.dynamicSmemBytes = smem; cfg.stream = st;
@@ -752,7 +845,7 @@ static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStre
   return (int)cudaLaunchKernelEx(&cfg, kernel, ma, mb, row_a, row_b, out, a);
 }
 
-template <class T, class TO, int MODE, int NT, int PAIR, bool GATHER, bool PARTS = false>
+template <class T, class TO, int MODE, int NT, int PAIR, bool GATHER, bool PARTS, bool ADAPT>
 static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
   const int sms = device_sm_count();
   // tiles of 128 rows, no more than these whatever the groups are
@@ -763,12 +856,12 @@ static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
   // What dividing saves is most of a tile's steps, 0.3 us each (a narrow tile's 0.13); what it costs is the parts' meeting, about 5 us (1.5).
   // us, whole / divided: 8 rows, one expert of 2048 x 4096 17.4 / 9.4; dw of 8192 rows, 1024 x 1024 43.8 / 22; but 4096 rows, two experts of
   // 512 x 512 (8 steps) 9.8 / 12.6.
-  constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, 1, true, GATHER, PARTS>;
+  constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, 1, true, GATHER, PARTS, ADAPT>;
   const int smem = grouped_smem<MODE, NT, 1, 1, (int)sizeof(TO)>(a.experts);
   for (int split = 8; split > 1; split /= 2) {
     if (most * split > sms || steps - steps / split < (NT > 64 ? 20 : 12)) continue;
     if (int e = allow_smem<divided>(smem)) return e;
-    if (most <= clusters_at_once<divided, grouped_threads(GATHER)>(split, smem)) return grouped_launch_as<T, TO, MODE, NT, 1, 1, true, GATHER, PARTS>(a, (int)most * split, split, st);
+    if (most <= clusters_at_once<divided, grouped_threads(GATHER)>(split, smem)) return grouped_launch_as<T, TO, MODE, NT, 1, 1, true, GATHER, PARTS, ADAPT>(a, (int)most * split, split, st);
   }
   // Tiles of both accumulators (HALVES = 2): a quarter less between L2 and the SMs for a tile's step, a stage less under way, and the end of a tile's
   // sum that only half of it is behind.  It pays where the sums are long and the tiles go round the pairs, most with gathered rows, which are gathered
@@ -778,18 +871,18 @@ static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
     const long long columns = MODE == kGroupedDw ? (long long)a.experts * ((a.k + NT - 1) / NT) : a.slots / NT + a.experts / 2;          // of tiles, about
     const int long_sum = MODE == kGroupedDw ? 16 : GATHER ? 32 : 40, half_rounds = MODE == kGroupedDw ? 20 : 3;
     if (steps >= long_sum && columns * ((a.n + 511) / 512) * 2 >= half_rounds * (sms / 2))
-      return grouped_launch_as<T, TO, MODE, NT, 2, 2, false, GATHER, false>(a, sms / 2 * 2, 1, st);
+      return grouped_launch_as<T, TO, MODE, NT, 2, 2, false, GATHER, false, ADAPT>(a, sms / 2 * 2, 1, st);
   }
-  return grouped_launch_as<T, TO, MODE, NT, PAIR, 1, false, GATHER, PARTS>(a, sms / PAIR * PAIR, 1, st);
+  return grouped_launch_as<T, TO, MODE, NT, PAIR, 1, false, GATHER, PARTS, ADAPT>(a, sms / PAIR * PAIR, 1, st);
 }
 
-template <class T, class TO, int MODE, bool GATHER>
+template <class T, class TO, int MODE, bool GATHER, bool ADAPT = false>
 static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
   if constexpr (MODE == kGroupedDw) {
     // us, whole / in parts: 200 000 rows of 2048 x 2048 in float16 1160 / 1195, 600 000 of 512 x 512 512 / 540, 102 400 in 32 such groups 591 / 597
     if constexpr (sizeof(TO) == 2)
-      if (a.slots <= kWholeRows<T>) return grouped_tiles<T, TO, MODE, 256, 2, GATHER, false>(a, st);
-    return grouped_tiles<T, TO, MODE, 256, 2, GATHER, true>(a, st);
+      if (a.slots <= kWholeRows<T>) return grouped_tiles<T, TO, MODE, 256, 2, GATHER, false, false>(a, st);
+    return grouped_tiles<T, TO, MODE, 256, 2, GATHER, true, false>(a, st);
   } else {
     // Tiles of 64 places and single CTAs for up to 32 places an expert on average: more of the weights on their way at once.  us, 64 / 256 places:
     // 16 an expert, 64 experts of 1408 x 2048 59.8 / 66.8; 32 experts of 2048 x 2048, 32 an expert 47.0 / 49.7, 48 51.0 / 50.5, 128 72.1 / 54.9.
@@ -797,8 +890,8 @@ static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
     // us, narrow / wide: 753 rows, 4 experts of 104 x 1512 8.9 / 15.1; 256 rows of 2048 x 2048 10.5 / 14.3, of a list 11.0 / 16.0; 512 rows of 1024 x 1024
     // 7.3 / 8.1; but 100 rows of 4096 x 4096 13.0 / 12.3.
     const long long narrow = ((MODE == kGroupedDx ? a.k : a.n) + 127) / 128 * ((a.slots < a.experts ? a.slots : a.experts) + a.slots / 64);
-    if (a.slots <= 32ll * a.experts || narrow <= device_sm_count()) return grouped_tiles<T, TO, MODE, 64, 1, GATHER>(a, st);
-    return grouped_tiles<T, TO, MODE, 256, 2, GATHER>(a, st);
+    if (a.slots <= 32ll * a.experts || narrow <= device_sm_count()) return grouped_tiles<T, TO, MODE, 64, 1, GATHER, false, ADAPT>(a, st);
+    return grouped_tiles<T, TO, MODE, 256, 2, GATHER, false, ADAPT>(a, st);
   }
 }
 
@@ -865,6 +958,19 @@ static int grouped_call(const flexspmv_expert_desc* d, const void* const* in, vo
     }
   };
   return d->type == FLEXSPMV_TYPE_BF16 ? go(__nv_bfloat16()) : go(__half());
+}
+
+int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* low, int low_width, const int* offsets,
+                    const int* ids, void* out, int* status, cudaStream_t st) {
+  GroupedArgs a = {x, weight, offsets, nullptr, out, d->tokens, d->tokens, d->x_stride, 0, 1, d->n, d->k, status};
+  a.ids = ids;
+  a.up = up;
+  a.low = low;
+  a.adapters = d->adapters;
+  a.rank = d->rank;
+  a.low_width = low_width;
+  if (d->type == FLEXSPMV_TYPE_BF16) return grouped_launch<__nv_bfloat16, __nv_bfloat16, kGroupedForward, false, true>(a, st);
+  return grouped_launch<__half, __half, kGroupedForward, false, true>(a, st);
 }
 
 }  // namespace flex

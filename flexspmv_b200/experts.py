@@ -9,8 +9,8 @@ values, data_struct_shared.cuh:80-659.)
     z = grouped_matmul(act(h), w2, plan.offsets)
     y = combine(z, plan.slots, plan.weights)                    # y[t] = sum_j weights[t, j] z[slots[t, j]]
 
-with the gradients ``route_backward``, ``grouped_matmul_dx``, ``grouped_matmul_dw`` and ``combine_backward``, and ``grad_norm`` and
-``clip_grad_norm`` over the many tensors that such a layer's training has.  ``expert_layer.RoutedExperts`` runs them together.
+with the gradients ``route_backward``, ``grouped_matmul_dx``, ``grouped_matmul_dw`` and ``combine_backward``, ``balance_loss`` with its gradient,
+which keeps a router from using few of its experts, and ``grad_norm`` and ``clip_grad_norm`` over the many tensors that such a layer's training has.  ``expert_layer.RoutedExperts`` runs them together.
 
 Results carry no gradient: while gradients are recorded, tensors that require one are refused (``expert_layer`` has the functions that do carry
 them); only the norm of the last two, as usual, is a plain number.
@@ -153,7 +153,7 @@ def _flag(device: int) -> _Flag:
 def _raise_flag(device: int):
     st = int(_flag(device).view[0])
     _flag(device).view[0] = 0
-    text = "offsets or rows that do not fit their arrays" if st == -5 else load_library().flexspmv_error_string(st).decode()
+    text = "offsets, rows or ids that do not fit their arrays" if st == -5 else load_library().flexspmv_error_string(st).decode()
     raise FlexSpmvError(f"an earlier grouped product on cuda:{device} failed: {text} (status {st}); its outputs are undefined", st)
 
 
@@ -237,15 +237,15 @@ def _operator(binder):
         return binder(*args, **kwargs).launch()
     op.__name__, op.__doc__, op.__wrapped__ = binder.__name__, binder.__doc__, binder
     op.__qualname__ = binder.__name__
-    op.__module__ = __name__
+    op.__module__ = binder.__module__
     _BINDERS[op] = binder
     return op
 
 
 def bind(op, *args, **kwargs) -> BoundCall:
-    """Checks the arguments of an operator of this module and allocates its outputs and workspace once; the ``BoundCall``'s ``launch()``
-    runs it on them as often as wanted."""
-    _need(op in _BINDERS, "bind takes an operator of this module")
+    """Checks the arguments of an operator of this module (or of ``residual``, ``adapters``) and allocates its outputs and workspace once; the
+    ``BoundCall``'s ``launch()`` runs it on them as often as wanted."""
+    _need(op in _BINDERS, "bind takes an operator of this module, of residual or of adapters")
     # the plan would run with the graph's replays only, and a launch before the first would take whatever the workspace holds for one
     if op in (grad_norm, clip_grad_norm) and torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
         raise FlexSpmvError(f"{op.__name__} is bound while a stream is captured: bind it before, or call it unbound")
@@ -313,6 +313,84 @@ def route_backward(dweights: torch.Tensor, logits: torch.Tensor, plan: Plan, out
     ins, outs = _pointers((dweights, logits, plan.weights, plan.experts)), _pointers((out,))
     return BoundCall(_function("expert_route_backward", _PLAIN), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs)), dev,
                      (d, ins, outs, dweights, logits, plan, out), out)
+
+
+class Balance(NamedTuple):
+    """What ``balance_loss`` returns."""
+    loss: torch.Tensor           # () float32
+    counts: torch.Tensor         # (experts) int32: the pairs of an expert
+    mean: torch.Tensor           # (experts) float32: its mean probability
+    tokens: torch.Tensor         # () int32: rows of the logits that are not all -infinity
+
+
+@functools.lru_cache(maxsize=256)
+def _balance_bytes(tokens: int, experts: int, device: int) -> int:
+    need = ctypes.c_size_t()
+    d = Desc(tokens, 0, experts)
+    with torch.cuda.device(device):
+        _check(_function("balance_loss_bytes", _BYTES)(ctypes.addressof(d), ctypes.addressof(need)), "balance_loss")
+    return need.value
+
+
+@_operator
+def balance_loss(logits: torch.Tensor, plan: Plan) -> Balance:
+    """How unevenly ``plan`` uses the experts: ``experts / pairs * sum_e counts[e] * mean[e]`` with the softmax's mean over the tokens, 1 where all are
+    used alike.  Rows of -infinity alone count for nothing.  Over several devices add up ``counts`` and ``tokens`` before the backward pass."""
+    dev = _tensor(logits, "logits", tuple(_TYPE), 2)
+    tokens, experts = logits.shape
+    if not (1 <= experts <= MAX_EXPERTS):
+        raise FlexSpmvError(f"1 to {MAX_EXPERTS} experts, not {experts}")
+    _tensor(plan.offsets, "plan.offsets", (torch.int32,), 1, dev)
+    _whole(plan.offsets, "plan.offsets")
+    _need(plan.offsets.numel() == experts + 1 and plan.experts.shape[0] == tokens, "the plan must be of these logits")
+    stride = _rows_of(logits, "logits", aligned=False)
+    d = Desc(tokens, 0, experts, 0, 0, 0, _TYPE[logits.dtype], 0, 0, 0, stride)
+    need = _balance_bytes(tokens, experts, dev)
+    # one allocation: mean, counts, loss and tokens, then the workspace on 16 bytes
+    at = (2 * experts + 2 + 3) // 4 * 4
+    buf = torch.empty(at + need // 4, dtype=torch.int32, device=logits.device)
+    mean, counts, loss, there, _ = buf.split_with_sizes((experts, experts, 1, 1, at + need // 4 - 2 * experts - 2))
+    out = Balance(loss.view(torch.float32).view(()), counts, mean.view(torch.float32), there.view(()))
+    ins, outs = _pointers((logits, plan.offsets)), _pointers((loss, counts, mean, there))
+    return BoundCall(_function("balance_loss", _WITH_WORKSPACE),
+                     (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), buf.data_ptr() + 4 * at, need), dev,
+                     (d, ins, outs, logits, plan, buf), out)
+
+
+@_operator
+def balance_loss_backward(dloss: torch.Tensor, logits: torch.Tensor, balance: Balance, plan: Optional[Plan] = None, dweights: Optional[torch.Tensor] = None,
+                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of ``balance_loss`` with respect to ``logits``, the counts being constants; ``dloss`` () float32.  With ``plan`` and ``dweights`` the
+    router's gradient (``route_backward``) is added, in one pass over the logits and with one rounding."""
+    dev = _tensor(logits, "logits", tuple(_TYPE), 2)
+    tokens, experts = logits.shape
+    if not (1 <= experts <= MAX_EXPERTS):
+        raise FlexSpmvError(f"1 to {MAX_EXPERTS} experts, not {experts}")
+    stride = _rows_of(logits, "logits", aligned=False)
+    _tensor(dloss, "dloss", (torch.float32,), 0, dev)
+    _tensor(balance.counts, "balance.counts", (torch.int32,), 1, dev)
+    _whole(balance.counts, "balance.counts")
+    _need(balance.counts.numel() == experts, "balance must be of the logits' experts")
+    _tensor(balance.tokens, "balance.tokens", (torch.int32,), 0, dev)
+    _need((plan is None) == (dweights is None), "the router's gradient takes both plan and dweights")
+    k, renormalize, weights, ids = 0, False, None, None
+    if plan is not None:
+        weights, ids, renormalize = plan.weights, plan.experts, plan.renormalize
+        _tensor(dweights, "dweights", (torch.float32,), 2, dev)
+        for name, t, dt in (("plan.weights", weights, torch.float32), ("plan.experts", ids, torch.int32)):
+            _tensor(t, name, (dt,), 2, dev)
+            _whole(t, name)
+        _whole(dweights, "dweights")
+        k = weights.shape[1]
+        _need(weights.shape[0] == tokens and ids.shape == weights.shape and dweights.shape == weights.shape, "dweights and the plan must be of the logits' rows")
+        _need(plan.offsets.numel() == experts + 1, "the plan must be of the logits' experts")
+    out = _out(out, (tokens, experts), logits.dtype, logits.device, dloss=dloss, logits=logits, counts=balance.counts, tokens=balance.tokens, dweights=dweights,
+               weights=weights, experts=ids)
+    d = Desc(tokens, tokens * k, experts, k, 0, 0, _TYPE[logits.dtype], 0, _RENORMALIZE if renormalize else 0, 0, stride)
+    ins = (_P * 7)(*[t.data_ptr() if t is not None else 0 for t in (dloss, logits, balance.counts, balance.tokens, dweights, weights, ids)])
+    outs = _pointers((out,))
+    return BoundCall(_function("balance_loss_backward", _PLAIN), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs)), dev,
+                     (d, ins, outs, dloss, logits, balance, plan, dweights, out), out)
 
 
 def _grouped(name: str, d: Desc, ins, out, dev: int, ws=None) -> BoundCall:

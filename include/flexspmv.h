@@ -489,6 +489,19 @@ int flexspmv_expert_route(const flexspmv_expert_desc *desc, const void *const *i
 int flexspmv_expert_route_backward(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *stream);
 
 /*
+ * Balance of the router's experts.  With counts[e] = offsets[e + 1] - offsets[e], pairs = their sum, p the softmax of a row, tokens the rows that are not
+ * all -infinity (pairs, tokens: 1 where there are none):   mean[e] = sum_t p[t, e] / tokens,   loss = experts / pairs * sum_e counts[e] mean[e].
+ *   balance_loss           in: logits (tokens x experts, any type), offsets; out: loss (f32), counts (int32), mean (f32), tokens (int32);
+ *                          workspace: _bytes, 16-byte aligned
+ *   balance_loss_backward  in: dloss (f32), logits, counts, tokens, and for the router's gradient added on top dweights, weights, experts (or null);
+ *                          out: dlogits (of the logits' type) = dloss experts / (pairs tokens) p (counts - sum_e p counts) [+ route_backward's]
+ */
+int flexspmv_balance_loss_bytes(const flexspmv_expert_desc *desc, size_t *bytes);
+int flexspmv_balance_loss(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *d_workspace, size_t workspace_bytes,
+                          void *stream);
+int flexspmv_balance_loss_backward(const flexspmv_expert_desc *desc, const void *const *inputs, void *const *outputs, void *stream);
+
+/*
  * Matrix products grouped by expert, ragged groups.  offsets (experts + 1) say which places are an expert's.
  *   grouped_matmul     in: x, weight (experts x n x k), offsets, rows (slots entries, or null: place i is x's row i); out: y (slots x n)
  *                      y[i] = weight[e] x[rows[i]]
@@ -530,6 +543,67 @@ int flexspmv_clip_gradients_bytes(int32_t count, const int64_t *lengths, size_t 
 int flexspmv_clip_gradients_plan(int32_t count, const void *const *grads, const int32_t *types, const int64_t *lengths, void *const *outs,
                                  const int32_t *out_types, void *d_workspace, size_t workspace_bytes, void *stream);
 int flexspmv_clip_gradients(int32_t pieces, int32_t write, float max_norm, float *d_norm, void *d_workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Rows of a residual stream (no reference counterpart): what stands around a routed expert layer.  flexspmv_b200/residual.py is the torch side.
+ * Rows are of any of the three types with contiguous values; inputs' rows may be apart, results are contiguous.  What a call writes may share no byte
+ * with what it reads or else writes (FLEXSPMV_ERR_BAD_ARG); every array begins on a value of its type (FLEXSPMV_ERR_ALIGN).
+ *
+ * seed: two 64-bit words in device memory, a seed and an offset; read where p > 0.  A value at (row, column) is dropped where word column % 4 of
+ * Philox4x32-10 with the key `seed` and the counter (column / 4, row, offset low, offset high) is below floor(p 2^32), else multiplied by 1 / (1 - p).
+ * A dropped value counts as 0 whatever it was.  No mask is stored: the backward pass gives the same seed and offset.
+ */
+#define FLEXSPMV_MAX_WIDTH (1 << 24)
+typedef struct flexspmv_rows_desc {
+  int64_t rows, width;
+  int64_t stride[3];       /* values between the rows of the inputs, in the order of each call; 0: contiguous */
+  int32_t type;            /* FLEXSPMV_TYPE_* of the rows                                             */
+  int32_t param_type;      /* of weight and bias and their gradients: FLEXSPMV_TYPE_F32 or the rows'   */
+  float eps;
+  int32_t reserved;        /* 0 */
+  double p;                /* 0 <= p < 1 */
+} flexspmv_rows_desc;
+
+/*
+ * layer_norm           in: x, residual (or null), weight, bias (or null: 1, 0), seed; strides: x, residual; out: y, sum (or null), mean, rstd
+ *                      s = residual + dropout(x), mean and rstd = 1 / sqrt(variance + eps) of its rows (f32), y = (s - mean) rstd weight + bias
+ * layer_norm_backward  in: dy, x (what was normalised: s), weight, mean, rstd, dsum (or null), seed; strides: dy, x, dsum;
+ *                      out: dx (p > 0), dresidual, dweight, dbias (both or neither null).
+ *                      dresidual = rstd (g - mean(g) - n mean(g n)) + dsum with n = (x - mean) rstd, g = dy weight;  dx = its values that were kept, scaled
+ *                      Workspace (_bytes, 16-byte aligned) where dweight is wanted.
+ * dropout              in: x, residual (or null), seed; strides: x, residual; out: residual + dropout(x)
+ */
+int flexspmv_layer_norm(const flexspmv_rows_desc *desc, const void *const *inputs, void *const *outputs, void *stream);
+int flexspmv_layer_norm_backward_bytes(const flexspmv_rows_desc *desc, size_t *bytes);
+int flexspmv_layer_norm_backward(const flexspmv_rows_desc *desc, const void *const *inputs, void *const *outputs, void *d_workspace,
+                                 size_t workspace_bytes, void *stream);
+int flexspmv_dropout(const flexspmv_rows_desc *desc, const void *const *inputs, void *const *outputs, void *stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection (no reference counterpart; flexspmv_b200/adapters.py is the torch side):
+ *   y[t] = weight x[t] + scale[a] b[a] (a[a] x[t]),   a = ids[t]; no adapter: y[t] = weight x[t]
+ * x (tokens x k), weight (n x k), a (adapters x rank x k), b (adapters x n x rank), y (tokens x n) of one 16-bit type; scale (adapters, f32) or null: ones.
+ * Sums are in 32 bits, y is rounded once; scale a x is kept to 2^-17 of it (float16: 2^-22) and must not exceed the type's largest value.  n, k, rank and the
+ * stride are multiples of 8, the matrices 16-byte aligned (FLEXSPMV_ERR_ALIGN).
+ *   adapter_plan       ids (tokens, int32; -1: none) -> a plan in d_plan (_bytes, 16-byte aligned), for all projections of the tokens.  d_status (or
+ *                      null) becomes FLEXSPMV_ERR_BAD_CSR where an id leaves [-1, adapters); it counts as none
+ *   adapted_project    in: x, weight, a, b, scale, the plan; out: y; workspace: _bytes, 16-byte aligned.  d_status (or null) becomes
+ *                      FLEXSPMV_ERR_TIMEOUT where a bounded wait ran out
+ */
+#define FLEXSPMV_MAX_ADAPTERS 1024
+#define FLEXSPMV_MAX_RANK 512
+typedef struct flexspmv_adapter_desc {
+  int64_t tokens;
+  int64_t x_stride;    /* values between the rows of x */
+  int32_t adapters, rank, n, k;
+  int32_t type;        /* FLEXSPMV_TYPE_BF16 or _F16 */
+  int32_t reserved;    /* 0 */
+} flexspmv_adapter_desc;
+int flexspmv_adapter_plan_bytes(const flexspmv_adapter_desc *desc, size_t *bytes);
+int flexspmv_adapter_plan(const flexspmv_adapter_desc *desc, const int32_t *d_ids, void *d_plan, size_t plan_bytes, int32_t *d_status, void *stream);
+int flexspmv_adapted_project_bytes(const flexspmv_adapter_desc *desc, size_t *bytes);
+int flexspmv_adapted_project(const flexspmv_adapter_desc *desc, const void *const *inputs, void *const *outputs, void *d_workspace, size_t workspace_bytes,
+                             int32_t *d_status, void *stream);
 
 #ifdef __cplusplus
 }
