@@ -16,59 +16,91 @@ int device_sm_count();
 // a row: counter (column / 4, row, offset), key = seed, so that a value's word goes by its place alone, whatever the launch, the strides or the type,
 // and the backward pass makes it again.
 struct Random {
-  uint32_t key0, key1, offset0, offset1;
-  __device__ __forceinline__ explicit Random(const unsigned long long* seed) {
-    const unsigned long long k = seed[0], o = seed[1];
-    key0 = (uint32_t)k; key1 = (uint32_t)(k >> 32); offset0 = (uint32_t)o; offset1 = (uint32_t)(o >> 32);
-  }
-  __device__ __forceinline__ Random() : key0(0), key1(0), offset0(0), offset1(0) {}
-  __device__ __forceinline__ void words(uint32_t group, uint32_t row, uint32_t (&w)[4]) const {
-    uint32_t c0 = group, c1 = row, c2 = offset0, c3 = offset1, k0 = key0, k1 = key1;
+  uint32_t offset1, first, second;     // the counter's last word, and what every first round makes of the one before it
+  uint32_t key0[10], key1[10];         // of the rounds; made once a thread
+  __device__ __forceinline__ Random(const unsigned long long* seed, bool used) {
+    unsigned long long k = 0, o = 0;
+    if (used) {
+      k = seed[0];
+      o = seed[1];
+    }
 #pragma unroll
     for (int i = 0; i < 10; ++i) {
+      key0[i] = (uint32_t)k + i * 0x9E3779B9u;
+      key1[i] = (uint32_t)(k >> 32) + i * 0xBB67AE85u;
+    }
+    const unsigned long long b = (o & 0xffffffffull) * 0xCD9E8D57u;
+    first = (uint32_t)(b >> 32) ^ key0[0];
+    second = (uint32_t)b;
+    offset1 = (uint32_t)(o >> 32) ^ key1[0];
+  }
+  __device__ __forceinline__ void words(uint32_t group, uint32_t row, uint32_t (&w)[4]) const {
+    const unsigned long long begin = (unsigned long long)group * 0xD2511F53u;
+    uint32_t c0 = first ^ row, c1 = second, c2 = (uint32_t)(begin >> 32) ^ offset1, c3 = (uint32_t)begin;
+#pragma unroll
+    for (int i = 1; i < 10; ++i) {
       const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
-      c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+      c0 = (uint32_t)(b >> 32) ^ c1 ^ key0[i];
       c1 = (uint32_t)b;
-      c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+      c2 = (uint32_t)(a >> 32) ^ c3 ^ key1[i];
       c3 = (uint32_t)a;
-      k0 += 0x9E3779B9u;
-      k1 += 0xBB67AE85u;
     }
     w[0] = c0; w[1] = c1; w[2] = c2; w[3] = c3;
   }
-  // C values from column c (a multiple of four) on: dropped, or scaled.
+  // C values from column c (a multiple of four) on: t plus what is kept of them, scaled.
   template <int C>
-  __device__ __forceinline__ void drop(float (&v)[C], int c, uint32_t row, uint32_t below, float scale) const {
+  __device__ __forceinline__ void drop(float (&v)[C], const float (&t)[C], int c, uint32_t row, uint32_t below, float scale) const {
     static_assert(C % 4 == 0, "whole groups");
 #pragma unroll
     for (int g = 0; g < C / 4; ++g) {
       uint32_t w[4];
       words((uint32_t)(c / 4 + g), row, w);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[g * 4 + j] = w[j] < below ? 0.f : v[g * 4 + j] * scale;
+      for (int j = 0; j < 4; ++j) v[g * 4 + j] = fmaf(w[j] < below ? 0.f : v[g * 4 + j], scale, t[g * 4 + j]);
     }
+  }
+  template <int C>
+  __device__ __forceinline__ void drop(float (&v)[C], int c, uint32_t row, uint32_t below, float scale) const {
+    float none[C];
+#pragma unroll
+    for (int j = 0; j < C; ++j) none[j] = 0.f;
+    drop(v, none, c, row, below, scale);
   }
 };
 
 // ---- rows ----------------------------------------------------------------------------------------------------------
 
-// C neighbouring values of a row, in one access (WIDE: all of them exist or none) or one by one.
+// C neighbouring values of a row as they are, in one access (WIDE: all of them exist or none) or one by one.
 template <class T, int C, bool WIDE>
-__device__ __forceinline__ void load_values(const T* row, int c, int width, float (&v)[C]) {
-  if constexpr (WIDE) {
-    Pack<T, C> q;
-    if (c < width) q.load(row + c);
-    else q.zero();
+struct Values {
+  static constexpr bool kPairs = WIDE && sizeof(T) == 2;
+  Pack<T, C> q;
+  __device__ __forceinline__ void load(const T* row, int c, int width) {
+    if constexpr (WIDE) {
+      if (c < width) q.load(row + c);
+      else q.zero();
+    } else {
+#pragma unroll
+      for (int j = 0; j < C; ++j) q.v[j] = c + j < width ? row[c + j] : from_float<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[C]) const {
 #pragma unroll
     for (int j = 0; j < C; ++j) v[j] = q.get(j);
-  } else {
-#pragma unroll
-    for (int j = 0; j < C; ++j) v[j] = c + j < width ? to_float(row[c + j]) : 0.f;
   }
+};
+template <class T, int C, bool WIDE>
+__device__ __forceinline__ void load_values(const T* row, int c, int width, float (&v)[C]) {
+  Values<T, C, WIDE> q;
+  q.load(row, c, width);
+  q.get(v);
 }
 template <class T, int C, bool WIDE>
 __device__ __forceinline__ void store_values(T* row, int c, int width, const float (&v)[C]) {
-  if constexpr (WIDE) {
+  if constexpr (WIDE && sizeof(T) == 2) {          // rounded by two: an instruction, and none to put them together
+    static_assert(C == 8, "16 bytes");
+    if (c < width) *reinterpret_cast<uint4*>(row + c) = make_uint4(two_of<T>(v[0], v[1]), two_of<T>(v[2], v[3]), two_of<T>(v[4], v[5]), two_of<T>(v[6], v[7]));
+  } else if constexpr (WIDE) {
     Pack<T, C> q;
 #pragma unroll
     for (int j = 0; j < C; ++j) q.set(j, v[j]);
@@ -128,60 +160,63 @@ struct NormArgs {
 };
 
 constexpr int row_threads(int tpr) { return tpr == 32 ? 256 : tpr; }
+// CTAs an SM that the registers leave room for: 64 a thread.
+constexpr int norm_ctas(int, int tpr) { return 1024 / row_threads(tpr); }
 
 // y = (s - mean) rstd weight + bias, s = residual + dropout(x).  Bound by memory: TPR threads hold a row in registers, L values each, so that every
 // array is read or written once; the variance is the mean square of the differences, from the registers too.  Statistics and sums in 32 bits; s is
 // normalised as it is there and rounded only where it is stored.
 template <class T, int C, bool WIDE, int L, int TPR>
-__global__ void __launch_bounds__(row_threads(TPR)) layer_norm_kernel(NormArgs a) {
+__global__ void __launch_bounds__(row_threads(TPR), norm_ctas(L, TPR)) layer_norm_kernel(NormArgs a) {
   constexpr int V = L / C, kRows = row_threads(TPR) / TPR;
   __shared__ float buf[2][1][32];
   const int at = threadIdx.x % TPR;
   int turn = 0;
   pdl_wait();
-  Random random;
-  if (a.seed) random = Random(a.seed);
+  const Random random(a.seed, a.seed != nullptr);
   const float inverse = 1.f / (float)a.width;
   for (long long r = (long long)blockIdx.x * kRows + threadIdx.x / TPR; r < a.rows; r += (long long)gridDim.x * kRows) {
     float s[V][C];
-    const T* const x = static_cast<const T*>(a.x) + r * a.x_stride;
+    Values<T, C, WIDE> x[V], t[V];
+    const T* const row = static_cast<const T*>(a.x) + r * a.x_stride;
 #pragma unroll
-    for (int i = 0; i < V; ++i) load_values<T, C, WIDE>(x, (i * TPR + at) * C, a.width, s[i]);
+    for (int i = 0; i < V; ++i) x[i].load(row, (i * TPR + at) * C, a.width);
     if (a.residual) {
-      float t[V][C];
       const T* const residual = static_cast<const T*>(a.residual) + r * a.residual_stride;
 #pragma unroll
-      for (int i = 0; i < V; ++i) load_values<T, C, WIDE>(residual, (i * TPR + at) * C, a.width, t[i]);
-      if (a.seed)
+      for (int i = 0; i < V; ++i) t[i].load(residual, (i * TPR + at) * C, a.width);
+    } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) random.drop(s[i], (i * TPR + at) * C, (uint32_t)r, a.below, a.scale);
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-#pragma unroll
-        for (int j = 0; j < C; ++j) s[i][j] += t[i][j];
-    } else if (a.seed) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) random.drop(s[i], (i * TPR + at) * C, (uint32_t)r, a.below, a.scale);
+      for (int i = 0; i < V; ++i) t[i].q.zero();
     }
-    if (a.sum)
-#pragma unroll
-      for (int i = 0; i < V; ++i) store_values<T, C, WIDE>(static_cast<T*>(a.sum) + r * a.width, (i * TPR + at) * C, a.width, s[i]);
     float total[1] = {0.f};
 #pragma unroll
-    for (int i = 0; i < V; ++i)
+    for (int i = 0; i < V; ++i) {
+      const int c = (i * TPR + at) * C;
+      float added[C];
+      x[i].get(s[i]);
+      t[i].get(added);
+      if (a.seed) {
+        random.drop(s[i], added, c, (uint32_t)r, a.below, a.scale);
+      } else {
+#pragma unroll
+        for (int j = 0; j < C; ++j) s[i][j] += added[j];
+      }
+      if (a.sum) store_values<T, C, WIDE>(static_cast<T*>(a.sum) + r * a.width, c, a.width, s[i]);
 #pragma unroll
       for (int j = 0; j < C; ++j) total[0] += s[i][j];          // beyond the width: zeros
+    }
     row_sums<TPR>(total, buf, turn);
     const float mean = total[0] * inverse;
     total[0] = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i)
+      if ((i * TPR + at) * C < a.width)
 #pragma unroll
-      for (int j = 0; j < C; ++j) {
-        s[i][j] -= mean;
-        const bool there = WIDE ? (i * TPR + at) * C < a.width : (i * TPR + at) * C + j < a.width;
-        total[0] = fmaf(there ? s[i][j] : 0.f, s[i][j], total[0]);
-      }
+        for (int j = 0; j < C; ++j) {
+          s[i][j] -= mean;
+          if (WIDE || (i * TPR + at) * C + j < a.width) total[0] = fmaf(s[i][j], s[i][j], total[0]);
+        }
     row_sums<TPR>(total, buf, turn);
     const float rstd = 1.f / sqrtf(fmaf(total[0], inverse, a.eps));
     if (at == 0) {
@@ -207,8 +242,7 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(NormArgs a) {
   __shared__ float buf[2][1][32];
   int turn = 0;
   pdl_wait();
-  Random random;
-  if (a.seed) random = Random(a.seed);
+  const Random random(a.seed, a.seed != nullptr);
   const float inverse = 1.f / (float)a.width;
   for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const auto sum_at = [&](int c, float (&s)[C]) {
@@ -269,11 +303,14 @@ struct NormGradArgs {
   uint32_t below;
 };
 
+// CTAs an SM, by the registers that the columns' sums leave.
+constexpr int norm_grad_ctas_an_sm(int l, int tpr) { return (l == 8 ? 768 : 512) / row_threads(tpr); }
+
 // With n = (x - mean) rstd and g = dy weight:  ds = rstd (g - mean(g) - n mean(g n)) + dsum,  dx = ds through the dropout,  dweight = sum over rows of
 // dy n,  dbias = sum of dy.  Bound by memory.  A CTA takes every gridDim-th row (TPR = 32: a warp does) and keeps its columns' sums in registers, so
 // that rows are read once; the CTAs' sums meet in a second launch, in the CTAs' order.
 template <class T, int C, bool WIDE, int L, int TPR>
-__global__ void __launch_bounds__(row_threads(TPR)) layer_norm_backward_kernel(NormGradArgs a) {
+__global__ void __launch_bounds__(row_threads(TPR), norm_grad_ctas_an_sm(L, TPR)) layer_norm_backward_kernel(NormGradArgs a) {
   constexpr int V = L / C, kRows = row_threads(TPR) / TPR;
   __shared__ float buf[2][2][32];
   const int at = threadIdx.x % TPR;
@@ -284,27 +321,34 @@ __global__ void __launch_bounds__(row_threads(TPR)) layer_norm_backward_kernel(N
 #pragma unroll
     for (int j = 0; j < C; ++j) dw[i][j] = db[i][j] = 0.f;
   pdl_wait();
-  Random random;
-  if (a.seed) random = Random(a.seed);
+  const Random random(a.seed, a.seed != nullptr);
   const float inverse = 1.f / (float)a.width;
   for (long long r = (long long)blockIdx.x * kRows + threadIdx.x / TPR; r < a.rows; r += (long long)gridDim.x * kRows) {
     const float mean = a.mean[r], rstd = a.rstd[r];
     float n[V][C], g[V][C];
+    Values<T, C, WIDE> x[V], dy[V], d[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      load_values<T, C, WIDE>(static_cast<const T*>(a.x) + r * a.x_stride, (i * TPR + at) * C, a.width, n[i]);
-      load_values<T, C, WIDE>(static_cast<const T*>(a.dy) + r * a.dy_stride, (i * TPR + at) * C, a.width, g[i]);
+      x[i].load(static_cast<const T*>(a.x) + r * a.x_stride, (i * TPR + at) * C, a.width);
+      dy[i].load(static_cast<const T*>(a.dy) + r * a.dy_stride, (i * TPR + at) * C, a.width);
+    }
+    if (a.dsum) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i].load(static_cast<const T*>(a.dsum) + r * a.dsum_stride, (i * TPR + at) * C, a.width);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i].q.zero();
     }
     float sums[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float w[C];
       load_params<T, C, WIDE>(a.weight, a.wide_params, (i * TPR + at) * C, a.width, 1.f, w);
+      x[i].get(n[i]);
+      dy[i].get(g[i]);
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        n[i][j] = (n[i][j] - mean) * rstd;                 // beyond the width finite or not: g is 0 there, and it is left out below
-        const bool there = WIDE ? (i * TPR + at) * C < a.width : (i * TPR + at) * C + j < a.width;
-        if (!there) n[i][j] = 0.f;
+        n[i][j] = (n[i][j] - mean) * rstd;                 // beyond the width g is 0
         dw[i][j] = fmaf(g[i][j], n[i][j], dw[i][j]);
         db[i][j] += g[i][j];
         g[i][j] *= w[j];
@@ -313,18 +357,14 @@ __global__ void __launch_bounds__(row_threads(TPR)) layer_norm_backward_kernel(N
       }
     }
     row_sums<TPR>(sums, buf, turn);
-    const float first = sums[0] * inverse, second = sums[1] * inverse;
+    const float first = -(sums[0] * inverse * rstd), second = -(sums[1] * inverse * rstd);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = (i * TPR + at) * C;
+      float added[C];
+      d[i].get(added);
 #pragma unroll
-      for (int j = 0; j < C; ++j) g[i][j] = rstd * (g[i][j] - first - n[i][j] * second);
-      if (a.dsum) {
-        float d[C];
-        load_values<T, C, WIDE>(static_cast<const T*>(a.dsum) + r * a.dsum_stride, c, a.width, d);
-#pragma unroll
-        for (int j = 0; j < C; ++j) g[i][j] += d[j];
-      }
+      for (int j = 0; j < C; ++j) g[i][j] = fmaf(n[i][j], second, fmaf(g[i][j], rstd, first)) + added[j];
       store_values<T, C, WIDE>(static_cast<T*>(a.dresidual) + r * a.width, c, a.width, g[i]);
       if (a.seed) {
         random.drop(g[i], c, (uint32_t)r, a.below, a.scale);
@@ -372,8 +412,7 @@ __global__ void __launch_bounds__(1024) layer_norm_backward_long_kernel(NormGrad
   __shared__ float buf[2][2][32];
   int turn = 0;
   pdl_wait();
-  Random random;
-  if (a.seed) random = Random(a.seed);
+  const Random random(a.seed, a.seed != nullptr);
   const float inverse = 1.f / (float)a.width;
   for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const float mean = a.mean[r], rstd = a.rstd[r];
@@ -481,38 +520,45 @@ struct DropoutArgs {
   uint32_t below;
 };
 
-// out = residual + x keep / (1 - p).  A thread takes C neighbouring columns at U places of the rows laid end to end.  Bound by memory; the generator is
-// 60 instructions for four values.
-template <class T, int C, bool WIDE, int U>
-__global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a) {
+// out = residual + x keep / (1 - p).  A thread takes C neighbouring columns at a time of the rows laid end to end, and has the next ones' loads under way.
+// Bound by memory, with the multiplier close behind: the generator's 19 products of 64 bits for four values keep it busy for four cycles each.
+template <class T, int C, bool WIDE>
+__global__ void __launch_bounds__(256, 4) dropout_kernel(DropoutArgs a) {
   pdl_wait();
-  const Random random(a.seed);
+  const Random random(a.seed, true);
   const int pieces = (a.width + C - 1) / C;
-  const long long work = a.rows * pieces;
-  for (long long i = (long long)blockIdx.x * 256 * U + threadIdx.x; i < work; i += (long long)gridDim.x * 256 * U) {
-    float v[U][C], t[U][C];
-    long long row[U];
-    int c[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long long at = i + u * 256;
-      row[u] = at >> 32 ? at / pieces : (unsigned)at / (unsigned)pieces;
-      c[u] = (int)(at - row[u] * pieces) * C;
-      if (at >= work) {
-        row[u] = 0;
-        c[u] = a.width;
-      }
-      load_values<T, C, WIDE>(static_cast<const T*>(a.x) + row[u] * a.x_stride, c[u], a.width, v[u]);
-      if (a.residual) load_values<T, C, WIDE>(static_cast<const T*>(a.residual) + row[u] * a.residual_stride, c[u], a.width, t[u]);
+  const long long work = a.rows * pieces, step = (long long)gridDim.x * 256;
+  const long long row_step = step / pieces;
+  const int piece_step = (int)(step - row_step * pieces);
+  long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= work) return;
+  long long row = i / pieces;
+  int piece = (int)(i - row * pieces);
+  Values<T, C, WIDE> x, t;
+  const auto load = [&] {
+    x.load(static_cast<const T*>(a.x) + row * a.x_stride, piece * C, a.width);
+    if (a.residual) t.load(static_cast<const T*>(a.residual) + row * a.residual_stride, piece * C, a.width);
+  };
+  t.q.zero();
+  load();
+  for (;;) {
+    float v[C], added[C];
+    x.get(v);
+    t.get(added);
+    const long long this_row = row;
+    const int c = piece * C;
+    i += step;
+    row += row_step;
+    piece += piece_step;
+    if (piece >= pieces) {
+      piece -= pieces;
+      ++row;
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      random.drop(v[u], c[u], (uint32_t)row[u], a.below, a.scale);
-      if (a.residual)
-#pragma unroll
-        for (int j = 0; j < C; ++j) v[u][j] += t[u][j];
-      store_values<T, C, WIDE>(static_cast<T*>(a.out) + row[u] * a.width, c[u], a.width, v[u]);
-    }
+    const bool more = i < work;
+    if (more) load();
+    random.drop(v, added, c, (uint32_t)this_row, a.below, a.scale);
+    store_values<T, C, WIDE>(static_cast<T*>(a.out) + this_row * a.width, c, a.width, v);
+    if (!more) break;
   }
 }
 
@@ -529,7 +575,7 @@ template <class T, int C, bool WIDE>
 static int norm_typed(const NormArgs& a, cudaStream_t st) {
   const auto go = [&](auto kernel, int tpr) {
     const int threads = row_threads(tpr);
-    return launch_pdl(kernel, row_grid(a.rows, threads / tpr, 1 << 20), threads, 0, st, a);
+    return launch_pdl(kernel, row_grid(a.rows, threads / tpr, device_sm_count() * (long long)norm_ctas(0, tpr)), threads, 0, st, a);
   };
   if (a.width <= 512) return go(layer_norm_kernel<T, C, WIDE, 16, 32>, 32);
   if (a.width <= 1024) return go(layer_norm_kernel<T, C, WIDE, 8, 128>, 128);
@@ -543,9 +589,10 @@ static int norm_typed(const NormArgs& a, cudaStream_t st) {
 // CTAs of the gradients: what an SM holds of them, times the SMs.
 static int norm_grad_ctas(long long rows, int width) {
   const int sms = device_sm_count();
-  if (width <= 512) return row_grid(rows, 8, sms * 3);
-  if (width <= 2048) return row_grid(rows, 1, sms * 5);
-  if (width <= 4096) return row_grid(rows, 1, sms * 2);
+  if (width <= 512) return row_grid(rows, 8, sms * norm_grad_ctas_an_sm(16, 32));
+  if (width <= 1024) return row_grid(rows, 1, sms * norm_grad_ctas_an_sm(8, 128));
+  if (width <= 2048) return row_grid(rows, 1, sms * norm_grad_ctas_an_sm(16, 128));
+  if (width <= 4096) return row_grid(rows, 1, sms * norm_grad_ctas_an_sm(16, 256));
   if (width <= kNormGradMost) return row_grid(rows, 1, sms);
   return row_grid(rows, 16, sms);
 }
@@ -574,10 +621,7 @@ static int norm_grad_typed(const NormGradArgs& a, cudaStream_t st) {
 
 template <class T, int C, bool WIDE>
 static int dropout_typed(const DropoutArgs& a, cudaStream_t st) {
-  const long long work = a.rows * ((a.width + C - 1) / C);
-  if (work >= (long long)device_sm_count() * 2048 * 4)
-    return launch_pdl(dropout_kernel<T, C, WIDE, 2>, row_grid(work, 512, 1 << 20), 256, 0, st, a);
-  return launch_pdl(dropout_kernel<T, C, WIDE, 1>, row_grid(work, 256, 1 << 20), 256, 0, st, a);
+  return launch_pdl(dropout_kernel<T, C, WIDE>, row_grid(a.rows * ((a.width + C - 1) / C), 256, device_sm_count() * 4ll), 256, 0, st, a);
 }
 
 // Accesses of 16 bytes where every row allows them.
