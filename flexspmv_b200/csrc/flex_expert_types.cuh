@@ -85,12 +85,13 @@ struct Pack {
   __device__ __forceinline__ void set(int i, float x) { v[i] = from_float<T>(x); }
 };
 
-// Lets a kernel have this much dynamic shared memory; the runtime is asked once for a kernel, a device and a size above 48 KB.
+// Lets a kernel have this much dynamic shared memory; the runtime is asked once for a kernel, a device and a size that with the
+// kernel's own arrays (8 KB at the most) may be above 48 KB.
 template <auto KERNEL>
 int allow_smem(int bytes) {
   static std::atomic<int> allowed[64];
   int device = 0;
-  if (bytes <= 48 * 1024) return 0;
+  if (bytes <= 40 * 1024) return 0;
   if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return (int)e;
   const bool known = device >= 0 && device < 64;
   if (known && allowed[device].load(std::memory_order_relaxed) >= bytes) return 0;

@@ -5,6 +5,7 @@
 
 #include "flex_common.cuh"
 #include "flex_expert_types.cuh"
+#include "flex_umma.cuh"
 
 namespace flex {
 
@@ -12,9 +13,14 @@ int device_sm_count();
 
 // ---- random numbers ------------------------------------------------------------------------------------------------
 
+__device__ __forceinline__ void product(uint32_t a, uint32_t b, uint32_t& high, uint32_t& low) {
+  asm("{\n\t.reg .b64 p;\n\tmul.wide.u32 p, %2, %3;\n\tmov.b64 {%1, %0}, p;\n\t}" : "=r"(high), "=r"(low) : "r"(a), "r"(b));
+}
+
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers, as easy as 1, 2, 3; 2011).  Four words for four neighbouring columns of
 // a row: counter (column / 4, row, offset), key = seed, so that a value's word goes by its place alone, whatever the launch, the strides or the type,
-// and the backward pass makes it again.
+// and the backward pass makes it again.  19 products of 64 bits for four values, of which the multiplier takes some 50 us for 2^26 values: as long as
+// DRAM takes for one array and a half of them in 16 bits.
 struct Random {
   uint32_t offset1, first, second;     // the counter's last word, and what every first round makes of the one before it
   uint32_t key0[10], key1[10];         // of the rounds; made once a thread
@@ -29,51 +35,88 @@ struct Random {
       key0[i] = (uint32_t)k + i * 0x9E3779B9u;
       key1[i] = (uint32_t)(k >> 32) + i * 0xBB67AE85u;
     }
-    const unsigned long long b = (o & 0xffffffffull) * 0xCD9E8D57u;
-    first = (uint32_t)(b >> 32) ^ key0[0];
-    second = (uint32_t)b;
+    uint32_t high;
+    product((uint32_t)o, 0xCD9E8D57u, high, second);
+    first = high ^ key0[0];
     offset1 = (uint32_t)(o >> 32) ^ key1[0];
   }
   __device__ __forceinline__ void words(uint32_t group, uint32_t row, uint32_t (&w)[4]) const {
-    const unsigned long long begin = (unsigned long long)group * 0xD2511F53u;
-    uint32_t c0 = first ^ row, c1 = second, c2 = (uint32_t)(begin >> 32) ^ offset1, c3 = (uint32_t)begin;
+    uint32_t c0 = first ^ row, c1 = second, c2, c3;
+    product(group, 0xD2511F53u, c2, c3);
+    c2 ^= offset1;
 #pragma unroll
     for (int i = 1; i < 10; ++i) {
-      const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
-      c0 = (uint32_t)(b >> 32) ^ c1 ^ key0[i];
-      c1 = (uint32_t)b;
-      c2 = (uint32_t)(a >> 32) ^ c3 ^ key1[i];
-      c3 = (uint32_t)a;
+      uint32_t a, b, low_a, low_b;
+      product(c0, 0xD2511F53u, a, low_a);
+      product(c2, 0xCD9E8D57u, b, low_b);
+      c0 = b ^ c1 ^ key0[i];
+      c1 = low_b;
+      c2 = a ^ c3 ^ key1[i];
+      c3 = low_a;
     }
     w[0] = c0; w[1] = c1; w[2] = c2; w[3] = c3;
   }
-  // C values from column c (a multiple of four) on: t plus what is kept of them, scaled.
+  // C values from column c (a multiple of four) on: t becomes t plus what is kept of them, scaled.  Not by a choice between the value and 0: a product under
+  // a predicate is an instruction less.
   template <int C>
-  __device__ __forceinline__ void drop(float (&v)[C], const float (&t)[C], int c, uint32_t row, uint32_t below, float scale) const {
+  __device__ __forceinline__ void drop(const float (&v)[C], float (&t)[C], int c, uint32_t row, uint32_t below, float scale) const {
     static_assert(C % 4 == 0, "whole groups");
 #pragma unroll
     for (int g = 0; g < C / 4; ++g) {
       uint32_t w[4];
       words((uint32_t)(c / 4 + g), row, w);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[g * 4 + j] = fmaf(w[j] < below ? 0.f : v[g * 4 + j], scale, t[g * 4 + j]);
+      for (int j = 0; j < 4; ++j)
+        if (w[j] >= below) t[g * 4 + j] = fmaf(v[g * 4 + j], scale, t[g * 4 + j]);
     }
   }
   template <int C>
   __device__ __forceinline__ void drop(float (&v)[C], int c, uint32_t row, uint32_t below, float scale) const {
-    float none[C];
+    float kept[C];
 #pragma unroll
-    for (int j = 0; j < C; ++j) none[j] = 0.f;
-    drop(v, none, c, row, below, scale);
+    for (int j = 0; j < C; ++j) kept[j] = 0.f;
+    drop(v, kept, c, row, below, scale);
+#pragma unroll
+    for (int j = 0; j < C; ++j) v[j] = kept[j];
   }
 };
+
+// ---- two values an instruction -------------------------------------------------------------------------------------
+
+struct Two {
+  float a, b;
+  __device__ __forceinline__ Two(float x, float y) : a(x), b(y) {}
+  __device__ __forceinline__ explicit Two(float x) : a(x), b(x) {}
+  __device__ __forceinline__ explicit Two(const float* p) : a(p[0]), b(p[1]) {}
+  __device__ __forceinline__ void put(float* p) const { p[0] = a; p[1] = b; }
+};
+__device__ __forceinline__ Two operator+(const Two& x, const Two& y) {
+  float a, b;
+  asm("{\n\t.reg .b64 x, y, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 r, x, y;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(a), "=f"(b)
+      : "f"(x.a), "f"(x.b), "f"(y.a), "f"(y.b));
+  return Two(a, b);
+}
+__device__ __forceinline__ Two operator*(const Two& x, const Two& y) {
+  float a, b;
+  asm("{\n\t.reg .b64 x, y, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 r, x, y;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(a), "=f"(b)
+      : "f"(x.a), "f"(x.b), "f"(y.a), "f"(y.b));
+  return Two(a, b);
+}
+__device__ __forceinline__ Two fma(const Two& x, const Two& y, const Two& z) {
+  float a, b;
+  asm("{\n\t.reg .b64 x, y, z, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 r, x, y, z;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(a), "=f"(b)
+      : "f"(x.a), "f"(x.b), "f"(y.a), "f"(y.b), "f"(z.a), "f"(z.b));
+  return Two(a, b);
+}
 
 // ---- rows ----------------------------------------------------------------------------------------------------------
 
 // C neighbouring values of a row as they are, in one access (WIDE: all of them exist or none) or one by one.
 template <class T, int C, bool WIDE>
 struct Values {
-  static constexpr bool kPairs = WIDE && sizeof(T) == 2;
   Pack<T, C> q;
   __device__ __forceinline__ void load(const T* row, int c, int width) {
     if constexpr (WIDE) {
@@ -98,8 +141,12 @@ __device__ __forceinline__ void load_values(const T* row, int c, int width, floa
 template <class T, int C, bool WIDE>
 __device__ __forceinline__ void store_values(T* row, int c, int width, const float (&v)[C]) {
   if constexpr (WIDE && sizeof(T) == 2) {          // rounded by two: an instruction, and none to put them together
-    static_assert(C == 8, "16 bytes");
-    if (c < width) *reinterpret_cast<uint4*>(row + c) = make_uint4(two_of<T>(v[0], v[1]), two_of<T>(v[2], v[3]), two_of<T>(v[4], v[5]), two_of<T>(v[6], v[7]));
+    static_assert(C % 8 == 0, "16 bytes");
+#pragma unroll
+    for (int j = 0; j < C; j += 8)
+      if (c < width)
+        *reinterpret_cast<uint4*>(row + c + j) =
+            make_uint4(two_of<T>(v[j], v[j + 1]), two_of<T>(v[j + 2], v[j + 3]), two_of<T>(v[j + 4], v[j + 5]), two_of<T>(v[j + 6], v[j + 7]));
   } else if constexpr (WIDE) {
     Pack<T, C> q;
 #pragma unroll
@@ -124,29 +171,110 @@ __device__ __forceinline__ void load_params(const void* p, bool wide_type, int c
   }
 }
 
-// Sums over the TPR threads of a row, the same bits in all of them.  `buf` alternates between two halves, so that a barrier lies between a half's reading
-// and its next writing.
+// Sums over the TPR threads of a row, the same bits in all of them; `group`: which of the CTA's rows.  `buf` (of the group) alternates between two halves,
+// so that a barrier lies between a half's reading and its next writing.
 template <int TPR, int N>
-__device__ __forceinline__ void row_sums(float (&v)[N], float (*buf)[N][32], int& turn) {
+__device__ __forceinline__ void row_sums(float (&v)[N], float (*buf)[N][32], int& turn, int group) {
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int o = 16; o; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
   if constexpr (TPR > 32) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kWarps = TPR / 32;
+    const int warp = (threadIdx.x % TPR) >> 5, lane = threadIdx.x & 31;
     if (lane == 0)
 #pragma unroll
       for (int n = 0; n < N; ++n) buf[turn][n][warp] = v[n];
-    __syncthreads();
+    named_bar_sync(1 + group, TPR);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      v[n] = lane < TPR / 32 ? buf[turn][n][lane] : 0.f;
+      if constexpr (kWarps <= 8) {             // every thread adds them up, in the same order
+        float part[kWarps];
 #pragma unroll
-      for (int o = 16; o; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+        for (int w = 0; w < kWarps; w += 4) {
+          const float4 q = *reinterpret_cast<const float4*>(&buf[turn][n][w]);
+          part[w] = q.x; part[w + 1] = q.y; part[w + 2] = q.z; part[w + 3] = q.w;
+        }
+#pragma unroll
+        for (int o = kWarps / 2; o; o >>= 1)
+#pragma unroll
+          for (int w = 0; w < o; ++w) part[w] += part[w + o];
+        v[n] = part[0];
+      } else {
+        v[n] = lane < kWarps ? buf[turn][n][lane] : 0.f;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+      }
     }
     turn ^= 1;
   }
 }
+
+// 1 / sqrt(x): the approximate one and a step of Newton's method.
+__device__ __forceinline__ float inverse_root(float x) {
+  const float y = rsqrtf(x), z = fmaf(0.5f * y, fmaf(-x * y, y, 1.f), y);
+  return x > 0.f && x < INFINITY ? z : y;
+}
+
+// ---- rows ahead ----------------------------------------------------------------------------------------------------
+
+// Many rows of 16-byte pieces: one CTA an SM, its THREADS in groups of TPR, a row each.  A thread's pieces of the rows to come are copied to shared memory, to
+// places of its own, so that no register holds them and no barrier is needed for them; PARAMS of weight and bias lie there in 32 bits, which all groups
+// share.  What it is for is bytes on their way: us, 16384 rows of 4096 in 16 bits with dropout and sum, loads of each row by itself 131.
+constexpr int kSmemAnSm = 226 * 1024;
+template <class T, int C, int L, int TPR, int THREADS, int ARRAYS, int PARAMS>
+struct Ahead {
+  static constexpr int kGroups = THREADS / TPR, kPieces = L * (int)sizeof(T) / 16, kEach = 16 / (int)sizeof(T);
+  static constexpr int kStageBytes = ARRAYS * kPieces * THREADS * 16, kParamBytes = PARAMS * L * TPR * 4;
+  static constexpr int kRoom = (kSmemAnSm - kParamBytes - 2048) / kStageBytes, kStages = kRoom > 4 ? 4 : kRoom;
+  static constexpr bool kFits = kStages >= 2;
+  static constexpr int kBytes = kParamBytes + kStages * kStageBytes;
+  uint32_t params, rows;
+  int stage = 0;
+  __device__ __forceinline__ explicit Ahead(const void* smem) : params(smem_u32(smem)), rows(smem_u32(smem) + kParamBytes) {}
+  __device__ __forceinline__ uint32_t place(int stage, int array, int piece) const {
+    return rows + (uint32_t)(stage * kStageBytes + ((array * kPieces + piece) * THREADS + (int)threadIdx.x) * 16);
+  }
+  __device__ __forceinline__ void copy(int stage, int array, const T* row, int at, int width) const {
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      const int c = (p * TPR + at) * kEach;
+      copy16(place(stage, array, p), c < width ? row + c : row, c < width ? 16 : 0);
+    }
+  }
+  // Where the row kStages - 1 ahead goes: it has been read.
+  __device__ __forceinline__ int last() const { return stage ? stage - 1 : kStages - 1; }
+  static __device__ __forceinline__ void done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory"); }
+  template <int V>
+  __device__ __forceinline__ void take(int array, Values<T, C, true> (&v)[V]) const {
+    static_assert(C == kEach, "a piece each");
+#pragma unroll
+    for (int p = 0; p < V; ++p) {
+      uint4& q = v[p].q.raw[0];
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(place(stage, array, p)));
+    }
+  }
+  __device__ __forceinline__ void next() { stage = stage + 1 == kStages ? 0 : stage + 1; }
+  // four of a thread's columns behind one another: neighbouring threads in neighbouring banks
+  __device__ __forceinline__ uint32_t param_place(int which, int four, int at) const { return params + (uint32_t)(((which * (L / 4) + four) * TPR + at) * 16); }
+  __device__ __forceinline__ void put_params(int which, int chunk, int at, const float (&v)[C]) const {
+#pragma unroll
+    for (int j = 0; j < C; j += 4)
+      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(param_place(which, (chunk * C + j) / 4, at)), "f"(v[j]), "f"(v[j + 1]), "f"(v[j + 2]),
+                   "f"(v[j + 3])
+                   : "memory");
+  }
+  __device__ __forceinline__ void get_params(int which, int chunk, int at, float (&v)[C]) const {
+#pragma unroll
+    for (int j = 0; j < C; j += 4)
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v[j]), "=f"(v[j + 1]), "=f"(v[j + 2]), "=f"(v[j + 3])
+                   : "r"(param_place(which, (chunk * C + j) / 4, at)));
+  }
+};
+
+constexpr int row_threads(int tpr) { return tpr == 32 ? 256 : tpr; }
 
 struct NormArgs {
   const void *x, *residual, *weight, *bias;
@@ -159,66 +287,102 @@ struct NormArgs {
   uint32_t below;
 };
 
-constexpr int row_threads(int tpr) { return tpr == 32 ? 256 : tpr; }
-// CTAs an SM that the registers leave room for: 64 a thread.
-constexpr int norm_ctas(int, int tpr) { return 1024 / row_threads(tpr); }
-
 // y = (s - mean) rstd weight + bias, s = residual + dropout(x).  Bound by memory: TPR threads hold a row in registers, L values each, so that every
 // array is read or written once; the variance is the mean square of the differences, from the registers too.  Statistics and sums in 32 bits; s is
-// normalised as it is there and rounded only where it is stored.
-template <class T, int C, bool WIDE, int L, int TPR>
-__global__ void __launch_bounds__(row_threads(TPR), norm_ctas(L, TPR)) layer_norm_kernel(NormArgs a) {
-  constexpr int V = L / C, kRows = row_threads(TPR) / TPR;
-  __shared__ float buf[2][1][32];
-  const int at = threadIdx.x % TPR;
+// normalised as it is there and rounded only where it is stored.  AHEAD: 0 (a CTA a row, or a warp), or the arrays that are read, whose rows are copied ahead.
+constexpr int kAheadThreads = 1024;
+template <class T, int C, bool WIDE, int L, int TPR, bool DROP, int AHEAD>
+__global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEAD ? 1 : 1024 / row_threads(TPR)) layer_norm_kernel(NormArgs a) {
+  constexpr int V = L / C, kThreads = AHEAD ? kAheadThreads : row_threads(TPR), kRows = kThreads / TPR;
+  extern __shared__ __align__(16) unsigned char rows_sm[];
+  __shared__ __align__(16) float buf[kRows][2][1][32];
+  const int at = threadIdx.x % TPR, group = threadIdx.x / TPR;
   int turn = 0;
   pdl_wait();
-  const Random random(a.seed, a.seed != nullptr);
+  const Random random(a.seed, DROP);
   const float inverse = 1.f / (float)a.width;
-  for (long long r = (long long)blockIdx.x * kRows + threadIdx.x / TPR; r < a.rows; r += (long long)gridDim.x * kRows) {
+  const long long step = (long long)gridDim.x * kRows, from = (long long)blockIdx.x * kRows + group;
+  Ahead<T, C, L, TPR, kThreads, AHEAD ? AHEAD : 1, 2> next(rows_sm);
+  const T *next_x = static_cast<const T*>(a.x) + from * a.x_stride, *next_t = static_cast<const T*>(a.residual) + from * a.residual_stride;
+  long long ahead = from;
+  const auto copy_next = [&](int to) {
+    if (ahead < a.rows) {
+      next.copy(to, 0, next_x, at, a.width);
+      if (AHEAD == 2) next.copy(to, 1, next_t, at, a.width);
+    }
+    next.done();
+    ahead += step;
+    next_x += step * a.x_stride;
+    next_t += step * a.residual_stride;
+  };
+  if constexpr (AHEAD > 0) {
+    for (int i = 0; i + 1 < next.kStages; ++i) copy_next(i);
+    if (group == 0)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float p[C];
+        load_params<T, C, WIDE>(a.weight, a.wide_params, (i * TPR + at) * C, a.width, 1.f, p);
+        next.put_params(0, i, at, p);
+        load_params<T, C, WIDE>(a.bias, a.wide_params, (i * TPR + at) * C, a.width, 0.f, p);
+        next.put_params(1, i, at, p);
+      }
+    __syncthreads();
+  }
+  for (long long r = from; r < a.rows; r += step) {
     float s[V][C];
     Values<T, C, WIDE> x[V], t[V];
-    const T* const row = static_cast<const T*>(a.x) + r * a.x_stride;
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i].load(row, (i * TPR + at) * C, a.width);
-    if (a.residual) {
-      const T* const residual = static_cast<const T*>(a.residual) + r * a.residual_stride;
-#pragma unroll
-      for (int i = 0; i < V; ++i) t[i].load(residual, (i * TPR + at) * C, a.width);
+    const bool sum = AHEAD ? AHEAD == 2 : a.residual != nullptr;
+    if constexpr (AHEAD > 0) {
+      copy_next(next.last());
+      next.wait();
+      next.take(0, x);
+      if (AHEAD == 2) next.take(1, t);
+      next.next();
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) t[i].q.zero();
+      for (int i = 0; i < V; ++i) x[i].load(static_cast<const T*>(a.x) + r * a.x_stride, (i * TPR + at) * C, a.width);
+      if (sum)
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i].load(static_cast<const T*>(a.residual) + r * a.residual_stride, (i * TPR + at) * C, a.width);
     }
-    float total[1] = {0.f};
+    if (!sum)
+#pragma unroll
+      for (int i = 0; i < V; ++i) t[i].q.zero();
+    Two two(0.f);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = (i * TPR + at) * C;
-      float added[C];
-      x[i].get(s[i]);
-      t[i].get(added);
-      if (a.seed) {
-        random.drop(s[i], added, c, (uint32_t)r, a.below, a.scale);
+      float v[C];
+      x[i].get(v);
+      t[i].get(s[i]);
+      if (DROP) {
+        random.drop(v, s[i], c, (uint32_t)r, a.below, a.scale);
       } else {
 #pragma unroll
-        for (int j = 0; j < C; ++j) s[i][j] += added[j];
+        for (int j = 0; j < C; j += 2) (Two(s[i] + j) + Two(v + j)).put(s[i] + j);
       }
-      if (a.sum) store_values<T, C, WIDE>(static_cast<T*>(a.sum) + r * a.width, c, a.width, s[i]);
+      if (DROP || sum) store_values<T, C, WIDE>(static_cast<T*>(a.sum) + r * a.width, c, a.sum ? a.width : 0, s[i]);
 #pragma unroll
-      for (int j = 0; j < C; ++j) total[0] += s[i][j];          // beyond the width: zeros
+      for (int j = 0; j < C; j += 2) two = two + Two(s[i] + j);          // beyond the width: zeros
     }
-    row_sums<TPR>(total, buf, turn);
+    float total[1] = {two.a + two.b};
+    row_sums<TPR>(total, buf[group], turn, group);
     const float mean = total[0] * inverse;
-    total[0] = 0.f;
+    two = Two(0.f);
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if ((i * TPR + at) * C < a.width)
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-          s[i][j] -= mean;
-          if (WIDE || (i * TPR + at) * C + j < a.width) total[0] = fmaf(s[i][j], s[i][j], total[0]);
+        for (int j = 0; j < C; j += 2) {
+          Two d = Two(s[i] + j) + Two(-mean);
+          d.put(s[i] + j);
+          if (!WIDE && (i * TPR + at) * C + j >= a.width) d.a = 0.f;
+          if (!WIDE && (i * TPR + at) * C + j + 1 >= a.width) d.b = 0.f;
+          two = fma(d, d, two);
         }
-    row_sums<TPR>(total, buf, turn);
-    const float rstd = 1.f / sqrtf(fmaf(total[0], inverse, a.eps));
+    total[0] = two.a + two.b;
+    row_sums<TPR>(total, buf[group], turn, group);
+    const float rstd = inverse_root(fmaf(total[0], inverse, a.eps));
     if (at == 0) {
       a.mean[r] = mean;
       a.rstd[r] = rstd;
@@ -227,10 +391,15 @@ __global__ void __launch_bounds__(row_threads(TPR), norm_ctas(L, TPR)) layer_nor
     for (int i = 0; i < V; ++i) {
       float w[C], b[C];
       const int c = (i * TPR + at) * C;
-      load_params<T, C, WIDE>(a.weight, a.wide_params, c, a.width, 1.f, w);
-      load_params<T, C, WIDE>(a.bias, a.wide_params, c, a.width, 0.f, b);
+      if constexpr (AHEAD > 0) {
+        next.get_params(0, i, at, w);
+        next.get_params(1, i, at, b);
+      } else {
+        load_params<T, C, WIDE>(a.weight, a.wide_params, c, a.width, 1.f, w);
+        load_params<T, C, WIDE>(a.bias, a.wide_params, c, a.width, 0.f, b);
+      }
 #pragma unroll
-      for (int j = 0; j < C; ++j) s[i][j] = fmaf(s[i][j] * rstd, w[j], b[j]);
+      for (int j = 0; j < C; j += 2) fma(Two(s[i] + j) * Two(rstd), Two(w + j), Two(b + j)).put(s[i] + j);
       store_values<T, C, WIDE>(static_cast<T*>(a.y) + r * a.width, c, a.width, s[i]);
     }
   }
@@ -239,7 +408,7 @@ __global__ void __launch_bounds__(row_threads(TPR), norm_ctas(L, TPR)) layer_nor
 // Rows beyond what registers hold: the row is read three times, from L2 as a rule.
 template <class T, int C, bool WIDE>
 __global__ void __launch_bounds__(1024) layer_norm_long_kernel(NormArgs a) {
-  __shared__ float buf[2][1][32];
+  __shared__ __align__(16) float buf[2][1][32];
   int turn = 0;
   pdl_wait();
   const Random random(a.seed, a.seed != nullptr);
@@ -247,10 +416,18 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(NormArgs a) {
   for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const auto sum_at = [&](int c, float (&s)[C]) {
       load_values<T, C, WIDE>(static_cast<const T*>(a.x) + r * a.x_stride, c, a.width, s);
-      if (a.seed) random.drop(s, c, (uint32_t)r, a.below, a.scale);
+      float t[C];
       if (a.residual) {
-        float t[C];
         load_values<T, C, WIDE>(static_cast<const T*>(a.residual) + r * a.residual_stride, c, a.width, t);
+      } else {
+#pragma unroll
+        for (int j = 0; j < C; ++j) t[j] = 0.f;
+      }
+      if (a.seed) {
+        random.drop(s, t, c, (uint32_t)r, a.below, a.scale);
+#pragma unroll
+        for (int j = 0; j < C; ++j) s[j] = t[j];
+      } else {
 #pragma unroll
         for (int j = 0; j < C; ++j) s[j] += t[j];
       }
@@ -261,7 +438,7 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(NormArgs a) {
 #pragma unroll
       for (int j = 0; j < C; ++j) total[0] += s[j];
     }
-    row_sums<1024>(total, buf, turn);
+    row_sums<1024>(total, buf, turn, 0);
     const float mean = total[0] * inverse;
     total[0] = 0.f;
     for (int c = threadIdx.x * C; c < a.width; c += 1024 * C) {
@@ -271,8 +448,8 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(NormArgs a) {
       for (int j = 0; j < C; ++j)
         if (c + j < a.width) total[0] = fmaf(s[j] - mean, s[j] - mean, total[0]);
     }
-    row_sums<1024>(total, buf, turn);
-    const float rstd = 1.f / sqrtf(fmaf(total[0], inverse, a.eps));
+    row_sums<1024>(total, buf, turn, 0);
+    const float rstd = inverse_root(fmaf(total[0], inverse, a.eps));
     if (threadIdx.x == 0) {
       a.mean[r] = mean;
       a.rstd[r] = rstd;
@@ -303,17 +480,18 @@ struct NormGradArgs {
   uint32_t below;
 };
 
-// CTAs an SM, by the registers that the columns' sums leave.
-constexpr int norm_grad_ctas_an_sm(int l, int tpr) { return (l == 8 ? 768 : 512) / row_threads(tpr); }
-
 // With n = (x - mean) rstd and g = dy weight:  ds = rstd (g - mean(g) - n mean(g n)) + dsum,  dx = ds through the dropout,  dweight = sum over rows of
-// dy n,  dbias = sum of dy.  Bound by memory.  A CTA takes every gridDim-th row (TPR = 32: a warp does) and keeps its columns' sums in registers, so
-// that rows are read once; the CTAs' sums meet in a second launch, in the CTAs' order.
-template <class T, int C, bool WIDE, int L, int TPR>
-__global__ void __launch_bounds__(row_threads(TPR), norm_grad_ctas_an_sm(L, TPR)) layer_norm_backward_kernel(NormGradArgs a) {
-  constexpr int V = L / C, kRows = row_threads(TPR) / TPR;
-  __shared__ float buf[2][2][32];
-  const int at = threadIdx.x % TPR;
+// dy n,  dbias = sum of dy.  Bound by memory.  TPR threads take every so-many-th row and keep its columns' sums in registers (which leave room for 512 threads
+// an SM), so that rows are read once; the groups' sums meet in shared memory, the CTAs' in a second launch, each in a fixed order.
+constexpr int kAheadGradThreads = 512;
+constexpr int norm_grad_threads(int l) { return l == 8 ? 768 : 512; }          // an SM
+template <class T, int C, bool WIDE, int L, int TPR, bool DROP, bool AHEAD>
+__global__ void __launch_bounds__(AHEAD ? kAheadGradThreads : row_threads(TPR), AHEAD ? 1 : norm_grad_threads(L) / row_threads(TPR))
+    layer_norm_backward_kernel(NormGradArgs a) {
+  constexpr int V = L / C, kThreads = AHEAD ? kAheadGradThreads : row_threads(TPR), kRows = kThreads / TPR;
+  extern __shared__ __align__(16) unsigned char rows_sm[];
+  __shared__ __align__(16) float buf[kRows][2][2][32];
+  const int at = threadIdx.x % TPR, group = threadIdx.x / TPR;
   int turn = 0;
   float dw[V][C], db[V][C];
 #pragma unroll
@@ -321,52 +499,102 @@ __global__ void __launch_bounds__(row_threads(TPR), norm_grad_ctas_an_sm(L, TPR)
 #pragma unroll
     for (int j = 0; j < C; ++j) dw[i][j] = db[i][j] = 0.f;
   pdl_wait();
-  const Random random(a.seed, a.seed != nullptr);
+  const Random random(a.seed, DROP);
   const float inverse = 1.f / (float)a.width;
-  for (long long r = (long long)blockIdx.x * kRows + threadIdx.x / TPR; r < a.rows; r += (long long)gridDim.x * kRows) {
-    const float mean = a.mean[r], rstd = a.rstd[r];
+  const long long step = (long long)gridDim.x * kRows, from = (long long)blockIdx.x * kRows + group;
+  Ahead<T, C, L, TPR, kThreads, 3, 1> next(rows_sm);
+  const T *next_x = static_cast<const T*>(a.x) + from * a.x_stride, *next_y = static_cast<const T*>(a.dy) + from * a.dy_stride,
+          *next_d = static_cast<const T*>(a.dsum) + from * a.dsum_stride;
+  long long ahead = from;
+  const auto copy_next = [&](int to) {
+    if (ahead < a.rows) {
+      next.copy(to, 0, next_x, at, a.width);
+      next.copy(to, 1, next_y, at, a.width);
+      if (a.dsum) next.copy(to, 2, next_d, at, a.width);
+    }
+    next.done();
+    ahead += step;
+    next_x += step * a.x_stride;
+    next_y += step * a.dy_stride;
+    next_d += step * a.dsum_stride;
+  };
+  float next_mean = 0.f, next_rstd = 0.f;
+  if (from < a.rows) {
+    next_mean = a.mean[from];
+    next_rstd = a.rstd[from];
+  }
+  if constexpr (AHEAD) {
+    for (int i = 0; i + 1 < next.kStages; ++i) copy_next(i);
+    if (group == 0)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float p[C];
+        load_params<T, C, WIDE>(a.weight, a.wide_params, (i * TPR + at) * C, a.width, 1.f, p);
+        next.put_params(0, i, at, p);
+      }
+    __syncthreads();
+  }
+  for (long long r = from; r < a.rows; r += step) {
+    const float mean = next_mean, rstd = next_rstd;
+    if (r + step < a.rows) {
+      next_mean = a.mean[r + step];
+      next_rstd = a.rstd[r + step];
+    }
     float n[V][C], g[V][C];
     Values<T, C, WIDE> x[V], dy[V], d[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      x[i].load(static_cast<const T*>(a.x) + r * a.x_stride, (i * TPR + at) * C, a.width);
-      dy[i].load(static_cast<const T*>(a.dy) + r * a.dy_stride, (i * TPR + at) * C, a.width);
-    }
-    if (a.dsum) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) d[i].load(static_cast<const T*>(a.dsum) + r * a.dsum_stride, (i * TPR + at) * C, a.width);
+    if constexpr (AHEAD) {
+      copy_next(next.last());
+      next.wait();
+      next.take(0, x);
+      next.take(1, dy);
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) d[i].q.zero();
+      for (int i = 0; i < V; ++i) {
+        x[i].load(static_cast<const T*>(a.x) + r * a.x_stride, (i * TPR + at) * C, a.width);
+        dy[i].load(static_cast<const T*>(a.dy) + r * a.dy_stride, (i * TPR + at) * C, a.width);
+      }
+      if (a.dsum)
+#pragma unroll
+        for (int i = 0; i < V; ++i) d[i].load(static_cast<const T*>(a.dsum) + r * a.dsum_stride, (i * TPR + at) * C, a.width);
     }
-    float sums[2] = {0.f, 0.f};
+    Two one(0.f), two(0.f);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float w[C];
-      load_params<T, C, WIDE>(a.weight, a.wide_params, (i * TPR + at) * C, a.width, 1.f, w);
+      if constexpr (AHEAD) next.get_params(0, i, at, w);
+      else load_params<T, C, WIDE>(a.weight, a.wide_params, (i * TPR + at) * C, a.width, 1.f, w);
       x[i].get(n[i]);
       dy[i].get(g[i]);
 #pragma unroll
-      for (int j = 0; j < C; ++j) {
-        n[i][j] = (n[i][j] - mean) * rstd;                 // beyond the width g is 0
-        dw[i][j] = fmaf(g[i][j], n[i][j], dw[i][j]);
-        db[i][j] += g[i][j];
-        g[i][j] *= w[j];
-        sums[0] += g[i][j];
-        sums[1] = fmaf(g[i][j], n[i][j], sums[1]);
+      for (int j = 0; j < C; j += 2) {
+        const Two normed = (Two(n[i] + j) + Two(-mean)) * Two(rstd), y(g[i] + j), scaled = y * Two(w + j);          // beyond the width y is 0
+        normed.put(n[i] + j);
+        scaled.put(g[i] + j);
+        fma(y, normed, Two(dw[i] + j)).put(dw[i] + j);
+        (Two(db[i] + j) + y).put(db[i] + j);
+        one = one + scaled;
+        two = fma(scaled, normed, two);
       }
     }
-    row_sums<TPR>(sums, buf, turn);
+    float sums[2] = {one.a + one.b, two.a + two.b};
+    row_sums<TPR>(sums, buf[group], turn, group);
     const float first = -(sums[0] * inverse * rstd), second = -(sums[1] * inverse * rstd);
+    if constexpr (AHEAD) {
+      if (a.dsum) next.take(2, d);
+      next.next();
+    }
+    if (!a.dsum)
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i].q.zero();
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = (i * TPR + at) * C;
       float added[C];
       d[i].get(added);
 #pragma unroll
-      for (int j = 0; j < C; ++j) g[i][j] = fmaf(n[i][j], second, fmaf(g[i][j], rstd, first)) + added[j];
+      for (int j = 0; j < C; j += 2) (fma(Two(n[i] + j), Two(second), fma(Two(g[i] + j), Two(rstd), Two(first))) + Two(added + j)).put(g[i] + j);
       store_values<T, C, WIDE>(static_cast<T*>(a.dresidual) + r * a.width, c, a.width, g[i]);
-      if (a.seed) {
+      if (DROP) {
         random.drop(g[i], c, (uint32_t)r, a.below, a.scale);
         store_values<T, C, WIDE>(static_cast<T*>(a.dx) + r * a.width, c, a.width, g[i]);
       }
@@ -374,23 +602,25 @@ __global__ void __launch_bounds__(row_threads(TPR), norm_grad_ctas_an_sm(L, TPR)
   }
   if (!a.parts) return;
   float* const mine = a.parts + (size_t)blockIdx.x * 2 * a.width;
-  if constexpr (kRows > 1) {                 // the warps' sums, one after the other
-    __shared__ float joined[2][L * 32];
+  if constexpr (kRows > 1) {                 // the groups' sums, one after the other, over the stages
+    float* const joined = reinterpret_cast<float*>(rows_sm);
+    copy16_wait_all();
+    __syncthreads();
     for (int w = 0; w < kRows; ++w) {
-      if ((int)threadIdx.x / TPR == w)
+      if (group == w)
 #pragma unroll
         for (int i = 0; i < V; ++i)
 #pragma unroll
           for (int j = 0; j < C; ++j) {
             const int c = (i * TPR + at) * C + j;
-            joined[0][c] = w ? joined[0][c] + dw[i][j] : dw[i][j];
-            joined[1][c] = w ? joined[1][c] + db[i][j] : db[i][j];
+            joined[c] = w ? joined[c] + dw[i][j] : dw[i][j];
+            joined[L * TPR + c] = w ? joined[L * TPR + c] + db[i][j] : db[i][j];
           }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < a.width; c += row_threads(TPR)) {
-      mine[c] = joined[0][c];
-      mine[a.width + c] = joined[1][c];
+    for (int c = threadIdx.x; c < a.width; c += kThreads) {
+      mine[c] = joined[c];
+      mine[a.width + c] = joined[L * TPR + c];
     }
   } else {
 #pragma unroll
@@ -409,7 +639,7 @@ __global__ void __launch_bounds__(row_threads(TPR), norm_grad_ctas_an_sm(L, TPR)
 // Rows beyond what registers hold: read twice, and the columns' sums by the kernel after this one.
 template <class T, int C, bool WIDE>
 __global__ void __launch_bounds__(1024) layer_norm_backward_long_kernel(NormGradArgs a) {
-  __shared__ float buf[2][2][32];
+  __shared__ __align__(16) float buf[2][2][32];
   int turn = 0;
   pdl_wait();
   const Random random(a.seed, a.seed != nullptr);
@@ -436,7 +666,7 @@ __global__ void __launch_bounds__(1024) layer_norm_backward_long_kernel(NormGrad
         sums[1] = fmaf(g[j], n[j], sums[1]);
       }
     }
-    row_sums<1024>(sums, buf, turn);
+    row_sums<1024>(sums, buf, turn, 0);
     const float first = sums[0] * inverse, second = sums[1] * inverse;
     for (int c = threadIdx.x * C; c < a.width; c += 1024 * C) {
       values_at(c, n, g);
@@ -521,9 +751,10 @@ struct DropoutArgs {
 };
 
 // out = residual + x keep / (1 - p).  A thread takes C neighbouring columns at a time of the rows laid end to end, and has the next ones' loads under way.
-// Bound by memory, with the multiplier close behind: the generator's 19 products of 64 bits for four values keep it busy for four cycles each.
+// Bound by memory (2^26 values in 16 bits and as many added: 6.26 TB/s), with the generator close behind, which is why C is 32 bytes where the width allows: what a
+// thread does for a place and not for a value is shared by twice as many (64.4 us, with 16 bytes 80.6).
 template <class T, int C, bool WIDE>
-__global__ void __launch_bounds__(256, 4) dropout_kernel(DropoutArgs a) {
+__global__ void __launch_bounds__(256, 3) dropout_kernel(DropoutArgs a) {
   pdl_wait();
   const Random random(a.seed, true);
   const int pieces = (a.width + C - 1) / C;
@@ -557,7 +788,7 @@ __global__ void __launch_bounds__(256, 4) dropout_kernel(DropoutArgs a) {
     const bool more = i < work;
     if (more) load();
     random.drop(v, added, c, (uint32_t)this_row, a.below, a.scale);
-    store_values<T, C, WIDE>(static_cast<T*>(a.out) + this_row * a.width, c, a.width, v);
+    store_values<T, C, WIDE>(static_cast<T*>(a.out) + this_row * a.width, c, a.width, added);
     if (!more) break;
   }
 }
@@ -571,42 +802,78 @@ static int row_grid(long long rows, int rows_a_cta, long long most) {
   return (int)(want < 1 ? 1 : want > most ? most : want);
 }
 
-template <class T, int C, bool WIDE>
-static int norm_typed(const NormArgs& a, cudaStream_t st) {
-  const auto go = [&](auto kernel, int tpr) {
-    const int threads = row_threads(tpr);
-    return launch_pdl(kernel, row_grid(a.rows, threads / tpr, device_sm_count() * (long long)norm_ctas(0, tpr)), threads, 0, st, a);
+// Rows are copied ahead where each group of an SM has some to copy.
+static bool many_rows(long long rows, int groups) { return rows >= 2ll * groups * device_sm_count(); }
+
+template <class T, int C, bool WIDE, int L, int TPR, bool DROP>
+static int norm_launch(const NormArgs& a, cudaStream_t st) {
+  const auto ahead = [&](auto arrays) {
+    using Next = Ahead<T, C, L, TPR, kAheadThreads, decltype(arrays)::value, 2>;
+    constexpr auto kernel = layer_norm_kernel<T, C, WIDE, L, TPR, DROP, decltype(arrays)::value>;
+    if (int e = allow_smem<kernel>(Next::kBytes)) return e;
+    return launch_pdl(kernel, row_grid(a.rows, Next::kGroups, device_sm_count()), kAheadThreads, Next::kBytes, st, a);
   };
-  if (a.width <= 512) return go(layer_norm_kernel<T, C, WIDE, 16, 32>, 32);
-  if (a.width <= 1024) return go(layer_norm_kernel<T, C, WIDE, 8, 128>, 128);
-  if (a.width <= 2048) return go(layer_norm_kernel<T, C, WIDE, 16, 128>, 128);
-  if (a.width <= 4096) return go(layer_norm_kernel<T, C, WIDE, 16, 256>, 256);
-  if (a.width <= 8192) return go(layer_norm_kernel<T, C, WIDE, 16, 512>, 512);
-  if (a.width <= kNormMost) return go(layer_norm_kernel<T, C, WIDE, 16, 1024>, 1024);
-  return go(layer_norm_long_kernel<T, C, WIDE>, 1024);
+  if constexpr (WIDE) {
+    if (many_rows(a.rows, kAheadThreads / TPR)) {
+      if constexpr (Ahead<T, C, L, TPR, kAheadThreads, 2, 2>::kFits)
+        return a.residual ? ahead(std::integral_constant<int, 2>()) : ahead(std::integral_constant<int, 1>());
+    }
+  }
+  constexpr int kThreads = row_threads(TPR);
+  return launch_pdl(layer_norm_kernel<T, C, WIDE, L, TPR, DROP, 0>, row_grid(a.rows, kThreads / TPR, device_sm_count() * (1024ll / kThreads)), kThreads, 0, st, a);
 }
 
-// CTAs of the gradients: what an SM holds of them, times the SMs.
+template <class T, int C, bool WIDE, bool DROP>
+static int norm_typed(const NormArgs& a, cudaStream_t st) {
+  if (a.width <= 256) return norm_launch<T, C, WIDE, 8, 32, DROP>(a, st);
+  if constexpr (sizeof(T) == 2)
+    if (a.width <= 512) return norm_launch<T, C, WIDE, 16, 32, DROP>(a, st);
+  if (a.width <= 1024) return norm_launch<T, C, WIDE, 8, 128, DROP>(a, st);
+  // 16 values a thread where they are of 16 bits, else 8: as many bytes
+  constexpr int L = (int)sizeof(T) == 2 ? 16 : 8;
+  if (a.width <= 128 * L) return norm_launch<T, C, WIDE, L, 128, DROP>(a, st);
+  if (a.width <= 256 * L) return norm_launch<T, C, WIDE, L, 256, DROP>(a, st);
+  if (a.width <= 512 * L) return norm_launch<T, C, WIDE, L, 512, DROP>(a, st);
+  if (a.width <= 1024 * L) return norm_launch<T, C, WIDE, L, 1024, DROP>(a, st);
+  if (a.width <= kNormMost) return norm_launch<T, C, WIDE, 16, 1024, DROP>(a, st);
+  return launch_pdl(layer_norm_long_kernel<T, C, WIDE>, row_grid(a.rows, 1, 1 << 20), 1024, 0, st, a);
+}
+
+// CTAs that may leave sums of their rows, of any variant.
 static int norm_grad_ctas(long long rows, int width) {
   const int sms = device_sm_count();
-  if (width <= 512) return row_grid(rows, 8, sms * norm_grad_ctas_an_sm(16, 32));
-  if (width <= 1024) return row_grid(rows, 1, sms * norm_grad_ctas_an_sm(8, 128));
-  if (width <= 2048) return row_grid(rows, 1, sms * norm_grad_ctas_an_sm(16, 128));
-  if (width <= 4096) return row_grid(rows, 1, sms * norm_grad_ctas_an_sm(16, 256));
+  if (width <= 512) return row_grid(rows, 8, sms * 2);
+  if (width <= 1024) return row_grid(rows, 1, sms * 6);
+  if (width <= 2048) return row_grid(rows, 1, sms * 4);
+  if (width <= 4096) return row_grid(rows, 1, sms * 2);
   if (width <= kNormGradMost) return row_grid(rows, 1, sms);
   return row_grid(rows, 16, sms);
 }
 
-template <class T, int C, bool WIDE>
+template <class T, int C, bool WIDE, int L, int TPR, bool DROP>
+static int norm_grad_launch(const NormGradArgs& a, int& ctas, cudaStream_t st) {
+  if constexpr (WIDE) {
+    using Next = Ahead<T, C, L, TPR, kAheadGradThreads, 3, 1>;
+    static_assert(Next::kFits && Next::kBytes >= 8 * L * TPR, "stages, and the groups' sums over them");
+    if (many_rows(a.rows, Next::kGroups)) {
+      constexpr auto kernel = layer_norm_backward_kernel<T, C, WIDE, L, TPR, DROP, true>;
+      if (int e = allow_smem<kernel>(Next::kBytes)) return e;
+      ctas = row_grid(a.rows, Next::kGroups, device_sm_count());
+      return launch_pdl(kernel, (unsigned)ctas, kAheadGradThreads, Next::kBytes, st, a);
+    }
+  }
+  constexpr int kThreads = row_threads(TPR);
+  return launch_pdl(layer_norm_backward_kernel<T, C, WIDE, L, TPR, DROP, false>, (unsigned)ctas, kThreads, kThreads > TPR ? 8 * L * TPR : 0, st, a);
+}
+
+template <class T, int C, bool WIDE, bool DROP>
 static int norm_grad_typed(const NormGradArgs& a, cudaStream_t st) {
-  const int ctas = norm_grad_ctas(a.rows, a.width);
-  const auto go = [&](auto kernel, int threads) { return launch_pdl(kernel, (unsigned)ctas, threads, 0, st, a); };
-  int e;
-  if (a.width <= 512) e = go(layer_norm_backward_kernel<T, C, WIDE, 16, 32>, 256);
-  else if (a.width <= 1024) e = go(layer_norm_backward_kernel<T, C, WIDE, 8, 128>, 128);
-  else if (a.width <= 2048) e = go(layer_norm_backward_kernel<T, C, WIDE, 16, 128>, 128);
-  else if (a.width <= 4096) e = go(layer_norm_backward_kernel<T, C, WIDE, 16, 256>, 256);
-  else if (a.width <= kNormGradMost) e = go(layer_norm_backward_kernel<T, C, WIDE, 16, 512>, 512);
+  int ctas = norm_grad_ctas(a.rows, a.width), e;
+  if (a.width <= 512) e = norm_grad_launch<T, C, WIDE, 16, 32, DROP>(a, ctas, st);
+  else if (a.width <= 1024) e = norm_grad_launch<T, C, WIDE, 8, 128, DROP>(a, ctas, st);
+  else if (a.width <= 2048) e = norm_grad_launch<T, C, WIDE, 16, 128, DROP>(a, ctas, st);
+  else if (a.width <= 4096) e = norm_grad_launch<T, C, WIDE, 16, 256, DROP>(a, ctas, st);
+  else if (a.width <= kNormGradMost) e = norm_grad_launch<T, C, WIDE, 16, 512, DROP>(a, ctas, st);
   else {
     e = launch_pdl(layer_norm_backward_long_kernel<T, C, WIDE>, row_grid(a.rows, 1, 1 << 20), 1024, 0, st, a);
     if (e || !a.parts) return e;
@@ -621,7 +888,7 @@ static int norm_grad_typed(const NormGradArgs& a, cudaStream_t st) {
 
 template <class T, int C, bool WIDE>
 static int dropout_typed(const DropoutArgs& a, cudaStream_t st) {
-  return launch_pdl(dropout_kernel<T, C, WIDE>, row_grid(a.rows * ((a.width + C - 1) / C), 256, device_sm_count() * 4ll), 256, 0, st, a);
+  return launch_pdl(dropout_kernel<T, C, WIDE>, row_grid(a.rows * ((a.width + C - 1) / C), 256, device_sm_count() * 3ll), 256, 0, st, a);
 }
 
 // Accesses of 16 bytes where every row allows them.
@@ -682,7 +949,11 @@ int flexspmv_layer_norm(const flexspmv_rows_desc* d, const void* const* in, void
                     wide_rows(d->type, d->width, d->width, out[1]) && aligned16(in[2]) && aligned16(in[3]);
   return by_type(d->type, [&](auto zero) {
     using T = decltype(zero);
-    return wide ? norm_typed<T, 16 / (int)sizeof(T), true>(a, static_cast<cudaStream_t>(stream)) : norm_typed<T, 4, false>(a, static_cast<cudaStream_t>(stream));
+    const auto go = [&](auto drop) {
+      constexpr bool kDrop = decltype(drop)::value;
+      return wide ? norm_typed<T, 16 / (int)sizeof(T), true, kDrop>(a, static_cast<cudaStream_t>(stream)) : norm_typed<T, 4, false, kDrop>(a, static_cast<cudaStream_t>(stream));
+    };
+    return a.seed ? go(std::true_type()) : go(std::false_type());
   });
 }
 
@@ -719,8 +990,12 @@ int flexspmv_layer_norm_backward(const flexspmv_rows_desc* d, const void* const*
                     wide_rows(d->type, d->width, d->width, d->p > 0.0 ? out[0] : nullptr) && wide_rows(d->type, d->width, d->width, out[1]) && aligned16(in[2]);
   return by_type(d->type, [&](auto zero) {
     using T = decltype(zero);
-    return wide ? norm_grad_typed<T, 16 / (int)sizeof(T), true>(a, static_cast<cudaStream_t>(stream))
-                : norm_grad_typed<T, 4, false>(a, static_cast<cudaStream_t>(stream));
+    const auto go = [&](auto drop) {
+      constexpr bool kDrop = decltype(drop)::value;
+      return wide ? norm_grad_typed<T, 16 / (int)sizeof(T), true, kDrop>(a, static_cast<cudaStream_t>(stream))
+                  : norm_grad_typed<T, 4, false, kDrop>(a, static_cast<cudaStream_t>(stream));
+    };
+    return a.seed ? go(std::true_type()) : go(std::false_type());
   });
 }
 
@@ -740,6 +1015,7 @@ int flexspmv_dropout(const flexspmv_rows_desc* d, const void* const* in, void* c
   const bool wide = wide_rows(d->type, d->width, xs, in[0]) && wide_rows(d->type, d->width, rs, in[1]) && wide_rows(d->type, d->width, d->width, out[0]);
   return by_type(d->type, [&](auto zero) {
     using T = decltype(zero);
+    if (wide && d->width % (32 / (int)sizeof(T)) == 0) return dropout_typed<T, 32 / (int)sizeof(T), true>(a, static_cast<cudaStream_t>(stream));
     return wide ? dropout_typed<T, 16 / (int)sizeof(T), true>(a, static_cast<cudaStream_t>(stream)) : dropout_typed<T, 4, false>(a, static_cast<cudaStream_t>(stream));
   });
 }
