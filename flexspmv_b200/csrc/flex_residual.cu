@@ -14,6 +14,7 @@ int device_sm_count();
 // ---- random numbers ------------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ void product(uint32_t a, uint32_t b, uint32_t& high, uint32_t& low) {
+  // not as the language's product, whose registers the compiler chooses differently: the gradients of 16384 rows of 4096 take 128 us, with that 157
   asm("{\n\t.reg .b64 p;\n\tmul.wide.u32 p, %2, %3;\n\tmov.b64 {%1, %0}, p;\n\t}" : "=r"(high), "=r"(low) : "r"(a), "r"(b));
 }
 
@@ -35,15 +36,14 @@ struct Random {
       key0[i] = (uint32_t)k + i * 0x9E3779B9u;
       key1[i] = (uint32_t)(k >> 32) + i * 0xBB67AE85u;
     }
-    uint32_t high;
-    product((uint32_t)o, 0xCD9E8D57u, high, second);
-    first = high ^ key0[0];
+    const unsigned long long b = (o & 0xffffffffull) * 0xCD9E8D57u;
+    first = (uint32_t)(b >> 32) ^ key0[0];
+    second = (uint32_t)b;
     offset1 = (uint32_t)(o >> 32) ^ key1[0];
   }
   __device__ __forceinline__ void words(uint32_t group, uint32_t row, uint32_t (&w)[4]) const {
-    uint32_t c0 = first ^ row, c1 = second, c2, c3;
-    product(group, 0xD2511F53u, c2, c3);
-    c2 ^= offset1;
+    const unsigned long long begin = (unsigned long long)group * 0xD2511F53u;
+    uint32_t c0 = first ^ row, c1 = second, c2 = (uint32_t)(begin >> 32) ^ offset1, c3 = (uint32_t)begin;
 #pragma unroll
     for (int i = 1; i < 10; ++i) {
       uint32_t a, b, low_a, low_b;
@@ -754,7 +754,7 @@ struct DropoutArgs {
 // Bound by memory (2^26 values in 16 bits and as many added: 6.26 TB/s), with the generator close behind, which is why C is 32 bytes where the width allows: what a
 // thread does for a place and not for a value is shared by twice as many (64.4 us, with 16 bytes 80.6).
 template <class T, int C, bool WIDE>
-__global__ void __launch_bounds__(256, 3) dropout_kernel(DropoutArgs a) {
+__global__ void __launch_bounds__(256, 4) dropout_kernel(DropoutArgs a) {
   pdl_wait();
   const Random random(a.seed, true);
   const int pieces = (a.width + C - 1) / C;
@@ -888,7 +888,7 @@ static int norm_grad_typed(const NormGradArgs& a, cudaStream_t st) {
 
 template <class T, int C, bool WIDE>
 static int dropout_typed(const DropoutArgs& a, cudaStream_t st) {
-  return launch_pdl(dropout_kernel<T, C, WIDE>, row_grid(a.rows * ((a.width + C - 1) / C), 256, device_sm_count() * 3ll), 256, 0, st, a);
+  return launch_pdl(dropout_kernel<T, C, WIDE>, row_grid(a.rows * ((a.width + C - 1) / C), 256, device_sm_count() * 4ll), 256, 0, st, a);
 }
 
 // Accesses of 16 bytes where every row allows them.
