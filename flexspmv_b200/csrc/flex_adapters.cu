@@ -17,17 +17,18 @@ struct AdapterTile {
 };
 
 // Where a plan's parts lie, in ints: [0] the number of tiles, [4, 5] the offsets of one group of all tokens.
+constexpr int kLowTile = 16;
+constexpr long long kLowFew = 1024;          // tokens up to which the first product is in such tiles
 struct AdapterPlan {
-  long long ids, rows, tiles, ints;
-  int most_tiles, tile;
+  long long ids, rows, tiles, offsets, ints;
+  int most_tiles;
 };
 static AdapterPlan adapter_plan_of(long long tokens, int adapters) {
   AdapterPlan p;
-  // few tokens: tiles of one instruction's rows, as many as can be for the sake of their latency; else of four, which read an adapter a quarter as often
-  p.tile = tokens <= 1024 ? 16 : 64;
-  p.most_tiles = (int)(tokens / p.tile + (tokens < adapters ? tokens : adapters));
+  p.most_tiles = tokens <= kLowFew ? (int)(tokens / kLowTile + (tokens < adapters ? tokens : adapters)) : 0;
   p.tiles = 8;
-  p.ids = p.tiles + 4ll * p.most_tiles;
+  p.offsets = p.tiles + 4ll * p.most_tiles;
+  p.ids = p.offsets + adapters + 1;
   p.rows = p.ids + tokens;
   p.ints = (p.rows + tokens + 3) / 4 * 4;
   return p;
@@ -36,8 +37,8 @@ static AdapterPlan adapter_plan_of(long long tokens, int adapters) {
 struct AdapterPlanArgs {
   const int* ids;
   int* plan;
-  long long tokens, at_ids, at_rows;
-  int adapters, tile;
+  long long tokens, at_ids, at_rows, at_offsets;
+  int adapters, most_tiles;
   int* status;
 };
 
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(AdapterPlanA
   if (warp == 0) {
     int places = 0, tiles = 0;
     for (int i0 = 0; i0 < a.adapters; i0 += 32) {
-      const int i = i0 + lane, n = i < a.adapters ? first[i] : 0, m = (n + a.tile - 1) / a.tile;
+      const int i = i0 + lane, n = i < a.adapters ? first[i] : 0, m = (n + kLowTile - 1) / kLowTile;
       int s = n, u = m;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -97,22 +98,25 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(AdapterPlanA
         first[i] = places + s - n;
         first_tile[i] = tiles + u - m;
         count[i] = n;
+        a.plan[a.at_offsets + i] = places + s - n;
       }
       places += __shfl_sync(0xffffffffu, s, 31);
       tiles += __shfl_sync(0xffffffffu, u, 31);
     }
     if (lane == 0) {
-      a.plan[0] = tiles;
+      a.plan[a.at_offsets + a.adapters] = places;
+      a.plan[0] = a.most_tiles ? tiles : 0;
       a.plan[4] = 0;
       a.plan[5] = (int)a.tokens;
     }
   }
   __syncthreads();
-  for (int i = warp; i < a.adapters; i += kWarps) {
-    AdapterTile* const out = reinterpret_cast<AdapterTile*>(a.plan + 8) + first_tile[i];
-    for (int j = lane; j * a.tile < count[i]; j += 32)
-      out[j] = {i, first[i] + j * a.tile, count[i] - j * a.tile < a.tile ? count[i] - j * a.tile : a.tile, 0};
-  }
+  if (a.most_tiles)
+    for (int i = warp; i < a.adapters; i += kWarps) {
+      AdapterTile* const out = reinterpret_cast<AdapterTile*>(a.plan + 8) + first_tile[i];
+      for (int j = lane; j * kLowTile < count[i]; j += 32)
+        out[j] = {i, first[i] + j * kLowTile, count[i] - j * kLowTile < kLowTile ? count[i] - j * kLowTile : kLowTile, 0};
+    }
   for (long long t0 = from; t0 < to; t0 += 32) {
     const long long t = t0 + lane;
     const int id = t < to ? a.plan[a.at_ids + t] : -1;
@@ -136,102 +140,79 @@ struct LowArgs {
   int rank, k, width;
 };
 
-// low[t] = scale A x[t]: a CTA takes a tile of up to 16 MB tokens of one adapter and 8 NB values of the rank (blockIdx.y), its eight warps every eighth 32 of the
-// sum, and their sums meet in shared memory in the warps' order.  Bound by reading x and the adapters, not by arithmetic, so the warps' own matrix instruction is
-// enough and its operands come from global memory as they are: as the sum's index may be permuted, a lane's share of two instructions is 16 contiguous
-// bytes of a row, and eight rows of 64 bytes are one load of the warp.
-template <class T, int MB, int NB>
-__global__ void __launch_bounds__(256) adapter_low_kernel(LowArgs a) {
-  __shared__ float joined[16 * MB][8 * NB + 1];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, g = lane >> 2, r0 = blockIdx.y * 8 * NB;
+// low[t] = scale A x[t] of few tokens: a CTA takes a tile of up to 16 tokens of one adapter and 16 values of the rank (blockIdx.y), its warps neighbouring
+// parts of the sum in turn, whose sums meet in shared memory in the warps' order.  Bound by the latency of reading the adapter, not by arithmetic, so the warp's own matrix
+// instruction is enough and its operands come from global memory as they are: as the sum's index may be permuted, a lane's share of two instructions
+// is 16 contiguous bytes of a row, and eight rows of 64 bytes are one load of the warp.  Many tokens: grouped_kernel.
+constexpr int kLowThreads = 512, kLowAhead = 4;          // loads of so many steps under way
+template <class T>
+__global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(LowArgs a) {
+  constexpr int kWarps = kLowThreads / 32, kStep = 32 * kWarps;
+  __shared__ float part[kWarps][16][17];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, g = lane >> 2, r0 = blockIdx.y * 16;
   pdl_wait();
   pdl_launch_dependents();
   if ((int)blockIdx.x >= *a.count) return;
   const AdapterTile tile = a.tiles[blockIdx.x];
-  const T* x[MB][2];
+  // rows and ranks that are not there: the first one's, whose results are left out
+  const T *x[2], *down[2];
 #pragma unroll
-  for (int m = 0; m < MB; ++m)
+  for (int i = 0; i < 2; ++i) {
+    const int p = i * 8 + g, r = r0 + i * 8 + g;
+    x[i] = static_cast<const T*>(a.x) + (long long)a.rows[tile.from + (p < tile.count ? p : 0)] * a.stride;
+    down[i] = static_cast<const T*>(a.down) + ((size_t)tile.adapter * a.rank + (r < a.rank ? r : r0)) * a.k;
+  }
+  float acc[2][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int p = m * 16 + i * 8 + g;
-      x[m][i] = p < tile.count ? static_cast<const T*>(a.x) + (long long)a.rows[tile.from + p] * a.stride : nullptr;
-    }
-  const T* const down = static_cast<const T*>(a.down) + ((size_t)tile.adapter * a.rank + r0 + g) * a.k;
-  const int blocks = (tile.count + 15) / 16;
-  float acc[MB][NB][4];
+  for (int i = 0; i < 8; ++i) acc[i / 4][i % 4] = 0.f;
+  const bool high = tile.count > 8;          // else the upper rows' loads are left out
+  for (int k0 = warp * 32; k0 < a.k; k0 += kStep * kLowAhead) {
+    uint4 v[kLowAhead][2], w[kLowAhead][2];
 #pragma unroll
-  for (int m = 0; m < MB; ++m)
-#pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
-  const uint4 none = make_uint4(0, 0, 0, 0);
-#pragma unroll MB == 1 ? 4 : 1
-  for (int k0 = warp * 32; k0 < a.k; k0 += 256) {
-    const int k = k0 + q * 8;
-    uint4 v[MB][2], w[NB];
-#pragma unroll
-    for (int m = 0; m < MB; ++m)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) v[m][i] = x[m][i] && k < a.k ? *reinterpret_cast<const uint4*>(x[m][i] + k) : none;
-#pragma unroll
-    for (int j = 0; j < NB; ++j) w[j] = r0 + j * 8 + g < a.rank && k < a.k ? *reinterpret_cast<const uint4*>(down + (size_t)j * 8 * a.k + k) : none;
-#pragma unroll
-    for (int m = 0; m < MB; ++m) {
-      if (m >= blocks) break;
-#pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        warp_mma<T>(acc[m][j], v[m][0].x, v[m][1].x, v[m][0].y, v[m][1].y, w[j].x, w[j].y);
-        warp_mma<T>(acc[m][j], v[m][0].z, v[m][1].z, v[m][0].w, v[m][1].w, w[j].z, w[j].w);
+    for (int u = 0; u < kLowAhead; ++u) {
+      const int k = k0 + u * kStep + q * 8;
+      v[u][0] = v[u][1] = w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+      if (k < a.k) {
+        v[u][0] = *reinterpret_cast<const uint4*>(x[0] + k);
+        if (high) v[u][1] = *reinterpret_cast<const uint4*>(x[1] + k);
+        w[u][0] = *reinterpret_cast<const uint4*>(down[0] + k);
+        w[u][1] = *reinterpret_cast<const uint4*>(down[1] + k);
       }
     }
+#pragma unroll
+    for (int u = 0; u < kLowAhead; ++u)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        warp_mma<T>(acc[j], v[u][0].x, v[u][1].x, v[u][0].y, v[u][1].y, w[u][j].x, w[u][j].y);
+        warp_mma<T>(acc[j], v[u][0].z, v[u][1].z, v[u][0].w, v[u][1].w, w[u][j].z, w[u][j].w);
+      }
   }
-  for (int turn = 0; turn < 8; ++turn) {
-    if (warp == turn)
 #pragma unroll
-      for (int m = 0; m < MB; ++m)
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
+    for (int i = 0; i < 4; ++i) part[warp][g + i / 2 * 8][j * 8 + q * 2 + i % 2] = acc[j][i];
+  __syncthreads();
+  if (threadIdx.x >= 256) return;
+  const int p = threadIdx.x / 16, r = r0 + threadIdx.x % 16;
+  if (p >= tile.count || r >= a.rank) return;
+  float h = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float& s = joined[m * 16 + g + i / 2 * 8][j * 8 + q * 2 + i % 2];
-            s = turn ? s + acc[m][j][i] : acc[m][j][i];
-          }
-    __syncthreads();
-  }
-  const float scale = a.scale ? a.scale[tile.adapter] : 1.f;
-  for (int i = threadIdx.x; i < tile.count * NB; i += 256) {
-    const int p = i / NB, j = i % NB * 8;
-    if (r0 + j >= a.rank) continue;
-    Pack<T, 8> high, rest;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const float h = joined[p][j + u] * scale;
-      high.set(u, h);
-      const float r = h - high.get(u);
-      rest.set(u, fabsf(high.get(u)) <= 3.4e38f ? r : 0.f);          // of what is not finite: none
-    }
-    T* const row = static_cast<T*>(a.low) + (long long)a.rows[tile.from + p] * a.width;
-    high.store(row + low_high(r0 + j, a.rank));
-    rest.store(row + low_rest(r0 + j, a.rank));
-  }
+  for (int w = 0; w < kWarps; ++w) h += part[w][p][threadIdx.x % 16];
+  if (a.scale) h *= a.scale[tile.adapter];
+  T* const row = static_cast<T*>(a.low) + (long long)a.rows[tile.from + p] * a.width;
+  row[low_high(r, a.rank)] = from_float<T>(h);
+  row[low_rest(r, a.rank)] = from_float<T>(low_rest_of<T>(h));
 }
 
 template <class T>
 static int low_product(const LowArgs& a, const AdapterPlan& p, cudaStream_t st) {
-  const auto go = [&](auto kernel, int ranks) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.most_tiles, (unsigned)((a.rank + ranks - 1) / ranks)); cfg.blockDim = dim3(256); cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = pdl_enabled() ? 1 : 0;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, a);
-  };
-  if (p.tile == 16) return go(adapter_low_kernel<T, 1, 2>, 16);
-  if (a.rank <= 16) return go(adapter_low_kernel<T, 4, 2>, 16);
-  if (a.rank <= 32) return go(adapter_low_kernel<T, 4, 4>, 32);
-  return go(adapter_low_kernel<T, 4, 8>, 64);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p.most_tiles, (unsigned)((a.rank + 15) / 16)); cfg.blockDim = dim3(kLowThreads); cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&cfg, adapter_low_kernel<T>, a);
 }
 
 // `product`: n, k and the rank count too.
@@ -267,7 +248,7 @@ int flexspmv_adapter_plan(const flexspmv_adapter_desc* d, const int32_t* ids, vo
   if (!plan || plan_bytes < (size_t)p.ints * 4) return FLEXSPMV_ERR_WORKSPACE;
   if (!aligned16(plan) || !aligned_to(4, ids, status)) return FLEXSPMV_ERR_ALIGN;
   if (!apart({{plan, p.ints * 4}}, {{ids, 4 * d->tokens}})) return FLEXSPMV_ERR_BAD_ARG;
-  const AdapterPlanArgs a = {ids, static_cast<int*>(plan), d->tokens, p.ids, p.rows, d->adapters, p.tile, status};
+  const AdapterPlanArgs a = {ids, static_cast<int*>(plan), d->tokens, p.ids, p.rows, p.offsets, d->adapters, p.most_tiles, status};
   const int smem = (kPlanThreads / 32 + 3) * d->adapters * 4;
   if (int e = allow_smem<adapter_plan_kernel>(smem)) return e;
   return launch_pdl(adapter_plan_kernel, 1, kPlanThreads, (size_t)smem, static_cast<cudaStream_t>(stream), a);
@@ -302,7 +283,10 @@ int flexspmv_adapted_project(const flexspmv_adapter_desc* d, const void* const* 
   const LowArgs a = {in[0], in[2], static_cast<const float*>(in[4]), plan + p.rows, plan, reinterpret_cast<const AdapterTile*>(plan + p.tiles), ws, d->x_stride,
                      d->rank, d->k, width};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int e = d->type == FLEXSPMV_TYPE_BF16 ? low_product<__nv_bfloat16>(a, p, st) : low_product<__half>(a, p, st)) return e;
+  int e;
+  if (d->tokens > kLowFew) e = low_product_of_many(d, in[0], in[2], a.scale, plan + p.offsets, a.rows, ws, width, status, st);
+  else e = d->type == FLEXSPMV_TYPE_BF16 ? low_product<__nv_bfloat16>(a, p, st) : low_product<__half>(a, p, st);
+  if (e) return e;
   return adapted_product(d, in[0], in[1], in[3], ws, width, plan + 4, plan + p.ids, out[0], status, st);
 }
 

@@ -15,6 +15,13 @@ __host__ __device__ constexpr int low_width(int rank) { return rank <= 32 ? 64 :
 __host__ __device__ constexpr int low_high(int k, int rank) { return rank <= 32 ? k : k / 64 * 128 + k % 64; }
 __host__ __device__ constexpr int low_rest(int k, int rank) { return low_high(k, rank) + (rank <= 32 ? 32 : 64); }
 
+// What of a value is left by its rounding to T; of what is not finite once rounded, nothing.
+template <class T>
+__device__ __forceinline__ float low_rest_of(float v) {
+  const float high = to_float(from_float<T>(v));
+  return fabsf(high) <= 3.4e38f ? v - high : 0.f;
+}
+
 // The warp's matrix instruction: d (16 x 8, 32-bit) += a (16 x 16) b (16 x 8).
 template <class T>
 __device__ __forceinline__ void warp_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -28,6 +35,9 @@ __device__ __forceinline__ void warp_mma(float (&d)[4], uint32_t a0, uint32_t a1
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// low[rows[i]] = scale[e] down[e] x[rows[i]] (flex_grouped.cu) for the places offsets[e] <= i < offsets[e + 1].
+int low_product_of_many(const flexspmv_adapter_desc* d, const void* x, const void* down, const float* scale, const int* offsets, const int* rows, void* low,
+                        int low_width, int* status, cudaStream_t st);
 // y = weight x + up low (flex_grouped.cu).  The kernel before it on the stream has been launched for it (see ADAPT there).
 int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* low, int low_width, const int* offsets,
                     const int* ids, void* out, int* status, cudaStream_t st);

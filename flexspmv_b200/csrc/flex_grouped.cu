@@ -27,7 +27,9 @@ struct GroupedArgs {
   const int* ids;
   const void *up, *low;
   int adapters, rank, low_width;
+  const float* scale;            // of the first product
 };
+enum GroupedAdapt { kPlain, kAddLow, kMakeLow };
 
 __device__ __forceinline__ void raise(int* status, int code) {
   if (status) *status = code;
@@ -70,7 +72,8 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict_
 // rows up to some thousand rows, 2 - 4 % slower for 32 768 of 2048.  (Tile copies that gather four rows each took 72 cycles an instruction: 2.2 ms
 // there instead of 0.43.)  dw's rows are other ones in every step: gathered like this they take 0.57 ms of the 32 768; a copy of them in the
 // workspace and contiguous tile copies 0.44.
-// ADAPT (forward, one expert): on a place's way out its adapter's up matrix times its vector of `rank` values is added (add_low_rank), before the only rounding.
+// ADAPT (forward): kAddLow, one expert: on a place's way out its adapter's up matrix times its vector of `rank` values is added (add_low_rank), before the only
+// rounding.  kMakeLow: those vectors, scale A x, rows by a list, in two 16-bit values each.
 // Warps 0-7 store finished accumulators, warp 8 issues the tile copies, warp 9 the matrix instructions; two accumulators in tensor memory,
 // so that one is stored while the next is computed (HALVES = 2: while the other half of the next tile begins).  The sum goes 64 values (128 bytes of a row) a stage.
 constexpr int kStoreWarps = 8, kCopyWarp = kStoreWarps, kMathWarp = kStoreWarps + 1, kGroupedThreads = (kStoreWarps + 2) * 32;
@@ -169,28 +172,34 @@ __device__ __forceinline__ void add_low_rank(const GroupedArgs& a, int m, int pl
 #pragma unroll
     for (int i = 0; i < 32; ++i) d[i / 16][i / 4 % 4][i % 4] = 0.f;
     const T* const up = static_cast<const T*>(a.up) + ((size_t)adapter * a.n + m + g) * a.rank;
+#pragma unroll 2
     for (int k = q * 8; k - q * 8 < a.rank; k += 32) {
       const bool inside = k < a.rank;
-      uint4 w[4];
+      uint4 w[4], h[4][2];                 // all under way at once
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = inside && m + g + i * 8 < a.n ? *reinterpret_cast<const uint4*>(up + (size_t)i * 8 * a.rank + k) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 4; ++i) {
+        w[i] = make_uint4(0, 0, 0, 0);
+        if (inside && m + g + i * 8 < a.n) w[i] = *reinterpret_cast<const uint4*>(up + (size_t)i * 8 * a.rank + k);
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        h[b][0] = h[b][1] = make_uint4(0, 0, 0, 0);
+        if (inside && (mine >> (b * 8 + g) & 1u)) {
+          const T* const row = static_cast<const T*>(a.low) + (size_t)(place + b * 8 + g) * a.low_width;
+          h[b][0] = *reinterpret_cast<const uint4*>(row + low_high(k, a.rank));
+          h[b][1] = *reinterpret_cast<const uint4*>(row + low_rest(k, a.rank));
+        }
+      }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         if (!(mine >> (b * 8) & 0xffu)) continue;
-        uint4 h = make_uint4(0, 0, 0, 0), rest = h;
-        if (inside && (mine >> (b * 8 + g) & 1u)) {
-          const T* const row = static_cast<const T*>(a.low) + (size_t)(place + b * 8 + g) * a.low_width;
-          h = *reinterpret_cast<const uint4*>(row + low_high(k, a.rank));
-          rest = *reinterpret_cast<const uint4*>(row + low_rest(k, a.rank));
-        }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          warp_mma<T>(d[i][b], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h.x, h.y);
-          warp_mma<T>(d[i][b], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, h.z, h.w);
-          warp_mma<T>(d[i][b], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, rest.x, rest.y);
-          warp_mma<T>(d[i][b], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, rest.z, rest.w);
-        }
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            warp_mma<T>(d[i][b], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h[b][x].x, h[b][x].y);
+            warp_mma<T>(d[i][b], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, h[b][x].z, h[b][x].w);
+          }
       }
     }
 #pragma unroll
@@ -232,7 +241,23 @@ __device__ __forceinline__ void add_low_rank(const GroupedArgs& a, int m, int pl
   for (int x = 0; x < 8; ++x) sum[x] += part[x];
 }
 
-template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER, bool PARTS, bool ADAPT>
+// SPLIT: asks for this CTA's rows of the up matrices, which its last step reads, while nothing else is to be done.
+template <class T>
+__device__ __forceinline__ void prefetch_up(const GroupedArgs& a, int share, int split, int tid) {
+  const int m0 = blockIdx.x / split * 128;
+  if (m0 >= a.n) return;
+  const int eights = (int)((a.slots + 7) / 8), from = eights * share / split * 8, to = eights * (share + 1) / split * 8;
+  const int lines = (128 * a.rank * 2 + 127) / 128;
+  for (int i = tid; i < (to - from) * lines; i += kStoreWarps * 32) {
+    const int p = from + i / lines;
+    const int id = p < a.slots ? a.ids[p] : -1;
+    const size_t at = ((size_t)id * a.n + m0) * a.rank * 2 + (size_t)(i % lines) * 128;
+    if ((unsigned)id < (unsigned)a.adapters && at < (size_t)(id + 1) * a.n * a.rank * 2)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(a.up) + at));
+  }
+}
+
+template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER, bool PARTS, int ADAPT>
 __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                      const __grid_constant__ CUtensorMap row_a, const __grid_constant__ CUtensorMap row_b,
                                                                      const __grid_constant__ CUtensorMap map_out,
@@ -266,7 +291,8 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   if (warp == kMathWarp) tmem_alloc<PAIR, Cfg::kTmemCols>(&bars.tmem);
   // ADAPT: the launch before this one is the adapters' first product, which lets this one begin once all before it is done; only the stores need
   // its result.
-  if (!ADAPT) pdl_wait();
+  if (ADAPT != kAddLow) pdl_wait();
+  if (ADAPT == kMakeLow) pdl_launch_dependents();
   for (int e = tid; e < a.experts; e += kThreads) {
     int from, to;
     group_of(a, e, from, to);
@@ -553,7 +579,10 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
     }
     copy16_wait_all();
   } else {
-    if (ADAPT) pdl_wait();
+    if (ADAPT == kAddLow) {
+      if (SPLIT) prefetch_up<T>(a, share, split, tid);
+      pdl_wait();
+    }
     int acc = 0;
     uint32_t acc_phase = 0, second_phase = 0;
     TO* const out = static_cast<TO*>(a.out);
@@ -672,31 +701,53 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
         }
         if (last) free_accumulator();
         if (!there) break;
-        if constexpr (ADAPT) add_low_rank<T>(a, m, t.from + c0, t.count - c0, lane, low, high);
+        if constexpr (ADAPT == kAddLow) add_low_rank<T>(a, m, t.from + c0, t.count - c0, lane, low, high);
         if (MODE == kGroupedDw) {
           store_rows(c0, [&](int x) { return __uint_as_float(v[x]); });
         } else {
           // blocks of 8 features by 8 places, turned on their way into rows of 32 features a place (16-byte pieces, exchanged so that neither
           // way meets in a bank)
-          if constexpr (sizeof(TO) == 2) {
+          const auto turn = [&](const auto& pair) {
+            if constexpr (sizeof(TO) == 2) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              const auto pair = [&](const uint32_t (&w)[16], int i) {
-                return two_of<TO>(__uint_as_float(w[b * 4 + i]), __uint_as_float(w[b * 4 + i + 1]));
-              };
-              const int p = b * 8 + (lane & 7);
-              store_blocks_turned(mine + p * 64 + (((lane >> 3) ^ (p >> 1)) & 3) * 16, pair(low, 0), pair(low, 2), pair(high, 0), pair(high, 2));
+              for (int b = 0; b < 4; ++b) {
+                const int p = b * 8 + (lane & 7);
+                store_blocks_turned(mine + p * 64 + (((lane >> 3) ^ (p >> 1)) & 3) * 16, pair(low, b * 4), pair(low, b * 4 + 2), pair(high, b * 4),
+                                    pair(high, b * 4 + 2));
+              }
             }
-          }
-          __syncwarp();
-          const int width = MODE == kGroupedDx ? a.k : a.n;
+            __syncwarp();
+          };
+          const auto piece = [&](int p) { return reinterpret_cast<const uint4*>(mine)[p * 4 + (((lane & 3) ^ (p >> 1)) & 3)]; };
+          if constexpr (ADAPT == kMakeLow) {
+            const float scale = a.scale ? a.scale[t.e] : 1.f;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int p = x * 8 + (lane >> 2), c = m + (lane & 3) * 8;
-            if (c0 + p < t.count && c < width)
-              *reinterpret_cast<uint4*>(out + (size_t)(t.from + c0 + p) * width + c) = reinterpret_cast<const uint4*>(mine)[p * 4 + (((lane & 3) ^ (p >> 1)) & 3)];
+            for (int rest = 0; rest < 2; ++rest) {
+              turn([&](const uint32_t (&w)[16], int i) {
+                const float u = __uint_as_float(w[i]) * scale, v = __uint_as_float(w[i + 1]) * scale;
+                return rest ? two_of<TO>(low_rest_of<TO>(u), low_rest_of<TO>(v)) : two_of<TO>(u, v);
+              });
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const int p = x * 8 + (lane >> 2), c = m + (lane & 3) * 8;
+                if (c0 + p < t.count && c < a.n) {
+                  const int row = a.rows[t.from + c0 + p];
+                  if ((unsigned)row < (unsigned)a.tokens)
+                    *reinterpret_cast<uint4*>(out + (size_t)row * a.low_width + (rest ? low_rest(c, a.n) : low_high(c, a.n))) = piece(p);
+                }
+              }
+              __syncwarp();
+            }
+          } else {
+            turn([&](const uint32_t (&w)[16], int i) { return two_of<TO>(__uint_as_float(w[i]), __uint_as_float(w[i + 1])); });
+            const int width = MODE == kGroupedDx ? a.k : a.n;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int p = x * 8 + (lane >> 2), c = m + (lane & 3) * 8;
+              if (c0 + p < t.count && c < width) *reinterpret_cast<uint4*>(out + (size_t)(t.from + c0 + p) * width + c) = piece(p);
+            }
+            __syncwarp();
           }
-          __syncwarp();
         }
         if (last) break;
       }
@@ -709,7 +760,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
       }
     }
     if (MODE == kGroupedDw && lane == 0) tma_stores_done();
-    if (MODE != kGroupedDw) {     // places of no expert: before the first group and after the last
+    if (MODE != kGroupedDw && ADAPT == kPlain) {     // places of no expert: before the first group and after the last
       const int width = (MODE == kGroupedDx ? a.k : a.n) / 8;
       const long long head = table[0].from, tail = table[a.experts - 1].from + table[a.experts - 1].count, none = head + a.slots - tail;
       for (long long x = blockIdx.x; x < none; x += gridDim.x) {
@@ -721,7 +772,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   if (SPLIT) {
     // every CTA stores some of the tile's columns, eight neighbouring rows (dw: columns) at a time
     cluster_sync();
-    if (ADAPT) pdl_wait();
+    if (ADAPT == kAddLow) pdl_wait();
     if (first < tiles && !*abort) {
       const GroupedTile t = tile_at<MODE, NT, PAIR, HALVES>(a, table, first);
       const int eights = (t.cols + 7) / 8, c_from = eights * share / split * 8, c_to = eights * (share + 1) / split * 8;
@@ -748,7 +799,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
 #pragma unroll
           for (int x = 0; x < 8; ++x) sum[x] += v[x];
         }
-        if constexpr (ADAPT)
+        if constexpr (ADAPT == kAddLow)
           if (c < t.count && t.m0 + r < a.n) add_low_rank<T>(a, t.m0 + r, t.from + c, sum);
         Pack<TO, 8> q;
 #pragma unroll
@@ -798,7 +849,7 @@ static int grouped_smem(int experts) {
 }
 
 // `split`: CTAs that share a tile, `grid` of them altogether; 1: whole tiles.
-template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER, bool PARTS, bool ADAPT>
+template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER, bool PARTS, int ADAPT>
 static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStream_t st) {
   constexpr CUtensorMapDataType kIn = std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap ma, mb, row_a, row_b, out;
@@ -845,7 +896,7 @@ static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStre
   return (int)cudaLaunchKernelEx(&cfg, kernel, ma, mb, row_a, row_b, out, a);
 }
 
-template <class T, class TO, int MODE, int NT, int PAIR, bool GATHER, bool PARTS, bool ADAPT>
+template <class T, class TO, int MODE, int NT, int PAIR, bool GATHER, bool PARTS, int ADAPT>
 static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
   const int sms = device_sm_count();
   // tiles of 128 rows, no more than these whatever the groups are
@@ -856,18 +907,21 @@ static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
   // What dividing saves is most of a tile's steps, 0.3 us each (a narrow tile's 0.13); what it costs is the parts' meeting, about 5 us (1.5).
   // us, whole / divided: 8 rows, one expert of 2048 x 4096 17.4 / 9.4; dw of 8192 rows, 1024 x 1024 43.8 / 22; but 4096 rows, two experts of
   // 512 x 512 (8 steps) 9.8 / 12.6.
-  constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, 1, true, GATHER, PARTS, ADAPT>;
-  const int smem = grouped_smem<MODE, NT, 1, 1, (int)sizeof(TO)>(a.experts);
-  for (int split = 8; split > 1; split /= 2) {
-    if (most * split > sms || steps - steps / split < (NT > 64 ? 20 : 12)) continue;
-    if (int e = allow_smem<divided>(smem)) return e;
-    if (most <= clusters_at_once<divided, grouped_threads(GATHER)>(split, smem)) return grouped_launch_as<T, TO, MODE, NT, 1, 1, true, GATHER, PARTS, ADAPT>(a, (int)most * split, split, st);
+  if constexpr (ADAPT != kMakeLow) {
+    constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, 1, true, GATHER, PARTS, ADAPT>;
+    const int smem = grouped_smem<MODE, NT, 1, 1, (int)sizeof(TO)>(a.experts);
+    for (int split = 8; split > 1; split /= 2) {
+      if (most * split > sms || steps - steps / split < (NT > 64 ? 20 : 12)) continue;
+      if (int e = allow_smem<divided>(smem)) return e;
+      if (most <= clusters_at_once<divided, grouped_threads(GATHER)>(split, smem)) return grouped_launch_as<T, TO, MODE, NT, 1, 1, true, GATHER, PARTS, ADAPT>(a, (int)most * split, split, st);
+    }
   }
   // Tiles of both accumulators (HALVES = 2): a quarter less between L2 and the SMs for a tile's step, a stage less under way, and the end of a tile's
   // sum that only half of it is behind.  It pays where the sums are long and the tiles go round the pairs, most with gathered rows, which are gathered
   // half as often.  us, one / both: 32 768 rows, 32 experts of 4096 x 2048, with a list 437 / 419, without 411 / 413, dw 418 / 410, dx 411 / 419;
   // 10 599 rows, 8 experts of 1488 x 2792 87.6 / 75.7; 8192 x 8192 x 8192 737 / 688; but 8192 rows of 328 85 / 89, 4102 rows of 2048 28 / 30.
-  if constexpr (NT > 64 && !PARTS && MODE != kGroupedDx) {
+  // An accumulator's way out is longer with adapters, and with one accumulator for each half of a tile less of it is hidden.
+  if constexpr (NT > 64 && !PARTS && MODE != kGroupedDx && ADAPT == kPlain) {
     const long long columns = MODE == kGroupedDw ? (long long)a.experts * ((a.k + NT - 1) / NT) : a.slots / NT + a.experts / 2;          // of tiles, about
     const int long_sum = MODE == kGroupedDw ? 16 : GATHER ? 32 : 40, half_rounds = MODE == kGroupedDw ? 20 : 3;
     if (steps >= long_sum && columns * ((a.n + 511) / 512) * 2 >= half_rounds * (sms / 2))
@@ -876,13 +930,13 @@ static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
   return grouped_launch_as<T, TO, MODE, NT, PAIR, 1, false, GATHER, PARTS, ADAPT>(a, sms / PAIR * PAIR, 1, st);
 }
 
-template <class T, class TO, int MODE, bool GATHER, bool ADAPT = false>
+template <class T, class TO, int MODE, bool GATHER, int ADAPT = kPlain>
 static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
   if constexpr (MODE == kGroupedDw) {
     // us, whole / in parts: 200 000 rows of 2048 x 2048 in float16 1160 / 1195, 600 000 of 512 x 512 512 / 540, 102 400 in 32 such groups 591 / 597
     if constexpr (sizeof(TO) == 2)
-      if (a.slots <= kWholeRows<T>) return grouped_tiles<T, TO, MODE, 256, 2, GATHER, false, false>(a, st);
-    return grouped_tiles<T, TO, MODE, 256, 2, GATHER, true, false>(a, st);
+      if (a.slots <= kWholeRows<T>) return grouped_tiles<T, TO, MODE, 256, 2, GATHER, false, kPlain>(a, st);
+    return grouped_tiles<T, TO, MODE, 256, 2, GATHER, true, kPlain>(a, st);
   } else {
     // Tiles of 64 places and single CTAs for up to 32 places an expert on average: more of the weights on their way at once.  us, 64 / 256 places:
     // 16 an expert, 64 experts of 1408 x 2048 59.8 / 66.8; 32 experts of 2048 x 2048, 32 an expert 47.0 / 49.7, 48 51.0 / 50.5, 128 72.1 / 54.9.
@@ -890,8 +944,9 @@ static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
     // us, narrow / wide: 753 rows, 4 experts of 104 x 1512 8.9 / 15.1; 256 rows of 2048 x 2048 10.5 / 14.3, of a list 11.0 / 16.0; 512 rows of 1024 x 1024
     // 7.3 / 8.1; but 100 rows of 4096 x 4096 13.0 / 12.3.
     const long long narrow = ((MODE == kGroupedDx ? a.k : a.n) + 127) / 128 * ((a.slots < a.experts ? a.slots : a.experts) + a.slots / 64);
-    if (a.slots <= 32ll * a.experts || narrow <= device_sm_count()) return grouped_tiles<T, TO, MODE, 64, 1, GATHER, false, ADAPT>(a, st);
-    return grouped_tiles<T, TO, MODE, 256, 2, GATHER, false, ADAPT>(a, st);
+    // kMakeLow: the rank is at most a few tiles' rows, so that narrow ones are what there is to run at once.
+    if (ADAPT == kMakeLow || a.slots <= 32ll * a.experts || narrow <= device_sm_count()) return grouped_tiles<T, TO, MODE, 64, 1, GATHER, false, ADAPT>(a, st);
+    if constexpr (ADAPT != kMakeLow) return grouped_tiles<T, TO, MODE, 256, 2, GATHER, false, ADAPT>(a, st);
   }
 }
 
@@ -969,8 +1024,17 @@ int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* w
   a.adapters = d->adapters;
   a.rank = d->rank;
   a.low_width = low_width;
-  if (d->type == FLEXSPMV_TYPE_BF16) return grouped_launch<__nv_bfloat16, __nv_bfloat16, kGroupedForward, false, true>(a, st);
-  return grouped_launch<__half, __half, kGroupedForward, false, true>(a, st);
+  if (d->type == FLEXSPMV_TYPE_BF16) return grouped_launch<__nv_bfloat16, __nv_bfloat16, kGroupedForward, false, kAddLow>(a, st);
+  return grouped_launch<__half, __half, kGroupedForward, false, kAddLow>(a, st);
+}
+
+int low_product_of_many(const flexspmv_adapter_desc* d, const void* x, const void* down, const float* scale, const int* offsets, const int* rows, void* low,
+                        int low_width, int* status, cudaStream_t st) {
+  GroupedArgs a = {x, down, offsets, rows, low, d->tokens, d->tokens, d->x_stride, 0, d->adapters, d->rank, d->k, status};
+  a.low_width = low_width;
+  a.scale = scale;
+  if (d->type == FLEXSPMV_TYPE_BF16) return grouped_launch<__nv_bfloat16, __nv_bfloat16, kGroupedForward, true, kMakeLow>(a, st);
+  return grouped_launch<__half, __half, kGroupedForward, true, kMakeLow>(a, st);
 }
 
 }  // namespace flex
