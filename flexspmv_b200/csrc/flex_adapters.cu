@@ -16,31 +16,62 @@ struct AdapterTile {
   int adapter, from, count, unused;          // places from .. from + count of `rows`, all of one adapter
 };
 
-// Where a plan's parts lie, in ints: [0] the number of tiles, [4, 5] the offsets of one group of all tokens.
+// Where a plan's parts lie, in ints; [0] is the number of tiles.  Groups: for the shared product of many tokens, runs of one adapter that are long enough for tiles of
+// their own, and what lies between them.
 constexpr int kLowTile = 16;
-constexpr long long kLowFew = 1024;          // tokens up to which the first product is in such tiles
+constexpr long long kOneGroup = 1024;        // tokens up to which they are one group
+constexpr long long kLowTiles = 4096;        // tokens up to which the first product may be in tiles
+// ... and is: as many as its CTAs read x again for every 16 of the rank.
+static bool low_in_tiles(long long tokens, int rank) { return tokens * ((rank + 15) / 16) <= kLowTiles; }
+constexpr int kLongRun = 128;
 struct AdapterPlan {
-  long long ids, rows, tiles, offsets, ints;
-  int most_tiles;
+  long long ids, rows, tiles, offsets, groups, group_adapters, runs, ints;
+  int most_tiles, most_groups, long_run;
 };
 static AdapterPlan adapter_plan_of(long long tokens, int adapters) {
   AdapterPlan p;
-  p.most_tiles = tokens <= kLowFew ? (int)(tokens / kLowTile + (tokens < adapters ? tokens : adapters)) : 0;
+  p.most_tiles = tokens <= kLowTiles ? (int)(tokens / kLowTile + (tokens < adapters ? tokens : adapters)) : 0;
   p.tiles = 8;
   p.offsets = p.tiles + 4ll * p.most_tiles;
   p.ids = p.offsets + adapters + 1;
   p.rows = p.ids + tokens;
-  p.ints = (p.rows + tokens + 3) / 4 * 4;
+  // at most some 1000 groups, which the product keeps in shared memory
+  p.long_run = (int)(tokens / 500 > kLongRun ? tokens / 500 : kLongRun);
+  p.most_groups = tokens <= kOneGroup ? 1 : (int)(2 * (tokens / p.long_run) + 1);
+  p.groups = p.rows + tokens;
+  p.group_adapters = p.groups + p.most_groups + 1;
+  p.runs = p.group_adapters + p.most_groups;
+  p.ints = p.runs + (tokens <= kOneGroup ? 0 : tokens);
+  p.ints = (p.ints + 3) / 4 * 4;
   return p;
 }
 
 struct AdapterPlanArgs {
   const int* ids;
   int* plan;
-  long long tokens, at_ids, at_rows, at_offsets;
-  int adapters, most_tiles;
+  AdapterPlan at;
+  long long tokens;
+  int adapters;
   int* status;
 };
+
+// Sums of `n` over the CTA's threads before each; `all` becomes the whole sum.
+template <int THREADS>
+__device__ __forceinline__ int sums_before_thread(int n, int* warp_sums, int& all) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int s = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += up;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = s;
+  __syncthreads();
+  const int mine = lane < THREADS / 32 ? warp_sums[lane] : 0;
+  all = __reduce_add_sync(0xffffffffu, mine);
+  return s - n + __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
+}
 
 // One CTA: a stable counting sort of the tokens by adapter, and each adapter's tiles.  A warp takes a run of the tokens, 32 at a time, and counts them in a row of
 // its own (shared, [warps][adapters]); lanes of one adapter agree by a match, so that there is no atomic.
@@ -65,7 +96,7 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(AdapterPlanA
       if (a.status) *a.status = FLEXSPMV_ERR_BAD_CSR;
       id = -1;
     }
-    if (t < to) a.plan[a.at_ids + t] = id;
+    if (t < to) a.plan[a.at.ids + t] = id;
     const unsigned same = __match_any_sync(0xffffffffu, id);
     if (id >= 0 && lane == __ffs(same) - 1) mine[id] += __popc(same);
     __syncwarp();
@@ -98,20 +129,18 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(AdapterPlanA
         first[i] = places + s - n;
         first_tile[i] = tiles + u - m;
         count[i] = n;
-        a.plan[a.at_offsets + i] = places + s - n;
+        a.plan[a.at.offsets + i] = places + s - n;
       }
       places += __shfl_sync(0xffffffffu, s, 31);
       tiles += __shfl_sync(0xffffffffu, u, 31);
     }
     if (lane == 0) {
-      a.plan[a.at_offsets + a.adapters] = places;
-      a.plan[0] = a.most_tiles ? tiles : 0;
-      a.plan[4] = 0;
-      a.plan[5] = (int)a.tokens;
+      a.plan[a.at.offsets + a.adapters] = places;
+      a.plan[0] = a.at.most_tiles ? tiles : 0;
     }
   }
   __syncthreads();
-  if (a.most_tiles)
+  if (a.at.most_tiles)
     for (int i = warp; i < a.adapters; i += kWarps) {
       AdapterTile* const out = reinterpret_cast<AdapterTile*>(a.plan + 8) + first_tile[i];
       for (int j = lane; j * kLowTile < count[i]; j += 32)
@@ -119,12 +148,55 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(AdapterPlanA
     }
   for (long long t0 = from; t0 < to; t0 += 32) {
     const long long t = t0 + lane;
-    const int id = t < to ? a.plan[a.at_ids + t] : -1;
+    const int id = t < to ? a.plan[a.at.ids + t] : -1;
     const unsigned same = __match_any_sync(0xffffffffu, id);
-    if (id >= 0) a.plan[a.at_rows + first[id] + mine[id] + __popc(same & ((1u << lane) - 1))] = (int)t;
+    if (id >= 0) a.plan[a.at.rows + first[id] + mine[id] + __popc(same & ((1u << lane) - 1))] = (int)t;
     __syncwarp();
     if (id >= 0 && lane == __ffs(same) - 1) mine[id] += __popc(same);
     __syncwarp();
+  }
+  // the groups
+  int* const groups = a.plan + a.at.groups;
+  int* const group_adapters = a.plan + a.at.group_adapters;
+  const int tokens = (int)a.tokens;
+  int found = 0;
+  if (a.at.most_groups == 1) {
+    if (tid == 0) {
+      groups[0] = 0;
+      group_adapters[0] = kGroupMixed;
+    }
+    found = 1;
+  } else {
+    __shared__ int warp_sums[kWarps];
+    const int* const ids = a.plan + a.at.ids;
+    int* const runs = a.plan + a.at.runs;
+    int starts = 0;
+    for (int t0 = 0; t0 < tokens; t0 += kPlanThreads) {
+      const int t = t0 + tid;
+      const bool begins = t < tokens && (t == 0 || ids[t] != ids[t - 1]);
+      int all;
+      const int before = sums_before_thread<kPlanThreads>(begins, warp_sums, all);
+      if (begins) runs[starts + before] = t;
+      starts += all;
+    }
+    __syncthreads();
+    const auto is_long = [&](int r) { return (r + 1 < starts ? runs[r + 1] : tokens) - runs[r] >= a.at.long_run; };
+    for (int r0 = 0; r0 < starts; r0 += kPlanThreads) {
+      const int r = r0 + tid;
+      const bool own = r < starts && is_long(r), begins = r < starts && (r == 0 || own || is_long(r - 1));
+      int all;
+      const int before = sums_before_thread<kPlanThreads>(begins, warp_sums, all);
+      if (begins && found + before < a.at.most_groups) {
+        groups[found + before] = runs[r];
+        const int id = ids[runs[r]];
+        group_adapters[found + before] = !own ? kGroupMixed : id >= 0 ? id : kGroupBare;
+      }
+      found += all;
+    }
+  }
+  for (int i = found + tid; i <= a.at.most_groups; i += kPlanThreads) {
+    groups[i] = tokens;
+    if (i < a.at.most_groups) group_adapters[i] = kGroupBare;
   }
 }
 
@@ -194,11 +266,13 @@ __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(LowArgs a) {
   __syncthreads();
   if (threadIdx.x >= 256) return;
   const int p = threadIdx.x / 16, r = r0 + threadIdx.x % 16;
-  if (p >= tile.count || r >= a.rank) return;
-  float h = 0.f;
+  if (p >= tile.count) return;
+  float h = 0.f;                           // 16 at a time, with zeros: the second product takes as many
+  if (r < a.rank) {
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) h += part[w][p][threadIdx.x % 16];
-  if (a.scale) h *= a.scale[tile.adapter];
+    for (int w = 0; w < kWarps; ++w) h += part[w][p][threadIdx.x % 16];
+    if (a.scale) h *= a.scale[tile.adapter];
+  }
   T* const row = static_cast<T*>(a.low) + (long long)a.rows[tile.from + p] * a.width;
   row[low_high(r, a.rank)] = from_float<T>(h);
   row[low_rest(r, a.rank)] = from_float<T>(low_rest_of<T>(h));
@@ -248,7 +322,7 @@ int flexspmv_adapter_plan(const flexspmv_adapter_desc* d, const int32_t* ids, vo
   if (!plan || plan_bytes < (size_t)p.ints * 4) return FLEXSPMV_ERR_WORKSPACE;
   if (!aligned16(plan) || !aligned_to(4, ids, status)) return FLEXSPMV_ERR_ALIGN;
   if (!apart({{plan, p.ints * 4}}, {{ids, 4 * d->tokens}})) return FLEXSPMV_ERR_BAD_ARG;
-  const AdapterPlanArgs a = {ids, static_cast<int*>(plan), d->tokens, p.ids, p.rows, p.offsets, d->adapters, p.most_tiles, status};
+  const AdapterPlanArgs a = {ids, static_cast<int*>(plan), p, d->tokens, d->adapters, status};
   const int smem = (kPlanThreads / 32 + 3) * d->adapters * 4;
   if (int e = allow_smem<adapter_plan_kernel>(smem)) return e;
   return launch_pdl(adapter_plan_kernel, 1, kPlanThreads, (size_t)smem, static_cast<cudaStream_t>(stream), a);
@@ -284,10 +358,10 @@ int flexspmv_adapted_project(const flexspmv_adapter_desc* d, const void* const* 
                      d->rank, d->k, width};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int e;
-  if (d->tokens > kLowFew) e = low_product_of_many(d, in[0], in[2], a.scale, plan + p.offsets, a.rows, ws, width, status, st);
+  if (!low_in_tiles(d->tokens, d->rank)) e = low_product_of_many(d, in[0], in[2], a.scale, plan + p.offsets, a.rows, ws, width, status, st);
   else e = d->type == FLEXSPMV_TYPE_BF16 ? low_product<__nv_bfloat16>(a, p, st) : low_product<__half>(a, p, st);
   if (e) return e;
-  return adapted_product(d, in[0], in[1], in[3], ws, width, plan + 4, plan + p.ids, out[0], status, st);
+  return adapted_product(d, in[0], in[1], in[3], ws, width, p.most_groups, plan + p.groups, plan + p.group_adapters, plan + p.ids, out[0], status, st);
 }
 
 }  // extern "C"

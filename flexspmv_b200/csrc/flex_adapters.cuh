@@ -38,8 +38,10 @@ __device__ __forceinline__ void warp_mma(float (&d)[4], uint32_t a0, uint32_t a1
 // low[rows[i]] = scale[e] down[e] x[rows[i]] (flex_grouped.cu) for the places offsets[e] <= i < offsets[e + 1].
 int low_product_of_many(const flexspmv_adapter_desc* d, const void* x, const void* down, const float* scale, const int* offsets, const int* rows, void* low,
                         int low_width, int* status, cudaStream_t st);
-// y = weight x + up low (flex_grouped.cu).  The kernel before it on the stream has been launched for it (see ADAPT there).
-int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* low, int low_width, const int* offsets,
-                    const int* ids, void* out, int* status, cudaStream_t st);
+// y = weight x + up low (flex_grouped.cu).  The kernel before it on the stream has been launched for it (see ADAPT there).  groups: offsets of groups of
+// tokens, group_adapters: the adapter that all tokens of a group have, or one of these.
+enum { kGroupMixed = -1, kGroupBare = -2 };
+int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* low, int low_width, int num_groups,
+                    const int* groups, const int* group_adapters, const int* ids, void* out, int* status, cudaStream_t st);
 
 }  // namespace flex

@@ -27,6 +27,7 @@ struct GroupedArgs {
   const int* ids;
   const void *up, *low;
   int adapters, rank, low_width;
+  const int* group_adapters;     // the adapter that all of a group's places have, or kGroupMixed, kGroupBare
   const float* scale;            // of the first product
 };
 enum GroupedAdapt { kPlain, kAddLow, kMakeLow };
@@ -72,8 +73,10 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict_
 // rows up to some thousand rows, 2 - 4 % slower for 32 768 of 2048.  (Tile copies that gather four rows each took 72 cycles an instruction: 2.2 ms
 // there instead of 0.43.)  dw's rows are other ones in every step: gathered like this they take 0.57 ms of the 32 768; a copy of them in the
 // workspace and contiguous tile copies 0.44.
-// ADAPT (forward): kAddLow, one expert: on a place's way out its adapter's up matrix times its vector of `rank` values is added (add_low_rank), before the only
-// rounding.  kMakeLow: those vectors, scale A x, rows by a list, in two 16-bit values each.
+// ADAPT (forward): kAddLow: one matrix for all groups, and each place's adapter's up matrix times its vector of `rank` values.  Groups of one adapter have it as one to
+// a few steps more of their sum; in mixed groups it is added on a place's way out, before the only rounding (add_low_rank), by the warps' own matrix instructions, which
+// keep the tensor cores from the sums for some eight times as long (us, 8192 tokens of rank 64 in 12 runs, all that way 313 altogether, as groups 200).
+// kMakeLow: those vectors, scale A x, rows by a list, in two 16-bit values each.
 // Warps 0-7 store finished accumulators, warp 8 issues the tile copies, warp 9 the matrix instructions; two accumulators in tensor memory,
 // so that one is stored while the next is computed (HALVES = 2: while the other half of the next tile begins).  The sum goes 64 values (128 bytes of a row) a stage.
 constexpr int kStoreWarps = 8, kCopyWarp = kStoreWarps, kMathWarp = kStoreWarps + 1, kGroupedThreads = (kStoreWarps + 2) * 32;
@@ -298,6 +301,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
     group_of(a, e, from, to);
     table[e].from = from;
     table[e].count = to - from;
+    if (ADAPT == kAddLow) reinterpret_cast<int*>(table + a.experts + 1)[e] = a.group_adapters[e];
   }
   __syncthreads();
   const int m_rows = MODE == kGroupedDx ? a.k : a.n;
@@ -326,6 +330,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   const int first = blockIdx.x / (PAIR * split);
   const int stride = gridDim.x / PAIR;
   volatile int* const abort = &bars.abort;
+  int* const group_adapters = reinterpret_cast<int*>(table + a.experts + 1);          // kAddLow
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
     if (*abort) return false;
@@ -337,8 +342,10 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   // for a whole warp: all of its lanes go on, or none
   auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
   auto stopped = [&] { return __any_sync(0xffffffffu, *abort) != 0; };
+  auto sum_steps = [&](const GroupedTile& t) { return ((MODE == kGroupedForward ? a.k : MODE == kGroupedDx ? a.n : t.count) + 63) / 64; };
+  // kAddLow: steps of 64 high and then as many rests of the vectors, or 32 of both
   auto steps_of = [&](const GroupedTile& t) {
-    return ((MODE == kGroupedForward ? a.k : MODE == kGroupedDx ? a.n : t.count) + 63) / 64;
+    return sum_steps(t) + (ADAPT == kAddLow && group_adapters[t.e] >= 0 ? (a.rank <= 32 ? 1 : (a.rank + 63) / 64 * 2) : 0);
   };
   // This cluster's tile of round u.  Where the last round has tiles for half or a quarter of the clusters at most, each is divided in two or four: HALVES = 2
   // in two by rows, else by places.  us, whole / divided: 4102 rows of 16 experts of 1024 x 2048 26.8 / 25.1, dx 22.8 / 22.3, with a list of rows
@@ -375,6 +382,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   if (warp == kCopyWarp) {
     int stage = 0, issued = 0;
     uint32_t phase = 0;
+    bool waited = false;                   // kAddLow: for the launch before
     if (elect_one()) {
       GroupedTile t;
       for (int u = 0; !*abort && tile_of(u, t); ++u) {
@@ -409,13 +417,20 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
                 for (int g = 0; g < pieces; ++g) tma_2d<PAIR>(sb + g * 8192 + r * 128, &row_b, n0 + g * 64, y, bar);
               }
             }
+          } else if (ADAPT == kAddLow && s >= sum_steps(t)) {
+            const int low_step = s - sum_steps(t);
+            if (!waited) pdl_wait();
+            waited = true;
+            if (rank == 0) mbar_expect_tx(&bars.full[stage], PAIR * (kTileBytesA + pieces * 4096));
+            tma_3d<PAIR>(sa, &row_a, low_step / 2 * 64, m0, group_adapters[t.e], bar);
+            for (int g = 0; g < pieces; ++g) tma_2d<PAIR>(sb + g * 4096, &row_b, low_step * 64, t.from + rank * half + g * 32, bar);
           } else {
             if (rank == 0) mbar_expect_tx(&bars.full[stage], PAIR * (halves * kTileBytesA + pieces * 4096));
             for (int h = t.half; h < t.halves_end; ++h) {
               unsigned char* const half_a = sa + h * kTileBytesA;
               const int row = m0 + h * 128 * PAIR;
               if (MODE == kGroupedForward) {
-                tma_3d<PAIR>(half_a, &map_a, s * 64, row, t.e, bar);
+                tma_3d<PAIR>(half_a, &map_a, s * 64, row, ADAPT == kAddLow ? 0 : t.e, bar);
               } else {
                 tma_3d<PAIR>(half_a, &map_a, row, s * 64, t.e, bar);
                 tma_3d<PAIR>(half_a + 8192, &map_a, row + 64, s * 64, t.e, bar);
@@ -459,6 +474,14 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           const uint32_t sa = smem_u32(base + stage * Cfg::kStageBytes) + h * kTileBytesA, sb = smem_u32(base + stage * Cfg::kStageBytes) + Cfg::kBytesA;
           const uint64_t da = kA_mn ? umma_desc(sa, 8192, 1024) : umma_desc(sa, 16, 1024);
           const uint64_t db = kB_mn ? umma_desc(sb, 8192, 1024) : umma_desc(sb, 16, 1024);
+          if (ADAPT == kAddLow && s >= sum_steps(t)) {
+            const int low_step = s - sum_steps(t), left = a.rank - low_step / 2 * 64, slices = left < 64 ? (left + 15) / 16 : 4;
+            for (int x = 0; x < slices; ++x) {
+              umma<PAIR>(tmem + acc * NT, da + x * 2, db + x * 2, instr, true);
+              if (a.rank <= 32) umma<PAIR>(tmem + acc * NT, da + x * 2, db + (x + 2) * 2, instr, true);
+            }
+            return;
+          }
           const int inner = MODE == kGroupedDw && t.count - s * 64 < 64 ? (t.count - s * 64 + 15) / 16 : 4;
           for (int x = 0; x < inner; ++x)  // the descriptors' addresses are in 16 bytes
             umma<PAIR>(tmem + acc * NT, da + x * (kA_mn ? 128 : 2), db + x * (kB_mn ? 128 : 2), instr, !begins || x > 0);
@@ -701,7 +724,8 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
         }
         if (last) free_accumulator();
         if (!there) break;
-        if constexpr (ADAPT == kAddLow) add_low_rank<T>(a, m, t.from + c0, t.count - c0, lane, low, high);
+        if constexpr (ADAPT == kAddLow)
+          if (group_adapters[t.e] == kGroupMixed) add_low_rank<T>(a, m, t.from + c0, t.count - c0, lane, low, high);
         if (MODE == kGroupedDw) {
           store_rows(c0, [&](int x) { return __uint_as_float(v[x]); });
         } else {
@@ -730,7 +754,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
 #pragma unroll
               for (int x = 0; x < 4; ++x) {
                 const int p = x * 8 + (lane >> 2), c = m + (lane & 3) * 8;
-                if (c0 + p < t.count && c < a.n) {
+                if (c0 + p < t.count && c < ((a.n + 15) & ~15)) {          // 16 at a time, with zeros (kAddLow takes as many)
                   const int row = a.rows[t.from + c0 + p];
                   if ((unsigned)row < (unsigned)a.tokens)
                     *reinterpret_cast<uint4*>(out + (size_t)row * a.low_width + (rest ? low_rest(c, a.n) : low_high(c, a.n))) = piece(p);
@@ -800,7 +824,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           for (int x = 0; x < 8; ++x) sum[x] += v[x];
         }
         if constexpr (ADAPT == kAddLow)
-          if (c < t.count && t.m0 + r < a.n) add_low_rank<T>(a, t.m0 + r, t.from + c, sum);
+          if (group_adapters[t.e] == kGroupMixed && c < t.count && t.m0 + r < a.n) add_low_rank<T>(a, t.m0 + r, t.from + c, sum);
         Pack<TO, 8> q;
 #pragma unroll
         for (int x = 0; x < 8; ++x) q.set(x, sum[x]);
@@ -842,10 +866,11 @@ static int clusters_at_once(int ctas, int smem) {
   return n - 1;
 }
 
-template <int MODE, int NT, int PAIR, int HALVES, int OUT_BYTES>
+template <int MODE, int NT, int PAIR, int HALVES, int OUT_BYTES, int ADAPT>
 static int grouped_smem(int experts) {
   using Cfg = GroupedCfg<MODE, NT, PAIR, HALVES, OUT_BYTES>;
-  return 1024 + Cfg::kStages * Cfg::kStageBytes + Cfg::kStoreBytes + (int)sizeof(GroupedBars) + (experts + 1) * (int)sizeof(GroupedTable);
+  return 1024 + Cfg::kStages * Cfg::kStageBytes + Cfg::kStoreBytes + (int)sizeof(GroupedBars) + (experts + 1) * (int)sizeof(GroupedTable) +
+         (ADAPT == kAddLow ? experts * 4 : 0);
 }
 
 // `split`: CTAs that share a tile, `grid` of them altogether; 1: whole tiles.
@@ -871,7 +896,7 @@ static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStre
                          kWide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
       return e;
   } else {
-    const uint64_t dw[3] = {(uint64_t)a.k, (uint64_t)a.n, (uint64_t)a.experts}, sw[2] = {(uint64_t)a.k, (uint64_t)a.k * a.n};
+    const uint64_t dw[3] = {(uint64_t)a.k, (uint64_t)a.n, ADAPT == kAddLow ? 1 : (uint64_t)a.experts}, sw[2] = {(uint64_t)a.k, (uint64_t)a.k * a.n};
     const uint32_t wide[3] = {64, 128, 1}, high[3] = {64, 64, 1};
     if (int e = make_map(&ma, a.b, kIn, 3, dw, sw, MODE == kGroupedForward ? wide : high)) return e;
     const uint64_t dx[2] = {(uint64_t)(MODE == kGroupedForward ? a.k : a.n), (uint64_t)a.slots}, sx[1] = {(uint64_t)a.a_stride};
@@ -881,8 +906,14 @@ static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStre
       if (int e = make_map(&mb, a.a, kIn, 2, dx, sx, box)) return e;
     row_a = out = ma;
     row_b = mb;
+    if (ADAPT == kAddLow) {
+      const uint64_t du[3] = {(uint64_t)a.rank, (uint64_t)a.n, (uint64_t)a.adapters}, su[2] = {(uint64_t)a.rank, (uint64_t)a.rank * a.n};
+      if (int e = make_map(&row_a, a.up, kIn, 3, du, su, wide)) return e;
+      const uint64_t dl[2] = {(uint64_t)a.low_width, (uint64_t)a.slots}, sl[1] = {(uint64_t)a.low_width};
+      if (int e = make_map(&row_b, a.low, kIn, 2, dl, sl, box)) return e;
+    }
   }
-  const int smem = grouped_smem<MODE, NT, PAIR, HALVES, (int)sizeof(TO)>(a.experts);
+  const int smem = grouped_smem<MODE, NT, PAIR, HALVES, (int)sizeof(TO), ADAPT>(a.experts);
   constexpr auto kernel = grouped_kernel<T, TO, MODE, NT, PAIR, HALVES, SPLIT, GATHER, PARTS, ADAPT>;
   if (int e = allow_smem<kernel>(smem)) return e;
   cudaLaunchConfig_t cfg = {};
@@ -909,7 +940,7 @@ static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
   // 512 x 512 (8 steps) 9.8 / 12.6.
   if constexpr (ADAPT != kMakeLow) {
     constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, 1, true, GATHER, PARTS, ADAPT>;
-    const int smem = grouped_smem<MODE, NT, 1, 1, (int)sizeof(TO)>(a.experts);
+    const int smem = grouped_smem<MODE, NT, 1, 1, (int)sizeof(TO), ADAPT>(a.experts);
     for (int split = 8; split > 1; split /= 2) {
       if (most * split > sms || steps - steps / split < (NT > 64 ? 20 : 12)) continue;
       if (int e = allow_smem<divided>(smem)) return e;
@@ -943,7 +974,7 @@ static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
     // And where as narrow tiles all of them run at once: a part of the sum is a quarter as much to add up, a gathered step a quarter of the rows.
     // us, narrow / wide: 753 rows, 4 experts of 104 x 1512 8.9 / 15.1; 256 rows of 2048 x 2048 10.5 / 14.3, of a list 11.0 / 16.0; 512 rows of 1024 x 1024
     // 7.3 / 8.1; but 100 rows of 4096 x 4096 13.0 / 12.3.
-    const long long narrow = ((MODE == kGroupedDx ? a.k : a.n) + 127) / 128 * ((a.slots < a.experts ? a.slots : a.experts) + a.slots / 64);
+    const long long narrow = ((MODE == kGroupedDx ? a.k : a.n) + 127) / 128 * ((ADAPT == kAddLow ? 1 + a.experts / 4 : a.slots < a.experts ? a.slots : a.experts) + a.slots / 64);
     // kMakeLow: the rank is at most a few tiles' rows, so that narrow ones are what there is to run at once.
     if (ADAPT == kMakeLow || a.slots <= 32ll * a.experts || narrow <= device_sm_count()) return grouped_tiles<T, TO, MODE, 64, 1, GATHER, false, ADAPT>(a, st);
     if constexpr (ADAPT != kMakeLow) return grouped_tiles<T, TO, MODE, 256, 2, GATHER, false, ADAPT>(a, st);
@@ -1015,9 +1046,10 @@ static int grouped_call(const flexspmv_expert_desc* d, const void* const* in, vo
   return d->type == FLEXSPMV_TYPE_BF16 ? go(__nv_bfloat16()) : go(__half());
 }
 
-int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* low, int low_width, const int* offsets,
-                    const int* ids, void* out, int* status, cudaStream_t st) {
-  GroupedArgs a = {x, weight, offsets, nullptr, out, d->tokens, d->tokens, d->x_stride, 0, 1, d->n, d->k, status};
+int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* low, int low_width, int num_groups,
+                    const int* groups, const int* group_adapters, const int* ids, void* out, int* status, cudaStream_t st) {
+  GroupedArgs a = {x, weight, groups, nullptr, out, d->tokens, d->tokens, d->x_stride, 0, num_groups, d->n, d->k, status};
+  a.group_adapters = group_adapters;
   a.ids = ids;
   a.up = up;
   a.low = low;
