@@ -2,9 +2,12 @@
 // Here: the plan of a batch and the first product, low[t] = scale A x[t].  The rest is the shared product's epilogue (flex_grouped.cu).
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "flex_adapters.cuh"
 #include "flex_common.cuh"
 #include "flex_expert_types.cuh"
+#include "flex_umma.cuh"
 
 namespace flex {
 
@@ -212,19 +215,20 @@ struct LowArgs {
   int rank, k, width;
 };
 
-// low[t] = scale A x[t] of few tokens: a CTA takes a tile of up to 16 tokens of one adapter and 16 values of the rank (blockIdx.y), its warps neighbouring
-// parts of the sum in turn, whose sums meet in shared memory in the warps' order.  Bound by the latency of reading the adapter, not by arithmetic, so the warp's own matrix
-// instruction is enough and its operands come from global memory as they are: as the sum's index may be permuted, a lane's share of two instructions
-// is 16 contiguous bytes of a row, and eight rows of 64 bytes are one load of the warp.  Many tokens: grouped_kernel.
-constexpr int kLowThreads = 512, kLowAhead = 4;          // loads of so many steps under way
+// low[t] = scale A x[t] of few tokens: a cluster of four CTAs takes a tile of up to 16 tokens of one adapter and 16 values of the rank (blockIdx.y), their warps every 32nd 32 of
+// the sum, so that a long one is one round of loads; the warps' and the CTAs' sums meet in shared memory in their order.  Bound by the latency of reading the adapter, not
+// by arithmetic, so the warp's own matrix instruction is enough and its operands come from global memory as they are: as the sum's index may be permuted, a lane's share of
+// two instructions is 16 contiguous bytes of a row, and eight rows of 64 bytes are one load of the warp.  Many tokens: grouped_kernel.
+// 256 threads leave room on their SM for a CTA of the product that begins meanwhile.
+constexpr int kLowThreads = 256, kLowCtas = 4, kLowAhead = 4;          // loads of so many steps under way
 template <class T>
 __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(LowArgs a) {
-  constexpr int kWarps = kLowThreads / 32, kStep = 32 * kWarps;
-  __shared__ float part[kWarps][16][17];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, g = lane >> 2, r0 = blockIdx.y * 16;
+  constexpr int kWarps = kLowThreads / 32, kStep = 32 * kWarps * kLowCtas;
+  __shared__ float part[kWarps][16][17], sums[256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, g = lane >> 2, r0 = blockIdx.y * 16, share = (int)cluster_rank();
   pdl_wait();
   pdl_launch_dependents();
-  if ((int)blockIdx.x >= *a.count) return;
+  if ((int)blockIdx.x >= *a.count) return;          // the whole cluster
   const AdapterTile tile = a.tiles[blockIdx.x];
   // rows and ranks that are not there: the first one's, whose results are left out
   const T *x[2], *down[2];
@@ -238,17 +242,17 @@ __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(LowArgs a) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i / 4][i % 4] = 0.f;
   const bool high = tile.count > 8;          // else the upper rows' loads are left out
-  for (int k0 = warp * 32; k0 < a.k; k0 += kStep * kLowAhead) {
+  for (int k0 = (share * kWarps + warp) * 32; k0 < a.k; k0 += kStep * kLowAhead) {
     uint4 v[kLowAhead][2], w[kLowAhead][2];
 #pragma unroll
     for (int u = 0; u < kLowAhead; ++u) {
       const int k = k0 + u * kStep + q * 8;
       v[u][0] = v[u][1] = w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
       if (k < a.k) {
-        v[u][0] = *reinterpret_cast<const uint4*>(x[0] + k);
-        if (high) v[u][1] = *reinterpret_cast<const uint4*>(x[1] + k);
         w[u][0] = *reinterpret_cast<const uint4*>(down[0] + k);
         w[u][1] = *reinterpret_cast<const uint4*>(down[1] + k);
+        v[u][0] = *reinterpret_cast<const uint4*>(x[0] + k);
+        if (high) v[u][1] = *reinterpret_cast<const uint4*>(x[1] + k);
       }
     }
 #pragma unroll
@@ -264,28 +268,52 @@ __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(LowArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[warp][g + i / 2 * 8][j * 8 + q * 2 + i % 2] = acc[j][i];
   __syncthreads();
-  if (threadIdx.x >= 256) return;
   const int p = threadIdx.x / 16, r = r0 + threadIdx.x % 16;
-  if (p >= tile.count) return;
-  float h = 0.f;                           // 16 at a time, with zeros: the second product takes as many
-  if (r < a.rank) {
+  float h = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) h += part[w][p][threadIdx.x % 16];
-    if (a.scale) h *= a.scale[tile.adapter];
+  for (int w = 0; w < kWarps; ++w) h += part[w][p][threadIdx.x % 16];
+  sums[threadIdx.x] = h;
+  cluster_sync();
+  // each CTA some of the tokens; 16 of the rank at a time, with zeros: the second product takes as many
+  if (p < tile.count && p % kLowCtas == share) {
+    h = 0.f;
+    if (r < a.rank) {
+#pragma unroll
+      for (int c = 0; c < kLowCtas; ++c) h += cluster_load(cluster_smem(&sums[threadIdx.x], c));
+      if (a.scale) h *= a.scale[tile.adapter];
+    }
+    T* const row = static_cast<T*>(a.low) + (long long)a.rows[tile.from + p] * a.width;
+    row[low_high(r, a.rank)] = from_float<T>(h);
+    row[low_rest(r, a.rank)] = from_float<T>(low_rest_of<T>(h));
   }
-  T* const row = static_cast<T*>(a.low) + (long long)a.rows[tile.from + p] * a.width;
-  row[low_high(r, a.rank)] = from_float<T>(h);
-  row[low_rest(r, a.rank)] = from_float<T>(low_rest_of<T>(h));
+  cluster_sync();                          // no CTA leaves while its sums may be read
+}
+
+// The SMs divide their memory as for the kernel that follows: else a CTA of that one waits until an SM is empty.
+template <auto KERNEL>
+static int shared_memory_first() {
+  static std::atomic<bool> done[64];
+  int device = 0;
+  if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return (int)e;
+  const bool known = device >= 0 && device < 64;
+  if (known && done[device].load(std::memory_order_relaxed)) return 0;
+  if (cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared); e != cudaSuccess)
+    return (int)e;
+  if (known) done[device].store(true, std::memory_order_relaxed);
+  return 0;
 }
 
 template <class T>
 static int low_product(const LowArgs& a, const AdapterPlan& p, cudaStream_t st) {
+  if (int e = shared_memory_first<adapter_low_kernel<T>>()) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.most_tiles, (unsigned)((a.rank + 15) / 16)); cfg.blockDim = dim3(kLowThreads); cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr; cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  cfg.gridDim = dim3((unsigned)p.most_tiles, (unsigned)((a.rank + 15) / 16), kLowCtas); cfg.blockDim = dim3(kLowThreads); cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = kLowCtas;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = pdl_enabled() ? 2 : 1;
   return (int)cudaLaunchKernelEx(&cfg, adapter_low_kernel<T>, a);
 }
 

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict_
 // there instead of 0.43.)  dw's rows are other ones in every step: gathered like this they take 0.57 ms of the 32 768; a copy of them in the
 // workspace and contiguous tile copies 0.44.
 // ADAPT (forward): kAddLow: one matrix for all groups, and each place's adapter's up matrix times its vector of `rank` values.  Groups of one adapter have it as one to
-// a few steps more of their sum; in mixed groups it is added on a place's way out, before the only rounding (add_low_rank), by the warps' own matrix instructions, which
+// a few steps more of their sum; in mixed groups it is added on a place's way out, before the only rounding (low_rank_part), by the warps' own matrix instructions, which
 // keep the tensor cores from the sums for some eight times as long (us, 8192 tokens of rank 64 in 12 runs, all that way 313 altogether, as groups 200).
 // kMakeLow: those vectors, scale A x, rows by a list, in two 16-bit values each.
 // Warps 0-7 store finished accumulators, warp 8 issues the tile copies, warp 9 the matrix instructions; two accumulators in tensor memory,
@@ -158,15 +158,21 @@ __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const Group
   return r;
 }
 
-// Adds the low-rank parts of 32 features from m on by 32 places: the accumulator's registers (tmem_load_blocks) are laid out as those of the warp's own
-// matrix instruction, 16 features by 8 places, so that it can finish here what the tensor memory holds.  Each adapter among the places has a product of
-// its own and only its places take it up: what is not finite in one request's adapter stays out of the others.  The sum's index may be permuted as long as both
-// operands are alike, so a lane takes 8 neighbouring values of a row in one load, which are its share of two instructions.
+// The low-rank parts of 32 features from m on by 32 places, laid out as the accumulator's registers are (tmem_load_blocks), since the warp's own matrix
+// instruction, 16 features by 8 places, has them so.  Each adapter among the places has a product of its own and only its places take it up: what is not finite in
+// one request's adapter stays out of the others.  The sum's index may be permuted as long as both operands are alike, so a lane takes 8 (ranks up to 16: 4)
+// neighbouring values of a row in one load, which are its share of two instructions (one).
+struct LowPart {
+  float low[16], high[16];
+};
 template <class T>
-__device__ __forceinline__ void add_low_rank(const GroupedArgs& a, int m, int place, int left, int lane, uint32_t (&low)[16], uint32_t (&high)[16]) {
+__device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int place, int left, int lane, LowPart& r) {
   const int q = lane & 3, g = lane >> 2;
   const int id = lane < left ? a.ids[place + lane] : -1;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r.low[i] = r.high[i] = 0.f;
   unsigned todo = __ballot_sync(0xffffffffu, (unsigned)id < (unsigned)a.adapters);
+  const T* const low = static_cast<const T*>(a.low) + (size_t)(place + g) * a.low_width;
   while (todo) {
     const int adapter = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
     const unsigned mine = __ballot_sync(0xffffffffu, id == adapter);
@@ -175,22 +181,23 @@ __device__ __forceinline__ void add_low_rank(const GroupedArgs& a, int m, int pl
 #pragma unroll
     for (int i = 0; i < 32; ++i) d[i / 16][i / 4 % 4][i % 4] = 0.f;
     const T* const up = static_cast<const T*>(a.up) + ((size_t)adapter * a.n + m + g) * a.rank;
-#pragma unroll 2
-    for (int k = q * 8; k - q * 8 < a.rank; k += 32) {
-      const bool inside = k < a.rank;
-      uint4 w[4], h[4][2];                 // all under way at once
+    // all loads of a step under way at once
+    if (a.rank <= 16) {
+      const int k = q * 4;
+      const uint2 none = make_uint2(0, 0);
+      uint2 w[4], h[4][2];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        w[i] = make_uint4(0, 0, 0, 0);
-        if (inside && m + g + i * 8 < a.n) w[i] = *reinterpret_cast<const uint4*>(up + (size_t)i * 8 * a.rank + k);
+        w[i] = none;
+        if (k < a.rank && m + g + i * 8 < a.n) w[i] = *reinterpret_cast<const uint2*>(up + (size_t)i * 8 * a.rank + k);
       }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        h[b][0] = h[b][1] = make_uint4(0, 0, 0, 0);
-        if (inside && (mine >> (b * 8 + g) & 1u)) {
-          const T* const row = static_cast<const T*>(a.low) + (size_t)(place + b * 8 + g) * a.low_width;
-          h[b][0] = *reinterpret_cast<const uint4*>(row + low_high(k, a.rank));
-          h[b][1] = *reinterpret_cast<const uint4*>(row + low_rest(k, a.rank));
+        h[b][0] = h[b][1] = none;
+        if (k < a.rank && (mine >> (b * 8 + g) & 1u)) {
+          const T* const row = low + (size_t)b * 8 * a.low_width + k;
+          h[b][0] = *reinterpret_cast<const uint2*>(row);
+          h[b][1] = *reinterpret_cast<const uint2*>(row + 32);
         }
       }
 #pragma unroll
@@ -199,10 +206,38 @@ __device__ __forceinline__ void add_low_rank(const GroupedArgs& a, int m, int pl
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            warp_mma<T>(d[i][b], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h[b][x].x, h[b][x].y);
-            warp_mma<T>(d[i][b], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, h[b][x].z, h[b][x].w);
+          for (int x = 0; x < 2; ++x) warp_mma<T>(d[i][b], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h[b][x].x, h[b][x].y);
+      }
+    } else {
+#pragma unroll 1
+      for (int k = q * 8; k - q * 8 < a.rank; k += 32) {
+        const bool inside = k < a.rank;
+        uint4 w[4], h[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] = make_uint4(0, 0, 0, 0);
+          if (inside && m + g + i * 8 < a.n) w[i] = *reinterpret_cast<const uint4*>(up + (size_t)i * 8 * a.rank + k);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          h[b][0] = h[b][1] = make_uint4(0, 0, 0, 0);
+          if (inside && (mine >> (b * 8 + g) & 1u)) {
+            const T* const row = low + (size_t)b * 8 * a.low_width;
+            h[b][0] = *reinterpret_cast<const uint4*>(row + low_high(k, a.rank));
+            h[b][1] = *reinterpret_cast<const uint4*>(row + low_rest(k, a.rank));
           }
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          if (!(mine >> (b * 8) & 0xffu)) continue;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              warp_mma<T>(d[i][b], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h[b][x].x, h[b][x].y);
+              warp_mma<T>(d[i][b], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, h[b][x].z, h[b][x].w);
+            }
+        }
       }
     }
 #pragma unroll
@@ -210,22 +245,21 @@ __device__ __forceinline__ void add_low_rank(const GroupedArgs& a, int m, int pl
 #pragma unroll
       for (int x = 0; x < 4; ++x)
         if (mine >> (b * 8 + q * 2 + (x & 1)) & 1u) {
-          low[b * 4 + x] = __float_as_uint(__uint_as_float(low[b * 4 + x]) + d[0][b][x]);
-          high[b * 4 + x] = __float_as_uint(__uint_as_float(high[b * 4 + x]) + d[1][b][x]);
+          r.low[b * 4 + x] = d[0][b][x];
+          r.high[b * 4 + x] = d[1][b][x];
         }
   }
 }
 
 // The same for eight neighbouring features of one place, by one thread.
 template <class T>
-__device__ __forceinline__ void add_low_rank(const GroupedArgs& a, int m, int place, float (&sum)[8]) {
+__device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int place, float (&part)[8]) {
   const int id = a.ids[place];
+#pragma unroll
+  for (int x = 0; x < 8; ++x) part[x] = 0.f;
   if ((unsigned)id >= (unsigned)a.adapters) return;
   const T* const up = static_cast<const T*>(a.up) + ((size_t)id * a.n + m) * a.rank;
   const T* const row = static_cast<const T*>(a.low) + (size_t)place * a.low_width;
-  float part[8];
-#pragma unroll
-  for (int x = 0; x < 8; ++x) part[x] = 0.f;
   for (int k = 0; k < a.rank; k += 8) {
     Pack<T, 8> h, rest, w[8];
     h.load(row + low_high(k, a.rank));
@@ -240,8 +274,6 @@ __device__ __forceinline__ void add_low_rank(const GroupedArgs& a, int m, int pl
 #pragma unroll
       for (int i = 0; i < 8; ++i) part[x] = fmaf(w[x].get(i), v[i], part[x]);
   }
-#pragma unroll
-  for (int x = 0; x < 8; ++x) sum[x] += part[x];
 }
 
 // SPLIT: asks for this CTA's rows of the up matrices, which its last step reads, while nothing else is to be done.
@@ -379,6 +411,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   auto step_from = [&](int steps) { return SPLIT ? steps * share / split : 0; };
   auto step_to = [&](int steps) { return SPLIT ? steps * (share + 1) / split : steps; };
 
+  float early[8];                          // kAddLow, SPLIT: what a thread adds to its first item
   if (warp == kCopyWarp) {
     int stage = 0, issued = 0;
     uint32_t phase = 0;
@@ -605,6 +638,13 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
     if (ADAPT == kAddLow) {
       if (SPLIT) prefetch_up<T>(a, share, split, tid);
       pdl_wait();
+      if (SPLIT && first < tiles) {        // while the sum is still under way
+        const GroupedTile t = tile_at<MODE, NT, PAIR, HALVES>(a, table, first);
+        const int eights = (t.cols + 7) / 8, c_from = eights * share / split * 8, c_to = eights * (share + 1) / split * 8;
+        const int c = c_from + tid / 16, r = tid % 16 * 8;
+        if (tid < (c_to - c_from) * 16 && c < t.count && t.m0 + r < a.n && group_adapters[t.e] == kGroupMixed)
+          low_rank_part<T>(a, t.m0 + r, t.from + c, early);
+      }
     }
     int acc = 0;
     uint32_t acc_phase = 0, second_phase = 0;
@@ -707,6 +747,11 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           if (part * 32 + g * 64 < t.cols) store_rows(part * 32 + g * 64, [&](int x) { return sum[g][x]; });
         continue;
       }
+      // kAddLow: made while the sum is still under way
+      LowPart parts;
+      const bool mixed = ADAPT == kAddLow && group_adapters[t.e] == kGroupMixed;
+      if constexpr (ADAPT == kAddLow)
+        if (mixed) low_rank_part<T>(a, m, t.from + part * 32, t.count - part * 32, lane, parts);
       if (!wait_warp(&bars.acc_full[acc], full_phase)) break;
       tmem_fence_after();
       const uint32_t d = tmem + acc * NT + ((uint32_t)(quarter * 32) << 16);
@@ -725,7 +770,12 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
         if (last) free_accumulator();
         if (!there) break;
         if constexpr (ADAPT == kAddLow)
-          if (group_adapters[t.e] == kGroupMixed) add_low_rank<T>(a, m, t.from + c0, t.count - c0, lane, low, high);
+          if (mixed)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              low[i] = __float_as_uint(__uint_as_float(low[i]) + parts.low[i]);
+              high[i] = __float_as_uint(__uint_as_float(high[i]) + parts.high[i]);
+            }
         if (MODE == kGroupedDw) {
           store_rows(c0, [&](int x) { return __uint_as_float(v[x]); });
         } else {
@@ -774,6 +824,8 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           }
         }
         if (last) break;
+        if constexpr (ADAPT == kAddLow)
+          if (mixed) low_rank_part<T>(a, m, t.from + c0 + 64, t.count - c0 - 64, lane, parts);
       }
       if (HALVES == 2) {
         if (half) second_phase ^= 1;
@@ -795,8 +847,8 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   }
   if (SPLIT) {
     // every CTA stores some of the tile's columns, eight neighbouring rows (dw: columns) at a time
+    constexpr int kStoreThreads = ADAPT == kAddLow ? kStoreWarps * 32 : kThreads;
     cluster_sync();
-    if (ADAPT == kAddLow) pdl_wait();
     if (first < tiles && !*abort) {
       const GroupedTile t = tile_at<MODE, NT, PAIR, HALVES>(a, table, first);
       const int eights = (t.cols + 7) / 8, c_from = eights * share / split * 8, c_to = eights * (share + 1) / split * 8;
@@ -804,7 +856,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
       TO* const out = static_cast<TO*>(a.out);
       constexpr bool kDw = MODE == kGroupedDw;
       const int items = (c_to - c_from) * 16;            // of eight values
-      for (int i = tid; i < items; i += kThreads) {
+      for (int i = tid; i < items && tid < kStoreThreads; i += kStoreThreads) {
         // forward, dx: 16 items a column; dw: 128 items for eight columns
         const int c = kDw ? c_from + i / 128 * 8 : c_from + i / 16, r = kDw ? i % 128 : i % 16 * 8;
         float sum[8];
@@ -824,7 +876,11 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           for (int x = 0; x < 8; ++x) sum[x] += v[x];
         }
         if constexpr (ADAPT == kAddLow)
-          if (group_adapters[t.e] == kGroupMixed && c < t.count && t.m0 + r < a.n) add_low_rank<T>(a, t.m0 + r, t.from + c, sum);
+          if (group_adapters[t.e] == kGroupMixed && c < t.count && t.m0 + r < a.n) {
+            if (i != tid) low_rank_part<T>(a, t.m0 + r, t.from + c, early);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) sum[x] += early[x];
+          }
         Pack<TO, 8> q;
 #pragma unroll
         for (int x = 0; x < 8; ++x) q.set(x, sum[x]);
@@ -974,7 +1030,7 @@ static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
     // And where as narrow tiles all of them run at once: a part of the sum is a quarter as much to add up, a gathered step a quarter of the rows.
     // us, narrow / wide: 753 rows, 4 experts of 104 x 1512 8.9 / 15.1; 256 rows of 2048 x 2048 10.5 / 14.3, of a list 11.0 / 16.0; 512 rows of 1024 x 1024
     // 7.3 / 8.1; but 100 rows of 4096 x 4096 13.0 / 12.3.
-    const long long narrow = ((MODE == kGroupedDx ? a.k : a.n) + 127) / 128 * ((ADAPT == kAddLow ? 1 + a.experts / 4 : a.slots < a.experts ? a.slots : a.experts) + a.slots / 64);
+    const long long narrow = ((MODE == kGroupedDx ? a.k : a.n) + 127) / 128 * ((ADAPT == kAddLow ? 1 + a.experts / 16 : a.slots < a.experts ? a.slots : a.experts) + a.slots / 64);
     // kMakeLow: the rank is at most a few tiles' rows, so that narrow ones are what there is to run at once.
     if (ADAPT == kMakeLow || a.slots <= 32ll * a.experts || narrow <= device_sm_count()) return grouped_tiles<T, TO, MODE, 64, 1, GATHER, false, ADAPT>(a, st);
     if constexpr (ADAPT != kMakeLow) return grouped_tiles<T, TO, MODE, 256, 2, GATHER, false, ADAPT>(a, st);
