@@ -14,6 +14,7 @@ twice, with its gradients).  Ids that are no adapter are noticed on the device a
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -46,8 +47,14 @@ def _bytes(name: str, d: Desc) -> int:
     return need.value
 
 
-def _int32(n: int, what: str):
-    _need(n <= 0x7fffffff, f"{what} is too large: {n}")
+@functools.lru_cache(maxsize=256)
+def _project_bytes(tokens: int, rank: int) -> int:
+    return _bytes("adapted_project_bytes", Desc(tokens, 8, 1, rank, 8, 8, _TYPE[torch.bfloat16]))
+
+
+@functools.lru_cache(maxsize=256)
+def _plan_bytes(tokens: int, adapters: int) -> int:
+    return _bytes("adapter_plan_bytes", Desc(tokens, 0, adapters))
 
 
 @_operator
@@ -58,7 +65,7 @@ def plan(ids: torch.Tensor, num_adapters: int) -> Plan:
     if not (1 <= num_adapters <= MAX_ADAPTERS):
         raise FlexSpmvError(f"1 to {MAX_ADAPTERS} adapters, not {num_adapters}")
     d = Desc(ids.numel(), 0, num_adapters)
-    need = _bytes("adapter_plan_bytes", d)
+    need = _plan_bytes(d.tokens, num_adapters)
     data = torch.empty(need // 4, dtype=torch.int32, device=ids.device)
     flag = _flag(dev)
     return BoundCall(_function("adapter_plan", _PLAN), (ctypes.addressof(d), ids.data_ptr(), data.data_ptr(), need, flag.tensor.data_ptr()), dev,
@@ -77,29 +84,39 @@ def project(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: torch.Ten
     _tensor(weight, "weight", (x.dtype,), 2, dev)
     _tensor(a, "a", (x.dtype,), 3, dev)
     _tensor(b, "b", (x.dtype,), 3, dev)
-    for name, t in (("weight", weight), ("a", a), ("b", b)):
+    at = [x.data_ptr(), weight.data_ptr(), a.data_ptr(), b.data_ptr(), 0, 0]
+    for name, t, first in (("weight", weight, at[1]), ("a", a, at[2]), ("b", b, at[3])):
         _whole(t, name)
-        _need(t.data_ptr() % 16 == 0, f"{name}: the first value must be on 16 bytes")
-    tokens, (n, k), (adapters, rank, _) = x.shape[0], weight.shape, a.shape
-    _need(x.shape[1] == k and a.shape[2] == k, f"x's rows and a's must have {k} values, as weight's, not {x.shape[1]} and {a.shape[2]}")
-    _need(tuple(b.shape) == (adapters, n, rank), f"b must have the shape {(adapters, n, rank)}, not {tuple(b.shape)}")
+        if first % 16:
+            raise FlexSpmvError(f"{name}: the first value must be on 16 bytes")
+    (tokens, width), (n, k), (adapters, rank, k_a) = x.shape, weight.shape, a.shape
+    if width != k or k_a != k:
+        raise FlexSpmvError(f"x's rows and a's must have {k} values, as weight's, not {width} and {k_a}")
+    if b.shape != (adapters, n, rank):
+        raise FlexSpmvError(f"b must have the shape {(adapters, n, rank)}, not {tuple(b.shape)}")
     if not (n >= 8 and k >= 8 and rank >= 8 and n % 8 == 0 and k % 8 == 0 and rank % 8 == 0):
         raise FlexSpmvError(f"both sides of weight and the rank must be multiples of 8, not {n} x {k} and {rank}")
-    _need(rank <= MAX_RANK, f"a rank of at most {MAX_RANK}, not {rank}")
-    _int32(n, "n")
-    _int32(k, "k")
-    _need(isinstance(plan, Plan) and plan.data.device == x.device, "plan must be one of this module, on x's device")
-    _need(plan.tokens == tokens and plan.adapters == adapters, f"the plan is of {plan.tokens} tokens and {plan.adapters} adapters, not of {tokens} and {adapters}")
+    if not (rank <= MAX_RANK and n <= 0x7fffffff and k <= 0x7fffffff):
+        raise FlexSpmvError(f"a rank of at most {MAX_RANK} and sides of 31 bits, not {rank} and {n} x {k}")
+    if not (isinstance(plan, Plan) and plan.data.get_device() == dev):
+        raise FlexSpmvError("plan must be one of this module, on x's device")
+    if plan.tokens != tokens or plan.adapters != adapters:
+        raise FlexSpmvError(f"the plan is of {plan.tokens} tokens and {plan.adapters} adapters, not of {tokens} and {adapters}")
     if scale is not None:
         _tensor(scale, "scale", (torch.float32,), 1, dev)
         _whole(scale, "scale")
         _need(scale.numel() == adapters, "scale must have a value for each adapter")
+        at[4] = scale.data_ptr()
+    at[5] = plan.data.data_ptr()
     stride = _rows_of(x, "x")
-    out = _out(out, (tokens, n), x.dtype, x.device, x=x, weight=weight, a=a, b=b, scale=scale, plan=plan.data)
+    if out is None:
+        out = torch.empty((tokens, n), dtype=x.dtype, device=x.device)
+    else:
+        out = _out(out, (tokens, n), x.dtype, x.device, x=x, weight=weight, a=a, b=b, scale=scale, plan=plan.data)
     d = Desc(tokens, stride, adapters, rank, n, k, _TYPE[x.dtype])
-    need = _bytes("adapted_project_bytes", d)
+    need = _project_bytes(tokens, rank)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-    ins = (_P * 6)(*[t.data_ptr() if t is not None else 0 for t in (x, weight, a, b, scale, plan.data)])
+    ins = (_P * 6)(*at)
     outs = (_P * 1)(out.data_ptr())
     flag = _flag(dev)
     return BoundCall(_function("adapted_project", _PROJECT),

@@ -346,14 +346,14 @@ def balance_loss(logits: torch.Tensor, plan: Plan) -> Balance:
     stride = _rows_of(logits, "logits", aligned=False)
     d = Desc(tokens, 0, experts, 0, 0, 0, _TYPE[logits.dtype], 0, 0, 0, stride)
     need = _balance_bytes(tokens, experts, dev)
-    # one allocation: mean, counts, loss and tokens, then the workspace on 16 bytes
+    # one allocation: loss, tokens, mean and counts, then the workspace on 16 bytes
     at = (2 * experts + 2 + 3) // 4 * 4
     buf = torch.empty(at + need // 4, dtype=torch.int32, device=logits.device)
-    mean, counts, loss, there, _ = buf.split_with_sizes((experts, experts, 1, 1, at + need // 4 - 2 * experts - 2))
-    out = Balance(loss.view(torch.float32).view(()), counts, mean.view(torch.float32), there.view(()))
-    ins, outs = _pointers((logits, plan.offsets)), _pointers((loss, counts, mean, there))
-    return BoundCall(_function("balance_loss", _WITH_WORKSPACE),
-                     (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), buf.data_ptr() + 4 * at, need), dev,
+    reals = buf.view(torch.float32)
+    out = Balance(reals[0], buf[2 + experts:2 + 2 * experts], reals[2:2 + experts], buf[1])
+    base = buf.data_ptr()
+    ins, outs = (_P * 2)(logits.data_ptr(), plan.offsets.data_ptr()), (_P * 4)(base, base + 8 + 4 * experts, base + 8, base + 4)
+    return BoundCall(_function("balance_loss", _WITH_WORKSPACE), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), base + 4 * at, need), dev,
                      (d, ins, outs, logits, plan, buf), out)
 
 

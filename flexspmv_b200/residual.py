@@ -21,7 +21,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from .binding import FlexSpmvError, _pointers
-from .experts import _BYTES, _PLAIN, _TYPE, _WITH_WORKSPACE, BoundCall, _check, _function, _need, _operator, _out, _rows_of, _tensor, _whole
+from .experts import _BYTES, _PLAIN, _TYPE, _WITH_WORKSPACE, BoundCall, _check, _function, _operator, _out, _rows_of, _tensor, _whole
 
 MAX_WIDTH = 1 << 24                          # FLEXSPMV_MAX_WIDTH
 
@@ -46,35 +46,62 @@ class NormGradients(NamedTuple):
     dbias: Optional[torch.Tensor]
 
 
-def _matrix(t, name: str, like=None) -> int:
-    """Checks a matrix argument, of the type, shape and device of ``like``; returns its row stride."""
-    _tensor(t, name, tuple(_TYPE) if like is None else (like.dtype,), 2, None if like is None else like.get_device())
-    if like is not None and t.shape != like.shape:
-        raise FlexSpmvError(f"{name} must have the shape {tuple(like.shape)}, not {tuple(t.shape)}")
-    _need(1 <= t.shape[1] <= MAX_WIDTH, f"{name} must have 1 to {MAX_WIDTH} columns")
+_ANY, _WIDE, _SEED = tuple(_TYPE), {t: (torch.float32, t) for t in _TYPE}, (torch.int64,)
+
+
+def _stride(t, name: str, rows: int, width: int) -> int:
+    """Row stride of a checked matrix, whose rows must be contiguous."""
+    if t.is_contiguous():
+        return width
     return _rows_of(t, name, aligned=False)
 
 
-def _params(weight, bias, x) -> int:
+def _first(x, name: str):
+    """Checks the matrix that says the type, shape and device of a call's others; returns device, rows, width and row stride."""
+    dev = _tensor(x, name, _ANY, 2)
+    rows, width = x.shape
+    if not 1 <= width <= MAX_WIDTH:
+        raise FlexSpmvError(f"{name} must have 1 to {MAX_WIDTH} columns, not {width}")
+    return dev, rows, width, _stride(x, name, rows, width)
+
+
+def _matrix(t, name: str, like, dev: int, rows: int, width: int) -> int:
+    """Checks another matrix of the call; returns its row stride.  None: 0."""
+    if t is None:
+        return 0
+    _tensor(t, name, (like.dtype,), 2, dev)
+    if t.shape != like.shape:
+        raise FlexSpmvError(f"{name} must have the shape {tuple(like.shape)}, not {tuple(t.shape)}")
+    return _stride(t, name, rows, width)
+
+
+def _vector(t, name: str, dtypes, n: int, dev: int, of: str):
+    _tensor(t, name, dtypes, 1, dev)
+    if t.shape[0] != n:
+        raise FlexSpmvError(f"{name} must have {n} values, one for each {of}, not {t.shape[0]}")
+    _whole(t, name)
+
+
+def _params(weight, bias, x, width: int, dev: int) -> int:
     """Checks weight and bias; returns their type."""
-    kind = None
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _tensor(t, name, (torch.float32, x.dtype) if kind is None else (kind,), 1, x.get_device())
-            _whole(t, name)
-            _need(t.shape[0] == x.shape[1], f"{name} must have a value for each column")
-            kind = t.dtype
-    return _TYPE[kind or torch.float32]
+    kinds = _WIDE[x.dtype]
+    if weight is not None:
+        _vector(weight, "weight", kinds, width, dev, "column")
+        kinds = (weight.dtype,)
+    if bias is not None:
+        _vector(bias, "bias", kinds, width, dev, "column")
+        kinds = (bias.dtype,)
+    return _TYPE[kinds[0]]
 
 
-def _drops(p, seed, x) -> float:
+def _drops(p, seed, dev: int) -> float:
     p = float(p)
-    _need(0.0 <= p < 1.0, f"p must be at least 0 and below 1, not {p}")
+    if not 0.0 <= p < 1.0:
+        raise FlexSpmvError(f"p must be at least 0 and below 1, not {p}")
     if p > 0.0:
-        _need(seed is not None, "p > 0 takes a seed")
-        _tensor(seed, "seed", (torch.int64,), 1, x.get_device())
-        _whole(seed, "seed")
-        _need(seed.shape[0] == 2, "seed must have two values, a seed and an offset")
+        if seed is None:
+            raise FlexSpmvError("p > 0 takes a seed")
+        _vector(seed, "seed", _SEED, 2, dev, "of seed and offset")
     return p
 
 
@@ -89,17 +116,14 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     ``x`` and ``residual`` (rows, width) of one type; ``weight`` and ``bias`` (width) of that type or float32.  ``s`` is normalised before it is
     rounded; it is returned, rounded, where it is not ``x`` itself."""
-    dev = _tensor(x, "x", tuple(_TYPE), 2)
-    xs = _matrix(x, "x")
-    rs = _matrix(residual, "residual", x) if residual is not None else 0
-    kind, p = _params(weight, bias, x), _drops(p, seed, x)
-    eps = float(eps)
-    _need(eps >= 0.0, f"eps must not be negative or NaN: {eps}")
-    rows, width = x.shape
+    dev, rows, width, xs = _first(x, "x")
+    rs = _matrix(residual, "residual", x, dev, rows, width)
+    kind, p, eps = _params(weight, bias, x, width, dev), _drops(p, seed, dev), float(eps)
+    if not eps >= 0.0:
+        raise FlexSpmvError(f"eps must not be negative or NaN: {eps}")
     y = torch.empty((rows, width), dtype=x.dtype, device=x.device)
     total = torch.empty_like(y) if residual is not None or p > 0.0 else None
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    out = Normed(y, total, stats[0], stats[1])
+    out = Normed(y, total, *torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind())
     d = Desc(rows, width, (xs, rs, 0), _TYPE[x.dtype], kind, eps, 0, p)
     ins, outs = _at(x, residual, weight, bias, seed if p > 0.0 else None), _at(y, total, out.mean, out.rstd)
     return BoundCall(_function("layer_norm", _PLAIN), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs)), dev,
@@ -120,21 +144,19 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
                         dsum: Optional[torch.Tensor] = None, p: float = 0.0, seed: Optional[torch.Tensor] = None) -> NormGradients:
     """Gradients of ``layer_norm``.  ``x`` is what was normalised (``Normed.sum`` where there is one), ``dsum`` a gradient that reaches it directly;
     ``dx`` is what passes the dropout of ``p`` and ``seed``.  ``dweight`` and ``dbias`` are of the weight's type; without a weight there are none."""
-    dev = _tensor(dy, "dy", tuple(_TYPE), 2)
-    ys, xs = _matrix(dy, "dy"), _matrix(x, "x", dy)
-    ds = _matrix(dsum, "dsum", dy) if dsum is not None else 0
-    kind, p = _params(weight, None, dy), _drops(p, seed, dy)
-    rows, width = dy.shape
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        _tensor(t, name, (torch.float32,), 1, dev)
-        _whole(t, name)
-        _need(t.shape[0] == rows, f"{name} must have a value for each row")
+    dev, rows, width, ys = _first(dy, "dy")
+    if x is None:
+        raise FlexSpmvError("x is what was normalised")
+    xs, ds = _matrix(x, "x", dy, dev, rows, width), _matrix(dsum, "dsum", dy, dev, rows, width)
+    kind, p = _params(weight, None, dy, width, dev), _drops(p, seed, dev)
+    _vector(mean, "mean", (torch.float32,), rows, dev, "row")
+    _vector(rstd, "rstd", (torch.float32,), rows, dev, "row")
     dresidual = torch.empty((rows, width), dtype=dy.dtype, device=dy.device)
     dx = torch.empty_like(dresidual) if p > 0.0 else dresidual
     dweight = dbias = ws = None
     need = 0
     if weight is not None:
-        dweight, dbias = torch.empty_like(weight), torch.empty_like(weight)
+        dweight, dbias = torch.empty((2, width), dtype=weight.dtype, device=weight.device).unbind()
         need = _backward_bytes(rows, width, dev)
         ws = torch.empty(need, dtype=torch.uint8, device=dy.device)
     out = NormGradients(dx, dresidual, dweight, dbias)
@@ -149,15 +171,16 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
 def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``residual + x * keep / (1 - p)`` (no residual: 0), where ``keep`` is 1 with the probability ``1 - p``.  Its gradient with respect to ``x`` is
     ``dropout(dout, p, seed)``."""
-    dev = _tensor(x, "x", tuple(_TYPE), 2)
-    xs = _matrix(x, "x")
-    rs = _matrix(residual, "residual", x) if residual is not None else 0
-    _need(seed is not None, "dropout takes a seed")
-    p = _drops(p, seed, x)
+    dev, rows, width, xs = _first(x, "x")
+    rs = _matrix(residual, "residual", x, dev, rows, width)
+    p = _drops(p, seed, dev)
     if p == 0.0:
-        _drops(0.5, seed, x)                 # the seed is not used, but is one
-    out = _out(out, tuple(x.shape), x.dtype, x.device, x=x, residual=residual, seed=seed)
-    d = Desc(x.shape[0], x.shape[1], (xs, rs, 0), _TYPE[x.dtype], 0, 0.0, 0, p)
+        _drops(0.5, seed, dev)               # the seed is not used, but is one
+    if out is None:
+        out = torch.empty((rows, width), dtype=x.dtype, device=x.device)
+    else:
+        out = _out(out, (rows, width), x.dtype, x.device, x=x, residual=residual, seed=seed)
+    d = Desc(rows, width, (xs, rs, 0), _TYPE[x.dtype], 0, 0.0, 0, p)
     ins, outs = _at(x, residual, seed), _pointers((out,))
     return BoundCall(_function("dropout", _PLAIN), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs)), dev,
                      (d, ins, outs, x, residual, seed, out), out)
