@@ -9,6 +9,7 @@
 
 #include "flex_common.cuh"
 #include "flex_expert_types.cuh"
+#include "flex_umma.cuh"
 
 namespace flex {
 
@@ -408,15 +409,20 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const float* __rest
 
 // ---- balance -------------------------------------------------------------------------------------------------------
 
+// The largest of a warp's values; NaN only where all are.
+__device__ __forceinline__ float warp_largest(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
 // The softmax of a row whose part is in this warp's lanes: powers in e, their base and the factor that makes probabilities of them.  A row of -infinity
-// alone has none: its powers are 0.
-template <class T, int V, int W>
-__device__ __forceinline__ bool softmax_of(const LanePart<T, V, W>& part, bool exact, float (&e)[V], float& base, float& factor) {
+// alone has none: its powers are 0.  `more`: other values that are added up over the lanes, in the same steps; it gets the powers first.
+template <class T, int V, int W, int N, class F>
+__device__ __forceinline__ bool softmax_of(const LanePart<T, V, W>& part, bool exact, float (&e)[V], float& base, float& factor, float (&more)[N], const F& before) {
   float top = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) top = fmaxf(top, part.piece[i / W].get(i % W));
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  top = warp_largest(top);
   const bool there = top > -INFINITY;
   base = there ? top : 0.f;
   // results of 32 bits far below the largest: as in the router's gradient
@@ -434,8 +440,13 @@ __device__ __forceinline__ bool softmax_of(const LanePart<T, V, W>& part, bool e
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) sum += e[i];
+  before();
 #pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int o = 16; o; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+    for (int n = 0; n < N; ++n) more[n] += __shfl_xor_sync(0xffffffffu, more[n], o);
+  }
   factor = there ? __frcp_rn(sum) : 1.f;
   return there;
 }
@@ -445,8 +456,8 @@ struct BalanceArgs {
   const int* offsets;
   long long tokens, stride;
   int experts;
-  float* parts;                    // [CTAs][experts]: sums of the probabilities of a CTA's tokens
-  int* part_tokens;                // [CTAs]: its rows that are not all -infinity
+  float* parts;                    // [clusters][experts]: sums of the probabilities of a cluster's tokens
+  int* part_tokens;                // [clusters]: its rows that are not all -infinity
   float *loss, *mean;
   int *counts, *there;
 };
@@ -477,8 +488,11 @@ __device__ __forceinline__ void balance_end(const BalanceArgs& a, const float* t
   }
 }
 
-// A warp takes every so-many-th token and keeps its lanes' experts' sums in registers; the warps' sums meet in shared memory, the CTAs' in a second
+// A warp takes every so-many-th token and keeps its lanes' experts' sums in registers; the warps' and two CTAs' sums meet in shared memory, the clusters' in a second
 // launch, each in a fixed order.  Bound by memory with many tokens (the logits are read once), by the launch with few (SMALL: one CTA does it all).
+// us, 32 771 tokens of 256 experts in 16 bits: 13.5; with 16 warps an SM 15.9, two tokens a warp at a time 14.3, single CTAs 14.4, clusters of four, not all of which
+// are on the chip at once, 19.8.
+constexpr int kBalanceCtas = 2;
 template <class T, int V, int W, int THREADS, bool SMALL>
 __global__ void __launch_bounds__(THREADS) balance_kernel(BalanceArgs a) {
   extern __shared__ __align__(16) float balance_sm[];          // [warps][experts]
@@ -500,8 +514,8 @@ __global__ void __launch_bounds__(THREADS) balance_kernel(BalanceArgs a) {
   for (; t < a.tokens; t += step) {
     const LanePart<T, V, W> part = next;
     if (t + step < a.tokens) next.load(logits + (t + step) * a.stride, a.experts, lane);
-    float e[V], base, factor;
-    there += softmax_of<T, V, W>(part, false, e, base, factor);
+    float e[V], base, factor, none[1] = {0.f};
+    there += softmax_of<T, V, W>(part, false, e, base, factor, none, [] {});
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = fmaf(e[i], factor, acc[i]);
   }
@@ -518,32 +532,46 @@ __global__ void __launch_bounds__(THREADS) balance_kernel(BalanceArgs a) {
     float sum = 0.f;
 #pragma unroll 8
     for (int w = 0; w < kWarps; ++w) sum += balance_sm[w * a.experts + e];
-    if (SMALL) balance_sm[e] = sum;          // column e is this thread's alone
-    else a.parts[(size_t)blockIdx.x * a.experts + e] = sum;
+    balance_sm[e] = sum;                   // column e is this thread's alone
   }
   if (SMALL) {
     __syncthreads();
     balance_end<THREADS>(a, balance_sm, tokens);
-  } else if (threadIdx.x == 0) {
-    a.part_tokens[blockIdx.x] = tokens;
+    return;
   }
+  __shared__ int cta_tokens;
+  if (threadIdx.x == 0) cta_tokens = tokens;
+  cluster_sync();
+  const int share = (int)cluster_rank(), cluster = blockIdx.x / kBalanceCtas;
+  for (int e = threadIdx.x * kBalanceCtas + share; e < a.experts; e += THREADS * kBalanceCtas) {
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < kBalanceCtas; ++c) sum += cluster_load(cluster_smem(&balance_sm[e], c));
+    a.parts[(size_t)cluster * a.experts + e] = sum;
+  }
+  if (share == 0 && threadIdx.x == 0) {
+    int all = 0;
+    for (int c = 0; c < kBalanceCtas; ++c) all += __float_as_int(cluster_load(cluster_smem(&cta_tokens, c)));
+    a.part_tokens[cluster] = all;
+  }
+  cluster_sync();                          // no CTA leaves while its sums may be read
 }
 
-__global__ void __launch_bounds__(1024) balance_end_kernel(BalanceArgs a, int ctas) {
+__global__ void __launch_bounds__(1024) balance_end_kernel(BalanceArgs a, int clusters) {
   __shared__ float total[FLEXSPMV_MAX_EXPERTS], group_sum[1024];
   __shared__ int tokens;
   const int tid = threadIdx.x, wide = (a.experts + 31) / 32 * 32, groups = 1024 / wide, group = tid / wide, e = tid % wide;
   pdl_wait();
   if (tid < 32) {
     int n = 0;
-    for (int p = tid; p < ctas; p += 32) n += a.part_tokens[p];
+    for (int p = tid; p < clusters; p += 32) n += a.part_tokens[p];
     n = __reduce_add_sync(0xffffffffu, n);
     if (tid == 0) tokens = n;
   }
   float sum = 0.f;
   if (e < a.experts && group < groups)
 #pragma unroll 8
-    for (int p = group; p < ctas; p += groups) sum += a.parts[(size_t)p * a.experts + e];
+    for (int p = group; p < clusters; p += groups) sum += a.parts[(size_t)p * a.experts + e];
   group_sum[tid] = sum;
   __syncthreads();
   if (tid < a.experts) {
@@ -583,39 +611,36 @@ __global__ void __launch_bounds__(256) balance_backward_kernel(BalanceGradArgs a
   const int there = *a.there;
   const float scale = *a.dloss * (float)a.experts / ((float)(pairs > 0 ? pairs : 1) * (float)(there > 0 ? there : 1));
   const T* const logits = static_cast<const T*>(a.logits);
+  // one token at a time: with two (us, 32 771 tokens of 256 experts) 20.4 for 15.0
   const long long step = (long long)gridDim.x * 8;
   LanePart<T, V, W> next;
+  struct Choice { int id; float w, g; } next_choice;          // a lane's choice of a token
+  const auto load = [&](long long t) {
+    next_choice = {-1, 0.f, 0.f};
+    next.load(logits + t * a.stride, a.experts, lane);
+    if (a.dweights && lane < a.k) {
+      const long long p = t * a.k + lane;
+      next_choice = {a.ids[p], a.weights[p], a.dweights[p]};
+    }
+  };
   next.clear();
   long long t = (long long)blockIdx.x * 8 + warp;
-  if (t < a.tokens) next.load(logits + t * a.stride, a.experts, lane);
+  if (t < a.tokens) load(t);
   for (; t < a.tokens; t += step) {
     const LanePart<T, V, W> part = next;
-    if (t + step < a.tokens) next.load(logits + (t + step) * a.stride, a.experts, lane);
-    int id = -1;
-    float w = 0.f, g = 0.f, chosen_logit = 0.f, chosen_count = 0.f;
-    if (a.dweights && lane < a.k) {
-      id = a.ids[t * a.k + lane];
-      if (id < 0 || id >= a.experts) id = -1;          // not an expert of these logits: no choice
-      else {
-        w = a.weights[t * a.k + lane];
-        g = a.dweights[t * a.k + lane];
-        chosen_logit = to_float(logits[t * a.stride + id]);
-        chosen_count = (float)a.counts[id];
-      }
-    }
-    float e[V], base, factor, mean = w * g, expected = 0.f;
-    softmax_of<T, V, W>(part, true, e, base, factor);
+    Choice c = next_choice;
+    float chosen = 0.f;
+    if ((unsigned)c.id >= (unsigned)a.experts) c = {-1, 0.f, 0.f};          // not an expert of these logits: no choice
+    else chosen = to_float(logits[t * a.stride + c.id]);
+    if (t + step < a.tokens) load(t + step);
+    float e[V], base, factor, sums[2] = {c.w * c.g, 0.f};
+    softmax_of<T, V, W>(part, true, e, base, factor, sums, [&] {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      e[i] *= factor;
-      expected = fmaf(e[i], count[i], expected);
-    }
+      for (int i = 0; i < V; ++i) sums[1] = fmaf(e[i], count[i], sums[1]);
+    });
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      mean += __shfl_xor_sync(0xffffffffu, mean, o);
-      expected += __shfl_xor_sync(0xffffffffu, expected, o);
-    }
-    const float common = a.renormalize ? 0.f : mean;
+    for (int i = 0; i < V; ++i) e[i] *= factor;
+    const float mean = sums[0], expected = sums[1] * factor, common = a.renormalize ? 0.f : mean;
     T* const out = static_cast<T*>(a.dlogits) + t * a.experts;
 #pragma unroll
     for (int i = 0; i < V / W; ++i) {
@@ -626,9 +651,9 @@ __global__ void __launch_bounds__(256) balance_backward_kernel(BalanceGradArgs a
       if (first < a.experts) r.store(out + first);
     }
     __syncwarp();
-    if (id >= 0) {
-      const float p = exp_below_exact(chosen_logit, base) * factor;
-      out[id] = from_float<T>(fmaf(p, scale * (chosen_count - expected) - common, a.renormalize ? w * (g - mean) : w * g));
+    if (c.id >= 0) {
+      const float p = exp_below_exact(chosen, base) * factor, n = (float)a.counts[c.id];
+      out[c.id] = from_float<T>(fmaf(p, scale * (n - expected) - common, a.renormalize ? c.w * (c.g - mean) : c.w * c.g));
     }
     __syncwarp();
   }
@@ -801,22 +826,33 @@ static int route_typed(const RouteArgs& a, cudaStream_t st) {
   return route_width<T, 32, 256>(a, st);
 }
 
-// CTAs of the balance loss: a token a warp up to one CTA an SM.
+// Clusters of the balance loss: a few tokens a warp, up to one CTA an SM.
 constexpr long long kBalanceSmall = 64;      // tokens up to which one CTA does it all
-static int balance_ctas(long long tokens) {
-  const long long want = (tokens + 15) / 16;
-  const int sms = device_sm_count();
-  return (int)(want < 1 ? 1 : want > sms ? sms : want);
+static int balance_clusters(long long tokens) {
+  const long long want = (tokens + 63) / 64;
+  const int most = device_sm_count() / kBalanceCtas;
+  return (int)(want < 1 ? 1 : want > most ? most : want);
 }
 
 template <class T, int V, int W>
 static int balance_launch(const BalanceArgs& a, cudaStream_t st) {
-  constexpr int kThreads = V <= 12 ? 512 : 256;          // 32 KB for the warps' sums at the most
+  constexpr int kThreads = V <= 8 ? 1024 : V <= 16 ? 512 : 256;          // 32 KB for the warps' sums at the most
   const size_t smem = (size_t)a.experts * (kThreads / 32) * 4;
-  if (a.tokens <= kBalanceSmall) return launch_pdl(balance_kernel<T, V, W, kThreads, true>, 1, kThreads, smem, st, a);
-  const int ctas = balance_ctas(a.tokens);
-  if (int e = launch_pdl(balance_kernel<T, V, W, kThreads, false>, ctas, kThreads, smem, st, a)) return e;
-  return launch_pdl(balance_end_kernel, 1, 1024, 0, st, a, ctas);
+  if (a.tokens <= kBalanceSmall) {
+    constexpr int kFew = V <= 12 ? 512 : 256;
+    return launch_pdl(balance_kernel<T, V, W, kFew, true>, 1, kFew, (size_t)a.experts * (kFew / 32) * 4, st, a);
+  }
+  const int clusters = balance_clusters(a.tokens);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(clusters * kBalanceCtas)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kBalanceCtas; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  if (int e = (int)cudaLaunchKernelEx(&cfg, balance_kernel<T, V, W, kThreads, false>, a)) return e;
+  return launch_pdl(balance_end_kernel, 1, 1024, 0, st, a, clusters);
 }
 template <class T, int V, int W>
 static int balance_launch(const BalanceGradArgs& a, cudaStream_t st) {
@@ -961,7 +997,7 @@ static int check_balance(const flexspmv_expert_desc* d) {
 int flexspmv_balance_loss_bytes(const flexspmv_expert_desc* d, size_t* bytes) {
   if (!d || !bytes || d->tokens < 0 || d->experts < 1) return FLEXSPMV_ERR_BAD_ARG;
   if (d->experts > FLEXSPMV_MAX_EXPERTS) return FLEXSPMV_ERR_TOO_LARGE;
-  *bytes = (size_t)flex::balance_ctas(d->tokens) * (d->experts + 1) * 4;
+  *bytes = (size_t)flex::balance_clusters(d->tokens) * (d->experts + 1) * 4;
   return 0;
 }
 
@@ -979,7 +1015,7 @@ int flexspmv_balance_loss(const flexspmv_expert_desc* d, const void* const* in, 
     return FLEXSPMV_ERR_BAD_ARG;
   float* const parts = static_cast<float*>(ws);
   const flex::BalanceArgs a = {in[0], static_cast<const int*>(in[1]), d->tokens, d->in_stride, d->experts, parts,
-                               reinterpret_cast<int*>(parts + (size_t)flex::balance_ctas(d->tokens) * d->experts), static_cast<float*>(out[0]),
+                               reinterpret_cast<int*>(parts + (size_t)flex::balance_clusters(d->tokens) * d->experts), static_cast<float*>(out[0]),
                                static_cast<float*>(out[2]), static_cast<int*>(out[1]), static_cast<int*>(out[3])};
   return flex::balance_call(a, d->type, flex::aligned16(in[0]), static_cast<cudaStream_t>(stream));
 }
