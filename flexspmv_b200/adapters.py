@@ -110,12 +110,12 @@ def project(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: torch.Ten
     at[5] = plan.data.data_ptr()
     stride = _rows_of(x, "x")
     if out is None:
-        out = torch.empty((tokens, n), dtype=x.dtype, device=x.device)
+        out = x.new_empty((tokens, n))
     else:
         out = _out(out, (tokens, n), x.dtype, x.device, x=x, weight=weight, a=a, b=b, scale=scale, plan=plan.data)
     d = Desc(tokens, stride, adapters, rank, n, k, _TYPE[x.dtype])
     need = _project_bytes(tokens, rank)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    ws = x.new_empty(need, dtype=torch.uint8)
     ins = (_P * 6)(*at)
     outs = (_P * 1)(out.data_ptr())
     flag = _flag(dev)

@@ -114,8 +114,8 @@ __device__ __forceinline__ Two fma(const Two& x, const Two& y, const Two& z) {
 
 // ---- rows ----------------------------------------------------------------------------------------------------------
 
-// C neighbouring values of a row as they are, in one access (WIDE: all of them exist or none) or one by one.
-template <class T, int C, bool WIDE>
+// C values of a row as they are: neighbouring ones in one access (WIDE: all of them exist or none), or one by one, S columns apart.
+template <class T, int C, bool WIDE, int S = 1>
 struct Values {
   Pack<T, C> q;
   __device__ __forceinline__ void load(const T* row, int c, int width) {
@@ -124,7 +124,7 @@ struct Values {
       else q.zero();
     } else {
 #pragma unroll
-      for (int j = 0; j < C; ++j) q.v[j] = c + j < width ? row[c + j] : from_float<T>(0.f);
+      for (int j = 0; j < C; ++j) q.v[j] = c + j * S < width ? row[c + j * S] : from_float<T>(0.f);
     }
   }
   __device__ __forceinline__ void get(float (&v)[C]) const {
@@ -132,13 +132,13 @@ struct Values {
     for (int j = 0; j < C; ++j) v[j] = q.get(j);
   }
 };
-template <class T, int C, bool WIDE>
+template <class T, int C, bool WIDE, int S = 1>
 __device__ __forceinline__ void load_values(const T* row, int c, int width, float (&v)[C]) {
-  Values<T, C, WIDE> q;
+  Values<T, C, WIDE, S> q;
   q.load(row, c, width);
   q.get(v);
 }
-template <class T, int C, bool WIDE>
+template <class T, int C, bool WIDE, int S = 1>
 __device__ __forceinline__ void store_values(T* row, int c, int width, const float (&v)[C]) {
   if constexpr (WIDE && sizeof(T) == 2) {          // rounded by two: an instruction, and none to put them together
     static_assert(C % 8 == 0, "16 bytes");
@@ -155,21 +155,27 @@ __device__ __forceinline__ void store_values(T* row, int c, int width, const flo
   } else {
 #pragma unroll
     for (int j = 0; j < C; ++j)
-      if (c + j < width) row[c + j] = from_float<T>(v[j]);
+      if (c + j * S < width) row[c + j * S] = from_float<T>(v[j]);
   }
 }
 // Weights are 32-bit or of the rows' type; none: `value`.
-template <class T, int C, bool WIDE>
+template <class T, int C, bool WIDE, int S = 1>
 __device__ __forceinline__ void load_params(const void* p, bool wide_type, int c, int width, float value, float (&v)[C]) {
   if (!p) {
 #pragma unroll
     for (int j = 0; j < C; ++j) v[j] = value;
   } else if (std::is_same<T, float>::value || wide_type) {
-    load_values<float, C, WIDE>(static_cast<const float*>(p), c, width, v);
+    load_values<float, C, WIDE, S>(static_cast<const float*>(p), c, width, v);
   } else {
-    load_values<T, C, WIDE>(static_cast<const T*>(p), c, width, v);
+    load_values<T, C, WIDE, S>(static_cast<const T*>(p), c, width, v);
   }
 }
+
+// The columns of a thread that shares a row with TPR - 1 others: V times C of them.  Rows that are not WIDE are accessed value by value, neighbouring threads on
+// neighbouring values, but for those that are dropped by four.
+constexpr int apart_by(bool wide, bool drop, int tpr) { return wide || drop ? 1 : tpr; }
+template <int C, int S, int TPR>
+__device__ __forceinline__ int first_column(int i, int at) { return S > 1 ? i * C * TPR + at : (i * TPR + at) * C; }
 
 // Sums over the TPR threads of a row, the same bits in all of them; `group`: which of the CTA's rows.  `buf` (of the group) alternates between two halves,
 // so that a barrier lies between a half's reading and its next writing.
@@ -218,16 +224,20 @@ __device__ __forceinline__ float inverse_root(float x) {
 
 // ---- rows ahead ----------------------------------------------------------------------------------------------------
 
-// Many rows of 16-byte pieces: one CTA an SM, its THREADS in groups of TPR, a row each.  A thread's pieces of the rows to come are copied to shared memory, to
+// Many rows: one CTA an SM, its THREADS in groups of TPR, a row each.  A thread's pieces of the rows to come are copied to shared memory, to
 // places of its own, so that no register holds them and no barrier is needed for them; PARAMS of weight and bias lie there in 32 bits, which all groups
 // share.  What it is for is bytes on their way: us, 16384 rows of 4096 in 16 bits with dropout and sum, loads of each row by itself 131.
 constexpr int kSmemAnSm = 226 * 1024;
-template <class T, int C, int L, int TPR, int THREADS, int ARRAYS, int PARAMS>
+// `bytes`: 4, or 0 for zeros.
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(bytes));
+}
+template <class T, int C, bool WIDE, int S, int L, int TPR, int THREADS, int ARRAYS, int PARAMS>
 struct Ahead {
   static constexpr int kGroups = THREADS / TPR, kPieces = L * (int)sizeof(T) / 16, kEach = 16 / (int)sizeof(T);
   static constexpr int kStageBytes = ARRAYS * kPieces * THREADS * 16, kParamBytes = PARAMS * L * TPR * 4;
   static constexpr int kRoom = (kSmemAnSm - kParamBytes - 2048) / kStageBytes, kStages = kRoom > 4 ? 4 : kRoom;
-  static constexpr bool kFits = kStages >= 2;
+  static constexpr bool kFits = kStages >= 2 && (WIDE || sizeof(T) == 4);          // a copy takes 4 bytes at the least
   static constexpr int kBytes = kParamBytes + kStages * kStageBytes;
   uint32_t params, rows;
   int stage = 0;
@@ -238,8 +248,13 @@ struct Ahead {
   __device__ __forceinline__ void copy(int stage, int array, const T* row, int at, int width) const {
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
-      const int c = (p * TPR + at) * kEach;
-      copy16(place(stage, array, p), c < width ? row + c : row, c < width ? 16 : 0);
+      const int c = first_column<C, S, TPR>(p, at);
+      if constexpr (WIDE) {
+        copy16(place(stage, array, p), c < width ? row + c : row, c < width ? 16 : 0);
+      } else {
+#pragma unroll
+        for (int j = 0; j < C; ++j) copy4(place(stage, array, p) + j * 4, c + j * S < width ? row + c + j * S : row, c + j * S < width ? 4 : 0);
+      }
     }
   }
   // Where the row kStages - 1 ahead goes: it has been read.
@@ -247,7 +262,7 @@ struct Ahead {
   static __device__ __forceinline__ void done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
   static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory"); }
   template <int V>
-  __device__ __forceinline__ void take(int array, Values<T, C, true> (&v)[V]) const {
+  __device__ __forceinline__ void take(int array, Values<T, C, WIDE, S> (&v)[V]) const {
     static_assert(C == kEach, "a piece each");
 #pragma unroll
     for (int p = 0; p < V; ++p) {
@@ -293,7 +308,7 @@ struct NormArgs {
 constexpr int kAheadThreads = 1024;
 template <class T, int C, bool WIDE, int L, int TPR, bool DROP, int AHEAD>
 __global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEAD ? 1 : 1024 / row_threads(TPR)) layer_norm_kernel(NormArgs a) {
-  constexpr int V = L / C, kThreads = AHEAD ? kAheadThreads : row_threads(TPR), kRows = kThreads / TPR;
+  constexpr int S = apart_by(WIDE, DROP, TPR), V = L / C, kThreads = AHEAD ? kAheadThreads : row_threads(TPR), kRows = kThreads / TPR;
   extern __shared__ __align__(16) unsigned char rows_sm[];
   __shared__ __align__(16) float buf[kRows][2][1][32];
   const int at = threadIdx.x % TPR, group = threadIdx.x / TPR;
@@ -302,7 +317,7 @@ __global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEA
   const Random random(a.seed, DROP);
   const float inverse = 1.f / (float)a.width;
   const long long step = (long long)gridDim.x * kRows, from = (long long)blockIdx.x * kRows + group;
-  Ahead<T, C, L, TPR, kThreads, AHEAD ? AHEAD : 1, 2> next(rows_sm);
+  Ahead<T, C, WIDE, S, L, TPR, kThreads, AHEAD ? AHEAD : 1, 2> next(rows_sm);
   const T *next_x = static_cast<const T*>(a.x) + from * a.x_stride, *next_t = static_cast<const T*>(a.residual) + from * a.residual_stride;
   long long ahead = from;
   const auto copy_next = [&](int to) {
@@ -321,16 +336,16 @@ __global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEA
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float p[C];
-        load_params<T, C, WIDE>(a.weight, a.wide_params, (i * TPR + at) * C, a.width, 1.f, p);
+        load_params<T, C, WIDE, S>(a.weight, a.wide_params, first_column<C, S, TPR>(i, at), a.width, 1.f, p);
         next.put_params(0, i, at, p);
-        load_params<T, C, WIDE>(a.bias, a.wide_params, (i * TPR + at) * C, a.width, 0.f, p);
+        load_params<T, C, WIDE, S>(a.bias, a.wide_params, first_column<C, S, TPR>(i, at), a.width, 0.f, p);
         next.put_params(1, i, at, p);
       }
     __syncthreads();
   }
   for (long long r = from; r < a.rows; r += step) {
     float s[V][C];
-    Values<T, C, WIDE> x[V], t[V];
+    Values<T, C, WIDE, S> x[V], t[V];
     const bool sum = AHEAD ? AHEAD == 2 : a.residual != nullptr;
     if constexpr (AHEAD > 0) {
       copy_next(next.last());
@@ -340,10 +355,10 @@ __global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEA
       next.next();
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) x[i].load(static_cast<const T*>(a.x) + r * a.x_stride, (i * TPR + at) * C, a.width);
+      for (int i = 0; i < V; ++i) x[i].load(static_cast<const T*>(a.x) + r * a.x_stride, first_column<C, S, TPR>(i, at), a.width);
       if (sum)
 #pragma unroll
-        for (int i = 0; i < V; ++i) t[i].load(static_cast<const T*>(a.residual) + r * a.residual_stride, (i * TPR + at) * C, a.width);
+        for (int i = 0; i < V; ++i) t[i].load(static_cast<const T*>(a.residual) + r * a.residual_stride, first_column<C, S, TPR>(i, at), a.width);
     }
     if (!sum)
 #pragma unroll
@@ -351,7 +366,7 @@ __global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEA
     Two two(0.f);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int c = (i * TPR + at) * C;
+      const int c = first_column<C, S, TPR>(i, at);
       float v[C];
       x[i].get(v);
       t[i].get(s[i]);
@@ -361,7 +376,7 @@ __global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEA
 #pragma unroll
         for (int j = 0; j < C; j += 2) (Two(s[i] + j) + Two(v + j)).put(s[i] + j);
       }
-      if (DROP || sum) store_values<T, C, WIDE>(static_cast<T*>(a.sum) + r * a.width, c, a.sum ? a.width : 0, s[i]);
+      if (DROP || sum) store_values<T, C, WIDE, S>(static_cast<T*>(a.sum) + r * a.width, c, a.sum ? a.width : 0, s[i]);
 #pragma unroll
       for (int j = 0; j < C; j += 2) two = two + Two(s[i] + j);          // beyond the width: zeros
     }
@@ -371,13 +386,13 @@ __global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEA
     two = Two(0.f);
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if ((i * TPR + at) * C < a.width)
+      if (first_column<C, S, TPR>(i, at) < a.width)
 #pragma unroll
         for (int j = 0; j < C; j += 2) {
           Two d = Two(s[i] + j) + Two(-mean);
           d.put(s[i] + j);
-          if (!WIDE && (i * TPR + at) * C + j >= a.width) d.a = 0.f;
-          if (!WIDE && (i * TPR + at) * C + j + 1 >= a.width) d.b = 0.f;
+          if (!WIDE && first_column<C, S, TPR>(i, at) + j * S >= a.width) d.a = 0.f;
+          if (!WIDE && first_column<C, S, TPR>(i, at) + (j + 1) * S >= a.width) d.b = 0.f;
           two = fma(d, d, two);
         }
     total[0] = two.a + two.b;
@@ -390,17 +405,17 @@ __global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEA
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float w[C], b[C];
-      const int c = (i * TPR + at) * C;
+      const int c = first_column<C, S, TPR>(i, at);
       if constexpr (AHEAD > 0) {
         next.get_params(0, i, at, w);
         next.get_params(1, i, at, b);
       } else {
-        load_params<T, C, WIDE>(a.weight, a.wide_params, c, a.width, 1.f, w);
-        load_params<T, C, WIDE>(a.bias, a.wide_params, c, a.width, 0.f, b);
+        load_params<T, C, WIDE, S>(a.weight, a.wide_params, c, a.width, 1.f, w);
+        load_params<T, C, WIDE, S>(a.bias, a.wide_params, c, a.width, 0.f, b);
       }
 #pragma unroll
       for (int j = 0; j < C; j += 2) fma(Two(s[i] + j) * Two(rstd), Two(w + j), Two(b + j)).put(s[i] + j);
-      store_values<T, C, WIDE>(static_cast<T*>(a.y) + r * a.width, c, a.width, s[i]);
+      store_values<T, C, WIDE, S>(static_cast<T*>(a.y) + r * a.width, c, a.width, s[i]);
     }
   }
 }
@@ -488,7 +503,7 @@ constexpr int norm_grad_threads(int l) { return l == 8 ? 768 : 512; }          /
 template <class T, int C, bool WIDE, int L, int TPR, bool DROP, bool AHEAD>
 __global__ void __launch_bounds__(AHEAD ? kAheadGradThreads : row_threads(TPR), AHEAD ? 1 : norm_grad_threads(L) / row_threads(TPR))
     layer_norm_backward_kernel(NormGradArgs a) {
-  constexpr int V = L / C, kThreads = AHEAD ? kAheadGradThreads : row_threads(TPR), kRows = kThreads / TPR;
+  constexpr int S = apart_by(WIDE, DROP, TPR), V = L / C, kThreads = AHEAD ? kAheadGradThreads : row_threads(TPR), kRows = kThreads / TPR;
   extern __shared__ __align__(16) unsigned char rows_sm[];
   __shared__ __align__(16) float buf[kRows][2][2][32];
   const int at = threadIdx.x % TPR, group = threadIdx.x / TPR;
@@ -502,7 +517,7 @@ __global__ void __launch_bounds__(AHEAD ? kAheadGradThreads : row_threads(TPR), 
   const Random random(a.seed, DROP);
   const float inverse = 1.f / (float)a.width;
   const long long step = (long long)gridDim.x * kRows, from = (long long)blockIdx.x * kRows + group;
-  Ahead<T, C, L, TPR, kThreads, 3, 1> next(rows_sm);
+  Ahead<T, C, WIDE, S, L, TPR, kThreads, 3, 1> next(rows_sm);
   const T *next_x = static_cast<const T*>(a.x) + from * a.x_stride, *next_y = static_cast<const T*>(a.dy) + from * a.dy_stride,
           *next_d = static_cast<const T*>(a.dsum) + from * a.dsum_stride;
   long long ahead = from;
@@ -529,7 +544,7 @@ __global__ void __launch_bounds__(AHEAD ? kAheadGradThreads : row_threads(TPR), 
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float p[C];
-        load_params<T, C, WIDE>(a.weight, a.wide_params, (i * TPR + at) * C, a.width, 1.f, p);
+        load_params<T, C, WIDE, S>(a.weight, a.wide_params, first_column<C, S, TPR>(i, at), a.width, 1.f, p);
         next.put_params(0, i, at, p);
       }
     __syncthreads();
@@ -541,7 +556,7 @@ __global__ void __launch_bounds__(AHEAD ? kAheadGradThreads : row_threads(TPR), 
       next_rstd = a.rstd[r + step];
     }
     float n[V][C], g[V][C];
-    Values<T, C, WIDE> x[V], dy[V], d[V];
+    Values<T, C, WIDE, S> x[V], dy[V], d[V];
     if constexpr (AHEAD) {
       copy_next(next.last());
       next.wait();
@@ -550,19 +565,19 @@ __global__ void __launch_bounds__(AHEAD ? kAheadGradThreads : row_threads(TPR), 
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        x[i].load(static_cast<const T*>(a.x) + r * a.x_stride, (i * TPR + at) * C, a.width);
-        dy[i].load(static_cast<const T*>(a.dy) + r * a.dy_stride, (i * TPR + at) * C, a.width);
+        x[i].load(static_cast<const T*>(a.x) + r * a.x_stride, first_column<C, S, TPR>(i, at), a.width);
+        dy[i].load(static_cast<const T*>(a.dy) + r * a.dy_stride, first_column<C, S, TPR>(i, at), a.width);
       }
       if (a.dsum)
 #pragma unroll
-        for (int i = 0; i < V; ++i) d[i].load(static_cast<const T*>(a.dsum) + r * a.dsum_stride, (i * TPR + at) * C, a.width);
+        for (int i = 0; i < V; ++i) d[i].load(static_cast<const T*>(a.dsum) + r * a.dsum_stride, first_column<C, S, TPR>(i, at), a.width);
     }
     Two one(0.f), two(0.f);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float w[C];
       if constexpr (AHEAD) next.get_params(0, i, at, w);
-      else load_params<T, C, WIDE>(a.weight, a.wide_params, (i * TPR + at) * C, a.width, 1.f, w);
+      else load_params<T, C, WIDE, S>(a.weight, a.wide_params, first_column<C, S, TPR>(i, at), a.width, 1.f, w);
       x[i].get(n[i]);
       dy[i].get(g[i]);
 #pragma unroll
@@ -588,15 +603,15 @@ __global__ void __launch_bounds__(AHEAD ? kAheadGradThreads : row_threads(TPR), 
       for (int i = 0; i < V; ++i) d[i].q.zero();
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int c = (i * TPR + at) * C;
+      const int c = first_column<C, S, TPR>(i, at);
       float added[C];
       d[i].get(added);
 #pragma unroll
       for (int j = 0; j < C; j += 2) (fma(Two(n[i] + j), Two(second), fma(Two(g[i] + j), Two(rstd), Two(first))) + Two(added + j)).put(g[i] + j);
-      store_values<T, C, WIDE>(static_cast<T*>(a.dresidual) + r * a.width, c, a.width, g[i]);
+      store_values<T, C, WIDE, S>(static_cast<T*>(a.dresidual) + r * a.width, c, a.width, g[i]);
       if (DROP) {
         random.drop(g[i], c, (uint32_t)r, a.below, a.scale);
-        store_values<T, C, WIDE>(static_cast<T*>(a.dx) + r * a.width, c, a.width, g[i]);
+        store_values<T, C, WIDE, S>(static_cast<T*>(a.dx) + r * a.width, c, a.width, g[i]);
       }
     }
   }
@@ -612,7 +627,7 @@ __global__ void __launch_bounds__(AHEAD ? kAheadGradThreads : row_threads(TPR), 
         for (int i = 0; i < V; ++i)
 #pragma unroll
           for (int j = 0; j < C; ++j) {
-            const int c = (i * TPR + at) * C + j;
+            const int c = first_column<C, S, TPR>(i, at) + j * S;
             joined[c] = w ? joined[c] + dw[i][j] : dw[i][j];
             joined[L * TPR + c] = w ? joined[L * TPR + c] + db[i][j] : db[i][j];
           }
@@ -627,7 +642,7 @@ __global__ void __launch_bounds__(AHEAD ? kAheadGradThreads : row_threads(TPR), 
     for (int i = 0; i < V; ++i)
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        const int c = (i * TPR + at) * C + j;
+        const int c = first_column<C, S, TPR>(i, at) + j * S;
         if (c < a.width) {
           mine[c] = dw[i][j];
           mine[a.width + c] = db[i][j];
@@ -807,18 +822,15 @@ static bool many_rows(long long rows, int groups) { return rows >= 2ll * groups 
 
 template <class T, int C, bool WIDE, int L, int TPR, bool DROP>
 static int norm_launch(const NormArgs& a, cudaStream_t st) {
+  constexpr int S = apart_by(WIDE, DROP, TPR);
   const auto ahead = [&](auto arrays) {
-    using Next = Ahead<T, C, L, TPR, kAheadThreads, decltype(arrays)::value, 2>;
+    using Next = Ahead<T, C, WIDE, S, L, TPR, kAheadThreads, decltype(arrays)::value, 2>;
     constexpr auto kernel = layer_norm_kernel<T, C, WIDE, L, TPR, DROP, decltype(arrays)::value>;
     if (int e = allow_smem<kernel>(Next::kBytes)) return e;
     return launch_pdl(kernel, row_grid(a.rows, Next::kGroups, device_sm_count()), kAheadThreads, Next::kBytes, st, a);
   };
-  if constexpr (WIDE) {
-    if (many_rows(a.rows, kAheadThreads / TPR)) {
-      if constexpr (Ahead<T, C, L, TPR, kAheadThreads, 2, 2>::kFits)
-        return a.residual ? ahead(std::integral_constant<int, 2>()) : ahead(std::integral_constant<int, 1>());
-    }
-  }
+  if constexpr (Ahead<T, C, WIDE, S, L, TPR, kAheadThreads, 2, 2>::kFits)
+    if (many_rows(a.rows, kAheadThreads / TPR)) return a.residual ? ahead(std::integral_constant<int, 2>()) : ahead(std::integral_constant<int, 1>());
   constexpr int kThreads = row_threads(TPR);
   return launch_pdl(layer_norm_kernel<T, C, WIDE, L, TPR, DROP, 0>, row_grid(a.rows, kThreads / TPR, device_sm_count() * (1024ll / kThreads)), kThreads, 0, st, a);
 }
@@ -852,9 +864,9 @@ static int norm_grad_ctas(long long rows, int width) {
 
 template <class T, int C, bool WIDE, int L, int TPR, bool DROP>
 static int norm_grad_launch(const NormGradArgs& a, int& ctas, cudaStream_t st) {
-  if constexpr (WIDE) {
-    using Next = Ahead<T, C, L, TPR, kAheadGradThreads, 3, 1>;
-    static_assert(Next::kFits && Next::kBytes >= 8 * L * TPR, "stages, and the groups' sums over them");
+  using Next = Ahead<T, C, WIDE, apart_by(WIDE, DROP, TPR), L, TPR, kAheadGradThreads, 3, 1>;
+  if constexpr (Next::kFits) {
+    static_assert(Next::kBytes >= 8 * L * TPR, "the groups' sums lie over the stages");
     if (many_rows(a.rows, Next::kGroups)) {
       constexpr auto kernel = layer_norm_backward_kernel<T, C, WIDE, L, TPR, DROP, true>;
       if (int e = allow_smem<kernel>(Next::kBytes)) return e;

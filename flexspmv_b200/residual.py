@@ -121,9 +121,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     kind, p, eps = _params(weight, bias, x, width, dev), _drops(p, seed, dev), float(eps)
     if not eps >= 0.0:
         raise FlexSpmvError(f"eps must not be negative or NaN: {eps}")
-    y = torch.empty((rows, width), dtype=x.dtype, device=x.device)
+    y = x.new_empty((rows, width))
     total = torch.empty_like(y) if residual is not None or p > 0.0 else None
-    out = Normed(y, total, *torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind())
+    mean = x.new_empty(rows, dtype=torch.float32)
+    out = Normed(y, total, mean, torch.empty_like(mean))
     d = Desc(rows, width, (xs, rs, 0), _TYPE[x.dtype], kind, eps, 0, p)
     ins, outs = _at(x, residual, weight, bias, seed if p > 0.0 else None), _at(y, total, out.mean, out.rstd)
     return BoundCall(_function("layer_norm", _PLAIN), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs)), dev,
@@ -151,14 +152,14 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
     kind, p = _params(weight, None, dy, width, dev), _drops(p, seed, dev)
     _vector(mean, "mean", (torch.float32,), rows, dev, "row")
     _vector(rstd, "rstd", (torch.float32,), rows, dev, "row")
-    dresidual = torch.empty((rows, width), dtype=dy.dtype, device=dy.device)
+    dresidual = dy.new_empty((rows, width))
     dx = torch.empty_like(dresidual) if p > 0.0 else dresidual
     dweight = dbias = ws = None
     need = 0
     if weight is not None:
-        dweight, dbias = torch.empty((2, width), dtype=weight.dtype, device=weight.device).unbind()
+        dweight, dbias = torch.empty_like(weight), torch.empty_like(weight)
         need = _backward_bytes(rows, width, dev)
-        ws = torch.empty(need, dtype=torch.uint8, device=dy.device)
+        ws = dy.new_empty(need, dtype=torch.uint8)
     out = NormGradients(dx, dresidual, dweight, dbias)
     d = Desc(rows, width, (ys, xs, ds), _TYPE[dy.dtype], kind, 0.0, 0, p)
     ins, outs = _at(dy, x, weight, mean, rstd, dsum, seed if p > 0.0 else None), _at(dx if p > 0.0 else None, dresidual, dweight, dbias)
@@ -177,7 +178,7 @@ def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, residual: Optional[to
     if p == 0.0:
         _drops(0.5, seed, dev)               # the seed is not used, but is one
     if out is None:
-        out = torch.empty((rows, width), dtype=x.dtype, device=x.device)
+        out = x.new_empty((rows, width))
     else:
         out = _out(out, (rows, width), x.dtype, x.device, x=x, residual=residual, seed=seed)
     d = Desc(rows, width, (xs, rs, 0), _TYPE[x.dtype], 0, 0.0, 0, p)
