@@ -24,8 +24,9 @@ struct AdapterTile {
 constexpr int kLowTile = 16;
 constexpr long long kOneGroup = 1024;        // tokens up to which they are one group
 constexpr long long kLowTiles = 4096;        // tokens up to which the first product may be in tiles
-// ... and is: as many as its CTAs read x again for every 16 of the rank.
-static bool low_in_tiles(long long tokens, int rank) { return tokens * ((rank + 15) / 16) <= kLowTiles; }
+// ... and is: an adapter is read again for every 16 tokens.  us, both products, tiles / the grouped kernel: 600 tokens of rank 128 (50 adapters, 2000 x 2000) 55.2 / 44.9,
+// 2000 of rank 64 60.1 / 45.3; 1500 of rank 16 34.9, 300 of rank 64 (4096 x 1000) 22.3 in tiles.
+static bool low_in_tiles(long long tokens, int rank) { return tokens <= kLowTiles && tokens * rank <= 32768; }
 constexpr int kLongRun = 128;
 struct AdapterPlan {
   long long ids, rows, tiles, offsets, groups, group_adapters, runs, ints;
@@ -215,71 +216,82 @@ struct LowArgs {
   int rank, k, width;
 };
 
-// low[t] = scale A x[t] of few tokens: a cluster of four CTAs takes a tile of up to 16 tokens of one adapter and 16 values of the rank (blockIdx.y), their warps every 32nd 32 of
-// the sum, so that a long one is one round of loads; the warps' and the CTAs' sums meet in shared memory in their order.  Bound by the latency of reading the adapter, not
-// by arithmetic, so the warp's own matrix instruction is enough and its operands come from global memory as they are: as the sum's index may be permuted, a lane's share of
-// two instructions is 16 contiguous bytes of a row, and eight rows of 64 bytes are one load of the warp.  Many tokens: grouped_kernel.
-// 256 threads leave room on their SM for a CTA of the product that begins meanwhile.
-constexpr int kLowThreads = 256, kLowCtas = 4, kLowAhead = 4;          // loads of so many steps under way
-template <class T>
+// low[t] = scale A x[t] of few tokens: a cluster of four CTAs takes a tile of up to 16 tokens of one adapter and 8 NB values of the rank (blockIdx.y), their warps every 32nd 32
+// of the sum, so that a long one is a few rounds of loads; the warps' and the CTAs' sums meet in shared memory in their order.  Bound by the latency of reading the
+// adapter, not by arithmetic, so the warp's own matrix instruction is enough and its operands come from global memory as they are: as the sum's index may be permuted, a
+// lane's share of two instructions is 16 contiguous bytes of a row, and eight rows of 64 bytes are one load of the warp.  Many tokens: grouped_kernel.
+// 256 threads leave room on their SM for a CTA of the product that begins meanwhile (NB = 2).
+constexpr int kLowThreads = 256, kLowCtas = 4;
+template <class T, int NB>
 __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(LowArgs a) {
-  constexpr int kWarps = kLowThreads / 32, kStep = 32 * kWarps * kLowCtas;
-  __shared__ float part[kWarps][16][17], sums[256];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, g = lane >> 2, r0 = blockIdx.y * 16, share = (int)cluster_rank();
+  constexpr int kAhead = NB == 2 ? 4 : 2;          // loads of so many steps under way
+  constexpr int kWarps = kLowThreads / 32, kStep = 32 * kWarps * kLowCtas, kRanks = 8 * NB, kValues = 16 * kRanks;
+  __shared__ float part[kWarps][16][kRanks + 1], sums[kValues];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, g = lane >> 2, r0 = blockIdx.y * kRanks, share = (int)cluster_rank();
   pdl_wait();
   pdl_launch_dependents();
   if ((int)blockIdx.x >= *a.count) return;          // the whole cluster
   const AdapterTile tile = a.tiles[blockIdx.x];
   // rows and ranks that are not there: the first one's, whose results are left out
-  const T *x[2], *down[2];
+  const T *x[2], *down[NB];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int p = i * 8 + g, r = r0 + i * 8 + g;
+    const int p = i * 8 + g;
     x[i] = static_cast<const T*>(a.x) + (long long)a.rows[tile.from + (p < tile.count ? p : 0)] * a.stride;
-    down[i] = static_cast<const T*>(a.down) + ((size_t)tile.adapter * a.rank + (r < a.rank ? r : r0)) * a.k;
   }
-  float acc[2][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) acc[i / 4][i % 4] = 0.f;
+  for (int j = 0; j < NB; ++j) {
+    const int r = r0 + j * 8 + g;
+    down[j] = static_cast<const T*>(a.down) + ((size_t)tile.adapter * a.rank + (r < a.rank ? r : r0)) * a.k;
+  }
+  float acc[NB][4];
+#pragma unroll
+  for (int i = 0; i < 4 * NB; ++i) acc[i / 4][i % 4] = 0.f;
   const bool high = tile.count > 8;          // else the upper rows' loads are left out
-  for (int k0 = (share * kWarps + warp) * 32; k0 < a.k; k0 += kStep * kLowAhead) {
-    uint4 v[kLowAhead][2], w[kLowAhead][2];
+  for (int k0 = (share * kWarps + warp) * 32; k0 < a.k; k0 += kStep * kAhead) {
+    uint4 v[kAhead][2], w[kAhead][NB];
 #pragma unroll
-    for (int u = 0; u < kLowAhead; ++u) {
+    for (int u = 0; u < kAhead; ++u) {
       const int k = k0 + u * kStep + q * 8;
-      v[u][0] = v[u][1] = w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+      v[u][0] = v[u][1] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) w[u][j] = v[u][0];
       if (k < a.k) {
-        w[u][0] = *reinterpret_cast<const uint4*>(down[0] + k);
-        w[u][1] = *reinterpret_cast<const uint4*>(down[1] + k);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) w[u][j] = *reinterpret_cast<const uint4*>(down[j] + k);
         v[u][0] = *reinterpret_cast<const uint4*>(x[0] + k);
         if (high) v[u][1] = *reinterpret_cast<const uint4*>(x[1] + k);
       }
     }
 #pragma unroll
-    for (int u = 0; u < kLowAhead; ++u)
+    for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < NB; ++j) {
         warp_mma<T>(acc[j], v[u][0].x, v[u][1].x, v[u][0].y, v[u][1].y, w[u][j].x, w[u][j].y);
         warp_mma<T>(acc[j], v[u][0].z, v[u][1].z, v[u][0].w, v[u][1].w, w[u][j].z, w[u][j].w);
       }
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < NB; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[warp][g + i / 2 * 8][j * 8 + q * 2 + i % 2] = acc[j][i];
   __syncthreads();
-  const int p = threadIdx.x / 16, r = r0 + threadIdx.x % 16;
-  float h = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) h += part[w][p][threadIdx.x % 16];
-  sums[threadIdx.x] = h;
+  for (int i = threadIdx.x; i < kValues; i += kLowThreads) {
+    float h = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) h += part[w][i / kRanks][i % kRanks];
+    sums[i] = h;
+  }
   cluster_sync();
   // each CTA some of the tokens; 16 of the rank at a time, with zeros: the second product takes as many
-  if (p < tile.count && p % kLowCtas == share) {
-    h = 0.f;
+  for (int i = threadIdx.x; i < kValues / kLowCtas; i += kLowThreads) {
+    const int p = i / kRanks * kLowCtas + share, j = i % kRanks, r = r0 + j;
+    if (p >= tile.count || r >= ((a.rank + 15) & ~15)) continue;
+    float h = 0.f;
     if (r < a.rank) {
 #pragma unroll
-      for (int c = 0; c < kLowCtas; ++c) h += cluster_load(cluster_smem(&sums[threadIdx.x], c));
+      for (int c = 0; c < kLowCtas; ++c) h += cluster_load(cluster_smem(&sums[p * kRanks + j], c));
       if (a.scale) h *= a.scale[tile.adapter];
     }
     T* const row = static_cast<T*>(a.low) + (long long)a.rows[tile.from + p] * a.width;
@@ -303,18 +315,24 @@ static int shared_memory_first() {
   return 0;
 }
 
-template <class T>
-static int low_product(const LowArgs& a, const AdapterPlan& p, cudaStream_t st) {
-  if (int e = shared_memory_first<adapter_low_kernel<T>>()) return e;
+template <class T, int NB>
+static int low_launch(const LowArgs& a, const AdapterPlan& p, cudaStream_t st) {
+  if (int e = shared_memory_first<adapter_low_kernel<T, NB>>()) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.most_tiles, (unsigned)((a.rank + 15) / 16), kLowCtas); cfg.blockDim = dim3(kLowThreads); cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)p.most_tiles, (unsigned)((a.rank + 8 * NB - 1) / (8 * NB)), kLowCtas); cfg.blockDim = dim3(kLowThreads); cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = kLowCtas;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr; cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, adapter_low_kernel<T>, a);
+  return (int)cudaLaunchKernelEx(&cfg, adapter_low_kernel<T, NB>, a);
+}
+template <class T>
+static int low_product(const LowArgs& a, const AdapterPlan& p, cudaStream_t st) {
+  if (a.rank <= 16) return low_launch<T, 2>(a, p, st);
+  if (a.rank <= 32) return low_launch<T, 4>(a, p, st);
+  return low_launch<T, 8>(a, p, st);
 }
 
 // `product`: n, k and the rank count too.

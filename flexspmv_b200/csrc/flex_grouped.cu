@@ -251,28 +251,74 @@ __device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int p
   }
 }
 
-// The same for eight neighbouring features of one place, by one thread.
-template <class T>
-__device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int place, float (&part)[8]) {
-  const int id = a.ids[place];
+// SPLIT: the same for 128 features from m on by places from .. to, into out (128 features a place), by the storing warps, each ROWS features of a place at a time with
+// as many loads under way as there are rows to a lane.  Ranks of 32 and more: four lanes a row, 64 bytes of it at a time.
+template <class T, int ROWS>
+__device__ __forceinline__ void low_rank_rows(const GroupedArgs& a, int m, int from, int to, int warp, int lane, float* out) {
+  constexpr int kParts = 128 / ROWS;
+  for (int unit = warp; unit < (to - from) * kParts; unit += kStoreWarps) {
+    const int p = from + unit / kParts, f0 = unit % kParts * ROWS, id = a.ids[p];
+    float* const to_place = out + (p - from) * 128 + f0;
+    if ((unsigned)id >= (unsigned)a.adapters) {
 #pragma unroll
-  for (int x = 0; x < 8; ++x) part[x] = 0.f;
-  if ((unsigned)id >= (unsigned)a.adapters) return;
-  const T* const up = static_cast<const T*>(a.up) + ((size_t)id * a.n + m) * a.rank;
-  const T* const row = static_cast<const T*>(a.low) + (size_t)place * a.low_width;
-  for (int k = 0; k < a.rank; k += 8) {
-    Pack<T, 8> h, rest, w[8];
-    h.load(row + low_high(k, a.rank));
-    rest.load(row + low_rest(k, a.rank));
+      for (int i = 0; i < ROWS / 32; ++i) to_place[i * 32 + lane] = 0.f;
+      continue;
+    }
+    const T* const row = static_cast<const T*>(a.low) + (size_t)p * a.low_width;
+    const T* const up = static_cast<const T*>(a.up) + ((size_t)id * a.n + m + f0) * a.rank;
+    const int there = a.n - m - f0;          // features that there are; others count as the last of them
+    Pack<T, 8> h, rest;
+    if (a.rank >= 32) {
+      constexpr int kRows = ROWS / 8;
+      float sum[kRows];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) w[x].load(up + (size_t)x * a.rank + k);          // n is a multiple of 8: all eight are there
-    float v[8];
+      for (int i = 0; i < kRows; ++i) sum[i] = 0.f;
+      for (int k = lane % 4 * 8; k < a.rank; k += 32) {
+        Pack<T, 8> w[kRows];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = h.get(i) + rest.get(i);
+        for (int i = 0; i < kRows; ++i) {
+          const int f = i * 8 + lane / 4;
+          w[i].load(up + (size_t)(f < there ? f : there > 0 ? there - 1 : -f0) * a.rank + k);
+        }
+        h.load(row + low_high(k, a.rank));
+        rest.load(row + low_rest(k, a.rank));
+        float v[8];
 #pragma unroll
-    for (int x = 0; x < 8; ++x)
+        for (int x = 0; x < 8; ++x) v[x] = h.get(x) + rest.get(x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) part[x] = fmaf(w[x].get(i), v[i], part[x]);
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+          for (int x = 0; x < 8; ++x) sum[i] = fmaf(w[i].get(x), v[x], sum[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+        if (lane % 4 == 0) to_place[i * 8 + lane / 4] = sum[i];
+      }
+    } else {
+      constexpr int kRows = ROWS / 32;
+      float sum[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) sum[i] = 0.f;
+#pragma unroll 2
+      for (int k = 0; k < a.rank; k += 8) {
+        Pack<T, 8> w[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          const int f = i * 32 + lane;
+          w[i].load(up + (size_t)(f < there ? f : there > 0 ? there - 1 : -f0) * a.rank + k);
+        }
+        h.load(row + low_high(k, a.rank));
+        rest.load(row + low_rest(k, a.rank));
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+          for (int x = 0; x < 8; ++x) sum[i] = fmaf(w[i].get(x), h.get(x) + rest.get(x), sum[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) to_place[i * 32 + lane] = sum[i];
+    }
   }
 }
 
@@ -411,7 +457,6 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   auto step_from = [&](int steps) { return SPLIT ? steps * share / split : 0; };
   auto step_to = [&](int steps) { return SPLIT ? steps * (share + 1) / split : steps; };
 
-  float early[8];                          // kAddLow, SPLIT: what a thread adds to its first item
   if (warp == kCopyWarp) {
     int stage = 0, issued = 0;
     uint32_t phase = 0;
@@ -638,12 +683,16 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
     if (ADAPT == kAddLow) {
       if (SPLIT) prefetch_up<T>(a, share, split, tid);
       pdl_wait();
-      if (SPLIT && first < tiles) {        // while the sum is still under way
+      if (SPLIT && first < tiles) {        // while the sum is still under way; the tiles' store is free
         const GroupedTile t = tile_at<MODE, NT, PAIR, HALVES>(a, table, first);
         const int eights = (t.cols + 7) / 8, c_from = eights * share / split * 8, c_to = eights * (share + 1) / split * 8;
-        const int c = c_from + tid / 16, r = tid % 16 * 8;
-        if (tid < (c_to - c_from) * 16 && c < t.count && t.m0 + r < a.n && group_adapters[t.e] == kGroupMixed)
-          low_rank_part<T>(a, t.m0 + r, t.from + c, early);
+        static_assert(!SPLIT || ADAPT != kAddLow || NT / 2 * 512 <= Cfg::kStoreBytes, "half of a tile's places, the most that a CTA stores");
+        if (group_adapters[t.e] == kGroupMixed) {
+          const int to = c_to < t.count ? c_to : t.count;
+          float* const low = reinterpret_cast<float*>(store);
+          if (c_to - c_from >= kStoreWarps) low_rank_rows<T, 128>(a, t.m0, t.from + c_from, t.from + to, warp, lane, low);
+          else low_rank_rows<T, 32>(a, t.m0, t.from + c_from, t.from + to, warp, lane, low);
+        }
       }
     }
     int acc = 0;
@@ -847,7 +896,6 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   }
   if (SPLIT) {
     // every CTA stores some of the tile's columns, eight neighbouring rows (dw: columns) at a time
-    constexpr int kStoreThreads = ADAPT == kAddLow ? kStoreWarps * 32 : kThreads;
     cluster_sync();
     if (first < tiles && !*abort) {
       const GroupedTile t = tile_at<MODE, NT, PAIR, HALVES>(a, table, first);
@@ -856,7 +904,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
       TO* const out = static_cast<TO*>(a.out);
       constexpr bool kDw = MODE == kGroupedDw;
       const int items = (c_to - c_from) * 16;            // of eight values
-      for (int i = tid; i < items && tid < kStoreThreads; i += kStoreThreads) {
+      for (int i = tid; i < items; i += kThreads) {
         // forward, dx: 16 items a column; dw: 128 items for eight columns
         const int c = kDw ? c_from + i / 128 * 8 : c_from + i / 16, r = kDw ? i % 128 : i % 16 * 8;
         float sum[8];
@@ -876,10 +924,10 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           for (int x = 0; x < 8; ++x) sum[x] += v[x];
         }
         if constexpr (ADAPT == kAddLow)
-          if (group_adapters[t.e] == kGroupMixed && c < t.count && t.m0 + r < a.n) {
-            if (i != tid) low_rank_part<T>(a, t.m0 + r, t.from + c, early);
+          if (group_adapters[t.e] == kGroupMixed && c < t.count) {
+            const float* const low = reinterpret_cast<const float*>(store) + (c - c_from) * 128 + r;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) sum[x] += early[x];
+            for (int x = 0; x < 8; ++x) sum[x] += low[x];
           }
         Pack<TO, 8> q;
 #pragma unroll
@@ -994,7 +1042,8 @@ static int grouped_tiles(const GroupedArgs& a, cudaStream_t st) {
   // What dividing saves is most of a tile's steps, 0.3 us each (a narrow tile's 0.13); what it costs is the parts' meeting, about 5 us (1.5).
   // us, whole / divided: 8 rows, one expert of 2048 x 4096 17.4 / 9.4; dw of 8192 rows, 1024 x 1024 43.8 / 22; but 4096 rows, two experts of
   // 512 x 512 (8 steps) 9.8 / 12.6.
-  if constexpr (ADAPT != kMakeLow) {
+  // kAddLow: only where a CTA's share of a tile's low-rank parts fits beside the stages.
+  if constexpr (ADAPT == kPlain || (ADAPT == kAddLow && NT == 64)) {
     constexpr auto divided = grouped_kernel<T, TO, MODE, NT, 1, 1, true, GATHER, PARTS, ADAPT>;
     const int smem = grouped_smem<MODE, NT, 1, 1, (int)sizeof(TO), ADAPT>(a.experts);
     for (int split = 8; split > 1; split /= 2) {

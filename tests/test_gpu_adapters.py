@@ -64,7 +64,7 @@ def patterns(tokens, count, seed=0):
 @pytest.mark.parametrize("tokens,n,k,count,rank", [
     (1, 8, 8, 1, 8), (1, 4096, 2048, 3, 16), (2, 136, 72, 4, 16), (7, 1000, 1416, 5, 24), (16, 64, 64, 2, 8), (17, 128, 4096, 40, 32), (48, 4096, 4096, 64, 16),
     (48, 520, 264, 64, 40), (64, 256, 512, 9, 64), (65, 1032, 200, 70, 72), (200, 384, 1000, 200, 128), (513, 4096, 256, 30, 8), (1024, 512, 512, 3, 48),
-    (1025, 520, 520, 1024, 16), (1031, 1000, 1416, 96, 8), (2500, 2048, 1024, 20, 64), (5000, 264, 136, 7, 256), (300, 136, 264, 3, 512)])
+    (1025, 520, 520, 1024, 16), (1031, 1000, 1416, 96, 8), (2500, 2048, 1024, 20, 64), (5000, 264, 136, 7, 256), (300, 136, 264, 3, 512), (300, 4096, 4096, 20, 16), (130, 2048, 2048, 40, 32), (150, 1000, 6000, 64, 128)])
 def test_project(tokens, n, k, count, rank, dtype):
     x, w, a, b, scale = operands(tokens, n, k, count, rank, dtype)
     for i, values in enumerate(patterns(tokens, count)):
