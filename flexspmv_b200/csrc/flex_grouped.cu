@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict_
 // workspace and contiguous tile copies 0.44.
 // ADAPT (forward): kAddLow: one matrix for all groups, and each place's adapter's up matrix times its vector of `rank` values.  Groups of one adapter have it as one to
 // a few steps more of their sum; in mixed groups it is added on a place's way out, before the only rounding (low_rank_part), by the warps' own matrix instructions, which
-// keep the tensor cores from the sums for some eight times as long (us, 8192 tokens of rank 64 in 12 runs, all that way 313 altogether, as groups 200).
+// keep the tensor cores from the sums for some eight times as long (us, both products of 8192 tokens of rank 64 in 12 runs, all that way 313, as groups 250).
 // kMakeLow: those vectors, scale A x, rows by a list, in two 16-bit values each.
 // Warps 0-7 store finished accumulators, warp 8 issues the tile copies, warp 9 the matrix instructions; two accumulators in tensor memory,
 // so that one is stored while the next is computed (HALVES = 2: while the other half of the next tile begins).  The sum goes 64 values (128 bytes of a row) a stage.

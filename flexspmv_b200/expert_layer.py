@@ -250,7 +250,7 @@ class RoutedStack(nn.Module):
         """``x`` (tokens, width) of the matrices' type.  ``mask`` (tokens) bool: tokens that are there; the others count as rows of zeros, whatever they hold."""
         if mask is not None:
             x = x.masked_fill(~mask[:, None], 0.0)
-        all_tokens = torch.tensor([0, x.shape[0]], dtype=torch.int32, device=x.device)
+        all_tokens = torch.arange(2, dtype=torch.int32, device=x.device) * x.shape[0]          # made on the device: a step may be captured
         p = self.p if self.training else 0.0
         stream, normed, loss = x, layer_norm(x, self.weight[0], self.bias[0]), torch.zeros((), device=x.device)
         for i, layer in enumerate(self.layers):

@@ -64,7 +64,8 @@ def patterns(tokens, count, seed=0):
 @pytest.mark.parametrize("tokens,n,k,count,rank", [
     (1, 8, 8, 1, 8), (1, 4096, 2048, 3, 16), (2, 136, 72, 4, 16), (7, 1000, 1416, 5, 24), (16, 64, 64, 2, 8), (17, 128, 4096, 40, 32), (48, 4096, 4096, 64, 16),
     (48, 520, 264, 64, 40), (64, 256, 512, 9, 64), (65, 1032, 200, 70, 72), (200, 384, 1000, 200, 128), (513, 4096, 256, 30, 8), (1024, 512, 512, 3, 48),
-    (1025, 520, 520, 1024, 16), (1031, 1000, 1416, 96, 8), (2500, 2048, 1024, 20, 64), (5000, 264, 136, 7, 256), (300, 136, 264, 3, 512), (300, 4096, 4096, 20, 16), (130, 2048, 2048, 40, 32), (150, 1000, 6000, 64, 128)])
+    (1025, 520, 520, 1024, 16), (1031, 1000, 1416, 96, 8), (2500, 2048, 1024, 20, 64), (5000, 264, 136, 7, 256), (300, 136, 264, 3, 512), (300, 4096, 4096, 20, 16), (130, 2048, 2048, 40, 32), (150, 1000, 6000, 64, 128), (3000, 512, 264, 5, 24), (2100, 520, 1000, 3, 40),
+    (1500, 264, 264, 4, 72), (4097, 136, 72, 300, 16)])
 def test_project(tokens, n, k, count, rank, dtype):
     x, w, a, b, scale = operands(tokens, n, k, count, rank, dtype)
     for i, values in enumerate(patterns(tokens, count)):
@@ -87,7 +88,29 @@ def test_project_large(tokens, n, k, count, rank):
         check(adapters.project(x, w, a, b, adapters.plan(ids, count), scale=scale), x, w, a, b, ids, scale)
 
 
-@pytest.mark.parametrize("tokens,n,k,rank", [(5, 136, 264, 16), (48, 512, 512, 32), (300, 512, 264, 16), (3000, 1024, 512, 64)])
+def test_so_many_tokens_that_groups_are_longer_runs():
+    """More than 64 000 tokens: at most some 1000 groups, and runs around their limit."""
+    tokens, n, k, count, rank = 150_000, 72, 64, 50, 16
+    x, w, a, b, scale = operands(tokens, n, k, count, rank, torch.bfloat16)
+    r = np.random.default_rng(3)
+    for lengths in (r.integers(1, 700, 1000), np.full(600, 299), np.full(600, 300), r.integers(1, 3, 110_000)):
+        ids = np.repeat(np.arange(lengths.size) * 7 % (count + 1) - 1, lengths)[:tokens]
+        ids = ids_of(np.concatenate([ids, np.full(tokens - ids.size, 2)]))
+        check(adapters.project(x, w, a, b, adapters.plan(ids, count), scale=scale), x, w, a, b, ids, scale)
+    experts.check()
+
+
+@pytest.mark.parametrize("tokens", [1100, 3000])
+def test_runs_around_the_length_of_a_group(tokens):
+    n, k, count, rank = 520, 136, 9, 40
+    x, w, a, b, scale = operands(tokens, n, k, count, rank, torch.float16)
+    for lengths in ([127, 128, 129, 1, 128, 64, 64, 200, 1, 1], [1] * 10 + [128] * 3 + [5] + [300], [tokens], [tokens - 1, 1], [1, tokens - 1]):
+        values = np.resize(np.repeat(np.arange(len(lengths)) % (count + 1) - 1, lengths), tokens)
+        ids = ids_of(values)
+        check(adapters.project(x, w, a, b, adapters.plan(ids, count), scale=scale), x, w, a, b, ids, scale)
+
+
+@pytest.mark.parametrize("tokens,n,k,rank", [(5, 136, 264, 16), (48, 512, 512, 32), (300, 512, 264, 16), (3000, 1024, 512, 64), (300, 4096, 512, 128)])
 def test_an_adapter_reaches_its_own_tokens_only(tokens, n, k, rank):
     """NaN and infinity in one adapter, in one token and in adapters that nobody has: every other token as without."""
     count = 6
@@ -108,13 +131,28 @@ def test_an_adapter_reaches_its_own_tokens_only(tokens, n, k, rank):
     assert not got[ids == 2].isfinite().any() and got[1].isnan().all()
 
 
+def test_a_long_run_keeps_to_itself():
+    """Groups of one adapter each, one of them infinite and one not a number, between others and tokens without any."""
+    tokens, n, k, count, rank = 2000, 520, 264, 6, 24
+    x, w, a, b, scale = operands(tokens, n, k, count, rank, torch.bfloat16)
+    ids = ids_of(np.repeat([0, 2, 1, -1, 3, 0, 2, 1], [300, 250, 150, 333, 267, 40, 260, 400]))
+    want = adapters.project(x, w, a, b, adapters.plan(ids, count), scale=scale)
+    a2, b2, s2 = a.clone(), b.clone(), scale.clone()
+    b2[2], a2[3] = float("inf"), float("nan")
+    s2[3:] = float("nan")
+    got = adapters.project(x, w, a2, b2, adapters.plan(ids, count), scale=s2)
+    bad = (ids == 2) | (ids == 3)
+    assert torch.equal(got[~bad], want[~bad]) and not got[bad].isfinite().any()
+
+
 def test_more_precise_than_a_16_bit_vector():
     """W x and B A x cancel: what is left shows scale A x to more than 16 bits."""
-    tokens, n, k, rank = 96, 256, 512, 16
-    x, w, a, b, _ = operands(tokens, n, k, 2, rank, torch.bfloat16)
-    w = (-(b[1].double() @ a[1].double())).bfloat16()
-    ids = ids_of(np.full(tokens, 1))
-    check(adapters.project(x, w, a, b, adapters.plan(ids, 2)), x, w, a, b, ids, None)
+    for tokens in (3, 96, 700, 1500):                                        # the divided, the mixed and the grouped form
+        n, k, rank = 256, 512, 16
+        x, w, a, b, _ = operands(tokens, n, k, 2, rank, torch.bfloat16)
+        w = (-(b[1].double() @ a[1].double())).bfloat16()
+        ids = ids_of(np.full(tokens, 1))
+        check(adapters.project(x, w, a, b, adapters.plan(ids, 2)), x, w, a, b, ids, None)
 
 
 def test_a_bound_plan_follows_its_ids_in_a_graph():

@@ -132,6 +132,38 @@ def test_stack_trains_with_every_gradient():
     experts.check()
 
 
+def test_captured_training_step_drops_other_places_in_every_replay():
+    stack = RoutedStack(64, 128, 8, 2, 2, p=0.3, generator=gen(18))
+    x, target = normal(19, (160, 64), torch.bfloat16), normal(20, (160, 64))
+
+    def step():
+        out = stack(x)
+        (F.mse_loss(out.y.float(), target) + 0.01 * out.loss).backward()
+
+    want = []
+    for offset in (2, 4):
+        stack.seed[1] = offset
+        step()
+        want.append([p.grad.clone() for p in stack.parameters()])
+        stack.zero_grad(set_to_none=True)
+    stack.seed[1] = 0
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()                               # two layers: the offset is 2 then
+    torch.cuda.current_stream().wait_stream(side)
+    stack.zero_grad(set_to_none=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for grads in want:
+        for p in stack.parameters():
+            p.grad.zero_()
+        graph.replay()
+        assert all(torch.equal(p.grad, g) for p, g in zip(stack.parameters(), grads))
+    experts.check()
+
+
 def test_decoding_stack_is_the_stack():
     stack = RoutedStack(256, 128, 16, 2, 2, generator=gen(14)).eval()
     for tokens in (1, 5):
