@@ -230,8 +230,9 @@ __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(LowArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, g = lane >> 2, r0 = blockIdx.y * kRanks, share = (int)cluster_rank();
   pdl_wait();
   pdl_launch_dependents();
-  if ((int)blockIdx.x >= *a.count) return;          // the whole cluster
-  const AdapterTile tile = a.tiles[blockIdx.x];
+  const int count = *a.count;
+  const AdapterTile tile = a.tiles[blockIdx.x];     // on its way with the count; the plan has room for all that are launched
+  if ((int)blockIdx.x >= count) return;             // the whole cluster
   // rows and ranks that are not there: the first one's, whose results are left out
   const T *x[2], *down[NB];
 #pragma unroll

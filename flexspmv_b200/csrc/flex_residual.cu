@@ -13,15 +13,24 @@ int device_sm_count();
 
 // ---- random numbers ------------------------------------------------------------------------------------------------
 
+// The product's two halves.  BY_HAND: not as the language's product, for which the compiler chooses registers differently: us, the gradients of 16384 rows of 4096
+// 128 / 157, dropout 65 / 72, the norm 95 / 91.5.
+template <bool BY_HAND>
 __device__ __forceinline__ void product(uint32_t a, uint32_t b, uint32_t& high, uint32_t& low) {
-  // not as the language's product, whose registers the compiler chooses differently: the gradients of 16384 rows of 4096 take 128 us, with that 157
-  asm("{\n\t.reg .b64 p;\n\tmul.wide.u32 p, %2, %3;\n\tmov.b64 {%1, %0}, p;\n\t}" : "=r"(high), "=r"(low) : "r"(a), "r"(b));
+  if constexpr (BY_HAND) {
+    asm("{\n\t.reg .b64 p;\n\tmul.wide.u32 p, %2, %3;\n\tmov.b64 {%1, %0}, p;\n\t}" : "=r"(high), "=r"(low) : "r"(a), "r"(b));
+  } else {
+    const unsigned long long p = (unsigned long long)a * b;
+    high = (uint32_t)(p >> 32);
+    low = (uint32_t)p;
+  }
 }
 
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers, as easy as 1, 2, 3; 2011).  Four words for four neighbouring columns of
 // a row: counter (column / 4, row, offset), key = seed, so that a value's word goes by its place alone, whatever the launch, the strides or the type,
 // and the backward pass makes it again.  19 products of 64 bits for four values, of which the multiplier takes some 50 us for 2^26 values: as long as
 // DRAM takes for one array and a half of them in 16 bits.
+template <bool BY_HAND = true>
 struct Random {
   uint32_t offset1, first, second;     // the counter's last word, and what every first round makes of the one before it
   uint32_t key0[10], key1[10];         // of the rounds; made once a thread
@@ -47,8 +56,8 @@ struct Random {
 #pragma unroll
     for (int i = 1; i < 10; ++i) {
       uint32_t a, b, low_a, low_b;
-      product(c0, 0xD2511F53u, a, low_a);
-      product(c2, 0xCD9E8D57u, b, low_b);
+      product<BY_HAND>(c0, 0xD2511F53u, a, low_a);
+      product<BY_HAND>(c2, 0xCD9E8D57u, b, low_b);
       c0 = b ^ c1 ^ key0[i];
       c1 = low_b;
       c2 = a ^ c3 ^ key1[i];
@@ -314,7 +323,7 @@ __global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEA
   const int at = threadIdx.x % TPR, group = threadIdx.x / TPR;
   int turn = 0;
   pdl_wait();
-  const Random random(a.seed, DROP);
+  const Random<!(WIDE && AHEAD > 0)> random(a.seed, DROP);
   const float inverse = 1.f / (float)a.width;
   const long long step = (long long)gridDim.x * kRows, from = (long long)blockIdx.x * kRows + group;
   Ahead<T, C, WIDE, S, L, TPR, kThreads, AHEAD ? AHEAD : 1, 2> next(rows_sm);
@@ -426,7 +435,7 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(NormArgs a) {
   __shared__ __align__(16) float buf[2][1][32];
   int turn = 0;
   pdl_wait();
-  const Random random(a.seed, a.seed != nullptr);
+  const Random<> random(a.seed, a.seed != nullptr);
   const float inverse = 1.f / (float)a.width;
   for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const auto sum_at = [&](int c, float (&s)[C]) {
@@ -514,7 +523,7 @@ __global__ void __launch_bounds__(AHEAD ? kAheadGradThreads : row_threads(TPR), 
 #pragma unroll
     for (int j = 0; j < C; ++j) dw[i][j] = db[i][j] = 0.f;
   pdl_wait();
-  const Random random(a.seed, DROP);
+  const Random<> random(a.seed, DROP);
   const float inverse = 1.f / (float)a.width;
   const long long step = (long long)gridDim.x * kRows, from = (long long)blockIdx.x * kRows + group;
   Ahead<T, C, WIDE, S, L, TPR, kThreads, 3, 1> next(rows_sm);
@@ -657,7 +666,7 @@ __global__ void __launch_bounds__(1024) layer_norm_backward_long_kernel(NormGrad
   __shared__ __align__(16) float buf[2][2][32];
   int turn = 0;
   pdl_wait();
-  const Random random(a.seed, a.seed != nullptr);
+  const Random<> random(a.seed, a.seed != nullptr);
   const float inverse = 1.f / (float)a.width;
   for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const float mean = a.mean[r], rstd = a.rstd[r];
@@ -771,7 +780,7 @@ struct DropoutArgs {
 template <class T, int C, bool WIDE>
 __global__ void __launch_bounds__(256, 4) dropout_kernel(DropoutArgs a) {
   pdl_wait();
-  const Random random(a.seed, true);
+  const Random<> random(a.seed, true);
   const int pieces = (a.width + C - 1) / C;
   const long long work = a.rows * pieces, step = (long long)gridDim.x * 256;
   const long long row_step = step / pieces;
