@@ -200,6 +200,28 @@ def test_back_to_back_launches_follow_their_inputs():
     assert torch.equal(again, second)
 
 
+def test_two_streams_at_once():
+    """Calls of two batches on two streams, each two launches of which the second begins early."""
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    calls, want = [], []
+    for i, tokens in enumerate((48, 2000)):
+        x, w, a, b, scale = operands(tokens, 1024, 1024, 8, 32, torch.bfloat16, seed=10 * i)
+        ids = ids_of(np.sort(np.random.default_rng(i).integers(-1, 8, tokens)))
+        plan = adapters.plan(ids, 8)
+        want.append(adapters.project(x, w, a, b, plan, scale=scale))
+        check(want[-1], x, w, a, b, ids, scale)
+        calls.append(experts.bind(adapters.project, x, w, a, b, plan, scale=scale))
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for side, call in zip(sides, calls):
+            with torch.cuda.stream(side):
+                call.launch()
+    torch.cuda.synchronize()
+    for call, exact in zip(calls, want):
+        assert torch.equal(call.outputs, exact)
+    experts.check()
+
+
 def test_ids_that_are_no_adapter_are_noticed():
     x, w, a, b, _ = operands(20, 64, 64, 3, 8, torch.bfloat16)
     values = np.arange(20) % 4 - 1

@@ -111,6 +111,25 @@ def test_layer_norm(rows, width, dtype):
         check_norm(a, *c)
 
 
+# as many rows as are copied ahead, in every number of threads a row, on and off 16 bytes
+MANY = [(10_003, 64), (9_700, 33), (10_001, 504), (5_001, 768), (5_003, 1001), (4_750, 1024), (2_501, 2048), (2_400, 2001), (1_301, 4096), (610, 8192), (330, 16384)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", MANY)
+def test_layer_norm_of_many_rows(rows, width, dtype):
+    x, r = normal(1, (rows, width), dtype, 1.5, 0.3), normal(2, (rows, width), dtype, 2.0, -0.5)
+    w, b = normal(3, (width,), torch.float32, 0.2, 1.0), normal(4, (width,), torch.float32, 0.3)
+    seed = seed_of(77, rows)
+    for residual_rows, p in ((r, 0.2), (r, 0.0), (None, 0.0), (None, 0.5)):
+        out = residual.layer_norm(x, w, b, residual=residual_rows, p=p, seed=seed)
+        check_norm(out, x, w, b, 1e-5, residual_rows, p, seed)
+        again = residual.layer_norm(x, w, b, residual=residual_rows, p=p, seed=seed)
+        assert all(torch.equal(s, t) for s, t in zip(out, again) if s is not None)
+    gap = 8 if width % 8 == 0 else 3
+    check_norm(residual.layer_norm(apart(x, gap), None, None, residual=apart(r, gap), p=0.2, seed=seed), x, None, None, 1e-5, r, 0.2, seed)
+
+
 def test_layer_norm_of_special_rows():
     x = normal(5, (8, 640), torch.bfloat16)
     x[0] = 0.0                                                               # no variance: 0 times 1 / sqrt(eps)
@@ -177,6 +196,23 @@ def test_layer_norm_backward(rows, width, dtype):
     again = residual.layer_norm_backward(dy, x, w, mean, rstd, dsum=dsum, p=0.3, seed=seed)
     assert all(torch.equal(a, b) for a, b in zip(out, again))
     check_backward(residual.layer_norm_backward(apart(dy, 5), apart(x, 8), None, mean, rstd, dsum=apart(dsum, 1)), dy, x, None, mean, rstd, dsum, 0.0, None)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", MANY)
+def test_layer_norm_backward_of_many_rows(rows, width, dtype):
+    x, dy, dsum = normal(1, (rows, width), dtype, 1.5, 0.3), normal(2, (rows, width), dtype, 0.5, 0.1), normal(3, (rows, width), dtype)
+    var, mean = torch.var_mean(x.double(), dim=1, correction=0)
+    mean, rstd = mean.float(), ((var + 1e-5) ** -0.5).float()
+    w, seed = normal(4, (width,), torch.float32, 0.2, 1.0), seed_of(18, rows)
+    for d, p in ((dsum, 0.2), (None, 0.0)):
+        out = residual.layer_norm_backward(dy, x, w, mean, rstd, dsum=d, p=p, seed=seed)
+        check_backward(out, dy, x, w, mean, rstd, d, p, seed)
+        again = residual.layer_norm_backward(dy, x, w, mean, rstd, dsum=d, p=p, seed=seed)
+        assert all(torch.equal(s, t) for s, t in zip(out, again))
+    gap = 8 if width % 8 == 0 else 3
+    out = residual.layer_norm_backward(apart(dy, gap), apart(x, 2 * gap), None, mean, rstd, dsum=apart(dsum, gap))
+    check_backward(out, dy, x, None, mean, rstd, dsum, 0.0, None)
 
 
 def test_layer_norm_gradients_are_differences():
