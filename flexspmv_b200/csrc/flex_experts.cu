@@ -827,7 +827,8 @@ static int route_typed(const RouteArgs& a, cudaStream_t st) {
 }
 
 // Clusters of the balance loss: a few tokens a warp, up to one CTA an SM.
-constexpr long long kBalanceSmall = 64;      // tokens up to which one CTA does it all
+// Tokens up to which one CTA does it all; us, one / two launches: 48 tokens of 64 experts 3.3 / 6.3, 128 3.9 / 6.3, 128 of 384 5.8 / 7.4, 300 of 128 8.2 / 6.8.
+constexpr long long kBalanceSmall = 128;
 static int balance_clusters(long long tokens) {
   const long long want = (tokens + 63) / 64;
   const int most = device_sm_count() / kBalanceCtas;

@@ -1079,9 +1079,10 @@ static int grouped_launch(const GroupedArgs& a, cudaStream_t st) {
     // And where as narrow tiles all of them run at once: a part of the sum is a quarter as much to add up, a gathered step a quarter of the rows.
     // us, narrow / wide: 753 rows, 4 experts of 104 x 1512 8.9 / 15.1; 256 rows of 2048 x 2048 10.5 / 14.3, of a list 11.0 / 16.0; 512 rows of 1024 x 1024
     // 7.3 / 8.1; but 100 rows of 4096 x 4096 13.0 / 12.3.
-    const long long narrow = ((MODE == kGroupedDx ? a.k : a.n) + 127) / 128 * ((ADAPT == kAddLow ? 1 + a.experts / 16 : a.slots < a.experts ? a.slots : a.experts) + a.slots / 64);
+    const long long narrow = ((MODE == kGroupedDx ? a.k : a.n) + 127) / 128 * ((ADAPT == kAddLow ? 2 : a.slots < a.experts ? a.slots : a.experts) + a.slots / 64);
+    // kAddLow has as many groups as there may be, most of them empty: one more tile for each column of tiles, and a matrix, are counted.
     // kMakeLow: the rank is at most a few tiles' rows, so that narrow ones are what there is to run at once.
-    if (ADAPT == kMakeLow || a.slots <= 32ll * a.experts || narrow <= device_sm_count()) return grouped_tiles<T, TO, MODE, 64, 1, GATHER, false, ADAPT>(a, st);
+    if (ADAPT == kMakeLow || a.slots <= 32ll * (ADAPT == kAddLow ? 1 : a.experts) || narrow <= device_sm_count()) return grouped_tiles<T, TO, MODE, 64, 1, GATHER, false, ADAPT>(a, st);
     if constexpr (ADAPT != kMakeLow) return grouped_tiles<T, TO, MODE, 256, 2, GATHER, false, ADAPT>(a, st);
   }
 }
