@@ -48,8 +48,8 @@ def _bytes(name: str, d: Desc) -> int:
 
 
 @functools.lru_cache(maxsize=256)
-def _project_bytes(tokens: int, rank: int) -> int:
-    return _bytes("adapted_project_bytes", Desc(tokens, 8, 1, rank, 8, 8, _TYPE[torch.bfloat16]))
+def _project_bytes(tokens: int, rank: int, kind: int) -> int:
+    return _bytes("adapted_project_bytes", Desc(tokens, 8, 1, rank, 8, 8, kind))
 
 
 @functools.lru_cache(maxsize=256)
@@ -114,7 +114,7 @@ def project(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: torch.Ten
     else:
         out = _out(out, (tokens, n), x.dtype, x.device, x=x, weight=weight, a=a, b=b, scale=scale, plan=plan.data)
     d = Desc(tokens, stride, adapters, rank, n, k, _TYPE[x.dtype])
-    need = _project_bytes(tokens, rank)
+    need = _project_bytes(tokens, rank, d.type)
     ws = x.new_empty(need, dtype=torch.uint8)
     ins = (_P * 6)(*at)
     outs = (_P * 1)(out.data_ptr())

@@ -298,8 +298,10 @@ __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(LowArgs a) {
       if (a.scale) h *= a.scale[tile.adapter];
     }
     T* const row = static_cast<T*>(a.low) + (long long)a.rows[tile.from + p] * a.width;
-    row[low_high(r, a.rank)] = from_float<T>(h);
-    row[low_rest(r, a.rank)] = from_float<T>(low_rest_of<T>(h));
+    float part[kLowParts<T>];
+    low_parts<T>(h, part);
+#pragma unroll
+    for (int x = 0; x < kLowParts<T>; ++x) row[low_at<T>(r, a.rank, x)] = from_float<T>(part[x]);
   }
   cluster_sync();                          // no CTA leaves while its sums may be read
 }
@@ -337,6 +339,8 @@ static int low_product(const LowArgs& a, const AdapterPlan& p, cudaStream_t st) 
   if (a.rank <= 32) return low_launch<T, 4>(a, p, st);
   return low_launch<T, 8>(a, p, st);
 }
+
+static int low_parts_of(int type) { return type == FLEXSPMV_TYPE_BF16 ? kLowParts<__nv_bfloat16> : kLowParts<__half>; }
 
 // `product`: n, k and the rank count too.
 static int check_adapters(const flexspmv_adapter_desc* d, bool product) {
@@ -380,7 +384,7 @@ int flexspmv_adapter_plan(const flexspmv_adapter_desc* d, const int32_t* ids, vo
 int flexspmv_adapted_project_bytes(const flexspmv_adapter_desc* d, size_t* bytes) {
   if (!bytes) return FLEXSPMV_ERR_BAD_ARG;
   if (int e = flex::check_adapters(d, true)) return e;
-  *bytes = (size_t)d->tokens * flex::low_width(d->rank) * 2;
+  *bytes = (size_t)d->tokens * flex::low_width(d->rank, flex::low_parts_of(d->type)) * 2;
   return 0;
 }
 
@@ -390,7 +394,7 @@ int flexspmv_adapted_project(const flexspmv_adapter_desc* d, const void* const* 
   if (!in || !out) return FLEXSPMV_ERR_BAD_ARG;
   if (d->tokens == 0) return 0;
   if (!in[0] || !in[1] || !in[2] || !in[3] || !in[5] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
-  const int width = low_width(d->rank);
+  const int width = low_width(d->rank, low_parts_of(d->type));
   const size_t need = (size_t)d->tokens * width * 2;
   if (!ws || ws_bytes < need) return FLEXSPMV_ERR_WORKSPACE;
   if (!aligned16(in[0]) || !aligned16(in[1]) || !aligned16(in[2]) || !aligned16(in[3]) || !aligned16(in[5]) || !aligned16(out[0]) || !aligned16(ws) ||

@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint4* __restrict_
 // ADAPT (forward): kAddLow: one matrix for all groups, and each place's adapter's up matrix times its vector of `rank` values.  Groups of one adapter have it as one to
 // a few steps more of their sum; in mixed groups it is added on a place's way out, before the only rounding (low_rank_part), by the warps' own matrix instructions, which
 // keep the tensor cores from the sums for some eight times as long (us, both products of 8192 tokens of rank 64 in 12 runs, all that way 313, as groups 250).
-// kMakeLow: those vectors, scale A x, rows by a list, in two 16-bit values each.
+// kMakeLow: those vectors, scale A x, rows by a list, in 16-bit parts (low_parts).
 // Warps 0-7 store finished accumulators, warp 8 issues the tile copies, warp 9 the matrix instructions; two accumulators in tensor memory,
 // so that one is stored while the next is computed (HALVES = 2: while the other half of the next tile begins).  The sum goes 64 values (128 bytes of a row) a stage.
 constexpr int kStoreWarps = 8, kCopyWarp = kStoreWarps, kMathWarp = kStoreWarps + 1, kGroupedThreads = (kStoreWarps + 2) * 32;
@@ -167,6 +167,7 @@ struct LowPart {
 };
 template <class T>
 __device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int place, int left, int lane, LowPart& r) {
+  constexpr int kParts = kLowParts<T>;
   const int q = lane & 3, g = lane >> 2;
   const int id = lane < left ? a.ids[place + lane] : -1;
 #pragma unroll
@@ -185,7 +186,7 @@ __device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int p
     if (a.rank <= 16) {
       const int k = q * 4;
       const uint2 none = make_uint2(0, 0);
-      uint2 w[4], h[4][2];
+      uint2 w[4], h[4][kParts];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         w[i] = none;
@@ -193,11 +194,12 @@ __device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int p
       }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        h[b][0] = h[b][1] = none;
+#pragma unroll
+        for (int x = 0; x < kParts; ++x) h[b][x] = none;
         if (k < a.rank && (mine >> (b * 8 + g) & 1u)) {
           const T* const row = low + (size_t)b * 8 * a.low_width + k;
-          h[b][0] = *reinterpret_cast<const uint2*>(row);
-          h[b][1] = *reinterpret_cast<const uint2*>(row + 32);
+#pragma unroll
+          for (int x = 0; x < kParts; ++x) h[b][x] = *reinterpret_cast<const uint2*>(row + x * 16);
         }
       }
 #pragma unroll
@@ -206,13 +208,13 @@ __device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int p
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) warp_mma<T>(d[i][b], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h[b][x].x, h[b][x].y);
+          for (int x = 0; x < kParts; ++x) warp_mma<T>(d[i][b], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h[b][x].x, h[b][x].y);
       }
     } else {
 #pragma unroll 1
       for (int k = q * 8; k - q * 8 < a.rank; k += 32) {
         const bool inside = k < a.rank;
-        uint4 w[4], h[4][2];
+        uint4 w[4], h[4][kParts];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           w[i] = make_uint4(0, 0, 0, 0);
@@ -220,11 +222,12 @@ __device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int p
         }
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          h[b][0] = h[b][1] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int x = 0; x < kParts; ++x) h[b][x] = make_uint4(0, 0, 0, 0);
           if (inside && (mine >> (b * 8 + g) & 1u)) {
             const T* const row = low + (size_t)b * 8 * a.low_width;
-            h[b][0] = *reinterpret_cast<const uint4*>(row + low_high(k, a.rank));
-            h[b][1] = *reinterpret_cast<const uint4*>(row + low_rest(k, a.rank));
+#pragma unroll
+            for (int x = 0; x < kParts; ++x) h[b][x] = *reinterpret_cast<const uint4*>(row + low_at<T>(k, a.rank, x));
           }
         }
 #pragma unroll
@@ -233,7 +236,7 @@ __device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int p
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
+            for (int x = 0; x < kParts; ++x) {
               warp_mma<T>(d[i][b], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h[b][x].x, h[b][x].y);
               warp_mma<T>(d[i][b], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, h[b][x].z, h[b][x].w);
             }
@@ -255,9 +258,20 @@ __device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int p
 // as many loads under way as there are rows to a lane.  Ranks of 32 and more: four lanes a row, 64 bytes of it at a time.
 template <class T, int ROWS>
 __device__ __forceinline__ void low_rank_rows(const GroupedArgs& a, int m, int from, int to, int warp, int lane, float* out) {
-  constexpr int kParts = 128 / ROWS;
-  for (int unit = warp; unit < (to - from) * kParts; unit += kStoreWarps) {
-    const int p = from + unit / kParts, f0 = unit % kParts * ROWS, id = a.ids[p];
+  constexpr int kPieces = 128 / ROWS;
+  const auto vector_of = [&](const T* row, int k, float (&v)[8]) {
+    Pack<T, 8> part[kLowParts<T>];
+#pragma unroll
+    for (int i = 0; i < kLowParts<T>; ++i) part[i].load(row + low_at<T>(k, a.rank, i));
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      v[x] = part[0].get(x);
+#pragma unroll
+      for (int i = 1; i < kLowParts<T>; ++i) v[x] += part[i].get(x);
+    }
+  };
+  for (int unit = warp; unit < (to - from) * kPieces; unit += kStoreWarps) {
+    const int p = from + unit / kPieces, f0 = unit % kPieces * ROWS, id = a.ids[p];
     float* const to_place = out + (p - from) * 128 + f0;
     if ((unsigned)id >= (unsigned)a.adapters) {
 #pragma unroll
@@ -267,7 +281,7 @@ __device__ __forceinline__ void low_rank_rows(const GroupedArgs& a, int m, int f
     const T* const row = static_cast<const T*>(a.low) + (size_t)p * a.low_width;
     const T* const up = static_cast<const T*>(a.up) + ((size_t)id * a.n + m + f0) * a.rank;
     const int there = a.n - m - f0;          // features that there are; others count as the last of them
-    Pack<T, 8> h, rest;
+    float v[8];
     if (a.rank >= 32) {
       constexpr int kRows = ROWS / 8;
       float sum[kRows];
@@ -280,11 +294,7 @@ __device__ __forceinline__ void low_rank_rows(const GroupedArgs& a, int m, int f
           const int f = i * 8 + lane / 4;
           w[i].load(up + (size_t)(f < there ? f : there > 0 ? there - 1 : -f0) * a.rank + k);
         }
-        h.load(row + low_high(k, a.rank));
-        rest.load(row + low_rest(k, a.rank));
-        float v[8];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) v[x] = h.get(x) + rest.get(x);
+        vector_of(row, k, v);
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
@@ -309,12 +319,11 @@ __device__ __forceinline__ void low_rank_rows(const GroupedArgs& a, int m, int f
           const int f = i * 32 + lane;
           w[i].load(up + (size_t)(f < there ? f : there > 0 ? there - 1 : -f0) * a.rank + k);
         }
-        h.load(row + low_high(k, a.rank));
-        rest.load(row + low_rest(k, a.rank));
+        vector_of(row, k, v);
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
-          for (int x = 0; x < 8; ++x) sum[i] = fmaf(w[i].get(x), h.get(x) + rest.get(x), sum[i]);
+          for (int x = 0; x < 8; ++x) sum[i] = fmaf(w[i].get(x), v[x], sum[i]);
       }
 #pragma unroll
       for (int i = 0; i < kRows; ++i) to_place[i * 32 + lane] = sum[i];
@@ -421,10 +430,10 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
   auto stopped = [&] { return __any_sync(0xffffffffu, *abort) != 0; };
   auto sum_steps = [&](const GroupedTile& t) { return ((MODE == kGroupedForward ? a.k : MODE == kGroupedDx ? a.n : t.count) + 63) / 64; };
-  // kAddLow: steps of 64 high and then as many rests of the vectors, or 32 of both
-  auto steps_of = [&](const GroupedTile& t) {
-    return sum_steps(t) + (ADAPT == kAddLow && group_adapters[t.e] >= 0 ? (a.rank <= 32 ? 1 : (a.rank + 63) / 64 * 2) : 0);
-  };
+  // kAddLow: the steps of 64 that the vectors' rows have
+  constexpr int kParts = kLowParts<T>;
+  auto steps_of = [&](const GroupedTile& t) { return sum_steps(t) + (ADAPT == kAddLow && group_adapters[t.e] >= 0 ? a.low_width / 64 : 0); };
+  auto low_column = [&](int low_step) { return a.rank <= 32 ? 0 : low_step / kParts * 64; };
   // This cluster's tile of round u.  Where the last round has tiles for half or a quarter of the clusters at most, each is divided in two or four: HALVES = 2
   // in two by rows, else by places.  us, whole / divided: 4102 rows of 16 experts of 1024 x 2048 26.8 / 25.1, dx 22.8 / 22.3, with a list of rows
   // 27.7 / 27.1; 5003 rows of 40 experts of 1000 x 1416 with a list 37.1 / 36.1; 1024 rows of 8 experts of 2048 x 2048 14.4 / 14.5.
@@ -500,7 +509,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
             if (!waited) pdl_wait();
             waited = true;
             if (rank == 0) mbar_expect_tx(&bars.full[stage], PAIR * (kTileBytesA + pieces * 4096));
-            tma_3d<PAIR>(sa, &row_a, low_step / 2 * 64, m0, group_adapters[t.e], bar);
+            tma_3d<PAIR>(sa, &row_a, low_column(low_step), m0, group_adapters[t.e], bar);
             for (int g = 0; g < pieces; ++g) tma_2d<PAIR>(sb + g * 4096, &row_b, low_step * 64, t.from + rank * half + g * 32, bar);
           } else {
             if (rank == 0) mbar_expect_tx(&bars.full[stage], PAIR * (halves * kTileBytesA + pieces * 4096));
@@ -553,11 +562,12 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           const uint64_t da = kA_mn ? umma_desc(sa, 8192, 1024) : umma_desc(sa, 16, 1024);
           const uint64_t db = kB_mn ? umma_desc(sb, 8192, 1024) : umma_desc(sb, 16, 1024);
           if (ADAPT == kAddLow && s >= sum_steps(t)) {
-            const int low_step = s - sum_steps(t), left = a.rank - low_step / 2 * 64, slices = left < 64 ? (left + 15) / 16 : 4;
-            for (int x = 0; x < slices; ++x) {
-              umma<PAIR>(tmem + acc * NT, da + x * 2, db + x * 2, instr, true);
-              if (a.rank <= 32) umma<PAIR>(tmem + acc * NT, da + x * 2, db + (x + 2) * 2, instr, true);
-            }
+            // slices of 16 of the up matrix, each with those of its parts that are in this step; a CTA's share of a divided sum may begin here
+            const int low_step = s - sum_steps(t), left = a.rank - low_column(low_step), slices = left < 64 ? (left + 15) / 16 : 4;
+            const int each = a.rank <= 16 ? 1 : a.rank <= 32 ? 2 : 4;          // slices that a part has room for
+            const int parts = a.rank > 32 ? 1 : a.rank <= 16 ? kParts : kParts - low_step * 2 < 2 ? kParts - low_step * 2 : 2;
+            for (int p = 0; p < parts; ++p)
+              for (int x = 0; x < slices; ++x) umma<PAIR>(tmem + acc * NT, da + x * 2, db + (p * each + x) * 2, instr, !begins || p + x > 0);
             return;
           }
           const int inner = MODE == kGroupedDw && t.count - s * 64 < 64 ? (t.count - s * 64 + 15) / 16 : 4;
@@ -845,10 +855,12 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           if constexpr (ADAPT == kMakeLow) {
             const float scale = a.scale ? a.scale[t.e] : 1.f;
 #pragma unroll
-            for (int rest = 0; rest < 2; ++rest) {
+            for (int part = 0; part < kLowParts<TO>; ++part) {
               turn([&](const uint32_t (&w)[16], int i) {
-                const float u = __uint_as_float(w[i]) * scale, v = __uint_as_float(w[i + 1]) * scale;
-                return rest ? two_of<TO>(low_rest_of<TO>(u), low_rest_of<TO>(v)) : two_of<TO>(u, v);
+                float u[kLowParts<TO>], v[kLowParts<TO>];
+                low_parts<TO>(__uint_as_float(w[i]) * scale, u);
+                low_parts<TO>(__uint_as_float(w[i + 1]) * scale, v);
+                return two_of<TO>(u[part], v[part]);
               });
 #pragma unroll
               for (int x = 0; x < 4; ++x) {
@@ -856,7 +868,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
                 if (c0 + p < t.count && c < ((a.n + 15) & ~15)) {          // 16 at a time, with zeros (kAddLow takes as many)
                   const int row = a.rows[t.from + c0 + p];
                   if ((unsigned)row < (unsigned)a.tokens)
-                    *reinterpret_cast<uint4*>(out + (size_t)row * a.low_width + (rest ? low_rest(c, a.n) : low_high(c, a.n))) = piece(p);
+                    *reinterpret_cast<uint4*>(out + (size_t)row * a.low_width + low_at<TO>(c, a.n, part)) = piece(p);
                 }
               }
               __syncwarp();
