@@ -8,8 +8,8 @@ that the token's request names.  Tokens stay in their order; one token or a prom
 two launches.  The second begins while the first runs: only its stores wait for the adapters' part, which is added before y's only rounding.
 
 Checks, streams, errors and ``experts.bind`` are those of ``experts``; results carry no gradient (an adapter is trained as ``experts.grouped_matmul``
-twice, with its gradients).  Ids that are no adapter are noticed on the device and count as none: the next call of a projection on the device, or
-``experts.check()``, raises.  (The reference has no operator of the kind.)
+twice, with its gradients).  Ids that are no adapter are noticed on the device and count as none; so is a bound plan that a projection reads before its
+first launch: the next call of a projection on the device, or ``experts.check()``, raises.  (The reference has no operator of the kind.)
 """
 from __future__ import annotations
 

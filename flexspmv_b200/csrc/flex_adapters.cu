@@ -19,7 +19,7 @@ struct AdapterTile {
   int adapter, from, count, unused;          // places from .. from + count of `rows`, all of one adapter
 };
 
-// Where a plan's parts lie, in ints; [0] is the number of tiles.  Groups: for the shared product of many tokens, runs of one adapter that are long enough for tiles of
+// Where a plan's parts lie, in ints; it begins with the number of tiles, the tokens and the adapters that it is of.  Groups: for the shared product of many tokens, runs of one adapter that are long enough for tiles of
 // their own, and what lies between them.
 constexpr int kLowTile = 16;
 // Tokens up to which they are one group; us, one / several: 1500 tokens in runs of 300 (2048 x 2048, rank 32) 29.9 / 33.2, 2000 in runs of 400 (4096 x 4096, rank 64) 83 / 77.
@@ -143,6 +143,8 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(AdapterPlanA
     if (lane == 0) {
       a.plan[a.at.offsets + a.adapters] = places;
       a.plan[0] = a.at.most_tiles ? tiles : 0;
+      a.plan[1] = (int)a.tokens;
+      a.plan[2] = a.adapters;
     }
   }
   __syncthreads();
@@ -211,11 +213,12 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(AdapterPlanA
 struct LowArgs {
   const void *x, *down;
   const float* scale;
-  const int *rows, *count;
+  const int *rows, *plan;
   const AdapterTile* tiles;
   void* low;
   long long stride;
-  int rank, k, width;
+  int tokens, adapters, rank, k, width;
+  int* status;
 };
 
 // low[t] = scale A x[t] of few tokens: a cluster of four CTAs takes a tile of up to 16 tokens of one adapter and 8 NB values of the rank (blockIdx.y), their warps every 32nd 32
@@ -232,15 +235,22 @@ __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(LowArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, g = lane >> 2, r0 = blockIdx.y * kRanks, share = (int)cluster_rank();
   pdl_wait();
   pdl_launch_dependents();
-  const int count = *a.count;
-  const AdapterTile tile = a.tiles[blockIdx.x];     // on its way with the count; the plan has room for all that are launched
-  if ((int)blockIdx.x >= count) return;             // the whole cluster
+  const int4 head = *reinterpret_cast<const int4*>(a.plan);
+  const AdapterTile tile = a.tiles[blockIdx.x];     // on its way with the head; the plan has room for all that are launched
+  // The whole cluster.  A plan of other tokens or adapters, or none yet: the next launch says so.
+  if ((int)blockIdx.x >= head.x || head.y != a.tokens || head.z != a.adapters) return;
+  if ((unsigned)tile.adapter >= (unsigned)a.adapters || tile.count < 1 || tile.count > kLowTile || tile.from < 0 || tile.from > a.tokens - tile.count) {
+    if (threadIdx.x == 0 && a.status) *a.status = FLEXSPMV_ERR_BAD_CSR;
+    return;
+  }
   // rows and ranks that are not there: the first one's, whose results are left out
   const T *x[2], *down[NB];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int p = i * 8 + g;
-    x[i] = static_cast<const T*>(a.x) + (long long)a.rows[tile.from + (p < tile.count ? p : 0)] * a.stride;
+    const int p = i * 8 + g, row = a.rows[tile.from + (p < tile.count ? p : 0)];
+    const bool there = (unsigned)row < (unsigned)a.tokens;
+    if (!there && a.status) *a.status = FLEXSPMV_ERR_BAD_CSR;
+    x[i] = static_cast<const T*>(a.x) + (there ? row : 0) * a.stride;
   }
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
@@ -297,7 +307,9 @@ __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(LowArgs a) {
       for (int c = 0; c < kLowCtas; ++c) h += cluster_load(cluster_smem(&sums[p * kRanks + j], c));
       if (a.scale) h *= a.scale[tile.adapter];
     }
-    T* const row = static_cast<T*>(a.low) + (long long)a.rows[tile.from + p] * a.width;
+    const int to = a.rows[tile.from + p];
+    if ((unsigned)to >= (unsigned)a.tokens) continue;
+    T* const row = static_cast<T*>(a.low) + (long long)to * a.width;
     float part[kLowParts<T>];
     low_parts<T>(h, part);
 #pragma unroll
@@ -408,13 +420,13 @@ int flexspmv_adapted_project(const flexspmv_adapter_desc* d, const void* const* 
     return FLEXSPMV_ERR_BAD_ARG;
   const int* const plan = static_cast<const int*>(in[5]);
   const LowArgs a = {in[0], in[2], static_cast<const float*>(in[4]), plan + p.rows, plan, reinterpret_cast<const AdapterTile*>(plan + p.tiles), ws, d->x_stride,
-                     d->rank, d->k, width};
+                     (int)d->tokens, d->adapters, d->rank, d->k, width, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int e;
   if (!low_in_tiles(d->tokens, d->rank)) e = low_product_of_many(d, in[0], in[2], a.scale, plan + p.offsets, a.rows, ws, width, status, st);
   else e = d->type == FLEXSPMV_TYPE_BF16 ? low_product<__nv_bfloat16>(a, p, st) : low_product<__half>(a, p, st);
   if (e) return e;
-  return adapted_product(d, in[0], in[1], in[3], ws, width, p.most_groups, plan + p.groups, plan + p.group_adapters, plan + p.ids, out[0], status, st);
+  return adapted_product(d, in[0], in[1], in[3], ws, width, plan, p.most_groups, plan + p.groups, plan + p.group_adapters, plan + p.ids, out[0], status, st);
 }
 
 }  // extern "C"

@@ -11,8 +11,8 @@ namespace flex {
 
 // A place's vector scale A x, a sum of 32 bits, is kept as 16-bit values that add up to it, which the matrix instructions take as they are: three bfloat16
 // have all 24 of its bits; two float16 22 of them, which is 2^-11 of what y's own rounding takes.  (Two bfloat16, 17 bits, made 1.1 of 1000 values of y another
-// one than the 32-bit vector does.)  us, two / three: 8192 tokens of rank 64 (4096 x 4096, 12 runs) 225 / 230, 2000 in 5 runs 74 / 87, 300 of rank 16 in short
-// runs 37.5 / 47.4, 48 of rank 16 14.6 / 14.7.
+// one than the 32-bit vector does.)  us, two / three: 8192 tokens of rank 64 (4096 x 4096, 12 runs) 223 / 227, 2000 in 5 runs 80.5 / 82, 300 of rank 16 in
+// short runs 42 / 46, 48 of rank 16 14.6 / 14.7.
 // In a row: ranks up to 16: a part behind the other, 16 values each; up to 32: 32 each; else 64 of the vector at a time, their parts behind one another.  Rows
 // are whole steps of 64 values.
 template <class T> constexpr int kLowParts = std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
@@ -53,9 +53,10 @@ __device__ __forceinline__ void warp_mma(float (&d)[4], uint32_t a0, uint32_t a1
 int low_product_of_many(const flexspmv_adapter_desc* d, const void* x, const void* down, const float* scale, const int* offsets, const int* rows, void* low,
                         int low_width, int* status, cudaStream_t st);
 // y = weight x + up low (flex_grouped.cu).  The kernel before it on the stream has been launched for it (see ADAPT there).  groups: offsets of groups of
-// tokens, group_adapters: the adapter that all tokens of a group have, or one of these.
+// tokens, group_adapters: the adapter that all tokens of a group have, or one of these.  plan: its second and third int say of how many tokens and adapters
+// all of this is; of others: nothing is written, and the status says so.
 enum { kGroupMixed = -1, kGroupBare = -2 };
-int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* low, int low_width, int num_groups,
+int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* low, int low_width, const int* plan, int num_groups,
                     const int* groups, const int* group_adapters, const int* ids, void* out, int* status, cudaStream_t st);
 
 }  // namespace flex

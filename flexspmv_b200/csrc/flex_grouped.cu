@@ -27,6 +27,7 @@ struct GroupedArgs {
   const int* ids;
   const void *up, *low;
   int adapters, rank, low_width;
+  const int* plan;               // [1]: the tokens, [2]: the adapters that the groups and places are of
   const int* group_adapters;     // the adapter that all of a group's places have, or kGroupMixed, kGroupBare
   const float* scale;            // of the first product
 };
@@ -383,11 +384,13 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
   // its result.
   if (ADAPT != kAddLow) pdl_wait();
   if (ADAPT == kMakeLow) pdl_launch_dependents();
+  const bool known = ADAPT != kAddLow || (a.plan[1] == (int)a.slots && a.plan[2] == a.adapters);          // else: no groups
+  if (!known && tid == 0) raise(a.status, FLEXSPMV_ERR_BAD_CSR);
   for (int e = tid; e < a.experts; e += kThreads) {
     int from, to;
     group_of(a, e, from, to);
     table[e].from = from;
-    table[e].count = to - from;
+    table[e].count = known ? to - from : 0;
     if (ADAPT == kAddLow) reinterpret_cast<int*>(table + a.experts + 1)[e] = a.group_adapters[e];
   }
   __syncthreads();
@@ -1164,9 +1167,10 @@ static int grouped_call(const flexspmv_expert_desc* d, const void* const* in, vo
   return d->type == FLEXSPMV_TYPE_BF16 ? go(__nv_bfloat16()) : go(__half());
 }
 
-int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* low, int low_width, int num_groups,
+int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* low, int low_width, const int* plan, int num_groups,
                     const int* groups, const int* group_adapters, const int* ids, void* out, int* status, cudaStream_t st) {
   GroupedArgs a = {x, weight, groups, nullptr, out, d->tokens, d->tokens, d->x_stride, 0, num_groups, d->n, d->k, status};
+  a.plan = plan;
   a.group_adapters = group_adapters;
   a.ids = ids;
   a.up = up;

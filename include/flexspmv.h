@@ -588,7 +588,8 @@ int flexspmv_dropout(const flexspmv_rows_desc *desc, const void *const *inputs, 
  *   adapter_plan       ids (tokens, int32; -1: none) -> a plan in d_plan (_bytes, 16-byte aligned), for all projections of the tokens.  d_status (or
  *                      null) becomes FLEXSPMV_ERR_BAD_CSR where an id leaves [-1, adapters); it counts as none
  *   adapted_project    in: x, weight, a, b, scale, the plan; out: y; workspace: _bytes, 16-byte aligned.  d_status (or null) becomes
- *                      FLEXSPMV_ERR_TIMEOUT where a bounded wait ran out
+ *                      FLEXSPMV_ERR_TIMEOUT where a bounded wait ran out, FLEXSPMV_ERR_BAD_CSR where the plan is of other tokens or adapters (y is not
+ *                      written then), has not been made yet, or names tokens or adapters that there are not
  */
 #define FLEXSPMV_MAX_ADAPTERS 1024
 #define FLEXSPMV_MAX_RANK 512
