@@ -23,6 +23,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from . import adapters, experts, residual
+from .binding import FlexSpmvError
 
 
 class _Route(torch.autograd.Function):
@@ -285,7 +286,12 @@ class DecodingStep:
     def __init__(self, layer: RoutedExperts, tokens: int, x: Optional[torch.Tensor] = None):
         """``x``: the buffer to read, where something else writes it."""
         w1 = layer.w1.detach()
-        self.x = torch.zeros((tokens, w1.shape[2]), dtype=w1.dtype, device=w1.device) if x is None else x
+        if x is None:
+            x = torch.zeros((tokens, w1.shape[2]), dtype=w1.dtype, device=w1.device)
+        experts._tensor(x, "x", (w1.dtype,), 2, w1.get_device())
+        if tuple(x.shape) != (tokens, w1.shape[2]):
+            raise FlexSpmvError(f"x must have the shape {(tokens, w1.shape[2])}, not {tuple(x.shape)}")
+        self.x = x
         self._router = layer.router.detach().t()          # a view: the bound step follows the weights
         self._x32 = torch.zeros(self.x.shape, dtype=torch.float32, device=w1.device)
         self._logits = torch.zeros((tokens, w1.shape[0]), dtype=torch.float32, device=w1.device)
@@ -317,6 +323,8 @@ class DecodingStack:
     ``y``.  Without ``low_rank`` the projections are the stack's own.  Nothing is allocated or checked per step, nothing is dropped."""
 
     def __init__(self, stack: RoutedStack, tokens: int, low_rank: Optional[Sequence[Adapter]] = None):
+        if low_rank and len(low_rank) != len(stack.layers):
+            raise FlexSpmvError(f"adapters of {len(low_rank)} projections for {len(stack.layers)} layers")
         first = stack.shared[0].detach()
         width, device = first.shape[1], first.device
         self.x = torch.zeros((tokens, width), dtype=first.dtype, device=device)
