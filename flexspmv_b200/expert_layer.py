@@ -107,31 +107,32 @@ class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         out = residual.layer_norm(x, weight, bias, eps=eps)
-        ctx.save_for_backward(x, weight, out.mean, out.rstd)
+        ctx.save_for_backward(x, weight, out.mean, out.rstd, bias if weight is None else None)
+        ctx.has_bias = bias is not None
         return out.y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        g = residual.layer_norm_backward(dy.contiguous(), x, weight, mean, rstd)
-        return g.dx, g.dweight, g.dbias, None
+        x, weight, mean, rstd, bias = ctx.saved_tensors
+        g = residual.layer_norm_backward(dy.contiguous(), x, weight, mean, rstd, bias=bias)
+        return g.dx, g.dweight, g.dbias if ctx.has_bias else None, None
 
 
 class _SumNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, stream, weight, bias, eps, p, seed):
         out = residual.layer_norm(x, weight, bias, eps=eps, residual=stream, p=p, seed=seed)
-        ctx.save_for_backward(out.sum, weight, out.mean, out.rstd, seed)
-        ctx.p = p
+        ctx.save_for_backward(out.sum, weight, out.mean, out.rstd, seed, bias if weight is None else None)
+        ctx.p, ctx.has_bias = p, bias is not None
         return out.sum, out.y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dsum, dy):
-        total, weight, mean, rstd, seed = ctx.saved_tensors
-        g = residual.layer_norm_backward(dy.contiguous(), total, weight, mean, rstd, dsum=dsum.contiguous(), p=ctx.p, seed=seed)
-        return g.dx, g.dresidual, g.dweight, g.dbias, None, None, None
+        total, weight, mean, rstd, seed, bias = ctx.saved_tensors
+        g = residual.layer_norm_backward(dy.contiguous(), total, weight, mean, rstd, dsum=dsum.contiguous(), p=ctx.p, seed=seed, bias=bias)
+        return g.dx, g.dresidual, g.dweight, g.dbias if ctx.has_bias else None, None, None, None
 
 
 class _Dropout(torch.autograd.Function):
@@ -159,12 +160,12 @@ def route_balanced(logits: torch.Tensor, k: int, renormalize: bool = False):
     return experts.Plan(weights, ids, offsets, rows, slots, renormalize), experts.Balance(loss, counts, mean, tokens)
 
 
-def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:
-    """``residual.layer_norm`` of ``x`` itself, with gradients for ``x``, ``weight`` and ``bias``."""
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float = 1e-5) -> torch.Tensor:
+    """``residual.layer_norm`` of ``x`` itself, with gradients for ``x`` and for ``weight`` and ``bias`` where they are given."""
     return _Norm.apply(x, weight, bias, eps)
 
 
-def sum_norm(x: torch.Tensor, stream: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: float = 1e-5, p: float = 0.0,
+def sum_norm(x: torch.Tensor, stream: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float = 1e-5, p: float = 0.0,
              seed: Optional[torch.Tensor] = None):
     """``stream + dropout(x)`` and its norm, with gradients.  ``seed`` must hold the same two values until the backward pass: give it a copy of one that is raised."""
     return _SumNorm.apply(x, stream, weight, bias, eps, p, seed)

@@ -142,30 +142,32 @@ def _backward_bytes(rows: int, width: int, device: int) -> int:
 
 @_operator
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor, rstd: torch.Tensor,
-                        dsum: Optional[torch.Tensor] = None, p: float = 0.0, seed: Optional[torch.Tensor] = None) -> NormGradients:
+                        dsum: Optional[torch.Tensor] = None, p: float = 0.0, seed: Optional[torch.Tensor] = None,
+                        bias: Optional[torch.Tensor] = None) -> NormGradients:
     """Gradients of ``layer_norm``.  ``x`` is what was normalised (``Normed.sum`` where there is one), ``dsum`` a gradient that reaches it directly;
-    ``dx`` is what passes the dropout of ``p`` and ``seed``.  ``dweight`` and ``dbias`` are of the weight's type; without a weight there are none."""
+    ``dx`` is what passes the dropout of ``p`` and ``seed``.  ``dweight`` and ``dbias`` are of the weight's type; without a weight there is ``dbias`` alone, of
+    the type of ``bias`` (whose values are not read), or none."""
     dev, rows, width, ys = _first(dy, "dy")
     if x is None:
         raise FlexSpmvError("x is what was normalised")
     xs, ds = _matrix(x, "x", dy, dev, rows, width), _matrix(dsum, "dsum", dy, dev, rows, width)
-    kind, p = _params(weight, None, dy, width, dev), _drops(p, seed, dev)
+    kind, p = _params(weight, bias, dy, width, dev), _drops(p, seed, dev)
     _vector(mean, "mean", (torch.float32,), rows, dev, "row")
     _vector(rstd, "rstd", (torch.float32,), rows, dev, "row")
     dresidual = dy.new_empty((rows, width))
     dx = torch.empty_like(dresidual) if p > 0.0 else dresidual
     dweight = dbias = ws = None
     need = 0
-    if weight is not None:
-        dweight, dbias = torch.empty_like(weight), torch.empty_like(weight)
+    if weight is not None or bias is not None:
+        dweight, dbias = (torch.empty_like(weight if weight is not None else bias) for _ in range(2))
         need = _backward_bytes(rows, width, dev)
         ws = dy.new_empty(need, dtype=torch.uint8)
-    out = NormGradients(dx, dresidual, dweight, dbias)
+    out = NormGradients(dx, dresidual, dweight if weight is not None else None, dbias)
     d = Desc(rows, width, (ys, xs, ds), _TYPE[dy.dtype], kind, 0.0, 0, p)
     ins, outs = _at(dy, x, weight, mean, rstd, dsum, seed if p > 0.0 else None), _at(dx if p > 0.0 else None, dresidual, dweight, dbias)
     return BoundCall(_function("layer_norm_backward", _WITH_WORKSPACE),
                      (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), ws.data_ptr() if ws is not None else None, need), dev,
-                     (d, ins, outs, dy, x, weight, mean, rstd, dsum, seed, ws, out), out)
+                     (d, ins, outs, dy, x, weight, mean, rstd, dsum, seed, ws, dweight, out), out)
 
 
 @_operator
