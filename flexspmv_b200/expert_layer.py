@@ -230,7 +230,9 @@ class RoutedStack(nn.Module):
         s' = s + dropout(experts(n) + W n),   n' = norm(s')
 
     with a norm of its own in front of the first.  Norms and routers are in 32 bits, the matrices in ``dtype``.  Dropout is on in training mode; ``seed``
-    (a seed and an offset, a buffer) is raised once a layer and step."""
+    (a seed and an offset, a buffer) is raised once a layer and step.  Stacks of one seed drop the same places: ranks that train together on tokens of their
+    own take different ones.  A pass that is run again in the backward pass (``torch.utils.checkpoint``) would find the buffer raised and drop other places than
+    its loss has, which is an error: give ``forward`` a seed then."""
 
     def __init__(self, width: int, hidden: int, num_experts: int, k: int, depth: int, p: float = 0.1, dtype: torch.dtype = torch.bfloat16, device="cuda",
                  generator: Optional[torch.Generator] = None, seed: int = 0):
@@ -244,12 +246,15 @@ class RoutedStack(nn.Module):
         self.register_buffer("seed", torch.tensor([seed, 0], dtype=torch.int64, device=device))
 
     def _next_seed(self) -> torch.Tensor:
+        if torch._C._current_graph_task_id() != -1:          # the autograd engine runs this
+            raise FlexSpmvError("a stack's forward pass is run again in a backward pass, with another offset than the first time: give forward a seed")
         used = self.seed.clone()
         self.seed[1] += 1
         return used
 
-    def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None) -> Stacked:
-        """``x`` (tokens, width) of the matrices' type.  ``mask`` (tokens) bool: tokens that are there; the others count as rows of zeros, whatever they hold."""
+    def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None, seed: Optional[torch.Tensor] = None) -> Stacked:
+        """``x`` (tokens, width) of the matrices' type.  ``mask`` (tokens) bool: tokens that are there; the others count as rows of zeros, whatever they hold.
+        ``seed`` (two int64 values): takes the place of the stack's own, which is then neither read nor raised; layer i has its offset plus i."""
         if mask is not None:
             x = x.masked_fill(~mask[:, None], 0.0)
         all_tokens = torch.arange(2, dtype=torch.int32, device=x.device) * x.shape[0]          # made on the device: a step may be captured
@@ -258,7 +263,10 @@ class RoutedStack(nn.Module):
         for i, layer in enumerate(self.layers):
             routed, even = layer(normed, mask, balance=True)
             z = routed + _Grouped.apply(normed, self.shared[i], all_tokens, None, None)
-            stream, normed = sum_norm(z, stream, self.weight[i + 1], self.bias[i + 1], p=p, seed=self._next_seed() if p > 0.0 else None)
+            used = None
+            if p > 0.0:
+                used = self._next_seed() if seed is None else torch.stack([seed[0], seed[1] + i])
+            stream, normed = sum_norm(z, stream, self.weight[i + 1], self.bias[i + 1], p=p, seed=used)
             loss = loss + even.loss
         return Stacked(normed, loss)
 
