@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <mutex>
 #include <type_traits>
 
 #include "../../include/flexspmv.h"
@@ -86,17 +87,21 @@ struct Pack {
 };
 
 // Lets a kernel have this much dynamic shared memory; the runtime is asked once for a kernel, a device and a size that with the
-// kernel's own arrays (8 KB at the most) may be above 48 KB.
+// kernel's own arrays (8 KB at the most) may be above 48 KB.  One thread at a time asks, so that no smaller size takes a larger one's place, which another
+// thread is about to launch with.
 template <auto KERNEL>
 int allow_smem(int bytes) {
   static std::atomic<int> allowed[64];
+  static std::mutex asking;
   int device = 0;
   if (bytes <= 40 * 1024) return 0;
   if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return (int)e;
   const bool known = device >= 0 && device < 64;
+  if (known && allowed[device].load(std::memory_order_acquire) >= bytes) return 0;
+  std::lock_guard<std::mutex> lock(asking);
   if (known && allowed[device].load(std::memory_order_relaxed) >= bytes) return 0;
   if (cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); e != cudaSuccess) return (int)e;
-  if (known) allowed[device].store(bytes, std::memory_order_relaxed);
+  if (known) allowed[device].store(bytes, std::memory_order_release);
   return 0;
 }
 
