@@ -216,8 +216,10 @@ struct LowArgs {
   const int *rows, *plan;
   const AdapterTile* tiles;
   void* low;
+  float* wide;
+  unsigned char* flags;
   long long stride;
-  int tokens, adapters, rank, k, width;
+  int tokens, adapters, rank, k, width, wide_width;
   int* status;
 };
 
@@ -298,17 +300,31 @@ __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(LowArgs a) {
   }
   cluster_sync();
   // each CTA some of the tokens; 16 of the rank at a time, with zeros: the second product takes as many
+  static_assert(kValues / kLowCtas % 32 == 0, "whole warps");
   for (int i = threadIdx.x; i < kValues / kLowCtas; i += kLowThreads) {
     const int p = i / kRanks * kLowCtas + share, j = i % kRanks, r = r0 + j;
-    if (p >= tile.count || r >= ((a.rank + 15) & ~15)) continue;
+    const int to = p < tile.count ? a.rows[tile.from + p] : -1;
     float h = 0.f;
-    if (r < a.rank) {
+    if (p < tile.count && r < a.rank) {
 #pragma unroll
       for (int c = 0; c < kLowCtas; ++c) h += cluster_load(cluster_smem(&sums[p * kRanks + j], c));
       if (a.scale) h *= a.scale[tile.adapter];
     }
-    const int to = a.rows[tile.from + p];
-    if ((unsigned)to >= (unsigned)a.tokens) continue;
+    bool wide = false;
+    if constexpr (kHasWide<T>) {             // the 32 that a flag is of (ranks up to 16: 16) are a warp's (a half's)
+      const unsigned mine = kRanks >= 32 ? 0xffffffffu : 0xffffu << (lane & 16);
+      const unsigned above = __ballot_sync(0xffffffffu, !(fabsf(h) <= kWideAbove)), some = __ballot_sync(0xffffffffu, h != 0.f),
+                     large = __ballot_sync(0xffffffffu, fabsf(h) >= kWideBelow);
+      wide = (above & mine) || ((some & mine) && !(large & mine));
+    }
+    if ((unsigned)to >= (unsigned)a.tokens || r >= ((a.rank + 15) & ~15)) continue;
+    if constexpr (kHasWide<T>) {
+      if (j % 32 == 0) a.flags[(long long)(r / 32) * a.tokens + to] = wide;
+      if (wide) {
+        a.wide[(long long)to * a.wide_width + r] = h;
+        h = 0.f;
+      }
+    }
     T* const row = static_cast<T*>(a.low) + (long long)to * a.width;
     float part[kLowParts<T>];
     low_parts<T>(h, part);
@@ -352,8 +368,6 @@ static int low_product(const LowArgs& a, const AdapterPlan& p, cudaStream_t st) 
   return low_launch<T, 8>(a, p, st);
 }
 
-static int low_parts_of(int type) { return type == FLEXSPMV_TYPE_BF16 ? kLowParts<__nv_bfloat16> : kLowParts<__half>; }
-
 // `product`: n, k and the rank count too.
 static int check_adapters(const flexspmv_adapter_desc* d, bool product) {
   if (!d || d->tokens < 0 || d->adapters < 1) return FLEXSPMV_ERR_BAD_ARG;
@@ -396,7 +410,7 @@ int flexspmv_adapter_plan(const flexspmv_adapter_desc* d, const int32_t* ids, vo
 int flexspmv_adapted_project_bytes(const flexspmv_adapter_desc* d, size_t* bytes) {
   if (!bytes) return FLEXSPMV_ERR_BAD_ARG;
   if (int e = flex::check_adapters(d, true)) return e;
-  *bytes = (size_t)d->tokens * flex::low_width(d->rank, flex::low_parts_of(d->type)) * 2;
+  *bytes = (size_t)flex::low_places(d->tokens, d->rank, d->type).bytes;
   return 0;
 }
 
@@ -406,8 +420,8 @@ int flexspmv_adapted_project(const flexspmv_adapter_desc* d, const void* const* 
   if (!in || !out) return FLEXSPMV_ERR_BAD_ARG;
   if (d->tokens == 0) return 0;
   if (!in[0] || !in[1] || !in[2] || !in[3] || !in[5] || !out[0]) return FLEXSPMV_ERR_BAD_ARG;
-  const int width = low_width(d->rank, low_parts_of(d->type));
-  const size_t need = (size_t)d->tokens * width * 2;
+  const LowPlaces low = low_places(d->tokens, d->rank, d->type);
+  const size_t need = (size_t)low.bytes;
   if (!ws || ws_bytes < need) return FLEXSPMV_ERR_WORKSPACE;
   if (!aligned16(in[0]) || !aligned16(in[1]) || !aligned16(in[2]) || !aligned16(in[3]) || !aligned16(in[5]) || !aligned16(out[0]) || !aligned16(ws) ||
       !aligned_to(4, in[4], status))
@@ -419,14 +433,15 @@ int flexspmv_adapted_project(const flexspmv_adapter_desc* d, const void* const* 
               {in[4], 4ll * d->adapters}, {in[5], p.ints * 4}}))
     return FLEXSPMV_ERR_BAD_ARG;
   const int* const plan = static_cast<const int*>(in[5]);
-  const LowArgs a = {in[0], in[2], static_cast<const float*>(in[4]), plan + p.rows, plan, reinterpret_cast<const AdapterTile*>(plan + p.tiles), ws, d->x_stride,
-                     (int)d->tokens, d->adapters, d->rank, d->k, width, status};
+  const LowArgs a = {in[0], in[2], static_cast<const float*>(in[4]), plan + p.rows, plan, reinterpret_cast<const AdapterTile*>(plan + p.tiles), ws,
+                     reinterpret_cast<float*>(static_cast<char*>(ws) + low.wide), static_cast<unsigned char*>(ws) + low.flags, d->x_stride, (int)d->tokens,
+                     d->adapters, d->rank, d->k, low.width, low.wide_width, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int e;
-  if (!low_in_tiles(d->tokens, d->rank)) e = low_product_of_many(d, in[0], in[2], a.scale, plan + p.offsets, a.rows, ws, width, status, st);
+  if (!low_in_tiles(d->tokens, d->rank)) e = low_product_of_many(d, in[0], in[2], a.scale, plan + p.offsets, a.rows, ws, status, st);
   else e = d->type == FLEXSPMV_TYPE_BF16 ? low_product<__nv_bfloat16>(a, p, st) : low_product<__half>(a, p, st);
   if (e) return e;
-  return adapted_product(d, in[0], in[1], in[3], ws, width, plan, p.most_groups, plan + p.groups, plan + p.group_adapters, plan + p.ids, out[0], status, st);
+  return adapted_product(d, in[0], in[1], in[3], ws, plan, p.most_groups, plan + p.groups, plan + p.group_adapters, plan + p.ids, out[0], status, st);
 }
 
 }  // extern "C"

@@ -32,8 +32,31 @@ __device__ __forceinline__ void low_parts(float v, float (&part)[kLowParts<T>]) 
   for (int p = 0; p < kLowParts<T>; ++p) {
     if constexpr (std::is_same<T, __nv_bfloat16>::value) part[p] = __uint_as_float(__float_as_uint(left) & 0xffff0000u);
     else part[p] = to_float(from_float<T>(left));
-    left = finite && fabsf(part[p]) <= 3.402823466e38f ? left - part[p] : 0.f;
+    left = finite ? left - part[p] : 0.f;
   }
+}
+// Float16 parts go from 65504 down to steps of 2^-24.  A vector's 32 neighbouring values that leave this range, by one that is larger (or not finite) or by all of them
+// being so small that the steps show, are kept as they are, in 32 bits, and their parts are zeros; a flag says so.  The flagged ones' products are added on the
+// result's way out (low_rank_wide), which costs the others the flags' loads (us, none flagged, without flags / with: one token 8.6 / 9.0, 8192 of rank 64 234 / 238; all
+// flagged 451, by ordinary arithmetic 2800).
+// kWideBelow: the largest of the 32 has 2^-17 of itself in those steps' halves then, a 32nd of y's own rounding.
+template <class T> constexpr bool kHasWide = std::is_same<T, __half>::value;
+constexpr float kWideAbove = 65504.f, kWideBelow = 0x1p-8f;
+// Where the vectors' workspace has what: the parts, then (float16) the values of flagged ones and the flags.
+struct LowPlaces {
+  long long wide, flags, bytes;          // bytes from its beginning
+  int width, wide_width;                 // values of a row
+};
+inline LowPlaces low_places(long long tokens, int rank, int type) {
+  const bool has_wide = type != FLEXSPMV_TYPE_BF16;
+  const int parts = type == FLEXSPMV_TYPE_BF16 ? kLowParts<__nv_bfloat16> : kLowParts<__half>;
+  LowPlaces p;
+  p.width = low_width(rank, parts);
+  p.wide_width = (rank + 31) / 32 * 32;
+  p.wide = tokens * p.width * 2;
+  p.flags = p.wide + (has_wide ? tokens * p.wide_width * 4 : 0);
+  p.bytes = p.flags + (has_wide ? (tokens * (p.wide_width / 32) + 15) / 16 * 16 : 0);
+  return p;
 }
 
 // The warp's matrix instruction: d (16 x 8, 32-bit) += a (16 x 16) b (16 x 8).
@@ -49,14 +72,22 @@ __device__ __forceinline__ void warp_mma(float (&d)[4], uint32_t a0, uint32_t a1
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// low[rows[i]] = scale[e] down[e] x[rows[i]] (flex_grouped.cu) for the places offsets[e] <= i < offsets[e + 1].
-int low_product_of_many(const flexspmv_adapter_desc* d, const void* x, const void* down, const float* scale, const int* offsets, const int* rows, void* low,
-                        int low_width, int* status, cudaStream_t st);
-// y = weight x + up low (flex_grouped.cu).  The kernel before it on the stream has been launched for it (see ADAPT there).  groups: offsets of groups of
-// tokens, group_adapters: the adapter that all tokens of a group have, or one of these.  plan: its second and third int say of how many tokens and adapters
-// all of this is; of others: nothing is written, and the status says so.
+// The same of 32-bit values whose last 13 bits are zeros, 8 of them: d (16 x 8) += a (16 x 8) b (8 x 8).
+__device__ __forceinline__ void warp_mma_wide(float (&d)[4], float a0, float a1, float a2, float a3, float b0, float b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(a2)), "r"(__float_as_uint(a3)), "r"(__float_as_uint(b0)),
+                 "r"(__float_as_uint(b1)));
+}
+
+// The vectors of the places offsets[e] <= i < offsets[e + 1], scale[e] down[e] x[rows[i]], into the workspace (flex_grouped.cu).
+int low_product_of_many(const flexspmv_adapter_desc* d, const void* x, const void* down, const float* scale, const int* offsets, const int* rows, void* ws,
+                        int* status, cudaStream_t st);
+// y = weight x + up low (flex_grouped.cu), with the vectors of the workspace.  The kernel before it on the stream has been launched for it (see ADAPT there).  groups:
+// offsets of groups of tokens, group_adapters: the adapter that all tokens of a group have, or one of these.  plan: its second and third int say of how many tokens
+// and adapters all of this is; of others: nothing is written, and the status says so.
 enum { kGroupMixed = -1, kGroupBare = -2 };
-int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* low, int low_width, const int* plan, int num_groups,
+int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* ws, const int* plan, int num_groups,
                     const int* groups, const int* group_adapters, const int* ids, void* out, int* status, cudaStream_t st);
 
 }  // namespace flex

@@ -26,7 +26,9 @@ struct GroupedArgs {
   // low-rank adapters (flex_adapters.cu): each place's adapter, all adapters' second matrices (adapters x n x rank), each place's scaled A x
   const int* ids;
   const void *up, *low;
-  int adapters, rank, low_width;
+  int adapters, rank, low_width, wide_width;
+  float* wide;                   // float16: the flagged vectors' values (tokens x wide_width), and the flags (wide_width / 32 x tokens)
+  unsigned char* flags;
   const int* plan;               // [1]: the tokens, [2]: the adapters that the groups and places are of
   const int* group_adapters;     // the adapter that all of a group's places have, or kGroupMixed, kGroupBare
   const float* scale;            // of the first product
@@ -255,12 +257,123 @@ __device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int p
   }
 }
 
+// Which of 32 places have flagged vectors (low_places); `left` of them are there.
+__device__ __forceinline__ unsigned wide_of(const GroupedArgs& a, int place, int left, int lane) {
+  bool wide = false;
+  if (lane < left && (unsigned)a.ids[place + lane] < (unsigned)a.adapters)          // others have no flags
+    for (int b = 0; b < a.wide_width / 32; ++b) wide |= a.flags[(long long)b * a.slots + place + lane] != 0;
+  return __ballot_sync(0xffffffffu, wide);
+}
+// Feature f's product with the flagged values of place p, whose adapter is `id`.
+template <class T>
+__device__ __forceinline__ float wide_low(const GroupedArgs& a, int id, int f, int p) {
+  float sum = 0.f;
+  for (int b = 0; b < a.wide_width / 32; ++b) {
+    if (!a.flags[(long long)b * a.slots + p]) continue;
+    for (int k = b * 32; k < a.rank && k < b * 32 + 32; k += 8) {
+      Pack<T, 8> w;
+      w.load(static_cast<const T*>(a.up) + ((size_t)id * a.n + f) * a.rank + k);
+      const float* const v = a.wide + (long long)p * a.wide_width + k;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) sum = fmaf(w.get(x), v[x], sum);
+    }
+  }
+  return sum;
+}
+// Adds the flagged places' products to those of low_rank_part: the same with 32-bit values in three parts of 11 bits, and B's, which have no more.
+template <class T>
+__device__ __forceinline__ void low_rank_wide(const GroupedArgs& a, int m, int place, unsigned wide, int lane, LowPart& r) {
+  const int q = lane & 3, g = lane >> 2;
+  const int id = wide >> lane & 1u ? a.ids[place + lane] : -1;
+  while (wide) {
+    const int adapter = __shfl_sync(0xffffffffu, id, __ffs(wide) - 1);
+    const unsigned mine = __ballot_sync(0xffffffffu, id == adapter) & wide;
+    wide &= ~mine;
+    float d[2][4][4];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) d[i / 16][i / 4 % 4][i % 4] = 0.f;
+    const T* const up = static_cast<const T*>(a.up) + ((size_t)adapter * a.n + m + g) * a.rank;
+#pragma unroll 1
+    for (int k0 = 0; k0 < a.rank; k0 += 32) {
+      const int k = k0 + q * 8;
+      Pack<T, 8> w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i].zero();
+        if (k < a.rank && m + g + i * 8 < a.n) w[i].load(up + (size_t)i * 8 * a.rank + k);
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        if (!(mine >> (b * 8) & 0xffu)) continue;
+        const int p = place + b * 8 + g;
+        Pack<float, 8> v;
+        v.zero();
+        if (k < a.rank && (mine >> (b * 8 + g) & 1u) && a.flags[(long long)(k0 / 32) * a.slots + p]) v.load(a.wide + (long long)p * a.wide_width + k);
+#pragma unroll
+        for (int x = 0; x < 3; ++x) {
+          float part[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            part[j] = __uint_as_float(__float_as_uint(v.v[j]) & 0xffffe000u);
+            v.v[j] = fabsf(v.v[j]) <= 3.402823466e38f ? v.v[j] - part[j] : 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+              warp_mma_wide(d[i][b], w[2 * i].get(j), w[2 * i + 1].get(j), w[2 * i].get(j + 1), w[2 * i + 1].get(j + 1), part[j], part[j + 1]);
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (mine >> (b * 8 + q * 2 + (x & 1)) & 1u) {
+          r.low[b * 4 + x] += d[0][b][x];
+          r.high[b * 4 + x] += d[1][b][x];
+        }
+  }
+}
+
+// kMakeLow, float16: of 32 places' vectors the 32 values from m on, laid out as above.  Those that leave the parts' range are put where flagged ones are, and zeros
+// take their place.
+__device__ __forceinline__ void flag_wide(const GroupedArgs& a, int m, int place, int left, int lane, uint32_t (&low)[16], uint32_t (&high)[16]) {
+  const int q = lane & 3, g = lane >> 2;
+  const uint32_t above = __float_as_uint(kWideAbove), below = __float_as_uint(kWideBelow);
+  unsigned wide = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {            // the places i / 2 * 8 + 2 q + i % 2
+    const int r = i / 2 * 4 + i % 2;
+    uint32_t most = max(max(low[r] & 0x7fffffffu, low[r + 2] & 0x7fffffffu), max(high[r] & 0x7fffffffu, high[r + 2] & 0x7fffffffu));          // NaN: the largest
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const unsigned of = __ballot_sync(0xffffffffu, most > above || (most != 0 && most < below)) & 15u;          // bit q
+#pragma unroll
+    for (int x = 0; x < 4; ++x) wide |= (of >> x & 1u) << (i / 2 * 8 + 2 * x + i % 2);
+  }
+  int row = lane < left ? a.rows[place + lane] : -1;
+  if ((unsigned)row >= (unsigned)a.tokens) row = -1;
+  if (row >= 0) a.flags[(long long)(m / 32) * a.tokens + row] = wide >> lane & 1u;
+  if (!wide) return;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int p = i / 4 * 8 + 2 * q + (i & 1), f = m + i % 4 / 2 * 8 + g, to = __shfl_sync(0xffffffffu, row, p);
+    if (!(wide >> p & 1u)) continue;
+    if (to >= 0 && f < a.n) a.wide[(long long)to * a.wide_width + f] = __uint_as_float(low[i]);
+    if (to >= 0 && f + 16 < a.n) a.wide[(long long)to * a.wide_width + f + 16] = __uint_as_float(high[i]);
+    low[i] = high[i] = 0u;
+  }
+}
+
 // SPLIT: the same for 128 features from m on by places from .. to, into out (128 features a place), by the storing warps, each ROWS features of a place at a time with
-// as many loads under way as there are rows to a lane.  Ranks of 32 and more: four lanes a row, 64 bytes of it at a time.
+// as many loads under way as there are rows to a lane.  Ranks of 32 and more: four lanes a row, 64 bytes of it at a time.  `parts`: else the flagged values alone.
 template <class T, int ROWS>
-__device__ __forceinline__ void low_rank_rows(const GroupedArgs& a, int m, int from, int to, int warp, int lane, float* out) {
+__device__ __forceinline__ void low_rank_rows(const GroupedArgs& a, int m, int from, int to, bool parts, int warp, int lane, float* out) {
   constexpr int kPieces = 128 / ROWS;
-  const auto vector_of = [&](const T* row, int k, float (&v)[8]) {
+  const auto vector_of = [&](const T* row, int p, int k, float (&v)[8]) {
+    bool wide = false;
+    if constexpr (kHasWide<T>) wide = a.flags[(long long)(k / 32) * a.slots + p] != 0;
     Pack<T, 8> part[kLowParts<T>];
 #pragma unroll
     for (int i = 0; i < kLowParts<T>; ++i) part[i].load(row + low_at<T>(k, a.rank, i));
@@ -270,6 +383,9 @@ __device__ __forceinline__ void low_rank_rows(const GroupedArgs& a, int m, int f
 #pragma unroll
       for (int i = 1; i < kLowParts<T>; ++i) v[x] += part[i].get(x);
     }
+    if (wide)
+#pragma unroll
+      for (int x = 0; x < 8; ++x) v[x] = a.wide[(long long)p * a.wide_width + k + x];
   };
   for (int unit = warp; unit < (to - from) * kPieces; unit += kStoreWarps) {
     const int p = from + unit / kPieces, f0 = unit % kPieces * ROWS, id = a.ids[p];
@@ -277,6 +393,14 @@ __device__ __forceinline__ void low_rank_rows(const GroupedArgs& a, int m, int f
     if ((unsigned)id >= (unsigned)a.adapters) {
 #pragma unroll
       for (int i = 0; i < ROWS / 32; ++i) to_place[i * 32 + lane] = 0.f;
+      continue;
+    }
+    if (kHasWide<T> && !parts) {
+#pragma unroll
+      for (int i = 0; i < ROWS / 32; ++i) {
+        const int f = f0 + i * 32 + lane;
+        to_place[i * 32 + lane] = m + f < a.n ? wide_low<T>(a, id, m + f, p) : 0.f;
+      }
       continue;
     }
     const T* const row = static_cast<const T*>(a.low) + (size_t)p * a.low_width;
@@ -295,7 +419,7 @@ __device__ __forceinline__ void low_rank_rows(const GroupedArgs& a, int m, int f
           const int f = i * 8 + lane / 4;
           w[i].load(up + (size_t)(f < there ? f : there > 0 ? there - 1 : -f0) * a.rank + k);
         }
-        vector_of(row, k, v);
+        vector_of(row, p, k, v);
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
@@ -320,7 +444,7 @@ __device__ __forceinline__ void low_rank_rows(const GroupedArgs& a, int m, int f
           const int f = i * 32 + lane;
           w[i].load(up + (size_t)(f < there ? f : there > 0 ? there - 1 : -f0) * a.rank + k);
         }
-        vector_of(row, k, v);
+        vector_of(row, p, k, v);
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
@@ -700,11 +824,12 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
         const GroupedTile t = tile_at<MODE, NT, PAIR, HALVES>(a, table, first);
         const int eights = (t.cols + 7) / 8, c_from = eights * share / split * 8, c_to = eights * (share + 1) / split * 8;
         static_assert(!SPLIT || ADAPT != kAddLow || NT / 2 * 512 <= Cfg::kStoreBytes, "half of a tile's places, the most that a CTA stores");
-        if (group_adapters[t.e] == kGroupMixed) {
+        const bool mixed = group_adapters[t.e] == kGroupMixed;
+        if (mixed || kHasWide<T>) {
           const int to = c_to < t.count ? c_to : t.count;
           float* const low = reinterpret_cast<float*>(store);
-          if (c_to - c_from >= kStoreWarps) low_rank_rows<T, 128>(a, t.m0, t.from + c_from, t.from + to, warp, lane, low);
-          else low_rank_rows<T, 32>(a, t.m0, t.from + c_from, t.from + to, warp, lane, low);
+          if (c_to - c_from >= kStoreWarps) low_rank_rows<T, 128>(a, t.m0, t.from + c_from, t.from + to, mixed, warp, lane, low);
+          else low_rank_rows<T, 32>(a, t.m0, t.from + c_from, t.from + to, mixed, warp, lane, low);
         }
       }
     }
@@ -812,8 +937,20 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
       // kAddLow: made while the sum is still under way
       LowPart parts;
       const bool mixed = ADAPT == kAddLow && group_adapters[t.e] == kGroupMixed;
-      if constexpr (ADAPT == kAddLow)
-        if (mixed) low_rank_part<T>(a, m, t.from + part * 32, t.count - part * 32, lane, parts);
+      unsigned wide = 0;
+      const auto low_of = [&](int c0) {
+        if constexpr (ADAPT == kAddLow) {
+          if (mixed) low_rank_part<T>(a, m, t.from + c0, t.count - c0, lane, parts);
+          if constexpr (kHasWide<T>) {
+            wide = group_adapters[t.e] != kGroupBare ? wide_of(a, t.from + c0, t.count - c0, lane) : 0;
+            if (wide && !mixed)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) parts.low[i] = parts.high[i] = 0.f;
+            if (wide) low_rank_wide<T>(a, m, t.from + c0, wide, lane, parts);
+          }
+        }
+      };
+      low_of(part * 32);
       if (!wait_warp(&bars.acc_full[acc], full_phase)) break;
       tmem_fence_after();
       const uint32_t d = tmem + acc * NT + ((uint32_t)(quarter * 32) << 16);
@@ -832,7 +969,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
         if (last) free_accumulator();
         if (!there) break;
         if constexpr (ADAPT == kAddLow)
-          if (mixed)
+          if (mixed || wide)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               low[i] = __float_as_uint(__uint_as_float(low[i]) + parts.low[i]);
@@ -856,13 +993,22 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           };
           const auto piece = [&](int p) { return reinterpret_cast<const uint4*>(mine)[p * 4 + (((lane & 3) ^ (p >> 1)) & 3)]; };
           if constexpr (ADAPT == kMakeLow) {
+            // features that there are not: zeros, whatever the scale
             const float scale = a.scale ? a.scale[t.e] : 1.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int eight = i % 4 / 2 * 8;
+              low[i] = m + eight < a.n ? __float_as_uint(__uint_as_float(low[i]) * scale) : 0u;
+              high[i] = m + 16 + eight < a.n ? __float_as_uint(__uint_as_float(high[i]) * scale) : 0u;
+            }
+            if constexpr (kHasWide<TO>)
+              if (m < a.n) flag_wide(a, m, t.from + c0, t.count - c0, lane, low, high);
 #pragma unroll
             for (int part = 0; part < kLowParts<TO>; ++part) {
               turn([&](const uint32_t (&w)[16], int i) {
                 float u[kLowParts<TO>], v[kLowParts<TO>];
-                low_parts<TO>(__uint_as_float(w[i]) * scale, u);
-                low_parts<TO>(__uint_as_float(w[i + 1]) * scale, v);
+                low_parts<TO>(__uint_as_float(w[i]), u);
+                low_parts<TO>(__uint_as_float(w[i + 1]), v);
                 return two_of<TO>(u[part], v[part]);
               });
 #pragma unroll
@@ -888,8 +1034,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           }
         }
         if (last) break;
-        if constexpr (ADAPT == kAddLow)
-          if (mixed) low_rank_part<T>(a, m, t.from + c0 + 64, t.count - c0 - 64, lane, parts);
+        low_of(c0 + 64);
       }
       if (HALVES == 2) {
         if (half) second_phase ^= 1;
@@ -939,7 +1084,7 @@ __global__ void __launch_bounds__(grouped_threads(GATHER), 1) grouped_kernel(con
           for (int x = 0; x < 8; ++x) sum[x] += v[x];
         }
         if constexpr (ADAPT == kAddLow)
-          if (group_adapters[t.e] == kGroupMixed && c < t.count) {
+          if ((kHasWide<T> || group_adapters[t.e] == kGroupMixed) && c < t.count) {
             const float* const low = reinterpret_cast<const float*>(store) + (c - c_from) * 128 + r;
 #pragma unroll
             for (int x = 0; x < 8; ++x) sum[x] += low[x];
@@ -1167,25 +1312,32 @@ static int grouped_call(const flexspmv_expert_desc* d, const void* const* in, vo
   return d->type == FLEXSPMV_TYPE_BF16 ? go(__nv_bfloat16()) : go(__half());
 }
 
-int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* low, int low_width, const int* plan, int num_groups,
+static GroupedArgs with_low(GroupedArgs a, const flexspmv_adapter_desc* d, void* ws) {
+  const LowPlaces p = low_places(d->tokens, d->rank, d->type);
+  a.low = ws;
+  a.wide = reinterpret_cast<float*>(static_cast<char*>(ws) + p.wide);
+  a.flags = static_cast<unsigned char*>(ws) + p.flags;
+  a.low_width = p.width;
+  a.wide_width = p.wide_width;
+  return a;
+}
+
+int adapted_product(const flexspmv_adapter_desc* d, const void* x, const void* weight, const void* up, const void* ws, const int* plan, int num_groups,
                     const int* groups, const int* group_adapters, const int* ids, void* out, int* status, cudaStream_t st) {
-  GroupedArgs a = {x, weight, groups, nullptr, out, d->tokens, d->tokens, d->x_stride, 0, num_groups, d->n, d->k, status};
+  GroupedArgs a = with_low({x, weight, groups, nullptr, out, d->tokens, d->tokens, d->x_stride, 0, num_groups, d->n, d->k, status}, d, const_cast<void*>(ws));
   a.plan = plan;
   a.group_adapters = group_adapters;
   a.ids = ids;
   a.up = up;
-  a.low = low;
   a.adapters = d->adapters;
   a.rank = d->rank;
-  a.low_width = low_width;
   if (d->type == FLEXSPMV_TYPE_BF16) return grouped_launch<__nv_bfloat16, __nv_bfloat16, kGroupedForward, false, kAddLow>(a, st);
   return grouped_launch<__half, __half, kGroupedForward, false, kAddLow>(a, st);
 }
 
-int low_product_of_many(const flexspmv_adapter_desc* d, const void* x, const void* down, const float* scale, const int* offsets, const int* rows, void* low,
-                        int low_width, int* status, cudaStream_t st) {
-  GroupedArgs a = {x, down, offsets, rows, low, d->tokens, d->tokens, d->x_stride, 0, d->adapters, d->rank, d->k, status};
-  a.low_width = low_width;
+int low_product_of_many(const flexspmv_adapter_desc* d, const void* x, const void* down, const float* scale, const int* offsets, const int* rows, void* ws,
+                        int* status, cudaStream_t st) {
+  GroupedArgs a = with_low({x, down, offsets, rows, ws, d->tokens, d->tokens, d->x_stride, 0, d->adapters, d->rank, d->k, status}, d, ws);
   a.scale = scale;
   if (d->type == FLEXSPMV_TYPE_BF16) return grouped_launch<__nv_bfloat16, __nv_bfloat16, kGroupedForward, true, kMakeLow>(a, st);
   return grouped_launch<__half, __half, kGroupedForward, true, kMakeLow>(a, st);

@@ -583,8 +583,8 @@ int flexspmv_dropout(const flexspmv_rows_desc *desc, const void *const *inputs, 
  * Low-rank adapters of many requests beside a shared projection (no reference counterpart; flexspmv_b200/adapters.py is the torch side):
  *   y[t] = weight x[t] + scale[a] b[a] (a[a] x[t]),   a = ids[t]; no adapter: y[t] = weight x[t]
  * x (tokens x k), weight (n x k), a (adapters x rank x k), b (adapters x n x rank), y (tokens x n) of one 16-bit type; scale (adapters, f32) or null: ones.
- * Sums are in 32 bits, y is rounded once; scale a x is kept to its 24 bits (float16: 22, and 2^-25) and must not exceed the type's largest value.  n, k, rank and the
- * stride are multiples of 8, the matrices 16-byte aligned (FLEXSPMV_ERR_ALIGN).
+ * Sums are in 32 bits, y is rounded once; scale a x is kept to its 24 bits, whatever its size (float16: to 2^-22, and 2^-17 of the largest of 32 neighbours).  n, k, rank
+ * and the stride are multiples of 8, the matrices 16-byte aligned (FLEXSPMV_ERR_ALIGN).
  *   adapter_plan       ids (tokens, int32; -1: none) -> a plan in d_plan (_bytes, 16-byte aligned), for all projections of the tokens.  d_status (or
  *                      null) becomes FLEXSPMV_ERR_BAD_CSR where an id leaves [-1, adapters); it counts as none
  *   adapted_project    in: x, weight, a, b, scale, the plan; out: y; workspace: _bytes, 16-byte aligned.  d_status (or null) becomes
