@@ -418,19 +418,18 @@ __device__ __forceinline__ float warp_largest(float v) {
 // The softmax of a row whose part is in this warp's lanes: powers in e, their base and the factor that makes probabilities of them.  A row of -infinity
 // alone has none: its powers are 0.  `more`: other values that are added up over the lanes, in the same steps; it gets the powers first.
 template <class T, int V, int W, int N, class F>
-__device__ __forceinline__ bool softmax_of(const LanePart<T, V, W>& part, bool exact, float (&e)[V], float& base, float& factor, float (&more)[N], const F& before) {
+__device__ __forceinline__ bool softmax_of(const LanePart<T, V, W>& part, float (&e)[V], float& base, float& factor, float (&more)[N], const F& before) {
   float top = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) top = fmaxf(top, part.piece[i / W].get(i % W));
   top = warp_largest(top);
   const bool there = top > -INFINITY;
   base = there ? top : 0.f;
-  // results of 32 bits far below the largest: as in the router's gradient
+  // 32-bit logits far below the largest: as in the router's gradient
   bool far = false;
   if constexpr (std::is_same<T, float>::value)
-    if (exact)
 #pragma unroll
-      for (int i = 0; i < V; ++i) far |= part.piece[i / W].get(i % W) < base - 8.f;
+    for (int i = 0; i < V; ++i) far |= part.piece[i / W].get(i % W) < base - 8.f;
   if (far) {
 #pragma unroll
     for (int i = 0; i < V; ++i) e[i] = exp_below_exact(part.piece[i / W].get(i % W), base);
@@ -515,7 +514,7 @@ __global__ void __launch_bounds__(THREADS) balance_kernel(BalanceArgs a) {
     const LanePart<T, V, W> part = next;
     if (t + step < a.tokens) next.load(logits + (t + step) * a.stride, a.experts, lane);
     float e[V], base, factor, none[1] = {0.f};
-    there += softmax_of<T, V, W>(part, false, e, base, factor, none, [] {});
+    there += softmax_of<T, V, W>(part, e, base, factor, none, [] {});
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = fmaf(e[i], factor, acc[i]);
   }
@@ -634,7 +633,7 @@ __global__ void __launch_bounds__(256) balance_backward_kernel(BalanceGradArgs a
     else chosen = to_float(logits[t * a.stride + c.id]);
     if (t + step < a.tokens) load(t + step);
     float e[V], base, factor, sums[2] = {c.w * c.g, 0.f};
-    softmax_of<T, V, W>(part, true, e, base, factor, sums, [&] {
+    softmax_of<T, V, W>(part, e, base, factor, sums, [&] {
 #pragma unroll
       for (int i = 0; i < V; ++i) sums[1] = fmaf(e[i], count[i], sums[1]);
     });
