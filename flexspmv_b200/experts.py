@@ -346,15 +346,16 @@ def balance_loss(logits: torch.Tensor, plan: Plan) -> Balance:
     stride = _rows_of(logits, "logits", aligned=False)
     d = Desc(tokens, 0, experts, 0, 0, 0, _TYPE[logits.dtype], 0, 0, 0, stride)
     need = _balance_bytes(tokens, experts, dev)
-    # one allocation: loss, tokens, mean and counts, then the workspace on 16 bytes
-    at = (2 * experts + 2 + 3) // 4 * 4
-    buf = torch.empty(at + need // 4, dtype=torch.int32, device=logits.device)
-    reals = buf.view(torch.float32)
-    out = Balance(reals[0], buf[2 + experts:2 + 2 * experts], reals[2:2 + experts], buf[1])
+    # The loss is what a training step goes on with, and may write to: no view.  The rest is small beside the workspace and one allocation: tokens, mean and
+    # counts.
+    loss, ws = torch.empty((), dtype=torch.float32, device=logits.device), torch.empty(need // 4, dtype=torch.int32, device=logits.device)
+    buf = torch.empty(1 + 2 * experts, dtype=torch.int32, device=logits.device)
+    out = Balance(loss, buf[1 + experts:], buf.view(torch.float32)[1:1 + experts], buf[0])
     base = buf.data_ptr()
-    ins, outs = (_P * 2)(logits.data_ptr(), plan.offsets.data_ptr()), (_P * 4)(base, base + 8 + 4 * experts, base + 8, base + 4)
-    return BoundCall(_function("balance_loss", _WITH_WORKSPACE), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), base + 4 * at, need), dev,
-                     (d, ins, outs, logits, plan, buf), out)
+    ins = (_P * 2)(logits.data_ptr(), plan.offsets.data_ptr())
+    outs = (_P * 4)(loss.data_ptr(), base + 4 + 4 * experts, base + 4, base)
+    return BoundCall(_function("balance_loss", _WITH_WORKSPACE), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), ws.data_ptr(), need), dev,
+                     (d, ins, outs, logits, plan, buf, ws, loss), out)
 
 
 @_operator

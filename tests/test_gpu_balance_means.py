@@ -54,3 +54,20 @@ def test_tokens_on_several_devices(dtype):
     mean = sum(b.mean * b.tokens for b in made) / tokens
     loss = 40.0 / counts.sum() * (counts * mean).sum()
     assert abs(float(loss) - float(whole.loss)) <= 300 * U * float(loss)
+
+
+def test_a_loss_may_be_added_to():
+    """In place, as training steps do; and no result of the call keeps its workspace."""
+    from flexspmv_b200.expert_layer import route_balanced
+    logits = torch.randn((5000, 256), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").requires_grad_()
+    plan, even = route_balanced(logits, 2)
+    want, = torch.autograd.grad(3.0 * even.loss + plan.weights.sum(), logits)
+    plan, even = route_balanced(logits, 2)
+    loss = even.loss
+    loss *= 3.0
+    loss += plan.weights.sum()
+    loss.backward()
+    assert torch.equal(logits.grad, want)
+    bound = experts.bind(experts.balance_loss, logits.detach(), plan._replace(weights=plan.weights.detach()))
+    held = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in bound.outputs}
+    assert sum(held.values()) == 4 * (2 + 2 * 256)
