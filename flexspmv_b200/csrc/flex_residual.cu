@@ -586,6 +586,7 @@ __global__ void __launch_bounds__(AHEAD ? kAheadGradThreads : row_threads(TPR), 
         for (int i = 0; i < V; ++i) d[i].load(static_cast<const T*>(a.dsum) + r * a.dsum_stride, first_column<C, S, TPR>(i, at), a.width);
     }
     Two one(0.f), two(0.f);
+    const bool beyond = !(fabsf(mean * rstd) <= 3.402823466e38f);          // what lies beyond the width would be infinite then, and 0 times that
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float w[C];
@@ -593,6 +594,10 @@ __global__ void __launch_bounds__(AHEAD ? kAheadGradThreads : row_threads(TPR), 
       else load_params<T, C, WIDE, S>(a.weight, a.wide_params, first_column<C, S, TPR>(i, at), a.width, 1.f, w);
       x[i].get(n[i]);
       dy[i].get(g[i]);
+      if (beyond)
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+          if (first_column<C, S, TPR>(i, at) + j * S >= a.width) n[i][j] = mean;
 #pragma unroll
       for (int j = 0; j < C; j += 2) {
         const Two normed = (Two(n[i] + j) + Two(-mean)) * Two(rstd), y(g[i] + j), scaled = y * Two(w + j);          // beyond the width y is 0
