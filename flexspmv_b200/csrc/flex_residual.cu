@@ -313,12 +313,61 @@ struct NormArgs {
   uint32_t below;
 };
 
+// Rows whose sum, or whose differences' squares, leave 32 bits: their rstd is 0 or no number.  After all rows, from memory once more, with sums of values that are so much
+// smaller that none leaves (less than 2^-149 of them does not show there).  A function of its own, since its registers cost all rows (us, 16384 of 4096 with dropout
+// and sum: without it 91.6, this 92.0, as part of the kernel 94.1, where such a row is met 111).
+constexpr float kMostSum = 3.402823466e38f;
+template <class T, int TPR>
+__device__ __noinline__ void large_rows(const NormArgs& a, long long from, long long step, int at, float (*buf)[1][32], int& turn, int barrier) {
+  constexpr float kSmall = 0x1p-60f, kLarge = 0x1p60f, kSmaller = 0x1p-80f;
+  if constexpr (TPR > 32) named_bar_sync(barrier, TPR);
+  else __syncwarp();
+  const Random<> random(a.seed, a.seed != nullptr);
+  const float inverse = 1.f / (float)a.width;
+#pragma unroll 1
+  for (long long r = from; r < a.rows; r += step) {
+    if (a.rstd[r] > 0.f) continue;
+    const T* const x = static_cast<const T*>(a.x) + r * a.x_stride;
+    const T* const t = a.residual ? static_cast<const T*>(a.residual) + r * a.residual_stride : nullptr;
+    const auto sum_at = [&](int c) {
+      const float v = to_float(x[c]), s = t ? to_float(t[c]) : 0.f;
+      if (!a.seed) return s + v;
+      uint32_t w[4];
+      random.words((uint32_t)(c / 4), (uint32_t)r, w);
+      return (c % 4 == 0 ? w[0] : c % 4 == 1 ? w[1] : c % 4 == 2 ? w[2] : w[3]) >= a.below ? fmaf(v, a.scale, s) : s;
+    };
+    float total[1] = {0.f};
+#pragma unroll 1
+    for (int c = at; c < a.width; c += TPR) total[0] = fmaf(sum_at(c), kSmall, total[0]);
+    row_sums<TPR>(total, buf, turn, barrier);
+    const float mean = total[0] * inverse * kLarge;
+    total[0] = 0.f;
+#pragma unroll 1
+    for (int c = at; c < a.width; c += TPR) {
+      const float d = (sum_at(c) - mean) * kSmaller;
+      total[0] = fmaf(d, d, total[0]);
+    }
+    row_sums<TPR>(total, buf, turn, barrier);
+    const float rstd = inverse_root(fmaf(total[0], inverse, a.eps * kSmaller * kSmaller)) * kSmaller;
+    if (at == 0) {
+      a.mean[r] = mean;
+      a.rstd[r] = rstd;
+    }
+    const auto param = [&](const void* p, int c, float none) {
+      return !p ? none : a.wide_params ? static_cast<const float*>(p)[c] : to_float(static_cast<const T*>(p)[c]);
+    };
+#pragma unroll 1
+    for (int c = at; c < a.width; c += TPR)
+      static_cast<T*>(a.y)[r * a.width + c] = from_float<T>(fmaf((sum_at(c) - mean) * rstd, param(a.weight, c, 1.f), param(a.bias, c, 0.f)));
+  }
+}
+
 // y = (s - mean) rstd weight + bias, s = residual + dropout(x).  Bound by memory: TPR threads hold a row in registers, L values each, so that every
 // array is read or written once; the variance is the mean square of the differences, from the registers too.  Statistics and sums in 32 bits; s is
 // normalised as it is there and rounded only where it is stored.  AHEAD: 0 (a CTA a row, or a warp), or the arrays that are read, whose rows are copied ahead.
 constexpr int kAheadThreads = 1024;
 template <class T, int C, bool WIDE, int L, int TPR, bool DROP, int AHEAD>
-__global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEAD ? 1 : 1024 / row_threads(TPR)) layer_norm_kernel(NormArgs a) {
+__global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEAD ? 1 : 1024 / row_threads(TPR)) layer_norm_kernel(const __grid_constant__ NormArgs a) {
   constexpr int S = apart_by(WIDE, DROP, TPR), V = L / C, kThreads = AHEAD ? kAheadThreads : row_threads(TPR), kRows = kThreads / TPR;
   extern __shared__ __align__(16) unsigned char rows_sm[];
   __shared__ __align__(16) float buf[kRows][2][1][32];
@@ -355,6 +404,7 @@ __global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEA
       }
     __syncthreads();
   }
+  bool large = false;
   for (long long r = from; r < a.rows; r += step) {
     float s[V][C];
     Values<T, C, WIDE, S> x[V], t[V];
@@ -409,6 +459,7 @@ __global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEA
         }
     total[0] = two.a + two.b;
     row_sums<TPR>(total, buf[group], turn, barrier);
+    large |= !(total[0] <= kMostSum);
     const float rstd = inverse_root(fmaf(total[0], inverse, a.eps));
     if (at == 0) {
       a.mean[r] = mean;
@@ -430,16 +481,18 @@ __global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEA
       store_values<T, C, WIDE, S>(static_cast<T*>(a.y) + r * a.width, c, a.width, s[i]);
     }
   }
+  if (large) large_rows<T, TPR>(a, from, step, at, buf[group], turn, barrier);
 }
 
 // Rows beyond what registers hold: the row is read three times, from L2 as a rule.
 template <class T, int C, bool WIDE>
-__global__ void __launch_bounds__(1024) layer_norm_long_kernel(NormArgs a) {
+__global__ void __launch_bounds__(1024) layer_norm_long_kernel(const __grid_constant__ NormArgs a) {
   __shared__ __align__(16) float buf[2][1][32];
   int turn = 0;
   pdl_wait();
   const Random<> random(a.seed, a.seed != nullptr);
   const float inverse = 1.f / (float)a.width;
+  bool large = false;
   for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const auto sum_at = [&](int c, float (&s)[C]) {
       load_values<T, C, WIDE>(static_cast<const T*>(a.x) + r * a.x_stride, c, a.width, s);
@@ -476,6 +529,7 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(NormArgs a) {
         if (c + j < a.width) total[0] = fmaf(s[j] - mean, s[j] - mean, total[0]);
     }
     row_sums<1024>(total, buf, turn, 1);
+    large |= !(total[0] <= kMostSum);
     const float rstd = inverse_root(fmaf(total[0], inverse, a.eps));
     if (threadIdx.x == 0) {
       a.mean[r] = mean;
@@ -491,6 +545,7 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(NormArgs a) {
       store_values<T, C, WIDE>(static_cast<T*>(a.y) + r * a.width, c, a.width, s);
     }
   }
+  if (large) large_rows<T, 1024>(a, blockIdx.x, gridDim.x, threadIdx.x, buf, turn, 1);
 }
 
 // ---- gradients -----------------------------------------------------------------------------------------------------
