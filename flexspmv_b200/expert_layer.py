@@ -167,7 +167,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[t
 
 def sum_norm(x: torch.Tensor, stream: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float = 1e-5, p: float = 0.0,
              seed: Optional[torch.Tensor] = None):
-    """``stream + dropout(x)`` and its norm, with gradients.  ``seed`` must hold the same two values until the backward pass: give it a copy of one that is raised."""
+    """``stream + dropout(x)`` and its norm, with gradients.  ``seed`` must hold the same two values until the backward pass: give it a copy of one that is raised.
+
+    The norm is of the sum as it is in 32 bits; what is kept of it for the backward pass is the sum that is returned, rounded to the rows' type.  In 16 bits the
+    gradients are those of normalised values that are off by that rounding over the row's deviation: a 256th (bfloat16) of |s| / deviation at the most."""
     return _SumNorm.apply(x, stream, weight, bias, eps, p, seed)
 
 

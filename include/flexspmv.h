@@ -569,7 +569,9 @@ typedef struct flexspmv_rows_desc {
  *                      s = residual + dropout(x), mean and rstd = 1 / sqrt(variance + eps) of its rows (f32), y = (s - mean) rstd weight + bias
  * layer_norm_backward  in: dy, x (what was normalised: s), weight, mean, rstd, dsum (or null), seed; strides: dy, x, dsum;
  *                      out: dx (p > 0), dresidual, dweight, dbias (both or neither null).
- *                      dresidual = rstd (g - mean(g) - n mean(g n)) + dsum with n = (x - mean) rstd, g = dy weight;  dx = its values that were kept, scaled
+ *                      dresidual = rstd (g - mean(g) - n mean(g n)) + dsum with n = (x - mean) rstd, g = dy weight;  dx = its values that were kept, scaled.
+ *                      With x the sum that layer_norm has rounded and mean, rstd those that it gave, which are of the sum before its rounding, n is off by that
+ *                      rounding times rstd.
  *                      Workspace (_bytes, 16-byte aligned) where dweight is wanted.
  * dropout              in: x, residual (or null), seed; strides: x, residual; out: residual + dropout(x)
  */
