@@ -11,8 +11,8 @@ namespace flex {
 
 // A place's vector scale A x, a sum of 32 bits, is kept as 16-bit values that add up to it, which the matrix instructions take as they are: three bfloat16
 // have all 24 of its bits; two float16 22 of them, which is 2^-11 of what y's own rounding takes.  (Two bfloat16, 17 bits, made 1.1 of 1000 values of y another
-// one than the 32-bit vector does.)  us, two / three: 8192 tokens of rank 64 (4096 x 4096, 12 runs) 223 / 227, 2000 in 5 runs 80.5 / 82, 300 of rank 16 in
-// short runs 42 / 46, 48 of rank 16 14.6 / 14.7.
+// one than the 32-bit vector does.)  us, two / three: 8192 tokens of rank 64 (4096 x 4096, 12 runs) 223 / 227, 300 of rank 16 in short runs 36.4 / 37.4, 48 of
+// rank 16 14.6 / 15.2.
 // In a row: ranks up to 16: a part behind the other, 16 values each; up to 32: 32 each; else 64 of the vector at a time, their parts behind one another.  Rows
 // are whole steps of 64 values.
 template <class T> constexpr int kLowParts = std::is_same<T, __nv_bfloat16>::value ? 3 : 2;

@@ -168,6 +168,69 @@ __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const Group
 struct LowPart {
   float low[16], high[16];
 };
+// An adapter of at most kFewPlaces of the places, `mine`: their parts beside one another in the instruction's eight columns, so that it takes one instruction where
+// low_rank_part takes one for each part and each eight places.  us, without / with: 300 tokens, each with its own adapter of rank 16 (4096 x 4096) 96 / 60, of
+// rank 64 173 / 126, in float16 of rank 16 75 / 62; 600 of rank 128 in 50 runs 61 / 52, 1000 of rank 32 in 40 runs 59 / 56.
+template <class T> constexpr int kFewPlaces = kLowParts<T> == 2 ? 4 : 2;
+template <class T>
+__device__ __forceinline__ void low_rank_few(const GroupedArgs& a, const T* up, int m, int place, unsigned mine, int lane, LowPart& r) {
+  constexpr int kPlaces = kFewPlaces<T>, kEach = 8 / kPlaces;
+  const int q = lane & 3, g = lane >> 2;
+  unsigned from = mine;
+  for (int i = 0; i < g / kEach; ++i) from &= from - 1;
+  const bool there = from != 0 && g % kEach < kLowParts<T>;          // this lane's column has a place
+  const T* const row = static_cast<const T*>(a.low) + (size_t)(place + (there ? __ffs(from) - 1 : 0)) * a.low_width;
+  float d[2][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) d[i / 4][i % 4] = 0.f;
+  if (a.rank <= 16) {
+    const int k = q * 4;
+    uint2 w[4], h = make_uint2(0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = make_uint2(0, 0);
+      if (k < a.rank && m + g + i * 8 < a.n) w[i] = *reinterpret_cast<const uint2*>(up + (size_t)i * 8 * a.rank + k);
+    }
+    if (there && k < a.rank) h = *reinterpret_cast<const uint2*>(row + low_at<T>(k, a.rank, g % kEach));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) warp_mma<T>(d[i], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h.x, h.y);
+  } else {
+#pragma unroll 2
+    for (int k = q * 8; k - q * 8 < a.rank; k += 32) {
+      uint4 w[4], h = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = make_uint4(0, 0, 0, 0);
+        if (k < a.rank && m + g + i * 8 < a.n) w[i] = *reinterpret_cast<const uint4*>(up + (size_t)i * 8 * a.rank + k);
+      }
+      if (there && k < a.rank) h = *reinterpret_cast<const uint4*>(row + low_at<T>(k, a.rank, g % kEach));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        warp_mma<T>(d[i], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h.x, h.y);
+        warp_mma<T>(d[i], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, h.z, h.w);
+      }
+    }
+  }
+  float sum[4];                            // of features g, g + 8, ..
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sum[i] = d[i / 2][i % 2 * 2] + d[i / 2][i % 2 * 2 + 1];
+    if (kEach == 4) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+  }
+#pragma unroll
+  for (int i = 0; i < kPlaces; ++i) {
+    if (!mine) break;
+    const int p = __ffs(mine) - 1;
+    mine &= mine - 1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float of = __shfl_sync(0xffffffffu, sum[j], (lane & ~3) | i * kEach / 2);
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (x == ((p >> 3 << 1) | (p & 1)) && q == (p & 7) >> 1) (j < 2 ? r.low : r.high)[x / 2 * 4 + x % 2 + j % 2 * 2] = of;
+    }
+  }
+}
 template <class T>
 __device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int place, int left, int lane, LowPart& r) {
   constexpr int kParts = kLowParts<T>;
@@ -181,15 +244,32 @@ __device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int p
     const int adapter = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
     const unsigned mine = __ballot_sync(0xffffffffu, id == adapter);
     todo &= ~mine;
-    float d[2][4][4];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) d[i / 16][i / 4 % 4][i % 4] = 0.f;
     const T* const up = static_cast<const T*>(a.up) + ((size_t)adapter * a.n + m + g) * a.rank;
-    // all loads of a step under way at once
+    if (__popc(mine) <= kFewPlaces<T>) {
+      low_rank_few<T>(a, up, m, place, mine, lane, r);
+      continue;
+    }
+    // eight places at a time, or 16 where their loads are many; each part's sum by itself and then one after the other, as low_rank_few has them: what a place gets does
+    // not depend on how many others have its adapter
+    const auto take_up = [&](int b, const float (&d)[kParts][2][4]) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float sum[2] = {d[0][0][x], d[0][1][x]};
+#pragma unroll
+        for (int i = 1; i < kParts; ++i) {
+          sum[0] += d[i][0][x];
+          sum[1] += d[i][1][x];
+        }
+        if (mine >> (b * 8 + q * 2 + (x & 1)) & 1u) {
+          r.low[b * 4 + x] = sum[0];
+          r.high[b * 4 + x] = sum[1];
+        }
+      }
+    };
     if (a.rank <= 16) {
       const int k = q * 4;
       const uint2 none = make_uint2(0, 0);
-      uint2 w[4], h[4][kParts];
+      uint2 w[4], h[4][kParts];              // all loads under way at once
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         w[i] = none;
@@ -208,52 +288,57 @@ __device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int p
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         if (!(mine >> (b * 8) & 0xffu)) continue;
+        float d[kParts][2][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < kParts * 8; ++i) d[i / 8][i / 4 % 2][i % 4] = 0.f;
 #pragma unroll
-          for (int x = 0; x < kParts; ++x) warp_mma<T>(d[i][b], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h[b][x].x, h[b][x].y);
+        for (int x = 0; x < kParts; ++x)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) warp_mma<T>(d[x][i], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h[b][x].x, h[b][x].y);
+        take_up(b, d);
       }
     } else {
+#pragma unroll
+      for (int b0 = 0; b0 < 4; b0 += 2) {
+        if (!(mine >> (b0 * 8) & 0xffffu)) continue;
+        float d[2][kParts][2][4];
+#pragma unroll
+        for (int i = 0; i < kParts * 16; ++i) d[i / (kParts * 8)][i / 8 % kParts][i / 4 % 2][i % 4] = 0.f;
 #pragma unroll 1
-      for (int k = q * 8; k - q * 8 < a.rank; k += 32) {
-        const bool inside = k < a.rank;
-        uint4 w[4], h[4][kParts];
+        for (int k = q * 8; k - q * 8 < a.rank; k += 32) {
+          const bool inside = k < a.rank;
+          uint4 w[4], h[2][kParts];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[i] = make_uint4(0, 0, 0, 0);
-          if (inside && m + g + i * 8 < a.n) w[i] = *reinterpret_cast<const uint4*>(up + (size_t)i * 8 * a.rank + k);
-        }
+          for (int i = 0; i < 4; ++i) {
+            w[i] = make_uint4(0, 0, 0, 0);
+            if (inside && m + g + i * 8 < a.n) w[i] = *reinterpret_cast<const uint4*>(up + (size_t)i * 8 * a.rank + k);
+          }
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+          for (int b = 0; b < 2; ++b) {
 #pragma unroll
-          for (int x = 0; x < kParts; ++x) h[b][x] = make_uint4(0, 0, 0, 0);
-          if (inside && (mine >> (b * 8 + g) & 1u)) {
-            const T* const row = low + (size_t)b * 8 * a.low_width;
+            for (int x = 0; x < kParts; ++x) h[b][x] = make_uint4(0, 0, 0, 0);
+            if (inside && (mine >> ((b0 + b) * 8 + g) & 1u)) {
+              const T* const row = low + (size_t)(b0 + b) * 8 * a.low_width;
 #pragma unroll
-            for (int x = 0; x < kParts; ++x) h[b][x] = *reinterpret_cast<const uint4*>(row + low_at<T>(k, a.rank, x));
+              for (int x = 0; x < kParts; ++x) h[b][x] = *reinterpret_cast<const uint4*>(row + low_at<T>(k, a.rank, x));
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            if (!(mine >> ((b0 + b) * 8) & 0xffu)) continue;
+#pragma unroll
+            for (int x = 0; x < kParts; ++x)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                warp_mma<T>(d[b][x][i], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h[b][x].x, h[b][x].y);
+                warp_mma<T>(d[b][x][i], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, h[b][x].z, h[b][x].w);
+              }
           }
         }
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          if (!(mine >> (b * 8) & 0xffu)) continue;
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int x = 0; x < kParts; ++x) {
-              warp_mma<T>(d[i][b], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h[b][x].x, h[b][x].y);
-              warp_mma<T>(d[i][b], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, h[b][x].z, h[b][x].w);
-            }
-        }
+        take_up(b0, d[0]);
+        take_up(b0 + 1, d[1]);
       }
     }
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (mine >> (b * 8 + q * 2 + (x & 1)) & 1u) {
-          r.low[b * 4 + x] = d[0][b][x];
-          r.high[b * 4 + x] = d[1][b][x];
-        }
   }
 }
 

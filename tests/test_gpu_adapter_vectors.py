@@ -52,3 +52,20 @@ def test_divided_sums_that_begin_with_the_vector():
     eh = torch.einsum("tk,trk->tr", x.double().abs(), a.double().abs()[ids.long()]) * k * 2.0 ** -23
     bound = (k + 3 * rank) * 2.0 ** -23 * size + torch.einsum("tr,tnr->tn", eh, b.double().abs()[ids.long()]) + 2.0 ** -8 * 1.01 * want.abs()
     assert ((y.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,n,k,rank", [(48, 264, 200, 16), (48, 264, 200, 40), (40, 128, 2048, 16), (40, 128, 2048, 64), (700, 264, 64, 8), (700, 1000, 72, 72)])
+def test_a_token_gets_the_same_bits_whoever_shares_its_adapter(tokens, n, k, rank, dtype):
+    """One, two, some or all of the others, in a row or scattered, with the adapter's own weights under another number."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x, w, a, b = (torch.randn(s, generator=g, device="cuda").mul_(0.3).to(dtype) for s in ((tokens, k), (n, k), (8, rank, k), (8, n, rank)))
+    a[1:] = a[0]
+    b[1:] = b[0]
+    base = torch.zeros(tokens, dtype=torch.int32, device="cuda")
+    want = adapters.project(x, w, a, b, adapters.plan(base, 8))
+    r = np.random.default_rng(1)
+    for values in (np.arange(tokens) % 8, np.arange(tokens) // 2 % 8, np.arange(tokens) // 3 % 8, np.arange(tokens) // 5 % 8, r.integers(0, 8, tokens), r.integers(0, 8, tokens) // 6,
+                   r.integers(0, 8, tokens) // 7):
+        ids = torch.from_numpy(values.astype(np.int32)).cuda()
+        assert torch.equal(adapters.project(x, w, a, b, adapters.plan(ids, 8)), want)
