@@ -25,8 +25,9 @@ constexpr int kLowTile = 16;
 // Tokens up to which they are one group; us, one / several: 1500 tokens in runs of 300 (2048 x 2048, rank 32) 29.9 / 33.2, 2000 in runs of 400 (4096 x 4096, rank 64) 83 / 77.
 constexpr long long kOneGroup = 1536;
 constexpr long long kLowTiles = 4096;        // tokens up to which the first product may be in tiles
-// ... and is: an adapter is read again for every 16 tokens.  us, both products, tiles / the grouped kernel: 600 tokens of rank 128 (50 adapters, 2000 x 2000) 55.2 / 44.9,
-// 2000 of rank 64 60.1 / 45.3; 1500 of rank 16 34.9, 300 of rank 64 (4096 x 1000) 22.3 in tiles.
+// ... and is: an adapter is read again for every 16 tokens.  us, both products (2048 x 2048, runs of 10 to 100 tokens), tiles / the grouped kernel: rank 16, 100 tokens
+// 13.6 / 21.3, 600 24.6 / 27.6, 1500 33.3 / 31.1, 2000 38.1 / 43.5, 4000 57.5 / 52.3; rank 64, 300 26.9 / 29.1, 500 28.9 / 32.7, 600 36.5 / 38.6, 2000 65.6 / 59.5; rank 128, 250
+// 60.8 / 52.7, 600 59.8 / 51.9.
 static bool low_in_tiles(long long tokens, int rank) { return tokens <= kLowTiles && tokens * rank <= 32768; }
 // us, runs of 100 and 200 tokens: from 64 on 54.7 and 41.2 (3000 tokens, 2048 x 2048, ranks 32 and 64), from 128 on 50.3 and 41.0, from 256 on 50.2 and 54.9.
 constexpr int kLongRun = 128;

@@ -826,7 +826,8 @@ static int route_typed(const RouteArgs& a, cudaStream_t st) {
 }
 
 // Clusters of the balance loss: a few tokens a warp, up to one CTA an SM.
-// Tokens up to which one CTA does it all; us, one / two launches: 48 tokens of 64 experts 3.3 / 6.3, 128 3.9 / 6.3, 128 of 384 5.8 / 7.4, 300 of 128 8.2 / 6.8.
+// Tokens up to which one CTA does it all, half as many where it has half the threads; us, one / two launches: 48 tokens of 64 experts 3.0 / 5.8, 128 5.1 / 5.3, 200
+// 7.0 / 5.4; 128 of 256 5.2 / 6.6, 200 6.8 / 6.8; 128 of 384 5.7 / 6.2, 200 7.8 / 6.1; 64 of 1024 9.0 / 9.1, 128 14.5 / 9.5.
 constexpr long long kBalanceSmall = 128;
 static int balance_clusters(long long tokens) {
   const long long want = (tokens + 63) / 64;
@@ -838,8 +839,8 @@ template <class T, int V, int W>
 static int balance_launch(const BalanceArgs& a, cudaStream_t st) {
   constexpr int kThreads = V <= 8 ? 1024 : V <= 16 ? 512 : 256;          // 32 KB for the warps' sums at the most
   const size_t smem = (size_t)a.experts * (kThreads / 32) * 4;
-  if (a.tokens <= kBalanceSmall) {
-    constexpr int kFew = V <= 12 ? 512 : 256;
+  constexpr int kFew = V <= 12 ? 512 : 256;
+  if (a.tokens <= kBalanceSmall * kFew / 512) {
     return launch_pdl(balance_kernel<T, V, W, kFew, true>, 1, kFew, (size_t)a.experts * (kFew / 32) * 4, st, a);
   }
   const int clusters = balance_clusters(a.tokens);
