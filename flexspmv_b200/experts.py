@@ -346,16 +346,14 @@ def balance_loss(logits: torch.Tensor, plan: Plan) -> Balance:
     stride = _rows_of(logits, "logits", aligned=False)
     d = Desc(tokens, 0, experts, 0, 0, 0, _TYPE[logits.dtype], 0, 0, 0, stride)
     need = _balance_bytes(tokens, experts, dev)
-    # The loss is what a training step goes on with, and may write to: no view.  The rest is small beside the workspace and one allocation: tokens, mean and
-    # counts.
-    loss, ws = torch.empty((), dtype=torch.float32, device=logits.device), torch.empty(need // 4, dtype=torch.int32, device=logits.device)
-    buf = torch.empty(1 + 2 * experts, dtype=torch.int32, device=logits.device)
-    out = Balance(loss, buf[1 + experts:], buf.view(torch.float32)[1:1 + experts], buf[0])
-    base = buf.data_ptr()
-    ins = (_P * 2)(logits.data_ptr(), plan.offsets.data_ptr())
-    outs = (_P * 4)(loss.data_ptr(), base + 4 + 4 * experts, base + 4, base)
+    # no views: a training step may add to its loss, and no result keeps the workspace
+    empty, device = torch.empty, logits.device
+    out = Balance(empty((), dtype=torch.float32, device=device), empty(experts, dtype=torch.int32, device=device),
+                  empty(experts, dtype=torch.float32, device=device), empty((), dtype=torch.int32, device=device))
+    ws = empty(need, dtype=torch.uint8, device=device)
+    ins, outs = (_P * 2)(logits.data_ptr(), plan.offsets.data_ptr()), (_P * 4)(*[t.data_ptr() for t in out])
     return BoundCall(_function("balance_loss", _WITH_WORKSPACE), (ctypes.addressof(d), ctypes.addressof(ins), ctypes.addressof(outs), ws.data_ptr(), need), dev,
-                     (d, ins, outs, logits, plan, buf, ws, loss), out)
+                     (d, ins, outs, logits, plan, ws, out), out)
 
 
 @_operator

@@ -158,8 +158,9 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
     dx = torch.empty_like(dresidual) if p > 0.0 else dresidual
     dweight = dbias = ws = None
     need = 0
-    if weight is not None or bias is not None:
-        dweight, dbias = (torch.empty_like(weight if weight is not None else bias) for _ in range(2))
+    of = weight if weight is not None else bias
+    if of is not None:
+        dweight, dbias = torch.empty_like(of), torch.empty_like(of)
         need = _backward_bytes(rows, width, dev)
         ws = dy.new_empty(need, dtype=torch.uint8)
     out = NormGradients(dx, dresidual, dweight if weight is not None else None, dbias)
