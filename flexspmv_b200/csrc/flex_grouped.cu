@@ -168,66 +168,69 @@ __device__ __forceinline__ GroupedTile tile_at(const GroupedArgs& a, const Group
 struct LowPart {
   float low[16], high[16];
 };
-// An adapter of at most kFewPlaces of the places, `mine`: their parts beside one another in the instruction's eight columns, so that it takes one instruction where
-// low_rank_part takes one for each part and each eight places.  us, without / with: 300 tokens, each with its own adapter of rank 16 (4096 x 4096) 96 / 60, of
-// rank 64 173 / 126, in float16 of rank 16 75 / 62; 600 of rank 128 in 50 runs 61 / 52, 1000 of rank 32 in 40 runs 59 / 56.
+// An adapter of few of the places, `mine`: their parts beside one another in the instruction's eight columns, kFewPlaces at a time, so that it takes one instruction
+// where low_rank_part takes one for each part and each eight places.  us, without / with: 300 tokens, each with its own adapter of rank 16 (4096 x 4096) 96 / 60, of rank
+// 64 173 / 126, in float16 of rank 16 75 / 62; 600 of rank 128 in 50 runs 61 / 52, 1000 of rank 32 in 40 runs 59 / 56.  In more than one round only for ranks whose loads are
+// several and where the places are scattered: 300 tokens with ten adapters of rank 64 in turn (4096 x 1000) 76 / 55, but 1100 with ten of rank 16 85 / 93.
 template <class T> constexpr int kFewPlaces = kLowParts<T> == 2 ? 4 : 2;
 template <class T>
 __device__ __forceinline__ void low_rank_few(const GroupedArgs& a, const T* up, int m, int place, unsigned mine, int lane, LowPart& r) {
   constexpr int kPlaces = kFewPlaces<T>, kEach = 8 / kPlaces;
   const int q = lane & 3, g = lane >> 2;
-  unsigned from = mine;
-  for (int i = 0; i < g / kEach; ++i) from &= from - 1;
-  const bool there = from != 0 && g % kEach < kLowParts<T>;          // this lane's column has a place
-  const T* const row = static_cast<const T*>(a.low) + (size_t)(place + (there ? __ffs(from) - 1 : 0)) * a.low_width;
-  float d[2][4];
+  while (mine) {
+    unsigned from = mine;
+    for (int i = 0; i < g / kEach; ++i) from &= from - 1;
+    const bool there = from != 0 && g % kEach < kLowParts<T>;          // this lane's column has a place
+    const T* const row = static_cast<const T*>(a.low) + (size_t)(place + (there ? __ffs(from) - 1 : 0)) * a.low_width;
+    float d[2][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) d[i / 4][i % 4] = 0.f;
-  if (a.rank <= 16) {
-    const int k = q * 4;
-    uint2 w[4], h = make_uint2(0, 0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i] = make_uint2(0, 0);
-      if (k < a.rank && m + g + i * 8 < a.n) w[i] = *reinterpret_cast<const uint2*>(up + (size_t)i * 8 * a.rank + k);
-    }
-    if (there && k < a.rank) h = *reinterpret_cast<const uint2*>(row + low_at<T>(k, a.rank, g % kEach));
-#pragma unroll
-    for (int i = 0; i < 2; ++i) warp_mma<T>(d[i], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h.x, h.y);
-  } else {
-#pragma unroll 2
-    for (int k = q * 8; k - q * 8 < a.rank; k += 32) {
-      uint4 w[4], h = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < 8; ++i) d[i / 4][i % 4] = 0.f;
+    if (a.rank <= 16) {
+      const int k = q * 4;
+      uint2 w[4], h = make_uint2(0, 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        w[i] = make_uint4(0, 0, 0, 0);
-        if (k < a.rank && m + g + i * 8 < a.n) w[i] = *reinterpret_cast<const uint4*>(up + (size_t)i * 8 * a.rank + k);
+        w[i] = make_uint2(0, 0);
+        if (k < a.rank && m + g + i * 8 < a.n) w[i] = *reinterpret_cast<const uint2*>(up + (size_t)i * 8 * a.rank + k);
       }
-      if (there && k < a.rank) h = *reinterpret_cast<const uint4*>(row + low_at<T>(k, a.rank, g % kEach));
+      if (there && k < a.rank) h = *reinterpret_cast<const uint2*>(row + low_at<T>(k, a.rank, g % kEach));
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        warp_mma<T>(d[i], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h.x, h.y);
-        warp_mma<T>(d[i], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, h.z, h.w);
+      for (int i = 0; i < 2; ++i) warp_mma<T>(d[i], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h.x, h.y);
+    } else {
+#pragma unroll 2
+      for (int k = q * 8; k - q * 8 < a.rank; k += 32) {
+        uint4 w[4], h = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] = make_uint4(0, 0, 0, 0);
+          if (k < a.rank && m + g + i * 8 < a.n) w[i] = *reinterpret_cast<const uint4*>(up + (size_t)i * 8 * a.rank + k);
+        }
+        if (there && k < a.rank) h = *reinterpret_cast<const uint4*>(row + low_at<T>(k, a.rank, g % kEach));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          warp_mma<T>(d[i], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, h.x, h.y);
+          warp_mma<T>(d[i], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, h.z, h.w);
+        }
       }
     }
-  }
-  float sum[4];                            // of features g, g + 8, ..
+    float sum[4];                            // of features g, g + 8, ..
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    sum[i] = d[i / 2][i % 2 * 2] + d[i / 2][i % 2 * 2 + 1];
-    if (kEach == 4) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-  }
+    for (int i = 0; i < 4; ++i) {
+      sum[i] = d[i / 2][i % 2 * 2] + d[i / 2][i % 2 * 2 + 1];
+      if (kEach == 4) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+    }
 #pragma unroll
-  for (int i = 0; i < kPlaces; ++i) {
-    if (!mine) break;
-    const int p = __ffs(mine) - 1;
-    mine &= mine - 1;
+    for (int i = 0; i < kPlaces; ++i) {
+      if (!mine) break;
+      const int p = __ffs(mine) - 1;
+      mine &= mine - 1;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float of = __shfl_sync(0xffffffffu, sum[j], (lane & ~3) | i * kEach / 2);
+      for (int j = 0; j < 4; ++j) {
+        const float of = __shfl_sync(0xffffffffu, sum[j], (lane & ~3) | i * kEach / 2);
 #pragma unroll
-      for (int x = 0; x < 8; ++x)
-        if (x == ((p >> 3 << 1) | (p & 1)) && q == (p & 7) >> 1) (j < 2 ? r.low : r.high)[x / 2 * 4 + x % 2 + j % 2 * 2] = of;
+        for (int x = 0; x < 8; ++x)
+          if (x == ((p >> 3 << 1) | (p & 1)) && q == (p & 7) >> 1) (j < 2 ? r.low : r.high)[x / 2 * 4 + x % 2 + j % 2 * 2] = of;
+      }
     }
   }
 }
@@ -245,7 +248,11 @@ __device__ __forceinline__ void low_rank_part(const GroupedArgs& a, int m, int p
     const unsigned mine = __ballot_sync(0xffffffffu, id == adapter);
     todo &= ~mine;
     const T* const up = static_cast<const T*>(a.up) + ((size_t)adapter * a.n + m + g) * a.rank;
-    if (__popc(mine) <= kFewPlaces<T>) {
+    int eights = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) eights += (mine >> (b * 8) & 0xffu) != 0;
+    const int rounds = (__popc(mine) + kFewPlaces<T> - 1) / kFewPlaces<T>;
+    if (rounds == 1 || (a.rank > 16 && rounds < eights)) {
       low_rank_few<T>(a, up, m, place, mine, lane, r);
       continue;
     }
