@@ -314,11 +314,11 @@ struct NormArgs {
 };
 
 // Rows whose sum, or whose differences' squares, leave 32 bits: their rstd is 0 or no number.  After all rows, from memory once more, with sums of values that are so much
-// smaller that none leaves (less than 2^-149 of them does not show there).  A function of its own, since its registers cost all rows (us, 16384 of 4096 with dropout
-// and sum: without it 91.6, this 92.0, as part of the kernel 94.1, where such a row is met 111).
+// smaller that none leaves (less than 2^-149 of them does not show there).  us, 16384 rows of 4096 with dropout and sum, without it 91.3, as a function 91.7, as part of the
+// kernel 94.1, where such a row is met 111; elsewhere a function's registers cost more than it saves (4000 rows of 20 000: without 360, part of the kernel 363, function 414).
 constexpr float kMostSum = 3.402823466e38f;
 template <class T, int TPR>
-__device__ __noinline__ void large_rows(const NormArgs& a, long long from, long long step, int at, float (*buf)[1][32], int& turn, int barrier) {
+__device__ __forceinline__ void large_rows(const NormArgs& a, long long from, long long step, int at, float (*buf)[1][32], int& turn, int barrier) {
   constexpr float kSmall = 0x1p-60f, kLarge = 0x1p60f, kSmaller = 0x1p-80f;
   if constexpr (TPR > 32) named_bar_sync(barrier, TPR);
   else __syncwarp();
@@ -360,6 +360,11 @@ __device__ __noinline__ void large_rows(const NormArgs& a, long long from, long 
     for (int c = at; c < a.width; c += TPR)
       static_cast<T*>(a.y)[r * a.width + c] = from_float<T>(fmaf((sum_at(c) - mean) * rstd, param(a.weight, c, 1.f), param(a.bias, c, 0.f)));
   }
+}
+
+template <class T, int TPR>
+__device__ __noinline__ void large_rows_apart(const NormArgs& a, long long from, long long step, int at, float (*buf)[1][32], int& turn, int barrier) {
+  large_rows<T, TPR>(a, from, step, at, buf, turn, barrier);
 }
 
 // y = (s - mean) rstd weight + bias, s = residual + dropout(x).  Bound by memory: TPR threads hold a row in registers, L values each, so that every
@@ -481,12 +486,15 @@ __global__ void __launch_bounds__(AHEAD ? kAheadThreads : row_threads(TPR), AHEA
       store_values<T, C, WIDE, S>(static_cast<T*>(a.y) + r * a.width, c, a.width, s[i]);
     }
   }
-  if (large) large_rows<T, TPR>(a, from, step, at, buf[group], turn, barrier);
+  if (large) {
+    if constexpr (WIDE && DROP && AHEAD > 0) large_rows_apart<T, TPR>(a, from, step, at, buf[group], turn, barrier);
+    else large_rows<T, TPR>(a, from, step, at, buf[group], turn, barrier);
+  }
 }
 
 // Rows beyond what registers hold: the row is read three times, from L2 as a rule.
 template <class T, int C, bool WIDE>
-__global__ void __launch_bounds__(1024) layer_norm_long_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(1024) layer_norm_long_kernel(NormArgs a) {
   __shared__ __align__(16) float buf[2][1][32];
   int turn = 0;
   pdl_wait();

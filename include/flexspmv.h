@@ -566,7 +566,8 @@ typedef struct flexspmv_rows_desc {
 
 /*
  * layer_norm           in: x, residual (or null), weight, bias (or null: 1, 0), seed; strides: x, residual; out: y, sum (or null), mean, rstd
- *                      s = residual + dropout(x), mean and rstd = 1 / sqrt(variance + eps) of its rows (f32), y = (s - mean) rstd weight + bias
+ *                      s = residual + dropout(x), mean and rstd = 1 / sqrt(variance + eps) of its rows (f32), y = (s - mean) rstd weight + bias;
+ *                      values of s of any size up to 2^126
  * layer_norm_backward  in: dy, x (what was normalised: s), weight, mean, rstd, dsum (or null), seed; strides: dy, x, dsum;
  *                      out: dx (p > 0), dresidual, dweight, dbias (both or neither null).
  *                      dresidual = rstd (g - mean(g) - n mean(g n)) + dsum with n = (x - mean) rstd, g = dy weight;  dx = its values that were kept, scaled.
