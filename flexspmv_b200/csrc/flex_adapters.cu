@@ -22,7 +22,9 @@ struct AdapterTile {
 // Where a plan's parts lie, in ints; it begins with the number of tiles, the tokens and the adapters that it is of.  Groups: for the shared product of many tokens, runs of one adapter that are long enough for tiles of
 // their own, and what lies between them.
 constexpr int kLowTile = 16;
-// Tokens up to which they are one group; us, one / several: 1500 tokens in runs of 300 (2048 x 2048, rank 32) 29.9 / 33.2, 2000 in runs of 400 (4096 x 4096, rank 64) 83 / 77.
+// Tokens up to which they are one group, whose tiles go round the SMs better than those of many short groups; us, one / several: 900 tokens of rank 64 in 60 runs (2048 x 2048,
+// float16) 36 / 47, 1000 of rank 32 in 40 (4096 x 4096) 57 / 64, 1031 of rank 8 in 40 (1000 x 1416) 19.5 / 20.1, but 600 of rank 128 with one adapter (2000 x 2000) 37 / 23, 1400 of rank 64 in
+// 20 runs (5000 x 1024) 67 / 53, 2000 in runs of 400 (4096 x 4096) 83 / 77.
 constexpr long long kOneGroup = 1536;
 constexpr long long kLowTiles = 4096;        // tokens up to which the first product may be in tiles
 // ... and is: an adapter is read again for every 16 tokens.  us, both products (2048 x 2048, runs of 10 to 100 tokens), tiles / the grouped kernel: rank 16, 100 tokens
