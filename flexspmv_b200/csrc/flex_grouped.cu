@@ -179,7 +179,8 @@ __device__ __forceinline__ void low_rank_few(const GroupedArgs& a, const T* up, 
   const int q = lane & 3, g = lane >> 2;
   while (mine) {
     unsigned from = mine;
-    for (int i = 0; i < g / kEach; ++i) from &= from - 1;
+#pragma unroll
+    for (int i = 1; i < kPlaces; ++i) from = i <= g / kEach ? from & (from - 1) : from;          // no branch that lanes take apart
     const bool there = from != 0 && g % kEach < kLowParts<T>;          // this lane's column has a place
     const T* const row = static_cast<const T*>(a.low) + (size_t)(place + (there ? __ffs(from) - 1 : 0)) * a.low_width;
     float d[2][4];

@@ -258,6 +258,8 @@ class RoutedStack(nn.Module):
     def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None, seed: Optional[torch.Tensor] = None) -> Stacked:
         """``x`` (tokens, width) of the matrices' type.  ``mask`` (tokens) bool: tokens that are there; the others count as rows of zeros, whatever they hold.
         ``seed`` (two int64 values): takes the place of the stack's own, which is then neither read nor raised; layer i has its offset plus i."""
+        if seed is not None:
+            residual._vector(seed, "seed", (torch.int64,), 2, x.get_device(), "of seed and offset")
         if mask is not None:
             x = x.masked_fill(~mask[:, None], 0.0)
         all_tokens = torch.arange(2, dtype=torch.int32, device=x.device) * x.shape[0]          # made on the device: a step may be captured

@@ -74,3 +74,13 @@ def test_layers_of_a_given_seed():
     finally:
         residual.layer_norm = plain
     assert used == [[7, 40], [7, 41], [7, 42]]
+
+
+def test_what_is_no_seed():
+    stack, x = made()
+    for bad in (torch.zeros(3, dtype=torch.int64, device="cuda"), torch.zeros(2, device="cuda"), torch.zeros(2, dtype=torch.int64), 5):
+        with pytest.raises(FlexSpmvError, match="seed"):
+            stack(x, seed=bad)
+    stack.eval()
+    with pytest.raises(FlexSpmvError, match="seed"):
+        stack(x, seed=torch.zeros(1, dtype=torch.int64, device="cuda"))
