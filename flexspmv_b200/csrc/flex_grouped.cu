@@ -1230,6 +1230,14 @@ static int grouped_smem(int experts) {
          (ADAPT == kAddLow ? experts * 4 : 0);
 }
 
+// dw's maps count rows by two dimensions of one stride, y + z, of which y ends at 64 (fewer rows: with them).  z ends so that the last row of the last z is the tensor's
+// last: nothing that a map is of lies outside its tensor, whether it is copied or not.
+constexpr uint64_t dw_rows_y(uint64_t rows) { return rows < 64 ? rows : 64; }
+constexpr uint64_t dw_rows_z(uint64_t rows) { return rows - dw_rows_y(rows) + 1; }
+static_assert(dw_rows_y(1) - 1 + dw_rows_z(1) - 1 == 0 && dw_rows_y(63) - 1 + dw_rows_z(63) - 1 == 62 && dw_rows_y(64) - 1 + dw_rows_z(64) - 1 == 63 &&
+                  dw_rows_y(1000) - 1 + dw_rows_z(1000) - 1 == 999,
+              "the map ends with the tensor");
+
 // `split`: CTAs that share a tile, `grid` of them altogether; 1: whole tiles.
 template <class T, class TO, int MODE, int NT, int PAIR, int HALVES, bool SPLIT, bool GATHER, bool PARTS, int ADAPT>
 static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStream_t st) {
@@ -1237,8 +1245,8 @@ static int grouped_launch_as(const GroupedArgs& a, int grid, int split, cudaStre
   CUtensorMap ma, mb, row_a, row_b, out;
   if (MODE == kGroupedDw) {
     const uint64_t rows = a.slots ? a.slots : 1;
-    const uint64_t da[3] = {(uint64_t)a.n, 64, rows}, sa[2] = {(uint64_t)a.a_stride, (uint64_t)a.a_stride};
-    const uint64_t db[3] = {(uint64_t)a.k, 64, rows}, sb[2] = {(uint64_t)a.b_stride, (uint64_t)a.b_stride};
+    const uint64_t da[3] = {(uint64_t)a.n, dw_rows_y(rows), dw_rows_z(rows)}, sa[2] = {(uint64_t)a.a_stride, (uint64_t)a.a_stride};
+    const uint64_t db[3] = {(uint64_t)a.k, dw_rows_y(rows), dw_rows_z(rows)}, sb[2] = {(uint64_t)a.b_stride, (uint64_t)a.b_stride};
     const uint64_t ra[2] = {(uint64_t)a.n, rows}, rb[2] = {(uint64_t)a.k, rows};
     const uint32_t box[3] = {64, 64, 1}, one[2] = {64, 1};
     const void *pa = a.slots ? a.a : a.out, *pb = a.slots ? a.b : a.out;          // without rows nothing is copied
